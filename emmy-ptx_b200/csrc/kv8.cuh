@@ -1,0 +1,113 @@
+// Shared by the kernels of the paged 8-bit key/value cache (kv8_*.cu).
+//
+// A cache layer is a pool of pages codes[page][K or V][kv head][slot][d] in
+// e4m3 and one exponent exps[page][K or V][kv head]; a held value is
+// code * 2^exp.  The scale is a power of two because e4m3 is a floating
+// format: a general scale buys no precision, only a better fit of the top
+// binade, while a power of two makes every held value exact in f16 and bf16
+// after scaling, makes a change of scale exact above e4m3's subnormals, and
+// lets the kernels fold it into exponents they compute anyway.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "emmyrt.h"
+
+namespace kv8 {
+
+// Exponents of a page.  448 * 2^63 = 4e21 is the largest magnitude held.  The
+// span of 95 keeps an accumulator of 2^20 terms of 448 finite in f32 when it
+// moves from the units of one page to those of any other.
+constexpr int E_MIN = -32, E_MAX = 63;
+
+// What a kernel leaves in the status word (0: nothing was wrong).
+constexpr unsigned STATUS_PAGE = 0x401;    // a page number outside the pool
+constexpr unsigned STATUS_LENGTH = 0x402;  // a sequence longer than its row of the table, or
+                                           // more new tokens than keys or than rows given
+constexpr unsigned STATUS_WAIT = 0x403;    // a bounded wait inside a kernel ran out
+
+struct Seqs {
+  const int *table;     // [seqs][width] page numbers
+  const int *kv_lens;   // [seqs] keys, the new tokens included
+  const int *q_starts;  // [seqs + 1] first row of each sequence's new tokens
+  unsigned *status;     // may be null
+  int seqs, width, pages, tokens, kv_heads, page_shift;
+};
+
+__device__ __forceinline__ void report(unsigned *status, unsigned code) {
+  if (status != nullptr) *status = code;
+}
+
+// Lengths of sequence b, or n = 0 (nothing to do) where they cannot be right.
+__device__ __forceinline__ void lengths(const Seqs &s, int b, int &start, int &n, int &len) {
+  start = s.q_starts[b];
+  n = s.q_starts[b + 1] - start;
+  len = s.kv_lens[b];
+  if (n < 0 || n > len || start < 0 || start + n > s.tokens ||
+      len > (int64_t(s.width) << s.page_shift)) {
+    report(s.status, STATUS_LENGTH);
+    n = 0;
+  }
+}
+
+// Two e4m3 codes (bits 0-15 of w) as f16x2; every e4m3 value is exact in f16.
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<unsigned short>(w)));
+  return r;
+}
+
+// hi, lo -> packed e4m3x2 (round to nearest even, saturating; NaN -> 0x7f).
+__device__ __forceinline__ uint32_t f32x2_e4m3x2(float hi, float lo) {
+  unsigned short r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ float pow2(int e) {  // -126 <= e <= 127
+  return __int_as_float((e + 127) << 23);
+}
+
+// 0x80 in each byte of w whose code is NaN (0x7f or 0xff).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+// Status of a call, with its message for emmy_last_error().
+int fail(int code, const char *what, const char *msg);
+int cuda_fail(const char *what, cudaError_t e);
+
+// Makes `device` the runtime's current device for a scope.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    err = cudaGetDevice(&prev_);
+    if (err == cudaSuccess && prev_ != device) {
+      err = cudaSetDevice(device);
+      moved_ = err == cudaSuccess;
+    }
+  }
+  ~OnDevice() {
+    if (moved_) cudaSetDevice(prev_);
+  }
+  cudaError_t err = cudaSuccess;
+
+ private:
+  int prev_ = 0;
+  bool moved_ = false;
+};
+
+// Checks what every call shares and fills the kernels' view of the sequences.
+int check_cache(const char *what, const emmy_kv8 *c);
+int check_seqs(const char *what, const emmy_kv8 *c);
+Seqs seqs_of(const emmy_kv8 &c);
+int sm_count(int device);
+// Whether [a, a + na) and [b, b + nb) share a byte.
+inline bool overlap(emmy_dptr a, uint64_t na, emmy_dptr b, uint64_t nb) {
+  return a < b + nb && b < a + na;
+}
+
+}  // namespace kv8

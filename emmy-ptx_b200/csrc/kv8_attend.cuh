@@ -1,0 +1,108 @@
+// Shared by the attention kernels over the paged 8-bit cache.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "kv8.cuh"
+
+namespace kv8 {
+
+struct AttendParams {
+  Seqs s;
+  const uint8_t *codes;
+  const int8_t *exps;
+  const void *q;
+  void *out;
+  int64_t q_ts, q_hs, o_ts, o_hs;  // token and head strides, elements
+  float *partial;
+  unsigned *counters;
+  float scale_log2;  // scale * log2(e)
+  int group;         // query heads of a kv head
+  int window, sinks;
+  int only_rows;     // sequences with more rows than this are not this launch's (0: all are)
+  int most_rows;     // rows of a kv head in the largest sequence
+};
+
+// Which keys a block of query rows sees, and the 64-key chunks that hold
+// them: those of the sinks, then those of the window.  Chunks never straddle
+// a page (page sizes are multiples of 64).
+struct Span {
+  int first, last;  // positions of the first and last token
+  int window, sinks;
+  int sink_chunks, window_chunk0, chunks;
+
+  Span() = default;
+  __device__ __forceinline__ Span(const AttendParams &p, int n, int len)
+      : first(len - n), last(len - 1), window(p.window), sinks(p.sinks) {
+    const int low = window > 0 ? max(0, first - window + 1) : 0;
+    window_chunk0 = low >> 6;
+    sink_chunks = min((sinks + 63) >> 6, window_chunk0);
+    chunks = n > 0 ? sink_chunks + ((len + 63) >> 6) - window_chunk0 : 0;
+  }
+  // first key of chunk i of the line
+  __device__ __forceinline__ int key0(int i) const {
+    return (i < sink_chunks ? i : i - sink_chunks + window_chunk0) << 6;
+  }
+  __device__ __forceinline__ bool sees(int pos, int key) const {
+    return key <= pos && (window == 0 || pos - key < window || key < sinks);
+  }
+  __device__ __forceinline__ bool any_sees(int key) const {
+    return key <= last && (window == 0 || first - key < window || key < sinks);
+  }
+  // every token sees keys a .. b
+  __device__ __forceinline__ bool all_see(int a, int b) const {
+    return b <= first && (window == 0 || last - a < window || b < sinks);
+  }
+  // some token sees some key of a .. b
+  __device__ __forceinline__ bool wanted(int a, int b) const {
+    return a <= last && (window == 0 || first - b < window || a < sinks);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t w, float &lo, float &hi);
+template <>
+__device__ __forceinline__ void unpack2<__nv_bfloat16>(uint32_t w, float &lo, float &hi) {
+  lo = __uint_as_float(w << 16);
+  hi = __uint_as_float(w & 0xffff0000u);
+}
+template <>
+__device__ __forceinline__ void unpack2<__half>(uint32_t w, float &lo, float &hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  lo = f.x;
+  hi = f.y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// 2^x: subnormal results are zero, 2^-inf = 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Exponent k of a row's largest finite magnitude, 2^k <= amax < 2^(k + 1),
+// kept where 2^k and 2^-k are normal f32; 0 for a row of zeros.
+__device__ __forceinline__ int row_exponent(float amax) {
+  const int e = int(__float_as_uint(amax) >> 23) - 127;
+  return amax == 0.0f ? 0 : max(min(e, 126), -126);
+}
+
+int rows_blocks(int64_t rows);
+uint64_t rows_partial_bytes(int nt, int head_dim, int device);
+cudaError_t rows_attend(const AttendParams &p, int nt, int head_dim, bool bf16, int device,
+                        cudaStream_t stream);
+
+}  // namespace kv8

@@ -1,0 +1,74 @@
+// Host-side checks shared by the entry points of the paged 8-bit cache.
+#include <cstdio>
+
+#include "kv8.cuh"
+
+void emmyrt_set_last_error(const char *msg);  // emmyrt.cpp; not exported
+
+namespace kv8 {
+
+int fail(int code, const char *what, const char *msg) {
+  char buf[256];
+  snprintf(buf, sizeof buf, "%s: %s", what, msg);
+  emmyrt_set_last_error(buf);
+  return code;
+}
+
+int cuda_fail(const char *what, cudaError_t e) {
+  return fail(EMMY_ECUDART, what, cudaGetErrorString(e));
+}
+
+int check_cache(const char *what, const emmy_kv8 *c) {
+  if (c == nullptr) return fail(EMMY_EINVAL, what, "null cache description");
+  if (c->codes == 0 || c->exps == 0) return fail(EMMY_EINVAL, what, "null cache storage");
+  if (c->codes % 16 != 0) return fail(EMMY_EINVAL, what, "codes must be 16-byte aligned");
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(EMMY_EINVAL, what, "head_dim must be 64 or 128");
+  if (c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
+    return fail(EMMY_EINVAL, what, "page_size must be 64, 128 or 256");
+  if (c->kv_heads < 1 || c->kv_heads > 1024)
+    return fail(EMMY_EINVAL, what, "kv_heads must be between 1 and 1024");
+  if (c->pages < 1) return fail(EMMY_EINVAL, what, "the cache has no pages");
+  if (c->device < 0) return fail(EMMY_EINVAL, what, "negative device");
+  return EMMY_OK;
+}
+
+Seqs seqs_of(const emmy_kv8 &c) {
+  Seqs s;
+  s.table = reinterpret_cast<const int *>(c.page_table);
+  s.kv_lens = reinterpret_cast<const int *>(c.kv_lens);
+  s.q_starts = reinterpret_cast<const int *>(c.q_starts);
+  s.status = reinterpret_cast<unsigned *>(c.status);
+  s.seqs = c.seqs;
+  s.width = c.table_width;
+  s.pages = c.pages;
+  s.tokens = c.tokens;
+  s.kv_heads = c.kv_heads;
+  s.page_shift = c.page_size == 64 ? 6 : c.page_size == 128 ? 7 : 8;
+  return s;
+}
+
+int check_seqs(const char *what, const emmy_kv8 *c) {
+  if (c->page_table == 0 || c->kv_lens == 0 || c->q_starts == 0)
+    return fail(EMMY_EINVAL, what, "null page table, kv_lens or q_starts");
+  if (c->page_table % 4 || c->kv_lens % 4 || c->q_starts % 4 || c->status % 4)
+    return fail(EMMY_EINVAL, what, "page table, lengths and status must be 4-byte aligned");
+  if (c->seqs < 1 || c->seqs > EMMY_KV8_MAX_SEQS)
+    return fail(EMMY_EINVAL, what, "seqs must be between 1 and 4096");
+  if (c->table_width < 1 || c->tokens < 0 || c->max_q < 0 || c->max_q > c->tokens)
+    return fail(EMMY_EINVAL, what, "bad table_width, tokens or max_q");
+  if (int64_t(c->table_width) * c->page_size > (int64_t(1) << 30))
+    return fail(EMMY_EINVAL, what, "a sequence holds at most 2^30 keys");
+  return EMMY_OK;
+}
+
+int sm_count(int device) {
+  static int known[64] = {};
+  if (device >= 0 && device < 64 && known[device] > 0) return known[device];
+  int n = 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+  if (device >= 0 && device < 64) known[device] = n;
+  return n;
+}
+
+}  // namespace kv8

@@ -23,4 +23,13 @@ def run_problem(pdir, **kw):
     return _run(pdir, **kw)
 
 
-__all__ = ["load_kernel", "compile_kernel", "compile_file", "run_kernel", "run_problem"]
+def __getattr__(name):
+    # the paged key/value cache needs the runtime library, the compiler does not
+    if name in ("KVCache", "KVSequences", "DeviceArray"):
+        from . import kvcache
+        return getattr(kvcache, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+__all__ = ["load_kernel", "compile_kernel", "compile_file", "run_kernel", "run_problem",
+           "KVCache", "KVSequences", "DeviceArray"]

@@ -1,0 +1,576 @@
+"""A paged 8-bit key/value cache and the attention that reads it.
+
+The compiled attention kernels recompute nothing but keep nothing either: a
+caller that generates tokens one at a time needs the keys and values of all
+earlier tokens again at each step.  ``KVCache`` holds them on one GPU, one
+byte a value, in pages that sequences share and exchange; its kernels are
+hand-written CUDA in ``libemmyrt.so`` (``emmy_kv8_*`` in ``emmyrt.h``).  The
+reference has no counterpart.
+
+    cache = KVCache(pages=4096, kv_heads=8, head_dim=128, layers=32)
+    seqs = KVSequences(cache)                 # page bookkeeping on the host
+    a = seqs.new()
+    batch = seqs.batch([a], [prompt_tokens])  # room for the prompt
+    for layer in range(32):
+        ...
+        batch.append(layer, k, v)             # [tokens, kv_heads, head_dim]
+        batch.attend(layer, q, out)           # [tokens, heads, head_dim]
+    b = seqs.fork(a)                          # shares a's pages; copied on write
+    batch = seqs.batch([a, b])                # one more token each
+
+A held value is an e4m3 code times 2**e, with one exponent e for each page,
+side (K or V) and kv head; ``append`` picks the smallest e in [-32, 63] that
+holds the page's largest finite magnitude and re-rounds a page's older codes
+when a new token needs a larger one.  Query i of the n new tokens of a
+sequence of L keys sees key j <= L - n + i, and with a window W only those
+with L - n + i - j < W or j < sinks.
+
+Arrays are device arrays: anything with ``data_ptr()``, ``stride()``,
+``shape``, ``dtype`` and ``device`` as torch tensors have them, or a
+``DeviceArray`` over a raw address.  No gradients are recorded.  Calls are
+queued on ``stream`` (an address, or an object with ``cuda_stream``; default
+the device's stream, ``Device.stream``; 0 is the legacy default stream),
+return at once and allocate nothing after the first ``attend`` of a batch;
+the caller keeps the arrays alive until the work is done and orders streams,
+as with every other call here.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from .runtime import Device, EmmyError, check, load_library
+
+E_MIN, E_MAX = -32, 63
+HEAD_DIMS = (64, 128)
+PAGE_SIZES = (64, 128, 256)
+MAX_SEQS = 4096
+MAX_PAIRS = 480            # pages a launch of copy_pages takes
+WORKSPACE_ZERO = 16384     # bytes of a workspace that start as zeros
+
+STATUS = {0x401: "a page number outside the pool",
+          0x402: "a sequence longer than its row of the table, or more new tokens than keys or rows",
+          0x403: "a bounded wait inside a kernel ran out"}
+
+
+class _Cache(C.Structure):
+    """``emmy_kv8``."""
+    _fields_ = [(n, C.c_uint64) for n in ("codes", "exps", "page_table", "kv_lens", "q_starts",
+                                          "status")] \
+        + [(n, C.c_int32) for n in ("device", "pages", "kv_heads", "head_dim", "page_size",
+                                    "seqs", "table_width", "tokens", "max_q")]
+
+
+class _Attend(C.Structure):
+    """``emmy_kv8_attend_args``."""
+    _fields_ = [("q", C.c_uint64), ("out", C.c_uint64), ("workspace", C.c_uint64),
+                ("workspace_bytes", C.c_uint64), ("q_strides", C.c_int64 * 2),
+                ("out_strides", C.c_int64 * 2), ("dtype", C.c_int32), ("heads", C.c_int32),
+                ("window", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float)]
+
+
+_Strides = C.c_int64 * 2
+
+
+class DeviceArray:
+    """A view of device memory at a raw address: ``dtype`` one of "f32",
+    "bf16", "f16", "u8", "i8"; strides in elements, row-major by default."""
+
+    def __init__(self, ptr: int, dtype: str, shape, strides=None, device: int = 0):
+        self.ptr, self.dtype, self.shape, self.device = int(ptr), dtype, tuple(shape), device
+        if strides is None:
+            strides, n = [], 1
+            for s in reversed(self.shape):
+                strides.append(n)
+                n *= s
+            strides.reverse()
+        self.strides = tuple(strides)
+
+    def data_ptr(self) -> int:
+        return self.ptr
+
+    def stride(self) -> tuple:
+        return self.strides
+
+
+_DTYPES = {"f32": 0, "bf16": 1, "f16": 2, "u8": 3, "i8": 4}
+_NAMES = {"float32": "f32", "bfloat16": "bf16", "float16": "f16", "half": "f16", "uint8": "u8",
+          "int8": "i8", "float8_e4m3fn": "u8"}
+
+
+def _dtype_code(dtype) -> int:
+    code = _DTYPES.get(dtype)
+    if code is None:
+        name = str(dtype).split(".")[-1]
+        code = _DTYPES.get(_NAMES.get(name, name))
+        if code is None:
+            raise EmmyError(f"unsupported dtype {dtype}")
+        _DTYPES[dtype] = code
+    return code
+
+
+def _ordinal(dev, name: str) -> int:
+    if isinstance(dev, int):
+        return dev
+    if getattr(dev, "type", None) != "cuda":
+        raise EmmyError(f"{name} is not on a GPU")
+    return dev.index
+
+
+def _stream_of(stream, dev: Device):
+    if stream is None:
+        return dev.stream
+    return getattr(stream, "cuda_stream", stream)
+
+
+def _ints(x, name: str) -> np.ndarray:
+    a = np.asarray(x)
+    if a.size == 0:
+        return a.astype(np.int64)
+    if a.dtype.kind not in "iu":
+        raise EmmyError(f"{name} must be whole numbers")
+    return a.astype(np.int64)
+
+
+class KVCache:
+    """``layers`` layers of ``pages`` pages of ``page_size`` tokens each, on
+    one GPU.  ``storage``: (codes, exps) to adopt instead of allocating --
+    contiguous 8-bit arrays [layers, pages, 2, kv_heads, page_size, head_dim]
+    (e4m3 codes; K, then V) and [layers, pages, 2, kv_heads] (int8)."""
+
+    def __init__(self, pages: int, kv_heads: int, head_dim: int, page_size: int = 64,
+                 layers: int = 1, device: int = 0, storage=None):
+        if head_dim not in HEAD_DIMS:
+            raise EmmyError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
+        if page_size not in PAGE_SIZES:
+            raise EmmyError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+        if not 1 <= kv_heads <= 1024:
+            raise EmmyError(f"kv_heads must be between 1 and 1024, got {kv_heads}")
+        if not 1 <= pages < 2 ** 31:
+            raise EmmyError(f"pages must be between 1 and 2^31 - 1, got {pages}")
+        if not 1 <= layers <= 65535:
+            raise EmmyError(f"layers must be between 1 and 65535, got {layers}")
+        self.pages, self.kv_heads, self.head_dim = pages, kv_heads, head_dim
+        self.page_size, self.layers, self.ordinal = page_size, layers, device
+        self.layer_codes = pages * 2 * kv_heads * page_size * head_dim
+        self.layer_exps = pages * 2 * kv_heads
+        self._own: list[int] = []
+        self._storage = storage
+        if storage is not None:
+            codes, exps = storage
+            shape = (layers, pages, 2, kv_heads, page_size, head_dim)
+            for name, x, want, types in (("codes", codes, shape, (3, 4)),
+                                         ("exps", exps, shape[:4], (4,))):
+                if tuple(x.shape) != want:
+                    raise EmmyError(f"storage: {name} has shape {tuple(x.shape)}, expected {want}")
+                if _dtype_code(x.dtype) not in types:
+                    raise EmmyError(f"storage: {name} must be an 8-bit array, got {x.dtype}")
+                n = 1
+                for size, stride in zip(reversed(want), reversed(tuple(x.stride()))):
+                    if size != 1 and stride != n:
+                        raise EmmyError(f"storage: {name} must be contiguous")
+                    n *= size
+                if _ordinal(x.device, name) != device:
+                    raise EmmyError(f"storage: {name} is not on device {device}")
+            self.codes, self.exps = codes.data_ptr(), exps.data_ptr()
+            if self.codes % 16:
+                raise EmmyError("storage: codes must be 16-byte aligned")
+        self.dev = Device.get(device)
+        self.L = load_library()
+        if storage is None:
+            for attr, n in (("codes", layers * self.layer_codes), ("exps", layers * self.layer_exps)):
+                ptr = self.dev.alloc(n)
+                self._own.append(ptr)
+                setattr(self, attr, ptr)
+            # pages that nothing wrote hold zeros
+            self.dev.memset32(self.codes, 0, (layers * self.layer_codes + 3) // 4)
+            self.dev.memset32(self.exps, 0, (layers * self.layer_exps + 3) // 4)
+            self.dev.sync()
+
+    def _desc(self) -> _Cache:
+        d = _Cache()
+        d.codes, d.exps, d.device = self.codes, self.exps, self.ordinal
+        d.pages, d.kv_heads = self.pages, self.kv_heads
+        d.head_dim, d.page_size = self.head_dim, self.page_size
+        return d
+
+    def batch(self, page_table, kv_lens, q_lens=None, stream=None) -> "Batch":
+        """The sequences of one step: ``page_table`` [seqs, width] page
+        numbers, ``kv_lens`` keys of each sequence with its new tokens,
+        ``q_lens`` new tokens of each (default 1).  Host arrays, checked
+        here and copied to the device on ``stream``."""
+        return Batch(self, page_table, kv_lens, q_lens, stream)
+
+    def copy_pages(self, src, dst, stream=None) -> None:
+        """Copy pages ``src[i]`` to ``dst[i]`` in every layer (host lists);
+        no page twice in ``dst`` nor in both lists."""
+        src, dst = _ints(src, "src"), _ints(dst, "dst")
+        if src.ndim != 1 or src.shape != dst.shape:
+            raise EmmyError("copy_pages: src and dst are lists of the same length")
+        n = len(src)
+        if n == 0:
+            return
+        if min(src.min(), dst.min()) < 0 or max(src.max(), dst.max()) >= self.pages:
+            raise EmmyError(f"copy_pages: a page is outside 0..{self.pages - 1}")
+        targets = set(dst.tolist())
+        if len(targets) != n:
+            raise EmmyError("copy_pages: a page is in dst twice")
+        if not targets.isdisjoint(src.tolist()):
+            raise EmmyError("copy_pages: a page is in both src and dst")
+        src, dst = src.astype(np.int32), dst.astype(np.int32)
+        d, st = self._desc(), _stream_of(stream, self.dev)
+        for i in range(0, n, MAX_PAIRS):
+            check(self.L.emmy_kv8_copy_pages(C.byref(d), self.layers, src[i:].ctypes.data,
+                                             dst[i:].ctypes.data, min(MAX_PAIRS, n - i), st),
+                  "copy_pages")
+
+    def close(self) -> None:
+        """Free what this cache allocated (not adopted storage)."""
+        for p in self._own:
+            self.dev.free(p)
+        self._own = []
+
+
+class Batch:
+    """One step's sequences on the device.  Rows of the arrays given to
+    ``append`` and ``attend`` are the new tokens, sequence after sequence;
+    rows behind the last one are left alone.  Calls of one batch share a
+    workspace, so they must not overlap on the GPU: two captured graphs, or
+    two streams, that run at once need a batch each.  A graph captured over
+    these calls replays with what ``update`` last put there."""
+
+    def __init__(self, cache: KVCache, page_table, kv_lens, q_lens=None, stream=None):
+        self.cache, self.dev, self.L = cache, cache.dev, cache.L
+        table = _ints(page_table, "page_table")
+        if table.ndim != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+            raise EmmyError("page_table must be [sequences, pages]")
+        if table.shape[0] > MAX_SEQS:
+            raise EmmyError(f"a batch holds at most {MAX_SEQS} sequences")
+        self.seqs, self.width = table.shape
+        if self.width * cache.page_size > 2 ** 30:
+            raise EmmyError("a sequence holds at most 2^30 keys")
+        self.tokens = self.max_q = None
+        self._buf = self._ws = 0
+        self._ws_bytes, self._ws_heads = 0, 0
+        self._stale = False
+        host = self._packed(table, kv_lens, q_lens)
+        self._buf = self.dev.alloc(host.nbytes)
+        self.dev.htod(self._buf, host, _stream_of(stream, self.dev))
+        d = self._d = cache._desc()
+        d.status = self._buf
+        d.kv_lens = self._buf + 16
+        d.q_starts = d.kv_lens + 4 * self.seqs
+        d.page_table = d.q_starts + 4 * (self.seqs + 1)
+        d.seqs, d.table_width, d.tokens, d.max_q = self.seqs, self.width, self.tokens, self.max_q
+        self._ref = C.byref(d)
+        self._a = _Attend()
+        self._aref = C.byref(self._a)
+
+    def _packed(self, table, kv_lens, q_lens) -> np.ndarray:
+        """Checked lengths and table as one int32 array: status word and
+        padding, kv_lens, q_starts, table."""
+        P, B = self.cache.page_size, self.seqs
+        kv = _ints(kv_lens, "kv_lens").reshape(-1)
+        q = np.ones(B, np.int64) if q_lens is None else _ints(q_lens, "q_lens").reshape(-1)
+        if len(kv) != B or len(q) != B or table.shape != (B, self.width):
+            raise EmmyError(f"expected {B} lengths and a page table [{B}, {self.width}]")
+        if (q < 0).any() or (q > kv).any():
+            raise EmmyError("a sequence has between 0 and its kv_len new tokens")
+        if (kv > self.width * P).any():
+            raise EmmyError(f"a sequence is longer than its {self.width} pages of {P} tokens")
+        used = np.arange(self.width) < -(-kv // P)[:, None]
+        if ((table < 0) | (table >= self.cache.pages))[used].any():
+            raise EmmyError(f"page_table: a page is outside 0..{self.cache.pages - 1}")
+        tokens, most = int(q.sum()), int(q.max())
+        if tokens >= 2 ** 31:
+            raise EmmyError("too many new tokens")
+        if self.tokens is None:
+            self.tokens, self.max_q = tokens, most
+        elif tokens > self.tokens or most > self.max_q:
+            raise EmmyError(f"update: the batch was made for {self.tokens} new tokens, "
+                            f"at most {self.max_q} of a sequence")
+        # pages that append writes: of no more than one sequence
+        span = np.arange(self.width)
+        written = table[(span >= ((kv - q) // P)[:, None]) & (span <= ((kv - 1) // P)[:, None])
+                        & (q > 0)[:, None]]
+        self._clash = len(np.unique(written)) != len(written)
+        host = np.zeros(4 + 2 * B + 1 + B * self.width, np.int32)
+        host[4:4 + B] = kv
+        host[5 + B:5 + 2 * B] = np.cumsum(q)
+        host[5 + 2 * B:] = np.where(used, table, 0).reshape(-1)
+        return host
+
+    def update(self, page_table, kv_lens, q_lens=None, stream=None) -> None:
+        """New contents in the same device arrays, for the next replay of a
+        graph or the next step: as many sequences, a table as wide, no more
+        new tokens than the batch was made for."""
+        self._live()
+        host = self._packed(_ints(page_table, "page_table"), kv_lens, q_lens)
+        self.dev.htod(self._buf + 16, host[4:], _stream_of(stream, self.dev))
+        self._stale = False
+
+    def _live(self) -> None:
+        if not self._buf:
+            raise EmmyError("the batch is closed")
+
+    def _usable(self, layer: int) -> None:
+        self._live()
+        if self._stale:
+            raise EmmyError("the batch names pages that compact() moved: update it or make a new one")
+        if not 0 <= layer < self.cache.layers:
+            raise EmmyError(f"layer {layer} is outside 0..{self.cache.layers - 1}")
+        d, c = self._d, self.cache
+        d.codes = c.codes + layer * c.layer_codes
+        d.exps = c.exps + layer * c.layer_exps
+
+    def _array(self, x, name: str, heads: int | None):
+        """(address, dtype code, (token, head) strides, heads) of a
+        [tokens, heads, head_dim] argument."""
+        shape, stride = x.shape, x.stride()
+        if len(shape) != 3 or shape[0] < self.tokens or shape[2] != self.cache.head_dim \
+                or (heads is not None and shape[1] != heads):
+            raise EmmyError(f"{name} has shape {tuple(shape)}, expected "
+                            f"[>= {self.tokens}, {heads or 'heads'}, {self.cache.head_dim}]")
+        if stride[2] != 1:
+            raise EmmyError(f"{name}: the last dimension must be contiguous")
+        if _ordinal(x.device, name) != self.cache.ordinal:
+            raise EmmyError(f"{name} is not on device {self.cache.ordinal}")
+        return x.data_ptr(), _dtype_code(x.dtype), stride, shape[1]
+
+    def append(self, layer: int, k, v, stream=None) -> None:
+        """Write the new tokens' keys and values (f32, bf16 or f16) into
+        their pages of ``layer``."""
+        self._usable(layer)
+        if self._clash:
+            raise EmmyError("append: two sequences of the batch write to the same page")
+        kp, kt, ks, _ = self._array(k, "k", self.cache.kv_heads)
+        vp, vt, vs, _ = self._array(v, "v", self.cache.kv_heads)
+        if kt != vt or kt > 2:
+            raise EmmyError("append: k and v must both be f32, bf16 or f16")
+        rc = self.L.emmy_kv8_append(self._ref, kp, vp, kt, _Strides(ks[0], ks[1]),
+                                    _Strides(vs[0], vs[1]), _stream_of(stream, self.dev))
+        if rc:
+            check(rc, "append")
+
+    def reserve(self, heads: int, stream=None) -> None:
+        """Allocate the workspace that ``attend`` with ``heads`` query heads
+        needs (done by the first call otherwise): before a graph is captured."""
+        if heads == self._ws_heads:
+            return
+        self._live()
+        need = C.c_uint64()
+        check(self.L.emmy_kv8_attend_workspace(self._ref, heads, C.byref(need)), "attend")
+        if need.value > self._ws_bytes:
+            new = self.dev.alloc(need.value)
+            if self._ws:
+                self.dev.free(self._ws)      # waits for what still runs on it
+            self._ws, self._ws_bytes = new, need.value
+            self.dev.memset32(new, 0, WORKSPACE_ZERO // 4, _stream_of(stream, self.dev))
+        self._ws_heads = heads
+
+    def attend(self, layer: int, q, out, scale: float | None = None, window: int = 0,
+               sinks: int = 0, stream=None):
+        """Attention of the new tokens' queries ``q`` [tokens, heads,
+        head_dim] (bf16 or f16) over ``layer`` into ``out`` (same type and
+        shape, not overlapping ``q``); returns ``out``.  ``scale`` defaults
+        to head_dim ** -0.5.  ``window``: only the last ``window`` positions,
+        and the first ``sinks`` ones (0: all)."""
+        self._usable(layer)
+        a = self._a
+        qp, qt, qs, heads = self._array(q, "q", None)
+        op, ot, os_, _ = self._array(out, "out", heads)
+        if qt != ot or qt not in (1, 2):
+            raise EmmyError("attend: q and out must both be bf16 or f16")
+        if heads != self._ws_heads:
+            self.reserve(heads, stream)
+        a.q, a.out, a.workspace, a.workspace_bytes = qp, op, self._ws, self._ws_bytes
+        a.q_strides[0], a.q_strides[1] = qs[0], qs[1]
+        a.out_strides[0], a.out_strides[1] = os_[0], os_[1]
+        a.dtype, a.heads, a.window, a.sinks = qt, heads, window, sinks
+        a.scale = self.cache.head_dim ** -0.5 if scale is None else scale
+        rc = self.L.emmy_kv8_attend(self._ref, self._aref, _stream_of(stream, self.dev))
+        if rc:
+            check(rc, "attend")
+        return out
+
+    def check_errors(self, stream=None) -> None:
+        """Wait for ``stream`` and raise if a kernel of this batch reported
+        something in its status word; clears it."""
+        self._live()
+        word = np.zeros(1, np.uint32)
+        st = _stream_of(stream, self.dev)
+        self.dev.dtoh(word, self._buf, st)
+        self.dev.sync(st)
+        if word[0]:
+            self.dev.memset32(self._buf, 0, 1, st)
+            raise EmmyError(f"cache kernel reported error 0x{word[0]:x}: "
+                            f"{STATUS.get(int(word[0]), 'unknown')}")
+
+    def close(self) -> None:
+        buf, ws = self._buf, self._ws
+        self._buf = self._ws = 0
+        self._ws_bytes, self._ws_heads = 0, 0
+        for p in (buf, ws):
+            if p:
+                self.dev.free(p)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # the context may be gone when the process ends
+            pass
+
+
+class KVSequences:
+    """Which pages of a cache hold which sequence: reference counts, copy on
+    write, and the page moves of ``compact``.  Host bookkeeping; the copies
+    it needs are queued on the stream given, which must be the one that
+    appends, or one ordered with it."""
+
+    def __init__(self, cache: KVCache):
+        self.cache = cache
+        self._refs = [0] * cache.pages
+        self._free = list(range(cache.pages - 1, -1, -1))   # the lowest page is taken first
+        self._pages: dict[int, list[int]] = {}
+        self._len: dict[int, int] = {}
+        self._next = 0
+        self._batches: list = []
+
+    # -- sequences ----------------------------------------------------------
+
+    def new(self) -> int:
+        """An empty sequence."""
+        sid, self._next = self._next, self._next + 1
+        self._pages[sid], self._len[sid] = [], 0
+        return sid
+
+    def _known(self, sid: int) -> None:
+        if sid not in self._pages:
+            raise EmmyError(f"no sequence {sid}")
+
+    def length(self, sid: int) -> int:
+        self._known(sid)
+        return self._len[sid]
+
+    def pages(self, sid: int) -> list[int]:
+        self._known(sid)
+        return list(self._pages[sid])
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def fork(self, sid: int) -> int:
+        """A sequence with the same tokens, on the same pages; a shared page
+        is copied when one of its sequences writes to it."""
+        self._known(sid)
+        new = self.new()
+        self._pages[new], self._len[new] = list(self._pages[sid]), self._len[sid]
+        for p in self._pages[new]:
+            self._refs[p] += 1
+        return new
+
+    def _drop(self, page: int) -> None:
+        self._refs[page] -= 1
+        if self._refs[page] == 0:
+            self._free.append(page)
+
+    def truncate(self, sid: int, length: int) -> None:
+        """Forget the tokens from position ``length`` on (rejected drafts)."""
+        self._known(sid)
+        if not 0 <= length <= self._len[sid]:
+            raise EmmyError(f"truncate: sequence {sid} has {self._len[sid]} tokens")
+        keep = -(-length // self.cache.page_size)
+        for p in self._pages[sid][keep:]:
+            self._drop(p)
+        del self._pages[sid][keep:]
+        self._len[sid] = length
+
+    def free(self, sid: int) -> None:
+        """Forget a sequence; pages no other sequence shares are free again."""
+        self.truncate(sid, 0)
+        del self._pages[sid], self._len[sid]
+
+    # -- steps --------------------------------------------------------------
+
+    def batch(self, sids, q_lens=None, stream=None) -> Batch:
+        """Room for ``q_lens[i]`` (default 1) more tokens of each sequence:
+        pages are taken, shared ones about to be written to copied, and the
+        lengths moved on.  Raises, with nothing changed, when pages run out."""
+        sids = list(sids)
+        q = [1] * len(sids) if q_lens is None else [int(n) for n in _ints(q_lens, "q_lens")]
+        if not sids or len(q) != len(sids):
+            raise EmmyError("batch: at least one sequence, and a q_len for each")
+        if len(set(sids)) != len(sids):
+            raise EmmyError("batch: a sequence is named twice")
+        for sid, n in zip(sids, q):
+            self._known(sid)
+            if n < 0:
+                raise EmmyError("batch: a q_len is negative")
+        P = self.cache.page_size
+        refs, need, copies = {}, 0, []
+        for sid, n in zip(sids, q):
+            have, length = self._pages[sid], self._len[sid]
+            need += max(0, -(-(length + n) // P) - len(have))
+            if n and length % P:
+                last = have[-1]
+                held = refs.get(last, self._refs[last])
+                if held > 1:
+                    refs[last] = held - 1
+                    copies.append(sid)
+                    need += 1
+        if need > len(self._free):
+            raise EmmyError(f"batch: {need} pages needed, {len(self._free)} free")
+        src, dst = [], []
+        for sid in copies:
+            page, old = self._free.pop(), self._pages[sid][-1]
+            self._refs[page] = 1
+            src.append(old)
+            dst.append(page)
+            self._refs[old] -= 1
+            self._pages[sid][-1] = page
+        for sid, n in zip(sids, q):
+            self._len[sid] += n
+            while len(self._pages[sid]) * P < self._len[sid]:
+                page = self._free.pop()
+                self._refs[page] = 1
+                self._pages[sid].append(page)
+        self.cache.copy_pages(src, dst, stream)
+        b = Batch(self.cache, self.table(sids), [self._len[s] for s in sids], q, stream)
+        self._track(b)
+        return b
+
+    def table(self, sids) -> np.ndarray:
+        """Page numbers [sequences, pages of the longest], rows filled up with 0."""
+        rows = [self._pages[s] for s in sids]
+        out = np.zeros((len(rows), max(1, max(map(len, rows), default=1))), np.int32)
+        for i, r in enumerate(rows):
+            out[i, :len(r)] = r
+        return out
+
+    def _track(self, batch: Batch) -> None:
+        import weakref
+        self._batches = [r for r in self._batches if r() is not None]
+        self._batches.append(weakref.ref(batch))
+
+    def compact(self, stream=None) -> int:
+        """Move pages so that those in use are the first ones of the pool;
+        returns how many are in use.  Batches made before name old pages and
+        refuse to run until updated."""
+        used = [p for p, n in enumerate(self._refs) if n]
+        n = len(used)
+        holes = [p for p in range(n) if not self._refs[p]]
+        moved = dict(zip([p for p in used if p >= n], holes))
+        if moved:
+            self.cache.copy_pages(list(moved), list(moved.values()), stream)
+            for old, new in moved.items():
+                self._refs[new], self._refs[old] = self._refs[old], 0
+            for pages in self._pages.values():
+                pages[:] = [moved.get(p, p) for p in pages]
+            for r in self._batches:
+                if r() is not None:
+                    r()._stale = True
+        self._free = list(range(self.cache.pages - 1, n - 1, -1))
+        return n

@@ -102,6 +102,10 @@ def load_library():
         "emmy_nccl_async_error": (i32, [vp, C.POINTER(i32)]),
         "emmy_nccl_abort": (i32, [vp]),
         "emmy_nccl_destroy": (i32, [vp]),
+        "emmy_kv8_append": (i32, [vp, u64, u64, i32, vp, vp, vp]),
+        "emmy_kv8_attend_workspace": (i32, [vp, i32, C.POINTER(u64)]),
+        "emmy_kv8_attend": (i32, [vp, vp, vp]),
+        "emmy_kv8_copy_pages": (i32, [vp, i32, vp, vp, i32, vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)

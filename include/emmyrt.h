@@ -45,7 +45,7 @@ enum {
   EMMY_ENOENTRY = -4,   /* entry point not in module (runner stage "lookup") */
   EMMY_EKERNEL = -5,    /* a kernel reported an error in its error word */
   EMMY_ESYMBOL = -6,    /* module global not found */
-  EMMY_ECUDART = -7     /* a CUDA runtime call failed (emmy_sum_f32_noalloc) */
+  EMMY_ECUDART = -7     /* a CUDA runtime call failed (emmy_sum_f32_noalloc, emmy_kv8_*) */
 };
 
 /* Library identity and the last error message of the calling thread. */
@@ -186,6 +186,80 @@ int emmy_nccl_destroy(emmy_comm *comm);
  * caller.  A failing CUDA runtime call returns EMMY_ECUDART (its message in
  * emmy_last_error()), never a raw cudaError_t. */
 int emmy_sum_f32_noalloc(emmy_dptr x, size_t n, emmy_dptr out, emmy_stream stream);
+
+/* ---- paged 8-bit key/value cache ----
+ * No counterpart in the reference, whose attention recomputes every key.  A
+ * layer of the cache is a pool of pages in caller-owned device memory:
+ *   codes  uint8  [pages][2][kv_heads][page_size][head_dim]   (K, then V)
+ *   exps   int8   [pages][2][kv_heads]
+ * A held value is e4m3(code) * 2^exp, exp in [-32, 63].  A sequence is a row
+ * of page numbers and a length; its new tokens, consecutive rows of the
+ * tensors given, are the last ones of that length.  The arrays below are
+ * device memory, read by the kernels, so a captured CUDA graph replays with
+ * whatever they hold then.  What they say is checked on the device: a page
+ * outside the pool is left out (append skips it, attend treats its keys as
+ * hidden) and a sequence whose lengths cannot be right is skipped, its output
+ * rows left as they were; either is reported in *status.  The contents of a
+ * valid page that no call wrote are hidden from every query.
+ * Calls run in stream order on `stream`, on device `device` whatever the
+ * thread's current device is, allocate nothing and do not synchronise.  A
+ * page must not be appended to by two sequences of one call. */
+typedef struct {
+  emmy_dptr codes;      /* one layer, 16-byte aligned */
+  emmy_dptr exps;
+  emmy_dptr page_table; /* int32 [seqs][table_width] */
+  emmy_dptr kv_lens;    /* int32 [seqs], the new tokens included */
+  emmy_dptr q_starts;   /* int32 [seqs + 1]: rows of sequence b are
+                           q_starts[b] .. q_starts[b + 1] - 1, none allowed */
+  emmy_dptr status;     /* uint32, or 0: not reported */
+  int32_t device;
+  int32_t pages, kv_heads, head_dim, page_size; /* head_dim 64 or 128, page_size 64, 128 or 256 */
+  int32_t seqs, table_width;                    /* seqs at most 4096 */
+  int32_t tokens;                               /* rows of the tensors given, at least q_starts[seqs] */
+  int32_t max_q;                                /* at least the new tokens of any sequence */
+} emmy_kv8;
+
+enum { EMMY_KV8_MAX_SEQS = 4096, EMMY_KV8_MAX_PAIRS = 480 };
+enum { EMMY_KV8_F32 = 0, EMMY_KV8_BF16 = 1, EMMY_KV8_F16 = 2 };
+
+/* Write the new tokens' keys and values, k and v [tokens][kv_heads][head_dim]
+ * of `dtype`, innermost dimension contiguous, strides in elements (token,
+ * head), base and strides multiples of 16 bytes.  A page's scale is the
+ * smallest that holds its largest finite magnitude; a page that already held
+ * tokens of the sequence keeps its scale unless the new ones need a larger
+ * one, and then its older codes are rounded to that.  Magnitudes above
+ * 448 * 2^63 and infinities saturate; NaN stays NaN. */
+int emmy_kv8_append(const emmy_kv8 *cache, emmy_dptr k, emmy_dptr v, int32_t dtype,
+                    const int64_t k_strides[2], const int64_t v_strides[2], emmy_stream stream);
+
+/* out = softmax(scale * q K^T, hidden keys left out) V for the new tokens'
+ * queries, q and out [tokens][heads][head_dim] of `dtype` (bf16 or f16),
+ * laid out as for append and not overlapping; heads a multiple of kv_heads, query head h
+ * reads kv head h / (heads / kv_heads).  Query i of n in a sequence of L keys
+ * stands at position p = L - n + i and sees key j when j <= p and (window ==
+ * 0, or p - j < window, or j < sinks).  A query that sees no key gives zeros.
+ * `workspace`: emmy_kv8_attend_workspace() bytes, 16-byte aligned, its first
+ * EMMY_KV8_WORKSPACE_ZERO bytes zero before the first call and left zero by
+ * each; calls that may overlap on the GPU need workspaces of their own. */
+typedef struct {
+  emmy_dptr q, out, workspace;
+  uint64_t workspace_bytes;
+  int64_t q_strides[2], out_strides[2];
+  int32_t dtype, heads;
+  int32_t window, sinks;
+  float scale;
+} emmy_kv8_attend_args;
+enum { EMMY_KV8_WORKSPACE_ZERO = 16384 };
+int emmy_kv8_attend_workspace(const emmy_kv8 *cache, int32_t heads, uint64_t *bytes);
+int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args *args, emmy_stream stream);
+
+/* In each of `layers` layers, laid out one after another, copy page src[i]
+ * with its exponents to page dst[i], i < n (host arrays, read during the
+ * call; n at most EMMY_KV8_MAX_PAIRS).  No page may be in dst twice, or in
+ * both lists.  Uses codes, exps, device, pages, kv_heads, head_dim and
+ * page_size of `cache`. */
+int emmy_kv8_copy_pages(const emmy_kv8 *cache, int32_t layers, const int32_t *src,
+                        const int32_t *dst, int32_t n, emmy_stream stream);
 
 #ifdef __cplusplus
 }
