@@ -27,7 +27,8 @@ extern "C" int emmy_kv8_attend_workspace(const emmy_kv8 *cache, int32_t heads, u
   if (rc == EMMY_OK) rc = check_heads(what, cache, heads);
   if (rc != EMMY_OK) return rc;
   if (sm_count(cache->device) == 0) return fail(EMMY_ECUDART, what, "cannot read the device's SM count");
-  const int nt = rows_blocks(int64_t(heads / cache->kv_heads) * cache->max_q);
+  const int64_t rows = int64_t(heads / cache->kv_heads) * cache->max_q;
+  const int nt = rows_blocks(rows < ROWS_MOST ? rows : ROWS_MOST);
   *bytes = EMMY_KV8_WORKSPACE_ZERO + rows_partial_bytes(nt, cache->head_dim, cache->device);
   return EMMY_OK;
 }
@@ -77,16 +78,24 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   p.group = a->heads / cache->kv_heads;
   p.window = a->window;
   p.sinks = a->sinks;
-  p.only_rows = 0;
   p.most_rows = p.group * cache->max_q;
+  // A sequence with up to ROWS_MOST rows of a kv head is the row kernel's,
+  // others the tile kernel's, which takes the one sequence of a call that may
+  // be either.
+  const bool tiles = p.most_rows > ROWS_MOST, rows = !tiles || cache->seqs > 1;
+  p.row_limit = rows ? ROWS_MOST : 0;
+  if (tiles && rows) p.most_rows = ROWS_MOST;
   const int nt = rows_blocks(p.most_rows);
   // the line of chunks is counted in 32 bits
-  const double line = double(cache->seqs) * cache->kv_heads * ((p.most_rows + 8 * nt - 1) / (8 * nt)) *
+  const double line = double(cache->seqs) * cache->kv_heads * 4 *
                       (double(cache->table_width) * cache->page_size / 64);
   if (line > 4e9) return fail(EMMY_EINVAL, WHAT, "too many sequences, heads and keys for one call");
   const OnDevice on(cache->device);
   if (on.err != cudaSuccess) return cuda_fail(WHAT, on.err);
-  const cudaError_t e = rows_attend(p, nt, cache->head_dim, a->dtype == EMMY_KV8_BF16, cache->device,
-                                    static_cast<cudaStream_t>(stream));
+  const bool bf16 = a->dtype == EMMY_KV8_BF16;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (tiles) e = tiles_attend(p, cache->head_dim, bf16, st);
+  if (e == cudaSuccess && rows) e = rows_attend(p, nt, cache->head_dim, bf16, cache->device, st);
   return e == cudaSuccess ? EMMY_OK : cuda_fail(WHAT, e);
 }

@@ -19,7 +19,7 @@ struct AttendParams {
   float scale_log2;  // scale * log2(e)
   int group;         // query heads of a kv head
   int window, sinks;
-  int only_rows;     // sequences with more rows than this are not this launch's (0: all are)
+  int row_limit;     // sequences with more rows of a kv head than this are the tile kernel's
   int most_rows;     // rows of a kv head in the largest sequence
 };
 
@@ -32,12 +32,13 @@ struct Span {
   int sink_chunks, window_chunk0, chunks;
 
   Span() = default;
-  __device__ __forceinline__ Span(const AttendParams &p, int n, int len)
-      : first(len - n), last(len - 1), window(p.window), sinks(p.sinks) {
+  // tokens at positions first_ .. last_, first_ <= last_
+  __device__ __forceinline__ Span(const AttendParams &p, int first_, int last_)
+      : first(first_), last(last_), window(p.window), sinks(p.sinks) {
     const int low = window > 0 ? max(0, first - window + 1) : 0;
     window_chunk0 = low >> 6;
     sink_chunks = min((sinks + 63) >> 6, window_chunk0);
-    chunks = n > 0 ? sink_chunks + ((len + 63) >> 6) - window_chunk0 : 0;
+    chunks = sink_chunks + (last >> 6) + 1 - window_chunk0;
   }
   // first key of chunk i of the line
   __device__ __forceinline__ int key0(int i) const {
@@ -100,6 +101,10 @@ __device__ __forceinline__ int row_exponent(float amax) {
   return amax == 0.0f ? 0 : max(min(e, 126), -126);
 }
 
+// Rows of a kv head up to which a sequence is the row kernel's.
+constexpr int ROWS_MOST = 32;
+
+cudaError_t tiles_attend(const AttendParams &p, int head_dim, bool bf16, cudaStream_t stream);
 int rows_blocks(int64_t rows);
 uint64_t rows_partial_bytes(int nt, int head_dim, int device);
 cudaError_t rows_attend(const AttendParams &p, int nt, int head_dim, bool bf16, int device,

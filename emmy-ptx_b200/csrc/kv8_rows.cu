@@ -305,9 +305,9 @@ rows_kernel(const AttendParams p) {
     for (int b = b0; b < b1; ++b) {
       int start, n, len;
       lengths(s, b, start, n, len);
-      if (p.only_rows > 0 && n * p.group > p.only_rows) n = 0;
-      const Span span(p, n, len);
-      const unsigned c = unsigned(span.chunks) * ((n * p.group + ROWS - 1) / ROWS) * s.kv_heads;
+      if (n * p.group > p.row_limit) n = 0;
+      unsigned c = 0;
+      if (n > 0) c = unsigned(Span(p, len - n, len - 1).chunks) * ((n * p.group + ROWS - 1) / ROWS) * s.kv_heads;
       line[b] = c;
       sum += c;
     }
@@ -345,7 +345,7 @@ rows_kernel(const AttendParams p) {
       g.b = lo;
     }
     lengths(s, g.b, g.start, g.n, g.len);
-    g.span = Span(p, g.n, g.len);
+    g.span = Span(p, g.len - g.n, g.len - 1);
     g.rows = g.n * p.group;
     const int chunks = g.span.chunks;
     const unsigned rel = pos - line[g.b], hr = rel / chunks;

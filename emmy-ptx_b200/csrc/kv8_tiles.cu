@@ -1,0 +1,618 @@
+// Attention of many query rows over the paged 8-bit cache (prompts, chunks of
+// prompts behind a history), on tcgen05.
+//
+// A CTA takes 256 query rows of one (sequence, kv head) -- tokens x the query
+// heads that share the kv head, so these share one pass over its keys -- as
+// two tiles A and B of 128 rows, and walks the 64-key chunks that some row
+// sees.  Warps:
+//   0       tcgen05 O += P V of both tiles (one thread); owns the TMEM
+//   1       tcgen05 S = Q K^T of both tiles (one thread)
+//   2-5     softmax and output of tile A, a thread a row; 6-9 of tile B
+//   10-13   codes -> f16: global loads a chunk ahead, e4m3 -> f16 in
+//           registers, stored as the 128-byte-swizzled tiles the MMAs read
+//           (K as [keys][d], V as stored: an MN-major operand)
+// TMEM: per tile two 64-column S buffers (chunk g in buffer g % 2, P over its
+// first half as packed f16) and O.  With two buffers S of chunk g + 1 is
+// computed while the softmax works on chunk g.
+//
+// The numerics are those of kv8_rows.cu: e4m3 exact in f16, a query row scaled
+// by a power of two, scores and sums in f32, p rounded to f16, K's page
+// exponent in the factor that takes scores to log2 units and V's in the
+// exponent of p; O moves (a pass over its columns) only when a row's maximum
+// grew by more than 2^8 or V's exponent strayed by more than 2^6.
+#include "kv8_attend.cuh"
+
+namespace kv8 {
+namespace {
+
+constexpr int TILE = 128, CHUNK = 64, STAGES = 4, THREADS = 448;
+constexpr int W_PV = 0, W_QK = 1, W_LOAD = 10;  // warps; 2-9 are the softmax
+constexpr float LAZY = 8.0f, NONE = -1e30f, LEAST = 1e-37f;
+constexpr int UNIT_LAZY = 6;
+constexpr unsigned long long WAIT_NS = 2000000000ull;
+
+template <int D>
+struct Layout {
+  static constexpr int Q_TILE = TILE * D * 2, KV = CHUNK * D * 2;  // bytes
+  static constexpr int STAGE0 = 2 * Q_TILE;
+  static constexpr int NAN_ROWS = STAGE0 + STAGES * 2 * KV;  // D bits a row
+  static constexpr int END = NAN_ROWS + 2 * TILE * (D / 8);
+  // 1 KB to align the tiles; above half an SM's shared memory, so that two
+  // CTAs of one SM never wait for each other's TMEM
+  static constexpr int DYN = END + 1024 > 120 * 1024 ? END + 1024 : 120 * 1024;
+  static constexpr int O_COL = 4 * CHUNK;
+};
+
+struct Bars {
+  uint64_t q_full, kv_full[STAGES], kv_empty[STAGES];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], drain;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void bar_init(uint64_t *b, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t *b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 100000;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(b), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+// Waits for the phase of parity `parity`; false when the kernel gives up.
+__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile unsigned *stop,
+                                         unsigned *status) {
+  const uint32_t at = smem_addr(b);
+  if (bar_try(at, parity)) return true;
+  const unsigned long long t0 = now_ns();
+  for (;;) {
+    if (bar_try(at, parity)) return true;
+    if (*stop != 0) return false;
+    if (now_ns() - t0 > WAIT_NS) {
+      *stop = 1;
+      report(status, STATUS_WAIT);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t *b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(b))
+               : "memory");
+}
+// D (+)= A B with A and B in shared memory, or A (TS) in TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tm_ld32(uint32_t (&r)[32], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory matrix descriptor, 128-byte swizzle: start address, leading
+// and stride byte offsets in 16-byte units, version 1 (bit 46), layout 2.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t at, uint32_t lbo, uint32_t sbo) {
+  return uint64_t((at >> 4) & 0x3fff) | uint64_t(lbo >> 4) << 16 | uint64_t(sbo >> 4) << 32 | 1ull << 46 |
+         2ull << 61;
+}
+// kind::f16, f16 operands, f32 sums; bit 16: B is MN-major.
+template <int M, int N, bool B_MN>
+constexpr uint32_t IDESC = 1u << 4 | uint32_t(B_MN) << 16 | uint32_t(N >> 3) << 17 | uint32_t(M >> 4) << 24;
+
+// 16-byte piece j (0-7) of 128-byte row r of a swizzled tile.
+__device__ __forceinline__ uint32_t swizzled(int r, int j) { return r * 128 + ((j ^ (r & 7)) << 4); }
+
+// What the unit is: 256 rows of one (sequence, kv head).
+struct Unit {
+  int b, head, start, n, len, rows, row0;
+  Span span;
+};
+
+// ---- codes -> f16 tiles (warps 10-13) ----
+template <int D>
+struct Codes {
+  static constexpr int N = D / 32;  // 16-byte pieces of K, and of V, a thread
+  uint4 k[N], v[N];
+  int key0, ek, ev;
+  bool dead;
+};
+
+template <int D>
+__device__ __forceinline__ void load_codes(Codes<D> &c, const AttendParams &p, const Unit &u, int key0,
+                                           int page, int t) {
+  c.key0 = key0;
+  c.dead = page < 0 || page >= p.s.pages;
+  if (c.dead) {
+    report(p.s.status, STATUS_PAGE);
+    page = 0;
+  }
+  const int64_t unit = int64_t(page) * 2 * p.s.kv_heads + u.head;
+  c.ek = p.exps[unit];
+  c.ev = p.exps[unit + p.s.kv_heads];
+  const int slot = key0 & ((1 << p.s.page_shift) - 1);
+  const uint4 *k = reinterpret_cast<const uint4 *>(p.codes + ((unit << p.s.page_shift) + slot) * D);
+  const uint4 *v = k + ((int64_t(p.s.kv_heads) << p.s.page_shift) * D >> 4);
+#pragma unroll
+  for (int i = 0; i < Codes<D>::N; ++i) c.k[i] = k[i * 128 + t];
+#pragma unroll
+  for (int i = 0; i < Codes<D>::N; ++i) c.v[i] = v[i * 128 + t];
+}
+
+// One 16-byte piece of codes as 32 bytes of a swizzled f16 tile of 64 rows.
+template <int D>
+__device__ __forceinline__ void store_piece(uint8_t *tile, int piece, const uint4 &w) {
+  const int r = piece / (D / 16), col = piece % (D / 16), half = col / 4, j = 2 * (col % 4);
+  uint8_t *at = tile + half * (CHUNK * 128);
+  const uint4 lo = make_uint4(e4m3x2_f16x2(w.x), e4m3x2_f16x2(w.x >> 16), e4m3x2_f16x2(w.y), e4m3x2_f16x2(w.y >> 16));
+  const uint4 hi = make_uint4(e4m3x2_f16x2(w.z), e4m3x2_f16x2(w.z >> 16), e4m3x2_f16x2(w.w), e4m3x2_f16x2(w.w >> 16));
+  // the second 128-byte half starts with its odd piece: eight lanes that
+  // store together then touch eight different pieces
+  *reinterpret_cast<uint4 *>(at + swizzled(r, j + half)) = half ? hi : lo;
+  *reinterpret_cast<uint4 *>(at + swizzled(r, j + 1 - half)) = half ? lo : hi;
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p) {
+  using L = Layout<D>;
+  extern __shared__ uint8_t dyn_raw[];
+  uint8_t *const dyn = dyn_raw + ((1024 - (smem_addr(dyn_raw) & 1023)) & 1023);
+  __shared__ Bars bars;
+  __shared__ uint32_t tmem_slot;
+  __shared__ unsigned stop_word, scan[THREADS / 32], stage_nan[STAGES];
+  __shared__ float2 stage_scale[STAGES];  // 2^ek, ev
+  __shared__ int found[2];
+  volatile unsigned *const stop = &stop_word;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Seqs &s = p.s;
+
+  // ---- which unit: the grid counts row blocks of all sequences, each for
+  // every kv head, the blocks with the most keys first ----
+  Unit u;
+  {
+    const int per = (s.seqs + THREADS - 1) / THREADS, b0 = min(tid * per, s.seqs), b1 = min(b0 + per, s.seqs);
+    const unsigned want = blockIdx.x;
+    unsigned sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      int start, n, len;
+      lengths(s, b, start, n, len);
+      if (n * p.group <= p.row_limit) n = 0;
+      sum += unsigned((n * p.group + 2 * TILE - 1) / (2 * TILE)) * s.kv_heads;
+    }
+    unsigned at = sum;
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned x = __shfl_up_sync(0xffffffffu, at, d);
+      if (lane >= d) at += x;
+    }
+    if (lane == 31) scan[warp] = at;
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) at += scan[w];
+    at -= sum;
+    if (want >= at && want < at + sum) {  // one thread's share holds it
+      for (int b = b0; b < b1; ++b) {
+        int start, n, len;
+        lengths(s, b, start, n, len);
+        if (n * p.group <= p.row_limit) n = 0;
+        const unsigned c = unsigned((n * p.group + 2 * TILE - 1) / (2 * TILE)) * s.kv_heads;
+        if (want < at + c) {
+          found[0] = b;
+          found[1] = int(want - at);
+          break;
+        }
+        at += c;
+      }
+    }
+    __syncthreads();
+    if (found[0] < 0) return;
+    u.b = found[0];
+    lengths(s, u.b, u.start, u.n, u.len);
+    u.rows = u.n * p.group;
+    u.head = found[1] % s.kv_heads;
+    u.row0 = ((u.rows + 2 * TILE - 1) / (2 * TILE) - 1 - found[1] / s.kv_heads) * (2 * TILE);
+    const int last_row = min(u.row0 + 2 * TILE, u.rows) - 1;
+    u.span = Span(p, u.len - u.n + u.row0 / p.group, u.len - u.n + last_row / p.group);
+  }
+  const int tiles = u.rows - u.row0 > TILE ? 2 : 1;
+  const int chunks = u.span.chunks;
+
+  // ---- barriers, TMEM ----
+  if (tid == 0) {
+    bar_init(&bars.q_full, tiles * TILE);
+    for (int i = 0; i < STAGES; ++i) {
+      bar_init(&bars.kv_full[i], 128);
+      bar_init(&bars.kv_empty[i], 1);
+      stage_nan[i] = 0;
+    }
+    for (int x = 0; x < 2; ++x)
+      for (int i = 0; i < 2; ++i) {
+        bar_init(&bars.s_full[x][i], 1);
+        bar_init(&bars.p_full[x][i], TILE);
+        bar_init(&bars.pv_done[x][i], 1);
+      }
+    bar_init(&bars.drain, 2);
+    stop_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == W_PV) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == W_PV) {
+    // ---- O += P V ----
+    if (lane == 0) {
+      constexpr uint32_t id = IDESC<TILE, D, true>;
+      bool ok = true;
+      for (int g = 0; ok && g < chunks; ++g) {
+        const int st = g % STAGES, buf = g & 1;
+        ok = bar_wait(&bars.kv_full[st], g / STAGES & 1, stop, s.status);
+        // V rows are 128 bytes (64 values of d), the second half of d follows
+        // CHUNK rows on; 16 keys are 2 KB
+        const uint64_t vd = smem_desc(smem_addr(dyn + L::STAGE0 + st * 2 * L::KV + L::KV), CHUNK * 128, 1024);
+        for (int x = 0; ok && x < tiles; ++x) {
+          ok = bar_wait(&bars.p_full[x][buf], g >> 1 & 1, stop, s.status);
+          if (!ok) break;
+          tc_after();
+          const uint32_t o = tmem + L::O_COL + x * D, pa = tmem + (2 * x + buf) * CHUNK;
+#pragma unroll
+          for (int k = 0; k < CHUNK / 16; ++k)
+            mma_ts(o, pa + k * 8, vd + (k * 2048 >> 4), id, g > 0 || k > 0);
+          tc_commit(&bars.pv_done[x][buf]);
+        }
+        if (ok) tc_commit(&bars.kv_empty[st]);
+      }
+    }
+  } else if (warp == W_QK) {
+    // ---- S = Q K^T ----
+    if (lane == 0) {
+      constexpr uint32_t id = IDESC<TILE, CHUNK, false>;
+      bool ok = bar_wait(&bars.q_full, 0, stop, s.status);
+      for (int g = 0; ok && g < chunks; ++g) {
+        const int st = g % STAGES, buf = g & 1;
+        ok = bar_wait(&bars.kv_full[st], g / STAGES & 1, stop, s.status);
+        const uint64_t kd = smem_desc(smem_addr(dyn + L::STAGE0 + st * 2 * L::KV), 16, 1024);
+        for (int x = 0; ok && x < tiles; ++x) {
+          // the buffer holds P of chunk g - 2 until its P V is done
+          if (g >= 2) ok = bar_wait(&bars.pv_done[x][buf], (g >> 1 & 1) ^ 1, stop, s.status);
+          if (!ok) break;
+          tc_after();
+          const uint64_t qd = smem_desc(smem_addr(dyn + x * L::Q_TILE), 16, 1024);
+          const uint32_t at = tmem + (2 * x + buf) * CHUNK;
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_ss(at, qd + ((h * TILE * 128 + k * 32) >> 4), kd + ((h * CHUNK * 128 + k * 32) >> 4), id, h > 0 || k > 0);
+          tc_commit(&bars.s_full[x][buf]);
+        }
+      }
+    }
+  } else if (warp >= W_LOAD) {
+    // ---- codes -> f16 ----
+    const int t = tid - W_LOAD * 32;
+    const int *row = s.table + int64_t(u.b) * s.width;
+    const auto page_of = [&](int g) { return g < chunks ? row[u.span.key0(g) >> s.page_shift] : 0; };
+    const auto put = [&](Codes<D> &c, int g) {
+      const int st = g % STAGES;
+      if (g >= STAGES && !bar_wait(&bars.kv_empty[st], (g / STAGES & 1) ^ 1, stop, s.status)) return false;
+      uint8_t *k = dyn + L::STAGE0 + st * 2 * L::KV, *v = k + L::KV;
+      // chunks some row does not see whole: values no row sees are zeroed and
+      // a NaN is taken out here (0 * NaN would reach rows it is hidden from)
+      // and put into the rows that see it at the end
+      if (c.dead || !u.span.all_see(c.key0, c.key0 + CHUNK - 1)) {
+#pragma unroll
+        for (int i = 0; i < Codes<D>::N; ++i) {
+          const int key = c.key0 + (i * 128 + t) / (D / 16);
+          if (c.dead || !u.span.any_sees(key)) c.v[i] = make_uint4(0, 0, 0, 0);
+          uint32_t *w = &c.v[i].x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t bad = nan_bytes(w[j]);
+            if (bad != 0) {
+              w[j] &= ~((bad >> 7) * 0xffu);
+              stage_nan[st] = 1;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < Codes<D>::N; ++i) store_piece<D>(k, i * 128 + t, c.k[i]);
+#pragma unroll
+      for (int i = 0; i < Codes<D>::N; ++i) store_piece<D>(v, i * 128 + t, c.v[i]);
+      if (t == 0) stage_scale[st] = make_float2(c.dead ? 0.0f : pow2(c.ek), float(c.ev));
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(&bars.kv_full[st]);
+      return true;
+    };
+    Codes<D> a, b;
+    int page = page_of(1);
+    load_codes(a, p, u, u.span.key0(0), page_of(0), t);
+    for (int g = 0; g < chunks; g += 2) {
+      if (g + 1 < chunks) load_codes(b, p, u, u.span.key0(g + 1), page, t);
+      page = page_of(g + 2);
+      if (!put(a, g)) break;
+      if (g + 1 < chunks) {
+        if (g + 2 < chunks) load_codes(a, p, u, u.span.key0(g + 2), page, t);
+        page = page_of(g + 3);
+        if (!put(b, g + 1)) break;
+      }
+    }
+  } else {
+    // ---- softmax: a thread a row ----
+    const int x = (warp - 2) >> 2, quad = warp & 3, r = quad * 32 + lane;
+    if (x < tiles) {
+      const int row = u.row0 + x * TILE + r;
+      const bool real = row < u.rows;
+      const int token = min(row, u.rows - 1) / p.group;
+      const int head = u.head * p.group + min(row, u.rows - 1) - token * p.group;
+      const int pos = u.len - u.n + token;
+      float mult;
+      {
+        // the query row: f16, scaled by a power of two, the scale's sign in it
+        const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) +
+                                                           (int64_t(u.start) + token) * p.q_ts + head * p.q_hs);
+        uint4 w[D / 8];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) w[i] = src[i];
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t *v = &w[i].x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float a, b;
+            unpack2<T>(v[j], a, b);
+            a = fabsf(a), b = fabsf(b);
+            amax = a < INFINITY ? fmaxf(amax, a) : amax;
+            amax = b < INFINITY ? fmaxf(amax, b) : amax;
+          }
+        }
+        const int e = row_exponent(amax);
+        const float by = p.scale_log2 < 0.0f ? -pow2(-e) : pow2(-e);
+        mult = fabsf(p.scale_log2) * pow2(e);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          uint32_t *v = &w[i].x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float a, b;
+            unpack2<T>(v[j], a, b);
+            v[j] = pack2<__half>(a * by, b * by);
+          }
+          *reinterpret_cast<uint4 *>(dyn + x * L::Q_TILE + i / 8 * (TILE * 128) + swizzled(r, i % 8)) = w[i];
+        }
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+          *reinterpret_cast<uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8) + 4 * i) = 0;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(&bars.q_full);
+
+      const uint32_t lanes = uint32_t(quad * 32) << 16;
+      const uint32_t s_at = tmem + lanes + 2 * x * CHUNK, o_at = tmem + lanes + L::O_COL + x * D;
+      float m = NONE, l = 0.0f;
+      int unit = 0;
+      bool ok = true, nan_seen = false;
+      for (int g = 0; g < chunks; ++g) {
+        const int buf = g & 1, st = g % STAGES, key0 = u.span.key0(g);
+        // S is there, and what the loading warps left beside the codes
+        ok = bar_wait(&bars.s_full[x][buf], g >> 1 & 1, stop, s.status) &&
+             bar_wait(&bars.kv_full[st], g / STAGES & 1, stop, s.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_after();
+        uint32_t sv[2][32];
+        tm_ld32(sv[0], s_at + buf * CHUNK);
+        tm_ld32(sv[1], s_at + buf * CHUNK + 32);
+        const float2 sc = stage_scale[st];
+        const int ev = int(sc.y);
+        const float rm = fmaxf(mult * sc.x, LEAST);
+        tm_wait_ld();
+        const bool dead = sc.x == 0.0f;
+        if (dead || !u.span.all_see(key0, key0 + CHUNK - 1)) {
+          // bit i: the row sees key key0 + i
+          const auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
+          uint64_t see = below(pos - key0 + 1);
+          if (p.window > 0) see &= ~below(pos - p.window + 1 - key0) | below(p.sinks - key0);
+          if (dead) see = 0;
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (!(see >> i & 1)) sv[i / 32][i % 32] = 0xff800000u;
+          if (stage_nan[st] != 0 && real) {
+            // (rare) this chunk holds NaN values: which of them this row sees
+            const int page = s.table[int64_t(u.b) * s.width + (key0 >> s.page_shift)];
+            const int64_t at = (int64_t(page) * 2 + 1) * s.kv_heads + u.head;
+            const uint32_t *v = reinterpret_cast<const uint32_t *>(
+                p.codes + ((at << s.page_shift) + (key0 & ((1 << s.page_shift) - 1))) * D);
+            uint32_t *bits = reinterpret_cast<uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8));
+            for (int i = 0; i < CHUNK; ++i)
+              if (see >> i & 1)
+                for (int w = 0; w < D / 4; ++w) {
+                  const uint32_t bad = nan_bytes(v[i * (D / 4) + w]);
+                  if (bad != 0)
+                    bits[w / 8] |= ((bad >> 7 & 1) | (bad >> 14 & 2) | (bad >> 21 & 4) | (bad >> 28 & 8)) << (w % 8 * 4);
+                }
+            nan_seen = true;
+          }
+        }
+        float top[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(sv[0][i]);
+#pragma unroll
+        for (int i = 4; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(sv[i / 32][i % 32]));
+        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * rm;
+        const int stray = ev - unit;
+        const bool first = g == 0, move = stray > UNIT_LAZY || stray < -UNIT_LAZY;
+        const bool fix = __any_sync(0xffffffffu, best > m + LAZY) || move;
+        float alpha = 1.0f;
+        if (fix) {
+          const float to = fmaxf(m, best);
+          alpha = exp2_fast(m - to);
+          m = to;
+          l *= alpha;
+          if (first) unit = ev;
+          if (move) {
+            alpha *= pow2(unit - ev);
+            unit = ev;
+          }
+        }
+        const float shift = float(ev - unit) - m;
+        float sum[4] = {};
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float a = exp2_fast(fmaf(__uint_as_float(sv[i / 16][2 * i % 32]), rm, shift));
+          const float b = exp2_fast(fmaf(__uint_as_float(sv[i / 16][2 * i % 32 + 1]), rm, shift));
+          sum[i & 3] += a + b;
+          pk[i] = pack2<__half>(a, b);
+        }
+        tm_st32(s_at + buf * CHUNK, pk);
+        l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2(unit - ev), l);
+        tm_wait_st();
+        if (fix && !first) {
+          // P V of chunk g - 1 is the last to have touched O
+          ok = bar_wait(&bars.pv_done[x][(g - 1) & 1], (g - 1) >> 1 & 1, stop, s.status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_after();
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tm_ld32(o, o_at + c);
+            tm_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tm_st32(o_at + c, o);
+          }
+          tm_wait_st();
+        }
+        tc_before();
+        bar_arrive(&bars.p_full[x][buf]);
+      }
+      if (ok) {
+        ok = bar_wait(&bars.pv_done[x][(chunks - 1) & 1], (chunks - 1) >> 1 & 1, stop, s.status);
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      if (ok) {
+        tc_after();
+        const float by = l == 0.0f ? 0.0f : pow2(unit) / l;
+        const uint32_t *bits = reinterpret_cast<const uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8));
+        T *out = static_cast<T *>(p.out) + (int64_t(u.start) + token) * p.o_ts + head * p.o_hs;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tm_ld32(o, o_at + c);
+          tm_wait_ld();
+          const uint32_t nan = nan_seen ? bits[c / 32] : 0;
+          if (nan != 0)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (nan >> i & 1) o[i] = 0x7fc00000u;
+          if (real) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint4 w;
+              w.x = pack2<T>(__uint_as_float(o[8 * i]) * by, __uint_as_float(o[8 * i + 1]) * by);
+              w.y = pack2<T>(__uint_as_float(o[8 * i + 2]) * by, __uint_as_float(o[8 * i + 3]) * by);
+              w.z = pack2<T>(__uint_as_float(o[8 * i + 4]) * by, __uint_as_float(o[8 * i + 5]) * by);
+              w.w = pack2<T>(__uint_as_float(o[8 * i + 6]) * by, __uint_as_float(o[8 * i + 7]) * by);
+              *reinterpret_cast<uint4 *>(out + c + 8 * i) = w;
+            }
+          }
+        }
+        tc_before();
+      }
+    }
+  }
+
+  // ---- every MMA issued has completed before the TMEM goes (bounded) ----
+  __syncthreads();
+  if (lane == 0 && warp <= W_QK) {
+    tc_commit(&bars.drain);
+    if (warp == W_PV) {
+      const unsigned long long t0 = now_ns();
+      while (!bar_try(smem_addr(&bars.drain), 0))
+        if (now_ns() - t0 > WAIT_NS) {
+          report(s.status, STATUS_WAIT);
+          break;
+        }
+    }
+  }
+  __syncthreads();
+  if (warp == W_PV) {
+    __syncwarp();
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+template <int D, typename T>
+cudaError_t launch(const AttendParams &p, unsigned grid, cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(tiles_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             Layout<D>::DYN);
+  if (e != cudaSuccess) return e;
+  tiles_kernel<D, T><<<grid, THREADS, Layout<D>::DYN, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t tiles_attend(const AttendParams &p, int head_dim, bool bf16, cudaStream_t stream) {
+  // row blocks of all sequences: at most one part-filled one each
+  const int64_t blocks = (int64_t(p.s.tokens) * p.group) / (2 * TILE) + p.s.seqs;
+  const int64_t grid = blocks * p.s.kv_heads;
+  if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  if (head_dim == 64)
+    return bf16 ? launch<64, __nv_bfloat16>(p, unsigned(grid), stream) : launch<64, __half>(p, unsigned(grid), stream);
+  return bf16 ? launch<128, __nv_bfloat16>(p, unsigned(grid), stream) : launch<128, __half>(p, unsigned(grid), stream);
+}
+
+}  // namespace kv8
