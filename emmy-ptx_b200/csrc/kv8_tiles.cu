@@ -7,10 +7,12 @@
 // sees.  Warps:
 //   0       tcgen05 O += P V of both tiles (one thread); owns the TMEM
 //   1       tcgen05 S = Q K^T of both tiles (one thread)
-//   2-5     softmax and output of tile A, a thread a row; 6-9 of tile B
-//   10-13   codes -> f16: global loads a chunk ahead, e4m3 -> f16 in
-//           registers, stored as the 128-byte-swizzled tiles the MMAs read
-//           (K as [keys][d], V as stored: an MN-major operand)
+//   2       bulk copies of the codes into shared memory, chunks ahead; 3 idle
+//   4-7     softmax and output of tile A, a thread a row; 8-11 of tile B
+//   12-15   codes -> f16, stored as the 128-byte-swizzled tiles the MMAs
+//           read (K as [keys][d], V as stored: an MN-major operand)
+// 128 registers a thread at launch; the softmax warps take 176 (a row's 64
+// scores and its packed weights are live together) from the others.
 // TMEM: per tile two 64-column S buffers (chunk g in buffer g % 2, P over its
 // first half as packed f16) and O.  With two buffers S of chunk g + 1 is
 // computed while the softmax works on chunk g.
@@ -25,8 +27,13 @@
 namespace kv8 {
 namespace {
 
-constexpr int TILE = 128, CHUNK = 64, STAGES = 4, THREADS = 448;
-constexpr int W_PV = 0, W_QK = 1, W_LOAD = 10;  // warps; 2-9 are the softmax
+constexpr int TILE = 128, CHUNK = 64, THREADS = 512;
+constexpr int STAGES = 3, RAW = 3;  // f16 chunks, and chunks of codes, in shared memory
+constexpr int W_PV = 0, W_QK = 1, W_FETCH = 2, W_SOFTMAX = 4, W_LOAD = 12;  // warps
+// Registers of the four warpgroups after the split.  The sum is what the
+// block was launched with: a split above it would wait for ever.
+constexpr int REGS_LAUNCH = 128, REGS_ISSUE = 64, REGS_SOFTMAX = 176, REGS_LOAD = 96;
+static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX + REGS_LOAD == 4 * REGS_LAUNCH, "register split");
 constexpr float LAZY = 8.0f, NONE = -1e30f, LEAST = 1e-37f;
 constexpr int UNIT_LAZY = 6;
 constexpr unsigned long long WAIT_NS = 2000000000ull;
@@ -35,7 +42,8 @@ template <int D>
 struct Layout {
   static constexpr int Q_TILE = TILE * D * 2, KV = CHUNK * D * 2;  // bytes
   static constexpr int STAGE0 = 2 * Q_TILE;
-  static constexpr int NAN_ROWS = STAGE0 + STAGES * 2 * KV;  // D bits a row
+  static constexpr int RAW0 = STAGE0 + STAGES * 2 * KV;    // K codes, then V codes
+  static constexpr int NAN_ROWS = RAW0 + RAW * KV;         // D bits a row
   static constexpr int END = NAN_ROWS + 2 * TILE * (D / 8);
   // 1 KB to align the tiles; above half an SM's shared memory, so that two
   // CTAs of one SM never wait for each other's TMEM
@@ -44,7 +52,7 @@ struct Layout {
 };
 
 struct Bars {
-  uint64_t q_full, kv_full[STAGES], kv_empty[STAGES];
+  uint64_t q_full, kv_full[STAGES], kv_empty[STAGES], raw_full[RAW], raw_empty[RAW];
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], drain;
 };
 
@@ -60,7 +68,7 @@ __device__ __forceinline__ void bar_arrive(uint64_t *b) {
 __device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 100000;\n\t"
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(b), "r"(parity)
@@ -72,42 +80,61 @@ __device__ __forceinline__ unsigned long long now_ns() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-// Waits for the phase of parity `parity`; false when the kernel gives up.
-__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile unsigned *stop,
-                                         unsigned *status) {
+// Waits with a whole warp, which stays converged, for the phase of parity
+// `parity`; false when the kernel gives up.
+__device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, volatile unsigned *stop,
+                                          unsigned *status) {
   const uint32_t at = smem_addr(b);
-  if (bar_try(at, parity)) return true;
+  if (__all_sync(0xffffffffu, bar_try(at, parity))) return true;
   const unsigned long long t0 = now_ns();
   for (;;) {
-    if (bar_try(at, parity)) return true;
-    if (*stop != 0) return false;
+    if (__all_sync(0xffffffffu, bar_try(at, parity))) return true;
+    bool over = *stop != 0;
     if (now_ns() - t0 > WAIT_NS) {
       *stop = 1;
       report(status, STATUS_WAIT);
-      return false;
+      over = true;
     }
+    if (__any_sync(0xffffffffu, over)) return false;
   }
+}
+// Every lane's earlier work is done: one arrival for the warp.
+__device__ __forceinline__ void warp_arrive(uint64_t *b) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) bar_arrive(b);
+}
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
 }
 
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t *b) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(b))
-               : "memory");
-}
-// D (+)= A B with A and B in shared memory, or A (TS) in TMEM.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// The issuing warps stay converged, so that descriptors live in uniform
+// registers; `who` is 1 in the one lane that issues.
+__device__ __forceinline__ void tc_commit(uint64_t *b, uint32_t who) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred e;\n\tsetp.ne.u32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(b)),
+      "r"(who)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// D (+)= A B with A and B in shared memory, or A (TS) in TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                                       uint32_t who) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(who)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                                       uint32_t who) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(who)
       : "memory");
 }
 __device__ __forceinline__ void tm_ld32(uint32_t (&r)[32], uint32_t at) {
@@ -129,6 +156,34 @@ __device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t (&r)[32]) {
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two f32 in one register pair.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -152,47 +207,24 @@ struct Unit {
   Span span;
 };
 
-// ---- codes -> f16 tiles (warps 10-13) ----
-template <int D>
-struct Codes {
-  static constexpr int N = D / 32;  // 16-byte pieces of K, and of V, a thread
-  uint4 k[N], v[N];
-  int key0, ek, ev;
-  bool dead;
+// A ring of n slots: slot and phase of step after step.
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++slot == n) slot = 0, phase ^= 1;
+  }
 };
 
-template <int D>
-__device__ __forceinline__ void load_codes(Codes<D> &c, const AttendParams &p, const Unit &u, int key0,
-                                           int page, int t) {
-  c.key0 = key0;
-  c.dead = page < 0 || page >= p.s.pages;
-  if (c.dead) {
-    report(p.s.status, STATUS_PAGE);
-    page = 0;
-  }
-  const int64_t unit = int64_t(page) * 2 * p.s.kv_heads + u.head;
-  c.ek = p.exps[unit];
-  c.ev = p.exps[unit + p.s.kv_heads];
-  const int slot = key0 & ((1 << p.s.page_shift) - 1);
-  const uint4 *k = reinterpret_cast<const uint4 *>(p.codes + ((unit << p.s.page_shift) + slot) * D);
-  const uint4 *v = k + ((int64_t(p.s.kv_heads) << p.s.page_shift) * D >> 4);
-#pragma unroll
-  for (int i = 0; i < Codes<D>::N; ++i) c.k[i] = k[i * 128 + t];
-#pragma unroll
-  for (int i = 0; i < Codes<D>::N; ++i) c.v[i] = v[i * 128 + t];
-}
+// What goes with a chunk of codes.
+struct ChunkInfo {
+  int ek, ev, key0, dead;
+};
 
-// One 16-byte piece of codes as 32 bytes of a swizzled f16 tile of 64 rows.
-template <int D>
-__device__ __forceinline__ void store_piece(uint8_t *tile, int piece, const uint4 &w) {
-  const int r = piece / (D / 16), col = piece % (D / 16), half = col / 4, j = 2 * (col % 4);
-  uint8_t *at = tile + half * (CHUNK * 128);
-  const uint4 lo = make_uint4(e4m3x2_f16x2(w.x), e4m3x2_f16x2(w.x >> 16), e4m3x2_f16x2(w.y), e4m3x2_f16x2(w.y >> 16));
-  const uint4 hi = make_uint4(e4m3x2_f16x2(w.z), e4m3x2_f16x2(w.z >> 16), e4m3x2_f16x2(w.w), e4m3x2_f16x2(w.w >> 16));
-  // the second 128-byte half starts with its odd piece: eight lanes that
-  // store together then touch eight different pieces
-  *reinterpret_cast<uint4 *>(at + swizzled(r, j + half)) = half ? hi : lo;
-  *reinterpret_cast<uint4 *>(at + swizzled(r, j + 1 - half)) = half ? lo : hi;
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_addr(bar))
+               : "memory");
 }
 
 template <int D, typename T>
@@ -202,8 +234,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
   uint8_t *const dyn = dyn_raw + ((1024 - (smem_addr(dyn_raw) & 1023)) & 1023);
   __shared__ Bars bars;
   __shared__ uint32_t tmem_slot;
-  __shared__ unsigned stop_word, scan[THREADS / 32], stage_nan[STAGES];
-  __shared__ float2 stage_scale[STAGES];  // 2^ek, ev
+  // Chunk g's scales (2^ek, ev) and whether it holds NaN values, in slot g % 4:
+  // by the time chunk g + 4 is written there, P V of chunk g + 1 is done and
+  // with it every softmax warp past chunk g.
+  __shared__ float2 chunk_scale[4];
+  __shared__ unsigned stop_word, scan[THREADS / 32], chunk_nan[4];
+  __shared__ ChunkInfo raw_info[RAW];
   __shared__ int found[2];
   volatile unsigned *const stop = &stop_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -261,16 +297,20 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 
   // ---- barriers, TMEM ----
   if (tid == 0) {
-    bar_init(&bars.q_full, tiles * TILE);
+    bar_init(&bars.q_full, tiles * 4);  // warps
     for (int i = 0; i < STAGES; ++i) {
-      bar_init(&bars.kv_full[i], 128);
+      bar_init(&bars.kv_full[i], 4);
       bar_init(&bars.kv_empty[i], 1);
-      stage_nan[i] = 0;
+    }
+    for (int i = 0; i < 4; ++i) chunk_nan[i] = 0;
+    for (int i = 0; i < RAW; ++i) {
+      bar_init(&bars.raw_full[i], 1);
+      bar_init(&bars.raw_empty[i], 4);
     }
     for (int x = 0; x < 2; ++x)
       for (int i = 0; i < 2; ++i) {
-        bar_init(&bars.s_full[x][i], 1);
-        bar_init(&bars.p_full[x][i], TILE);
+        bar_init(&bars.s_full[x][i], 2);
+        bar_init(&bars.p_full[x][i], 4);
         bar_init(&bars.pv_done[x][i], 1);
       }
     bar_init(&bars.drain, 2);
@@ -286,108 +326,170 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
   tc_after();
   const uint32_t tmem = tmem_slot;
 
+  bool issuer = false;  // the lane that issued this warp's MMAs
+  if (warp < W_SOFTMAX) regs_down<REGS_ISSUE>();
   if (warp == W_PV) {
     // ---- O += P V ----
-    if (lane == 0) {
-      constexpr uint32_t id = IDESC<TILE, D, true>;
-      bool ok = true;
-      for (int g = 0; ok && g < chunks; ++g) {
-        const int st = g % STAGES, buf = g & 1;
-        ok = bar_wait(&bars.kv_full[st], g / STAGES & 1, stop, s.status);
-        // V rows are 128 bytes (64 values of d), the second half of d follows
-        // CHUNK rows on; 16 keys are 2 KB
-        const uint64_t vd = smem_desc(smem_addr(dyn + L::STAGE0 + st * 2 * L::KV + L::KV), CHUNK * 128, 1024);
-        for (int x = 0; ok && x < tiles; ++x) {
-          ok = bar_wait(&bars.p_full[x][buf], g >> 1 & 1, stop, s.status);
-          if (!ok) break;
-          tc_after();
-          const uint32_t o = tmem + L::O_COL + x * D, pa = tmem + (2 * x + buf) * CHUNK;
+    const uint32_t who = elected();
+    bool ok = true;
+    Ring kv;
+    for (int g = 0; ok && g < chunks; ++g, kv.next(STAGES)) {
+      const int st = kv.slot, buf = g & 1;
+      ok = warp_wait(&bars.kv_full[st], kv.phase, stop, s.status);
+      // V rows are 128 bytes (64 values of d), the second half of d follows
+      // CHUNK rows on; 16 keys are 2 KB
+      const uint64_t vd = smem_desc(smem_addr(dyn + L::STAGE0 + st * 2 * L::KV + L::KV), CHUNK * 128, 1024);
+      for (int x = 0; ok && x < tiles; ++x) {
+        ok = warp_wait(&bars.p_full[x][buf], g >> 1 & 1, stop, s.status);
+        if (!ok) break;
+        tc_after();
+        const uint32_t o = tmem + L::O_COL + x * D, pa = tmem + (2 * x + buf) * CHUNK;
 #pragma unroll
-          for (int k = 0; k < CHUNK / 16; ++k)
-            mma_ts(o, pa + k * 8, vd + (k * 2048 >> 4), id, g > 0 || k > 0);
-          tc_commit(&bars.pv_done[x][buf]);
-        }
-        if (ok) tc_commit(&bars.kv_empty[st]);
+        for (int k = 0; k < CHUNK / 16; ++k)
+          mma_ts(o, pa + k * 8, vd + (k * 2048 >> 4), IDESC<TILE, D, true>, g > 0 || k > 0, who);
+        tc_commit(&bars.pv_done[x][buf], who);
       }
+      if (ok) tc_commit(&bars.kv_empty[st], who);
     }
+    if (who) issuer = true;
   } else if (warp == W_QK) {
     // ---- S = Q K^T ----
-    if (lane == 0) {
-      constexpr uint32_t id = IDESC<TILE, CHUNK, false>;
-      bool ok = bar_wait(&bars.q_full, 0, stop, s.status);
-      for (int g = 0; ok && g < chunks; ++g) {
-        const int st = g % STAGES, buf = g & 1;
-        ok = bar_wait(&bars.kv_full[st], g / STAGES & 1, stop, s.status);
-        const uint64_t kd = smem_desc(smem_addr(dyn + L::STAGE0 + st * 2 * L::KV), 16, 1024);
-        for (int x = 0; ok && x < tiles; ++x) {
-          // the buffer holds P of chunk g - 2 until its P V is done
-          if (g >= 2) ok = bar_wait(&bars.pv_done[x][buf], (g >> 1 & 1) ^ 1, stop, s.status);
-          if (!ok) break;
-          tc_after();
-          const uint64_t qd = smem_desc(smem_addr(dyn + x * L::Q_TILE), 16, 1024);
-          const uint32_t at = tmem + (2 * x + buf) * CHUNK;
+    const uint32_t who = elected();
+    bool ok = warp_wait(&bars.q_full, 0, stop, s.status);
+    Ring kv;
+    for (int g = 0; ok && g < chunks; ++g, kv.next(STAGES)) {
+      const int st = kv.slot, buf = g & 1;
+      ok = warp_wait(&bars.kv_full[st], kv.phase, stop, s.status);
+      const uint64_t kd = smem_desc(smem_addr(dyn + L::STAGE0 + st * 2 * L::KV), 16, 1024);
+      for (int x = 0; ok && x < tiles; ++x) {
+        // the buffer holds P of chunk g - 2 until its P V is done
+        if (g >= 2) ok = warp_wait(&bars.pv_done[x][buf], (g >> 1 & 1) ^ 1, stop, s.status);
+        if (!ok) break;
+        tc_after();
+        const uint64_t qd = smem_desc(smem_addr(dyn + x * L::Q_TILE), 16, 1024);
+        const uint32_t at = tmem + (2 * x + buf) * CHUNK;
 #pragma unroll
-          for (int h = 0; h < D / 64; ++h)
+        for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_ss(at, qd + ((h * TILE * 128 + k * 32) >> 4), kd + ((h * CHUNK * 128 + k * 32) >> 4), id, h > 0 || k > 0);
-          tc_commit(&bars.s_full[x][buf]);
+          for (int k = 0; k < 4; ++k)
+            mma_ss(at, qd + ((h * TILE * 128 + k * 32) >> 4), kd + ((h * CHUNK * 128 + k * 32) >> 4),
+                   IDESC<TILE, CHUNK, false>, h > 0 || k > 0, who);
+        tc_commit(&bars.s_full[x][buf], who);
+        // and one ordinary arrival, which passes on what the loading warps
+        // left beside the codes
+        if (who) bar_arrive(&bars.s_full[x][buf]);
+      }
+    }
+    if (who) issuer = true;
+  } else if (warp == W_FETCH) {
+    // ---- codes of a page's chunk: K and V are one contiguous piece each ----
+    const uint32_t who = elected();
+    const int *row = s.table + int64_t(u.b) * s.width;
+    Ring raw;
+    bool ok = true;
+    for (int g0 = 0; ok && g0 < chunks; g0 += 32) {
+      // 32 chunks' pages and exponents at once, a lane a chunk
+      ChunkInfo mine = {0, 0, 0, 0};
+      int64_t unit = 0;
+      if (g0 + lane < chunks) {
+        mine.key0 = u.span.key0(g0 + lane);
+        int page = row[mine.key0 >> s.page_shift];
+        mine.dead = page < 0 || page >= s.pages;
+        if (mine.dead) {
+          report(s.status, STATUS_PAGE);
+          page = 0;
         }
+        unit = int64_t(page) * 2 * s.kv_heads + u.head;
+        mine.ek = p.exps[unit];
+        mine.ev = p.exps[unit + s.kv_heads];
+      }
+      for (int i = 0; ok && i < 32 && g0 + i < chunks; ++i, raw.next(RAW)) {
+        if (g0 + i >= RAW) ok = warp_wait(&bars.raw_empty[raw.slot], raw.phase ^ 1, stop, s.status);
+        if (!ok) break;
+        const int64_t at = __shfl_sync(0xffffffffu, unit, i);
+        ChunkInfo c;
+        c.ek = __shfl_sync(0xffffffffu, mine.ek, i);
+        c.ev = __shfl_sync(0xffffffffu, mine.ev, i);
+        c.key0 = __shfl_sync(0xffffffffu, mine.key0, i);
+        c.dead = __shfl_sync(0xffffffffu, mine.dead, i);
+        if (who) {
+          raw_info[raw.slot] = c;
+          const uint8_t *k = p.codes + ((at << s.page_shift) + (c.key0 & ((1 << s.page_shift) - 1))) * D;
+          const uint8_t *v = k + (int64_t(s.kv_heads) << s.page_shift) * D;
+          const uint32_t dst = smem_addr(dyn + L::RAW0 + raw.slot * L::KV);
+          uint64_t *bar = &bars.raw_full[raw.slot];
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(L::KV)
+                       : "memory");
+          bulk_copy(dst, k, CHUNK * D, bar);
+          bulk_copy(dst + CHUNK * D, v, CHUNK * D, bar);
+        }
+        __syncwarp();
       }
     }
   } else if (warp >= W_LOAD) {
     // ---- codes -> f16 ----
-    const int t = tid - W_LOAD * 32;
-    const int *row = s.table + int64_t(u.b) * s.width;
-    const auto page_of = [&](int g) { return g < chunks ? row[u.span.key0(g) >> s.page_shift] : 0; };
-    const auto put = [&](Codes<D> &c, int g) {
-      const int st = g % STAGES;
-      if (g >= STAGES && !bar_wait(&bars.kv_empty[st], (g / STAGES & 1) ^ 1, stop, s.status)) return false;
-      uint8_t *k = dyn + L::STAGE0 + st * 2 * L::KV, *v = k + L::KV;
+    regs_down<REGS_LOAD>();
+    // A lane's 16-byte pieces of codes become two neighbouring 16-byte pieces
+    // of f16.  D = 128: eight lanes that load or store together cover the two
+    // halves of d in two neighbouring rows, so that neither the loads (rows of
+    // 128 bytes) nor the stores (pieces exchanged by row & 7) meet in a bank.
+    constexpr int PASS_ROWS = D == 128 ? 16 : 32, PASSES = CHUNK / PASS_ROWS;
+    const int w = warp - W_LOAD, c = lane & 3, b2 = lane >> 2 & 1;
+    const int r0 = D == 128 ? w * 4 + b2 + 2 * (lane >> 4) : w * 8 + (lane >> 2);
+    const int half = D == 128 ? b2 ^ (lane >> 3 & 1) : 0;
+    const uint32_t from = r0 * D + (half * 4 + c) * 16;
+    const uint32_t to = half * (CHUNK * 128) + swizzled(r0, 2 * c);
+    const auto put = [&](uint8_t *tile, int pass, const uint4 &x) {
+      uint8_t *at = tile + pass * (PASS_ROWS * 128);
+      *reinterpret_cast<uint4 *>(at + to) =
+          make_uint4(e4m3x2_f16x2(x.x), e4m3x2_f16x2(x.x >> 16), e4m3x2_f16x2(x.y), e4m3x2_f16x2(x.y >> 16));
+      *reinterpret_cast<uint4 *>(at + (to ^ 16)) =
+          make_uint4(e4m3x2_f16x2(x.z), e4m3x2_f16x2(x.z >> 16), e4m3x2_f16x2(x.w), e4m3x2_f16x2(x.w >> 16));
+    };
+    Ring raw, kv;
+    for (int g = 0; g < chunks; ++g, raw.next(RAW), kv.next(STAGES)) {
+      if (!warp_wait(&bars.raw_full[raw.slot], raw.phase, stop, s.status)) break;
+      const uint8_t *src = dyn + L::RAW0 + raw.slot * L::KV + from;
+      uint4 k[PASSES], v[PASSES];
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) k[i] = *reinterpret_cast<const uint4 *>(src + i * PASS_ROWS * D);
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) v[i] = *reinterpret_cast<const uint4 *>(src + CHUNK * D + i * PASS_ROWS * D);
+      const ChunkInfo info = raw_info[raw.slot];
+      warp_arrive(&bars.raw_empty[raw.slot]);
+      const int st = kv.slot;
+      if (g >= STAGES && !warp_wait(&bars.kv_empty[st], kv.phase ^ 1, stop, s.status)) break;
       // chunks some row does not see whole: values no row sees are zeroed and
       // a NaN is taken out here (0 * NaN would reach rows it is hidden from)
       // and put into the rows that see it at the end
-      if (c.dead || !u.span.all_see(c.key0, c.key0 + CHUNK - 1)) {
+      if (info.dead || !u.span.all_see(info.key0, info.key0 + CHUNK - 1)) {
 #pragma unroll
-        for (int i = 0; i < Codes<D>::N; ++i) {
-          const int key = c.key0 + (i * 128 + t) / (D / 16);
-          if (c.dead || !u.span.any_sees(key)) c.v[i] = make_uint4(0, 0, 0, 0);
-          uint32_t *w = &c.v[i].x;
+        for (int i = 0; i < PASSES; ++i) {
+          if (info.dead || !u.span.any_sees(info.key0 + r0 + i * PASS_ROWS)) v[i] = make_uint4(0, 0, 0, 0);
+          uint32_t *x = &v[i].x;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t bad = nan_bytes(w[j]);
+            const uint32_t bad = nan_bytes(x[j]);
             if (bad != 0) {
-              w[j] &= ~((bad >> 7) * 0xffu);
-              stage_nan[st] = 1;
+              x[j] &= ~((bad >> 7) * 0xffu);
+              chunk_nan[g & 3] = 1;
             }
           }
         }
       }
+      uint8_t *tile = dyn + L::STAGE0 + st * 2 * L::KV;
 #pragma unroll
-      for (int i = 0; i < Codes<D>::N; ++i) store_piece<D>(k, i * 128 + t, c.k[i]);
+      for (int i = 0; i < PASSES; ++i) put(tile, i, k[i]);
 #pragma unroll
-      for (int i = 0; i < Codes<D>::N; ++i) store_piece<D>(v, i * 128 + t, c.v[i]);
-      if (t == 0) stage_scale[st] = make_float2(c.dead ? 0.0f : pow2(c.ek), float(c.ev));
+      for (int i = 0; i < PASSES; ++i) put(tile + L::KV, i, v[i]);
+      if (tid == W_LOAD * 32) chunk_scale[g & 3] = make_float2(info.dead ? 0.0f : pow2(info.ek), float(info.ev));
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(&bars.kv_full[st]);
-      return true;
-    };
-    Codes<D> a, b;
-    int page = page_of(1);
-    load_codes(a, p, u, u.span.key0(0), page_of(0), t);
-    for (int g = 0; g < chunks; g += 2) {
-      if (g + 1 < chunks) load_codes(b, p, u, u.span.key0(g + 1), page, t);
-      page = page_of(g + 2);
-      if (!put(a, g)) break;
-      if (g + 1 < chunks) {
-        if (g + 2 < chunks) load_codes(a, p, u, u.span.key0(g + 2), page, t);
-        page = page_of(g + 3);
-        if (!put(b, g + 1)) break;
-      }
+      warp_arrive(&bars.kv_full[st]);
     }
-  } else {
+  } else if (warp >= W_SOFTMAX) {
     // ---- softmax: a thread a row ----
-    const int x = (warp - 2) >> 2, quad = warp & 3, r = quad * 32 + lane;
+    regs_up<REGS_SOFTMAX>();
+    const int x = (warp - W_SOFTMAX) >> 2, quad = warp & 3, r = quad * 32 + lane;
     if (x < tiles) {
       const int row = u.row0 + x * TILE + r;
       const bool real = row < u.rows;
@@ -434,30 +536,39 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
           *reinterpret_cast<uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8) + 4 * i) = 0;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(&bars.q_full);
+      warp_arrive(&bars.q_full);
 
       const uint32_t lanes = uint32_t(quad * 32) << 16;
       const uint32_t s_at = tmem + lanes + 2 * x * CHUNK, o_at = tmem + lanes + L::O_COL + x * D;
       float m = NONE, l = 0.0f;
       int unit = 0;
       bool ok = true, nan_seen = false;
+      // chunks whole_lo .. whole_hi - 1 every row sees whole
+      int whole_lo = 0, whole_hi = chunks;
+      {
+        const Span &sp = u.span;
+        if (p.window > 0) {
+          // from the first window chunk that starts inside the last token's window
+          const int low = max(0, sp.last - p.window + 1);
+          whole_lo = sp.sink_chunks + max(0, ((low + CHUNK - 1) >> 6) - sp.window_chunk0);
+        }
+        whole_hi = sp.sink_chunks + ((sp.first + 1) >> 6) - sp.window_chunk0;
+      }
       for (int g = 0; g < chunks; ++g) {
-        const int buf = g & 1, st = g % STAGES, key0 = u.span.key0(g);
-        // S is there, and what the loading warps left beside the codes
-        ok = bar_wait(&bars.s_full[x][buf], g >> 1 & 1, stop, s.status) &&
-             bar_wait(&bars.kv_full[st], g / STAGES & 1, stop, s.status);
-        ok = __all_sync(0xffffffffu, ok);
+        const int buf = g & 1;
+        ok = warp_wait(&bars.s_full[x][buf], g >> 1 & 1, stop, s.status);
         if (!ok) break;
+        const float2 sc = chunk_scale[g & 3];
+        const int ev = int(sc.y);
+        const float rm = fmaxf(mult * sc.x, LEAST);
         tc_after();
         uint32_t sv[2][32];
         tm_ld32(sv[0], s_at + buf * CHUNK);
         tm_ld32(sv[1], s_at + buf * CHUNK + 32);
-        const float2 sc = stage_scale[st];
-        const int ev = int(sc.y);
-        const float rm = fmaxf(mult * sc.x, LEAST);
         tm_wait_ld();
         const bool dead = sc.x == 0.0f;
-        if (dead || !u.span.all_see(key0, key0 + CHUNK - 1)) {
+        if (dead || g < whole_lo || g >= whole_hi) {
+          const int key0 = u.span.key0(g);
           // bit i: the row sees key key0 + i
           const auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
           uint64_t see = below(pos - key0 + 1);
@@ -466,7 +577,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 #pragma unroll
           for (int i = 0; i < 64; ++i)
             if (!(see >> i & 1)) sv[i / 32][i % 32] = 0xff800000u;
-          if (stage_nan[st] != 0 && real) {
+          if (chunk_nan[g & 3] != 0 && real) {
             // (rare) this chunk holds NaN values: which of them this row sees
             const int page = s.table[int64_t(u.b) * s.width + (key0 >> s.page_shift)];
             const int64_t at = (int64_t(page) * 2 + 1) * s.kv_heads + u.head;
@@ -483,12 +594,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
             nan_seen = true;
           }
         }
+        const auto score = [&](int i) { return __uint_as_float(sv[i / 32][i % 32]); };
         float top[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(sv[0][i]);
+        for (int i = 0; i < 4; ++i) top[i] = score(i);
 #pragma unroll
-        for (int i = 4; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(sv[i / 32][i % 32]));
-        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * rm;
+        for (int i = 4; i < 64; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], score(i), score(i + 1));
+        const float best = fmaxf(max3(top[0], top[1], top[2]), top[3]) * rm;
         const int stray = ev - unit;
         const bool first = g == 0, move = stray > UNIT_LAZY || stray < -UNIT_LAZY;
         const bool fix = __any_sync(0xffffffffu, best > m + LAZY) || move;
@@ -505,22 +617,26 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
           }
         }
         const float shift = float(ev - unit) - m;
-        float sum[4] = {};
+        const uint64_t rm2 = pair(rm, rm), shift2 = pair(shift, shift);
+        uint64_t sum[4] = {};
         uint32_t pk[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const float a = exp2_fast(fmaf(__uint_as_float(sv[i / 16][2 * i % 32]), rm, shift));
-          const float b = exp2_fast(fmaf(__uint_as_float(sv[i / 16][2 * i % 32 + 1]), rm, shift));
-          sum[i & 3] += a + b;
+          float a, b;
+          unpair(fma2(pair(score(2 * i), score(2 * i + 1)), rm2, shift2), a, b);
+          a = exp2_fast(a);
+          b = exp2_fast(b);
+          sum[i & 3] = add2(sum[i & 3], pair(a, b));
           pk[i] = pack2<__half>(a, b);
         }
         tm_st32(s_at + buf * CHUNK, pk);
-        l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), pow2(unit - ev), l);
+        float even, odd;
+        unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), even, odd);
+        l = fmaf(even + odd, pow2(unit - ev), l);
         tm_wait_st();
         if (fix && !first) {
           // P V of chunk g - 1 is the last to have touched O
-          ok = bar_wait(&bars.pv_done[x][(g - 1) & 1], (g - 1) >> 1 & 1, stop, s.status);
-          ok = __all_sync(0xffffffffu, ok);
+          ok = warp_wait(&bars.pv_done[x][(g - 1) & 1], (g - 1) >> 1 & 1, stop, s.status);
           if (!ok) break;
           tc_after();
 #pragma unroll
@@ -535,12 +651,9 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
           tm_wait_st();
         }
         tc_before();
-        bar_arrive(&bars.p_full[x][buf]);
+        warp_arrive(&bars.p_full[x][buf]);
       }
-      if (ok) {
-        ok = bar_wait(&bars.pv_done[x][(chunks - 1) & 1], (chunks - 1) >> 1 & 1, stop, s.status);
-        ok = __all_sync(0xffffffffu, ok);
-      }
+      if (ok) ok = warp_wait(&bars.pv_done[x][(chunks - 1) & 1], (chunks - 1) >> 1 & 1, stop, s.status);
       if (ok) {
         tc_after();
         const float by = l == 0.0f ? 0.0f : pow2(unit) / l;
@@ -575,8 +688,14 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 
   // ---- every MMA issued has completed before the TMEM goes (bounded) ----
   __syncthreads();
-  if (lane == 0 && warp <= W_QK) {
-    tc_commit(&bars.drain);
+  if (*stop != 0 && tid == W_FETCH * 32) {
+    // given up: copies in flight land before the block may end (50 ms)
+    const unsigned long long t0 = now_ns();
+    while (now_ns() - t0 < 50000000ull) {
+    }
+  }
+  if (issuer) {
+    tc_commit(&bars.drain, 1);
     if (warp == W_PV) {
       const unsigned long long t0 = now_ns();
       while (!bar_try(smem_addr(&bars.drain), 0))
@@ -596,8 +715,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 
 template <int D, typename T>
 cudaError_t launch(const AttendParams &p, unsigned grid, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(tiles_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             Layout<D>::DYN);
+  cudaFuncAttributes at;
+  cudaError_t e = cudaFuncGetAttributes(&at, tiles_kernel<D, T>);
+  if (e != cudaSuccess) return e;
+  if (at.numRegs != REGS_LAUNCH) return cudaErrorInvalidKernelImage;  // the split would not add up
+  e = cudaFuncSetAttribute(tiles_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::DYN);
   if (e != cudaSuccess) return e;
   tiles_kernel<D, T><<<grid, THREADS, Layout<D>::DYN, stream>>>(p);
   return cudaGetLastError();
