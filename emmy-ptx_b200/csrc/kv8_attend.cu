@@ -78,24 +78,25 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   p.group = a->heads / cache->kv_heads;
   p.window = a->window;
   p.sinks = a->sinks;
-  p.most_rows = p.group * cache->max_q;
+  p.target = 0;
   // A sequence with up to ROWS_MOST rows of a kv head is the row kernel's,
   // others the tile kernel's, which takes the one sequence of a call that may
   // be either.
-  const bool tiles = p.most_rows > ROWS_MOST, rows = !tiles || cache->seqs > 1;
+  const int64_t most = int64_t(p.group) * cache->max_q;
+  const bool tiles = most > ROWS_MOST, rows = !tiles || cache->seqs > 1;
   p.row_limit = rows ? ROWS_MOST : 0;
-  if (tiles && rows) p.most_rows = ROWS_MOST;
-  const int nt = rows_blocks(p.most_rows);
-  // the line of chunks is counted in 32 bits
-  const double line = double(cache->seqs) * cache->kv_heads * 4 *
-                      (double(cache->table_width) * cache->page_size / 64);
-  if (line > 4e9) return fail(EMMY_EINVAL, WHAT, "too many sequences, heads and keys for one call");
+  const int nt = rows_blocks(most < ROWS_MOST ? most : ROWS_MOST);
+  if (int64_t(cache->pages) * 2 * cache->kv_heads * cache->page_size > 0x7fffffff)
+    return fail(EMMY_EINVAL, WHAT, "a layer holds at most 2^31 - 1 rows of head_dim codes");
+  if (int64_t(cache->seqs) * cache->kv_heads > (1 << 24))
+    return fail(EMMY_EINVAL, WHAT, "too many sequences and heads for one call");
   const OnDevice on(cache->device);
   if (on.err != cudaSuccess) return cuda_fail(WHAT, on.err);
   const bool bf16 = a->dtype == EMMY_KV8_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaSuccess;
-  if (tiles) e = tiles_attend(p, cache->head_dim, bf16, st);
-  if (e == cudaSuccess && rows) e = rows_attend(p, nt, cache->head_dim, bf16, cache->device, st);
-  return e == cudaSuccess ? EMMY_OK : cuda_fail(WHAT, e);
+  if (tiles) {
+    const cudaError_t e = tiles_attend(p, cache->head_dim, bf16, st);
+    if (e != cudaSuccess) return cuda_fail(WHAT, e);
+  }
+  return rows ? rows_attend(p, *cache, nt, bf16, st) : EMMY_OK;
 }

@@ -20,7 +20,7 @@ struct AttendParams {
   int group;         // query heads of a kv head
   int window, sinks;
   int row_limit;     // sequences with more rows of a kv head than this are the tile kernel's
-  int most_rows;     // rows of a kv head in the largest sequence
+  int target;        // parts that the row kernel is to cut its segments into
 };
 
 // Which keys a block of query rows sees, and the 64-key chunks that hold
@@ -107,7 +107,6 @@ constexpr int ROWS_MOST = 32;
 cudaError_t tiles_attend(const AttendParams &p, int head_dim, bool bf16, cudaStream_t stream);
 int rows_blocks(int64_t rows);
 uint64_t rows_partial_bytes(int nt, int head_dim, int device);
-cudaError_t rows_attend(const AttendParams &p, int nt, int head_dim, bool bf16, int device,
-                        cudaStream_t stream);
+int rows_attend(AttendParams p, const emmy_kv8 &cache, int nt, bool bf16, cudaStream_t stream);
 
 }  // namespace kv8

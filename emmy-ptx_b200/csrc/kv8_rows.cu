@@ -14,27 +14,36 @@
 // maxima, sums and O are f32; p is rounded to f16 (2^-12 relative), the only
 // rounding of width before the output's.
 //
-// No operand goes through shared memory.  The order of a contraction's terms
-// is free, so each lane's 16 consecutive bytes of a key serve as its shares
-// of four k-steps, and of a value row as the rows 2i, 2i+1 of D / 16 m-tiles:
-// every load is 8 or 16 bytes and a warp's cover whole 64-128-byte pieces of rows.
+// The order of a contraction's terms is free, so a lane's 16 consecutive bytes
+// of a key serve as its shares of four k-steps, and of a value row as the rows
+// 2i, 2i+1 of D / 16 m-tiles: codes go from shared memory to MMA fragments by
+// 8- and 16-byte loads and one conversion, with no shuffles.  A fifth warp
+// brings 64-key chunks of K and V by TMA, several ahead: the bytes in flight
+// that HBM's latency asks for cost no registers.  The TMA's swizzle spreads
+// the rows that the lanes of a load read over all banks.
 //
-// Bound by memory: codes are read once per kv head.  The visible 64-key
-// chunks of all (sequence, head, row block) lie on one line that the grid
-// cuts into equal parts, so uneven lengths balance and one long sequence
-// fills the GPU.  A part that covers a segment only partly leaves (m, l, O)
-// in the workspace; the last of the segment's parts to arrive joins them in
-// the parts' order, so results do not depend on which came last.
+// Bound by memory: codes are read once per kv head.  A segment -- one sequence
+// and kv head -- is cut into about as many parts of 64-key chunks as its share
+// of a target number of parts, a CTA a part, so uneven lengths balance and
+// one long sequence fills the GPU, while a segment of about a part's length
+// stays whole and needs no join.  Parts of a cut segment leave (m, l, O) in
+// the workspace; the last of each 16 parts to arrive joins them in their
+// order, the last of those their sums, so results do not depend on the order
+// of arrival.
 #include <cuda_bf16.h>
 
-#include "kv8.cuh"
+#include <cuda.h>  // CUtensorMap
+
+#include "kv8_async.cuh"
 #include "kv8_attend.cuh"
 
 namespace kv8 {
 namespace {
 
-constexpr int THREADS = 128, WARPS = 4;
+constexpr int WARPS = 4, THREADS = 160, ALL_WARPS = 5;  // four that compute, one that loads
 constexpr float LAZY = 8.0f;  // log2 units that scores may pass the reference before O moves
+constexpr int GROUP = 16;     // parts of a segment that one CTA joins at once,
+constexpr int ONE_LEVEL = 24; // or up to this many where that leaves one level
 constexpr int UNIT_LAZY = 6;  // the same for V's exponent: p stays below 2^14 in f16
 constexpr float NONE = -1e30f;
 
@@ -51,55 +60,160 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return r;
 }
 
-// The geometry of one (sequence, head, row block) and of its chunk line.
+// The geometry of one (sequence, head) and of its chunk line.
 struct Segment {
   int b, head, start, n, len;  // n new tokens, rows from `start`; len keys
-  int rows, row0;              // rows of the kv head, first row of this block
+  int rows;                    // rows of the kv head, at most 8 NT
+  int part, parts, slot0;      // this CTA's part, of how many; workspace slot of part 0
   Span span;
 };
 
-// Codes and exponents of 16 keys, as a lane holds them: K rows g and g + 8
-// (16 bytes at 64 j + 16 q), V rows 2q, 2q+1, 2q+8, 2q+9 (D / 8 bytes at
-// g D / 8), with g = lane / 4, q = lane % 4.
-template <int D>
-struct Tile {
-  uint32_t k[2][D / 16], v[4][D / 32];
-  int ek, ev, key0;
-  bool dead;  // the page number was bad: every key hidden
+// 64-key chunks of sequence b that this kernel is to read (0: not its own).
+__device__ __forceinline__ int seq_chunks(const AttendParams &p, int b) {
+  int start, n, len;
+  if (b >= p.s.seqs) return 0;
+  lengths(p.s, b, start, n, len);
+  return n == 0 || n * p.group > p.row_limit ? 0 : Span(p, len - n, len - 1).chunks;
+}
+// Parts of a segment of c chunks, at q chunks a part.
+__device__ __forceinline__ int parts_of(int c, int q) {
+  return c == 0 ? 0 : max(1, min((2 * c + q) / (2 * q), c));
+}
+// Chunks a part so that there are about p.target parts.
+__device__ __forceinline__ int part_chunks(const AttendParams &p, int64_t total) {
+  return int((total * p.s.kv_heads + p.target - 1) / p.target);
+}
+
+__device__ __forceinline__ int warp_sum(int x) {
+  for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
+__device__ __forceinline__ int warp_scan(int x, int lane) {  // inclusive
+  for (int d = 1; d < 32; d <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += u;
+  }
+  return x;
+}
+
+// Which segment and part is CTA `want`'s: g.b, g.head, g.part, g.parts, g.slot0.
+// Up to 32 sequences every warp finds it for itself, a lane a sequence.
+__device__ __forceinline__ bool locate(const AttendParams &p, Segment &g, int want, int lane, int warp) {
+  const int H = p.s.kv_heads;
+  if (p.s.seqs <= 32) {
+    const int c = seq_chunks(p, lane);
+    const int q = part_chunks(p, warp_sum(c));
+    const int k = q == 0 ? 0 : parts_of(c, q);
+    const int at = warp_scan(k * H, lane), slot = warp_scan(k > 1 ? k * H : 0, lane);
+    const int b = __popc(__ballot_sync(0xffffffffu, at <= want));
+    if (b >= p.s.seqs) return false;
+    g.b = b;
+    g.parts = __shfl_sync(0xffffffffu, k, b);
+    const int rel = want - (__shfl_sync(0xffffffffu, at, b) - g.parts * H);
+    g.head = rel / g.parts;
+    g.part = rel - g.head * g.parts;
+    g.slot0 = __shfl_sync(0xffffffffu, slot, b) - g.parts * H + g.head * g.parts;
+    return true;
+  }
+  __shared__ long long sums[ALL_WARPS];
+  __shared__ int scans[2][ALL_WARPS], found[5];
+  const int tid = threadIdx.x, per = (p.s.seqs + THREADS - 1) / THREADS;
+  const int b0 = min(tid * per, p.s.seqs), b1 = min(b0 + per, p.s.seqs);
+  long long chunks = 0;
+  for (int b = b0; b < b1; ++b) chunks += seq_chunks(p, b);
+  for (int d = 16; d > 0; d >>= 1) chunks += __shfl_xor_sync(0xffffffffu, chunks, d);
+  if (lane == 0) sums[warp] = chunks;
+  if (tid == 0) found[0] = -1;
+  __syncthreads();
+  chunks = 0;
+  for (int w = 0; w < ALL_WARPS; ++w) chunks += sums[w];
+  const int q = part_chunks(p, chunks);
+  if (q == 0) return false;
+  int parts = 0, slots = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int k = parts_of(seq_chunks(p, b), q);
+    parts += k * H;
+    slots += k > 1 ? k * H : 0;
+  }
+  int at = warp_scan(parts, lane), slot = warp_scan(slots, lane);
+  if (lane == 31) scans[0][warp] = at, scans[1][warp] = slot;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) at += scans[0][w], slot += scans[1][w];
+  at -= parts;
+  slot -= slots;
+  if (want >= at && want < at + parts) {  // one thread's share holds it
+    for (int b = b0; b < b1; ++b) {
+      const int k = parts_of(seq_chunks(p, b), q);
+      if (want < at + k * H) {
+        found[0] = b;
+        found[1] = (want - at) / k;
+        found[2] = (want - at) % k;
+        found[3] = k;
+        found[4] = slot + found[1] * k;
+        break;
+      }
+      at += k * H;
+      slot += k > 1 ? k * H : 0;
+    }
+  }
+  __syncthreads();
+  g.b = found[0], g.head = found[1], g.part = found[2], g.parts = found[3], g.slot0 = found[4];
+  return g.b >= 0;
+}
+
+// What goes with a chunk of codes.
+struct ChunkInfo {
+  int key0, ek, ev, dead;
 };
 
+// Shared memory: the ring of chunks (K rows, then V rows; the join of the warps
+// once the loop is over), then the staged queries.
+template <int D, int NT>
+struct Layout {
+  static constexpr int CHUNK = 2 * 64 * D;
+  static constexpr int STAGES = (NT <= 2 ? 64 : 96) * 1024 / CHUNK;
+  static constexpr int QUERIES = STAGES * CHUNK, END = QUERIES + NT * 16 * D;
+  static constexpr int DYN = END + 1024;  // the swizzle repeats every 1 KB
+  static constexpr int LD = D + 8;        // floats of a row of the join
+  static_assert(WARPS * 8 * NT * LD * 4 <= QUERIES, "the join fits over the ring");
+  static_assert(2 * 64 * 8 * NT * 4 <= QUERIES, "so do the maxima and sums of 64 parts");
+};
+
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, int row, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
+          "r"(dst),
+      "l"(map), "r"(0), "r"(row), "r"(smem_addr(bar))
+      : "memory");
+}
+
+// Codes of 16 keys as a lane holds them, g = lane / 4, q = lane % 4: K rows g
+// and g + 8 (D / 4 bytes at q D / 4), V rows 2q, 2q+1, 2q+8, 2q+9 (D / 8 bytes
+// at g D / 8).  The swizzle exchanges a row's 16-byte pieces: by row & 7 in
+// rows of 128 bytes, by row / 2 & 3 in rows of 64.
 template <int D>
-__device__ __forceinline__ void load_tile(Tile<D> &t, const AttendParams &p, const Segment &g,
-                                          int key0, int page, int lane) {
-  t.key0 = key0;
-  t.dead = page < 0 || page >= p.s.pages;
-  if (t.dead) {
-    report(p.s.status, STATUS_PAGE);
-    page = 0;
-  }
-  const int64_t unit = int64_t(page) * 2 * p.s.kv_heads + g.head;
-  t.ek = p.exps[unit];
-  t.ev = p.exps[unit + p.s.kv_heads];
-  const int slot = key0 & ((1 << p.s.page_shift) - 1);
-  const uint8_t *k = p.codes + ((unit << p.s.page_shift) + slot) * D;
-  const uint8_t *v = k + ((int64_t(p.s.kv_heads) << p.s.page_shift) * D);
-  const int gr = lane >> 2, q = lane & 3;
+__device__ __forceinline__ void load_k(uint32_t (&k)[2][D / 16], const uint8_t *rows, int gr, int q) {
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
-      const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(k + (gr + 8 * i) * D + 64 * j + 16 * q));
-      t.k[i][4 * j] = w.x, t.k[i][4 * j + 1] = w.y, t.k[i][4 * j + 2] = w.z, t.k[i][4 * j + 3] = w.w;
+      const int piece = D == 128 ? (2 * q + j) ^ gr : q ^ (gr >> 1 & 3);
+      const uint4 w = *reinterpret_cast<const uint4 *>(rows + (gr + 8 * i) * D + 16 * piece);
+      k[i][4 * j] = w.x, k[i][4 * j + 1] = w.y, k[i][4 * j + 2] = w.z, k[i][4 * j + 3] = w.w;
     }
+}
+template <int D>
+__device__ __forceinline__ void load_v(uint32_t (&v)[4][D / 32], const uint8_t *rows, int gr, int q) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint8_t *at = v + (2 * q + (i & 1) + 8 * (i >> 1)) * D + gr * (D / 8);
+    const int r = 2 * q + (i & 1);  // row & 7
+    const uint8_t *row = rows + (r + 8 * (i >> 1)) * D;
     if constexpr (D == 64) {
-      const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(at));
-      t.v[i][0] = w.x, t.v[i][1] = w.y;
+      const uint2 w = *reinterpret_cast<const uint2 *>(row + 16 * ((gr >> 1) ^ q) + 8 * (gr & 1));
+      v[i][0] = w.x, v[i][1] = w.y;
     } else {
-      const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(at));
-      t.v[i][0] = w.x, t.v[i][1] = w.y, t.v[i][2] = w.z, t.v[i][3] = w.w;
+      const uint4 w = *reinterpret_cast<const uint4 *>(row + 16 * (gr ^ r));
+      v[i][0] = w.x, v[i][1] = w.y, v[i][2] = w.z, v[i][3] = w.w;
     }
   }
 }
@@ -109,85 +223,25 @@ template <int D, int NT>
 struct State {
   float o[D / 16][NT][4];
   float m[NT][2], l[NT][2];
-  float mult[NT][2];  // scale * log2(e) * the row's power of two
-  int pos[NT][2];     // position of the row's token, -1: no such row
   int unit;           // O is in units of 2^unit
 };
 
+// Scores in log2 units -> weights, b = P^T as B fragments; moves the maxima
+// and O where it must.
 template <int D, int NT>
-__device__ __forceinline__ void scale_o(State<D, NT> &st, const float (&f)[NT][2]) {
-#pragma unroll
-  for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      st.o[i][t][0] *= f[t][0], st.o[i][t][2] *= f[t][0];
-      st.o[i][t][1] *= f[t][1], st.o[i][t][3] *= f[t][1];
-    }
-}
-
-template <int D, int NT, typename Q>
-__device__ __forceinline__ void tile_step(State<D, NT> &st, Tile<D> &t, const AttendParams &p,
-                                          const Segment &g, const Q &query, int lane) {
-  const int gr = lane >> 2, q = lane & 3;
-  // ---- S^T = K Q^T ----
-  float s[NT][4] = {};
-#pragma unroll
-  for (int w = 0; w < D / 16; ++w) {
-    const uint32_t a[4] = {e4m3x2_f16x2(t.k[0][w]), e4m3x2_f16x2(t.k[1][w]),
-                           e4m3x2_f16x2(t.k[0][w] >> 16), e4m3x2_f16x2(t.k[1][w] >> 16)};
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const uint2 b = query(w, i);
-      mma(s[i], a, b.x, b.y);
-    }
-  }
-  const float mk = pow2(t.ek);
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) s[i][c] *= st.mult[i][c & 1] * mk;
-  // ---- hidden keys: only in tiles that some row does not see whole ----
-  const bool masked = t.dead || !g.span.all_see(t.key0, t.key0 + 15);
-  uint32_t nan_at[4] = {};  // bit d: value d of the lane's V row i is NaN
-  bool any_nan = false;
-  if (masked) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (t.dead || !g.span.sees(st.pos[i][c & 1], t.key0 + gr + 8 * (c >> 1))) s[i][c] = -INFINITY;
-    // A hidden key has p = 0, but 0 * NaN is NaN: values no row sees become
-    // zero, and a NaN that only some rows see is taken out here and put into
-    // those rows' sums below.
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool seen = !t.dead && g.span.any_sees(t.key0 + 2 * q + (i & 1) + 8 * (i >> 1));
-#pragma unroll
-      for (int w = 0; w < D / 32; ++w) {
-        if (!seen) t.v[i][w] = 0;
-        const uint32_t bad = nan_bytes(t.v[i][w]);
-        if (bad != 0) {
-          t.v[i][w] &= ~((bad >> 7) * 0xffu);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) nan_at[i] |= ((bad >> (8 * j + 7)) & 1u) << (4 * w + j);
-        }
-      }
-    }
-    any_nan = __any_sync(0xffffffffu, (nan_at[0] | nan_at[1] | nan_at[2] | nan_at[3]) != 0);
-  }
-  // ---- running maxima, kept while no score passes them by more than LAZY ----
+__device__ __forceinline__ void softmax_step(State<D, NT> &st, float (&s)[NT][4], uint32_t (&b)[NT][2], int ev) {
   bool grow = false;
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int c = 0; c < 4; ++c) grow |= s[i][c] > st.m[i][c & 1] + LAZY;
-  const bool move = t.ev - st.unit > UNIT_LAZY || st.unit - t.ev > UNIT_LAZY;
+  const bool move = ev - st.unit > UNIT_LAZY || st.unit - ev > UNIT_LAZY;
   if (__any_sync(0xffffffffu, grow) || move) {
-    float f[NT][2];
-    const float unit = move ? pow2(st.unit - t.ev) : 1.0f;
-    if (move) st.unit = t.ev;
+    const float unit = move ? pow2(st.unit - ev) : 1.0f;
+    if (move) st.unit = ev;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < NT; ++i) {
+      float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float top = fmaxf(s[i][c], s[i][c + 2]);
@@ -195,16 +249,20 @@ __device__ __forceinline__ void tile_step(State<D, NT> &st, Tile<D> &t, const At
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
         top = fmaxf(top, st.m[i][c]);
-        f[i][c] = exp2_fast(st.m[i][c] - top);
+        f[c] = exp2_fast(st.m[i][c] - top);
         st.m[i][c] = top;
-        st.l[i][c] *= f[i][c];
-        f[i][c] *= unit;
+        st.l[i][c] *= f[c];
+        f[c] *= unit;
       }
-    scale_o(st, f);
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        st.o[j][i][0] *= f[0], st.o[j][i][2] *= f[0];
+        st.o[j][i][1] *= f[1], st.o[j][i][3] *= f[1];
+      }
+    }
   }
-  // ---- p = 2^(s - m) in units of 2^(unit - ev); P^T by 8 x 8 transposes ----
-  const float dev = float(t.ev - st.unit), undo = pow2(st.unit - t.ev);
-  uint32_t b[NT][2];
+  // p = 2^(s - m) in units of 2^(unit - ev); P^T by 8 x 8 transposes
+  const float dev = float(ev - st.unit), undo = pow2(st.unit - ev);
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     float e[4];
@@ -216,41 +274,72 @@ __device__ __forceinline__ void tile_step(State<D, NT> &st, Tile<D> &t, const At
     b[i][0] = transpose8x8(*reinterpret_cast<const uint32_t *>(&lo));
     b[i][1] = transpose8x8(*reinterpret_cast<const uint32_t *>(&hi));
   }
-  // ---- O^T += V^T P^T ----
+}
+
+// O^T += V^T P^T of 16 keys.
+template <int D, int NT>
+__device__ __forceinline__ void pv_step(State<D, NT> &st, const uint32_t (&v)[4][D / 32], const uint32_t (&b)[NT][2]) {
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) {
     const uint32_t sel = i & 1 ? 0x7362 : 0x5140;  // (key 2q, key 2q+1) of two neighbouring d
-    const uint32_t x = __byte_perm(t.v[0][i / 2], t.v[1][i / 2], sel);
-    const uint32_t y = __byte_perm(t.v[2][i / 2], t.v[3][i / 2], sel);
+    const uint32_t x = __byte_perm(v[0][i / 2], v[1][i / 2], sel);
+    const uint32_t y = __byte_perm(v[2][i / 2], v[3][i / 2], sel);
     const uint32_t a[4] = {e4m3x2_f16x2(x), e4m3x2_f16x2(x >> 16), e4m3x2_f16x2(y), e4m3x2_f16x2(y >> 16)};
 #pragma unroll
     for (int r = 0; r < NT; ++r) mma(st.o[i][r], a, b[r][0], b[r][1]);
   }
-  if (any_nan) {
-    uint32_t rows[NT][2] = {};  // bit d: the row sees a NaN in value d
-    for (int from = 0; from < 4; ++from)
+}
+
+// A hidden key has p = 0, but 0 * NaN is NaN: values of a tile that no row sees
+// become zero, and a NaN that only some rows see is taken out and put into
+// those rows' sums (after their P V) by put_nan.
+template <int D>
+__device__ __forceinline__ bool take_nan(uint32_t (&v)[4][D / 32], uint32_t (&nan_at)[4], const Segment &g,
+                                         int key0, bool dead, int q) {
+  uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t bits = __shfl_sync(0xffffffffu, nan_at[i], (lane & ~3) | from);
-        const int key = t.key0 + 2 * from + (i & 1) + 8 * (i >> 1);
+  for (int i = 0; i < 4; ++i) {
+    nan_at[i] = 0;  // bit d: value d of the lane's V row i is NaN
+    const bool seen = !dead && g.span.any_sees(key0 + 2 * q + (i & 1) + 8 * (i >> 1));
 #pragma unroll
-        for (int r = 0; r < NT; ++r)
+    for (int w = 0; w < D / 32; ++w) {
+      if (!seen) v[i][w] = 0;
+      const uint32_t bad = nan_bytes(v[i][w]);
+      if (bad != 0) {
+        v[i][w] &= ~((bad >> 7) * 0xffu);
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-            if (g.span.sees(st.pos[r][c], key)) rows[r][c] |= bits;
+        for (int j = 0; j < 4; ++j) nan_at[i] |= ((bad >> (8 * j + 7)) & 1u) << (4 * w + j);
       }
+    }
+    any |= nan_at[i];
+  }
+  return __any_sync(0xffffffffu, any != 0);
+}
+template <int D, int NT>
+__device__ __forceinline__ void put_nan(State<D, NT> &st, const uint32_t (&nan_at)[4], const Segment &g,
+                                        const int *row_pos, int key0, int lane) {
+  uint32_t rows[NT][2] = {};  // bit d: the row sees a NaN in value d
+  for (int from = 0; from < 4; ++from)
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i)
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t bits = __shfl_sync(0xffffffffu, nan_at[i], (lane & ~3) | from);
+      const int key = key0 + 2 * from + (i & 1) + 8 * (i >> 1);
 #pragma unroll
       for (int r = 0; r < NT; ++r)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (rows[r][c & 1] >> (2 * i + (c >> 1)) & 1u) st.o[i][r][c] = NAN;
-  }
+        for (int c = 0; c < 2; ++c)
+          if (g.span.sees(row_pos[8 * r + 2 * (lane & 3) + c], key)) rows[r][c] |= bits;
+    }
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int r = 0; r < NT; ++r)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (rows[r][c & 1] >> (2 * i + (c >> 1)) & 1u) st.o[i][r][c] = NAN;
 }
 
-// One row's share of a lane: Q[64 j + 16 q .. + 15] for each j, scaled into
-// f16; returns the row's exponent (row = f16 row * 2^exponent).
+// One row's share of a lane: Q[q D / 4 .. + D / 4 - 1], scaled into f16; returns the row's exponent (row = f16 row * 2^exponent).
 template <int D, typename T>
 __device__ __forceinline__ int query_row(uint32_t (&f)[D / 8], const T *row, int q) {
   float x[D / 4];
@@ -260,7 +349,7 @@ __device__ __forceinline__ int query_row(uint32_t (&f)[D / 8], const T *row, int
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint4 w = make_uint4(0, 0, 0, 0);
-      if (row != nullptr) w = *reinterpret_cast<const uint4 *>(row + 64 * j + 16 * q + 8 * h);
+      if (row != nullptr) w = *reinterpret_cast<const uint4 *>(row + D / 4 * q + 16 * j + 8 * h);
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) unpack2<T>(u[i], x[16 * j + 8 * h + 2 * i], x[16 * j + 8 * h + 2 * i + 1]);
@@ -280,306 +369,424 @@ __device__ __forceinline__ int query_row(uint32_t (&f)[D / 8], const T *row, int
 }
 
 // Shared memory: first the joined rows of the four warps, over the staged queries.
-template <int D, int NT>
-constexpr int SMEM_JOIN = WARPS * 8 * NT * (D + 8) * 4;
-static_assert(SMEM_JOIN<64, 1> >= 1 * 32 * 64 / 8 * 4, "the staged queries fit under the join");
-
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(THREADS, NT == 1 ? 4 : NT == 2 ? 3 : 2)
-rows_kernel(const AttendParams p) {
-  constexpr int ROWS = 8 * NT, LD = D + 8;
-  extern __shared__ __align__(16) uint8_t dyn[];
+__global__ void __launch_bounds__(THREADS, NT <= 2 ? 3 : 2)
+rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map) {
+  using L = Layout<D, NT>;
+  constexpr int ROWS = 8 * NT, LD = L::LD;
+  extern __shared__ uint8_t dyn_raw[];
+  uint8_t *const dyn = dyn_raw + ((1024 - (smem_addr(dyn_raw) & 1023)) & 1023);
   float *const join = reinterpret_cast<float *>(dyn);
   __shared__ float sm_m[WARPS][ROWS], sm_l[WARPS][ROWS], weight[WARPS][ROWS], row_l[ROWS], row_m[ROWS];
-  __shared__ int sm_unit[WARPS], row_exp[ROWS];
-  __shared__ unsigned ticket;
-  __shared__ unsigned scan[WARPS];
-  uint32_t *const line = reinterpret_cast<uint32_t *>(dyn + SMEM_JOIN<D, NT>);  // [seqs + 1]
+  __shared__ int sm_unit[WARPS], row_pos[ROWS];  // position of the row's token, -1: no such row
+  __shared__ float row_mult[ROWS];               // scale * log2(e) * the row's power of two
+  __shared__ unsigned ticket, stop_word;
+  __shared__ uint64_t full[L::STAGES], empty[L::STAGES];
+  __shared__ ChunkInfo infos[L::STAGES];
+  volatile unsigned *const stop = &stop_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gr = lane >> 2, q = lane & 3;
   const Seqs &s = p.s;
-
-  // ---- the line of chunks: where each sequence starts ----
-  {
-    const int per = (s.seqs + THREADS - 1) / THREADS, b0 = min(tid * per, s.seqs), b1 = min(b0 + per, s.seqs);
-    unsigned sum = 0;
-    for (int b = b0; b < b1; ++b) {
-      int start, n, len;
-      lengths(s, b, start, n, len);
-      if (n * p.group > p.row_limit) n = 0;
-      unsigned c = 0;
-      if (n > 0) c = unsigned(Span(p, len - n, len - 1).chunks) * ((n * p.group + ROWS - 1) / ROWS) * s.kv_heads;
-      line[b] = c;
-      sum += c;
+  Segment g;
+  if (!locate(p, g, blockIdx.x, lane, warp)) return;
+  if (tid == 0) {
+    for (int i = 0; i < L::STAGES; ++i) {
+      bar_init(&full[i], 1);
+      bar_init(&empty[i], WARPS);
     }
-    unsigned at = sum;
-    for (int d = 1; d < 32; d <<= 1) {
-      const unsigned u = __shfl_up_sync(0xffffffffu, at, d);
-      if (lane >= d) at += u;
-    }
-    if (lane == 31) scan[warp] = at;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) at += scan[w];
-    at -= sum;
-    for (int b = b0; b < b1; ++b) {
-      const unsigned c = line[b];
-      line[b] = at;
-      at += c;
-    }
-    if (tid == THREADS - 1) line[s.seqs] = at;
-    __syncthreads();
+    stop_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const uint64_t total = line[s.seqs];
-  const uint64_t N = gridDim.x < total ? gridDim.x : total;  // every part has a chunk
-  if (blockIdx.x >= N) return;
-  const unsigned from = unsigned(blockIdx.x * total / N), to = unsigned((blockIdx.x + 1) * total / N);
+  lengths(s, g.b, g.start, g.n, g.len);
+  g.span = Span(p, g.len - g.n, g.len - 1);
+  g.rows = g.n * p.group;
+  const int chunks = g.span.chunks;
+  if (tid < ROWS) row_pos[tid] = tid < g.rows ? g.len - g.n + tid / p.group : -1;
+  const int c0 = int(int64_t(chunks) * g.part / g.parts), c1 = int(int64_t(chunks) * (g.part + 1) / g.parts);
+  __syncthreads();
 
-  for (unsigned pos = from; pos < to;) {
-    // ---- the segment at `pos` ----
-    Segment g;
-    {
-      int lo = 0, hi = s.seqs - 1;  // last b with line[b] <= pos (empty ones come before it)
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (line[mid] <= pos) lo = mid; else hi = mid - 1;
-      }
-      g.b = lo;
+  State<D, NT> st;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      st.m[i][c] = NONE;
+      st.l[i][c] = 0.0f;
     }
-    lengths(s, g.b, g.start, g.n, g.len);
-    g.span = Span(p, g.len - g.n, g.len - 1);
-    g.rows = g.n * p.group;
-    const int chunks = g.span.chunks;
-    const unsigned rel = pos - line[g.b], hr = rel / chunks;
-    const int c0 = rel - hr * chunks, c1 = int(min(unsigned(chunks), c0 + (to - pos)));
-    g.head = hr % s.kv_heads;
-    g.row0 = hr / s.kv_heads * ROWS;
-    const unsigned seg0 = pos - c0;
-    pos += c1 - c0;
-    // rows of this block see only part of the sequence's keys
-    const int t0 = g.row0 / p.group, t1 = min(g.row0 + ROWS, g.rows) - 1;
-    g.span.first = g.len - g.n + t0;
-    g.span.last = g.len - g.n + t1 / p.group;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) st.o[i][t][c] = 0.0f;
+  st.unit = 0;
+  const auto row_at = [&](int r, int64_t ts, int64_t hs) {
+    const int i = r / p.group, h = g.head * p.group + r - i * p.group;
+    return (g.start + i) * ts + h * hs;
+  };
 
+  if (warp == WARPS) {
+    // ---- chunks of codes, 32 chunks' pages and exponents at once ----
+    const uint32_t who = elected();
+    const int *table = s.table + int64_t(g.b) * s.width;
+    Ring ring;
+    bool ok = true;
+    for (int base = c0; ok && base < c1; base += 32) {
+      ChunkInfo mine = {0, 0, 0, 0};
+      int64_t unit = 0;
+      if (base + lane < c1) {
+        mine.key0 = g.span.key0(base + lane);
+        int page = table[mine.key0 >> s.page_shift];
+        mine.dead = page < 0 || page >= s.pages;
+        if (mine.dead) {
+          report(s.status, STATUS_PAGE);
+          page = 0;
+        }
+        unit = int64_t(page) * 2 * s.kv_heads + g.head;
+        mine.ek = p.exps[unit];
+        mine.ev = p.exps[unit + s.kv_heads];
+      }
+      const int k_row = int((unit << s.page_shift) + (mine.key0 & ((1 << s.page_shift) - 1)));
+      const auto copy = [&](int i, int slot) {
+        const int row = __shfl_sync(0xffffffffu, k_row, i);
+        if (who) {
+          const uint32_t dst = smem_addr(dyn + slot * L::CHUNK);
+          asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(&full[slot])),
+                       "r"(L::CHUNK)
+                       : "memory");
+          tma_rows(dst, &codes_map, row, &full[slot]);
+          tma_rows(dst + 64 * D, &codes_map, row + (s.kv_heads << s.page_shift), &full[slot]);
+        }
+      };
+      const int count = min(32, c1 - base);
+      // the first chunks' copies start before their exponents are here
+      const int early = base == c0 ? min(count, L::STAGES) : 0;
+      for (int i = 0; i < early; ++i) copy(i, i);
+      for (int i = 0; i < count; ++i, ring.next(L::STAGES)) {
+        if (i >= early) {
+          ok = warp_wait(&empty[ring.slot], ring.phase ^ 1, stop, s.status);
+          if (!ok) break;
+          copy(i, ring.slot);
+        }
+        ChunkInfo c;
+        c.key0 = __shfl_sync(0xffffffffu, mine.key0, i);
+        c.ek = __shfl_sync(0xffffffffu, mine.ek, i);
+        c.ev = __shfl_sync(0xffffffffu, mine.ev, i);
+        c.dead = __shfl_sync(0xffffffffu, mine.dead, i);
+        if (who) {
+          infos[ring.slot] = c;
+          bar_arrive(&full[ring.slot]);
+        }
+      }
+    }
+  } else {
     // ---- queries ----
-    State<D, NT> st;
     uint32_t own[NT == 1 ? D / 8 : 1];
-    uint32_t *const staged = reinterpret_cast<uint32_t *>(dyn);
-    const auto row_at = [&](int r, int64_t ts, int64_t hs) {
-      const int i = (g.row0 + r) / p.group, h = g.head * p.group + (g.row0 + r) - i * p.group;
-      return (g.start + i) * ts + h * hs;
-    };
+    float mult[2];
+    uint32_t *const staged = reinterpret_cast<uint32_t *>(dyn + L::QUERIES);
     if constexpr (NT == 1) {
-      const T *row = gr + g.row0 < g.rows ? static_cast<const T *>(p.q) + row_at(gr, p.q_ts, p.q_hs) : nullptr;
+      const T *row = gr < g.rows ? static_cast<const T *>(p.q) + row_at(gr, p.q_ts, p.q_hs) : nullptr;
       const int e = query_row<D>(own, row, q);
-      st.mult[0][0] = p.scale_log2 * pow2(__shfl_sync(0xffffffffu, e, 8 * q));
-      st.mult[0][1] = p.scale_log2 * pow2(__shfl_sync(0xffffffffu, e, 8 * q + 4));
+      mult[0] = p.scale_log2 * pow2(__shfl_sync(0xffffffffu, e, 8 * q));
+      mult[1] = p.scale_log2 * pow2(__shfl_sync(0xffffffffu, e, 8 * q + 4));
     } else {
-      __syncthreads();  // the last segment's join is read
-      for (int i = warp; i < NT; i += WARPS) {
-        const int r = 8 * i + gr;
+      if (warp < NT) {
+        const int r = 8 * warp + gr;
         uint32_t f[D / 8];
-        const T *row = r + g.row0 < g.rows ? static_cast<const T *>(p.q) + row_at(r, p.q_ts, p.q_hs) : nullptr;
+        const T *row = r < g.rows ? static_cast<const T *>(p.q) + row_at(r, p.q_ts, p.q_hs) : nullptr;
         const int e = query_row<D>(f, row, q);
-        if (q == 0) row_exp[r] = e;
+        if (q == 0) row_mult[r] = p.scale_log2 * pow2(e);
 #pragma unroll
         for (int w = 0; w < D / 16; ++w)
-          *reinterpret_cast<uint2 *>(&staged[((w * NT + i) * 32 + lane) * 2]) = make_uint2(f[2 * w], f[2 * w + 1]);
+          *reinterpret_cast<uint2 *>(&staged[((w * NT + warp) * 32 + lane) * 2]) = make_uint2(f[2 * w], f[2 * w + 1]);
       }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) st.mult[i][c] = p.scale_log2 * pow2(row_exp[8 * i + 2 * q + c]);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
     }
+    const auto mult_of = [&](int i, int c) {
+      if constexpr (NT == 1)
+        return mult[c];
+      else
+        return row_mult[8 * i + 2 * q + c];
+    };
     const auto query = [&](int w, int i) {
       if constexpr (NT == 1)
         return make_uint2(own[2 * w], own[2 * w + 1]);
       else
         return *reinterpret_cast<const uint2 *>(&staged[((w * NT + i) * 32 + lane) * 2]);
     };
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = g.row0 + 8 * i + 2 * q + c;
-        st.pos[i][c] = r < g.rows ? g.len - g.n + r / p.group : -1;
-        st.m[i][c] = NONE;
-        st.l[i][c] = 0.0f;
-      }
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) st.o[i][t][c] = 0.0f;
-    st.unit = 0;
+    // chunks whole_lo .. whole_hi - 1 every row sees whole
+    int whole_lo = 0;
+    const int whole_hi = g.span.sink_chunks + ((g.span.first + 1) >> 6) - g.span.window_chunk0;
+    if (p.window > 0)
+      whole_lo = g.span.sink_chunks + max(0, ((max(0, g.span.last - p.window + 1) + 63) >> 6) - g.span.window_chunk0);
 
-    // ---- this warp's quarter of the part, 16 keys a tile, one tile ahead ----
-    const int tiles = c1 - c0, first_tile = 4 * c0 + warp * tiles;
-    const int *row = s.table + int64_t(g.b) * s.width;
-    const auto key_of = [&](int i) { return g.span.key0((first_tile + i) >> 2) + 16 * ((first_tile + i) & 3); };
-    const auto page_of = [&](int i) { return i < tiles ? row[key_of(i) >> s.page_shift] : 0; };
-    Tile<D> a, b;
-    int page = page_of(1);
-    load_tile(a, p, g, key_of(0), page_of(0), lane);
-    st.unit = a.ev;
-    for (int i = 0; i < tiles; i += 2) {
-      if (i + 1 < tiles) load_tile(b, p, g, key_of(i + 1), page, lane);
-      page = page_of(i + 2);
-      if (g.span.wanted(a.key0, a.key0 + 15)) tile_step(st, a, p, g, query, lane);
-      if (i + 1 < tiles) {
-        if (i + 2 < tiles) load_tile(a, p, g, key_of(i + 2), page, lane);
-        page = page_of(i + 3);
-        if (g.span.wanted(b.key0, b.key0 + 15)) tile_step(st, b, p, g, query, lane);
+    // ---- 16 keys of each chunk a warp ----
+    Ring ring;
+    for (int chunk = c0; chunk < c1; ++chunk, ring.next(L::STAGES)) {
+      if (!warp_wait(&full[ring.slot], ring.phase, stop, s.status)) break;
+      const uint8_t *rows = dyn + ring.slot * L::CHUNK + 16 * warp * D;
+      const ChunkInfo info = infos[ring.slot];
+      // S^T = K Q^T: two chains of sums where there is one block of rows
+      constexpr int CHAINS = NT == 1 ? 2 : 1;
+      float sum[CHAINS][NT][4] = {};
+      {
+        uint32_t k[2][D / 16];
+        load_k<D>(k, rows, gr, q);
+#pragma unroll
+        for (int w = 0; w < D / 16; ++w) {
+          const uint32_t a[4] = {e4m3x2_f16x2(k[0][w]), e4m3x2_f16x2(k[1][w]), e4m3x2_f16x2(k[0][w] >> 16),
+                                 e4m3x2_f16x2(k[1][w] >> 16)};
+#pragma unroll
+          for (int r = 0; r < NT; ++r) {
+            const uint2 q2 = query(w, r);
+            mma(sum[w % CHAINS][r], a, q2.x, q2.y);
+          }
+        }
+      }
+      uint32_t v[4][D / 32];
+      load_v<D>(v, rows + 64 * D, gr, q);
+      warp_arrive(&empty[ring.slot]);
+      if (chunk == c0) st.unit = info.ev;
+      const float mk = pow2(info.ek);
+      float sc[NT][4];
+#pragma unroll
+      for (int r = 0; r < NT; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          sc[r][c] = (CHAINS == 2 ? sum[0][r][c] + sum[CHAINS - 1][r][c] : sum[0][r][c]) * (mult_of(r, c & 1) * mk);
+      uint32_t b[NT][2];
+      if (info.dead || chunk < whole_lo || chunk >= whole_hi) {
+        const int key0 = info.key0 + 16 * warp;
+        uint32_t nan_at[4];
+#pragma unroll
+        for (int r = 0; r < NT; ++r)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (info.dead || !g.span.sees(row_pos[8 * r + 2 * q + (c & 1)], key0 + gr + 8 * (c >> 1))) sc[r][c] = -INFINITY;
+        const bool any = take_nan<D>(v, nan_at, g, key0, info.dead, q);
+        softmax_step(st, sc, b, info.ev);
+        pv_step(st, v, b);
+        if (any) put_nan(st, nan_at, g, row_pos, key0, lane);
+      } else {
+        softmax_step(st, sc, b, info.ev);
+        pv_step(st, v, b);
       }
     }
+  }
 
-    // ---- join the warps ----
-    __syncthreads();  // staged queries and the last join are read
+  // ---- join the warps ----
+  __syncthreads();
+  if (*stop != 0) {
+    // given up: copies in flight land before the block may end (50 ms)
+    const unsigned long long t0 = now_ns();
+    while (now_ns() - t0 < 50000000ull) {
+    }
+    return;
+  }
+  if (warp < WARPS) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float l = st.l[i][c];
-        l += __shfl_xor_sync(0xffffffffu, l, 4);
-        l += __shfl_xor_sync(0xffffffffu, l, 8);
-        l += __shfl_xor_sync(0xffffffffu, l, 16);
-        const int r = 8 * i + 2 * q + c;
-        if (gr == 0) sm_m[warp][r] = st.m[i][c], sm_l[warp][r] = l;
+    for (int c = 0; c < 2; ++c) {
+      float l = st.l[i][c];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      const int r = 8 * i + 2 * q + c;
+      if (gr == 0) sm_m[warp][r] = st.m[i][c], sm_l[warp][r] = l;
 #pragma unroll
-        for (int j = 0; j < D / 16; ++j)
-          *reinterpret_cast<float2 *>(&join[(warp * ROWS + r) * LD + gr * (D / 8) + 2 * j]) =
-              make_float2(st.o[j][i][c], st.o[j][i][c + 2]);
-      }
+      for (int j = 0; j < D / 16; ++j)
+        *reinterpret_cast<float2 *>(&join[(warp * ROWS + r) * LD + gr * (D / 8) + 2 * j]) =
+            make_float2(st.o[j][i][c], st.o[j][i][c + 2]);
+    }
     if (lane == 0) sm_unit[warp] = st.unit;
+  }
+  __syncthreads();
+  if (tid < ROWS) {
+    float m = NONE, l = 0.0f;
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, sm_m[w][tid]);
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = exp2_fast(sm_m[w][tid] - m);
+      l += f * sm_l[w][tid];
+      weight[w][tid] = f * pow2(sm_unit[w]);
+    }
+    row_m[tid] = m;
+    row_l[tid] = l;
+  }
+  __syncthreads();
+  const bool whole = g.parts == 1;
+  const int rows = g.rows;
+  const auto store = [&](int r, int d, const float (&x)[8], float l) {
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    uint4 w;
+    w.x = pack2<T>(x[0] * by, x[1] * by);
+    w.y = pack2<T>(x[2] * by, x[3] * by);
+    w.z = pack2<T>(x[4] * by, x[5] * by);
+    w.w = pack2<T>(x[6] * by, x[7] * by);
+    *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) = w;
+  };
+  const auto part_slot = [&](int c) { return p.partial + int64_t(g.slot0 + c) * ROWS * (D + 2); };
+  float *const slot = part_slot(g.part);
+  for (int i = tid; i < rows * (D / 8); i += THREADS) {
+    const int r = i / (D / 8), d = i % (D / 8) * 8;
+    float x[8] = {};
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = weight[w][r];
+      const float4 u = *reinterpret_cast<const float4 *>(&join[(w * ROWS + r) * LD + d]);
+      const float4 v = *reinterpret_cast<const float4 *>(&join[(w * ROWS + r) * LD + d + 4]);
+      x[0] += f * u.x, x[1] += f * u.y, x[2] += f * u.z, x[3] += f * u.w;
+      x[4] += f * v.x, x[5] += f * v.y, x[6] += f * v.z, x[7] += f * v.w;
+    }
+    if (whole) {
+      store(r, d, x, row_l[r]);
+    } else {
+      __stcg(reinterpret_cast<float4 *>(slot + r * D + d), make_float4(x[0], x[1], x[2], x[3]));
+      __stcg(reinterpret_cast<float4 *>(slot + r * D + d + 4), make_float4(x[4], x[5], x[6], x[7]));
+    }
+  }
+  if (whole) return;
+  if (tid < ROWS) {
+    __stcg(slot + ROWS * D + tid, row_m[tid]);
+    __stcg(slot + ROWS * D + ROWS + tid, row_l[tid]);
+  }
+  // ---- parts join in groups of GROUP, groups in the segment: the last of
+  // each to arrive does it, in the parts' order ----
+  const auto last_of = [&](int c, int level, int count) {
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      unsigned *at = p.counters + (g.slot0 + c) * 2 + level;
+      ticket = atomicAdd(at, 1u);
+      if (ticket == unsigned(count - 1)) *at = 0;
+      __threadfence();
+    }
+    __syncthreads();
+    return ticket == unsigned(count - 1);
+  };
+  // parts a, a + step, .. as one: into `out`, or over part a
+  float *const part_m = join, *const part_l = join + 64 * ROWS;  // at most 64 parts at once
+  const auto gather = [&](int a, int count, int step, bool last) {
+    for (int i = tid; i < count * ROWS; i += THREADS) {
+      const float *at = part_slot(a + i / ROWS * step) + ROWS * D + i % ROWS;
+      part_m[i] = __ldcg(at);
+      part_l[i] = __ldcg(at + ROWS);
+    }
     __syncthreads();
     if (tid < ROWS) {
       float m = NONE, l = 0.0f;
-      for (int w = 0; w < WARPS; ++w) m = fmaxf(m, sm_m[w][tid]);
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = exp2_fast(sm_m[w][tid] - m);
-        l += f * sm_l[w][tid];
-        weight[w][tid] = f * pow2(sm_unit[w]);
+      for (int c = 0; c < count; ++c) m = fmaxf(m, part_m[c * ROWS + tid]);
+      for (int c = 0; c < count; ++c) {
+        const float f = exp2_fast(part_m[c * ROWS + tid] - m);
+        part_m[c * ROWS + tid] = f;
+        l += f * part_l[c * ROWS + tid];
       }
       row_m[tid] = m;
       row_l[tid] = l;
     }
     __syncthreads();
-    const bool whole = c1 - c0 == chunks;
-    const int rows = min(ROWS, g.rows - g.row0);
-    const auto store = [&](int r, int d, const float (&x)[8], float l) {
-      const float by = l == 0.0f ? 0.0f : 1.0f / l;
-      uint4 w;
-      w.x = pack2<T>(x[0] * by, x[1] * by);
-      w.y = pack2<T>(x[2] * by, x[3] * by);
-      w.z = pack2<T>(x[4] * by, x[5] * by);
-      w.w = pack2<T>(x[6] * by, x[7] * by);
-      *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) = w;
-    };
-    // partial results: two slots a CTA (a segment it ends, one it begins)
-    float *const slot = p.partial + (int64_t(blockIdx.x) * 2 + (c0 == 0)) * ROWS * (D + 2);
     for (int i = tid; i < rows * (D / 8); i += THREADS) {
       const int r = i / (D / 8), d = i % (D / 8) * 8;
       float x[8] = {};
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = weight[w][r];
-        const float4 u = *reinterpret_cast<const float4 *>(&join[(w * ROWS + r) * LD + d]);
-        const float4 v = *reinterpret_cast<const float4 *>(&join[(w * ROWS + r) * LD + d + 4]);
+#pragma unroll 8
+      for (int c = 0; c < count; ++c) {
+        const float *at = part_slot(a + c * step) + r * D + d;
+        const float f = part_m[c * ROWS + r];
+        const float4 u = __ldcg(reinterpret_cast<const float4 *>(at));
+        const float4 v4 = __ldcg(reinterpret_cast<const float4 *>(at + 4));
         x[0] += f * u.x, x[1] += f * u.y, x[2] += f * u.z, x[3] += f * u.w;
-        x[4] += f * v.x, x[5] += f * v.y, x[6] += f * v.z, x[7] += f * v.w;
+        x[4] += f * v4.x, x[5] += f * v4.y, x[6] += f * v4.z, x[7] += f * v4.w;
       }
-      if (whole) {
+      if (last) {
         store(r, d, x, row_l[r]);
-      } else {
-        __stcg(reinterpret_cast<float4 *>(slot + r * D + d), make_float4(x[0], x[1], x[2], x[3]));
-        __stcg(reinterpret_cast<float4 *>(slot + r * D + d + 4), make_float4(x[4], x[5], x[6], x[7]));
+      } else {  // only this thread reads or writes these values of part a now
+        float *to = part_slot(a) + r * D + d;
+        __stcg(reinterpret_cast<float4 *>(to), make_float4(x[0], x[1], x[2], x[3]));
+        __stcg(reinterpret_cast<float4 *>(to + 4), make_float4(x[4], x[5], x[6], x[7]));
       }
     }
-    if (whole) continue;
-    if (tid < ROWS) {
-      __stcg(slot + ROWS * D + tid, row_m[tid]);
-      __stcg(slot + ROWS * D + ROWS + tid, row_l[tid]);
+    if (!last && tid < ROWS) {
+      __stcg(part_slot(a) + ROWS * D + tid, row_m[tid]);
+      __stcg(part_slot(a) + ROWS * D + ROWS + tid, row_l[tid]);
     }
-    // ---- the last part of the segment to arrive joins all of them ----
-    const unsigned part0 = unsigned(((uint64_t(seg0) + 1) * N - 1) / total);
-    const unsigned part1 = unsigned(((uint64_t(seg0) + chunks) * N - 1) / total);
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-      ticket = atomicAdd(p.counters + part0, 1u);
-      if (ticket == part1 - part0) p.counters[part0] = 0;
-      __threadfence();
-    }
-    __syncthreads();
-    if (ticket != part1 - part0) continue;
-    const auto part_slot = [&](unsigned c) {
-      return p.partial + (int64_t(c) * 2 + (c == part0)) * ROWS * (D + 2);
-    };
-    for (int i = tid; i < rows * (D / 8); i += THREADS) {
-      const int r = i / (D / 8), d = i % (D / 8) * 8;
-      float m = NONE, l = 0.0f, x[8] = {};
-      for (unsigned c = part0; c <= part1; ++c) m = fmaxf(m, __ldcg(part_slot(c) + ROWS * D + r));
-      for (unsigned c = part0; c <= part1; ++c) {
-        const float *at = part_slot(c);
-        const float f = exp2_fast(__ldcg(at + ROWS * D + r) - m);
-        l += f * __ldcg(at + ROWS * D + ROWS + r);
-        const float4 u = __ldcg(reinterpret_cast<const float4 *>(at + r * D + d));
-        const float4 v = __ldcg(reinterpret_cast<const float4 *>(at + r * D + d + 4));
-        x[0] += f * u.x, x[1] += f * u.y, x[2] += f * u.z, x[3] += f * u.w;
-        x[4] += f * v.x, x[5] += f * v.y, x[6] += f * v.z, x[7] += f * v.w;
-      }
-      store(r, d, x, l);
-    }
-  }
+  };
+  // up to 64 parts at once where one level does, else groups of GROUP
+  const int group = g.parts <= ONE_LEVEL ? g.parts : max(GROUP, (g.parts + 63) / 64);
+  const int lead = g.part / group * group, count = min(group, g.parts - lead);
+  const int groups = (g.parts + group - 1) / group;
+  if (!last_of(lead, 0, count)) return;
+  gather(lead, count, 1, groups == 1);
+  if (groups == 1 || !last_of(0, 1, groups)) return;
+  gather(0, groups, group, true);
 }
 
 template <int D, int NT, typename T>
-cudaError_t launch(const AttendParams &p, int grid, int device, cudaStream_t stream) {
-  const int smem = SMEM_JOIN<D, NT> + (p.s.seqs + 1) * 4;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(
-        rows_kernel<D, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-        SMEM_JOIN<D, NT> + (EMMY_KV8_MAX_SEQS + 1) * 4);
-    if (e != cudaSuccess) return e;
+int launch(const AttendParams &p, const CUtensorMap &map, int grid, cudaStream_t stream) {
+  constexpr int smem = Layout<D, NT>::DYN;
+  cudaError_t e = cudaFuncSetAttribute(rows_kernel<D, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) {
+    rows_kernel<D, NT, T><<<grid, THREADS, smem, stream>>>(p, map);
+    e = cudaGetLastError();
   }
-  rows_kernel<D, NT, T><<<grid, THREADS, smem, stream>>>(p);
-  return cudaGetLastError();
+  return e == cudaSuccess ? EMMY_OK : cuda_fail("emmy_kv8_attend", e);
 }
 
 template <int D, typename T>
-cudaError_t launch_nt(const AttendParams &p, int nt, int grid, int device, cudaStream_t stream) {
+int launch_nt(const AttendParams &p, const CUtensorMap &map, int nt, int grid, cudaStream_t stream) {
   switch (nt) {
-    case 1: return launch<D, 1, T>(p, grid, device, stream);
-    case 2: return launch<D, 2, T>(p, grid, device, stream);
-    default: return launch<D, 4, T>(p, grid, device, stream);
+    case 1: return launch<D, 1, T>(p, map, grid, stream);
+    case 2: return launch<D, 2, T>(p, map, grid, stream);
+    case 3: return launch<D, 3, T>(p, map, grid, stream);
+    default: return launch<D, 4, T>(p, map, grid, stream);
   }
 }
 
 }  // namespace
 
 // 8-row blocks a CTA takes together, for the rows of the largest sequence.
-int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4; }
 
-// CTAs that fill the GPU, as the launch bounds allow them.
-int rows_grid(int nt, int device) { return sm_count(device) * (nt == 1 ? 4 : nt == 2 ? 3 : 2); }
+// Two counters for each part of a cut segment; see rows_partial_bytes.
+constexpr int MOST_PARTS = EMMY_KV8_WORKSPACE_ZERO / 12;
 
-uint64_t rows_partial_bytes(int nt, int head_dim, int device) {
-  return uint64_t(rows_grid(nt, device)) * 2 * 8 * nt * (head_dim + 2) * 4;
+// Parts wanted: twice the CTAs that the launch bounds let reside.
+int rows_target(int nt, int device) {
+  const int parts = 2 * sm_count(device) * (nt <= 2 ? 3 : 2);
+  return parts < MOST_PARTS ? parts : MOST_PARTS;
 }
 
-cudaError_t rows_attend(const AttendParams &p, int nt, int head_dim, bool bf16, int device,
-                        cudaStream_t stream) {
-  // no more CTAs than chunks that the table could hold
-  const int64_t most = ((int64_t(p.s.width) << p.s.page_shift) >> 6) * p.s.seqs * p.s.kv_heads *
-                       ((int64_t(p.most_rows) + 8 * nt - 1) / (8 * nt));
-  int grid = rows_grid(nt, device);
-  if (most < grid) grid = int(most);
-  if (grid < 1) return cudaSuccess;
-  if (head_dim == 64)
-    return bf16 ? launch_nt<64, __nv_bfloat16>(p, nt, grid, device, stream)
-                : launch_nt<64, __half>(p, nt, grid, device, stream);
-  return bf16 ? launch_nt<128, __nv_bfloat16>(p, nt, grid, device, stream)
-              : launch_nt<128, __half>(p, nt, grid, device, stream);
+// Parts of cut segments: one of c >= 1.5 q chunks has at most c / q + 1/2.
+uint64_t rows_partial_bytes(int nt, int head_dim, int device) {
+  return uint64_t(rows_target(nt, device)) * 3 / 2 * 8 * nt * (head_dim + 2) * 4;
+}
+
+int rows_attend(AttendParams p, const emmy_kv8 &cache, int nt, bool bf16, cudaStream_t stream) {
+  p.target = rows_target(nt, cache.device);
+  // a part and a half of the target, and the segments that stay whole, but no
+  // more than chunks that the table could hold
+  const int64_t segments = int64_t(p.s.seqs) * p.s.kv_heads;
+  const int64_t chunks = ((int64_t(p.s.width) << p.s.page_shift) >> 6) * segments;
+  int64_t grid = int64_t(p.target) * 3 / 2 + segments;
+  if (chunks < grid) grid = chunks;
+  // the pool as rows of head_dim bytes, 64 of them a box
+  const int64_t rows = int64_t(cache.pages) * 2 * cache.kv_heads * cache.page_size;
+  emmy_tmap_desc d = {};
+  d.base = cache.codes;
+  d.rank = 2;
+  d.dtype = EMMY_TMAP_U8;
+  d.dims[0] = d.strides[0] = cache.head_dim;
+  d.dims[1] = rows;
+  d.box[0] = cache.head_dim;
+  d.box[1] = 64;
+  d.swizzle = cache.head_dim;
+  d.l2_promote = 256;
+  alignas(64) CUtensorMap map;
+  const int rc = emmy_tmap_encode(&d, &map);
+  if (rc != EMMY_OK) return rc;
+  if (cache.head_dim == 64)
+    return bf16 ? launch_nt<64, __nv_bfloat16>(p, map, nt, int(grid), stream)
+                : launch_nt<64, __half>(p, map, nt, int(grid), stream);
+  return bf16 ? launch_nt<128, __nv_bfloat16>(p, map, nt, int(grid), stream)
+              : launch_nt<128, __half>(p, map, nt, int(grid), stream);
 }
 
 }  // namespace kv8

@@ -23,6 +23,7 @@
 // exponent of p; O moves (a pass over its columns) only when a row's maximum
 // grew by more than 2^8 or V's exponent strayed by more than 2^6.
 #include "kv8_attend.cuh"
+#include "kv8_async.cuh"
 
 namespace kv8 {
 namespace {
@@ -36,7 +37,6 @@ constexpr int REGS_LAUNCH = 128, REGS_ISSUE = 64, REGS_SOFTMAX = 176, REGS_LOAD 
 static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX + REGS_LOAD == 4 * REGS_LAUNCH, "register split");
 constexpr float LAZY = 8.0f, NONE = -1e30f, LEAST = 1e-37f;
 constexpr int UNIT_LAZY = 6;
-constexpr unsigned long long WAIT_NS = 2000000000ull;
 
 template <int D>
 struct Layout {
@@ -55,59 +55,6 @@ struct Bars {
   uint64_t q_full, kv_full[STAGES], kv_empty[STAGES], raw_full[RAW], raw_empty[RAW];
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], drain;
 };
-
-__device__ __forceinline__ uint32_t smem_addr(const void *p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void bar_init(uint64_t *b, int count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t *b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(b), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-// Waits with a whole warp, which stays converged, for the phase of parity
-// `parity`; false when the kernel gives up.
-__device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, volatile unsigned *stop,
-                                          unsigned *status) {
-  const uint32_t at = smem_addr(b);
-  if (__all_sync(0xffffffffu, bar_try(at, parity))) return true;
-  const unsigned long long t0 = now_ns();
-  for (;;) {
-    if (__all_sync(0xffffffffu, bar_try(at, parity))) return true;
-    bool over = *stop != 0;
-    if (now_ns() - t0 > WAIT_NS) {
-      *stop = 1;
-      report(status, STATUS_WAIT);
-      over = true;
-    }
-    if (__any_sync(0xffffffffu, over)) return false;
-  }
-}
-// Every lane's earlier work is done: one arrival for the warp.
-__device__ __forceinline__ void warp_arrive(uint64_t *b) {
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) bar_arrive(b);
-}
-__device__ __forceinline__ uint32_t elected() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r;
-}
 
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -205,15 +152,6 @@ __device__ __forceinline__ uint32_t swizzled(int r, int j) { return r * 128 + ((
 struct Unit {
   int b, head, start, n, len, rows, row0;
   Span span;
-};
-
-// A ring of n slots: slot and phase of step after step.
-struct Ring {
-  int slot = 0;
-  uint32_t phase = 0;
-  __device__ __forceinline__ void next(int n) {
-    if (++slot == n) slot = 0, phase ^= 1;
-  }
 };
 
 // What goes with a chunk of codes.
