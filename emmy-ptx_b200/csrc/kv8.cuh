@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "emmyrt.h"
@@ -76,6 +77,12 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
+// The kernels start with the end of the one before them in the stream
+// (programmatic dependent launch): they wait for it, and for all it wrote,
+// before they read anything, and let the next one be set up meanwhile.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependency_done() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Status of a call, with its message for emmy_last_error().
 int fail(int code, const char *what, const char *msg);
 int cuda_fail(const char *what, cudaError_t e);
@@ -99,6 +106,48 @@ class OnDevice {
   int prev_ = 0;
   bool moved_ = false;
 };
+
+// What a kernel needs once on each device: its dynamic shared memory allowed,
+// and (regs > 0) the register count that its register split counts on.
+class KernelSetup {
+ public:
+  template <typename K>
+  int ready(const char *what, K *kernel, int device, int smem, int regs = 0) {
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if (done_.load(std::memory_order_acquire) & bit) return EMMY_OK;
+    cudaError_t e = cudaSuccess;
+    if (regs > 0) {
+      cudaFuncAttributes at;
+      e = cudaFuncGetAttributes(&at, kernel);
+      if (e == cudaSuccess && at.numRegs != regs)
+        return fail(EMMY_ECUDART, what, "the kernel was built with another register count than its split needs");
+    }
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(what, e);
+    done_.fetch_or(bit, std::memory_order_release);
+    return EMMY_OK;
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
+
+template <typename... A>
+int launch_kernel(const char *what, void (*kernel)(A...), dim3 grid, int threads, int smem, cudaStream_t stream,
+                  const A &...args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &attr;
+  c.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
+  return e == cudaSuccess ? EMMY_OK : cuda_fail(what, e);
+}
 
 // Checks what every call shares and fills the kernels' view of the sequences.
 int check_cache(const char *what, const emmy_kv8 *c);

@@ -86,6 +86,8 @@ __global__ void append_kernel(const AppendParams p) {
   constexpr int LPR = D / 8;     // lanes per row, eight values each
   constexpr int RPW = 32 / LPR;  // rows per warp and pass
   const Seqs &s = p.s;
+  grid_dependency_wait();
+  grid_dependency_done();
   const int b = owner(s, blockIdx.x);
   if (b < 0) return;
   int start, n, len;
@@ -163,11 +165,10 @@ __global__ void append_kernel(const AppendParams p) {
 }
 
 template <int D, typename T>
-cudaError_t launch(const AppendParams &p, int slots, cudaStream_t stream) {
-  const dim3 grid(slots, p.s.kv_heads, 2);
+int launch(const AppendParams &p, int slots, cudaStream_t stream) {
   // 64 rows to 128 threads: D / 16 passes over the page
-  append_kernel<D, D / 16, T><<<grid, 2 << p.s.page_shift, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_kernel("emmy_kv8_append", append_kernel<D, D / 16, T>, dim3(slots, p.s.kv_heads, 2),
+                       2 << p.s.page_shift, 0, stream, p);
 }
 
 }  // namespace
@@ -204,13 +205,10 @@ extern "C" int emmy_kv8_append(const emmy_kv8 *cache, emmy_dptr k, emmy_dptr v, 
   const int64_t slots = (int64_t(cache->tokens) >> p.s.page_shift) + 2 * int64_t(cache->seqs);
   if (slots > 0x7fffffff) return fail(EMMY_EINVAL, what, "too many tokens");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e;
   const bool d64 = cache->head_dim == 64;
   if (dtype == EMMY_KV8_F32)
-    e = d64 ? launch<64, float>(p, int(slots), st) : launch<128, float>(p, int(slots), st);
-  else if (dtype == EMMY_KV8_BF16)
-    e = d64 ? launch<64, __nv_bfloat16>(p, int(slots), st) : launch<128, __nv_bfloat16>(p, int(slots), st);
-  else
-    e = d64 ? launch<64, __half>(p, int(slots), st) : launch<128, __half>(p, int(slots), st);
-  return e == cudaSuccess ? EMMY_OK : cuda_fail(what, e);
+    return d64 ? launch<64, float>(p, int(slots), st) : launch<128, float>(p, int(slots), st);
+  if (dtype == EMMY_KV8_BF16)
+    return d64 ? launch<64, __nv_bfloat16>(p, int(slots), st) : launch<128, __nv_bfloat16>(p, int(slots), st);
+  return d64 ? launch<64, __half>(p, int(slots), st) : launch<128, __half>(p, int(slots), st);
 }

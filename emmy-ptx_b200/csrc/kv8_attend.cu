@@ -79,6 +79,7 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   p.window = a->window;
   p.sinks = a->sinks;
   p.target = 0;
+  p.spread = false;
   // A sequence with up to ROWS_MOST rows of a kv head is the row kernel's,
   // others the tile kernel's, which takes the one sequence of a call that may
   // be either.
@@ -95,8 +96,8 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   const bool bf16 = a->dtype == EMMY_KV8_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (tiles) {
-    const cudaError_t e = tiles_attend(p, cache->head_dim, bf16, st);
-    if (e != cudaSuccess) return cuda_fail(WHAT, e);
+    rc = tiles_attend(p, *cache, bf16, st);
+    if (rc != EMMY_OK) return rc;
   }
   return rows ? rows_attend(p, *cache, nt, bf16, st) : EMMY_OK;
 }

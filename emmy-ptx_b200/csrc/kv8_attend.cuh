@@ -21,6 +21,7 @@ struct AttendParams {
   int window, sinks;
   int row_limit;     // sequences with more rows of a kv head than this are the tile kernel's
   int target;        // parts that the row kernel is to cut its segments into
+  bool spread;       // in two waves rather than one
 };
 
 // Which keys a block of query rows sees, and the 64-key chunks that hold
@@ -104,7 +105,7 @@ __device__ __forceinline__ int row_exponent(float amax) {
 // Rows of a kv head up to which a sequence is the row kernel's.
 constexpr int ROWS_MOST = 32;
 
-cudaError_t tiles_attend(const AttendParams &p, int head_dim, bool bf16, cudaStream_t stream);
+int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, bool bf16, cudaStream_t stream);
 int rows_blocks(int64_t rows);
 uint64_t rows_partial_bytes(int nt, int head_dim, int device);
 int rows_attend(AttendParams p, const emmy_kv8 &cache, int nt, bool bf16, cudaStream_t stream);

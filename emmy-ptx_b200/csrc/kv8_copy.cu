@@ -21,6 +21,8 @@ template <int N>
 __global__ void __launch_bounds__(COPY_THREADS)
 copy_kernel(uint4 *codes, int8_t *exps, int pages, int page_vecs, int page_exps, int chunks,
             const __grid_constant__ Pairs<N> pairs) {
+  grid_dependency_wait();
+  grid_dependency_done();
   const int pair = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const int64_t layer = int64_t(blockIdx.y) * pages;
   const int64_t src = layer + pairs.src[pair], dst = layer + pairs.dst[pair];
@@ -40,17 +42,16 @@ copy_kernel(uint4 *codes, int8_t *exps, int pages, int page_vecs, int page_exps,
 }
 
 template <int N>
-cudaError_t launch(const emmy_kv8 &c, int layers, const int32_t *src, const int32_t *dst, int n,
+int launch(const emmy_kv8 &c, int layers, const int32_t *src, const int32_t *dst, int n,
                    cudaStream_t stream) {
   Pairs<N> pairs = {};
   for (int i = 0; i < n; ++i) pairs.src[i] = src[i], pairs.dst[i] = dst[i];
   const int page_exps = 2 * c.kv_heads;
   const int page_vecs = page_exps * c.page_size * (c.head_dim / 16);
   const int per = COPY_THREADS * COPY_VEC, chunks = (page_vecs + per - 1) / per;
-  copy_kernel<N><<<dim3(n * chunks, layers), COPY_THREADS, 0, stream>>>(
-      reinterpret_cast<uint4 *>(c.codes), reinterpret_cast<int8_t *>(c.exps), c.pages, page_vecs,
-      page_exps, chunks, pairs);
-  return cudaGetLastError();
+  return launch_kernel("emmy_kv8_copy_pages", copy_kernel<N>, dim3(n * chunks, layers), COPY_THREADS, 0, stream,
+                       reinterpret_cast<uint4 *>(c.codes), reinterpret_cast<int8_t *>(c.exps), int(c.pages), page_vecs,
+                       page_exps, chunks, pairs);
 }
 
 }  // namespace
@@ -73,7 +74,6 @@ extern "C" int emmy_kv8_copy_pages(const emmy_kv8 *cache, int32_t layers, const 
   if (on.err != cudaSuccess) return cuda_fail(what, on.err);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // short lists travel in 512 bytes of parameters, long ones in 3840
-  const cudaError_t e = n <= 64 ? launch<64>(*cache, layers, src, dst, n, st)
-                                : launch<EMMY_KV8_MAX_PAIRS>(*cache, layers, src, dst, n, st);
-  return e == cudaSuccess ? EMMY_OK : cuda_fail(what, e);
+  return n <= 64 ? launch<64>(*cache, layers, src, dst, n, st)
+                 : launch<EMMY_KV8_MAX_PAIRS>(*cache, layers, src, dst, n, st);
 }

@@ -75,19 +75,12 @@ __device__ __forceinline__ int seq_chunks(const AttendParams &p, int b) {
   lengths(p.s, b, start, n, len);
   return n == 0 || n * p.group > p.row_limit ? 0 : Span(p, len - n, len - 1).chunks;
 }
-// Parts of a segment of c chunks, at q chunks a part.
-__device__ __forceinline__ int parts_of(int c, int q) {
-  return c == 0 ? 0 : max(1, min((2 * c + q) / (2 * q), c));
-}
-// Chunks a part so that there are about p.target parts.
-__device__ __forceinline__ int part_chunks(const AttendParams &p, int64_t total) {
-  return int((total * p.s.kv_heads + p.target - 1) / p.target);
+// Parts of a segment of c chunks, at no more than q chunks a part, or (spread)
+// as near to q as may be.
+__device__ __forceinline__ int parts_of(int c, int q, bool spread) {
+  return c == 0 ? 0 : spread ? max(1, min((2 * c + q) / (2 * q), c)) : (c + q - 1) / q;
 }
 
-__device__ __forceinline__ int warp_sum(int x) {
-  for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-  return x;
-}
 __device__ __forceinline__ int warp_scan(int x, int lane) {  // inclusive
   for (int d = 1; d < 32; d <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, x, d);
@@ -97,68 +90,110 @@ __device__ __forceinline__ int warp_scan(int x, int lane) {  // inclusive
 }
 
 // Which segment and part is CTA `want`'s: g.b, g.head, g.part, g.parts, g.slot0.
-// Up to 32 sequences every warp finds it for itself, a lane a sequence.
-__device__ __forceinline__ bool locate(const AttendParams &p, Segment &g, int want, int lane, int warp) {
-  const int H = p.s.kv_heads;
-  if (p.s.seqs <= 32) {
-    const int c = seq_chunks(p, lane);
-    const int q = part_chunks(p, warp_sum(c));
-    const int k = q == 0 ? 0 : parts_of(c, q);
-    const int at = warp_scan(k * H, lane), slot = warp_scan(k > 1 ? k * H : 0, lane);
-    const int b = __popc(__ballot_sync(0xffffffffu, at <= want));
-    if (b >= p.s.seqs) return false;
-    g.b = b;
-    g.parts = __shfl_sync(0xffffffffu, k, b);
-    const int rel = want - (__shfl_sync(0xffffffffu, at, b) - g.parts * H);
-    g.head = rel / g.parts;
-    g.part = rel - g.head * g.parts;
-    g.slot0 = __shfl_sync(0xffffffffu, slot, b) - g.parts * H + g.head * g.parts;
-    return true;
-  }
-  __shared__ long long sums[ALL_WARPS];
+//
+// Where all segments fit on the GPU at once (p.spread false), parts of at most
+// q chunks, q the least of a few tries that leaves them one wave: equal parts
+// that start together.  Otherwise two waves of parts of about equal length,
+// which the order of arrival evens out.  Measured (us, one wave | two): 2
+// sequences of 131071 keys 37 | 43, 48 with a window of 1024 19 | 28, 16 with
+// five drafts 33 | 41; but 64 of 700-8191 keys, 512 segments on 444 CTAs,
+// 111 | 97.
+//
+// Up to 128 sequences every warp finds it for itself, four sequences a lane;
+// more of them, the block together.
+template <int SEQS>
+__device__ __forceinline__ bool locate_in(const AttendParams &p, Segment &g, int want, int lane, int warp) {
+  constexpr bool BLOCK = SEQS == 0;
+  const int H = p.s.kv_heads, tid = threadIdx.x;
+  __shared__ long long sums[ALL_WARPS][5];
   __shared__ int scans[2][ALL_WARPS], found[5];
-  const int tid = threadIdx.x, per = (p.s.seqs + THREADS - 1) / THREADS;
-  const int b0 = min(tid * per, p.s.seqs), b1 = min(b0 + per, p.s.seqs);
+  const int per = BLOCK ? (p.s.seqs + THREADS - 1) / THREADS : SEQS;
+  const int b0 = (BLOCK ? tid : lane) * per;
+  int own[BLOCK ? 1 : SEQS];
+  if constexpr (!BLOCK) {
+#pragma unroll
+    for (int i = 0; i < SEQS; ++i) own[i] = seq_chunks(p, b0 + i);
+  }
+  const auto chunks_of = [&](int i) {
+    if constexpr (BLOCK)
+      return seq_chunks(p, b0 + i);
+    else
+      return own[i];
+  };
+  const auto total_of = [&](long long x, int slot) {
+    for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    if constexpr (BLOCK) {
+      if (lane == 0) sums[warp][slot] = x;
+      __syncthreads();
+      x = 0;
+      for (int w = 0; w < ALL_WARPS; ++w) x += sums[w][slot];
+    }
+    return x;
+  };
   long long chunks = 0;
-  for (int b = b0; b < b1; ++b) chunks += seq_chunks(p, b);
-  for (int d = 16; d > 0; d >>= 1) chunks += __shfl_xor_sync(0xffffffffu, chunks, d);
-  if (lane == 0) sums[warp] = chunks;
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  chunks = 0;
-  for (int w = 0; w < ALL_WARPS; ++w) chunks += sums[w];
-  const int q = part_chunks(p, chunks);
-  if (q == 0) return false;
+  if (BLOCK && tid == 0) found[0] = -1;
+  for (int i = 0; i < per; ++i) chunks += chunks_of(i);
+  chunks = total_of(chunks, 0);
+  const int q0 = int((chunks * H + p.target - 1) / p.target);
+  if (q0 == 0) return false;
+  int q = q0;
+  if (!p.spread) {
+    for (int t = 1; t < 5; ++t) {
+      long long parts = 0;
+      for (int i = 0; i < per; ++i) parts += parts_of(chunks_of(i), q, false);
+      if (total_of(parts, t) * H <= p.target) break;
+      q = q0 + (q0 * (1 << t) + 15) / 16;  // 1/8, 1/4, 1/2, 1 above q0
+    }
+  }
   int parts = 0, slots = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int k = parts_of(seq_chunks(p, b), q);
+  for (int i = 0; i < per; ++i) {
+    const int k = parts_of(chunks_of(i), q, p.spread);
     parts += k * H;
     slots += k > 1 ? k * H : 0;
   }
   int at = warp_scan(parts, lane), slot = warp_scan(slots, lane);
-  if (lane == 31) scans[0][warp] = at, scans[1][warp] = slot;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) at += scans[0][w], slot += scans[1][w];
+  if constexpr (BLOCK) {
+    if (lane == 31) scans[0][warp] = at, scans[1][warp] = slot;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) at += scans[0][w], slot += scans[1][w];
+  }
   at -= parts;
   slot -= slots;
-  if (want >= at && want < at + parts) {  // one thread's share holds it
-    for (int b = b0; b < b1; ++b) {
-      const int k = parts_of(seq_chunks(p, b), q);
-      if (want < at + k * H) {
-        found[0] = b;
-        found[1] = (want - at) / k;
-        found[2] = (want - at) % k;
-        found[3] = k;
-        found[4] = slot + found[1] * k;
-        break;
+  int f[5] = {-1, 0, 0, 0, 0};
+  const bool mine = want >= at && want < at + parts;  // one thread's share holds it
+  if (mine) {
+#pragma unroll 4
+    for (int i = 0; i < per; ++i) {
+      const int k = parts_of(chunks_of(i), q, p.spread);
+      if (f[0] < 0 && want < at + k * H) {
+        f[0] = b0 + i;
+        f[1] = (want - at) / k;
+        f[2] = (want - at) % k;
+        f[3] = k;
+        f[4] = slot + f[1] * k;
       }
       at += k * H;
       slot += k > 1 ? k * H : 0;
     }
   }
-  __syncthreads();
-  g.b = found[0], g.head = found[1], g.part = found[2], g.parts = found[3], g.slot0 = found[4];
+  if constexpr (BLOCK) {
+    if (mine)
+      for (int i = 0; i < 5; ++i) found[i] = f[i];
+    __syncthreads();
+    for (int i = 0; i < 5; ++i) f[i] = found[i];
+  } else {
+    const unsigned who = __ballot_sync(0xffffffffu, mine);
+    if (who == 0) return false;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) f[i] = __shfl_sync(0xffffffffu, f[i], __ffs(who) - 1);
+  }
+  g.b = f[0], g.head = f[1], g.part = f[2], g.parts = f[3], g.slot0 = f[4];
   return g.b >= 0;
+}
+__device__ __forceinline__ bool locate(const AttendParams &p, Segment &g, int want, int lane, int warp) {
+  if (p.s.seqs <= 32) return locate_in<1>(p, g, want, lane, warp);
+  if (p.s.seqs <= 128) return locate_in<4>(p, g, want, lane, warp);
+  return locate_in<0>(p, g, want, lane, warp);
 }
 
 // What goes with a chunk of codes.
@@ -291,29 +326,35 @@ __device__ __forceinline__ void pv_step(State<D, NT> &st, const uint32_t (&v)[4]
 }
 
 // A hidden key has p = 0, but 0 * NaN is NaN: values of a tile that no row sees
-// become zero, and a NaN that only some rows see is taken out and put into
-// those rows' sums (after their P V) by put_nan.
+// become zero, and a NaN that only some rows see is taken out (take_nan) and
+// put into those rows' sums after their P V (put_nan).
 template <int D>
-__device__ __forceinline__ bool take_nan(uint32_t (&v)[4][D / 32], uint32_t (&nan_at)[4], const Segment &g,
-                                         int key0, bool dead, int q) {
+__device__ __forceinline__ bool hide_values(uint32_t (&v)[4][D / 32], const Segment &g, int key0, bool dead, int q) {
   uint32_t any = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    nan_at[i] = 0;  // bit d: value d of the lane's V row i is NaN
-    const bool seen = !dead && g.span.any_sees(key0 + 2 * q + (i & 1) + 8 * (i >> 1));
+    const uint32_t keep = !dead && g.span.any_sees(key0 + 2 * q + (i & 1) + 8 * (i >> 1)) ? 0xffffffffu : 0u;
 #pragma unroll
     for (int w = 0; w < D / 32; ++w) {
-      if (!seen) v[i][w] = 0;
-      const uint32_t bad = nan_bytes(v[i][w]);
-      if (bad != 0) {
-        v[i][w] &= ~((bad >> 7) * 0xffu);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) nan_at[i] |= ((bad >> (8 * j + 7)) & 1u) << (4 * w + j);
-      }
+      v[i][w] &= keep;
+      any |= nan_bytes(v[i][w]);
     }
-    any |= nan_at[i];
   }
   return __any_sync(0xffffffffu, any != 0);
+}
+template <int D>
+__device__ __forceinline__ void take_nan(uint32_t (&v)[4][D / 32], uint32_t (&nan_at)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    nan_at[i] = 0;  // bit d: value d of the lane's V row i is NaN
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) {
+      const uint32_t bad = nan_bytes(v[i][w]);
+      v[i][w] &= ~((bad >> 7) * 0xffu);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) nan_at[i] |= ((bad >> (8 * j + 7)) & 1u) << (4 * w + j);
+    }
+  }
 }
 template <int D, int NT>
 __device__ __forceinline__ void put_nan(State<D, NT> &st, const uint32_t (&nan_at)[4], const Segment &g,
@@ -387,7 +428,9 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gr = lane >> 2, q = lane & 3;
   const Seqs &s = p.s;
   Segment g;
+  grid_dependency_wait();
   if (!locate(p, g, blockIdx.x, lane, warp)) return;
+  grid_dependency_done();
   if (tid == 0) {
     for (int i = 0; i < L::STAGES; ++i) {
       bar_init(&full[i], 1);
@@ -554,22 +597,22 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
         for (int c = 0; c < 4; ++c)
           sc[r][c] = (CHAINS == 2 ? sum[0][r][c] + sum[CHAINS - 1][r][c] : sum[0][r][c]) * (mult_of(r, c & 1) * mk);
       uint32_t b[NT][2];
+      bool nan = false;
+      const int key0 = info.key0 + 16 * warp;
       if (info.dead || chunk < whole_lo || chunk >= whole_hi) {
-        const int key0 = info.key0 + 16 * warp;
-        uint32_t nan_at[4];
 #pragma unroll
         for (int r = 0; r < NT; ++r)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            if (info.dead || !g.span.sees(row_pos[8 * r + 2 * q + (c & 1)], key0 + gr + 8 * (c >> 1))) sc[r][c] = -INFINITY;
-        const bool any = take_nan<D>(v, nan_at, g, key0, info.dead, q);
-        softmax_step(st, sc, b, info.ev);
-        pv_step(st, v, b);
-        if (any) put_nan(st, nan_at, g, row_pos, key0, lane);
-      } else {
-        softmax_step(st, sc, b, info.ev);
-        pv_step(st, v, b);
+            if (info.dead || !g.span.sees(row_pos[8 * r + 2 * q + (c & 1)], key0 + gr + 8 * (c >> 1)))
+              sc[r][c] = -INFINITY;
+        nan = hide_values<D>(v, g, key0, info.dead, q);
       }
+      softmax_step(st, sc, b, info.ev);
+      uint32_t nan_at[4];
+      if (nan) take_nan<D>(v, nan_at);
+      pv_step(st, v, b);
+      if (nan) put_nan(st, nan_at, g, row_pos, key0, lane);
     }
   }
 
@@ -652,10 +695,11 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
   // ---- parts join in groups of GROUP, groups in the segment: the last of
   // each to arrive does it, in the parts' order ----
   const auto last_of = [&](int c, int level, int count) {
-    __threadfence();
     __syncthreads();
     if (tid == 0) {
+      // the barrier orders the block's stores before this thread's fence
       unsigned *at = p.counters + (g.slot0 + c) * 2 + level;
+      __threadfence();
       ticket = atomicAdd(at, 1u);
       if (ticket == unsigned(count - 1)) *at = 0;
       __threadfence();
@@ -720,23 +764,20 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
 }
 
 template <int D, int NT, typename T>
-int launch(const AttendParams &p, const CUtensorMap &map, int grid, cudaStream_t stream) {
-  constexpr int smem = Layout<D, NT>::DYN;
-  cudaError_t e = cudaFuncSetAttribute(rows_kernel<D, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess) {
-    rows_kernel<D, NT, T><<<grid, THREADS, smem, stream>>>(p, map);
-    e = cudaGetLastError();
-  }
-  return e == cudaSuccess ? EMMY_OK : cuda_fail("emmy_kv8_attend", e);
+int launch(const AttendParams &p, const CUtensorMap &map, int device, int grid, cudaStream_t stream) {
+  static KernelSetup setup;
+  const int rc = setup.ready("emmy_kv8_attend", rows_kernel<D, NT, T>, device, Layout<D, NT>::DYN);
+  if (rc != EMMY_OK) return rc;
+  return launch_kernel("emmy_kv8_attend", rows_kernel<D, NT, T>, dim3(grid), THREADS, Layout<D, NT>::DYN, stream, p, map);
 }
 
 template <int D, typename T>
-int launch_nt(const AttendParams &p, const CUtensorMap &map, int nt, int grid, cudaStream_t stream) {
+int launch_nt(const AttendParams &p, const CUtensorMap &map, int nt, int device, int grid, cudaStream_t stream) {
   switch (nt) {
-    case 1: return launch<D, 1, T>(p, map, grid, stream);
-    case 2: return launch<D, 2, T>(p, map, grid, stream);
-    case 3: return launch<D, 3, T>(p, map, grid, stream);
-    default: return launch<D, 4, T>(p, map, grid, stream);
+    case 1: return launch<D, 1, T>(p, map, device, grid, stream);
+    case 2: return launch<D, 2, T>(p, map, device, grid, stream);
+    case 3: return launch<D, 3, T>(p, map, device, grid, stream);
+    default: return launch<D, 4, T>(p, map, device, grid, stream);
   }
 }
 
@@ -745,27 +786,29 @@ int launch_nt(const AttendParams &p, const CUtensorMap &map, int nt, int grid, c
 // 8-row blocks a CTA takes together, for the rows of the largest sequence.
 int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4; }
 
-// Two counters for each part of a cut segment; see rows_partial_bytes.
-constexpr int MOST_PARTS = EMMY_KV8_WORKSPACE_ZERO / 12;
+// CTAs that the launch bounds let reside.
+int rows_slots(int nt, int device) { return sm_count(device) * (nt <= 2 ? 3 : 2); }
 
-// Parts wanted: twice the CTAs that the launch bounds let reside.
-int rows_target(int nt, int device) {
-  const int parts = 2 * sm_count(device) * (nt <= 2 ? 3 : 2);
-  return parts < MOST_PARTS ? parts : MOST_PARTS;
+// Workspace slots, two counters each.  One wave: at most as many parts.  Two:
+// a cut segment has c >= 1.5 q chunks and at most c / q + 1/2 parts, a third
+// above its share.
+int rows_parts(int nt, int device) {
+  const int most = 3 * rows_slots(nt, device), fit = EMMY_KV8_WORKSPACE_ZERO / 8;
+  return most < fit ? most : fit;
 }
-
-// Parts of cut segments: one of c >= 1.5 q chunks has at most c / q + 1/2.
 uint64_t rows_partial_bytes(int nt, int head_dim, int device) {
-  return uint64_t(rows_target(nt, device)) * 3 / 2 * 8 * nt * (head_dim + 2) * 4;
+  return uint64_t(rows_parts(nt, device)) * 8 * nt * (head_dim + 2) * 4;
 }
 
 int rows_attend(AttendParams p, const emmy_kv8 &cache, int nt, bool bf16, cudaStream_t stream) {
-  p.target = rows_target(nt, cache.device);
-  // a part and a half of the target, and the segments that stay whole, but no
-  // more than chunks that the table could hold
   const int64_t segments = int64_t(p.s.seqs) * p.s.kv_heads;
   const int64_t chunks = ((int64_t(p.s.width) << p.s.page_shift) >> 6) * segments;
-  int64_t grid = int64_t(p.target) * 3 / 2 + segments;
+  const int slots = rows_slots(nt, cache.device), parts = rows_parts(nt, cache.device);
+  p.spread = segments > slots;
+  p.target = p.spread ? parts * 2 / 3 : slots < parts ? slots : parts;
+  // the parts wanted, or, where no try fitted, one of each segment more; but
+  // no more than chunks that the table could hold
+  int64_t grid = (p.spread ? parts : p.target) + segments;
   if (chunks < grid) grid = chunks;
   // the pool as rows of head_dim bytes, 64 of them a box
   const int64_t rows = int64_t(cache.pages) * 2 * cache.kv_heads * cache.page_size;
@@ -783,10 +826,10 @@ int rows_attend(AttendParams p, const emmy_kv8 &cache, int nt, bool bf16, cudaSt
   const int rc = emmy_tmap_encode(&d, &map);
   if (rc != EMMY_OK) return rc;
   if (cache.head_dim == 64)
-    return bf16 ? launch_nt<64, __nv_bfloat16>(p, map, nt, int(grid), stream)
-                : launch_nt<64, __half>(p, map, nt, int(grid), stream);
-  return bf16 ? launch_nt<128, __nv_bfloat16>(p, map, nt, int(grid), stream)
-              : launch_nt<128, __half>(p, map, nt, int(grid), stream);
+    return bf16 ? launch_nt<64, __nv_bfloat16>(p, map, nt, cache.device, int(grid), stream)
+                : launch_nt<64, __half>(p, map, nt, cache.device, int(grid), stream);
+  return bf16 ? launch_nt<128, __nv_bfloat16>(p, map, nt, cache.device, int(grid), stream)
+              : launch_nt<128, __half>(p, map, nt, cache.device, int(grid), stream);
 }
 
 }  // namespace kv8

@@ -183,6 +183,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Seqs &s = p.s;
 
+  grid_dependency_wait();
+  grid_dependency_done();
   // ---- which unit: the grid counts row blocks of all sequences, each for
   // every kv head, the blocks with the most keys first ----
   Unit u;
@@ -652,27 +654,26 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 }
 
 template <int D, typename T>
-cudaError_t launch(const AttendParams &p, unsigned grid, cudaStream_t stream) {
-  cudaFuncAttributes at;
-  cudaError_t e = cudaFuncGetAttributes(&at, tiles_kernel<D, T>);
-  if (e != cudaSuccess) return e;
-  if (at.numRegs != REGS_LAUNCH) return cudaErrorInvalidKernelImage;  // the split would not add up
-  e = cudaFuncSetAttribute(tiles_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::DYN);
-  if (e != cudaSuccess) return e;
-  tiles_kernel<D, T><<<grid, THREADS, Layout<D>::DYN, stream>>>(p);
-  return cudaGetLastError();
+int launch(const AttendParams &p, int device, unsigned grid, cudaStream_t stream) {
+  static KernelSetup setup;
+  const int rc = setup.ready("emmy_kv8_attend", tiles_kernel<D, T>, device, Layout<D>::DYN, REGS_LAUNCH);
+  if (rc != EMMY_OK) return rc;
+  return launch_kernel("emmy_kv8_attend", tiles_kernel<D, T>, dim3(grid), THREADS, Layout<D>::DYN, stream, p);
 }
 
 }  // namespace
 
-cudaError_t tiles_attend(const AttendParams &p, int head_dim, bool bf16, cudaStream_t stream) {
+int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, bool bf16, cudaStream_t stream) {
   // row blocks of all sequences: at most one part-filled one each
   const int64_t blocks = (int64_t(p.s.tokens) * p.group) / (2 * TILE) + p.s.seqs;
   const int64_t grid = blocks * p.s.kv_heads;
-  if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  if (head_dim == 64)
-    return bf16 ? launch<64, __nv_bfloat16>(p, unsigned(grid), stream) : launch<64, __half>(p, unsigned(grid), stream);
-  return bf16 ? launch<128, __nv_bfloat16>(p, unsigned(grid), stream) : launch<128, __half>(p, unsigned(grid), stream);
+  if (grid > 0x7fffffff) return fail(EMMY_EINVAL, "emmy_kv8_attend", "too many query rows");
+  const int dev = cache.device;
+  if (cache.head_dim == 64)
+    return bf16 ? launch<64, __nv_bfloat16>(p, dev, unsigned(grid), stream)
+                : launch<64, __half>(p, dev, unsigned(grid), stream);
+  return bf16 ? launch<128, __nv_bfloat16>(p, dev, unsigned(grid), stream)
+              : launch<128, __half>(p, dev, unsigned(grid), stream);
 }
 
 }  // namespace kv8
