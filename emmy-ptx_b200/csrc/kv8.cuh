@@ -29,6 +29,7 @@ constexpr unsigned STATUS_PAGE = 0x401;    // a page number outside the pool
 constexpr unsigned STATUS_LENGTH = 0x402;  // a sequence longer than its row of the table, or
                                            // more new tokens than keys or than rows given
 constexpr unsigned STATUS_WAIT = 0x403;    // a bounded wait inside a kernel ran out
+constexpr unsigned STATUS_PLAN = 0x404;    // a plan that was made for another call
 
 struct Seqs {
   const int *table;     // [seqs][width] page numbers

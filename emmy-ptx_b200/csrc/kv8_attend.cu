@@ -1,5 +1,5 @@
 // emmy_kv8_attend -- attention of new queries over the paged 8-bit cache:
-// checks, workspace, and which kernel takes which sequences.
+// checks, workspace and plan, and which kernel takes which sequences.
 #include <cmath>
 
 #include "kv8_attend.cuh"
@@ -7,67 +7,128 @@
 namespace kv8 {
 namespace {
 
-const char *const WHAT = "emmy_kv8_attend";
-
-int check_heads(const char *what, const emmy_kv8 *c, int heads) {
+// A sequence with up to ROWS_MOST rows of a kv head is the row kernel's, others
+// the tile kernel's; a call's only sequence is whichever's its most rows ask
+// for.
+int shape_of(const char *what, const emmy_kv8 *c, int heads, PlanShape &p) {
   if (heads < 1 || heads % c->kv_heads != 0)
     return fail(EMMY_EINVAL, what, "heads must be a positive multiple of kv_heads");
   if (int64_t(heads) * c->tokens > 0x7fffffff) return fail(EMMY_EINVAL, what, "too many query rows");
+  if (int64_t(c->pages) * 2 * c->kv_heads * c->page_size > 0x7fffffff)
+    return fail(EMMY_EINVAL, what, "a layer holds at most 2^31 - 1 rows of head_dim codes");
+  const int sms = sm_count(c->device);
+  if (sms == 0) return fail(EMMY_ECUDART, what, "cannot read the device's SM count");
+  const int64_t group = heads / c->kv_heads, most = group * c->max_q;
+  const int64_t segments = int64_t(c->seqs) * c->kv_heads;
+  p.tiles = most > ROWS_MOST;
+  p.rows = !p.tiles || c->seqs > 1;
+  p.nt = rows_blocks(most < ROWS_MOST ? most : ROWS_MOST);
+  const int wave = sms * rows_per_sm(p.nt);
+  p.spread = segments > wave;
+  // Workspace slots, two counters each.  Two waves: a cut segment has c >= 1.5 q
+  // chunks and at most c / q + 1/2 parts, a third above its share.
+  const int fit = EMMY_KV8_WORKSPACE_ZERO / 8;
+  p.slots = 3 * wave < fit ? 3 * wave : fit;
+  p.target = p.spread ? p.slots * 2 / 3 : wave < p.slots ? wave : p.slots;
+  // The parts wanted, or, where no try fitted, one of each segment more; but
+  // no more than chunks that the table could hold.
+  p.most_parts = (p.spread ? p.slots : p.target) + segments;
+  const int64_t chunks = int64_t(c->table_width) * c->page_size / 64 * segments;
+  if (chunks < p.most_parts) p.most_parts = chunks;
+  if (!p.rows) p.most_parts = 0;
+  // units of 256 rows: at most one part-filled one of a sequence
+  p.most_units = p.tiles ? (c->tokens * group / 256 + c->seqs) * c->kv_heads : 0;
+  if (p.most_units > 0x7fffffff || p.most_parts > 0x7fffffff || segments > (1 << 24))
+    return fail(EMMY_EINVAL, what, "too many sequences and heads for one call");
+  p.workspace_bytes = EMMY_KV8_WORKSPACE_ZERO + uint64_t(p.slots) * 8 * p.nt * (c->head_dim + 2) * 4;
+  // kernels read the record of their index before they know how many there are
+  p.plan_bytes = sizeof(PlanHead) + uint64_t(p.most_parts) * sizeof(PartRec) + uint64_t(p.most_units) * sizeof(UnitRec);
   return EMMY_OK;
 }
+
+// The checks that attend and its plan share.
+int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_attend_args *a, PlanShape &shape, AttendParams &p) {
+  int rc = check_cache(what, cache);
+  if (rc == EMMY_OK) rc = check_seqs(what, cache);
+  if (rc != EMMY_OK) return rc;
+  if (a == nullptr) return fail(EMMY_EINVAL, what, "null arguments");
+  rc = shape_of(what, cache, a->heads, shape);
+  if (rc != EMMY_OK) return rc;
+  if (a->window < 0 || a->sinks < 0) return fail(EMMY_EINVAL, what, "window and sinks must not be negative");
+  if (a->sinks > 0 && a->window == 0) return fail(EMMY_EINVAL, what, "sinks need a window");
+  if (a->plan == 0 || a->plan % 16 || a->plan_bytes < shape.plan_bytes)
+    return fail(EMMY_EINVAL, what, "plan is missing, unaligned or too small");
+  p = AttendParams{};
+  p.s = seqs_of(*cache);
+  p.codes = reinterpret_cast<const uint8_t *>(cache->codes);
+  p.exps = reinterpret_cast<const int8_t *>(cache->exps);
+  p.plan = reinterpret_cast<PlanHead *>(a->plan);
+  p.parts = reinterpret_cast<PartRec *>(p.plan + 1);
+  p.units = reinterpret_cast<UnitRec *>(p.parts + shape.most_parts);
+  p.group = a->heads / cache->kv_heads;
+  p.window = a->window;
+  p.sinks = a->sinks;
+  p.row_limit = shape.rows ? ROWS_MOST : 0;
+  p.nt = shape.nt;
+  return EMMY_OK;
+}
+
+static_assert(sizeof(PlanHead) % 16 == 0 && sizeof(PartRec) == 48 && sizeof(UnitRec) == 32, "plan layout");
 
 }  // namespace
 }  // namespace kv8
 
-extern "C" int emmy_kv8_attend_workspace(const emmy_kv8 *cache, int32_t heads, uint64_t *bytes) {
+extern "C" int emmy_kv8_attend_sizes(const emmy_kv8 *cache, int32_t heads, uint64_t *workspace_bytes,
+                                     uint64_t *plan_bytes) {
   using namespace kv8;
-  static const char *what = "emmy_kv8_attend_workspace";
+  static const char *what = "emmy_kv8_attend_sizes";
   int rc = check_cache(what, cache);
-  if (rc == EMMY_OK && bytes == nullptr) rc = fail(EMMY_EINVAL, what, "null result");
-  if (rc == EMMY_OK) rc = check_heads(what, cache, heads);
+  if (rc == EMMY_OK && (workspace_bytes == nullptr || plan_bytes == nullptr))
+    rc = fail(EMMY_EINVAL, what, "null result");
+  PlanShape shape;
+  if (rc == EMMY_OK) rc = shape_of(what, cache, heads, shape);
   if (rc != EMMY_OK) return rc;
-  if (sm_count(cache->device) == 0) return fail(EMMY_ECUDART, what, "cannot read the device's SM count");
-  const int64_t rows = int64_t(heads / cache->kv_heads) * cache->max_q;
-  const int nt = rows_blocks(rows < ROWS_MOST ? rows : ROWS_MOST);
-  *bytes = EMMY_KV8_WORKSPACE_ZERO + rows_partial_bytes(nt, cache->head_dim, cache->device);
+  *workspace_bytes = shape.workspace_bytes;
+  *plan_bytes = shape.plan_bytes;
   return EMMY_OK;
+}
+
+extern "C" int emmy_kv8_attend_plan(const emmy_kv8 *cache, const emmy_kv8_attend_args *a, emmy_stream stream) {
+  using namespace kv8;
+  static const char *what = "emmy_kv8_attend_plan";
+  PlanShape shape;
+  AttendParams p;
+  const int rc = check_args(what, cache, a, shape, p);
+  if (rc != EMMY_OK) return rc;
+  const OnDevice on(cache->device);
+  if (on.err != cudaSuccess) return cuda_fail(what, on.err);
+  return plan_attend(p, shape, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args *a, emmy_stream stream) {
   using namespace kv8;
-  int rc = check_cache(WHAT, cache);
-  if (rc == EMMY_OK) rc = check_seqs(WHAT, cache);
-  if (rc != EMMY_OK) return rc;
-  if (a == nullptr) return fail(EMMY_EINVAL, WHAT, "null arguments");
-  rc = check_heads(WHAT, cache, a->heads);
+  static const char *what = "emmy_kv8_attend";
+  PlanShape shape;
+  AttendParams p;
+  int rc = check_args(what, cache, a, shape, p);
   if (rc != EMMY_OK) return rc;
   if (a->dtype != EMMY_KV8_BF16 && a->dtype != EMMY_KV8_F16)
-    return fail(EMMY_EINVAL, WHAT, "dtype must be bf16 or f16");
-  if (a->window < 0 || a->sinks < 0) return fail(EMMY_EINVAL, WHAT, "window and sinks must not be negative");
-  if (a->sinks > 0 && a->window == 0) return fail(EMMY_EINVAL, WHAT, "sinks need a window");
-  if (!std::isfinite(a->scale)) return fail(EMMY_EINVAL, WHAT, "scale must be finite");
+    return fail(EMMY_EINVAL, what, "dtype must be bf16 or f16");
+  if (!std::isfinite(a->scale)) return fail(EMMY_EINVAL, what, "scale must be finite");
   if (cache->tokens == 0 || cache->max_q == 0) return EMMY_OK;
-  if (a->q == 0 || a->out == 0) return fail(EMMY_EINVAL, WHAT, "null q or out");
+  if (a->q == 0 || a->out == 0) return fail(EMMY_EINVAL, what, "null q or out");
   if (a->q % 16 || a->out % 16 || a->q_strides[0] % 8 || a->q_strides[1] % 8 || a->out_strides[0] % 8 ||
       a->out_strides[1] % 8)
-    return fail(EMMY_EINVAL, WHAT, "q and out: base and strides must be multiples of 16 bytes");
+    return fail(EMMY_EINVAL, what, "q and out: base and strides must be multiples of 16 bytes");
   if (a->q_strides[0] < 0 || a->q_strides[1] < 0 || a->out_strides[0] < 0 || a->out_strides[1] < 0)
-    return fail(EMMY_EINVAL, WHAT, "q and out: strides must not be negative");
+    return fail(EMMY_EINVAL, what, "q and out: strides must not be negative");
   const auto extent = [&](const int64_t st[2]) {
     return uint64_t((cache->tokens - 1) * st[0] + (a->heads - 1) * st[1] + cache->head_dim) * 2;
   };
   if (overlap(a->q, extent(a->q_strides), a->out, extent(a->out_strides)))
-    return fail(EMMY_EINVAL, WHAT, "q and out overlap");
-  uint64_t need = 0;
-  rc = emmy_kv8_attend_workspace(cache, a->heads, &need);
-  if (rc != EMMY_OK) return rc;
-  if (a->workspace == 0 || a->workspace % 16 || a->workspace_bytes < need)
-    return fail(EMMY_EINVAL, WHAT, "workspace is missing, unaligned or too small");
-
-  AttendParams p;
-  p.s = seqs_of(*cache);
-  p.codes = reinterpret_cast<const uint8_t *>(cache->codes);
-  p.exps = reinterpret_cast<const int8_t *>(cache->exps);
+    return fail(EMMY_EINVAL, what, "q and out overlap");
+  if (a->workspace == 0 || a->workspace % 16 || a->workspace_bytes < shape.workspace_bytes)
+    return fail(EMMY_EINVAL, what, "workspace is missing, unaligned or too small");
   p.q = reinterpret_cast<const void *>(a->q);
   p.out = reinterpret_cast<void *>(a->out);
   p.q_ts = a->q_strides[0], p.q_hs = a->q_strides[1];
@@ -75,29 +136,11 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   p.counters = reinterpret_cast<unsigned *>(a->workspace);
   p.partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO);
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  p.group = a->heads / cache->kv_heads;
-  p.window = a->window;
-  p.sinks = a->sinks;
-  p.target = 0;
-  p.spread = false;
-  // A sequence with up to ROWS_MOST rows of a kv head is the row kernel's,
-  // others the tile kernel's, which takes the one sequence of a call that may
-  // be either.
-  const int64_t most = int64_t(p.group) * cache->max_q;
-  const bool tiles = most > ROWS_MOST, rows = !tiles || cache->seqs > 1;
-  p.row_limit = rows ? ROWS_MOST : 0;
-  const int nt = rows_blocks(most < ROWS_MOST ? most : ROWS_MOST);
-  if (int64_t(cache->pages) * 2 * cache->kv_heads * cache->page_size > 0x7fffffff)
-    return fail(EMMY_EINVAL, WHAT, "a layer holds at most 2^31 - 1 rows of head_dim codes");
-  if (int64_t(cache->seqs) * cache->kv_heads > (1 << 24))
-    return fail(EMMY_EINVAL, WHAT, "too many sequences and heads for one call");
   const OnDevice on(cache->device);
-  if (on.err != cudaSuccess) return cuda_fail(WHAT, on.err);
+  if (on.err != cudaSuccess) return cuda_fail(what, on.err);
   const bool bf16 = a->dtype == EMMY_KV8_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (tiles) {
-    rc = tiles_attend(p, *cache, bf16, st);
-    if (rc != EMMY_OK) return rc;
-  }
-  return rows ? rows_attend(p, *cache, nt, bf16, st) : EMMY_OK;
+  if (shape.tiles) rc = tiles_attend(p, *cache, shape, bf16, st);
+  if (rc == EMMY_OK && shape.rows) rc = rows_attend(p, *cache, shape, bf16, st);
+  return rc;
 }

@@ -7,6 +7,22 @@
 
 namespace kv8 {
 
+// A plan (see kv8_plan.cu): head, then a record for each part of the row
+// kernel, then one for each unit of the tile kernel.
+struct PlanHead {
+  int parts, units;
+  int group, window, sinks, row_limit, seqs, kv_heads, nt, width, page_shift, pad;  // what it was made for
+};
+struct alignas(16) PartRec {
+  int b, head, c0, c1;  // chunks c0 .. c1 - 1 of the segment's line
+  int part, parts, slot0, chunks;
+  int start, n, len, pad;
+};
+struct alignas(16) UnitRec {
+  int b, head, row0, start;
+  int n, len, pad[2];
+};
+
 struct AttendParams {
   Seqs s;
   const uint8_t *codes;
@@ -16,13 +32,36 @@ struct AttendParams {
   int64_t q_ts, q_hs, o_ts, o_hs;  // token and head strides, elements
   float *partial;
   unsigned *counters;
+  PlanHead *plan;
+  PartRec *parts;
+  UnitRec *units;
   float scale_log2;  // scale * log2(e)
   int group;         // query heads of a kv head
   int window, sinks;
   int row_limit;     // sequences with more rows of a kv head than this are the tile kernel's
-  int target;        // parts that the row kernel is to cut its segments into
-  bool spread;       // in two waves rather than one
+  int nt;            // 8-row blocks of the row kernel
 };
+
+// How large a plan gets and what it aims at, from what the host knows.
+struct PlanShape {
+  bool rows, tiles;    // which kernels run
+  int nt;              // 8-row blocks of the row kernel
+  int target;          // parts that the row kernel's segments are to be cut into
+  bool spread;         // in two waves rather than one
+  int slots;           // workspace slots for cut segments' parts
+  int64_t most_parts, most_units;
+  uint64_t workspace_bytes, plan_bytes;
+};
+
+// The record is for this call, and what it says is within the arrays.
+__device__ __forceinline__ bool plan_fits(const AttendParams &p, const PlanHead &h, int b, int start, int n, int len) {
+  const bool ok = h.group == p.group && h.window == p.window && h.sinks == p.sinks && h.row_limit == p.row_limit &&
+                  h.seqs == p.s.seqs && h.kv_heads == p.s.kv_heads && h.nt == p.nt && h.width == p.s.width &&
+                  h.page_shift == p.s.page_shift && start + n <= p.s.tokens &&
+                  len <= (int64_t(p.s.width) << p.s.page_shift);
+  if (!ok) report(p.s.status, STATUS_PLAN);
+  return ok;
+}
 
 // Which keys a block of query rows sees, and the 64-key chunks that hold
 // them: those of the sinks, then those of the window.  Chunks never straddle
@@ -105,9 +144,13 @@ __device__ __forceinline__ int row_exponent(float amax) {
 // Rows of a kv head up to which a sequence is the row kernel's.
 constexpr int ROWS_MOST = 32;
 
-int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, bool bf16, cudaStream_t stream);
-int rows_blocks(int64_t rows);
-uint64_t rows_partial_bytes(int nt, int head_dim, int device);
-int rows_attend(AttendParams p, const emmy_kv8 &cache, int nt, bool bf16, cudaStream_t stream);
+// 8-row blocks a CTA of the row kernel takes together, for the rows of the
+// largest sequence, and how many such CTAs the launch bounds let an SM hold.
+inline int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4; }
+constexpr int rows_per_sm(int nt) { return nt <= 2 ? 3 : 2; }
+
+int plan_attend(const AttendParams &p, const PlanShape &shape, cudaStream_t stream);
+int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream);
+int rows_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream);
 
 }  // namespace kv8

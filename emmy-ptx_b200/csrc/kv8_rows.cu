@@ -68,134 +68,6 @@ struct Segment {
   Span span;
 };
 
-// 64-key chunks of sequence b that this kernel is to read (0: not its own).
-__device__ __forceinline__ int seq_chunks(const AttendParams &p, int b) {
-  int start, n, len;
-  if (b >= p.s.seqs) return 0;
-  lengths(p.s, b, start, n, len);
-  return n == 0 || n * p.group > p.row_limit ? 0 : Span(p, len - n, len - 1).chunks;
-}
-// Parts of a segment of c chunks, at no more than q chunks a part, or (spread)
-// as near to q as may be.
-__device__ __forceinline__ int parts_of(int c, int q, bool spread) {
-  return c == 0 ? 0 : spread ? max(1, min((2 * c + q) / (2 * q), c)) : (c + q - 1) / q;
-}
-
-__device__ __forceinline__ int warp_scan(int x, int lane) {  // inclusive
-  for (int d = 1; d < 32; d <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, x, d);
-    if (lane >= d) x += u;
-  }
-  return x;
-}
-
-// Which segment and part is CTA `want`'s: g.b, g.head, g.part, g.parts, g.slot0.
-//
-// Where all segments fit on the GPU at once (p.spread false), parts of at most
-// q chunks, q the least of a few tries that leaves them one wave: equal parts
-// that start together.  Otherwise two waves of parts of about equal length,
-// which the order of arrival evens out.  Measured (us, one wave | two): 2
-// sequences of 131071 keys 37 | 43, 48 with a window of 1024 19 | 28, 16 with
-// five drafts 33 | 41; but 64 of 700-8191 keys, 512 segments on 444 CTAs,
-// 111 | 97.
-//
-// Up to 128 sequences every warp finds it for itself, four sequences a lane;
-// more of them, the block together.
-template <int SEQS>
-__device__ __forceinline__ bool locate_in(const AttendParams &p, Segment &g, int want, int lane, int warp) {
-  constexpr bool BLOCK = SEQS == 0;
-  const int H = p.s.kv_heads, tid = threadIdx.x;
-  __shared__ long long sums[ALL_WARPS][5];
-  __shared__ int scans[2][ALL_WARPS], found[5];
-  const int per = BLOCK ? (p.s.seqs + THREADS - 1) / THREADS : SEQS;
-  const int b0 = (BLOCK ? tid : lane) * per;
-  int own[BLOCK ? 1 : SEQS];
-  if constexpr (!BLOCK) {
-#pragma unroll
-    for (int i = 0; i < SEQS; ++i) own[i] = seq_chunks(p, b0 + i);
-  }
-  const auto chunks_of = [&](int i) {
-    if constexpr (BLOCK)
-      return seq_chunks(p, b0 + i);
-    else
-      return own[i];
-  };
-  const auto total_of = [&](long long x, int slot) {
-    for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    if constexpr (BLOCK) {
-      if (lane == 0) sums[warp][slot] = x;
-      __syncthreads();
-      x = 0;
-      for (int w = 0; w < ALL_WARPS; ++w) x += sums[w][slot];
-    }
-    return x;
-  };
-  long long chunks = 0;
-  if (BLOCK && tid == 0) found[0] = -1;
-  for (int i = 0; i < per; ++i) chunks += chunks_of(i);
-  chunks = total_of(chunks, 0);
-  const int q0 = int((chunks * H + p.target - 1) / p.target);
-  if (q0 == 0) return false;
-  int q = q0;
-  if (!p.spread) {
-    for (int t = 1; t < 5; ++t) {
-      long long parts = 0;
-      for (int i = 0; i < per; ++i) parts += parts_of(chunks_of(i), q, false);
-      if (total_of(parts, t) * H <= p.target) break;
-      q = q0 + (q0 * (1 << t) + 15) / 16;  // 1/8, 1/4, 1/2, 1 above q0
-    }
-  }
-  int parts = 0, slots = 0;
-  for (int i = 0; i < per; ++i) {
-    const int k = parts_of(chunks_of(i), q, p.spread);
-    parts += k * H;
-    slots += k > 1 ? k * H : 0;
-  }
-  int at = warp_scan(parts, lane), slot = warp_scan(slots, lane);
-  if constexpr (BLOCK) {
-    if (lane == 31) scans[0][warp] = at, scans[1][warp] = slot;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) at += scans[0][w], slot += scans[1][w];
-  }
-  at -= parts;
-  slot -= slots;
-  int f[5] = {-1, 0, 0, 0, 0};
-  const bool mine = want >= at && want < at + parts;  // one thread's share holds it
-  if (mine) {
-#pragma unroll 4
-    for (int i = 0; i < per; ++i) {
-      const int k = parts_of(chunks_of(i), q, p.spread);
-      if (f[0] < 0 && want < at + k * H) {
-        f[0] = b0 + i;
-        f[1] = (want - at) / k;
-        f[2] = (want - at) % k;
-        f[3] = k;
-        f[4] = slot + f[1] * k;
-      }
-      at += k * H;
-      slot += k > 1 ? k * H : 0;
-    }
-  }
-  if constexpr (BLOCK) {
-    if (mine)
-      for (int i = 0; i < 5; ++i) found[i] = f[i];
-    __syncthreads();
-    for (int i = 0; i < 5; ++i) f[i] = found[i];
-  } else {
-    const unsigned who = __ballot_sync(0xffffffffu, mine);
-    if (who == 0) return false;
-#pragma unroll
-    for (int i = 0; i < 5; ++i) f[i] = __shfl_sync(0xffffffffu, f[i], __ffs(who) - 1);
-  }
-  g.b = f[0], g.head = f[1], g.part = f[2], g.parts = f[3], g.slot0 = f[4];
-  return g.b >= 0;
-}
-__device__ __forceinline__ bool locate(const AttendParams &p, Segment &g, int want, int lane, int warp) {
-  if (p.s.seqs <= 32) return locate_in<1>(p, g, want, lane, warp);
-  if (p.s.seqs <= 128) return locate_in<4>(p, g, want, lane, warp);
-  return locate_in<0>(p, g, want, lane, warp);
-}
-
 // What goes with a chunk of codes.
 struct ChunkInfo {
   int key0, ek, ev, dead;
@@ -410,8 +282,11 @@ __device__ __forceinline__ int query_row(uint32_t (&f)[D / 8], const T *row, int
 }
 
 // Shared memory: first the joined rows of the four warps, over the staged queries.
+template <int NT>
+constexpr int rows_per_sm_of = rows_per_sm(NT);
+
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(THREADS, NT <= 2 ? 3 : 2)
+__global__ void __launch_bounds__(THREADS, rows_per_sm_of<NT>)
 rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map) {
   using L = Layout<D, NT>;
   constexpr int ROWS = 8 * NT, LD = L::LD;
@@ -427,10 +302,14 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
   volatile unsigned *const stop = &stop_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gr = lane >> 2, q = lane & 3;
   const Seqs &s = p.s;
-  Segment g;
   grid_dependency_wait();
-  if (!locate(p, g, blockIdx.x, lane, warp)) return;
+  const PlanHead head = *p.plan;
+  const PartRec rec = p.parts[blockIdx.x];
   grid_dependency_done();
+  if (blockIdx.x >= head.parts || !plan_fits(p, head, rec.b, rec.start, rec.n, rec.len)) return;
+  const Segment g = {rec.b, rec.head, rec.start, rec.n, rec.len, rec.n * p.group, rec.part, rec.parts, rec.slot0,
+                     Span(p, rec.len - rec.n, rec.len - 1)};
+  const int c0 = rec.c0, c1 = rec.c1;
   if (tid == 0) {
     for (int i = 0; i < L::STAGES; ++i) {
       bar_init(&full[i], 1);
@@ -439,12 +318,7 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
     stop_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  lengths(s, g.b, g.start, g.n, g.len);
-  g.span = Span(p, g.len - g.n, g.len - 1);
-  g.rows = g.n * p.group;
-  const int chunks = g.span.chunks;
   if (tid < ROWS) row_pos[tid] = tid < g.rows ? g.len - g.n + tid / p.group : -1;
-  const int c0 = int(int64_t(chunks) * g.part / g.parts), c1 = int(int64_t(chunks) * (g.part + 1) / g.parts);
   __syncthreads();
 
   State<D, NT> st;
@@ -716,39 +590,51 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
       part_l[i] = __ldcg(at + ROWS);
     }
     __syncthreads();
-    if (tid < ROWS) {
-      float m = NONE, l = 0.0f;
-      for (int c = 0; c < count; ++c) m = fmaxf(m, part_m[c * ROWS + tid]);
-      for (int c = 0; c < count; ++c) {
-        const float f = exp2_fast(part_m[c * ROWS + tid] - m);
-        part_m[c * ROWS + tid] = f;
-        l += f * part_l[c * ROWS + tid];
+    for (int r = warp; r < rows; r += ALL_WARPS) {  // a lane two parts
+      const float m0 = lane < count ? part_m[lane * ROWS + r] : NONE;
+      const float m1 = lane + 32 < count ? part_m[(lane + 32) * ROWS + r] : NONE;
+      float m = fmaxf(m0, m1);
+      for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      const float f0 = exp2_fast(m0 - m), f1 = exp2_fast(m1 - m);
+      float l = 0.0f;
+      if (lane < count) {
+        part_m[lane * ROWS + r] = f0;
+        l = f0 * part_l[lane * ROWS + r];
       }
-      row_m[tid] = m;
-      row_l[tid] = l;
+      if (lane + 32 < count) {
+        part_m[(lane + 32) * ROWS + r] = f1;
+        l += f1 * part_l[(lane + 32) * ROWS + r];
+      }
+      for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      if (lane == 0) row_m[r] = m, row_l[r] = l;
     }
     __syncthreads();
-    for (int i = tid; i < rows * (D / 8); i += THREADS) {
-      const int r = i / (D / 8), d = i % (D / 8) * 8;
-      float x[8] = {};
-#pragma unroll 8
-      for (int c = 0; c < count; ++c) {
-        const float *at = part_slot(a + c * step) + r * D + d;
-        const float f = part_m[c * ROWS + r];
-        const float4 u = __ldcg(reinterpret_cast<const float4 *>(at));
-        const float4 v4 = __ldcg(reinterpret_cast<const float4 *>(at + 4));
-        x[0] += f * u.x, x[1] += f * u.y, x[2] += f * u.z, x[3] += f * u.w;
-        x[4] += f * v4.x, x[5] += f * v4.y, x[6] += f * v4.z, x[7] += f * v4.w;
+    for (int i = tid; i < rows * (D / 4); i += THREADS) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const float *at = part_slot(a) + r * D + d;
+      const int64_t stride = int64_t(step) * ROWS * (D + 2);
+      for (int c0 = 0; c0 < count; c0 += 16) {  // sixteen loads in flight
+        float4 u[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          if (c0 + c < count) u[c] = __ldcg(reinterpret_cast<const float4 *>(at + (c0 + c) * stride));
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          if (c0 + c < count) {
+            const float f = part_m[(c0 + c) * ROWS + r];
+            x.x += f * u[c].x, x.y += f * u[c].y, x.z += f * u[c].z, x.w += f * u[c].w;
+          }
       }
       if (last) {
-        store(r, d, x, row_l[r]);
+        const float by = row_l[r] == 0.0f ? 0.0f : 1.0f / row_l[r];
+        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) =
+            make_uint2(pack2<T>(x.x * by, x.y * by), pack2<T>(x.z * by, x.w * by));
       } else {  // only this thread reads or writes these values of part a now
-        float *to = part_slot(a) + r * D + d;
-        __stcg(reinterpret_cast<float4 *>(to), make_float4(x[0], x[1], x[2], x[3]));
-        __stcg(reinterpret_cast<float4 *>(to + 4), make_float4(x[4], x[5], x[6], x[7]));
+        __stcg(reinterpret_cast<float4 *>(part_slot(a) + r * D + d), x);
       }
     }
-    if (!last && tid < ROWS) {
+    if (!last && tid < rows) {
       __stcg(part_slot(a) + ROWS * D + tid, row_m[tid]);
       __stcg(part_slot(a) + ROWS * D + ROWS + tid, row_l[tid]);
     }
@@ -783,33 +669,9 @@ int launch_nt(const AttendParams &p, const CUtensorMap &map, int nt, int device,
 
 }  // namespace
 
-// 8-row blocks a CTA takes together, for the rows of the largest sequence.
-int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4; }
-
-// CTAs that the launch bounds let reside.
-int rows_slots(int nt, int device) { return sm_count(device) * (nt <= 2 ? 3 : 2); }
-
-// Workspace slots, two counters each.  One wave: at most as many parts.  Two:
-// a cut segment has c >= 1.5 q chunks and at most c / q + 1/2 parts, a third
-// above its share.
-int rows_parts(int nt, int device) {
-  const int most = 3 * rows_slots(nt, device), fit = EMMY_KV8_WORKSPACE_ZERO / 8;
-  return most < fit ? most : fit;
-}
-uint64_t rows_partial_bytes(int nt, int head_dim, int device) {
-  return uint64_t(rows_parts(nt, device)) * 8 * nt * (head_dim + 2) * 4;
-}
-
-int rows_attend(AttendParams p, const emmy_kv8 &cache, int nt, bool bf16, cudaStream_t stream) {
-  const int64_t segments = int64_t(p.s.seqs) * p.s.kv_heads;
-  const int64_t chunks = ((int64_t(p.s.width) << p.s.page_shift) >> 6) * segments;
-  const int slots = rows_slots(nt, cache.device), parts = rows_parts(nt, cache.device);
-  p.spread = segments > slots;
-  p.target = p.spread ? parts * 2 / 3 : slots < parts ? slots : parts;
-  // the parts wanted, or, where no try fitted, one of each segment more; but
-  // no more than chunks that the table could hold
-  int64_t grid = (p.spread ? parts : p.target) + segments;
-  if (chunks < grid) grid = chunks;
+int rows_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream) {
+  const int64_t grid = shape.most_parts;
+  const int nt = shape.nt;
   // the pool as rows of head_dim bytes, 64 of them a box
   const int64_t rows = int64_t(cache.pages) * 2 * cache.kv_heads * cache.page_size;
   emmy_tmap_desc d = {};

@@ -176,62 +176,19 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
   // by the time chunk g + 4 is written there, P V of chunk g + 1 is done and
   // with it every softmax warp past chunk g.
   __shared__ float2 chunk_scale[4];
-  __shared__ unsigned stop_word, scan[THREADS / 32], chunk_nan[4];
+  __shared__ unsigned stop_word, chunk_nan[4];
   __shared__ ChunkInfo raw_info[RAW];
-  __shared__ int found[2];
   volatile unsigned *const stop = &stop_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Seqs &s = p.s;
 
   grid_dependency_wait();
+  const PlanHead head = *p.plan;
+  const UnitRec rec = p.units[blockIdx.x];
   grid_dependency_done();
-  // ---- which unit: the grid counts row blocks of all sequences, each for
-  // every kv head, the blocks with the most keys first ----
-  Unit u;
-  {
-    const int per = (s.seqs + THREADS - 1) / THREADS, b0 = min(tid * per, s.seqs), b1 = min(b0 + per, s.seqs);
-    const unsigned want = blockIdx.x;
-    unsigned sum = 0;
-    for (int b = b0; b < b1; ++b) {
-      int start, n, len;
-      lengths(s, b, start, n, len);
-      if (n * p.group <= p.row_limit) n = 0;
-      sum += unsigned((n * p.group + 2 * TILE - 1) / (2 * TILE)) * s.kv_heads;
-    }
-    unsigned at = sum;
-    for (int d = 1; d < 32; d <<= 1) {
-      const unsigned x = __shfl_up_sync(0xffffffffu, at, d);
-      if (lane >= d) at += x;
-    }
-    if (lane == 31) scan[warp] = at;
-    if (tid == 0) found[0] = -1;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) at += scan[w];
-    at -= sum;
-    if (want >= at && want < at + sum) {  // one thread's share holds it
-      for (int b = b0; b < b1; ++b) {
-        int start, n, len;
-        lengths(s, b, start, n, len);
-        if (n * p.group <= p.row_limit) n = 0;
-        const unsigned c = unsigned((n * p.group + 2 * TILE - 1) / (2 * TILE)) * s.kv_heads;
-        if (want < at + c) {
-          found[0] = b;
-          found[1] = int(want - at);
-          break;
-        }
-        at += c;
-      }
-    }
-    __syncthreads();
-    if (found[0] < 0) return;
-    u.b = found[0];
-    lengths(s, u.b, u.start, u.n, u.len);
-    u.rows = u.n * p.group;
-    u.head = found[1] % s.kv_heads;
-    u.row0 = ((u.rows + 2 * TILE - 1) / (2 * TILE) - 1 - found[1] / s.kv_heads) * (2 * TILE);
-    const int last_row = min(u.row0 + 2 * TILE, u.rows) - 1;
-    u.span = Span(p, u.len - u.n + u.row0 / p.group, u.len - u.n + last_row / p.group);
-  }
+  if (blockIdx.x >= head.units || !plan_fits(p, head, rec.b, rec.start, rec.n, rec.len)) return;
+  Unit u = {rec.b, rec.head, rec.start, rec.n, rec.len, rec.n * p.group, rec.row0, {}};
+  u.span = Span(p, u.len - u.n + u.row0 / p.group, u.len - u.n + (min(u.row0 + 2 * TILE, u.rows) - 1) / p.group);
   const int tiles = u.rows - u.row0 > TILE ? 2 : 1;
   const int chunks = u.span.chunks;
 
@@ -663,11 +620,8 @@ int launch(const AttendParams &p, int device, unsigned grid, cudaStream_t stream
 
 }  // namespace
 
-int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, bool bf16, cudaStream_t stream) {
-  // row blocks of all sequences: at most one part-filled one each
-  const int64_t blocks = (int64_t(p.s.tokens) * p.group) / (2 * TILE) + p.s.seqs;
-  const int64_t grid = blocks * p.s.kv_heads;
-  if (grid > 0x7fffffff) return fail(EMMY_EINVAL, "emmy_kv8_attend", "too many query rows");
+int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream) {
+  const int64_t grid = shape.most_units;
   const int dev = cache.device;
   if (cache.head_dim == 64)
     return bf16 ? launch<64, __nv_bfloat16>(p, dev, unsigned(grid), stream)

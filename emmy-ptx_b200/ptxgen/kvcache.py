@@ -52,7 +52,8 @@ WORKSPACE_ZERO = 16384     # bytes of a workspace that start as zeros
 
 STATUS = {0x401: "a page number outside the pool",
           0x402: "a sequence longer than its row of the table, or more new tokens than keys or rows",
-          0x403: "a bounded wait inside a kernel ran out"}
+          0x403: "a bounded wait inside a kernel ran out",
+          0x404: "a plan that was made for another call"}
 
 
 class _Cache(C.Structure):
@@ -66,7 +67,8 @@ class _Cache(C.Structure):
 class _Attend(C.Structure):
     """``emmy_kv8_attend_args``."""
     _fields_ = [("q", C.c_uint64), ("out", C.c_uint64), ("workspace", C.c_uint64),
-                ("workspace_bytes", C.c_uint64), ("q_strides", C.c_int64 * 2),
+                ("plan", C.c_uint64), ("workspace_bytes", C.c_uint64), ("plan_bytes", C.c_uint64),
+                ("q_strides", C.c_int64 * 2),
                 ("out_strides", C.c_int64 * 2), ("dtype", C.c_int32), ("heads", C.c_int32),
                 ("window", C.c_int32), ("sinks", C.c_int32), ("scale", C.c_float)]
 
@@ -119,10 +121,19 @@ def _ordinal(dev, name: str) -> int:
     return dev.index
 
 
-def _stream_of(stream, dev: Device):
+def _stream_of(stream, dev: Device) -> int:
+    if type(stream) is int:
+        return stream
     if stream is None:
-        return dev.stream
-    return getattr(stream, "cuda_stream", stream)
+        stream = dev.stream
+    stream = getattr(stream, "cuda_stream", stream)
+    return stream if isinstance(stream, int) else stream.value or 0
+
+
+# Device's own copy calls take a null stream for "the device's"; these take the
+# handle as it is, 0 included.
+def _copy_in(dev: Device, dst: int, host: np.ndarray, st: int) -> None:
+    check(dev.L.emmy_memcpy_htod(dst, host.ctypes.data, host.nbytes, st), "htod")
 
 
 def _ints(x, name: str) -> np.ndarray:
@@ -157,6 +168,8 @@ class KVCache:
         self.layer_codes = pages * 2 * kv_heads * page_size * head_dim
         self.layer_exps = pages * 2 * kv_heads
         self._own: list[int] = []
+        self._spare: dict[tuple, list[int]] = {}
+        self._closed = False
         self._storage = storage
         if storage is not None:
             codes, exps = storage
@@ -226,11 +239,36 @@ class KVCache:
                                              dst[i:].ctypes.data, min(MAX_PAIRS, n - i), st),
                   "copy_pages")
 
+    def _take(self, use: str, nbytes: int, stream: int) -> tuple[int, tuple]:
+        """(address, key to give it back by) of a buffer for work on ``stream``:
+        one of a closed batch that was used on that stream alone, which needs
+        no wait, or a new one."""
+        key = (use, 1 << max(12, (nbytes - 1).bit_length()), stream)
+        held = self._spare.get(key)
+        if held:
+            return held.pop(), key
+        ptr = self.dev.alloc(key[1])
+        if use == "workspace":
+            check(self.L.emmy_memset_d32(ptr, 0, WORKSPACE_ZERO // 4, stream), "memset")
+        return ptr, key
+
+    def _give(self, ptr: int, key: tuple, reuse: bool) -> None:
+        if reuse and not self._closed and len(self._spare.setdefault(key, [])) < 8:
+            self._spare[key].append(ptr)
+        else:
+            self.dev.free(ptr)          # waits for what still runs on it
+
     def close(self) -> None:
         """Free what this cache allocated (not adopted storage)."""
-        for p in self._own:
+        for p in self._own + [p for held in self._spare.values() for p in held]:
             self.dev.free(p)
-        self._own = []
+        self._own, self._spare, self._closed = [], {}, True
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # the context may be gone when the process ends
+            pass
 
 
 class Batch:
@@ -239,7 +277,8 @@ class Batch:
     rows behind the last one are left alone.  Calls of one batch share a
     workspace, so they must not overlap on the GPU: two captured graphs, or
     two streams, that run at once need a batch each.  A graph captured over
-    these calls replays with what ``update`` last put there."""
+    these calls replays with what ``update`` last put there; the batch has to
+    live as long as the graph may run."""
 
     def __init__(self, cache: KVCache, page_table, kv_lens, q_lens=None, stream=None):
         self.cache, self.dev, self.L = cache, cache.dev, cache.L
@@ -252,12 +291,15 @@ class Batch:
         if self.width * cache.page_size > 2 ** 30:
             raise EmmyError("a sequence holds at most 2^30 keys")
         self.tokens = self.max_q = None
-        self._buf = self._ws = 0
-        self._ws_bytes, self._ws_heads = 0, 0
+        self._buf = 0
+        self._held: list[tuple[int, tuple]] = []   # buffers of this batch, to give back
+        self._ws: tuple[int, int] = (0, 0)         # workspace: address, bytes
+        self._plans: dict[tuple, tuple] = {}       # (heads, window, sinks): plan address and bytes
         self._stale = False
         host = self._packed(table, kv_lens, q_lens)
-        self._buf = self.dev.alloc(host.nbytes)
-        self.dev.htod(self._buf, host, _stream_of(stream, self.dev))
+        self._stream, self._reuse = _stream_of(stream, self.dev), True
+        self._buf = self._take("batch", host.nbytes)
+        _copy_in(self.dev, self._buf, host, self._stream)
         d = self._d = cache._desc()
         d.status = self._buf
         d.kv_lens = self._buf + 16
@@ -267,6 +309,17 @@ class Batch:
         self._ref = C.byref(d)
         self._a = _Attend()
         self._aref = C.byref(self._a)
+
+    def _take(self, use: str, nbytes: int) -> int:
+        held = self.cache._take(use, nbytes, self._stream)
+        self._held.append(held)
+        return held[0]
+
+    def _on(self, stream) -> int:
+        st = _stream_of(stream, self.dev)
+        if st != self._stream:
+            self._reuse = False
+        return st
 
     def _packed(self, table, kv_lens, q_lens) -> np.ndarray:
         """Checked lengths and table as one int32 array: status word and
@@ -308,7 +361,10 @@ class Batch:
         new tokens than the batch was made for."""
         self._live()
         host = self._packed(_ints(page_table, "page_table"), kv_lens, q_lens)
-        self.dev.htod(self._buf + 16, host[4:], _stream_of(stream, self.dev))
+        st = self._on(stream)
+        _copy_in(self.dev, self._buf + 16, host[4:], st)
+        for key in self._plans:
+            self._plan(key, st)
         self._stale = False
 
     def _live(self) -> None:
@@ -350,25 +406,34 @@ class Batch:
         if kt != vt or kt > 2:
             raise EmmyError("append: k and v must both be f32, bf16 or f16")
         rc = self.L.emmy_kv8_append(self._ref, kp, vp, kt, _Strides(ks[0], ks[1]),
-                                    _Strides(vs[0], vs[1]), _stream_of(stream, self.dev))
+                                    _Strides(vs[0], vs[1]), self._on(stream))
         if rc:
             check(rc, "append")
 
-    def reserve(self, heads: int, stream=None) -> None:
-        """Allocate the workspace that ``attend`` with ``heads`` query heads
-        needs (done by the first call otherwise): before a graph is captured."""
-        if heads == self._ws_heads:
-            return
+    def reserve(self, heads: int, window: int = 0, sinks: int = 0, stream=None) -> None:
+        """What ``attend`` needs for ``heads`` query heads, a window and sinks
+        besides its arrays: workspace and plan.  The first call does it
+        otherwise; before a graph is captured it has to be done."""
         self._live()
-        need = C.c_uint64()
-        check(self.L.emmy_kv8_attend_workspace(self._ref, heads, C.byref(need)), "attend")
-        if need.value > self._ws_bytes:
-            new = self.dev.alloc(need.value)
-            if self._ws:
-                self.dev.free(self._ws)      # waits for what still runs on it
-            self._ws, self._ws_bytes = new, need.value
-            self.dev.memset32(new, 0, WORKSPACE_ZERO // 4, _stream_of(stream, self.dev))
-        self._ws_heads = heads
+        key = (heads, window, sinks)
+        if key in self._plans:
+            return
+        ws, plan = C.c_uint64(), C.c_uint64()
+        check(self.L.emmy_kv8_attend_sizes(self._ref, heads, C.byref(ws), C.byref(plan)), "attend")
+        if ws.value > self._ws[1]:
+            self._ws = self._take("workspace", ws.value), ws.value
+        self._plans[key] = self._take("plan", plan.value), plan.value
+        try:
+            self._plan(key, self._on(stream))
+        except EmmyError:
+            del self._plans[key]
+            raise
+
+    def _plan(self, key: tuple, st: int) -> None:
+        a = self._a
+        a.heads, a.window, a.sinks = key
+        a.plan, a.plan_bytes = self._plans[key]
+        check(self.L.emmy_kv8_attend_plan(self._ref, self._aref, st), "attend")
 
     def attend(self, layer: int, q, out, scale: float | None = None, window: int = 0,
                sinks: int = 0, stream=None):
@@ -383,14 +448,18 @@ class Batch:
         op, ot, os_, _ = self._array(out, "out", heads)
         if qt != ot or qt not in (1, 2):
             raise EmmyError("attend: q and out must both be bf16 or f16")
-        if heads != self._ws_heads:
-            self.reserve(heads, stream)
-        a.q, a.out, a.workspace, a.workspace_bytes = qp, op, self._ws, self._ws_bytes
+        plan = self._plans.get((heads, window, sinks))
+        if plan is None:
+            self.reserve(heads, window, sinks, stream)
+            plan = self._plans[heads, window, sinks]
+        a.q, a.out = qp, op
+        a.workspace, a.workspace_bytes = self._ws
+        a.plan, a.plan_bytes = plan
         a.q_strides[0], a.q_strides[1] = qs[0], qs[1]
         a.out_strides[0], a.out_strides[1] = os_[0], os_[1]
         a.dtype, a.heads, a.window, a.sinks = qt, heads, window, sinks
         a.scale = self.cache.head_dim ** -0.5 if scale is None else scale
-        rc = self.L.emmy_kv8_attend(self._ref, self._aref, _stream_of(stream, self.dev))
+        rc = self.L.emmy_kv8_attend(self._ref, self._aref, self._on(stream))
         if rc:
             check(rc, "attend")
         return out
@@ -400,21 +469,21 @@ class Batch:
         something in its status word; clears it."""
         self._live()
         word = np.zeros(1, np.uint32)
-        st = _stream_of(stream, self.dev)
-        self.dev.dtoh(word, self._buf, st)
-        self.dev.sync(st)
+        st = self._on(stream)
+        check(self.L.emmy_memcpy_dtoh(word.ctypes.data, self._buf, 4, st), "dtoh")
+        check(self.L.emmy_stream_sync(st), "stream sync")
         if word[0]:
-            self.dev.memset32(self._buf, 0, 1, st)
+            check(self.L.emmy_memset_d32(self._buf, 0, 1, st), "memset")
             raise EmmyError(f"cache kernel reported error 0x{word[0]:x}: "
                             f"{STATUS.get(int(word[0]), 'unknown')}")
 
     def close(self) -> None:
-        buf, ws = self._buf, self._ws
-        self._buf = self._ws = 0
-        self._ws_bytes, self._ws_heads = 0, 0
-        for p in (buf, ws):
-            if p:
-                self.dev.free(p)
+        """Give the batch's buffers back to its cache: nothing that is not
+        queued on the batch's stream yet may use them after this."""
+        held, self._held = self._held, []
+        self._buf, self._ws, self._plans = 0, (0, 0), {}
+        for ptr, key in held:
+            self.cache._give(ptr, key, self._reuse)
 
     def __del__(self):
         try:

@@ -238,19 +238,27 @@ int emmy_kv8_append(const emmy_kv8 *cache, emmy_dptr k, emmy_dptr v, int32_t dty
  * reads kv head h / (heads / kv_heads).  Query i of n in a sequence of L keys
  * stands at position p = L - n + i and sees key j when j <= p and (window ==
  * 0, or p - j < window, or j < sinks).  A query that sees no key gives zeros.
- * `workspace`: emmy_kv8_attend_workspace() bytes, 16-byte aligned, its first
- * EMMY_KV8_WORKSPACE_ZERO bytes zero before the first call and left zero by
- * each; calls that may overlap on the GPU need workspaces of their own. */
+ * `workspace` and `plan`: emmy_kv8_attend_sizes() bytes, 16-byte aligned, the
+ * workspace's first EMMY_KV8_WORKSPACE_ZERO bytes zero before the first call
+ * and left zero by each; calls that may overlap on the GPU need workspaces of
+ * their own.  emmy_kv8_attend_plan writes the plan -- how the work is cut, from
+ * the lengths on the device -- on `stream`; it reads heads, window, sinks, plan
+ * and plan_bytes of `args`, and holds for every layer and call with the same
+ * cache description, heads, window and sinks until the lengths change.  A
+ * plan made for another call is noticed and reported, its output not written;
+ * one made from lengths that have changed since computes those lengths' rows. */
 typedef struct {
-  emmy_dptr q, out, workspace;
-  uint64_t workspace_bytes;
+  emmy_dptr q, out, workspace, plan;
+  uint64_t workspace_bytes, plan_bytes;
   int64_t q_strides[2], out_strides[2];
   int32_t dtype, heads;
   int32_t window, sinks;
   float scale;
 } emmy_kv8_attend_args;
 enum { EMMY_KV8_WORKSPACE_ZERO = 16384 };
-int emmy_kv8_attend_workspace(const emmy_kv8 *cache, int32_t heads, uint64_t *bytes);
+int emmy_kv8_attend_sizes(const emmy_kv8 *cache, int32_t heads, uint64_t *workspace_bytes,
+                          uint64_t *plan_bytes);
+int emmy_kv8_attend_plan(const emmy_kv8 *cache, const emmy_kv8_attend_args *args, emmy_stream stream);
 int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args *args, emmy_stream stream);
 
 /* In each of `layers` layers, laid out one after another, copy page src[i]
