@@ -26,7 +26,7 @@ sequence of L keys sees key j <= L - n + i, and with a window W only those
 with L - n + i - j < W or j < sinks.
 
 Arrays are device arrays: anything with ``data_ptr()``, ``stride()``,
-``shape``, ``dtype`` and ``device`` as torch tensors have them, or a
+``get_device()``, ``shape`` and ``dtype`` as torch tensors have them, or a
 ``DeviceArray`` over a raw address.  No gradients are recorded.  Calls are
 queued on ``stream`` (an address, or an object with ``cuda_stream``; default
 the device's stream, ``Device.stream``; 0 is the legacy default stream),
@@ -38,6 +38,7 @@ as with every other call here.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import numpy as np
 
@@ -96,6 +97,9 @@ class DeviceArray:
     def stride(self) -> tuple:
         return self.strides
 
+    def get_device(self) -> int:
+        return self.device
+
 
 _DTYPES = {"f32": 0, "bf16": 1, "f16": 2, "u8": 3, "i8": 4}
 _NAMES = {"float32": "f32", "bfloat16": "bf16", "float16": "f16", "half": "f16", "uint8": "u8",
@@ -111,14 +115,6 @@ def _dtype_code(dtype) -> int:
             raise EmmyError(f"unsupported dtype {dtype}")
         _DTYPES[dtype] = code
     return code
-
-
-def _ordinal(dev, name: str) -> int:
-    if isinstance(dev, int):
-        return dev
-    if getattr(dev, "type", None) != "cuda":
-        raise EmmyError(f"{name} is not on a GPU")
-    return dev.index
 
 
 def _stream_of(stream, dev: Device) -> int:
@@ -185,7 +181,7 @@ class KVCache:
                     if size != 1 and stride != n:
                         raise EmmyError(f"storage: {name} must be contiguous")
                     n *= size
-                if _ordinal(x.device, name) != device:
+                if x.get_device() != device:
                     raise EmmyError(f"storage: {name} is not on device {device}")
             self.codes, self.exps = codes.data_ptr(), exps.data_ptr()
             if self.codes % 16:
@@ -201,6 +197,8 @@ class KVCache:
             self.dev.memset32(self.codes, 0, (layers * self.layer_codes + 3) // 4)
             self.dev.memset32(self.exps, 0, (layers * self.layer_exps + 3) // 4)
             self.dev.sync()
+        self._cdesc = self._desc()
+        self._cref = C.byref(self._cdesc)
 
     def _desc(self) -> _Cache:
         d = _Cache()
@@ -219,25 +217,29 @@ class KVCache:
     def copy_pages(self, src, dst, stream=None) -> None:
         """Copy pages ``src[i]`` to ``dst[i]`` in every layer (host lists);
         no page twice in ``dst`` nor in both lists."""
-        src, dst = _ints(src, "src"), _ints(dst, "dst")
-        if src.ndim != 1 or src.shape != dst.shape:
-            raise EmmyError("copy_pages: src and dst are lists of the same length")
+        try:
+            src, dst = array("i", src), array("i", dst)
+        except (TypeError, OverflowError) as exc:
+            raise EmmyError(f"copy_pages: src and dst are lists of page numbers: {exc}") from None
         n = len(src)
+        if n != len(dst):
+            raise EmmyError("copy_pages: src and dst are lists of the same length")
         if n == 0:
             return
-        if min(src.min(), dst.min()) < 0 or max(src.max(), dst.max()) >= self.pages:
+        if min(src) < 0 or min(dst) < 0 or max(src) >= self.pages or max(dst) >= self.pages:
             raise EmmyError(f"copy_pages: a page is outside 0..{self.pages - 1}")
-        targets = set(dst.tolist())
+        targets = set(dst)
         if len(targets) != n:
             raise EmmyError("copy_pages: a page is in dst twice")
-        if not targets.isdisjoint(src.tolist()):
+        if not targets.isdisjoint(src):
             raise EmmyError("copy_pages: a page is in both src and dst")
-        src, dst = src.astype(np.int32), dst.astype(np.int32)
-        d, st = self._desc(), _stream_of(stream, self.dev)
+        st = _stream_of(stream, self.dev)
+        at, to = src.buffer_info()[0], dst.buffer_info()[0]
         for i in range(0, n, MAX_PAIRS):
-            check(self.L.emmy_kv8_copy_pages(C.byref(d), self.layers, src[i:].ctypes.data,
-                                             dst[i:].ctypes.data, min(MAX_PAIRS, n - i), st),
-                  "copy_pages")
+            rc = self.L.emmy_kv8_copy_pages(self._cref, self.layers, at + 4 * i, to + 4 * i,
+                                            min(MAX_PAIRS, n - i), st)
+            if rc:
+                check(rc, "copy_pages")
 
     def _take(self, use: str, nbytes: int, stream: int) -> tuple[int, tuple]:
         """(address, key to give it back by) of a buffer for work on ``stream``:
@@ -306,9 +308,11 @@ class Batch:
         d.q_starts = d.kv_lens + 4 * self.seqs
         d.page_table = d.q_starts + 4 * (self.seqs + 1)
         d.seqs, d.table_width, d.tokens, d.max_q = self.seqs, self.width, self.tokens, self.max_q
-        self._ref = C.byref(d)
+        self._ref, self._layer = C.byref(d), 0
         self._a = _Attend()
         self._aref = C.byref(self._a)
+        self._ks, self._vs = _Strides(), _Strides()
+        self._append, self._attend = self.L.emmy_kv8_append, self.L.emmy_kv8_attend
 
     def _take(self, use: str, nbytes: int) -> int:
         held = self.cache._take(use, nbytes, self._stream)
@@ -377,9 +381,11 @@ class Batch:
             raise EmmyError("the batch names pages that compact() moved: update it or make a new one")
         if not 0 <= layer < self.cache.layers:
             raise EmmyError(f"layer {layer} is outside 0..{self.cache.layers - 1}")
-        d, c = self._d, self.cache
-        d.codes = c.codes + layer * c.layer_codes
-        d.exps = c.exps + layer * c.layer_exps
+        if layer != self._layer:
+            d, c = self._d, self.cache
+            d.codes = c.codes + layer * c.layer_codes
+            d.exps = c.exps + layer * c.layer_exps
+            self._layer = layer
 
     def _array(self, x, name: str, heads: int | None):
         """(address, dtype code, (token, head) strides, heads) of a
@@ -391,9 +397,10 @@ class Batch:
                             f"[>= {self.tokens}, {heads or 'heads'}, {self.cache.head_dim}]")
         if stride[2] != 1:
             raise EmmyError(f"{name}: the last dimension must be contiguous")
-        if _ordinal(x.device, name) != self.cache.ordinal:
+        if x.get_device() != self.cache.ordinal:
             raise EmmyError(f"{name} is not on device {self.cache.ordinal}")
-        return x.data_ptr(), _dtype_code(x.dtype), stride, shape[1]
+        code = _DTYPES.get(x.dtype)
+        return x.data_ptr(), _dtype_code(x.dtype) if code is None else code, stride, shape[1]
 
     def append(self, layer: int, k, v, stream=None) -> None:
         """Write the new tokens' keys and values (f32, bf16 or f16) into
@@ -405,8 +412,9 @@ class Batch:
         vp, vt, vs, _ = self._array(v, "v", self.cache.kv_heads)
         if kt != vt or kt > 2:
             raise EmmyError("append: k and v must both be f32, bf16 or f16")
-        rc = self.L.emmy_kv8_append(self._ref, kp, vp, kt, _Strides(ks[0], ks[1]),
-                                    _Strides(vs[0], vs[1]), self._on(stream))
+        sk, sv = self._ks, self._vs
+        sk[0], sk[1], sv[0], sv[1] = ks[0], ks[1], vs[0], vs[1]
+        rc = self._append(self._ref, kp, vp, kt, sk, sv, self._on(stream))
         if rc:
             check(rc, "append")
 
@@ -459,7 +467,7 @@ class Batch:
         a.out_strides[0], a.out_strides[1] = os_[0], os_[1]
         a.dtype, a.heads, a.window, a.sinks = qt, heads, window, sinks
         a.scale = self.cache.head_dim ** -0.5 if scale is None else scale
-        rc = self.L.emmy_kv8_attend(self._ref, self._aref, self._on(stream))
+        rc = self._attend(self._ref, self._aref, self._on(stream))
         if rc:
             check(rc, "attend")
         return out
