@@ -43,16 +43,18 @@ __device__ __forceinline__ void report(unsigned *status, unsigned code) {
   if (status != nullptr) *status = code;
 }
 
-// Lengths of sequence b, or n = 0 (nothing to do) where they cannot be right.
+// n, or 0 (nothing to do), reported, where the lengths cannot be right.
+__device__ __forceinline__ int checked_n(const Seqs &s, int start, int n, int len) {
+  if (n >= 0 && n <= len && start >= 0 && start + n <= s.tokens && len <= (int64_t(s.width) << s.page_shift)) return n;
+  report(s.status, STATUS_LENGTH);
+  return 0;
+}
+// Lengths of sequence b: first row, new tokens, keys.
 __device__ __forceinline__ void lengths(const Seqs &s, int b, int &start, int &n, int &len) {
   start = s.q_starts[b];
   n = s.q_starts[b + 1] - start;
   len = s.kv_lens[b];
-  if (n < 0 || n > len || start < 0 || start + n > s.tokens ||
-      len > (int64_t(s.width) << s.page_shift)) {
-    report(s.status, STATUS_LENGTH);
-    n = 0;
-  }
+  n = checked_n(s, start, n, len);
 }
 
 // Two e4m3 codes (bits 0-15 of w) as f16x2; every e4m3 value is exact in f16.

@@ -8,12 +8,14 @@
 // scale by a power of two is exact above e4m3's subnormals).
 //
 // Bound by memory: each new value is read once (2 or 4 bytes) and written
-// once (1 byte).  One CTA does one (page, side, head), its rows spread over
-// the warps and held in registers, as they came, between the maximum and the
-// rounding, so nothing is read twice; a page's rows are contiguous in the pool.
-// Where no sequence has more than one new token, a warp does one (sequence,
-// side, head).
+// once (1 byte).  One CTA does one page, a few of its (side, head)s one after
+// another: a thread copies its own 16-byte pieces of the next one's rows into
+// shared memory (cp.async) while it takes the maximum of this one's and rounds
+// them, so loads stay in flight through the reductions.  Where no sequence has
+// more than one new token, a warp does one (sequence, side, head).
 #include <cuda_bf16.h>
+
+#include <algorithm>
 
 #include "kv8.cuh"
 
@@ -26,6 +28,7 @@ struct AppendParams {
   int8_t *exps;
   const void *x[2];
   int64_t ts[2], hs[2];  // token and head strides, elements
+  int units;             // (side, head)s of a page that a CTA does
 };
 
 // Sixteen bytes of values: as they are held, and as f32.
@@ -33,7 +36,7 @@ template <typename T>
 struct Vec {
   static constexpr int N = 16 / sizeof(T);
   uint4 w;
-  __device__ __forceinline__ void load(const T *p) { w = __ldg(reinterpret_cast<const uint4 *>(p)); }
+  __device__ __forceinline__ void load(const void *p) { w = *static_cast<const uint4 *>(p); }
   __device__ __forceinline__ float at(int i) const;
 };
 template <>
@@ -113,78 +116,121 @@ __device__ __forceinline__ void store_codes(uint8_t *at, const Vec<T> &v, int e)
 // Exponent of a page's side and head that was `held` before, as it may be.
 __device__ __forceinline__ int held_exponent(int8_t held) { return max(min(int(held), E_MAX), E_MIN); }
 
-// Slot of this grid's page list -> (sequence, page of the sequence).  The
-// pages that n tokens touch are at most n / P + 2, and floor((s + n) / P) -
-// floor(s / P) >= floor(n / P), so sequence b may own the slots from
-// q_starts[b] / P + 2 b on; the last b at or below the slot is the owner.
-__device__ __forceinline__ int owner(const Seqs &s, int slot) {
+// Slot of this grid's page list -> its sequence's lengths and the page of the
+// sequence; false: none.  The pages that n tokens touch are at most n / P + 2,
+// and floor((s + n) / P) - floor(s / P) >= floor(n / P), so sequence b may own
+// the slots from q_starts[b] / P + 2 b on; the last b at or below the slot is
+// the owner.  A warp reads 32 sequences' lengths at once.
+__device__ __forceinline__ bool owner(const Seqs &s, int slot, int &b, int &start, int &n, int &len, int &page_of_seq) {
   const int lane = threadIdx.x & 31;
-  int count = 0;
+  int from = -1, qs = 0, qe = 0, kv = 0;  // the last group that has a sequence at or below the slot
   for (int b0 = 0; b0 < s.seqs; b0 += 32) {
-    const int b = b0 + lane;
-    const bool at = b < s.seqs && (s.q_starts[b] >> s.page_shift) + 2 * b <= slot;
-    const int here = __popc(__ballot_sync(0xffffffffu, at));
-    count += here;
+    const bool in = b0 + lane < s.seqs;
+    const int q0 = in ? s.q_starts[b0 + lane] : 0, q1 = in ? s.q_starts[b0 + lane + 1] : 0;
+    const int k = in ? s.kv_lens[b0 + lane] : 0;
+    const int here = __popc(__ballot_sync(0xffffffffu, in && (q0 >> s.page_shift) + 2 * (b0 + lane) <= slot));
+    if (here > 0) from = b0 + here - 1, qs = q0, qe = q1, kv = k;
     if (here < 32) break;
   }
-  return count - 1;
+  if (from < 0) return false;
+  b = from;
+  start = __shfl_sync(0xffffffffu, qs, from & 31);
+  len = __shfl_sync(0xffffffffu, kv, from & 31);
+  n = checked_n(s, start, __shfl_sync(0xffffffffu, qe, from & 31) - start, len);
+  const int first = (len - n) >> s.page_shift;
+  page_of_seq = first + slot - ((start >> s.page_shift) + 2 * b);
+  return n > 0 && page_of_seq >= first && page_of_seq <= (len - 1) >> s.page_shift;
+}
+
+// Threads for a page of P rows: eight 16-byte pieces each.
+template <int D, typename T>
+constexpr int page_threads(int page) {
+  return page * D * int(sizeof(T)) / 128;
+}
+template <int D, typename T>
+constexpr int MOST_THREADS = page_threads<D, T>(256);
+
+// 16 bytes, or zeros where there is nothing to copy.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 
 template <int D, typename T>
-__global__ void append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(MOST_THREADS<D, T>) append_kernel(const AppendParams p) {
   using V = Vec<T>;
-  constexpr int LPR = D / V::N;             // lanes per row, 16 bytes each
-  constexpr int RPW = 32 / LPR;             // rows per warp and pass
-  constexpr int PASSES = 64 / (4 * RPW);    // 64 rows to 128 threads
+  constexpr int LPR = D / V::N;  // lanes per row, 16 bytes each
+  constexpr int RPW = 32 / LPR;  // rows per warp and pass
+  constexpr int PASSES = 8;
+  extern __shared__ uint4 pieces[];  // [2][PASSES][threads]
+  __shared__ float part[2][32];
   const Seqs &s = p.s;
   grid_dependency_wait();
   grid_dependency_done();
-  const int b = owner(s, blockIdx.x);
-  if (b < 0) return;
-  int start, n, len;
-  lengths(s, b, start, n, len);
-  if (n == 0) return;
-  const int P = 1 << s.page_shift, first = len - n;
-  const int page_of_seq = (first >> s.page_shift) + blockIdx.x - ((start >> s.page_shift) + 2 * b);
-  if (page_of_seq < first >> s.page_shift || page_of_seq > (len - 1) >> s.page_shift) return;
+  int b, start, n, len, page_of_seq;
+  if (!owner(s, blockIdx.x, b, start, n, len, page_of_seq)) return;
+  const int P = 1 << s.page_shift, first = len - n, H = s.kv_heads;
   const int page = s.table[int64_t(b) * s.width + page_of_seq];
-  const int head = blockIdx.y, side = blockIdx.z;
   const int pos0 = page_of_seq << s.page_shift;
   const int lo = max(first - pos0, 0), hi = min(len - pos0, P);  // new rows of the page
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
   const int col = lane % LPR * V::N, row0 = warp * RPW + lane / LPR, step = warps * RPW;
-  const T *x = static_cast<const T *>(side ? p.x[1] : p.x[0]) + head * (side ? p.hs[1] : p.hs[0]) + col;
-  const int64_t ts = side ? p.ts[1] : p.ts[0];
-  V v[PASSES];
+  const int64_t token0 = int64_t(start) + pos0 - first;  // row 0 of the page, were it new
+  const auto fetch = [&](int u, int buf) {
+    const int side = u >= H, head = u - side * H;
+    const int64_t ts = side ? p.ts[1] : p.ts[0];
+    const T *x = static_cast<const T *>(side ? p.x[1] : p.x[0]) + head * (side ? p.hs[1] : p.hs[0]) + col;
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(pieces + buf * PASSES * threads + tid));
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = row0 + i * step;
-    v[i].w = make_uint4(0, 0, 0, 0);
-    if (r >= lo && r < hi) v[i].load(x + (int64_t(start) + pos0 + r - first) * ts);
-  }
-  if (page < 0 || page >= s.pages) {
-    report(s.status, STATUS_PAGE);
-    return;
-  }
-  const int64_t unit = (int64_t(page) * 2 + side) * s.kv_heads + head;
-  uint8_t *codes = p.codes + (unit << s.page_shift) * D;
-  const int old = lo > 0 ? held_exponent(p.exps[unit]) : E_MIN;
-  float amax = 0.0f;
+    for (int i = 0; i < PASSES; ++i) {
+      const int r = row0 + i * step;
+      const bool real = r >= lo && r < hi;
+      copy16(to + i * threads * 16, x + (token0 + (real ? r : lo)) * ts, real);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int u0 = blockIdx.y * p.units, u1 = min(u0 + p.units, 2 * H);
+  fetch(u0, 0);
+  const bool bad = page < 0 || page >= s.pages;
+  if (bad && tid == 0) report(s.status, STATUS_PAGE);
+  const int64_t unit0 = int64_t(bad ? 0 : page) * 2 * H;
+  int held = lo > 0 ? p.exps[unit0 + u0] : 0;
+  for (int u = u0; u < u1; ++u) {
+    const int buf = (u - u0) & 1, old = lo > 0 ? held_exponent(held) : E_MIN;
+    if (u + 1 < u1) {
+      fetch(u + 1, buf ^ 1);
+      held = lo > 0 ? p.exps[unit0 + u + 1] : 0;
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    // every thread reads only the pieces it copied
+    const uint4 *mine = pieces + buf * PASSES * threads + tid;
+    float amax = 0.0f;
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) amax = max_finite(v[i], amax);
-  __shared__ float part[16];
-  amax = warp_max(amax);
-  if (lane == 0) part[warp] = amax;
-  __syncthreads();
-  for (int w = 0; w < warps; ++w) amax = fmaxf(amax, part[w]);
-  const int e = fit_exponent(amax, old);
-  if (threadIdx.x == 0) p.exps[unit] = int8_t(e);
+    for (int i = 0; i < PASSES; ++i) {
+      V v;
+      v.load(mine + i * threads);
+      amax = max_finite(v, amax);
+    }
+    amax = warp_max(amax);
+    if (lane == 0) part[buf][warp] = amax;
+    __syncthreads();
+    amax = warp_max(lane < warps ? part[buf][lane] : 0.0f);
+    if (bad) continue;
+    const int e = fit_exponent(amax, old);
+    uint8_t *codes = p.codes + ((unit0 + u) << s.page_shift) * D;
+    if (tid == 0) p.exps[unit0 + u] = int8_t(e);
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = row0 + i * step;
-    if (r >= lo && r < hi) store_codes(codes + int64_t(r) * D + col, v[i], e);
+    for (int i = 0; i < PASSES; ++i) {
+      const int r = row0 + i * step;
+      if (r >= lo && r < hi) {
+        V v;
+        v.load(mine + i * threads);
+        store_codes(codes + r * D + col, v, e);
+      }
+    }
+    if (lo > 0 && e > old) recode_rows<D>(codes, lo, old, e, tid, threads);
   }
-  if (lo > 0 && e > old) recode_rows<D>(codes, lo, old, e, threadIdx.x, blockDim.x);
 }
 
 // One new token of a sequence, or none: a warp a (sequence, side, head).
@@ -226,19 +272,30 @@ __global__ void __launch_bounds__(128) append_one_kernel(const AppendParams p) {
 }
 
 template <int D, typename T>
-int launch(const AppendParams &p, bool one, int64_t slots, cudaStream_t stream) {
+int launch(AppendParams p, bool one, int64_t slots, int device, cudaStream_t stream) {
+  const int units = 2 * p.s.kv_heads;
   if (one)
-    return launch_kernel("emmy_kv8_append", append_one_kernel<D, T>, dim3(p.s.seqs, (2 * p.s.kv_heads + 3) / 4), 128, 0,
-                         stream, p);
-  return launch_kernel("emmy_kv8_append", append_kernel<D, T>, dim3(unsigned(slots), p.s.kv_heads, 2),
-                       2 << p.s.page_shift, 0, stream, p);
+    return launch_kernel("emmy_kv8_append", append_one_kernel<D, T>, dim3(p.s.seqs, (units + 3) / 4), 128, 0, stream, p);
+  // several (side, head)s a CTA once there are more than fill the GPU twice
+  const int threads = page_threads<D, T>(1 << p.s.page_shift);
+  const int64_t fill = int64_t(sm_count(device)) * 2 * (2048 / threads < 7 ? 2048 / threads : 7);
+  p.units = int(std::min<int64_t>(units, std::max<int64_t>(1, slots * units / std::max<int64_t>(fill, 1))));
+  int smem = 2 * 8 * 16 * threads;
+  constexpr int ROOM = 200 * 1024;
+  if (smem > ROOM) smem /= 2, p.units = 1;  // no second buffer, so no second unit (f32 pages of 128 KB)
+  static KernelSetup setup;
+  const int rc = setup.ready("emmy_kv8_append", append_kernel<D, T>, device,
+                             std::min(ROOM, 2 * 8 * 16 * MOST_THREADS<D, T>));
+  if (rc != EMMY_OK) return rc;
+  return launch_kernel("emmy_kv8_append", append_kernel<D, T>, dim3(unsigned(slots), (units + p.units - 1) / p.units),
+                       threads, smem, stream, p);
 }
 
 template <int D>
-int launch_type(const AppendParams &p, int dtype, bool one, int64_t slots, cudaStream_t stream) {
-  if (dtype == EMMY_KV8_F32) return launch<D, float>(p, one, slots, stream);
-  if (dtype == EMMY_KV8_BF16) return launch<D, __nv_bfloat16>(p, one, slots, stream);
-  return launch<D, __half>(p, one, slots, stream);
+int launch_type(const AppendParams &p, int dtype, bool one, int64_t slots, int device, cudaStream_t stream) {
+  if (dtype == EMMY_KV8_F32) return launch<D, float>(p, one, slots, device, stream);
+  if (dtype == EMMY_KV8_BF16) return launch<D, __nv_bfloat16>(p, one, slots, device, stream);
+  return launch<D, __half>(p, one, slots, device, stream);
 }
 
 }  // namespace
@@ -275,6 +332,6 @@ extern "C" int emmy_kv8_append(const emmy_kv8 *cache, emmy_dptr k, emmy_dptr v, 
   const int64_t slots = (int64_t(cache->tokens) >> p.s.page_shift) + 2 * int64_t(cache->seqs);
   if (slots > 0x7fffffff) return fail(EMMY_EINVAL, what, "too many tokens");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return cache->head_dim == 64 ? launch_type<64>(p, dtype, cache->max_q == 1, slots, st)
-                               : launch_type<128>(p, dtype, cache->max_q == 1, slots, st);
+  return cache->head_dim == 64 ? launch_type<64>(p, dtype, cache->max_q == 1, slots, cache->device, st)
+                               : launch_type<128>(p, dtype, cache->max_q == 1, slots, cache->device, st);
 }
