@@ -9,8 +9,9 @@
 // a kernel of its own (us, one wave | two): 2 sequences of 131071 keys 37 | 43,
 // 48 with a window of 1024 19 | 28, 16 with five drafts 33 | 41; but 64 of
 // 700-8191 keys, 512 segments on 444 CTAs, 111 | 97.
-// Tile kernel: units of 256 query rows of one (sequence, kv head), a
-// sequence's units with the most keys first.
+// Tile kernel: units of 256 query rows of one (sequence, kv head), those with
+// the most chunks first (by 256 steps of the most): the hardware hands units
+// out in order, and the short ones fill up the end.
 //
 // One CTA: a thread takes a few sequences, scans give each its first record,
 // and the records are then written a thread each.  A layer's worth of work for
@@ -152,7 +153,8 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
       unit += blocks[i] * H;
     }
   __syncthreads();
-  for (int i = tid; i < n_units; i += THREADS) {
+  // counting sort by chunks, the most first; units alike in any order
+  const auto unit_of = [&](int i, int &chunks) {
     const int b = owner_of(part_at, s.seqs, i), rel = i - part_at[b];
     UnitRec r;
     r.b = b;
@@ -160,7 +162,36 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
     r.head = rel % H;
     r.row0 = ((r.n * p.a.group + TILE_ROWS - 1) / TILE_ROWS - 1 - rel / H) * TILE_ROWS;
     r.pad[0] = r.pad[1] = 0;
-    p.a.units[i] = r;
+    const int last = min(r.row0 + TILE_ROWS, r.n * p.a.group) - 1, first = r.len - r.n;
+    chunks = Span(p.a, first + r.row0 / p.a.group, first + last / p.a.group).chunks;
+    return r;
+  };
+  constexpr int STEPS = 256;
+  __shared__ int count[STEPS], most;
+  if (tid < STEPS) count[tid] = 0;
+  if (tid == 0) most = 1;
+  __syncthreads();
+  int c, top = 1;
+  for (int i = tid; i < n_units; i += THREADS) {
+    unit_of(i, c);
+    top = max(top, c);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((tid & 31) == 0) atomicMax(&most, top);
+  __syncthreads();
+  const auto step_of = [&](int chunks) { return int(int64_t(most - chunks) * STEPS / (most + 1)); };
+  for (int i = tid; i < n_units; i += THREADS) {
+    unit_of(i, c);
+    atomicAdd(&count[step_of(c)], 1);
+  }
+  __syncthreads();
+  const int mine_count = tid < STEPS ? count[tid] : 0;
+  const int before = block_scan(mine_count, c, sums);
+  if (tid < STEPS) count[tid] = before;
+  __syncthreads();
+  for (int i = tid; i < n_units; i += THREADS) {
+    const UnitRec r = unit_of(i, c);
+    p.a.units[atomicAdd(&count[step_of(c)], 1)] = r;
   }
 }
 

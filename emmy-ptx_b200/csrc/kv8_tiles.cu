@@ -5,11 +5,13 @@
 // heads that share the kv head, so these share one pass over its keys -- as
 // two tiles A and B of 128 rows, and walks the 64-key chunks that some row
 // sees.  Warps:
-//   0       tcgen05 O += P V of both tiles (one thread); owns the TMEM
-//   1       tcgen05 S = Q K^T of both tiles (one thread)
-//   2       bulk copies of the codes into shared memory, chunks ahead; 3 idle
+//   0, 1    tcgen05 O += P V of tile A, B (one thread each); 0 owns the TMEM
+//   2, 3    tcgen05 S = Q K^T of tile A, B: an issuing warp slows the softmax
+//           warps of its sub-partition, and the slowest of a tile sets its
+//           pace, so each sub-partition gets one
 //   4-7     softmax and output of tile A, a thread a row; 8-11 of tile B
-//   12-15   codes -> f16, stored as the 128-byte-swizzled tiles the MMAs
+//   12-15   bulk copies of codes into shared memory, chunks ahead (12), and
+//           codes -> f16, stored as the 128-byte-swizzled tiles the MMAs
 //           read (K as [keys][d], V as stored: an MN-major operand)
 // 128 registers a thread at launch; the softmax warps take 176 (a row's 64
 // scores and its packed weights are live together) from the others.
@@ -30,7 +32,7 @@ namespace {
 
 constexpr int TILE = 128, CHUNK = 64, THREADS = 512;
 constexpr int STAGES = 3, RAW = 3;  // f16 chunks, and chunks of codes, in shared memory
-constexpr int W_PV = 0, W_QK = 1, W_FETCH = 2, W_SOFTMAX = 4, W_LOAD = 12;  // warps
+constexpr int W_PV = 0, W_QK = 2, W_SOFTMAX = 4, W_LOAD = 12;  // warps
 // Registers of the four warpgroups after the split.  The sum is what the
 // block was launched with: a split above it would wait for ever.
 constexpr int REGS_LAUNCH = 128, REGS_ISSUE = 64, REGS_SOFTMAX = 176, REGS_LOAD = 96;
@@ -103,6 +105,14 @@ __device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t (&r)[32]) {
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+// Half a chunk's time: tile B starts so much later, so that its exponentials
+// fall between tile A's on the MUFU that they share (562 -> 542 us a prompt of
+// 8191 tokens, 238 -> 225 with a window of 512 and d = 64).
+__device__ __forceinline__ void stagger() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 900) {
+  }
 }
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -197,7 +207,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
     bar_init(&bars.q_full, tiles * 4);  // warps
     for (int i = 0; i < STAGES; ++i) {
       bar_init(&bars.kv_full[i], 4);
-      bar_init(&bars.kv_empty[i], 1);
+      bar_init(&bars.kv_empty[i], tiles);
     }
     for (int i = 0; i < 4; ++i) chunk_nan[i] = 0;
     for (int i = 0; i < RAW; ++i) {
@@ -210,7 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         bar_init(&bars.p_full[x][i], 4);
         bar_init(&bars.pv_done[x][i], 1);
       }
-    bar_init(&bars.drain, 2);
+    bar_init(&bars.drain, 4);
     stop_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -225,107 +235,107 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 
   bool issuer = false;  // the lane that issued this warp's MMAs
   if (warp < W_SOFTMAX) regs_down<REGS_ISSUE>();
-  if (warp == W_PV) {
-    // ---- O += P V ----
+  if (warp < W_QK) {
+    // ---- O += P V of one tile ----
     const uint32_t who = elected();
-    bool ok = true;
+    const int x = warp - W_PV;
+    bool ok = x < tiles;
     Ring kv;
     for (int g = 0; ok && g < chunks; ++g, kv.next(STAGES)) {
       const int st = kv.slot, buf = g & 1;
-      ok = warp_wait(&bars.kv_full[st], kv.phase, stop, s.status);
+      ok = warp_wait(&bars.kv_full[st], kv.phase, stop, s.status) &&
+           warp_wait(&bars.p_full[x][buf], g >> 1 & 1, stop, s.status);
+      if (!ok) break;
+      tc_after();
       // V rows are 128 bytes (64 values of d), the second half of d follows
       // CHUNK rows on; 16 keys are 2 KB
       const uint64_t vd = smem_desc(smem_addr(dyn + L::STAGE0 + st * 2 * L::KV + L::KV), CHUNK * 128, 1024);
-      for (int x = 0; ok && x < tiles; ++x) {
-        ok = warp_wait(&bars.p_full[x][buf], g >> 1 & 1, stop, s.status);
-        if (!ok) break;
-        tc_after();
-        const uint32_t o = tmem + L::O_COL + x * D, pa = tmem + (2 * x + buf) * CHUNK;
+      const uint32_t o = tmem + L::O_COL + x * D, pa = tmem + (2 * x + buf) * CHUNK;
 #pragma unroll
-        for (int k = 0; k < CHUNK / 16; ++k)
-          mma_ts(o, pa + k * 8, vd + (k * 2048 >> 4), IDESC<TILE, D, true>, g > 0 || k > 0, who);
-        tc_commit(&bars.pv_done[x][buf], who);
-      }
-      if (ok) tc_commit(&bars.kv_empty[st], who);
+      for (int k = 0; k < CHUNK / 16; ++k)
+        mma_ts(o, pa + k * 8, vd + (k * 2048 >> 4), IDESC<TILE, D, true>, g > 0 || k > 0, who);
+      tc_commit(&bars.pv_done[x][buf], who);
+      tc_commit(&bars.kv_empty[st], who);
     }
     if (who) issuer = true;
-  } else if (warp == W_QK) {
-    // ---- S = Q K^T ----
+  } else if (warp < W_SOFTMAX) {
+    // ---- S = Q K^T of one tile ----
     const uint32_t who = elected();
-    bool ok = warp_wait(&bars.q_full, 0, stop, s.status);
+    const int x = warp - W_QK;
+    bool ok = x < tiles && warp_wait(&bars.q_full, 0, stop, s.status);
+    const uint64_t qd = smem_desc(smem_addr(dyn + x * L::Q_TILE), 16, 1024);
     Ring kv;
     for (int g = 0; ok && g < chunks; ++g, kv.next(STAGES)) {
       const int st = kv.slot, buf = g & 1;
       ok = warp_wait(&bars.kv_full[st], kv.phase, stop, s.status);
+      // the buffer holds P of chunk g - 2 until its P V is done
+      if (ok && g >= 2) ok = warp_wait(&bars.pv_done[x][buf], (g >> 1 & 1) ^ 1, stop, s.status);
+      if (!ok) break;
+      tc_after();
       const uint64_t kd = smem_desc(smem_addr(dyn + L::STAGE0 + st * 2 * L::KV), 16, 1024);
-      for (int x = 0; ok && x < tiles; ++x) {
-        // the buffer holds P of chunk g - 2 until its P V is done
-        if (g >= 2) ok = warp_wait(&bars.pv_done[x][buf], (g >> 1 & 1) ^ 1, stop, s.status);
-        if (!ok) break;
-        tc_after();
-        const uint64_t qd = smem_desc(smem_addr(dyn + x * L::Q_TILE), 16, 1024);
-        const uint32_t at = tmem + (2 * x + buf) * CHUNK;
+      const uint32_t at = tmem + (2 * x + buf) * CHUNK;
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h)
+      for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_ss(at, qd + ((h * TILE * 128 + k * 32) >> 4), kd + ((h * CHUNK * 128 + k * 32) >> 4),
-                   IDESC<TILE, CHUNK, false>, h > 0 || k > 0, who);
-        tc_commit(&bars.s_full[x][buf], who);
-        // and one ordinary arrival, which passes on what the loading warps
-        // left beside the codes
-        if (who) bar_arrive(&bars.s_full[x][buf]);
-      }
+        for (int k = 0; k < 4; ++k)
+          mma_ss(at, qd + ((h * TILE * 128 + k * 32) >> 4), kd + ((h * CHUNK * 128 + k * 32) >> 4),
+                 IDESC<TILE, CHUNK, false>, h > 0 || k > 0, who);
+      tc_commit(&bars.s_full[x][buf], who);
+      // and one ordinary arrival, which passes on what the loading warps
+      // left beside the codes
+      if (who) bar_arrive(&bars.s_full[x][buf]);
     }
     if (who) issuer = true;
-  } else if (warp == W_FETCH) {
-    // ---- codes of a page's chunk: K and V are one contiguous piece each ----
+  } else if (warp >= W_LOAD) {
+    regs_down<REGS_LOAD>();
+    // ---- bulk copies: K and V of a page's chunk are one contiguous piece
+    // each; 32 chunks' pages and exponents are read at once, a lane a chunk ----
+    const bool fetches = warp == W_LOAD;
     const uint32_t who = elected();
     const int *row = s.table + int64_t(u.b) * s.width;
-    Ring raw;
-    bool ok = true;
-    for (int g0 = 0; ok && g0 < chunks; g0 += 32) {
-      // 32 chunks' pages and exponents at once, a lane a chunk
-      ChunkInfo mine = {0, 0, 0, 0};
-      int64_t unit = 0;
-      if (g0 + lane < chunks) {
-        mine.key0 = u.span.key0(g0 + lane);
-        int page = row[mine.key0 >> s.page_shift];
-        mine.dead = page < 0 || page >= s.pages;
-        if (mine.dead) {
-          report(s.status, STATUS_PAGE);
-          page = 0;
+    ChunkInfo next = {0, 0, 0, 0};
+    int64_t next_unit = 0;
+    Ring copied;
+    const auto fetch = [&](int g) {  // chunk g into the next slot, which is free
+      if ((g & 31) == 0) {
+        next = ChunkInfo{0, 0, 0, 0};
+        next_unit = 0;
+        if (g + lane < chunks) {
+          next.key0 = u.span.key0(g + lane);
+          int page = row[next.key0 >> s.page_shift];
+          next.dead = page < 0 || page >= s.pages;
+          if (next.dead) {
+            report(s.status, STATUS_PAGE);
+            page = 0;
+          }
+          next_unit = int64_t(page) * 2 * s.kv_heads + u.head;
+          next.ek = p.exps[next_unit];
+          next.ev = p.exps[next_unit + s.kv_heads];
         }
-        unit = int64_t(page) * 2 * s.kv_heads + u.head;
-        mine.ek = p.exps[unit];
-        mine.ev = p.exps[unit + s.kv_heads];
       }
-      for (int i = 0; ok && i < 32 && g0 + i < chunks; ++i, raw.next(RAW)) {
-        if (g0 + i >= RAW) ok = warp_wait(&bars.raw_empty[raw.slot], raw.phase ^ 1, stop, s.status);
-        if (!ok) break;
-        const int64_t at = __shfl_sync(0xffffffffu, unit, i);
-        ChunkInfo c;
-        c.ek = __shfl_sync(0xffffffffu, mine.ek, i);
-        c.ev = __shfl_sync(0xffffffffu, mine.ev, i);
-        c.key0 = __shfl_sync(0xffffffffu, mine.key0, i);
-        c.dead = __shfl_sync(0xffffffffu, mine.dead, i);
-        if (who) {
-          raw_info[raw.slot] = c;
-          const uint8_t *k = p.codes + ((at << s.page_shift) + (c.key0 & ((1 << s.page_shift) - 1))) * D;
-          const uint8_t *v = k + (int64_t(s.kv_heads) << s.page_shift) * D;
-          const uint32_t dst = smem_addr(dyn + L::RAW0 + raw.slot * L::KV);
-          uint64_t *bar = &bars.raw_full[raw.slot];
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(L::KV)
-                       : "memory");
-          bulk_copy(dst, k, CHUNK * D, bar);
-          bulk_copy(dst + CHUNK * D, v, CHUNK * D, bar);
-        }
-        __syncwarp();
+      const int64_t at = __shfl_sync(0xffffffffu, next_unit, g & 31);
+      ChunkInfo c;
+      c.ek = __shfl_sync(0xffffffffu, next.ek, g & 31);
+      c.ev = __shfl_sync(0xffffffffu, next.ev, g & 31);
+      c.key0 = __shfl_sync(0xffffffffu, next.key0, g & 31);
+      c.dead = __shfl_sync(0xffffffffu, next.dead, g & 31);
+      if (who) {
+        raw_info[copied.slot] = c;
+        const uint8_t *k = p.codes + ((at << s.page_shift) + (c.key0 & ((1 << s.page_shift) - 1))) * D;
+        const uint8_t *v = k + (int64_t(s.kv_heads) << s.page_shift) * D;
+        const uint32_t dst = smem_addr(dyn + L::RAW0 + copied.slot * L::KV);
+        uint64_t *bar = &bars.raw_full[copied.slot];
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(L::KV)
+                     : "memory");
+        bulk_copy(dst, k, CHUNK * D, bar);
+        bulk_copy(dst + CHUNK * D, v, CHUNK * D, bar);
       }
-    }
-  } else if (warp >= W_LOAD) {
+      __syncwarp();
+      copied.next(RAW);
+    };
+    if (fetches)
+      for (int g = 0; g < min(RAW, chunks); ++g) fetch(g);
     // ---- codes -> f16 ----
-    regs_down<REGS_LOAD>();
     // A lane's 16-byte pieces of codes become two neighbouring 16-byte pieces
     // of f16.  D = 128: eight lanes that load or store together cover the two
     // halves of d in two neighbouring rows, so that neither the loads (rows of
@@ -345,6 +355,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
     };
     Ring raw, kv;
     for (int g = 0; g < chunks; ++g, raw.next(RAW), kv.next(STAGES)) {
+      // the slot of chunk g - 1 gets chunk g - 1 + RAW once all four warps read it
+      if (fetches && g > 0 && g - 1 + RAW < chunks) {
+        if (!warp_wait(&bars.raw_empty[copied.slot], copied.phase ^ 1, stop, s.status)) break;
+        fetch(g - 1 + RAW);
+      }
       if (!warp_wait(&bars.raw_full[raw.slot], raw.phase, stop, s.status)) break;
       const uint8_t *src = dyn + L::RAW0 + raw.slot * L::KV + from;
       uint4 k[PASSES], v[PASSES];
@@ -455,6 +470,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         const int buf = g & 1;
         ok = warp_wait(&bars.s_full[x][buf], g >> 1 & 1, stop, s.status);
         if (!ok) break;
+        if (g == 0 && x == 1) stagger();
         const float2 sc = chunk_scale[g & 3];
         const int ev = int(sc.y);
         const float rm = fmaxf(mult * sc.x, LEAST);
@@ -585,7 +601,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 
   // ---- every MMA issued has completed before the TMEM goes (bounded) ----
   __syncthreads();
-  if (*stop != 0 && tid == W_FETCH * 32) {
+  if (*stop != 0 && tid == W_LOAD * 32) {
     // given up: copies in flight land before the block may end (50 ms)
     const unsigned long long t0 = now_ns();
     while (now_ns() - t0 < 50000000ull) {
