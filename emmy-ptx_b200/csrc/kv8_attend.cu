@@ -19,11 +19,12 @@ int shape_of(const char *what, const emmy_kv8 *c, int heads, PlanShape &p) {
   const int sms = sm_count(c->device);
   if (sms == 0) return fail(EMMY_ECUDART, what, "cannot read the device's SM count");
   const int64_t group = heads / c->kv_heads, most = group * c->max_q;
-  const int64_t segments = int64_t(c->seqs) * c->kv_heads;
   p.tiles = most > ROWS_MOST;
   p.rows = !p.tiles || c->seqs > 1;
-  p.nt = rows_blocks(most < ROWS_MOST ? most : ROWS_MOST);
-  const int wave = sms * rows_per_sm(p.nt);
+  const int64_t few = most < ROWS_MOST ? most : ROWS_MOST;
+  p.nt = rows_blocks(few);
+  const int64_t segments = int64_t(c->seqs) * c->kv_heads * ((few + ROWS_BLOCK - 1) / ROWS_BLOCK);
+  const int wave = sms * ROWS_PER_SM;
   p.spread = segments > wave;
   // Workspace slots, two counters each.  Two waves: a cut segment has c >= 1.5 q
   // chunks and at most c / q + 1/2 parts, a third above its share.
@@ -36,13 +37,20 @@ int shape_of(const char *what, const emmy_kv8 *c, int heads, PlanShape &p) {
   const int64_t chunks = int64_t(c->table_width) * c->page_size / 64 * segments;
   if (chunks < p.most_parts) p.most_parts = chunks;
   if (!p.rows) p.most_parts = 0;
-  // units of 256 rows: at most one part-filled one of a sequence
-  p.most_units = p.tiles ? (c->tokens * group / 256 + c->seqs) * c->kv_heads : 0;
+  // Units: at most one part-filled one of a sequence.  Fewer than SMs may be
+  // cut, into at most one more part each than their share of the SMs.
+  const int64_t units = p.tiles ? (c->tokens * group / TILE_ROWS + c->seqs) * c->kv_heads : 0;
+  p.tile_target = units > 0 && units < sms ? sms : 0;
+  p.most_units = units + p.tile_target;
+  p.most_joins = p.tile_target > 0 ? units : 0;
   if (p.most_units > 0x7fffffff || p.most_parts > 0x7fffffff || segments > (1 << 24))
     return fail(EMMY_EINVAL, what, "too many sequences and heads for one call");
-  p.workspace_bytes = EMMY_KV8_WORKSPACE_ZERO + uint64_t(p.slots) * 8 * p.nt * (c->head_dim + 2) * 4;
+  p.partial_bytes = uint64_t(p.slots) * 8 * p.nt * (c->head_dim + 2) * 4;
+  p.workspace_bytes = EMMY_KV8_WORKSPACE_ZERO + p.partial_bytes +
+                      (p.tile_target > 0 ? uint64_t(p.most_units) * TILE_ROWS * (c->head_dim + 2) * 4 : 0);
   // kernels read the record of their index before they know how many there are
-  p.plan_bytes = sizeof(PlanHead) + uint64_t(p.most_parts) * sizeof(PartRec) + uint64_t(p.most_units) * sizeof(UnitRec);
+  p.plan_bytes = sizeof(PlanHead) + uint64_t(p.most_parts) * sizeof(PartRec) +
+                 uint64_t(p.most_units) * sizeof(UnitRec) + uint64_t(p.most_joins) * sizeof(JoinRec);
   return EMMY_OK;
 }
 
@@ -65,6 +73,7 @@ int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_attend_ar
   p.plan = reinterpret_cast<PlanHead *>(a->plan);
   p.parts = reinterpret_cast<PartRec *>(p.plan + 1);
   p.units = reinterpret_cast<UnitRec *>(p.parts + shape.most_parts);
+  p.joins = reinterpret_cast<JoinRec *>(p.units + shape.most_units);
   p.group = a->heads / cache->kv_heads;
   p.window = a->window;
   p.sinks = a->sinks;
@@ -72,8 +81,6 @@ int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_attend_ar
   p.nt = shape.nt;
   return EMMY_OK;
 }
-
-static_assert(sizeof(PlanHead) % 16 == 0 && sizeof(PartRec) == 48 && sizeof(UnitRec) == 32, "plan layout");
 
 }  // namespace
 }  // namespace kv8
@@ -135,6 +142,7 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   p.o_ts = a->out_strides[0], p.o_hs = a->out_strides[1];
   p.counters = reinterpret_cast<unsigned *>(a->workspace);
   p.partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO);
+  p.tile_partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO + shape.partial_bytes);
   p.scale_log2 = a->scale * 1.4426950408889634f;
   const OnDevice on(cache->device);
   if (on.err != cudaSuccess) return cuda_fail(what, on.err);

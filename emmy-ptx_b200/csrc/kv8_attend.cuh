@@ -7,20 +7,25 @@
 
 namespace kv8 {
 
-// A plan (see kv8_plan.cu): head, then a record for each part of the row
-// kernel, then one for each unit of the tile kernel.
-struct PlanHead {
-  int parts, units;
-  int group, window, sinks, row_limit, seqs, kv_heads, nt, width, page_shift, pad;  // what it was made for
+// A plan (see kv8_plan.cu): head, then records for the parts of the row kernel,
+// for those of the tile kernel, and for the tile kernel's units that were cut.
+struct alignas(16) PlanHead {
+  int parts, units, joins;
+  int group, window, sinks, row_limit, seqs, kv_heads, nt, width, page_shift;  // what it was made for
 };
 struct alignas(16) PartRec {
   int b, head, c0, c1;  // chunks c0 .. c1 - 1 of the segment's line
-  int part, parts, slot0, chunks;
-  int start, n, len, pad;
+  int part, parts, slot0, row0;
+  int start, n, len, rows;
 };
 struct alignas(16) UnitRec {
   int b, head, row0, start;
-  int n, len, pad[2];
+  int n, len, c0, c1;  // chunks c0 .. c1 - 1 of the unit's line
+  int slot, pad[3];    // workspace slot of a cut unit's part, -1: the unit is whole
+};
+struct alignas(16) JoinRec {
+  int head, row0, start, rows;  // rows of the sequence's kv head
+  int slot0, parts, b, pad;
 };
 
 struct AttendParams {
@@ -30,11 +35,13 @@ struct AttendParams {
   const void *q;
   void *out;
   int64_t q_ts, q_hs, o_ts, o_hs;  // token and head strides, elements
-  float *partial;
+  float *partial;       // parts of the row kernel
+  float *tile_partial;  // parts of the tile kernel: O [head_dim][256 rows], maxima, sums
   unsigned *counters;
   PlanHead *plan;
   PartRec *parts;
   UnitRec *units;
+  JoinRec *joins;
   float scale_log2;  // scale * log2(e)
   int group;         // query heads of a kv head
   int window, sinks;
@@ -49,7 +56,9 @@ struct PlanShape {
   int target;          // parts that the row kernel's segments are to be cut into
   bool spread;         // in two waves rather than one
   int slots;           // workspace slots for cut segments' parts
-  int64_t most_parts, most_units;
+  int tile_target;     // parts that the tile kernel's units may be cut into, 0: none is
+  int64_t most_parts, most_units, most_joins;
+  uint64_t partial_bytes;  // of the row kernel's parts
   uint64_t workspace_bytes, plan_bytes;
 };
 
@@ -141,13 +150,15 @@ __device__ __forceinline__ int row_exponent(float amax) {
   return amax == 0.0f ? 0 : max(min(e, 126), -126);
 }
 
-// Rows of a kv head up to which a sequence is the row kernel's.
-constexpr int ROWS_MOST = 32;
-
-// 8-row blocks a CTA of the row kernel takes together, for the rows of the
-// largest sequence, and how many such CTAs the launch bounds let an SM hold.
-inline int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4; }
-constexpr int rows_per_sm(int nt) { return nt <= 2 ? 3 : 2; }
+// Rows of a kv head up to which a sequence is the row kernel's, in blocks of at
+// most ROWS_BLOCK rows that each read the keys again (from L2, as neighbours):
+// two CTAs of 16 rows hide more latency than one of 32 (28 -> 17 us for five
+// drafts of 16 sequences).
+constexpr int ROWS_MOST = 32, ROWS_BLOCK = 16;
+constexpr int ROWS_PER_SM = 3;  // CTAs of the row kernel, by its launch bounds
+constexpr int TILE_ROWS = 256;  // rows of a unit of the tile kernel
+// 8-row blocks of a CTA of the row kernel, for the rows of the largest sequence.
+inline int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
 int plan_attend(const AttendParams &p, const PlanShape &shape, cudaStream_t stream);
 int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream);

@@ -1,17 +1,18 @@
 // emmy_kv8_attend_plan -- how attend cuts its work, from the lengths on the
 // device.
 //
-// Row kernel: a segment is one (sequence, kv head) with its visible 64-key
-// chunks.  Where all segments fit on the GPU at once, parts of at most q
-// chunks, q the least of a few tries that leaves them one wave: equal parts
-// that start together.  Otherwise (spread) two waves of parts of about equal
-// length, which the order of arrival evens out.  Measured before the plan was
-// a kernel of its own (us, one wave | two): 2 sequences of 131071 keys 37 | 43,
-// 48 with a window of 1024 19 | 28, 16 with five drafts 33 | 41; but 64 of
-// 700-8191 keys, 512 segments on 444 CTAs, 111 | 97.
-// Tile kernel: units of 256 query rows of one (sequence, kv head), those with
-// the most chunks first (by 256 steps of the most): the hardware hands units
-// out in order, and the short ones fill up the end.
+// Row kernel: a segment is one (sequence, kv head, block of up to 16 rows) with
+// its visible 64-key chunks.  Where all segments fit on the GPU at once, parts
+// of at most q chunks, q the least of a few tries that leaves them one wave:
+// equal parts that start together.  Otherwise (spread) two waves of parts of
+// about equal length, which the order of arrival evens out.  Measured before
+// the plan was a kernel of its own (us, one wave | two): 2 sequences of 131071
+// keys 37 | 43, 48 with a window of 1024 19 | 28, 16 with five drafts 33 | 41;
+// but 64 of 700-8191 keys, 512 segments on 444 CTAs, 111 | 97.
+// Tile kernel: units of 256 query rows of one (sequence, kv head); where there
+// are fewer than SMs they are cut along the keys, too, and joined by a kernel
+// of their own.  The longest come first (by 256 steps of the longest): the
+// hardware hands them out in order, and the short ones fill up the end.
 //
 // One CTA: a thread takes a few sequences, scans give each its first record,
 // and the records are then written a thread each.  A layer's worth of work for
@@ -22,11 +23,10 @@ namespace kv8 {
 namespace {
 
 constexpr int THREADS = 1024, WARPS = 32, EACH = EMMY_KV8_MAX_SEQS / THREADS;
-constexpr int TILE_ROWS = 256;
 
 struct PlanParams {
   AttendParams a;
-  int target, min_chunks, most_parts, most_units;
+  int target, min_chunks, most_parts, most_units, most_joins, tile_target;
   bool spread;
 };
 
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   grid_dependency_done();
   const Seqs &s = p.a.s;
   const int tid = threadIdx.x, H = s.kv_heads, b0 = tid * EACH;
-  int chunks[EACH], blocks[EACH];
+  int chunks[EACH], blocks[EACH];  // segments' chunks; row blocks of 16, or units of 256
   int mine = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
@@ -82,13 +82,13 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
       int start, n, len;
       lengths(s, b0 + i, start, n, len);
       if (n > 0) {
-        if (n * p.a.group <= p.a.row_limit)
-          chunks[i] = Span(p.a, len - n, len - 1).chunks;
-        else
-          blocks[i] = (n * p.a.group + TILE_ROWS - 1) / TILE_ROWS;
+        const bool few = n * p.a.group <= p.a.row_limit;
+        if (few) chunks[i] = Span(p.a, len - n, len - 1).chunks;
+        const int rows = few ? ROWS_BLOCK : TILE_ROWS;
+        blocks[i] = (n * p.a.group + rows - 1) / rows;
       }
     }
-    mine += chunks[i];
+    mine += chunks[i] * blocks[i];
   }
   int all;
   block_scan(mine, all, sums);
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
     for (int t = 1; t < 5; ++t) {
       int parts = 0, total;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) parts += parts_of(chunks[i], q, false);
+      for (int i = 0; i < EACH; ++i) parts += parts_of(chunks[i], q, false) * blocks[i];
       block_scan(parts, total, sums);
       if (int64_t(total) * H <= p.target) break;
       q = q0 + (q0 * (1 << t) + 15) / 16;  // 1/8, 1/4, 1/2, 1 above q0
@@ -108,9 +108,9 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int k = parts_of(chunks[i], q, p.spread);
-    parts += k * H;
-    slots += k > 1 ? k * H : 0;
-    units += blocks[i] * H;
+    parts += k * blocks[i] * H;
+    slots += k > 1 ? k * blocks[i] * H : 0;
+    units += chunks[i] > 0 ? 0 : blocks[i] * H;
   }
   int at = block_scan(parts, n_parts, sums), slot = block_scan(slots, n_slots, sums);
   int unit = block_scan(units, n_units, sums);
@@ -120,29 +120,28 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
       const int k = parts_of(chunks[i], q, p.spread);
       part_at[b0 + i] = at;
       slot_at[b0 + i] = slot;
-      at += k * H;
-      slot += k > 1 ? k * H : 0;
+      at += k * blocks[i] * H;
+      slot += k > 1 ? k * blocks[i] * H : 0;
     }
   __syncthreads();
-  // the launches have room for so many (see rows_attend and tiles_attend)
   n_parts = min(n_parts, p.most_parts);
-  n_units = min(n_units, p.most_units);
-  if (tid == 0)
-    *p.a.plan = PlanHead{n_parts, n_units, p.a.group, p.a.window, p.a.sinks, p.a.row_limit, s.seqs, H, p.a.nt, s.width, s.page_shift, 0};
   for (int i = tid; i < n_parts; i += THREADS) {
     const int b = owner_of(part_at, s.seqs, i), rel = i - part_at[b];
     PartRec r;
     r.b = b;
     lengths(s, b, r.start, r.n, r.len);
     const int c = Span(p.a, r.len - r.n, r.len - 1).chunks, k = parts_of(c, q, p.spread);
-    r.head = rel / k;
-    r.part = rel - r.head * k;
+    const int rows = r.n * p.a.group, nb = (rows + ROWS_BLOCK - 1) / ROWS_BLOCK, each = (rows + nb - 1) / nb;
+    // row blocks of a part are neighbours: they share its keys in L2
+    const int block = rel % nb, cut = rel / nb;
+    r.head = cut / k;
+    r.part = cut - r.head * k;
     r.parts = k;
-    r.slot0 = slot_at[b] + r.head * k;
+    r.slot0 = slot_at[b] + (r.head * nb + block) * k;
     r.c0 = int(int64_t(c) * r.part / k);
     r.c1 = int(int64_t(c) * (r.part + 1) / k);
-    r.chunks = c;
-    r.pad = 0;
+    r.row0 = block * each;
+    r.rows = min(each, rows - r.row0);
     p.a.parts[i] = r;
   }
   __syncthreads();
@@ -150,49 +149,74 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   for (int i = 0; i < EACH; ++i)
     if (b0 + i < s.seqs) {
       part_at[b0 + i] = unit;
-      unit += blocks[i] * H;
+      unit += chunks[i] > 0 ? 0 : blocks[i] * H;
     }
   __syncthreads();
-  // counting sort by chunks, the most first; units alike in any order
-  const auto unit_of = [&](int i, int &chunks) {
+  // ---- units: whole or cut, then a counting sort by length, longest first ----
+  const auto unit_of = [&](int i) {
     const int b = owner_of(part_at, s.seqs, i), rel = i - part_at[b];
-    UnitRec r;
+    UnitRec r = {};
     r.b = b;
     lengths(s, b, r.start, r.n, r.len);
     r.head = rel % H;
-    r.row0 = ((r.n * p.a.group + TILE_ROWS - 1) / TILE_ROWS - 1 - rel / H) * TILE_ROWS;
-    r.pad[0] = r.pad[1] = 0;
+    r.row0 = rel / H * TILE_ROWS;
     const int last = min(r.row0 + TILE_ROWS, r.n * p.a.group) - 1, first = r.len - r.n;
-    chunks = Span(p.a, first + r.row0 / p.a.group, first + last / p.a.group).chunks;
+    r.c1 = Span(p.a, first + r.row0 / p.a.group, first + last / p.a.group).chunks;
+    r.slot = -1;
     return r;
   };
   constexpr int STEPS = 256;
-  __shared__ int count[STEPS], most;
+  __shared__ int count[STEPS], most, joins, tile_slots;
+  __shared__ unsigned long long sum;
   if (tid < STEPS) count[tid] = 0;
-  if (tid == 0) most = 1;
+  if (tid == 0) most = 1, joins = tile_slots = 0, sum = 0;
   __syncthreads();
-  int c, top = 1;
+  int top = 1;
+  unsigned long long all_chunks = 0;
   for (int i = tid; i < n_units; i += THREADS) {
-    unit_of(i, c);
+    const int c = unit_of(i).c1;
     top = max(top, c);
+    all_chunks += c;
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((tid & 31) == 0) atomicMax(&most, top);
+  atomicMax(&most, top);
+  atomicAdd(&sum, all_chunks);
   __syncthreads();
-  const auto step_of = [&](int chunks) { return int(int64_t(most - chunks) * STEPS / (most + 1)); };
+  // chunks a part; a cut has to be worth its join
+  const int limit = p.tile_target == 0 || n_units >= p.tile_target
+                        ? most
+                        : max(8, int((sum + p.tile_target - 1) / p.tile_target));
+  const auto step_of = [&](int c) { return int(int64_t(most - c) * STEPS / (most + 1)); };
+  const auto longest = [&](int c, int k) { return (c + k - 1) / k; };
   for (int i = tid; i < n_units; i += THREADS) {
-    unit_of(i, c);
-    atomicAdd(&count[step_of(c)], 1);
+    const int c = unit_of(i).c1, k = (c + limit - 1) / limit;
+    atomicAdd(&count[step_of(longest(c, k))], k);
   }
   __syncthreads();
-  const int mine_count = tid < STEPS ? count[tid] : 0;
-  const int before = block_scan(mine_count, c, sums);
+  int n_records;
+  const int before = block_scan(tid < STEPS ? count[tid] : 0, n_records, sums);
   if (tid < STEPS) count[tid] = before;
   __syncthreads();
   for (int i = tid; i < n_units; i += THREADS) {
-    const UnitRec r = unit_of(i, c);
-    p.a.units[atomicAdd(&count[step_of(c)], 1)] = r;
+    UnitRec r = unit_of(i);
+    const int c = r.c1, k = (c + limit - 1) / limit;
+    const int at0 = atomicAdd(&count[step_of(longest(c, k))], k);
+    const int slot0 = k > 1 ? atomicAdd(&tile_slots, k) : -1;
+    for (int part = 0; part < k; ++part) {
+      r.c0 = int(int64_t(c) * part / k);
+      r.c1 = int(int64_t(c) * (part + 1) / k);
+      if (k > 1) r.slot = slot0 + part;
+      if (at0 + part < p.most_units) p.a.units[at0 + part] = r;
+    }
+    if (k > 1) {
+      const int j = atomicAdd(&joins, 1);
+      if (j < p.most_joins) p.a.joins[j] = JoinRec{r.head, r.row0, r.start, r.n * p.a.group, slot0, k, r.b, 0};
+    }
   }
+  __syncthreads();
+  // the launches have room for so many (see shape_of)
+  if (tid == 0)
+    *p.a.plan = PlanHead{n_parts, min(n_records, p.most_units), min(joins, p.most_joins), p.a.group, p.a.window,
+                         p.a.sinks, p.a.row_limit, s.seqs, H, p.a.nt, s.width, s.page_shift};
 }
 
 }  // namespace
@@ -205,6 +229,8 @@ int plan_attend(const AttendParams &a, const PlanShape &shape, cudaStream_t stre
   p.min_chunks = 2;  // a join costs about what ten chunks do
   p.most_parts = int(shape.most_parts);
   p.most_units = int(shape.most_units);
+  p.most_joins = int(shape.most_joins);
+  p.tile_target = shape.tile_target;
   return launch_kernel("emmy_kv8_attend_plan", plan_kernel, dim3(1), THREADS, 0, stream, p);
 }
 

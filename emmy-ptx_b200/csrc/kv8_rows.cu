@@ -60,10 +60,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return r;
 }
 
-// The geometry of one (sequence, head) and of its chunk line.
+// The geometry of one (sequence, head, row block) and of its chunk line.
 struct Segment {
   int b, head, start, n, len;  // n new tokens, rows from `start`; len keys
-  int rows;                    // rows of the kv head, at most 8 NT
+  int row0, rows;              // first row of the kv head, and how many, at most 8 NT
   int part, parts, slot0;      // this CTA's part, of how many; workspace slot of part 0
   Span span;
 };
@@ -78,7 +78,7 @@ struct ChunkInfo {
 template <int D, int NT>
 struct Layout {
   static constexpr int CHUNK = 2 * 64 * D;
-  static constexpr int STAGES = (NT <= 2 ? 64 : 96) * 1024 / CHUNK;
+  static constexpr int STAGES = 64 * 1024 / CHUNK;
   static constexpr int QUERIES = STAGES * CHUNK, END = QUERIES + NT * 16 * D;
   static constexpr int DYN = END + 1024;  // the swizzle repeats every 1 KB
   static constexpr int LD = D + 8;        // floats of a row of the join
@@ -282,11 +282,8 @@ __device__ __forceinline__ int query_row(uint32_t (&f)[D / 8], const T *row, int
 }
 
 // Shared memory: first the joined rows of the four warps, over the staged queries.
-template <int NT>
-constexpr int rows_per_sm_of = rows_per_sm(NT);
-
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(THREADS, rows_per_sm_of<NT>)
+__global__ void __launch_bounds__(THREADS, ROWS_PER_SM)
 rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map) {
   using L = Layout<D, NT>;
   constexpr int ROWS = 8 * NT, LD = L::LD;
@@ -307,7 +304,7 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
   const PartRec rec = p.parts[blockIdx.x];
   grid_dependency_done();
   if (blockIdx.x >= head.parts || !plan_fits(p, head, rec.b, rec.start, rec.n, rec.len)) return;
-  const Segment g = {rec.b, rec.head, rec.start, rec.n, rec.len, rec.n * p.group, rec.part, rec.parts, rec.slot0,
+  const Segment g = {rec.b, rec.head, rec.start, rec.n, rec.len, rec.row0, rec.rows, rec.part, rec.parts, rec.slot0,
                      Span(p, rec.len - rec.n, rec.len - 1)};
   const int c0 = rec.c0, c1 = rec.c1;
   if (tid == 0) {
@@ -318,7 +315,7 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
     stop_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (tid < ROWS) row_pos[tid] = tid < g.rows ? g.len - g.n + tid / p.group : -1;
+  if (tid < ROWS) row_pos[tid] = tid < g.rows ? g.len - g.n + (g.row0 + tid) / p.group : -1;
   __syncthreads();
 
   State<D, NT> st;
@@ -337,7 +334,7 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
       for (int c = 0; c < 4; ++c) st.o[i][t][c] = 0.0f;
   st.unit = 0;
   const auto row_at = [&](int r, int64_t ts, int64_t hs) {
-    const int i = r / p.group, h = g.head * p.group + r - i * p.group;
+    const int i = (g.row0 + r) / p.group, h = g.head * p.group + (g.row0 + r) - i * p.group;
     return (g.start + i) * ts + h * hs;
   };
 
@@ -659,12 +656,7 @@ int launch(const AttendParams &p, const CUtensorMap &map, int device, int grid, 
 
 template <int D, typename T>
 int launch_nt(const AttendParams &p, const CUtensorMap &map, int nt, int device, int grid, cudaStream_t stream) {
-  switch (nt) {
-    case 1: return launch<D, 1, T>(p, map, device, grid, stream);
-    case 2: return launch<D, 2, T>(p, map, device, grid, stream);
-    case 3: return launch<D, 3, T>(p, map, device, grid, stream);
-    default: return launch<D, 4, T>(p, map, device, grid, stream);
-  }
+  return nt == 1 ? launch<D, 1, T>(p, map, device, grid, stream) : launch<D, 2, T>(p, map, device, grid, stream);
 }
 
 }  // namespace

@@ -162,6 +162,7 @@ __device__ __forceinline__ uint32_t swizzled(int r, int j) { return r * 128 + ((
 struct Unit {
   int b, head, start, n, len, rows, row0;
   Span span;
+  int c0, slot;  // first chunk of this part's; workspace slot, -1: the unit is whole
 };
 
 // What goes with a chunk of codes.
@@ -197,10 +198,10 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
   const UnitRec rec = p.units[blockIdx.x];
   grid_dependency_done();
   if (blockIdx.x >= head.units || !plan_fits(p, head, rec.b, rec.start, rec.n, rec.len)) return;
-  Unit u = {rec.b, rec.head, rec.start, rec.n, rec.len, rec.n * p.group, rec.row0, {}};
+  Unit u = {rec.b, rec.head, rec.start, rec.n, rec.len, rec.n * p.group, rec.row0, {}, rec.c0, rec.slot};
   u.span = Span(p, u.len - u.n + u.row0 / p.group, u.len - u.n + (min(u.row0 + 2 * TILE, u.rows) - 1) / p.group);
   const int tiles = u.rows - u.row0 > TILE ? 2 : 1;
-  const int chunks = u.span.chunks;
+  const int chunks = rec.c1 - rec.c0;
 
   // ---- barriers, TMEM ----
   if (tid == 0) {
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         next = ChunkInfo{0, 0, 0, 0};
         next_unit = 0;
         if (g + lane < chunks) {
-          next.key0 = u.span.key0(g + lane);
+          next.key0 = u.span.key0(u.c0 + g + lane);
           int page = row[next.key0 >> s.page_shift];
           next.dead = page < 0 || page >= s.pages;
           if (next.dead) {
@@ -464,7 +465,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
           const int low = max(0, sp.last - p.window + 1);
           whole_lo = sp.sink_chunks + max(0, ((low + CHUNK - 1) >> 6) - sp.window_chunk0);
         }
-        whole_hi = sp.sink_chunks + ((sp.first + 1) >> 6) - sp.window_chunk0;
+        whole_hi = sp.sink_chunks + ((sp.first + 1) >> 6) - sp.window_chunk0 - u.c0;
+        whole_lo -= u.c0;
       }
       for (int g = 0; g < chunks; ++g) {
         const int buf = g & 1;
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         tm_wait_ld();
         const bool dead = sc.x == 0.0f;
         if (dead || g < whole_lo || g >= whole_hi) {
-          const int key0 = u.span.key0(g);
+          const int key0 = u.span.key0(u.c0 + g);
           // bit i: the row sees key key0 + i
           const auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
           uint64_t see = below(pos - key0 + 1);
@@ -569,7 +571,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
       if (ok) ok = warp_wait(&bars.pv_done[x][(chunks - 1) & 1], (chunks - 1) >> 1 & 1, stop, s.status);
       if (ok) {
         tc_after();
-        const float by = l == 0.0f ? 0.0f : pow2(unit) / l;
+        const float by = u.slot >= 0 ? pow2(unit) : l == 0.0f ? 0.0f : pow2(unit) / l;
+        float *const part = p.tile_partial + int64_t(u.slot) * (D + 2) * (2 * TILE) + x * TILE + r;
         const uint32_t *bits = reinterpret_cast<const uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8));
         T *out = static_cast<T *>(p.out) + (int64_t(u.start) + token) * p.o_ts + head * p.o_hs;
 #pragma unroll
@@ -582,7 +585,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (nan >> i & 1) o[i] = 0x7fc00000u;
-          if (real) {
+          if (u.slot >= 0) {
+            // a part: O, and below its maximum and sum, a column of 256 rows each
+#pragma unroll
+            for (int i = 0; i < 32; ++i) __stcg(&part[(c + i) * (2 * TILE)], __uint_as_float(o[i]) * by);
+          } else if (real) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint4 w;
@@ -593,6 +600,10 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
               *reinterpret_cast<uint4 *>(out + c + 8 * i) = w;
             }
           }
+        }
+        if (u.slot >= 0) {
+          __stcg(&part[D * (2 * TILE)], m);
+          __stcg(&part[(D + 1) * (2 * TILE)], l);
         }
         tc_before();
       }
@@ -626,24 +637,61 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
   }
 }
 
+// Parts of a cut unit as one, in their order: a CTA takes 8 values of d of the
+// unit's 256 rows, a thread a row.
 template <int D, typename T>
-int launch(const AttendParams &p, int device, unsigned grid, cudaStream_t stream) {
+__global__ void __launch_bounds__(2 * TILE) join_kernel(const AttendParams p) {
+  grid_dependency_wait();
+  const PlanHead head = *p.plan;
+  const JoinRec j = p.joins[blockIdx.x];
+  grid_dependency_done();
+  if (blockIdx.x >= head.joins || !plan_fits(p, head, j.b, j.start, 0, 0)) return;
+  const int row = j.row0 + threadIdx.x, d0 = blockIdx.y * 8;
+  if (row >= j.rows) return;
+  constexpr int COL = 2 * TILE;
+  const float *base = p.tile_partial + int64_t(j.slot0) * (D + 2) * COL + threadIdx.x;
+  float m = NONE;
+#pragma unroll 8
+  for (int c = 0; c < j.parts; ++c) m = fmaxf(m, __ldcg(base + (int64_t(c) * (D + 2) + D) * COL));
+  float l = 0.0f, x[8] = {};
+#pragma unroll 4
+  for (int c = 0; c < j.parts; ++c) {
+    const float *at = base + int64_t(c) * (D + 2) * COL;
+    const float f = exp2_fast(__ldcg(at + D * COL) - m);
+    l += f * __ldcg(at + (D + 1) * COL);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] += f * __ldcg(at + (d0 + i) * COL);
+  }
+  const float by = l == 0.0f ? 0.0f : 1.0f / l;
+  const int token = row / p.group, h = j.head * p.group + row - token * p.group;
+  uint4 w;
+  w.x = pack2<T>(x[0] * by, x[1] * by);
+  w.y = pack2<T>(x[2] * by, x[3] * by);
+  w.z = pack2<T>(x[4] * by, x[5] * by);
+  w.w = pack2<T>(x[6] * by, x[7] * by);
+  *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + (int64_t(j.start) + token) * p.o_ts + h * p.o_hs + d0) = w;
+}
+
+template <int D, typename T>
+int launch(const AttendParams &p, int device, const PlanShape &shape, cudaStream_t stream) {
   static KernelSetup setup;
-  const int rc = setup.ready("emmy_kv8_attend", tiles_kernel<D, T>, device, Layout<D>::DYN, REGS_LAUNCH);
-  if (rc != EMMY_OK) return rc;
-  return launch_kernel("emmy_kv8_attend", tiles_kernel<D, T>, dim3(grid), THREADS, Layout<D>::DYN, stream, p);
+  int rc = setup.ready("emmy_kv8_attend", tiles_kernel<D, T>, device, Layout<D>::DYN, REGS_LAUNCH);
+  if (rc == EMMY_OK)
+    rc = launch_kernel("emmy_kv8_attend", tiles_kernel<D, T>, dim3(unsigned(shape.most_units)), THREADS,
+                       Layout<D>::DYN, stream, p);
+  if (rc == EMMY_OK && shape.tile_target > 0)
+    rc = launch_kernel("emmy_kv8_attend", join_kernel<D, T>, dim3(unsigned(shape.most_joins), D / 8), 2 * TILE, 0,
+                       stream, p);
+  return rc;
 }
 
 }  // namespace
 
 int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream) {
-  const int64_t grid = shape.most_units;
   const int dev = cache.device;
   if (cache.head_dim == 64)
-    return bf16 ? launch<64, __nv_bfloat16>(p, dev, unsigned(grid), stream)
-                : launch<64, __half>(p, dev, unsigned(grid), stream);
-  return bf16 ? launch<128, __nv_bfloat16>(p, dev, unsigned(grid), stream)
-              : launch<128, __half>(p, dev, unsigned(grid), stream);
+    return bf16 ? launch<64, __nv_bfloat16>(p, dev, shape, stream) : launch<64, __half>(p, dev, shape, stream);
+  return bf16 ? launch<128, __nv_bfloat16>(p, dev, shape, stream) : launch<128, __half>(p, dev, shape, stream);
 }
 
 }  // namespace kv8

@@ -97,6 +97,13 @@ CASES = [
     (1, 3, 128, 64, "bf16", 40, 5, [(333, 200), (20, 20)]),
     (1, 1, 64, 128, "bf16", 64, 64, [(400, 300)]),
     (2, 8, 128, 64, "bf16", 0, 0, [(1000, 70), (130, 130), (600, 1)]),
+    # few rows and many keys: units cut along the keys
+    (1, 4, 128, 64, "bf16", 0, 0, [(3000, 40)]),
+    (1, 8, 64, 128, "f16", 1700, 5, [(5000, 30)]),
+    (2, 2, 64, 64, "bf16", 0, 0, [(2500, 33), (1200, 150), (900, 1), (700, 2)]),
+    # blocks of rows
+    (1, 17, 64, 64, "f16", 0, 0, [(300, 1), (40, 1)]),
+    (2, 6, 128, 64, "f16", 30, 2, [(700, 5), (90, 3), (64, 1)]),
 ]
 
 
