@@ -151,9 +151,9 @@ __device__ __forceinline__ int row_exponent(float amax) {
 }
 
 // Rows of a kv head up to which a sequence is the row kernel's, in blocks of at
-// most ROWS_BLOCK rows that each read the keys again (from L2, as neighbours):
-// two CTAs of 16 rows hide more latency than one of 32 (28 -> 17 us for five
-// drafts of 16 sequences).
+// most ROWS_BLOCK rows that each read the keys again, from L2, as neighbours: 16
+// rows' sums are what registers hold at three CTAs an SM (blocks of 32 at two:
+// 28.4 us against 29.5 for five drafts of 16 sequences, but spills from 25 rows on).
 constexpr int ROWS_MOST = 32, ROWS_BLOCK = 16;
 constexpr int ROWS_PER_SM = 3;  // CTAs of the row kernel, by its launch bounds
 constexpr int TILE_ROWS = 256;  // rows of a unit of the tile kernel

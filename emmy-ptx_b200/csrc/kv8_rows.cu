@@ -22,8 +22,8 @@
 // that HBM's latency asks for cost no registers.  The TMA's swizzle spreads
 // the rows that the lanes of a load read over all banks.
 //
-// Bound by memory: codes are read once per kv head.  A segment -- one sequence
-// and kv head -- is cut into about as many parts of 64-key chunks as its share
+// Bound by memory: codes are read once per kv head.  A segment -- one sequence,
+// kv head and block of rows -- is cut into about as many parts of 64-key chunks as its share
 // of a target number of parts, a CTA a part, so uneven lengths balance and
 // one long sequence fills the GPU, while a segment of about a part's length
 // stays whole and needs no join.  Parts of a cut segment leave (m, l, O) in
@@ -439,8 +439,8 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
       if (!warp_wait(&full[ring.slot], ring.phase, stop, s.status)) break;
       const uint8_t *rows = dyn + ring.slot * L::CHUNK + 16 * warp * D;
       const ChunkInfo info = infos[ring.slot];
-      // S^T = K Q^T: two chains of sums where there is one block of rows
-      constexpr int CHAINS = NT == 1 ? 2 : 1;
+      // S^T = K Q^T, in two chains of sums
+      constexpr int CHAINS = 2;
       float sum[CHAINS][NT][4] = {};
       {
         uint32_t k[2][D / 16];
