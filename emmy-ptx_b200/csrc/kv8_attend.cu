@@ -43,7 +43,8 @@ int shape_of(const char *what, const emmy_kv8 *c, int heads, PlanShape &p) {
   p.tile_target = units > 0 && units < sms ? sms : 0;
   p.most_units = units + p.tile_target;
   p.most_joins = p.tile_target > 0 ? units : 0;
-  if (p.most_units > 0x7fffffff || p.most_parts > 0x7fffffff || segments > (1 << 24))
+  // the plan counts chunks in 32 bits
+  if (p.most_units > 0x7fffffff || segments > (1 << 24) || chunks / c->kv_heads > (1 << 30))
     return fail(EMMY_EINVAL, what, "too many sequences and heads for one call");
   p.partial_bytes = uint64_t(p.slots) * 8 * p.nt * (c->head_dim + 2) * 4;
   p.workspace_bytes = EMMY_KV8_WORKSPACE_ZERO + p.partial_bytes +

@@ -38,6 +38,8 @@ as with every other call here.
 from __future__ import annotations
 
 import ctypes as C
+import threading
+import weakref
 from array import array
 
 import numpy as np
@@ -141,6 +143,46 @@ def _ints(x, name: str) -> np.ndarray:
     return a.astype(np.int64)
 
 
+class _Pool:
+    """Buffers of closed batches on one device, by (use, bytes, the one stream
+    they were used on): the next batch on that stream takes them with no
+    wait.  Kept for the process, up to ``MOST`` bytes."""
+
+    MOST = 512 << 20
+
+    @classmethod
+    def of(cls, dev: Device) -> "_Pool":
+        pool = dev.__dict__.get("_kv_pool")
+        if pool is None:
+            pool = dev._kv_pool = cls(dev)
+        return pool
+
+    def __init__(self, dev: Device):
+        self.dev, self.held, self.bytes, self.lock = dev, {}, 0, threading.Lock()
+
+    def take(self, use: str, nbytes: int, stream: int) -> tuple[int, tuple]:
+        """(address, key to give it back by) of a buffer for work on ``stream``."""
+        key = (use, 1 << max(12, (nbytes - 1).bit_length()), stream)
+        with self.lock:
+            held = self.held.get(key)
+            if held:
+                self.bytes -= key[1]
+                return held.pop(), key
+        ptr = self.dev.alloc(key[1])
+        if use == "workspace":
+            check(self.dev.L.emmy_memset_d32(ptr, 0, WORKSPACE_ZERO // 4, stream), "memset")
+        return ptr, key
+
+    def give(self, ptr: int, key: tuple, reuse: bool) -> None:
+        with self.lock:
+            reuse = reuse and self.bytes + key[1] <= self.MOST
+            if reuse:
+                self.held.setdefault(key, []).append(ptr)
+                self.bytes += key[1]
+        if not reuse:
+            self.dev.free(ptr)          # waits for what still runs on it
+
+
 class KVCache:
     """``layers`` layers of ``pages`` pages of ``page_size`` tokens each, on
     one GPU.  ``storage``: (codes, exps) to adopt instead of allocating --
@@ -164,8 +206,6 @@ class KVCache:
         self.layer_codes = pages * 2 * kv_heads * page_size * head_dim
         self.layer_exps = pages * 2 * kv_heads
         self._own: list[int] = []
-        self._spare: dict[tuple, list[int]] = {}
-        self._closed = False
         self._storage = storage
         if storage is not None:
             codes, exps = storage
@@ -241,30 +281,11 @@ class KVCache:
             if rc:
                 check(rc, "copy_pages")
 
-    def _take(self, use: str, nbytes: int, stream: int) -> tuple[int, tuple]:
-        """(address, key to give it back by) of a buffer for work on ``stream``:
-        one of a closed batch that was used on that stream alone, which needs
-        no wait, or a new one."""
-        key = (use, 1 << max(12, (nbytes - 1).bit_length()), stream)
-        held = self._spare.get(key)
-        if held:
-            return held.pop(), key
-        ptr = self.dev.alloc(key[1])
-        if use == "workspace":
-            check(self.L.emmy_memset_d32(ptr, 0, WORKSPACE_ZERO // 4, stream), "memset")
-        return ptr, key
-
-    def _give(self, ptr: int, key: tuple, reuse: bool) -> None:
-        if reuse and not self._closed and len(self._spare.setdefault(key, [])) < 8:
-            self._spare[key].append(ptr)
-        else:
-            self.dev.free(ptr)          # waits for what still runs on it
-
     def close(self) -> None:
         """Free what this cache allocated (not adopted storage)."""
-        for p in self._own + [p for held in self._spare.values() for p in held]:
+        for p in self._own:
             self.dev.free(p)
-        self._own, self._spare, self._closed = [], {}, True
+        self._own = []
 
     def __del__(self):
         try:
@@ -300,6 +321,7 @@ class Batch:
         self._stale = False
         host = self._packed(table, kv_lens, q_lens)
         self._stream, self._reuse = _stream_of(stream, self.dev), True
+        self._pool = _Pool.of(self.dev)
         self._buf = self._take("batch", host.nbytes)
         _copy_in(self.dev, self._buf, host, self._stream)
         d = self._d = cache._desc()
@@ -315,7 +337,7 @@ class Batch:
         self._append, self._attend = self.L.emmy_kv8_append, self.L.emmy_kv8_attend
 
     def _take(self, use: str, nbytes: int) -> int:
-        held = self.cache._take(use, nbytes, self._stream)
+        held = self._pool.take(use, nbytes, self._stream)
         self._held.append(held)
         return held[0]
 
@@ -481,17 +503,18 @@ class Batch:
         check(self.L.emmy_memcpy_dtoh(word.ctypes.data, self._buf, 4, st), "dtoh")
         check(self.L.emmy_stream_sync(st), "stream sync")
         if word[0]:
+            self._reuse = False         # its counters may not be as they should
             check(self.L.emmy_memset_d32(self._buf, 0, 1, st), "memset")
             raise EmmyError(f"cache kernel reported error 0x{word[0]:x}: "
                             f"{STATUS.get(int(word[0]), 'unknown')}")
 
     def close(self) -> None:
-        """Give the batch's buffers back to its cache: nothing that is not
-        queued on the batch's stream yet may use them after this."""
+        """Give the batch's buffers back for later batches: nothing that is
+        not queued on the batch's stream yet may use them after this."""
         held, self._held = self._held, []
         self._buf, self._ws, self._plans = 0, (0, 0), {}
         for ptr, key in held:
-            self.cache._give(ptr, key, self._reuse)
+            self._pool.give(ptr, key, self._reuse)
 
     def __del__(self):
         try:
@@ -628,7 +651,6 @@ class KVSequences:
         return out
 
     def _track(self, batch: Batch) -> None:
-        import weakref
         self._batches = [r for r in self._batches if r() is not None]
         self._batches.append(weakref.ref(batch))
 

@@ -179,8 +179,22 @@ def test_closed_batches_give_their_buffers_to_the_next_on_their_stream(dev):
     assert not run(2, 2) & first                 # another stream
     mixed = run(1, 2)                            # used on two: freed, which waits
     assert mixed == first and not mixed & dev.live
-    cache.close()
-    assert not dev.live
+    other = small(dev)                           # another cache of the device
+    cache, second = other, run(2, 2)
+    assert run(2, 2) == second
+    storage = {other.codes, other.exps}
+    other.close()
+    assert not storage & dev.live and second <= dev.live
+
+
+def test_spare_buffers_are_bounded(dev, monkeypatch):
+    monkeypatch.setattr(kv._Pool, "MOST", 8192)
+    cache = small(dev)
+    batches = [cache.batch([[1]], [9], stream=1) for _ in range(5)]
+    for b in batches:
+        b.close()
+    assert len(dev._kv_pool.held["batch", 4096, 1]) == 2
+    assert dev._kv_pool.bytes == 8192 and len(dev.live - set(cache._own)) == 2
 
 
 def test_stream_arguments(dev):
