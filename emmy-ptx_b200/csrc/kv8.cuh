@@ -136,20 +136,29 @@ class KernelSetup {
 };
 
 template <typename... A>
-int launch_kernel(const char *what, void (*kernel)(A...), dim3 grid, int threads, int smem, cudaStream_t stream,
-                  const A &...args) {
+int launch_clusters(const char *what, void (*kernel)(A...), int cluster, dim3 grid, int threads, int smem,
+                    cudaStream_t stream, const A &...args) {
   cudaLaunchConfig_t c = {};
   c.gridDim = grid;
   c.blockDim = dim3(threads);
   c.dynamicSmemBytes = smem;
   c.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  c.attrs = &attr;
-  c.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  c.attrs = attr;
+  c.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
   return e == cudaSuccess ? EMMY_OK : cuda_fail(what, e);
+}
+
+template <typename... A>
+int launch_kernel(const char *what, void (*kernel)(A...), dim3 grid, int threads, int smem, cudaStream_t stream,
+                  const A &...args) {
+  return launch_clusters(what, kernel, 1, grid, threads, smem, stream, args...);
 }
 
 // Checks what every call shares and fills the kernels' view of the sequences.

@@ -62,6 +62,35 @@ __device__ __forceinline__ uint32_t elected() {
   return r;
 }
 
+// All threads of the cluster: what each wrote before is visible after.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The same place of this block's shared memory in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_addr(const void *mine, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(mine)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float peer_load(uint32_t at) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 peer_load4(uint32_t at) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "r"(at)
+               : "memory");
+  return x;
+}
+
 // A ring of n slots: slot and phase of step after step.
 struct Ring {
   int slot = 0;

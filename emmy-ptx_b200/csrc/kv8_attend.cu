@@ -37,6 +37,15 @@ int shape_of(const char *what, const emmy_kv8 *c, int heads, PlanShape &p) {
   const int64_t chunks = int64_t(c->table_width) * c->page_size / 64 * segments;
   if (chunks < p.most_parts) p.most_parts = chunks;
   if (!p.rows) p.most_parts = 0;
+  // Short segments as clusters of 8, 4 or 2 CTAs that join in shared memory.  In
+  // cycles, at about 700 a chunk: parts of a cluster and its join take cap / n
+  // chunks and 1500, parts that fill the GPU and their join through L2
+  // segments * cap / wave chunks and 8000.
+  p.cluster = 0;
+  const int64_t cap = int64_t(c->table_width) * c->page_size / 64;
+  for (int n = 8; n >= 2 && p.cluster == 0 && p.rows; n /= 2)
+    if (segments * n <= wave && cap >= n && 7 * cap * (wave - segments * n) < 65 * n * wave) p.cluster = n;
+  if (p.cluster > 0) p.most_parts = segments * p.cluster;
   // Units: at most one part-filled one of a sequence.  Fewer than SMs may be
   // cut, into at most one more part each than their share of the SMs.
   const int64_t units = p.tiles ? (c->tokens * group / TILE_ROWS + c->seqs) * c->kv_heads : 0;
@@ -80,6 +89,7 @@ int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_attend_ar
   p.sinks = a->sinks;
   p.row_limit = shape.rows ? ROWS_MOST : 0;
   p.nt = shape.nt;
+  p.cluster = shape.cluster;
   return EMMY_OK;
 }
 

@@ -11,7 +11,8 @@ namespace kv8 {
 // for those of the tile kernel, and for the tile kernel's units that were cut.
 struct alignas(16) PlanHead {
   int parts, units, joins;
-  int group, window, sinks, row_limit, seqs, kv_heads, nt, width, page_shift;  // what it was made for
+  int group, window, sinks, row_limit, seqs, kv_heads, nt, width, page_shift, cluster;  // what it was made for
+  int pad[3];
 };
 struct alignas(16) PartRec {
   int b, head, c0, c1;  // chunks c0 .. c1 - 1 of the segment's line
@@ -47,6 +48,7 @@ struct AttendParams {
   int window, sinks;
   int row_limit;     // sequences with more rows of a kv head than this are the tile kernel's
   int nt;            // 8-row blocks of the row kernel
+  int cluster;       // CTAs of a cluster of the row kernel, 0: none
 };
 
 // How large a plan gets and what it aims at, from what the host knows.
@@ -55,6 +57,7 @@ struct PlanShape {
   int nt;              // 8-row blocks of the row kernel
   int target;          // parts that the row kernel's segments are to be cut into
   bool spread;         // in two waves rather than one
+  int cluster;         // parts of every segment, a cluster of CTAs; 0: as the target says
   int slots;           // workspace slots for cut segments' parts
   int tile_target;     // parts that the tile kernel's units may be cut into, 0: none is
   int64_t most_parts, most_units, most_joins;
@@ -65,7 +68,7 @@ struct PlanShape {
 // The record is for this call, and what it says is within the arrays.
 __device__ __forceinline__ bool plan_fits(const AttendParams &p, const PlanHead &h, int b, int start, int n, int len) {
   const bool ok = h.group == p.group && h.window == p.window && h.sinks == p.sinks && h.row_limit == p.row_limit &&
-                  h.seqs == p.s.seqs && h.kv_heads == p.s.kv_heads && h.nt == p.nt && h.width == p.s.width &&
+                  h.seqs == p.s.seqs && h.kv_heads == p.s.kv_heads && h.nt == p.nt && h.width == p.s.width && h.cluster == p.cluster &&
                   h.page_shift == p.s.page_shift && start + n <= p.s.tokens &&
                   len <= (int64_t(p.s.width) << p.s.page_shift);
   if (!ok) report(p.s.status, STATUS_PLAN);

@@ -8,7 +8,9 @@
 // about equal length, which the order of arrival evens out.  Measured before
 // the plan was a kernel of its own (us, one wave | two): 2 sequences of 131071
 // keys 37 | 43, 48 with a window of 1024 19 | 28, 16 with five drafts 33 | 41;
-// but 64 of 700-8191 keys, 512 segments on 444 CTAs, 111 | 97.
+// but 64 of 700-8191 keys, 512 segments on 444 CTAs, 111 | 97.  Short segments
+// (by what the table can hold) are cut into as many parts as a cluster has
+// CTAs, which join in shared memory; some parts may be empty.
 // Tile kernel: units of 256 query rows of one (sequence, kv head); where there
 // are fewer than SMs they are cut along the keys, too, and joined by a kernel
 // of their own.  The longest come first (by 256 steps of the longest): the
@@ -50,10 +52,10 @@ __device__ __forceinline__ int block_scan(int x, int &total, int *sums) {
   return at - x;
 }
 
-// Parts of a segment of c chunks, at no more than q chunks a part, or (spread)
-// as near to q as may be.
-__device__ __forceinline__ int parts_of(int c, int q, bool spread) {
-  return c == 0 ? 0 : spread ? max(1, min((2 * c + q) / (2 * q), c)) : (c + q - 1) / q;
+// Parts of a segment of c chunks: a cluster's, or at no more than q chunks a
+// part, or (spread) as near to q as may be.
+__device__ __forceinline__ int parts_of(const PlanParams &p, int c, int q) {
+  return c == 0 ? 0 : p.a.cluster > 0 ? p.a.cluster : p.spread ? max(1, min((2 * c + q) / (2 * q), c)) : (c + q - 1) / q;
 }
 
 // Last i < n with first[i] <= x.
@@ -95,11 +97,11 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   const int64_t work = int64_t(all) * H;
   const int q0 = max(p.min_chunks, int((work + p.target - 1) / p.target));
   int q = q0;
-  if (!p.spread)
+  if (!p.spread && p.a.cluster == 0)
     for (int t = 1; t < 5; ++t) {
       int parts = 0, total;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) parts += parts_of(chunks[i], q, false) * blocks[i];
+      for (int i = 0; i < EACH; ++i) parts += parts_of(p, chunks[i], q) * blocks[i];
       block_scan(parts, total, sums);
       if (int64_t(total) * H <= p.target) break;
       q = q0 + (q0 * (1 << t) + 15) / 16;  // 1/8, 1/4, 1/2, 1 above q0
@@ -107,7 +109,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   int parts = 0, slots = 0, n_parts, n_slots, n_units, units = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    const int k = parts_of(chunks[i], q, p.spread);
+    const int k = parts_of(p, chunks[i], q);
     parts += k * blocks[i] * H;
     slots += k > 1 ? k * blocks[i] * H : 0;
     units += chunks[i] > 0 ? 0 : blocks[i] * H;
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
 #pragma unroll
   for (int i = 0; i < EACH; ++i)
     if (b0 + i < s.seqs) {
-      const int k = parts_of(chunks[i], q, p.spread);
+      const int k = parts_of(p, chunks[i], q);
       part_at[b0 + i] = at;
       slot_at[b0 + i] = slot;
       at += k * blocks[i] * H;
@@ -130,12 +132,18 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
     PartRec r;
     r.b = b;
     lengths(s, b, r.start, r.n, r.len);
-    const int c = Span(p.a, r.len - r.n, r.len - 1).chunks, k = parts_of(c, q, p.spread);
+    const int c = Span(p.a, r.len - r.n, r.len - 1).chunks, k = parts_of(p, c, q);
     const int rows = r.n * p.a.group, nb = (rows + ROWS_BLOCK - 1) / ROWS_BLOCK, each = (rows + nb - 1) / nb;
     // row blocks of a part are neighbours: they share its keys in L2
-    const int block = rel % nb, cut = rel / nb;
+    int block = rel % nb;
+    const int cut = rel / nb;
     r.head = cut / k;
     r.part = cut - r.head * k;
+    if (p.a.cluster > 0) {  // a cluster's CTAs are the neighbours
+      r.part = rel % k;
+      block = rel / k % nb;
+      r.head = rel / k / nb;
+    }
     r.parts = k;
     r.slot0 = slot_at[b] + (r.head * nb + block) * k;
     r.c0 = int(int64_t(c) * r.part / k);
@@ -216,7 +224,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   // the launches have room for so many (see shape_of)
   if (tid == 0)
     *p.a.plan = PlanHead{n_parts, min(n_records, p.most_units), min(joins, p.most_joins), p.a.group, p.a.window,
-                         p.a.sinks, p.a.row_limit, s.seqs, H, p.a.nt, s.width, s.page_shift};
+                         p.a.sinks, p.a.row_limit, s.seqs, H, p.a.nt, s.width, s.page_shift, p.a.cluster, {}};
 }
 
 }  // namespace

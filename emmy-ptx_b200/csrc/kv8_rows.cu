@@ -29,7 +29,9 @@
 // stays whole and needs no join.  Parts of a cut segment leave (m, l, O) in
 // the workspace; the last of each 16 parts to arrive joins them in their
 // order, the last of those their sums, so results do not depend on the order
-// of arrival.
+// of arrival.  The parts of a short segment are a cluster instead: each CTA
+// joins a share of the rows' values out of the others' shared memory, with
+// neither the workspace nor its round trips to L2.
 #include <cuda_bf16.h>
 
 #include <cuda.h>  // CUtensorMap
@@ -44,6 +46,7 @@ constexpr int WARPS = 4, THREADS = 160, ALL_WARPS = 5;  // four that compute, on
 constexpr float LAZY = 8.0f;  // log2 units that scores may pass the reference before O moves
 constexpr int GROUP = 16;     // parts of a segment that one CTA joins at once,
 constexpr int ONE_LEVEL = 24; // or up to this many where that leaves one level
+constexpr int MOST_CLUSTER = 8;
 constexpr int UNIT_LAZY = 6;  // the same for V's exponent: p stays below 2^14 in f16
 constexpr float NONE = -1e30f;
 
@@ -82,7 +85,7 @@ struct Layout {
   static constexpr int QUERIES = STAGES * CHUNK, END = QUERIES + NT * 16 * D;
   static constexpr int DYN = END + 1024;  // the swizzle repeats every 1 KB
   static constexpr int LD = D + 8;        // floats of a row of the join
-  static_assert(WARPS * 8 * NT * LD * 4 <= QUERIES, "the join fits over the ring");
+  static_assert((WARPS * LD + D) * 8 * NT * 4 <= QUERIES, "the join and a cluster's part fit over the ring");
   static_assert(2 * 64 * 8 * NT * 4 <= QUERIES, "so do the maxima and sums of 64 parts");
 };
 
@@ -282,7 +285,7 @@ __device__ __forceinline__ int query_row(uint32_t (&f)[D / 8], const T *row, int
 }
 
 // Shared memory: first the joined rows of the four warps, over the staged queries.
-template <int D, int NT, typename T>
+template <int D, int NT, bool CLUSTER, typename T>
 __global__ void __launch_bounds__(THREADS, ROWS_PER_SM)
 rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map) {
   using L = Layout<D, NT>;
@@ -494,7 +497,7 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
     const unsigned long long t0 = now_ns();
     while (now_ns() - t0 < 50000000ull) {
     }
-    return;
+    if (!CLUSTER) return;  // a cluster's blocks stay until all have read
   }
   if (warp < WARPS) {
 #pragma unroll
@@ -527,7 +530,7 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
     row_l[tid] = l;
   }
   __syncthreads();
-  const bool whole = g.parts == 1;
+  const bool whole = !CLUSTER && g.parts == 1;
   const int rows = g.rows;
   const auto store = [&](int r, int d, const float (&x)[8], float l) {
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
@@ -539,7 +542,8 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
     *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) = w;
   };
   const auto part_slot = [&](int c) { return p.partial + int64_t(g.slot0 + c) * ROWS * (D + 2); };
-  float *const slot = part_slot(g.part);
+  // a cluster's parts stay in shared memory, behind what is joined here
+  float *const slot = CLUSTER ? join + WARPS * ROWS * LD : part_slot(g.part);
   for (int i = tid; i < rows * (D / 8); i += THREADS) {
     const int r = i / (D / 8), d = i % (D / 8) * 8;
     float x[8] = {};
@@ -554,11 +558,40 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
     if (whole) {
       store(r, d, x, row_l[r]);
     } else {
-      __stcg(reinterpret_cast<float4 *>(slot + r * D + d), make_float4(x[0], x[1], x[2], x[3]));
-      __stcg(reinterpret_cast<float4 *>(slot + r * D + d + 4), make_float4(x[4], x[5], x[6], x[7]));
+      *reinterpret_cast<float4 *>(slot + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4 *>(slot + r * D + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
     }
   }
   if (whole) return;
+  if constexpr (CLUSTER) {
+    cluster_sync();
+    for (int i = cluster_rank() * THREADS + tid; i < rows * (D / 4); i += g.parts * THREADS) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float4 u[MOST_CLUSTER];
+      float ms[MOST_CLUSTER], ls[MOST_CLUSTER], m = NONE, l = 0.0f;
+#pragma unroll
+      for (int c = 0; c < MOST_CLUSTER; ++c)
+        if (c < g.parts) {
+          ms[c] = peer_load(peer_addr(&row_m[r], c));
+          ls[c] = peer_load(peer_addr(&row_l[r], c));
+          u[c] = peer_load4(peer_addr(slot + r * D + d, c));
+          m = fmaxf(m, ms[c]);
+        }
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int c = 0; c < MOST_CLUSTER; ++c)
+        if (c < g.parts) {
+          const float f = exp2_fast(ms[c] - m);
+          l += f * ls[c];
+          x.x += f * u[c].x, x.y += f * u[c].y, x.z += f * u[c].z, x.w += f * u[c].w;
+        }
+      const float by = l == 0.0f ? 0.0f : 1.0f / l;
+      *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) =
+          make_uint2(pack2<T>(x.x * by, x.y * by), pack2<T>(x.z * by, x.w * by));
+    }
+    cluster_sync();  // no block ends while another reads it
+    return;
+  }
   if (tid < ROWS) {
     __stcg(slot + ROWS * D + tid, row_m[tid]);
     __stcg(slot + ROWS * D + ROWS + tid, row_l[tid]);
@@ -646,24 +679,28 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
   gather(0, groups, group, true);
 }
 
-template <int D, int NT, typename T>
+template <int D, int NT, bool CLUSTER, typename T>
 int launch(const AttendParams &p, const CUtensorMap &map, int device, int grid, cudaStream_t stream) {
   static KernelSetup setup;
-  const int rc = setup.ready("emmy_kv8_attend", rows_kernel<D, NT, T>, device, Layout<D, NT>::DYN);
+  const int rc = setup.ready("emmy_kv8_attend", rows_kernel<D, NT, CLUSTER, T>, device, Layout<D, NT>::DYN);
   if (rc != EMMY_OK) return rc;
-  return launch_kernel("emmy_kv8_attend", rows_kernel<D, NT, T>, dim3(grid), THREADS, Layout<D, NT>::DYN, stream, p, map);
+  return launch_clusters("emmy_kv8_attend", rows_kernel<D, NT, CLUSTER, T>, CLUSTER ? p.cluster : 1, dim3(grid),
+                         THREADS, Layout<D, NT>::DYN, stream, p, map);
 }
 
 template <int D, typename T>
-int launch_nt(const AttendParams &p, const CUtensorMap &map, int nt, int device, int grid, cudaStream_t stream) {
-  return nt == 1 ? launch<D, 1, T>(p, map, device, grid, stream) : launch<D, 2, T>(p, map, device, grid, stream);
+int launch_nt(const AttendParams &p, const CUtensorMap &map, int device, int grid, cudaStream_t stream) {
+  if (p.cluster > 0)
+    return p.nt == 1 ? launch<D, 1, true, T>(p, map, device, grid, stream)
+                     : launch<D, 2, true, T>(p, map, device, grid, stream);
+  return p.nt == 1 ? launch<D, 1, false, T>(p, map, device, grid, stream)
+                   : launch<D, 2, false, T>(p, map, device, grid, stream);
 }
 
 }  // namespace
 
 int rows_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream) {
   const int64_t grid = shape.most_parts;
-  const int nt = shape.nt;
   // the pool as rows of head_dim bytes, 64 of them a box
   const int64_t rows = int64_t(cache.pages) * 2 * cache.kv_heads * cache.page_size;
   emmy_tmap_desc d = {};
@@ -680,10 +717,10 @@ int rows_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &s
   const int rc = emmy_tmap_encode(&d, &map);
   if (rc != EMMY_OK) return rc;
   if (cache.head_dim == 64)
-    return bf16 ? launch_nt<64, __nv_bfloat16>(p, map, nt, cache.device, int(grid), stream)
-                : launch_nt<64, __half>(p, map, nt, cache.device, int(grid), stream);
-  return bf16 ? launch_nt<128, __nv_bfloat16>(p, map, nt, cache.device, int(grid), stream)
-              : launch_nt<128, __half>(p, map, nt, cache.device, int(grid), stream);
+    return bf16 ? launch_nt<64, __nv_bfloat16>(p, map, cache.device, int(grid), stream)
+                : launch_nt<64, __half>(p, map, cache.device, int(grid), stream);
+  return bf16 ? launch_nt<128, __nv_bfloat16>(p, map, cache.device, int(grid), stream)
+              : launch_nt<128, __half>(p, map, cache.device, int(grid), stream);
 }
 
 }  // namespace kv8
