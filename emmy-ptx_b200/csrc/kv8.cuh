@@ -27,7 +27,7 @@ constexpr int E_MIN = -32, E_MAX = 63;
 // What a kernel leaves in the status word (0: nothing was wrong).
 constexpr unsigned STATUS_PAGE = 0x401;    // a page number outside the pool
 constexpr unsigned STATUS_LENGTH = 0x402;  // a sequence longer than its row of the table, or
-                                           // more new tokens than keys or than rows given
+                                           // more new tokens than keys, than rows given or than max_q
 constexpr unsigned STATUS_WAIT = 0x403;    // a bounded wait inside a kernel ran out
 constexpr unsigned STATUS_PLAN = 0x404;    // a plan that was made for another call
 
@@ -36,7 +36,7 @@ struct Seqs {
   const int *kv_lens;   // [seqs] keys, the new tokens included
   const int *q_starts;  // [seqs + 1] first row of each sequence's new tokens
   unsigned *status;     // may be null
-  int seqs, width, pages, tokens, kv_heads, page_shift;
+  int seqs, width, pages, tokens, max_q, kv_heads, page_shift;
 };
 
 __device__ __forceinline__ void report(unsigned *status, unsigned code) {
@@ -45,7 +45,7 @@ __device__ __forceinline__ void report(unsigned *status, unsigned code) {
 
 // n, or 0 (nothing to do), reported, where the lengths cannot be right.
 __device__ __forceinline__ int checked_n(const Seqs &s, int start, int n, int len) {
-  if (n >= 0 && n <= len && start >= 0 && start + n <= s.tokens && len <= (int64_t(s.width) << s.page_shift)) return n;
+  if (n >= 0 && n <= len && n <= s.max_q && start >= 0 && start + n <= s.tokens && len <= (int64_t(s.width) << s.page_shift)) return n;
   report(s.status, STATUS_LENGTH);
   return 0;
 }

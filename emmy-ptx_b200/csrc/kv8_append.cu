@@ -246,10 +246,6 @@ __global__ void __launch_bounds__(128) append_one_kernel(const AppendParams p) {
   int start, n, len;
   lengths(s, b, start, n, len);
   if (n == 0) return;
-  if (n > 1) {  // more than the call's max_q
-    report(s.status, STATUS_LENGTH);
-    return;
-  }
   const int page = s.table[int64_t(b) * s.width + ((len - 1) >> s.page_shift)];
   const int side = unit_of_seq >= s.kv_heads, head = unit_of_seq - side * s.kv_heads;
   V v;

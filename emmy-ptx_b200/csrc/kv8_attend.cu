@@ -85,8 +85,9 @@ int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_attend_ar
   p.units = reinterpret_cast<UnitRec *>(p.parts + shape.most_parts);
   p.joins = reinterpret_cast<JoinRec *>(p.units + shape.most_units);
   p.group = a->heads / cache->kv_heads;
-  p.window = a->window;
-  p.sinks = a->sinks;
+  // a sequence holds at most 2^30 keys; sums with more would overflow
+  p.window = a->window < 1 << 30 ? a->window : 1 << 30;
+  p.sinks = a->sinks < 1 << 30 ? a->sinks : 1 << 30;
   p.row_limit = shape.rows ? ROWS_MOST : 0;
   p.nt = shape.nt;
   p.cluster = shape.cluster;
@@ -140,6 +141,11 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
     return fail(EMMY_EINVAL, what, "q and out: base and strides must be multiples of 16 bytes");
   if (a->q_strides[0] < 0 || a->q_strides[1] < 0 || a->out_strides[0] < 0 || a->out_strides[1] < 0)
     return fail(EMMY_EINVAL, what, "q and out: strides must not be negative");
+  // rows of out one after another, tokens within heads or heads within tokens
+  const int64_t ts = a->out_strides[0], hs = a->out_strides[1], D = cache->head_dim;
+  const int64_t T = cache->tokens, Hq = a->heads;
+  if ((T > 1 && ts < D) || (Hq > 1 && hs < D) || (T > 1 && Hq > 1 && (ts <= hs ? hs < ts * (T - 1) + D : ts < hs * (Hq - 1) + D)))
+    return fail(EMMY_EINVAL, what, "rows of out overlap");
   const auto extent = [&](const int64_t st[2]) {
     return uint64_t((cache->tokens - 1) * st[0] + (a->heads - 1) * st[1] + cache->head_dim) * 2;
   };

@@ -43,6 +43,7 @@ Seqs seqs_of(const emmy_kv8 &c) {
   s.width = c.table_width;
   s.pages = c.pages;
   s.tokens = c.tokens;
+  s.max_q = c.max_q;
   s.kv_heads = c.kv_heads;
   s.page_shift = c.page_size == 64 ? 6 : c.page_size == 128 ? 7 : 8;
   return s;
@@ -72,3 +73,12 @@ int sm_count(int device) {
 }
 
 }  // namespace kv8
+
+extern "C" int emmy_stream_capturing(emmy_stream stream, int *capturing) {
+  if (capturing == nullptr) return kv8::fail(EMMY_EINVAL, "emmy_stream_capturing", "null result");
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &st);
+  if (e != cudaSuccess) return kv8::cuda_fail("emmy_stream_capturing", e);
+  *capturing = st != cudaStreamCaptureStatusNone;
+  return EMMY_OK;
+}

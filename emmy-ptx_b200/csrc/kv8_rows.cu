@@ -48,7 +48,6 @@ constexpr int GROUP = 16;     // parts of a segment that one CTA joins at once,
 constexpr int ONE_LEVEL = 24; // or up to this many where that leaves one level
 constexpr int MOST_CLUSTER = 8;
 constexpr int UNIT_LAZY = 6;  // the same for V's exponent: p stays below 2^14 in f16
-constexpr float NONE = -1e30f;
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -134,6 +133,7 @@ struct State {
   float o[D / 16][NT][4];
   float m[NT][2], l[NT][2];
   int unit;           // O is in units of 2^unit
+  bool big;           // some row's maximum is
 };
 
 // Scores in log2 units -> weights, b = P^T as B fragments; moves the maxima
@@ -145,13 +145,12 @@ __device__ __forceinline__ void softmax_step(State<D, NT> &st, float (&s)[NT][4]
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int c = 0; c < 4; ++c) grow |= s[i][c] > st.m[i][c & 1] + LAZY;
-  const bool move = ev - st.unit > UNIT_LAZY || st.unit - ev > UNIT_LAZY;
+  const bool move = ev - st.unit > UNIT_LAZY || st.unit - ev > UNIT_LAZY || (st.big && ev != st.unit);
   if (__any_sync(0xffffffffu, grow) || move) {
-    const float unit = move ? pow2(st.unit - ev) : 1.0f;
-    if (move) st.unit = ev;
+    bool big = false;
+    float f[NT][2];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      float f[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float top = fmaxf(s[i][c], s[i][c + 2]);
@@ -159,17 +158,25 @@ __device__ __forceinline__ void softmax_step(State<D, NT> &st, float (&s)[NT][4]
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
         top = fmaxf(top, st.m[i][c]);
-        f[c] = exp2_fast(st.m[i][c] - top);
+        f[i][c] = exp2_fast(st.m[i][c] - top);
         st.m[i][c] = top;
-        st.l[i][c] *= f[c];
-        f[c] *= unit;
-      }
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        st.o[j][i][0] *= f[0], st.o[j][i][2] *= f[0];
-        st.o[j][i][1] *= f[1], st.o[j][i][3] *= f[1];
+        st.l[i][c] *= f[i][c];
+        big |= is_big(top);
       }
     }
+    st.big = __any_sync(0xffffffffu, big);
+    float unit = 1.0f;
+    if (move || st.big) {
+      unit = pow2(st.unit - ev);
+      st.unit = ev;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        st.o[j][i][0] *= f[i][0] * unit, st.o[j][i][2] *= f[i][0] * unit;
+        st.o[j][i][1] *= f[i][1] * unit, st.o[j][i][3] *= f[i][1] * unit;
+      }
   }
   // p = 2^(s - m) in units of 2^(unit - ev); P^T by 8 x 8 transposes
   const float dev = float(ev - st.unit), undo = pow2(st.unit - ev);
@@ -336,6 +343,7 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
 #pragma unroll
       for (int c = 0; c < 4; ++c) st.o[i][t][c] = 0.0f;
   st.unit = 0;
+  st.big = false;
   const auto row_at = [&](int r, int64_t ts, int64_t hs) {
     const int i = (g.row0 + r) / p.group, h = g.head * p.group + (g.row0 + r) - i * p.group;
     return (g.start + i) * ts + h * hs;

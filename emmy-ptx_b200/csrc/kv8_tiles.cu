@@ -37,7 +37,12 @@ constexpr int W_PV = 0, W_QK = 2, W_SOFTMAX = 4, W_LOAD = 12;  // warps
 // block was launched with: a split above it would wait for ever.
 constexpr int REGS_LAUNCH = 128, REGS_ISSUE = 64, REGS_SOFTMAX = 176, REGS_LOAD = 96;
 static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX + REGS_LOAD == 4 * REGS_LAUNCH, "register split");
-constexpr float LAZY = 8.0f, NONE = -1e30f, LEAST = 1e-37f;
+constexpr float LAZY = 8.0f, LEAST = 1e-37f;
+// Weights are 2^(s rm - m) with one rounding of the difference, m = round(max s
+// rm): the two differ by up to 2^-25 |m|, a factor common to the row, which
+// stays in range up to this |m|.  Beyond it f32 scores are whole multiples of
+// 16 and more, and the factor rm is made a power of two, so that m is exact.
+constexpr float HUGE_SCORE = 134217728.0f;
 constexpr int UNIT_LAZY = 6;
 
 template <int D>
@@ -118,6 +123,8 @@ template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Exponent of a normal f32 above 0, least -126.
+__device__ __forceinline__ int ilogb_f32(float x) { return max(int(__float_as_uint(x) >> 23) - 127, -126); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -455,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
       const uint32_t s_at = tmem + lanes + 2 * x * CHUNK, o_at = tmem + lanes + L::O_COL + x * D;
       float m = NONE, l = 0.0f;
       int unit = 0;
-      bool ok = true, nan_seen = false;
+      bool ok = true, nan_seen = false, big = false;
       // chunks whole_lo .. whole_hi - 1 every row sees whole
       int whole_lo = 0, whole_hi = chunks;
       {
@@ -475,7 +482,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         if (g == 0 && x == 1) stagger();
         const float2 sc = chunk_scale[g & 3];
         const int ev = int(sc.y);
-        const float rm = fmaxf(mult * sc.x, LEAST);
+        float rm = fmaxf(mult * sc.x, LEAST);
         tc_after();
         uint32_t sv[2][32];
         tm_ld32(sv[0], s_at + buf * CHUNK);
@@ -515,18 +522,25 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         for (int i = 0; i < 4; ++i) top[i] = score(i);
 #pragma unroll
         for (int i = 4; i < 64; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], score(i), score(i + 1));
-        const float best = fmaxf(max3(top[0], top[1], top[2]), top[3]) * rm;
+        const float raw = fmaxf(max3(top[0], top[1], top[2]), top[3]), best = raw * rm;
         const int stray = ev - unit;
-        const bool first = g == 0, move = stray > UNIT_LAZY || stray < -UNIT_LAZY;
-        const bool fix = __any_sync(0xffffffffu, best > m + LAZY) || move;
+        const bool first = g == 0, move = stray > UNIT_LAZY || stray < -UNIT_LAZY || big;
+        const bool fix = __any_sync(0xffffffffu, best > m + LAZY || move);
         float alpha = 1.0f;
         if (fix) {
-          const float to = fmaxf(m, best);
+          float to = fmaxf(m, best);
+          if (fabsf(to) > HUGE_SCORE && m != to) {
+            // (rare) a power of two from here on: products are exact
+            mult = pow2(ilogb_f32(mult));
+            rm = fmaxf(mult * sc.x, LEAST);
+            to = fmaxf(m, raw * rm);
+          }
           alpha = exp2_fast(m - to);
           m = to;
           l *= alpha;
+          big |= is_big(m);
           if (first) unit = ev;
-          if (move) {
+          if (move || big) {
             alpha *= pow2(unit - ev);
             unit = ev;
           }

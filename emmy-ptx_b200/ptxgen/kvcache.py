@@ -32,7 +32,8 @@ queued on ``stream`` (an address, or an object with ``cuda_stream``; default
 the device's stream, ``Device.stream``; 0 is the legacy default stream),
 return at once and allocate nothing after the first ``attend`` of a batch;
 the caller keeps the arrays alive until the work is done and orders streams,
-as with every other call here.
+as with every other call here (a batch used on a stream other than the one it
+was made on waits for that once).
 """
 
 from __future__ import annotations
@@ -273,6 +274,8 @@ class KVCache:
             raise EmmyError("copy_pages: a page is in dst twice")
         if not targets.isdisjoint(src):
             raise EmmyError("copy_pages: a page is in both src and dst")
+        if not self.codes:
+            raise EmmyError("the cache is closed")
         st = _stream_of(stream, self.dev)
         at, to = src.buffer_info()[0], dst.buffer_info()[0]
         for i in range(0, n, MAX_PAIRS):
@@ -283,9 +286,10 @@ class KVCache:
 
     def close(self) -> None:
         """Free what this cache allocated (not adopted storage)."""
-        for p in self._own:
+        own, self._own = self._own, []
+        self.codes = self.exps = 0
+        for p in own:
             self.dev.free(p)
-        self._own = []
 
     def __del__(self):
         try:
@@ -322,7 +326,8 @@ class Batch:
         host = self._packed(table, kv_lens, q_lens)
         self._stream, self._reuse = _stream_of(stream, self.dev), True
         self._pool = _Pool.of(self.dev)
-        self._buf = self._take("batch", host.nbytes)
+        self._others: set[int] = set()             # further streams it was used on
+        self._buf = self._take("batch", host.nbytes, self._stream)
         _copy_in(self.dev, self._buf, host, self._stream)
         d = self._d = cache._desc()
         d.status = self._buf
@@ -336,15 +341,29 @@ class Batch:
         self._ks, self._vs = _Strides(), _Strides()
         self._append, self._attend = self.L.emmy_kv8_append, self.L.emmy_kv8_attend
 
-    def _take(self, use: str, nbytes: int) -> int:
-        held = self._pool.take(use, nbytes, self._stream)
+    def _take(self, use: str, nbytes: int, st: int) -> int:
+        held = self._pool.take(use, nbytes, st)
         self._held.append(held)
         return held[0]
 
     def _on(self, stream) -> int:
+        """The handle of ``stream``; one other than the batch's own waits, the
+        first time, for what is queued on that (its lengths, a page copy).
+        One that is being captured cannot wait: its graph is replayed after."""
         st = _stream_of(stream, self.dev)
-        if st != self._stream:
+        if st != self._stream and st not in self._others:
             self._reuse = False
+            capturing = C.c_int()
+            check(self.L.emmy_stream_capturing(st, C.byref(capturing)), "stream")
+            if capturing.value:
+                return st
+            ev = self.dev.event()
+            try:
+                check(self.L.emmy_event_record(ev, self._stream), "event record")
+                check(self.L.emmy_stream_wait_event(st, ev), "stream wait event")
+            finally:
+                self.L.emmy_event_destroy(ev)
+            self._others.add(st)
         return st
 
     def _packed(self, table, kv_lens, q_lens) -> np.ndarray:
@@ -403,8 +422,11 @@ class Batch:
             raise EmmyError("the batch names pages that compact() moved: update it or make a new one")
         if not 0 <= layer < self.cache.layers:
             raise EmmyError(f"layer {layer} is outside 0..{self.cache.layers - 1}")
+        c = self.cache
+        if not c.codes:
+            raise EmmyError("the cache is closed")
         if layer != self._layer:
-            d, c = self._d, self.cache
+            d = self._d
             d.codes = c.codes + layer * c.layer_codes
             d.exps = c.exps + layer * c.layer_exps
             self._layer = layer
@@ -448,13 +470,18 @@ class Batch:
         key = (heads, window, sinks)
         if key in self._plans:
             return
+        if not 0 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31:
+            raise EmmyError("attend: window and sinks are between 0 and 2^31 - 1")
+        if not 1 <= heads <= 2 ** 20:
+            raise EmmyError(f"attend: {heads} query heads")
+        st = self._on(stream)
         ws, plan = C.c_uint64(), C.c_uint64()
         check(self.L.emmy_kv8_attend_sizes(self._ref, heads, C.byref(ws), C.byref(plan)), "attend")
         if ws.value > self._ws[1]:
-            self._ws = self._take("workspace", ws.value), ws.value
-        self._plans[key] = self._take("plan", plan.value), plan.value
+            self._ws = self._take("workspace", ws.value, st), ws.value
+        self._plans[key] = self._take("plan", plan.value, st), plan.value
         try:
-            self._plan(key, self._on(stream))
+            self._plan(key, st)
         except EmmyError:
             del self._plans[key]
             raise

@@ -151,6 +151,9 @@ int emmy_event_elapsed(emmy_event start, emmy_event end, float *ms);
  * next kernels; no counterpart in the single-stream reference runner). */
 int emmy_stream_wait_event(emmy_stream stream, emmy_event ev);
 
+/* Whether `stream` is being captured into a graph (no counterpart either). */
+int emmy_stream_capturing(emmy_stream stream, int *capturing);
+
 /* ---- kernel error word ---- */
 /* Kernels that can fail (bounded waits that expire, index checks in the
  * checked build) write a nonzero code into the module global `emmy_err`

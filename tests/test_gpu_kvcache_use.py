@@ -81,6 +81,23 @@ def test_two_captured_graphs_at_once_and_replay_after_update():
     batch.check_errors(stream=st)
 
 
+def test_capture_on_a_stream_the_batch_never_saw():
+    """Made and warmed up on the default stream, captured on another."""
+    rng = np.random.default_rng(18)
+    kv, ql = [3000, 500], [2, 1]
+    cache, codes, exps, table, q = make(rng, kv, ql)
+    batch, out = cache.batch(table, kv, ql, stream=0), torch.zeros_like(q)
+    batch.attend(0, q, out, stream=0)
+    torch.cuda.synchronize()
+    out.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch.attend(0, q, out, stream=torch.cuda.current_stream())
+    graph.replay()
+    torch.cuda.synchronize()
+    assert right(out, codes, exps, table, kv, ql, q)
+
+
 def test_captured_step_appends_then_attends():
     """append and attend of one token in a graph, replayed as the sequence
     grows over a page's end."""
@@ -272,3 +289,85 @@ def test_results_do_not_depend_on_the_cut():
         both.append(out[:1])
     for out in both:
         assert right(out, codes, exps, table[:1], kv[:1], [1], q[:1])
+
+
+def test_more_new_tokens_than_max_q_are_reported():
+    """Lengths that grew on the device past what the call was made for: the
+    sequence is skipped, by either kernel and by append."""
+    from ptxgen.runtime import EmmyError
+    rng = np.random.default_rng(13)
+    for n in (1, 50):
+        cache, codes, exps, table, q = make(rng, [200, 70], [n, 1])
+        batch = cache.batch(table, [200, 70], [n, 1], stream=0)
+        q = torch.cat([q, q])
+        out = torch.full_like(q, 3.0)
+        batch._d.tokens += 1                                 # q and out have more rows
+        starts = np.array([0, n + 1, n + 2], np.int32)
+        torch.cuda.synchronize()
+        from ptxgen.kvcache import _copy_in
+        _copy_in(cache.dev, batch._d.q_starts, starts, 0)
+        batch.attend(0, q, out, stream=0)
+        with pytest.raises(EmmyError, match="0x402"):
+            batch.check_errors(stream=0)
+        assert (out[:n + 1] == 3.0).all() and (out[n + 1] != 3.0).any() and (out[n + 2:] == 3.0).all()
+        before = cache._storage[0].clone()
+        k = torch.ones((2 * n + 2, 2, 128), device="cuda")
+        batch.append(0, k, k, stream=0)
+        with pytest.raises(EmmyError, match="0x402"):
+            batch.check_errors(stream=0)
+        changed = (before != cache._storage[0]).flatten(2).any(2)[0].nonzero().flatten().tolist()
+        assert set(changed) <= {int(table[1, 1])}
+
+
+def test_out_whose_rows_overlap_is_refused():
+    from ptxgen.runtime import EmmyError
+    rng = np.random.default_rng(14)
+    cache, codes, exps, table, q = make(rng, [70, 5, 9], [1, 1, 1])
+    batch = cache.batch(table, [70, 5, 9], stream=0)
+    one = torch.zeros((1, 8, 128), dtype=torch.float16, device="cuda")
+    flat = torch.zeros(4096, dtype=torch.float16, device="cuda")
+    for bad in (one.expand(3, 8, 128), flat.as_strided((3, 8, 128), (128, 128, 1)),
+                flat.as_strided((3, 8, 128), (1024, 64, 1))):
+        with pytest.raises(EmmyError, match="rows of out overlap"):
+            batch.attend(0, q, bad, stream=0)
+    heads_first = torch.zeros((8, 3, 128), dtype=torch.float16, device="cuda").transpose(0, 1)
+    batch.attend(0, q, heads_first, stream=0)
+    assert right(heads_first, codes, exps, table, [70, 5, 9], [1, 1, 1], q)
+    with pytest.raises(EmmyError, match="q and out overlap"):
+        batch.attend(0, q, q, stream=0)
+
+
+def test_a_batch_used_on_another_stream_than_its_own():
+    """No order given by the caller: the batch's lengths are there all the same."""
+    rng = np.random.default_rng(15)
+    cache, codes, exps, table, q = make(rng, [3000, 70], [1, 1])
+    torch.cuda.synchronize()
+    for _ in range(10):
+        out = torch.zeros_like(q)
+        batch = cache.batch(table, [3000, 70])               # the framework's stream
+        batch.attend(0, q, out, stream=0)
+        torch.cuda.synchronize()
+        assert right(out, codes, exps, table, [3000, 70], [1, 1], q)
+
+
+def test_q_of_extreme_rows():
+    """Rows near the ends of bf16's range, zero rows, and rows with NaN."""
+    rng = np.random.default_rng(16)
+    kv, ql = [200, 65], [1, 40]
+    cache, codes, exps, table, _ = make(rng, kv, ql, H=1, G=4, D=64, spread=0.0)
+    q = rng.standard_normal((41, 4, 64))
+    q[:, 0] *= 1e36
+    q[:, 1] *= 1e-38
+    q[:, 2] = 0
+    q = torch.from_numpy(q).to(torch.bfloat16).cuda()
+    q[:, 3, 5] = float("nan")
+    out = torch.empty_like(q)
+    cache.batch(table, kv, ql, stream=0).attend(0, q, out, scale=1e-3, stream=0)
+    want, bound = ref.attend(codes, exps, table, kv, ql, q.float().cpu().numpy().astype(float), 1e-3)
+    got = out.float().cpu().numpy()
+    assert np.isnan(got[:, 3]).all()
+    # scores of 1e34, whose own rounding decides which key takes all
+    most = max(np.abs(x).max() for b in (0, 1) for x in ref.held(codes, exps, table, b, kv[b], 0)[1:])
+    assert np.isfinite(got[:, 0]).all() and (np.abs(got[:, 0]) <= most * (1 + 2.0 ** -8)).all()
+    assert (np.abs(got[:, 0]).max(1) > 0).all()
+    assert ref.close(got[:, 1:3], want[:, 1:3], bound[:, 1:3], "bf16")

@@ -45,6 +45,9 @@ class FakeDevice:
     def memset32(self, *a):
         pass
 
+    def event(self):
+        return 99
+
     def sync(self, *a):
         pass
 
@@ -127,6 +130,9 @@ def test_call_refusals(dev):
         (lambda: b.append(0, k, DeviceArray(1, "bf16", (3, 2, 64))), "both"),
         (lambda: b.append(0, DeviceArray(1, "f32", (3, 4, 64)), k), "k has shape"),
         (lambda: b.append(0, DeviceArray(1, "u8", (3, 2, 64)), DeviceArray(1, "u8", (3, 2, 64))), "both"),
+        (lambda: b.attend(0, q, out, window=2 ** 32 + 5), "window"),
+        (lambda: b.attend(0, q, out, window=-1), "window"),
+        (lambda: b.attend(0, q, out, window=1, sinks=2 ** 31), "sinks"),
         (lambda: b.update([[1], [2]], [5, 6], [2, 2]), "made for"),
         (lambda: b.update([[1, 2], [2, 3]], [5, 6], [1, 2]), "table"),
     ]
@@ -140,6 +146,22 @@ def test_call_refusals(dev):
     b.close()
     with pytest.raises(EmmyError, match="closed"):
         b.attend(0, q, out)
+    cache.close()
+    for call in (lambda: clash.attend(0, q, out), lambda: cache.copy_pages([1], [2])):
+        with pytest.raises(EmmyError, match="cache is closed"):
+            call()
+
+
+def test_another_stream_waits_for_the_batch_once(dev):
+    b = small(dev).batch([[1]], [9], stream=5)
+    q, out = DeviceArray(1 << 20, "bf16", (1, 4, 64)), DeviceArray(1 << 21, "bf16", (1, 4, 64))
+    dev.L.calls.clear()
+    for st in (5, 6, 6, 0, 6):
+        b.attend(0, q, out, stream=st)
+    waits = [a[0] for name, a in dev.L.calls if name == "emmy_stream_wait_event"]
+    assert waits == [6, 0]
+    zeroed = [a[3] for name, a in dev.L.calls if name == "emmy_memset_d32"]
+    assert zeroed == [5]                         # the workspace, on the stream that needed it
 
 
 def test_one_plan_for_each_heads_window_and_sinks(dev):
@@ -177,8 +199,7 @@ def test_closed_batches_give_their_buffers_to_the_next_on_their_stream(dev):
     first = run(1, 1)
     assert run(1, 1) == first                    # no wait is needed
     assert not run(2, 2) & first                 # another stream
-    mixed = run(1, 2)                            # used on two: freed, which waits
-    assert mixed == first and not mixed & dev.live
+    assert not run(1, 2) & dev.live              # used on two: freed, which waits
     other = small(dev)                           # another cache of the device
     cache, second = other, run(2, 2)
     assert run(2, 2) == second
