@@ -20,8 +20,9 @@
 namespace kv8 {
 
 // Exponents of a page.  448 * 2^63 = 4e21 is the largest magnitude held.  The
-// span of 95 keeps an accumulator of 2^20 terms of 448 finite in f32 when it
-// moves from the units of one page to those of any other.
+// span of 95 keeps an accumulator of 2^16 terms of 448 with weights of 2^8 (the
+// most the running maximum lags) finite in f32 when it moves from the units of
+// the largest pages to those of the smallest.
 constexpr int E_MIN = -32, E_MAX = 63;
 
 // What a kernel leaves in the status word (0: nothing was wrong).

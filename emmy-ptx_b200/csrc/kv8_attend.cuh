@@ -57,7 +57,8 @@ struct PlanShape {
   int nt;              // 8-row blocks of the row kernel
   int target;          // parts that the row kernel's segments are to be cut into
   bool spread;         // in two waves rather than one
-  int cluster;         // parts of every segment, a cluster of CTAs; 0: as the target says
+  int cluster;         // CTAs of a cluster, which joins its parts in shared memory; 0: no clusters
+  bool single;         // and every segment is one cluster
   int slots;           // workspace slots for cut segments' parts
   int tile_target;     // parts that the tile kernel's units may be cut into, 0: none is
   int64_t most_parts, most_units, most_joins;

@@ -9,8 +9,9 @@
 // the plan was a kernel of its own (us, one wave | two): 2 sequences of 131071
 // keys 37 | 43, 48 with a window of 1024 19 | 28, 16 with five drafts 33 | 41;
 // but 64 of 700-8191 keys, 512 segments on 444 CTAs, 111 | 97.  Short segments
-// (by what the table can hold) are cut into as many parts as a cluster has
-// CTAs, which join in shared memory; some parts may be empty.
+// (by what the table can hold) are a cluster each, whose CTAs join in shared
+// memory, and a few long ones some clusters each: fewer partial results go
+// through the workspace.  Some of a cluster's parts may be empty.
 // Tile kernel: units of 256 query rows of one (sequence, kv head); where there
 // are fewer than SMs they are cut along the keys, too, and joined by a kernel
 // of their own.  The longest come first (by 256 steps of the longest): the
@@ -29,7 +30,7 @@ constexpr int THREADS = 1024, WARPS = 32, EACH = EMMY_KV8_MAX_SEQS / THREADS;
 struct PlanParams {
   AttendParams a;
   int target, min_chunks, most_parts, most_units, most_joins, tile_target;
-  bool spread;
+  bool spread, single;
 };
 
 __device__ __forceinline__ int warp_scan(int x, int lane) {  // inclusive
@@ -52,10 +53,17 @@ __device__ __forceinline__ int block_scan(int x, int &total, int *sums) {
   return at - x;
 }
 
-// Parts of a segment of c chunks: a cluster's, or at no more than q chunks a
-// part, or (spread) as near to q as may be.
+// Parts of a segment of c chunks, at no more than q chunks a part: whole
+// clusters, or (spread) as near to q as may be.
 __device__ __forceinline__ int parts_of(const PlanParams &p, int c, int q) {
-  return c == 0 ? 0 : p.a.cluster > 0 ? p.a.cluster : p.spread ? max(1, min((2 * c + q) / (2 * q), c)) : (c + q - 1) / q;
+  const int n = p.a.cluster;
+  return c == 0 ? 0 : p.single ? n : n > 0 ? n * ((c + n * q - 1) / (n * q)) : p.spread ? max(1, min((2 * c + q) / (2 * q), c)) : (c + q - 1) / q;
+}
+
+// Workspace slots of a segment of k parts: one a part, or one a cluster.
+__device__ __forceinline__ int slots_of(const PlanParams &p, int k) {
+  const int n = p.a.cluster > 0 ? k / p.a.cluster : k;
+  return n > 1 ? n : 0;
 }
 
 // Last i < n with first[i] <= x.
@@ -97,21 +105,21 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   const int64_t work = int64_t(all) * H;
   const int q0 = max(p.min_chunks, int((work + p.target - 1) / p.target));
   int q = q0;
-  if (!p.spread && p.a.cluster == 0)
-    for (int t = 1; t < 5; ++t) {
+  if (!p.spread && !p.single)
+    for (int t = 1; t <= 16; t += t < 4 ? 1 : t < 8 ? 2 : 4) {
       int parts = 0, total;
 #pragma unroll
       for (int i = 0; i < EACH; ++i) parts += parts_of(p, chunks[i], q) * blocks[i];
       block_scan(parts, total, sums);
       if (int64_t(total) * H <= p.target) break;
-      q = q0 + (q0 * (1 << t) + 15) / 16;  // 1/8, 1/4, 1/2, 1 above q0
+      q = q0 + (q0 * t + 15) / 16;  // a sixteenth above q0, two, .. and at last all of it
     }
   int parts = 0, slots = 0, n_parts, n_slots, n_units, units = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int k = parts_of(p, chunks[i], q);
     parts += k * blocks[i] * H;
-    slots += k > 1 ? k * blocks[i] * H : 0;
+    slots += slots_of(p, k) * blocks[i] * H;
     units += chunks[i] > 0 ? 0 : blocks[i] * H;
   }
   int at = block_scan(parts, n_parts, sums), slot = block_scan(slots, n_slots, sums);
@@ -123,7 +131,7 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
       part_at[b0 + i] = at;
       slot_at[b0 + i] = slot;
       at += k * blocks[i] * H;
-      slot += k > 1 ? k * blocks[i] * H : 0;
+      slot += slots_of(p, k) * blocks[i] * H;
     }
   __syncthreads();
   n_parts = min(n_parts, p.most_parts);
@@ -139,13 +147,13 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
     const int cut = rel / nb;
     r.head = cut / k;
     r.part = cut - r.head * k;
-    if (p.a.cluster > 0) {  // a cluster's CTAs are the neighbours
-      r.part = rel % k;
-      block = rel / k % nb;
-      r.head = rel / k / nb;
+    if (const int n = p.a.cluster; n > 0) {  // a cluster's CTAs are the neighbours
+      block = rel / n % nb;
+      r.part = rel / n / nb % (k / n) * n + rel % n;
+      r.head = rel / nb / k;
     }
     r.parts = k;
-    r.slot0 = slot_at[b] + (r.head * nb + block) * k;
+    r.slot0 = slot_at[b] + (r.head * nb + block) * slots_of(p, k);
     r.c0 = int(int64_t(c) * r.part / k);
     r.c1 = int(int64_t(c) * (r.part + 1) / k);
     r.row0 = block * each;
@@ -234,7 +242,9 @@ int plan_attend(const AttendParams &a, const PlanShape &shape, cudaStream_t stre
   p.a = a;
   p.target = shape.target;
   p.spread = shape.spread;
-  p.min_chunks = 2;  // a join costs about what ten chunks do
+  p.single = shape.single;
+  // a join through the workspace costs about what ten chunks do
+  p.min_chunks = shape.cluster > 0 ? 10 : 2;
   p.most_parts = int(shape.most_parts);
   p.most_units = int(shape.most_units);
   p.most_joins = int(shape.most_joins);

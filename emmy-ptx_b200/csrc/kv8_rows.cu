@@ -29,9 +29,10 @@
 // stays whole and needs no join.  Parts of a cut segment leave (m, l, O) in
 // the workspace; the last of each 16 parts to arrive joins them in their
 // order, the last of those their sums, so results do not depend on the order
-// of arrival.  The parts of a short segment are a cluster instead: each CTA
-// joins a share of the rows' values out of the others' shared memory, with
-// neither the workspace nor its round trips to L2.
+// of arrival.  Where there are few segments, clusters of CTAs join their parts
+// first, each a share of the rows' values out of the others' shared memory:
+// a short segment is one cluster and needs neither the workspace nor its round
+// trips to L2, a long one leaves a result a cluster there.
 #include <cuda_bf16.h>
 
 #include <cuda.h>  // CUtensorMap
@@ -83,7 +84,7 @@ struct Layout {
   static constexpr int STAGES = 64 * 1024 / CHUNK;
   static constexpr int QUERIES = STAGES * CHUNK, END = QUERIES + NT * 16 * D;
   static constexpr int DYN = END + 1024;  // the swizzle repeats every 1 KB
-  static constexpr int LD = D + 8;        // floats of a row of the join
+  static constexpr int LD = D + 4;        // floats of a row of the join
   static_assert((WARPS * LD + D) * 8 * NT * 4 <= QUERIES, "the join and a cluster's part fit over the ring");
   static_assert(2 * 64 * 8 * NT * 4 <= QUERIES, "so do the maxima and sums of 64 parts");
 };
@@ -300,7 +301,7 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
   extern __shared__ uint8_t dyn_raw[];
   uint8_t *const dyn = dyn_raw + ((1024 - (smem_addr(dyn_raw) & 1023)) & 1023);
   float *const join = reinterpret_cast<float *>(dyn);
-  __shared__ float sm_m[WARPS][ROWS], sm_l[WARPS][ROWS], weight[WARPS][ROWS], row_l[ROWS], row_m[ROWS];
+  __shared__ float sm_m[WARPS][ROWS], sm_l[WARPS][ROWS], row_l[ROWS], row_m[ROWS];
   __shared__ int sm_unit[WARPS], row_pos[ROWS];  // position of the row's token, -1: no such row
   __shared__ float row_mult[ROWS];               // scale * log2(e) * the row's power of two
   __shared__ unsigned ticket, stop_word;
@@ -507,35 +508,25 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
     }
     if (!CLUSTER) return;  // a cluster's blocks stay until all have read
   }
+  // Value gr D / 8 + 2 j + e of a row lies at 16 j + 2 gr + e: the lanes that
+  // store together (gr and 8 q) then meet in no bank.
   if (warp < WARPS) {
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float l = st.l[i][c];
-      l += __shfl_xor_sync(0xffffffffu, l, 4);
-      l += __shfl_xor_sync(0xffffffffu, l, 8);
-      l += __shfl_xor_sync(0xffffffffu, l, 16);
-      const int r = 8 * i + 2 * q + c;
-      if (gr == 0) sm_m[warp][r] = st.m[i][c], sm_l[warp][r] = l;
+      for (int c = 0; c < 2; ++c) {
+        float l = st.l[i][c];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int r = 8 * i + 2 * q + c;
+        if (gr == 0) sm_m[warp][r] = st.m[i][c], sm_l[warp][r] = l;
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j)
-        *reinterpret_cast<float2 *>(&join[(warp * ROWS + r) * LD + gr * (D / 8) + 2 * j]) =
-            make_float2(st.o[j][i][c], st.o[j][i][c + 2]);
-    }
+        for (int j = 0; j < D / 16; ++j)
+          *reinterpret_cast<float2 *>(&join[(warp * ROWS + r) * LD + 16 * j + 2 * gr]) =
+              make_float2(st.o[j][i][c], st.o[j][i][c + 2]);
+      }
     if (lane == 0) sm_unit[warp] = st.unit;
-  }
-  __syncthreads();
-  if (tid < ROWS) {
-    float m = NONE, l = 0.0f;
-    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, sm_m[w][tid]);
-    for (int w = 0; w < WARPS; ++w) {
-      const float f = exp2_fast(sm_m[w][tid] - m);
-      l += f * sm_l[w][tid];
-      weight[w][tid] = f * pow2(sm_unit[w]);
-    }
-    row_m[tid] = m;
-    row_l[tid] = l;
   }
   __syncthreads();
   const bool whole = !CLUSTER && g.parts == 1;
@@ -554,32 +545,43 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
   float *const slot = CLUSTER ? join + WARPS * ROWS * LD : part_slot(g.part);
   for (int i = tid; i < rows * (D / 8); i += THREADS) {
     const int r = i / (D / 8), d = i % (D / 8) * 8;
-    float x[8] = {};
+    float m = NONE, l = 0.0f, x[8] = {};
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, sm_m[w][r]);
+    const float *at = &join[r * LD + d % (D / 8) * 8 + d / (D / 8) * 2];
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      const float f = weight[w][r];
-      const float4 u = *reinterpret_cast<const float4 *>(&join[(w * ROWS + r) * LD + d]);
-      const float4 v = *reinterpret_cast<const float4 *>(&join[(w * ROWS + r) * LD + d + 4]);
-      x[0] += f * u.x, x[1] += f * u.y, x[2] += f * u.z, x[3] += f * u.w;
-      x[4] += f * v.x, x[5] += f * v.y, x[6] += f * v.z, x[7] += f * v.w;
+      float f = exp2_fast(sm_m[w][r] - m);
+      l += f * sm_l[w][r];
+      f *= pow2(sm_unit[w]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 u = *reinterpret_cast<const float2 *>(at + w * ROWS * LD + 16 * j);
+        x[2 * j] += f * u.x, x[2 * j + 1] += f * u.y;
+      }
     }
+    if (!whole && d == 0) row_m[r] = m, row_l[r] = l;
     if (whole) {
-      store(r, d, x, row_l[r]);
+      store(r, d, x, l);
     } else {
       *reinterpret_cast<float4 *>(slot + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
       *reinterpret_cast<float4 *>(slot + r * D + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
     }
   }
   if (whole) return;
+  // results of the segment that go through the workspace, and which is this
+  const int results = CLUSTER ? g.parts / p.cluster : g.parts, result = CLUSTER ? g.part / p.cluster : g.part;
   if constexpr (CLUSTER) {
+    const int n = p.cluster;
     cluster_sync();
-    for (int i = cluster_rank() * THREADS + tid; i < rows * (D / 4); i += g.parts * THREADS) {
+    const int share = (rows * (D / 4) + n - 1) / n, i0 = cluster_rank() * share;
+    for (int i = i0 + tid; i < min(i0 + share, rows * (D / 4)); i += THREADS) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
       float4 u[MOST_CLUSTER];
       float ms[MOST_CLUSTER], ls[MOST_CLUSTER], m = NONE, l = 0.0f;
 #pragma unroll
       for (int c = 0; c < MOST_CLUSTER; ++c)
-        if (c < g.parts) {
+        if (c < n) {
           ms[c] = peer_load(peer_addr(&row_m[r], c));
           ls[c] = peer_load(peer_addr(&row_l[r], c));
           u[c] = peer_load4(peer_addr(slot + r * D + d, c));
@@ -588,21 +590,33 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
       float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int c = 0; c < MOST_CLUSTER; ++c)
-        if (c < g.parts) {
+        if (c < n) {
           const float f = exp2_fast(ms[c] - m);
           l += f * ls[c];
           x.x += f * u[c].x, x.y += f * u[c].y, x.z += f * u[c].z, x.w += f * u[c].w;
         }
+      if (results > 1) {
+        float *const to = part_slot(result);
+        __stcg(reinterpret_cast<float4 *>(to + r * D + d), x);
+        if (d == 0) {
+          __stcg(to + ROWS * D + r, m);
+          __stcg(to + ROWS * D + ROWS + r, l);
+        }
+        continue;
+      }
       const float by = l == 0.0f ? 0.0f : 1.0f / l;
       *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) =
           make_uint2(pack2<T>(x.x * by, x.y * by), pack2<T>(x.z * by, x.w * by));
     }
     cluster_sync();  // no block ends while another reads it
-    return;
+    if (results == 1 || cluster_rank() != 0) return;
   }
-  if (tid < ROWS) {
-    __stcg(slot + ROWS * D + tid, row_m[tid]);
-    __stcg(slot + ROWS * D + ROWS + tid, row_l[tid]);
+  if constexpr (!CLUSTER) {
+    __syncthreads();
+    if (tid < rows) {
+      __stcg(slot + ROWS * D + tid, row_m[tid]);
+      __stcg(slot + ROWS * D + ROWS + tid, row_l[tid]);
+    }
   }
   // ---- parts join in groups of GROUP, groups in the segment: the last of
   // each to arrive does it, in the parts' order ----
@@ -677,10 +691,10 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
       __stcg(part_slot(a) + ROWS * D + ROWS + tid, row_l[tid]);
     }
   };
-  // up to 64 parts at once where one level does, else groups of GROUP
-  const int group = g.parts <= ONE_LEVEL ? g.parts : max(GROUP, (g.parts + 63) / 64);
-  const int lead = g.part / group * group, count = min(group, g.parts - lead);
-  const int groups = (g.parts + group - 1) / group;
+  // up to 64 at once where one level does, else groups of GROUP
+  const int group = results <= ONE_LEVEL ? results : max(GROUP, (results + 63) / 64);
+  const int lead = result / group * group, count = min(group, results - lead);
+  const int groups = (results + group - 1) / group;
   if (!last_of(lead, 0, count)) return;
   gather(lead, count, 1, groups == 1);
   if (groups == 1 || !last_of(0, 1, groups)) return;
