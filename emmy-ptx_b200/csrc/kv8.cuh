@@ -46,7 +46,7 @@ __device__ __forceinline__ void report(unsigned *status, unsigned code) {
 
 // n, or 0 (nothing to do), reported, where the lengths cannot be right.
 __device__ __forceinline__ int checked_n(const Seqs &s, int start, int n, int len) {
-  if (n >= 0 && n <= len && n <= s.max_q && start >= 0 && start + n <= s.tokens && len <= (int64_t(s.width) << s.page_shift)) return n;
+  if (n >= 0 && n <= len && n <= s.max_q && start >= 0 && start <= s.tokens - n && len <= (int64_t(s.width) << s.page_shift)) return n;
   report(s.status, STATUS_LENGTH);
   return 0;
 }
@@ -164,6 +164,7 @@ int launch_kernel(const char *what, void (*kernel)(A...), dim3 grid, int threads
 
 // Checks what every call shares and fills the kernels' view of the sequences.
 int check_cache(const char *what, const emmy_kv8 *c);
+int check_counts(const char *what, const emmy_kv8 *c);  // of the sequences, without their arrays
 int check_seqs(const char *what, const emmy_kv8 *c);
 Seqs seqs_of(const emmy_kv8 &c);
 int sm_count(int device);

@@ -111,6 +111,7 @@ extern "C" int emmy_kv8_attend_sizes(const emmy_kv8 *cache, int32_t heads, uint6
   using namespace kv8;
   static const char *what = "emmy_kv8_attend_sizes";
   int rc = check_cache(what, cache);
+  if (rc == EMMY_OK) rc = check_counts(what, cache);
   if (rc == EMMY_OK && (workspace_bytes == nullptr || plan_bytes == nullptr))
     rc = fail(EMMY_EINVAL, what, "null result");
   PlanShape shape;
@@ -142,7 +143,8 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   if (rc != EMMY_OK) return rc;
   if (a->dtype != EMMY_KV8_BF16 && a->dtype != EMMY_KV8_F16)
     return fail(EMMY_EINVAL, what, "dtype must be bf16 or f16");
-  if (!std::isfinite(a->scale)) return fail(EMMY_EINVAL, what, "scale must be finite");
+  const float scale_log2 = a->scale * 1.4426950408889634f;
+  if (!std::isfinite(scale_log2)) return fail(EMMY_EINVAL, what, "scale must be finite, times log2(e) too");
   if (cache->tokens == 0 || cache->max_q == 0) return EMMY_OK;
   if (a->q == 0 || a->out == 0) return fail(EMMY_EINVAL, what, "null q or out");
   if (a->q % 16 || a->out % 16 || a->q_strides[0] % 8 || a->q_strides[1] % 8 || a->out_strides[0] % 8 ||
@@ -169,7 +171,7 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   p.counters = reinterpret_cast<unsigned *>(a->workspace);
   p.partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO);
   p.tile_partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO + shape.partial_bytes);
-  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   const OnDevice on(cache->device);
   if (on.err != cudaSuccess) return cuda_fail(what, on.err);
   const bool bf16 = a->dtype == EMMY_KV8_BF16;

@@ -54,6 +54,10 @@ int check_seqs(const char *what, const emmy_kv8 *c) {
     return fail(EMMY_EINVAL, what, "null page table, kv_lens or q_starts");
   if (c->page_table % 4 || c->kv_lens % 4 || c->q_starts % 4 || c->status % 4)
     return fail(EMMY_EINVAL, what, "page table, lengths and status must be 4-byte aligned");
+  return check_counts(what, c);
+}
+
+int check_counts(const char *what, const emmy_kv8 *c) {
   if (c->seqs < 1 || c->seqs > EMMY_KV8_MAX_SEQS)
     return fail(EMMY_EINVAL, what, "seqs must be between 1 and 4096");
   if (c->table_width < 1 || c->tokens < 0 || c->max_q < 0 || c->max_q > c->tokens)

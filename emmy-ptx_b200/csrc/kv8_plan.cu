@@ -103,7 +103,8 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   int all;
   block_scan(mine, all, sums);
   const int64_t work = int64_t(all) * H;
-  const int q0 = max(p.min_chunks, int((work + p.target - 1) / p.target));
+  const int64_t share = (work + p.target - 1) / p.target;
+  const int q0 = max(p.min_chunks, int(min(share, int64_t(1) << 24)));  // a sequence has no more chunks
   int q = q0;
   if (!p.spread && !p.single)
     for (int t = 1; t <= 16; t += t < 4 ? 1 : t < 8 ? 2 : 4) {

@@ -129,6 +129,19 @@ def _stream_of(stream, dev: Device) -> int:
     return stream if isinstance(stream, int) else stream.value or 0
 
 
+def _capturing(dev: Device, st: int) -> bool:
+    word = C.c_int()
+    check(dev.L.emmy_stream_capturing(st, C.byref(word)), "stream")
+    return word.value != 0
+
+
+def _outside_capture(dev: Device, st: int, why: str) -> None:
+    """A graph would keep the address of host memory that is gone when it
+    runs, or do what later calls count on only then."""
+    if _capturing(dev, st):
+        raise EmmyError(f"not while the stream is captured: {why}")
+
+
 # Device's own copy calls take a null stream for "the device's"; these take the
 # handle as it is, 0 included.
 def _copy_in(dev: Device, dst: int, host: np.ndarray, st: int) -> None:
@@ -325,6 +338,7 @@ class Batch:
         self._stale = False
         host = self._packed(table, kv_lens, q_lens)
         self._stream, self._reuse = _stream_of(stream, self.dev), True
+        _outside_capture(self.dev, self._stream, "lengths and page numbers are copied from the host")
         self._pool = _Pool.of(self.dev)
         self._others: set[int] = set()             # further streams it was used on
         self._buf = self._take("batch", host.nbytes, self._stream)
@@ -353,9 +367,7 @@ class Batch:
         st = _stream_of(stream, self.dev)
         if st != self._stream and st not in self._others:
             self._reuse = False
-            capturing = C.c_int()
-            check(self.L.emmy_stream_capturing(st, C.byref(capturing)), "stream")
-            if capturing.value:
+            if _capturing(self.dev, st):
                 return st
             ev = self.dev.event()
             try:
@@ -405,9 +417,15 @@ class Batch:
         graph or the next step: as many sequences, a table as wide, no more
         new tokens than the batch was made for."""
         self._live()
-        host = self._packed(_ints(page_table, "page_table"), kv_lens, q_lens)
-        st = self._on(stream)
-        _copy_in(self.dev, self._buf + 16, host[4:], st)
+        clash = self._clash
+        try:
+            host = self._packed(_ints(page_table, "page_table"), kv_lens, q_lens)
+            st = self._on(stream)
+            _outside_capture(self.dev, st, "lengths and page numbers are copied from the host")
+            _copy_in(self.dev, self._buf + 16, host[4:], st)
+        except EmmyError:
+            self._clash = clash         # of what the device still holds
+            raise
         for key in self._plans:
             self._plan(key, st)
         self._stale = False
@@ -475,6 +493,7 @@ class Batch:
         if not 1 <= heads <= 2 ** 20:
             raise EmmyError(f"attend: {heads} query heads")
         st = self._on(stream)
+        _outside_capture(self.dev, st, "reserve() for these heads, window and sinks comes before")
         ws, plan = C.c_uint64(), C.c_uint64()
         check(self.L.emmy_kv8_attend_sizes(self._ref, heads, C.byref(ws), C.byref(plan)), "attend")
         if ws.value > self._ws[1]:
@@ -527,6 +546,7 @@ class Batch:
         self._live()
         word = np.zeros(1, np.uint32)
         st = self._on(stream)
+        _outside_capture(self.dev, st, "the status word is read on the host")
         check(self.L.emmy_memcpy_dtoh(word.ctypes.data, self._buf, 4, st), "dtoh")
         check(self.L.emmy_stream_sync(st), "stream sync")
         if word[0]:
@@ -625,7 +645,8 @@ class KVSequences:
     def batch(self, sids, q_lens=None, stream=None) -> Batch:
         """Room for ``q_lens[i]`` (default 1) more tokens of each sequence:
         pages are taken, shared ones about to be written to copied, and the
-        lengths moved on.  Raises, with nothing changed, when pages run out."""
+        lengths moved on.  Where it raises (pages ran out), nothing has
+        changed."""
         sids = list(sids)
         q = [1] * len(sids) if q_lens is None else [int(n) for n in _ints(q_lens, "q_lens")]
         if not sids or len(q) != len(sids):
@@ -650,28 +671,39 @@ class KVSequences:
                     need += 1
         if need > len(self._free):
             raise EmmyError(f"batch: {need} pages needed, {len(self._free)} free")
-        src, dst = [], []
-        for sid in copies:
-            page, old = self._free.pop(), self._pages[sid][-1]
-            self._refs[page] = 1
-            src.append(old)
-            dst.append(page)
-            self._refs[old] -= 1
-            self._pages[sid][-1] = page
+        taken = self._free[:-need - 1:-1]          # the next ones, from the end
+        pages = {sid: list(self._pages[sid]) for sid in sids}
+        src, at = [pages[sid][-1] for sid in copies], len(copies)
+        for sid, page in zip(copies, taken):
+            pages[sid][-1] = page
         for sid, n in zip(sids, q):
-            self._len[sid] += n
-            while len(self._pages[sid]) * P < self._len[sid]:
-                page = self._free.pop()
-                self._refs[page] = 1
-                self._pages[sid].append(page)
-        self.cache.copy_pages(src, dst, stream)
-        b = Batch(self.cache, self.table(sids), [self._len[s] for s in sids], q, stream)
+            more = -(-(self._len[sid] + n) // P) - len(pages[sid])
+            if more > 0:
+                pages[sid] += taken[at:at + more]
+                at += more
+        lens = [self._len[sid] + n for sid, n in zip(sids, q)]
+        self.cache.copy_pages(src, taken[:len(src)], stream)
+        b = Batch(self.cache, self._table(list(pages.values())), lens, q, stream)
+        # the books follow once nothing can fail
+        del self._free[len(self._free) - need:]
+        for page in src:
+            self._refs[page] -= 1
+        for page in taken:
+            self._refs[page] = 1
+        self._pages.update(pages)
+        self._len.update(zip(sids, lens))
         self._track(b)
         return b
 
     def table(self, sids) -> np.ndarray:
         """Page numbers [sequences, pages of the longest], rows filled up with 0."""
-        rows = [self._pages[s] for s in sids]
+        sids = list(sids)
+        for sid in sids:
+            self._known(sid)
+        return self._table([self._pages[s] for s in sids])
+
+    @staticmethod
+    def _table(rows) -> np.ndarray:
         out = np.zeros((len(rows), max(1, max(map(len, rows), default=1))), np.int32)
         for i, r in enumerate(rows):
             out[i, :len(r)] = r

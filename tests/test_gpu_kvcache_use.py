@@ -371,3 +371,38 @@ def test_q_of_extreme_rows():
     assert np.isfinite(got[:, 0]).all() and (np.abs(got[:, 0]) <= most * (1 + 2.0 ** -8)).all()
     assert (np.abs(got[:, 0]).max(1) > 0).all()
     assert ref.close(got[:, 1:3], want[:, 1:3], bound[:, 1:3], "bf16")
+
+
+def test_what_a_capture_cannot_hold_is_refused():
+    """Copies from the host, and the first attend of a batch, during a
+    capture: refused, and the capture goes on."""
+    from ptxgen.runtime import EmmyError
+    rng = np.random.default_rng(21)
+    kv, ql = [300, 70], [1, 3]
+    cache, codes, exps, table, q = make(rng, kv, ql)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    batch = cache.batch(table, kv, ql, stream=st)
+    batch.reserve(q.shape[1], stream=st)
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        for call in (lambda: cache.batch(table, kv, ql, stream=st), lambda: batch.update(table, kv, ql, stream=st),
+                     lambda: batch.attend(0, q, out, window=64, stream=st), lambda: batch.check_errors(stream=st)):
+            with pytest.raises(EmmyError, match="captured"):
+                call()
+        batch.attend(0, q, out, stream=st)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert right(out, codes, exps, table, kv, ql, q)
+
+
+def test_a_scale_too_large_for_f32_is_refused():
+    from ptxgen.runtime import EmmyError
+    rng = np.random.default_rng(22)
+    cache, codes, exps, table, q = make(rng, [70], [1])
+    batch, out = cache.batch(table, [70], [1], stream=0), torch.empty_like(q)
+    for scale in (3e38, -3e38, float("inf"), float("nan")):
+        with pytest.raises(EmmyError, match="scale"):
+            batch.attend(0, q, out, scale=scale, stream=0)

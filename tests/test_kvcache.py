@@ -346,6 +346,51 @@ def test_sequence_refusals(dev):
     old.append(0, DeviceArray(16, "f32", (1, 2, 64)), DeviceArray(16, "f32", (1, 2, 64)))
 
 
+def test_a_batch_that_cannot_be_made_leaves_the_books(dev, monkeypatch):
+    """Too many sequences, a copy that fails, a closed cache: pages, lengths
+    and reference counts stay as they were."""
+    cache = KVCache(pages=5000, kv_heads=2, head_dim=64)
+    seqs = KVSequences(cache)
+    a = seqs.new()
+    seqs.batch([a], [70])
+    many = [a, seqs.fork(a)] + [seqs.new() for _ in range(4095)]
+
+    def books():
+        return ({s: seqs.pages(s) for s in many}, [seqs.length(s) for s in many], list(seqs._refs), list(seqs._free))
+    before = books()
+    with pytest.raises(EmmyError, match="4096"):
+        seqs.batch(many)
+    assert books() == before
+    with monkeypatch.context() as m:
+        m.setattr(kv, "_copy_in", lambda *a: kv.check(-3, "htod"))
+        with pytest.raises(EmmyError):
+            seqs.batch(many[:9], [100] * 9)
+    assert books() == before
+    cache.close()
+    with pytest.raises(EmmyError, match="closed"):
+        seqs.batch(many[:2])                     # one of them has to copy
+    assert books() == before
+    with pytest.raises(EmmyError, match="no sequence"):
+        seqs.table([a, 99999])
+
+
+def test_host_copies_are_refused_while_a_stream_is_captured(dev):
+    """Making, updating, planning and checking a batch; a refused update keeps
+    what append knows of the batch's pages."""
+    cache = small(dev)
+    b = cache.batch([[1], [2]], [9, 9], stream=5)
+    dev.L.emmy_stream_capturing = lambda st, word: setattr(word._obj, "value", 1) or 0
+    for call in (lambda: cache.batch([[1]], [9], stream=5), lambda: b.update([[1], [1]], [9, 9], stream=5),
+                 lambda: b.reserve(4, stream=5), lambda: b.check_errors(stream=5)):
+        with pytest.raises(EmmyError, match="captured"):
+            call()
+    x = DeviceArray(1 << 20, "bf16", (2, 2, 64))
+    b.append(0, x, x, stream=5)                  # the pages are still two
+    with pytest.raises(EmmyError):
+        b.update([[1], [99]], [9, 9])
+    b.append(0, x, x, stream=5)
+
+
 def _library():
     from ptxgen.runtime import lib_path, load_library
     if not lib_path().exists():
@@ -406,6 +451,8 @@ def test_c_entry_points_refuse_bad_arguments():
     assert L.emmy_kv8_attend_sizes(C.byref(d), 3, C.byref(u), C.byref(u)) == -3     # not a multiple
     assert L.emmy_kv8_attend_sizes(C.byref(d), 4, None, C.byref(u)) == -3
     assert L.emmy_kv8_attend_plan(C.byref(d), None, None) == -3
+    for kw in ({"seqs": -1}, {"tokens": -4, "max_q": -4}, {"max_q": 9}, {"table_width": 0}):
+        assert L.emmy_kv8_attend_sizes(C.byref(_desc(**kw)), 4, C.byref(u), C.byref(u)) == -3
 
 
 def test_oracle_rounds_as_e4m3_does():
