@@ -15,7 +15,8 @@
 // Tile kernel: units of 256 query rows of one (sequence, kv head); where there
 // are fewer than SMs they are cut along the keys, too, and joined by a kernel
 // of their own.  The longest come first (by 256 steps of the longest): the
-// hardware hands them out in order, and the short ones fill up the end.
+// CTAs take them in turn from the front and from the back, so that those with
+// the longest of one round get the shortest of the next.
 //
 // One CTA: a thread takes a few sequences, scans give each its first record,
 // and the records are then written a thread each.  A layer's worth of work for

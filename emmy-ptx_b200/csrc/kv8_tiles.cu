@@ -1,41 +1,47 @@
 // Attention of many query rows over the paged 8-bit cache (prompts, chunks of
 // prompts behind a history), on tcgen05.
 //
-// A CTA takes 256 query rows of one (sequence, kv head) -- tokens x the query
+// A unit is 256 query rows of one (sequence, kv head) -- tokens x the query
 // heads that share the kv head, so these share one pass over its keys -- as
-// two tiles A and B of 128 rows, and walks the 64-key chunks that some row
-// sees.  Warps:
-//   0, 1    tcgen05 O += P V of tile A, B (one thread each); 0 owns the TMEM
+// two tiles A and B of 128 rows, which walk the 64-key chunks that some row
+// sees.  One CTA an SM takes unit after unit, and every role runs on into the
+// next one as soon as its own work allows: codes and query rows of the next
+// unit are on their way, and its first scores are computed, while the softmax
+// warps still write this one's rows (a CTA a unit: 228 us a prompt of 8191
+// tokens with a window of 512 and d = 64, ten chunks a unit; so: 193).  Warps:
+//   0       tcgen05 O += P V of both tiles (one thread); owns the TMEM
+//   1       bulk copies of codes into shared memory, chunks ahead (in a loading
+//           warp, which they held up: 266 us a batch of prompts instead of 257)
 //   2, 3    tcgen05 S = Q K^T of tile A, B: an issuing warp slows the softmax
-//           warps of its sub-partition, and the slowest of a tile sets its
-//           pace, so each sub-partition gets one
+//           warps of its sub-partition, and the slowest of a tile sets its pace
 //   4-7     softmax and output of tile A, a thread a row; 8-11 of tile B
-//   12-15   bulk copies of codes into shared memory, chunks ahead (12), and
-//           codes -> f16, stored as the 128-byte-swizzled tiles the MMAs
+//   12-15   codes -> f16, stored as the 128-byte-swizzled tiles the MMAs
 //           read (K as [keys][d], V as stored: an MN-major operand)
-// 128 registers a thread at launch; the softmax warps take 176 (a row's 64
+// 128 registers a thread at launch; the softmax warps take 168 (a row's 64
 // scores and its packed weights are live together) from the others.
-// TMEM: per tile two 64-column S buffers (chunk g in buffer g % 2, P over its
-// first half as packed f16) and O.  With two buffers S of chunk g + 1 is
-// computed while the softmax works on chunk g.
+// TMEM: per tile two 64-column S buffers (chunk n of the tile in buffer n % 2,
+// P over its first half as packed f16) and O.  With two buffers S of chunk
+// n + 1 is computed while the softmax works on chunk n.
 //
 // The numerics are those of kv8_rows.cu: e4m3 exact in f16, a query row scaled
 // by a power of two, scores and sums in f32, p rounded to f16, K's page
 // exponent in the factor that takes scores to log2 units and V's in the
 // exponent of p; O moves (a pass over its columns) only when a row's maximum
 // grew by more than 2^8 or V's exponent strayed by more than 2^6.
-#include "kv8_attend.cuh"
+#include <algorithm>
+
 #include "kv8_async.cuh"
+#include "kv8_attend.cuh"
 
 namespace kv8 {
 namespace {
 
 constexpr int TILE = 128, CHUNK = 64, THREADS = 512;
 constexpr int STAGES = 3, RAW = 3;  // f16 chunks, and chunks of codes, in shared memory
-constexpr int W_PV = 0, W_QK = 2, W_SOFTMAX = 4, W_LOAD = 12;  // warps
+constexpr int W_PV = 0, W_FETCH = 1, W_QK = 2, W_SOFTMAX = 4, W_LOAD = 12;  // warps
 // Registers of the four warpgroups after the split.  The sum is what the
 // block was launched with: a split above it would wait for ever.
-constexpr int REGS_LAUNCH = 128, REGS_ISSUE = 64, REGS_SOFTMAX = 176, REGS_LOAD = 96;
+constexpr int REGS_LAUNCH = 128, REGS_ISSUE = 80, REGS_SOFTMAX = 168, REGS_LOAD = 96;
 static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX + REGS_LOAD == 4 * REGS_LAUNCH, "register split");
 constexpr float LAZY = 8.0f, LEAST = 1e-37f;
 // Weights are 2^(s rm - m) with one rounding of the difference, m = round(max s
@@ -59,7 +65,7 @@ struct Layout {
 };
 
 struct Bars {
-  uint64_t q_full, kv_full[STAGES], kv_empty[STAGES], raw_full[RAW], raw_empty[RAW];
+  uint64_t q_full[2], kv_full[STAGES], kv_empty[STAGES], raw_full[RAW], raw_empty[RAW];
   uint64_t s_full[2][2], p_full[2][2], pv_done[2][2], drain;
 };
 
@@ -165,11 +171,26 @@ constexpr uint32_t IDESC = 1u << 4 | uint32_t(B_MN) << 16 | uint32_t(N >> 3) << 
 // 16-byte piece j (0-7) of 128-byte row r of a swizzled tile.
 __device__ __forceinline__ uint32_t swizzled(int r, int j) { return r * 128 + ((j ^ (r & 7)) << 4); }
 
+// The record's rows and keys are within the arrays.
+__device__ __forceinline__ bool plan_holds(const AttendParams &p, int start, int n, int len) {
+  const bool ok = start + n <= p.s.tokens && len <= (int64_t(p.s.width) << p.s.page_shift);
+  if (!ok) report(p.s.status, STATUS_PLAN);
+  return ok;
+}
+
 // What the unit is: 256 rows of one (sequence, kv head).
 struct Unit {
   int b, head, start, n, len, rows, row0;
   Span span;
   int c0, slot;  // first chunk of this part's; workspace slot, -1: the unit is whole
+  int tiles, chunks;
+
+  Unit() = default;
+  __device__ __forceinline__ Unit(const AttendParams &p, const UnitRec &r)
+      : b(r.b), head(r.head), start(r.start), n(r.n), len(r.len), rows(r.n * p.group), row0(r.row0),
+        span(p, r.len - r.n + r.row0 / p.group,
+             r.len - r.n + (min(r.row0 + 2 * TILE, r.n * p.group) - 1) / p.group),
+        c0(r.c0), slot(r.slot), tiles(rows - r.row0 > TILE ? 2 : 1), chunks(r.c1 - r.c0) {}
 };
 
 // What goes with a chunk of codes.
@@ -190,11 +211,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
   uint8_t *const dyn = dyn_raw + ((1024 - (smem_addr(dyn_raw) & 1023)) & 1023);
   __shared__ Bars bars;
   __shared__ uint32_t tmem_slot;
-  // Chunk g's scales (2^ek, ev) and whether it holds NaN values, in slot g % 4:
-  // by the time chunk g + 4 is written there, P V of chunk g + 1 is done and
-  // with it every softmax warp past chunk g.
+  // Scales (2^ek, ev) of the CTA's chunk c and whether it holds NaN values, in
+  // slots c % 4 and c % 8: by the time chunk c + 4 is written there, P V of chunk c + 1 is
+  // done and with it every softmax warp past chunk c.
   __shared__ float2 chunk_scale[4];
-  __shared__ unsigned stop_word, chunk_nan[4];
+  __shared__ unsigned stop_word, chunk_nan[8];
   __shared__ ChunkInfo raw_info[RAW];
   volatile unsigned *const stop = &stop_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -202,22 +223,33 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 
   grid_dependency_wait();
   const PlanHead head = *p.plan;
-  const UnitRec rec = p.units[blockIdx.x];
+  const UnitRec first_rec = p.units[blockIdx.x];
   grid_dependency_done();
-  if (blockIdx.x >= head.units || !plan_fits(p, head, rec.b, rec.start, rec.n, rec.len)) return;
-  Unit u = {rec.b, rec.head, rec.start, rec.n, rec.len, rec.n * p.group, rec.row0, {}, rec.c0, rec.slot};
-  u.span = Span(p, u.len - u.n + u.row0 / p.group, u.len - u.n + (min(u.row0 + 2 * TILE, u.rows) - 1) / p.group);
-  const int tiles = u.rows - u.row0 > TILE ? 2 : 1;
-  const int chunks = rec.c1 - rec.c0;
+  if (blockIdx.x >= head.units || !plan_fits(p, head, first_rec.b, first_rec.start, first_rec.n, first_rec.len)) return;
+  // The units of this CTA: one of each gridDim.x, in turn from the front and
+  // from the back, since the longest come first.
+  const int units = head.units;
+  const auto index_of = [&](int k) {
+    return k * int(gridDim.x) + (k & 1 ? int(gridDim.x) - 1 - int(blockIdx.x) : int(blockIdx.x));
+  };
+  const auto load_unit = [&](int k, Unit &u) {  // false: there is no such unit
+    const int i = index_of(k);
+    if (i >= units) return false;
+    const UnitRec r = p.units[i];
+    if (!plan_holds(p, r.start, r.n, r.len)) return false;
+    u = Unit(p, r);
+    return true;
+  };
 
   // ---- barriers, TMEM ----
   if (tid == 0) {
-    bar_init(&bars.q_full, tiles * 4);  // warps
+    bar_init(&bars.q_full[0], 4);  // warps
+    bar_init(&bars.q_full[1], 4);
     for (int i = 0; i < STAGES; ++i) {
       bar_init(&bars.kv_full[i], 4);
-      bar_init(&bars.kv_empty[i], tiles);
+      bar_init(&bars.kv_empty[i], 2);  // P V of both tiles, and tile B's S, which may have none
     }
-    for (int i = 0; i < 4; ++i) chunk_nan[i] = 0;
+    for (int i = 0; i < 8; ++i) chunk_nan[i] = 0;
     for (int i = 0; i < RAW; ++i) {
       bar_init(&bars.raw_full[i], 1);
       bar_init(&bars.raw_empty[i], 4);
@@ -228,7 +260,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         bar_init(&bars.p_full[x][i], 4);
         bar_init(&bars.pv_done[x][i], 1);
       }
-    bar_init(&bars.drain, 4);
+    bar_init(&bars.drain, 3);
     stop_word = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -243,117 +275,148 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 
   bool issuer = false;  // the lane that issued this warp's MMAs
   if (warp < W_SOFTMAX) regs_down<REGS_ISSUE>();
-  if (warp < W_QK) {
-    // ---- O += P V of one tile ----
+  if (warp == W_PV) {
+    // ---- O += P V of both tiles ----
     const uint32_t who = elected();
-    const int x = warp - W_PV;
-    bool ok = x < tiles;
+    bool ok = true;
     Ring kv;
-    for (int g = 0; ok && g < chunks; ++g, kv.next(STAGES)) {
-      const int st = kv.slot, buf = g & 1;
-      ok = warp_wait(&bars.kv_full[st], kv.phase, stop, s.status) &&
-           warp_wait(&bars.p_full[x][buf], g >> 1 & 1, stop, s.status);
-      if (!ok) break;
-      tc_after();
-      // V rows are 128 bytes (64 values of d), the second half of d follows
-      // CHUNK rows on; 16 keys are 2 KB
-      const uint64_t vd = smem_desc(smem_addr(dyn + L::STAGE0 + st * 2 * L::KV + L::KV), CHUNK * 128, 1024);
-      const uint32_t o = tmem + L::O_COL + x * D, pa = tmem + (2 * x + buf) * CHUNK;
+    int n[2] = {0, 0};  // chunks of each tile so far
+    Unit u;
+    for (int k = 0; ok && load_unit(k, u); ++k)
+      for (int g = 0; ok && g < u.chunks; ++g, kv.next(STAGES)) {
+        ok = warp_wait(&bars.kv_full[kv.slot], kv.phase, stop, s.status);
 #pragma unroll
-      for (int k = 0; k < CHUNK / 16; ++k)
-        mma_ts(o, pa + k * 8, vd + (k * 2048 >> 4), IDESC<TILE, D, true>, g > 0 || k > 0, who);
-      tc_commit(&bars.pv_done[x][buf], who);
-      tc_commit(&bars.kv_empty[st], who);
-    }
+        for (int x = 0; x < 2; ++x) {
+          if (!ok || x >= u.tiles) break;
+          const int buf = n[x] & 1;
+          ok = warp_wait(&bars.p_full[x][buf], n[x] >> 1 & 1, stop, s.status);
+          if (!ok) break;
+          ++n[x];
+          tc_after();
+          // V rows are 128 bytes (64 values of d), the second half of d follows
+          // CHUNK rows on; 16 keys are 2 KB
+          const uint64_t vd = smem_desc(smem_addr(dyn + L::STAGE0 + kv.slot * 2 * L::KV + L::KV), CHUNK * 128, 1024);
+          const uint32_t o = tmem + L::O_COL + x * D, pa = tmem + (2 * x + buf) * CHUNK;
+#pragma unroll
+          for (int i = 0; i < CHUNK / 16; ++i)
+            mma_ts(o, pa + i * 8, vd + (i * 2048 >> 4), IDESC<TILE, D, true>, g > 0 || i > 0, who);
+          tc_commit(&bars.pv_done[x][buf], who);
+        }
+        if (ok) tc_commit(&bars.kv_empty[kv.slot], who);
+      }
     if (who) issuer = true;
+  } else if (warp == W_FETCH) {
+    // ---- bulk copies: K and V of a page's chunk are one contiguous piece
+    // each; 32 chunks' pages and exponents are read at once, a lane a chunk ----
+    const uint32_t who = elected();
+    bool ok = true;
+    int so_far = 0;
+    Ring copied;
+    Unit u;
+    for (int k = 0; ok && load_unit(k, u); ++k) {
+      const int *row = s.table + int64_t(u.b) * s.width;
+      ChunkInfo next = {0, 0, 0, 0};
+      int64_t next_unit = 0;
+      const auto fetch = [&](int g) {  // chunk g into the next slot, which is free
+        if ((g & 31) == 0) {
+          next = ChunkInfo{0, 0, 0, 0};
+          next_unit = 0;
+          if (g + lane < u.chunks) {
+            next.key0 = u.span.key0(u.c0 + g + lane);
+            int page = row[next.key0 >> s.page_shift];
+            next.dead = page < 0 || page >= s.pages;
+            if (next.dead) {
+              report(s.status, STATUS_PAGE);
+              page = 0;
+            }
+            next_unit = int64_t(page) * 2 * s.kv_heads + u.head;
+            next.ek = p.exps[next_unit];
+            next.ev = p.exps[next_unit + s.kv_heads];
+          }
+        }
+        const int64_t at = __shfl_sync(0xffffffffu, next_unit, g & 31);
+        ChunkInfo c;
+        c.ek = __shfl_sync(0xffffffffu, next.ek, g & 31);
+        c.ev = __shfl_sync(0xffffffffu, next.ev, g & 31);
+        c.key0 = __shfl_sync(0xffffffffu, next.key0, g & 31);
+        c.dead = __shfl_sync(0xffffffffu, next.dead, g & 31);
+        if (who) {
+          raw_info[copied.slot] = c;
+          const uint8_t *k = p.codes + ((at << s.page_shift) + (c.key0 & ((1 << s.page_shift) - 1))) * D;
+          const uint8_t *v = k + (int64_t(s.kv_heads) << s.page_shift) * D;
+          const uint32_t dst = smem_addr(dyn + L::RAW0 + copied.slot * L::KV);
+          uint64_t *bar = &bars.raw_full[copied.slot];
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(L::KV)
+                       : "memory");
+          bulk_copy(dst, k, CHUNK * D, bar);
+          bulk_copy(dst + CHUNK * D, v, CHUNK * D, bar);
+        }
+        __syncwarp();
+        copied.next(RAW);
+      };
+      // its query rows on their way into L2
+      for (int i = lane; i < min(2 * TILE, u.rows - u.row0); i += 32) {
+        const int token = (u.row0 + i) / p.group, h = u.head * p.group + u.row0 + i - token * p.group;
+        const T *q = static_cast<const T *>(p.q) + (int64_t(u.start) + token) * p.q_ts + h * p.q_hs;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+        if (D == 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + D / 2));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(q + D - 8));
+      }
+      for (int g = 0; g < u.chunks; ++g, ++so_far) {
+        if (so_far >= RAW) ok = warp_wait(&bars.raw_empty[copied.slot], copied.phase ^ 1, stop, s.status);
+        if (!ok) break;
+        fetch(g);
+      }
+    }
   } else if (warp < W_SOFTMAX) {
     // ---- S = Q K^T of one tile ----
     const uint32_t who = elected();
     const int x = warp - W_QK;
-    bool ok = x < tiles && warp_wait(&bars.q_full, 0, stop, s.status);
     const uint64_t qd = smem_desc(smem_addr(dyn + x * L::Q_TILE), 16, 1024);
+    bool ok = true;
     Ring kv;
-    for (int g = 0; ok && g < chunks; ++g, kv.next(STAGES)) {
-      const int st = kv.slot, buf = g & 1;
-      ok = warp_wait(&bars.kv_full[st], kv.phase, stop, s.status);
-      // the buffer holds P of chunk g - 2 until its P V is done
-      if (ok && g >= 2) ok = warp_wait(&bars.pv_done[x][buf], (g >> 1 & 1) ^ 1, stop, s.status);
-      if (!ok) break;
-      tc_after();
-      const uint64_t kd = smem_desc(smem_addr(dyn + L::STAGE0 + st * 2 * L::KV), 16, 1024);
-      const uint32_t at = tmem + (2 * x + buf) * CHUNK;
+    int n = 0, mine = 0;  // chunks and units of this tile so far
+    Unit u;
+    for (int k = 0; ok && load_unit(k, u); ++k) {
+      if (x < u.tiles) ok = warp_wait(&bars.q_full[x], mine++ & 1, stop, s.status);
+      for (int g = 0; ok && g < u.chunks; ++g, kv.next(STAGES)) {
+        ok = warp_wait(&bars.kv_full[kv.slot], kv.phase, stop, s.status);
+        if (x == 1 && who) bar_arrive(&bars.kv_empty[kv.slot]);
+        if (x >= u.tiles) continue;
+        const int buf = n & 1;
+        // the buffer holds P of chunk n - 2 until its P V is done
+        if (ok && n >= 2) ok = warp_wait(&bars.pv_done[x][buf], (n >> 1 & 1) ^ 1, stop, s.status);
+        if (!ok) break;
+        ++n;
+        tc_after();
+        const uint64_t kd = smem_desc(smem_addr(dyn + L::STAGE0 + kv.slot * 2 * L::KV), 16, 1024);
+        const uint32_t at = tmem + (2 * x + buf) * CHUNK;
 #pragma unroll
-      for (int h = 0; h < D / 64; ++h)
+        for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_ss(at, qd + ((h * TILE * 128 + k * 32) >> 4), kd + ((h * CHUNK * 128 + k * 32) >> 4),
-                 IDESC<TILE, CHUNK, false>, h > 0 || k > 0, who);
-      tc_commit(&bars.s_full[x][buf], who);
-      // and one ordinary arrival, which passes on what the loading warps
-      // left beside the codes
-      if (who) bar_arrive(&bars.s_full[x][buf]);
+          for (int i = 0; i < 4; ++i)
+            mma_ss(at, qd + ((h * TILE * 128 + i * 32) >> 4), kd + ((h * CHUNK * 128 + i * 32) >> 4),
+                   IDESC<TILE, CHUNK, false>, h > 0 || i > 0, who);
+        tc_commit(&bars.s_full[x][buf], who);
+        // and one ordinary arrival, which passes on what the loading warps
+        // left beside the codes
+        if (who) bar_arrive(&bars.s_full[x][buf]);
+      }
     }
     if (who) issuer = true;
   } else if (warp >= W_LOAD) {
     regs_down<REGS_LOAD>();
-    // ---- bulk copies: K and V of a page's chunk are one contiguous piece
-    // each; 32 chunks' pages and exponents are read at once, a lane a chunk ----
-    const bool fetches = warp == W_LOAD;
-    const uint32_t who = elected();
-    const int *row = s.table + int64_t(u.b) * s.width;
-    ChunkInfo next = {0, 0, 0, 0};
-    int64_t next_unit = 0;
-    Ring copied;
-    const auto fetch = [&](int g) {  // chunk g into the next slot, which is free
-      if ((g & 31) == 0) {
-        next = ChunkInfo{0, 0, 0, 0};
-        next_unit = 0;
-        if (g + lane < chunks) {
-          next.key0 = u.span.key0(u.c0 + g + lane);
-          int page = row[next.key0 >> s.page_shift];
-          next.dead = page < 0 || page >= s.pages;
-          if (next.dead) {
-            report(s.status, STATUS_PAGE);
-            page = 0;
-          }
-          next_unit = int64_t(page) * 2 * s.kv_heads + u.head;
-          next.ek = p.exps[next_unit];
-          next.ev = p.exps[next_unit + s.kv_heads];
-        }
-      }
-      const int64_t at = __shfl_sync(0xffffffffu, next_unit, g & 31);
-      ChunkInfo c;
-      c.ek = __shfl_sync(0xffffffffu, next.ek, g & 31);
-      c.ev = __shfl_sync(0xffffffffu, next.ev, g & 31);
-      c.key0 = __shfl_sync(0xffffffffu, next.key0, g & 31);
-      c.dead = __shfl_sync(0xffffffffu, next.dead, g & 31);
-      if (who) {
-        raw_info[copied.slot] = c;
-        const uint8_t *k = p.codes + ((at << s.page_shift) + (c.key0 & ((1 << s.page_shift) - 1))) * D;
-        const uint8_t *v = k + (int64_t(s.kv_heads) << s.page_shift) * D;
-        const uint32_t dst = smem_addr(dyn + L::RAW0 + copied.slot * L::KV);
-        uint64_t *bar = &bars.raw_full[copied.slot];
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(L::KV)
-                     : "memory");
-        bulk_copy(dst, k, CHUNK * D, bar);
-        bulk_copy(dst + CHUNK * D, v, CHUNK * D, bar);
-      }
-      __syncwarp();
-      copied.next(RAW);
-    };
-    if (fetches)
-      for (int g = 0; g < min(RAW, chunks); ++g) fetch(g);
     // ---- codes -> f16 ----
     // A lane's 16-byte pieces of codes become two neighbouring 16-byte pieces
     // of f16.  D = 128: eight lanes that load or store together cover the two
     // halves of d in two neighbouring rows, so that neither the loads (rows of
     // 128 bytes) nor the stores (pieces exchanged by row & 7) meet in a bank.
     constexpr int PASS_ROWS = D == 128 ? 16 : 32, PASSES = CHUNK / PASS_ROWS;
-    const int w = warp - W_LOAD, c = lane & 3, b2 = lane >> 2 & 1;
+    const int w = warp - W_LOAD, piece = lane & 3, b2 = lane >> 2 & 1;
     const int r0 = D == 128 ? w * 4 + b2 + 2 * (lane >> 4) : w * 8 + (lane >> 2);
     const int half = D == 128 ? b2 ^ (lane >> 3 & 1) : 0;
-    const uint32_t from = r0 * D + (half * 4 + c) * 16;
-    const uint32_t to = half * (CHUNK * 128) + swizzled(r0, 2 * c);
+    const uint32_t from = r0 * D + (half * 4 + piece) * 16;
+    const uint32_t to = half * (CHUNK * 128) + swizzled(r0, 2 * piece);
     const auto put = [&](uint8_t *tile, int pass, const uint4 &x) {
       uint8_t *at = tile + pass * (PASS_ROWS * 128);
       *reinterpret_cast<uint4 *>(at + to) =
@@ -362,107 +425,138 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
           make_uint4(e4m3x2_f16x2(x.z), e4m3x2_f16x2(x.z >> 16), e4m3x2_f16x2(x.w), e4m3x2_f16x2(x.w >> 16));
     };
     Ring raw, kv;
-    for (int g = 0; g < chunks; ++g, raw.next(RAW), kv.next(STAGES)) {
-      // the slot of chunk g - 1 gets chunk g - 1 + RAW once all four warps read it
-      if (fetches && g > 0 && g - 1 + RAW < chunks) {
-        if (!warp_wait(&bars.raw_empty[copied.slot], copied.phase ^ 1, stop, s.status)) break;
-        fetch(g - 1 + RAW);
-      }
-      if (!warp_wait(&bars.raw_full[raw.slot], raw.phase, stop, s.status)) break;
-      const uint8_t *src = dyn + L::RAW0 + raw.slot * L::KV + from;
-      uint4 k[PASSES], v[PASSES];
+    int c = 0;  // chunks so far
+    bool ok = true;
+    Unit u;
+    for (int k = 0; ok && load_unit(k, u); ++k)
+      for (int g = 0; g < u.chunks; ++g, ++c, raw.next(RAW), kv.next(STAGES)) {
+        ok = warp_wait(&bars.raw_full[raw.slot], raw.phase, stop, s.status);
+        if (!ok) break;
+        const uint8_t *src = dyn + L::RAW0 + raw.slot * L::KV + from;
+        uint4 k[PASSES], v[PASSES];
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i) k[i] = *reinterpret_cast<const uint4 *>(src + i * PASS_ROWS * D);
+        for (int i = 0; i < PASSES; ++i) k[i] = *reinterpret_cast<const uint4 *>(src + i * PASS_ROWS * D);
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i) v[i] = *reinterpret_cast<const uint4 *>(src + CHUNK * D + i * PASS_ROWS * D);
-      const ChunkInfo info = raw_info[raw.slot];
-      warp_arrive(&bars.raw_empty[raw.slot]);
-      const int st = kv.slot;
-      if (g >= STAGES && !warp_wait(&bars.kv_empty[st], kv.phase ^ 1, stop, s.status)) break;
-      // chunks some row does not see whole: values no row sees are zeroed and
-      // a NaN is taken out here (0 * NaN would reach rows it is hidden from)
-      // and put into the rows that see it at the end
-      if (info.dead || !u.span.all_see(info.key0, info.key0 + CHUNK - 1)) {
+        for (int i = 0; i < PASSES; ++i) v[i] = *reinterpret_cast<const uint4 *>(src + CHUNK * D + i * PASS_ROWS * D);
+        const ChunkInfo info = raw_info[raw.slot];
+        warp_arrive(&bars.raw_empty[raw.slot]);
+        const int st = kv.slot;
+        if (c >= STAGES) ok = warp_wait(&bars.kv_empty[st], kv.phase ^ 1, stop, s.status);
+        if (!ok) break;
+        // chunks some row does not see whole: values no row sees are zeroed and
+        // a NaN is taken out here (0 * NaN would reach rows it is hidden from)
+        // and put into the rows that see it at the end
+        if (info.dead || !u.span.all_see(info.key0, info.key0 + CHUNK - 1)) {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-          if (info.dead || !u.span.any_sees(info.key0 + r0 + i * PASS_ROWS)) v[i] = make_uint4(0, 0, 0, 0);
-          uint32_t *x = &v[i].x;
+          for (int i = 0; i < PASSES; ++i) {
+            if (info.dead || !u.span.any_sees(info.key0 + r0 + i * PASS_ROWS)) v[i] = make_uint4(0, 0, 0, 0);
+            uint32_t *x = &v[i].x;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t bad = nan_bytes(x[j]);
-            if (bad != 0) {
-              x[j] &= ~((bad >> 7) * 0xffu);
-              chunk_nan[g & 3] = 1;
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t bad = nan_bytes(x[j]);
+              if (bad != 0) {
+                x[j] &= ~((bad >> 7) * 0xffu);
+                chunk_nan[c & 7] = 1;
+              }
             }
           }
         }
+        uint8_t *tile = dyn + L::STAGE0 + st * 2 * L::KV;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) put(tile, i, k[i]);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) put(tile + L::KV, i, v[i]);
+        if (tid == W_LOAD * 32) {
+          chunk_scale[c & 3] = make_float2(info.dead ? 0.0f : pow2(info.ek), float(info.ev));
+          chunk_nan[(c + 4) & 7] = 0;  // no loading warp is three chunks ahead
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        warp_arrive(&bars.kv_full[st]);
       }
-      uint8_t *tile = dyn + L::STAGE0 + st * 2 * L::KV;
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) put(tile, i, k[i]);
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) put(tile + L::KV, i, v[i]);
-      if (tid == W_LOAD * 32) chunk_scale[g & 3] = make_float2(info.dead ? 0.0f : pow2(info.ek), float(info.ev));
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      warp_arrive(&bars.kv_full[st]);
-    }
   } else if (warp >= W_SOFTMAX) {
     // ---- softmax: a thread a row ----
     regs_up<REGS_SOFTMAX>();
     const int x = (warp - W_SOFTMAX) >> 2, quad = warp & 3, r = quad * 32 + lane;
-    if (x < tiles) {
-      const int row = u.row0 + x * TILE + r;
-      const bool real = row < u.rows;
-      const int token = min(row, u.rows - 1) / p.group;
-      const int head = u.head * p.group + min(row, u.rows - 1) - token * p.group;
-      const int pos = u.len - u.n + token;
-      float mult;
-      {
-        // the query row: f16, scaled by a power of two, the scale's sign in it
-        const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) +
-                                                           (int64_t(u.start) + token) * p.q_ts + head * p.q_hs);
-        uint4 w[D / 8];
+    const uint32_t lanes = uint32_t(quad * 32) << 16;
+    const uint32_t s_at = tmem + lanes + 2 * x * CHUNK, o_at = tmem + lanes + L::O_COL + x * D;
+    // the unit from the k-th on that has this tile
+    const auto next_unit = [&](int &k, int &before, Unit &u) {
+      for (; load_unit(k, u); ++k, before += u.chunks)
+        if (x < u.tiles) return true;
+      return false;
+    };
+    struct Row {
+      int token, head, pos;
+      bool real;
+    };
+    const auto row_of = [&](const Unit &u) {
+      const int row = u.row0 + x * TILE + r, at = min(row, u.rows - 1);
+      Row w;
+      w.token = at / p.group;
+      w.head = u.head * p.group + at - w.token * p.group;
+      w.pos = u.len - u.n + w.token;
+      w.real = row < u.rows;
+      return w;
+    };
+    // The unit's query rows, f16, scaled by a power of two, the scale's sign in
+    // them; returns the factor of the row's scores.  The products that read the
+    // rows before are done: their scores were here.
+    const auto put_query = [&](const Unit &u, const Row &row) {
+      const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) +
+                                                         (int64_t(u.start) + row.token) * p.q_ts + row.head * p.q_hs);
+      uint4 w[D / 8];
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) w[i] = src[i];
-        float amax = 0.0f;
+      for (int i = 0; i < D / 8; ++i) w[i] = src[i];
+      float amax = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint32_t *v = &w[i].x;
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t *v = &w[i].x;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float a, b;
-            unpack2<T>(v[j], a, b);
-            a = fabsf(a), b = fabsf(b);
-            amax = a < INFINITY ? fmaxf(amax, a) : amax;
-            amax = b < INFINITY ? fmaxf(amax, b) : amax;
-          }
+        for (int j = 0; j < 4; ++j) {
+          float a, b;
+          unpack2<T>(v[j], a, b);
+          a = fabsf(a), b = fabsf(b);
+          amax = a < INFINITY ? fmaxf(amax, a) : amax;
+          amax = b < INFINITY ? fmaxf(amax, b) : amax;
         }
-        const int e = row_exponent(amax);
-        const float by = p.scale_log2 < 0.0f ? -pow2(-e) : pow2(-e);
-        mult = fabsf(p.scale_log2) * pow2(e);
+      }
+      const int e = row_exponent(amax);
+      const float by = p.scale_log2 < 0.0f ? -pow2(-e) : pow2(-e);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          uint32_t *v = &w[i].x;
+      for (int i = 0; i < D / 8; ++i) {
+        uint32_t *v = &w[i].x;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float a, b;
-            unpack2<T>(v[j], a, b);
-            v[j] = pack2<__half>(a * by, b * by);
-          }
-          *reinterpret_cast<uint4 *>(dyn + x * L::Q_TILE + i / 8 * (TILE * 128) + swizzled(r, i % 8)) = w[i];
+        for (int j = 0; j < 4; ++j) {
+          float a, b;
+          unpack2<T>(v[j], a, b);
+          v[j] = pack2<__half>(a * by, b * by);
         }
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-          *reinterpret_cast<uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8) + 4 * i) = 0;
+        *reinterpret_cast<uint4 *>(dyn + x * L::Q_TILE + i / 8 * (TILE * 128) + swizzled(r, i % 8)) = w[i];
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      warp_arrive(&bars.q_full);
-
-      const uint32_t lanes = uint32_t(quad * 32) << 16;
-      const uint32_t s_at = tmem + lanes + 2 * x * CHUNK, o_at = tmem + lanes + L::O_COL + x * D;
+      warp_arrive(&bars.q_full[x]);
+      return fabsf(p.scale_log2) * pow2(e);
+    };
+    bool ok = true;
+    int k = 0, n = 0, before = 0;  // chunks of this tile, and of all units before this
+    Unit u;
+    float mult = 0.0f;
+    Row at;
+    bool more = next_unit(k, before, u);
+    if (more) {
+      at = row_of(u);
+      mult = put_query(u, at);
+    }
+    while (more) {
+      // of the unit only what the loop needs stays in registers
+      const int pos = at.pos, chunks = u.chunks, c0 = u.c0, sink_chunks = u.span.sink_chunks, window_chunk0 = u.span.window_chunk0;
+      const bool real = at.real;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        *reinterpret_cast<uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8) + 4 * i) = 0;
       float m = NONE, l = 0.0f;
       int unit = 0;
-      bool ok = true, nan_seen = false, big = false;
+      bool nan_seen = false, big = false;
       // chunks whole_lo .. whole_hi - 1 every row sees whole
       int whole_lo = 0, whole_hi = chunks;
       {
@@ -475,12 +569,13 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         whole_hi = sp.sink_chunks + ((sp.first + 1) >> 6) - sp.window_chunk0 - u.c0;
         whole_lo -= u.c0;
       }
-      for (int g = 0; g < chunks; ++g) {
-        const int buf = g & 1;
-        ok = warp_wait(&bars.s_full[x][buf], g >> 1 & 1, stop, s.status);
+      for (int g = 0; g < chunks; ++g, ++n) {
+        const int buf = n & 1;
+        ok = warp_wait(&bars.s_full[x][buf], n >> 1 & 1, stop, s.status);
         if (!ok) break;
         if (g == 0 && x == 1) stagger();
-        const float2 sc = chunk_scale[g & 3];
+        const int c = before + g;  // chunks of the CTA so far
+        const float2 sc = chunk_scale[c & 3];
         const int ev = int(sc.y);
         float rm = fmaxf(mult * sc.x, LEAST);
         tc_after();
@@ -490,7 +585,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         tm_wait_ld();
         const bool dead = sc.x == 0.0f;
         if (dead || g < whole_lo || g >= whole_hi) {
-          const int key0 = u.span.key0(u.c0 + g);
+          const int i0 = c0 + g, key0 = (i0 < sink_chunks ? i0 : i0 - sink_chunks + window_chunk0) << 6;
           // bit i: the row sees key key0 + i
           const auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
           uint64_t see = below(pos - key0 + 1);
@@ -499,10 +594,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 #pragma unroll
           for (int i = 0; i < 64; ++i)
             if (!(see >> i & 1)) sv[i / 32][i % 32] = 0xff800000u;
-          if (chunk_nan[g & 3] != 0 && real) {
+          if (chunk_nan[c & 7] != 0 && real) {
             // (rare) this chunk holds NaN values: which of them this row sees
-            const int page = s.table[int64_t(u.b) * s.width + (key0 >> s.page_shift)];
-            const int64_t at = (int64_t(page) * 2 + 1) * s.kv_heads + u.head;
+            const UnitRec rec = p.units[index_of(k)];
+            const int page = s.table[int64_t(rec.b) * s.width + (key0 >> s.page_shift)];
+            const int64_t at = (int64_t(page) * 2 + 1) * s.kv_heads + rec.head;
             const uint32_t *v = reinterpret_cast<const uint32_t *>(
                 p.codes + ((at << s.page_shift) + (key0 & ((1 << s.page_shift) - 1))) * D);
             uint32_t *bits = reinterpret_cast<uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8));
@@ -564,8 +660,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         l = fmaf(even + odd, pow2(unit - ev), l);
         tm_wait_st();
         if (fix && !first) {
-          // P V of chunk g - 1 is the last to have touched O
-          ok = warp_wait(&bars.pv_done[x][(g - 1) & 1], (g - 1) >> 1 & 1, stop, s.status);
+          // P V of chunk n - 1 is the last to have touched O
+          ok = warp_wait(&bars.pv_done[x][(n - 1) & 1], (n - 1) >> 1 & 1, stop, s.status);
           if (!ok) break;
           tc_after();
 #pragma unroll
@@ -582,13 +678,26 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         tc_before();
         warp_arrive(&bars.p_full[x][buf]);
       }
-      if (ok) ok = warp_wait(&bars.pv_done[x][(chunks - 1) & 1], (chunks - 1) >> 1 & 1, stop, s.status);
-      if (ok) {
+      if (!ok) break;
+      // the next unit's queries first: its products start under this one's end
+      const int i = index_of(k);
+      u = Unit(p, p.units[i]);
+      at = row_of(u);
+      const int slot = u.slot;
+      T *const out = static_cast<T *>(p.out) + (int64_t(u.start) + at.token) * p.o_ts + at.head * p.o_hs;
+      before += chunks;
+      more = next_unit(++k, before, u);
+      if (more) {
+        at = row_of(u);
+        mult = put_query(u, at);
+      }
+      ok = warp_wait(&bars.pv_done[x][(n - 1) & 1], (n - 1) >> 1 & 1, stop, s.status);
+      if (!ok) break;
+      {
         tc_after();
-        const float by = u.slot >= 0 ? pow2(unit) : l == 0.0f ? 0.0f : pow2(unit) / l;
-        float *const part = p.tile_partial + int64_t(u.slot) * (D + 2) * (2 * TILE) + x * TILE + r;
+        const float by = slot >= 0 ? pow2(unit) : l == 0.0f ? 0.0f : pow2(unit) / l;
+        float *const part = p.tile_partial + int64_t(slot) * (D + 2) * (2 * TILE) + x * TILE + r;
         const uint32_t *bits = reinterpret_cast<const uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8));
-        T *out = static_cast<T *>(p.out) + (int64_t(u.start) + token) * p.o_ts + head * p.o_hs;
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
@@ -599,7 +708,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (nan >> i & 1) o[i] = 0x7fc00000u;
-          if (u.slot >= 0) {
+          if (slot >= 0) {
             // a part: O, and below its maximum and sum, a column of 256 rows each
 #pragma unroll
             for (int i = 0; i < 32; ++i) __stcg(&part[(c + i) * (2 * TILE)], __uint_as_float(o[i]) * by);
@@ -615,7 +724,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
             }
           }
         }
-        if (u.slot >= 0) {
+        if (slot >= 0) {
           __stcg(&part[D * (2 * TILE)], m);
           __stcg(&part[(D + 1) * (2 * TILE)], l);
         }
@@ -691,7 +800,7 @@ int launch(const AttendParams &p, int device, const PlanShape &shape, cudaStream
   static KernelSetup setup;
   int rc = setup.ready("emmy_kv8_attend", tiles_kernel<D, T>, device, Layout<D>::DYN, REGS_LAUNCH);
   if (rc == EMMY_OK)
-    rc = launch_kernel("emmy_kv8_attend", tiles_kernel<D, T>, dim3(unsigned(shape.most_units)), THREADS,
+    rc = launch_kernel("emmy_kv8_attend", tiles_kernel<D, T>, dim3(unsigned(std::min<int64_t>(shape.most_units, sm_count(device)))), THREADS,
                        Layout<D>::DYN, stream, p);
   if (rc == EMMY_OK && shape.tile_target > 0)
     rc = launch_kernel("emmy_kv8_attend", join_kernel<D, T>, dim3(unsigned(shape.most_joins), D / 8), 2 * TILE, 0,

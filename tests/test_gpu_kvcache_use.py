@@ -406,3 +406,30 @@ def test_a_scale_too_large_for_f32_is_refused():
     for scale in (3e38, -3e38, float("inf"), float("nan")):
         with pytest.raises(EmmyError, match="scale"):
             batch.attend(0, q, out, scale=scale, stream=0)
+
+
+@pytest.mark.parametrize("D,window,sinks", [(64, 0, 0), (64, 100, 3), (128, 0, 0), (128, 200, 70)])
+def test_many_units_of_one_and_two_tiles(D, window, sinks):
+    """More units of the tile kernel than SMs, so that a CTA goes from one to
+    the next: whole ones, ones with a single tile, histories of every length,
+    and NaN values that only some of the units see."""
+    rng = np.random.default_rng(23)
+    H, G, B = 5, 2, 80
+    ql = rng.integers(17, 300, B)
+    ql[:6] = 128, 64, 65, 192, 256, 1
+    kv = ql + np.where(rng.random(B) < 0.5, 0, rng.integers(0, 400, B))
+    cache, codes, exps, table, q = make(rng, kv.tolist(), ql.tolist(), H=H, G=G, D=D)
+    for b in (7, 20, 41):                           # one NaN each, in the middle of the keys
+        at = int(kv[b]) // 2
+        codes[table[b, at // 64], 1, b % H, at % 64, b] = 0x7f
+    cache._storage[0].copy_(torch.from_numpy(codes)[None])
+    batch, out = cache.batch(table, kv, ql, stream=0), torch.empty_like(q)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        batch.attend(0, q, out, window=window, sinks=sinks, stream=0)
+    batch.check_errors(stream=0)
+    assert right(out, codes, exps, table, kv, ql, q, window=window, sinks=sinks)
+    first = out.clone()
+    batch.attend(0, q, out, window=window, sinks=sinks, stream=0)
+    torch.cuda.synchronize()
+    assert torch.equal(out.view(torch.int16), first.view(torch.int16))
