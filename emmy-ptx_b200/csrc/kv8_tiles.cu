@@ -8,7 +8,8 @@
 // next one as soon as its own work allows: codes and query rows of the next
 // unit are on their way, and its first scores are computed, while the softmax
 // warps still write this one's rows (a CTA a unit: 228 us a prompt of 8191
-// tokens with a window of 512 and d = 64, ten chunks a unit; so: 193).  Warps:
+// tokens with a window of 512 and d = 64, ten chunks a unit; so: 193).
+// Warps:
 //   0       tcgen05 O += P V of both tiles (one thread); owns the TMEM
 //   1       bulk copies of codes into shared memory, chunks ahead (in a loading
 //           warp, which they held up: 266 us a batch of prompts instead of 257)
@@ -20,7 +21,7 @@
 // 128 registers a thread at launch; the softmax warps take 168 (a row's 64
 // scores and its packed weights are live together) from the others.
 // TMEM: per tile two 64-column S buffers (chunk n of the tile in buffer n % 2,
-// P over its first half as packed f16) and O.  With two buffers S of chunk
+// P over its first half as packed f16), O and, with d = 64, the query rows.  With two buffers S of chunk
 // n + 1 is computed while the softmax works on chunk n.
 //
 // The numerics are those of kv8_rows.cu: e4m3 exact in f16, a query row scaled
@@ -50,10 +51,15 @@ constexpr float LAZY = 8.0f, LEAST = 1e-37f;
 // 16 and more, and the factor rm is made a power of two, so that m is exact.
 constexpr float HUGE_SCORE = 134217728.0f;
 constexpr int UNIT_LAZY = 6;
+constexpr int Q_COL = 4 * CHUNK + 2 * 64;  // TMEM column of the query rows, d = 64 only
 
 template <int D>
 struct Layout {
-  static constexpr int Q_TILE = TILE * D * 2, KV = CHUNK * D * 2;  // bytes
+  // With d = 64 TMEM has room for the query rows, too: products that read them
+  // there leave shared memory's bandwidth to the keys (193 -> 189 us a prompt of
+  // 8191 tokens with a window of 512).
+  static constexpr bool Q_TMEM = D == 64;
+  static constexpr int Q_TILE = Q_TMEM ? 0 : TILE * D * 2, KV = CHUNK * D * 2;  // bytes
   static constexpr int STAGE0 = 2 * Q_TILE;
   static constexpr int RAW0 = STAGE0 + STAGES * 2 * KV;    // K codes, then V codes
   static constexpr int NAN_ROWS = RAW0 + RAW * KV;         // D bits a row
@@ -395,8 +401,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         for (int h = 0; h < D / 64; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            mma_ss(at, qd + ((h * TILE * 128 + i * 32) >> 4), kd + ((h * CHUNK * 128 + i * 32) >> 4),
-                   IDESC<TILE, CHUNK, false>, h > 0 || i > 0, who);
+            if constexpr (L::Q_TMEM)
+              mma_ts(at, tmem + Q_COL + x * (D / 2) + i * 8, kd + (i * 32 >> 4), IDESC<TILE, CHUNK, false>, i > 0, who);
+            else
+              mma_ss(at, qd + ((h * TILE * 128 + i * 32) >> 4), kd + ((h * CHUNK * 128 + i * 32) >> 4),
+                     IDESC<TILE, CHUNK, false>, h > 0 || i > 0, who);
         tc_commit(&bars.s_full[x][buf], who);
         // and one ordinary arrival, which passes on what the loading warps
         // left beside the codes
@@ -531,9 +540,19 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
           unpack2<T>(v[j], a, b);
           v[j] = pack2<__half>(a * by, b * by);
         }
-        *reinterpret_cast<uint4 *>(dyn + x * L::Q_TILE + i / 8 * (TILE * 128) + swizzled(r, i % 8)) = w[i];
+        if constexpr (!L::Q_TMEM)
+          *reinterpret_cast<uint4 *>(dyn + x * L::Q_TILE + i / 8 * (TILE * 128) + swizzled(r, i % 8)) = w[i];
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if constexpr (L::Q_TMEM) {
+        uint32_t all[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) all[i] = (&w[i / 4].x)[i % 4];
+        tm_st32(tmem + lanes + Q_COL + x * (D / 2), all);
+        tm_wait_st();
+        tc_before();
+      } else {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
       warp_arrive(&bars.q_full[x]);
       return fabsf(p.scale_log2) * pow2(e);
     };
