@@ -21,8 +21,9 @@
 // 128 registers a thread at launch; the softmax warps take 168 (a row's 64
 // scores and its packed weights are live together) from the others.
 // TMEM: per tile two 64-column S buffers (chunk n of the tile in buffer n % 2,
-// P over its first half as packed f16), O and, with d = 64, the query rows.  With two buffers S of chunk
-// n + 1 is computed while the softmax works on chunk n.
+// P over its first half as packed f16), O and, with d = 64, the query rows.
+// With two buffers S of chunk n + 1 is computed while the softmax works on
+// chunk n.
 //
 // The numerics are those of kv8_rows.cu: e4m3 exact in f16, a query row scaled
 // by a power of two, scores and sums in f32, p rounded to f16, K's page
@@ -124,8 +125,8 @@ __device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t (&r)[32]) {
       : "memory");
 }
 // Half a chunk's time: tile B starts so much later, so that its exponentials
-// fall between tile A's on the MUFU that they share (562 -> 542 us a prompt of
-// 8191 tokens, 238 -> 225 with a window of 512 and d = 64).
+// fall between tile A's on the MUFU that they share (196 -> 190 us a prompt of
+// 8191 tokens with a window of 512 and d = 64, 560 -> 557 without one).
 __device__ __forceinline__ void stagger() {
   const long long t0 = clock64();
   while (clock64() - t0 < 900) {

@@ -317,8 +317,10 @@ class Batch:
     rows behind the last one are left alone.  Calls of one batch share a
     workspace, so they must not overlap on the GPU: two captured graphs, or
     two streams, that run at once need a batch each.  A graph captured over
-    these calls replays with what ``update`` last put there; the batch has to
-    live as long as the graph may run."""
+    ``append`` and ``attend`` replays with what ``update`` last put there; the
+    batch has to live as long as the graph may run.  Making, ``reserve`` (or
+    the first ``attend`` with some heads, window and sinks), ``update`` and
+    ``check_errors`` stay outside of captures."""
 
     def __init__(self, cache: KVCache, page_table, kv_lens, q_lens=None, stream=None):
         self.cache, self.dev, self.L = cache, cache.dev, cache.L
