@@ -177,6 +177,8 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   const bool bf16 = a->dtype == EMMY_KV8_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (shape.tiles) rc = tiles_attend(p, *cache, shape, bf16, st);
+  p.beside = shape.tiles;
   if (rc == EMMY_OK && shape.rows) rc = rows_attend(p, *cache, shape, bf16, st);
+  if (rc == EMMY_OK && shape.tile_target > 0) rc = tiles_join(p, *cache, shape, bf16, st);
   return rc;
 }

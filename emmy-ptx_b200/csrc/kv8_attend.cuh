@@ -49,6 +49,7 @@ struct AttendParams {
   int row_limit;     // sequences with more rows of a kv head than this are the tile kernel's
   int nt;            // 8-row blocks of the row kernel
   int cluster;       // CTAs of a cluster of the row kernel, 0: none
+  bool beside;       // the row kernel was launched to run beside the tile kernel
 };
 
 // How large a plan gets and what it aims at, from what the host knows.
@@ -172,6 +173,7 @@ inline int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
 int plan_attend(const AttendParams &p, const PlanShape &shape, cudaStream_t stream);
 int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream);
+int tiles_join(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream);
 int rows_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream);
 
 }  // namespace kv8

@@ -294,8 +294,7 @@ __device__ __forceinline__ int query_row(uint32_t (&f)[D / 8], const T *row, int
 
 // Shared memory: first the joined rows of the four warps, over the staged queries.
 template <int D, int NT, bool CLUSTER, typename T>
-__global__ void __launch_bounds__(THREADS, ROWS_PER_SM)
-rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map) {
+__device__ __forceinline__ void attend_part(const AttendParams &p, const CUtensorMap &codes_map) {
   using L = Layout<D, NT>;
   constexpr int ROWS = 8 * NT, LD = L::LD;
   extern __shared__ uint8_t dyn_raw[];
@@ -310,10 +309,12 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
   volatile unsigned *const stop = &stop_word;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gr = lane >> 2, q = lane & 3;
   const Seqs &s = p.s;
-  grid_dependency_wait();
   const PlanHead head = *p.plan;
   const PartRec rec = p.parts[blockIdx.x];
-  grid_dependency_done();
+  // (the block that waits in the end lets the next kernel start after that only:
+  // its CTAs would take SMs in the order that these leave them, 257 for 248 us a
+  // batch of prompts)
+  if (!p.beside || blockIdx.x != 0) grid_dependency_done();
   if (blockIdx.x >= head.parts || !plan_fits(p, head, rec.b, rec.start, rec.n, rec.len)) return;
   const Segment g = {rec.b, rec.head, rec.start, rec.n, rec.len, rec.row0, rec.rows, rec.part, rec.parts, rec.slot0,
                      Span(p, rec.len - rec.n, rec.len - 1)};
@@ -699,6 +700,20 @@ rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map)
   gather(lead, count, 1, groups == 1);
   if (groups == 1 || !last_of(0, 1, groups)) return;
   gather(0, groups, group, true);
+}
+
+// Beside the tile kernel, which was launched before it and whose sequences are
+// others, it starts when all of that kernel's CTAs run: what they waited for is
+// done then, so nothing is read early, and SMs without a unit, or past their
+// last, take parts (512 tokens behind 3584 keys with 47 single tokens of
+// 700-8191 keys: 175 -> 131 us a call).  One block waits for that kernel in the
+// end, so that what comes after this kernel comes after both.
+template <int D, int NT, bool CLUSTER, typename T>
+__global__ void __launch_bounds__(THREADS, ROWS_PER_SM)
+rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map) {
+  if (!p.beside) grid_dependency_wait();
+  attend_part<D, NT, CLUSTER, T>(p, codes_map);
+  if (p.beside && blockIdx.x == 0) grid_dependency_wait();
 }
 
 template <int D, int NT, bool CLUSTER, typename T>

@@ -818,14 +818,16 @@ __global__ void __launch_bounds__(2 * TILE) join_kernel(const AttendParams p) {
 template <int D, typename T>
 int launch(const AttendParams &p, int device, const PlanShape &shape, cudaStream_t stream) {
   static KernelSetup setup;
-  int rc = setup.ready("emmy_kv8_attend", tiles_kernel<D, T>, device, Layout<D>::DYN, REGS_LAUNCH);
-  if (rc == EMMY_OK)
-    rc = launch_kernel("emmy_kv8_attend", tiles_kernel<D, T>, dim3(unsigned(std::min<int64_t>(shape.most_units, sm_count(device)))), THREADS,
-                       Layout<D>::DYN, stream, p);
-  if (rc == EMMY_OK && shape.tile_target > 0)
-    rc = launch_kernel("emmy_kv8_attend", join_kernel<D, T>, dim3(unsigned(shape.most_joins), D / 8), 2 * TILE, 0,
+  const int rc = setup.ready("emmy_kv8_attend", tiles_kernel<D, T>, device, Layout<D>::DYN, REGS_LAUNCH);
+  if (rc != EMMY_OK) return rc;
+  return launch_kernel("emmy_kv8_attend", tiles_kernel<D, T>,
+                       dim3(unsigned(std::min<int64_t>(shape.most_units, sm_count(device)))), THREADS, Layout<D>::DYN,
                        stream, p);
-  return rc;
+}
+template <int D, typename T>
+int launch_join(const AttendParams &p, const PlanShape &shape, cudaStream_t stream) {
+  return launch_kernel("emmy_kv8_attend", join_kernel<D, T>, dim3(unsigned(shape.most_joins), D / 8), 2 * TILE, 0,
+                       stream, p);
 }
 
 }  // namespace
@@ -835,6 +837,12 @@ int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &
   if (cache.head_dim == 64)
     return bf16 ? launch<64, __nv_bfloat16>(p, dev, shape, stream) : launch<64, __half>(p, dev, shape, stream);
   return bf16 ? launch<128, __nv_bfloat16>(p, dev, shape, stream) : launch<128, __half>(p, dev, shape, stream);
+}
+
+int tiles_join(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream) {
+  if (cache.head_dim == 64)
+    return bf16 ? launch_join<64, __nv_bfloat16>(p, shape, stream) : launch_join<64, __half>(p, shape, stream);
+  return bf16 ? launch_join<128, __nv_bfloat16>(p, shape, stream) : launch_join<128, __half>(p, shape, stream);
 }
 
 }  // namespace kv8

@@ -433,3 +433,32 @@ def test_many_units_of_one_and_two_tiles(D, window, sinks):
     batch.attend(0, q, out, window=window, sinks=sinks, stream=0)
     torch.cuda.synchronize()
     assert torch.equal(out.view(torch.int16), first.view(torch.int16))
+
+
+@pytest.mark.parametrize("prompts,singles", [([700, 90], 40), ([33], 3), ([1500], 300)])
+def test_prompts_beside_single_tokens_and_what_follows(prompts, singles):
+    """Both kernels of a call run at once; what is queued after it (copies over
+    every page it reads, at once, and a write to q) still comes after both."""
+    rng = np.random.default_rng(24)
+    ql = prompts + [1] * singles
+    kv = [n + int(rng.integers(0, 300)) for n in prompts] + rng.integers(1, 1200, singles).tolist()
+    used = sum(-(-n // 64) for n in kv)
+    cache, codes, exps, table, q = make(rng, kv, ql, extra=used + 2)
+    pages = sorted({int(table[b, i]) for b, n in enumerate(kv) for i in range(-(-n // 64))})
+    spare = [p for p in range(cache.pages) if p not in set(pages)][:len(pages)]
+    st = torch.cuda.current_stream()
+    batch, out = cache.batch(table, kv, ql, stream=st), torch.empty_like(q)
+    batch.attend(0, q, out, stream=st)
+    batch.check_errors(stream=st)
+    assert right(out, codes, exps, table, kv, ql, q)
+    want, kept, q0 = out.clone(), [x.clone() for x in cache._storage], q.clone()
+    for _ in range(10):
+        for x, y in zip(cache._storage, kept):
+            x.copy_(y)
+        q.copy_(q0)
+        out.zero_()
+        batch.attend(0, q, out, stream=st)
+        cache.copy_pages(spare[:len(pages)], pages, stream=st)
+        q.zero_()
+        assert torch.equal(out, want)
+    batch.check_errors(stream=st)
