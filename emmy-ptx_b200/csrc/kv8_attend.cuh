@@ -168,6 +168,7 @@ __device__ __forceinline__ int row_exponent(float amax) {
 constexpr int ROWS_MOST = 32, ROWS_BLOCK = 16;
 constexpr int ROWS_PER_SM = 3;  // CTAs of the row kernel, by its launch bounds
 constexpr int TILE_ROWS = 256;  // rows of a unit of the tile kernel
+constexpr int TILE_CUT = 8;     // chunks of a unit's part at least: a cut has to be worth its join
 // 8-row blocks of a CTA of the row kernel, for the rows of the largest sequence.
 inline int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 

@@ -199,10 +199,10 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   atomicMax(&most, top);
   atomicAdd(&sum, all_chunks);
   __syncthreads();
-  // chunks a part; a cut has to be worth its join
+  // chunks a part
   const int limit = p.tile_target == 0 || n_units >= p.tile_target
                         ? most
-                        : max(8, int((sum + p.tile_target - 1) / p.tile_target));
+                        : max(TILE_CUT, int((sum + p.tile_target - 1) / p.tile_target));
   const auto step_of = [&](int c) { return int(int64_t(most - c) * STEPS / (most + 1)); };
   const auto longest = [&](int c, int k) { return (c + k - 1) / k; };
   for (int i = tid; i < n_units; i += THREADS) {
