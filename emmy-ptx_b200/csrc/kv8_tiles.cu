@@ -60,6 +60,11 @@ struct Layout {
   // there leave shared memory's bandwidth to the keys (193 -> 189 us a prompt of
   // 8191 tokens with a window of 512).
   static constexpr bool Q_TMEM = D == 64;
+  // Rows that lanes hold each one of, read or written 64 bytes at a time by four
+  // lanes.  d = 128: read so 242 us a batch of prompts (250 each lane its own),
+  // written so, too, 243 and 0.6 us more for a short prompt; d = 64, 8191 tokens
+  // with a window: written so 186 us (190), read so 197.
+  static constexpr bool READ4 = D == 128, WRITE4 = D == 64;
   static constexpr int Q_TILE = Q_TMEM ? 0 : TILE * D * 2, KV = CHUNK * D * 2;  // bytes
   static constexpr int STAGE0 = 2 * Q_TILE;
   static constexpr int RAW0 = STAGE0 + STAGES * 2 * KV;    // K codes, then V codes
@@ -136,6 +141,24 @@ template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Four lanes' 16-byte pieces, transposed: piece i of lane j <-> piece j of lane i.
+// Threads that hold a row each then read and write 64 bytes of a row together.
+__device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
+#pragma unroll
+  for (int bit = 1; bit <= 2; bit <<= 1) {
+    const bool up = (lane & bit) != 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int a = bit == 1 ? 2 * i : i, b = a + bit;
+      uint32_t *x = &w[a].x, *y = &w[b].x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? x[j] : y[j], bit);
+        (up ? x[j] : y[j]) = got;
+      }
+    }
+  }
+}
 // Exponent of a normal f32 above 0, least -126.
 __device__ __forceinline__ int ilogb_f32(float x) { return max(int(__float_as_uint(x) >> 23) - 127, -126); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -512,11 +535,21 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
     // them; returns the factor of the row's scores.  The products that read the
     // rows before are done: their scores were here.
     const auto put_query = [&](const Unit &u, const Row &row) {
-      const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) +
-                                                         (int64_t(u.start) + row.token) * p.q_ts + row.head * p.q_hs);
+      const int64_t mine = (int64_t(u.start) + row.token) * p.q_ts + row.head * p.q_hs;
+      const T *const q = static_cast<const T *>(p.q);
       uint4 w[D / 8];
+      if constexpr (L::READ4) {
+        const T *src[4];
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) w[i] = src[i];
+        for (int i = 0; i < 4; ++i) src[i] = q + __shfl_sync(0xffffffffu, mine, (lane & ~3) | i) + 8 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) w[i] = *reinterpret_cast<const uint4 *>(src[i % 4] + i / 4 * 32);
+#pragma unroll
+        for (int i = 0; i < D / 8; i += 4) transpose4(*reinterpret_cast<uint4(*)[4]>(&w[i]), lane);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) w[i] = *reinterpret_cast<const uint4 *>(q + mine + 8 * i);
+      }
       float amax = 0.0f;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
@@ -704,7 +737,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
       u = Unit(p, p.units[i]);
       at = row_of(u);
       const int slot = u.slot;
-      T *const out = static_cast<T *>(p.out) + (int64_t(u.start) + at.token) * p.o_ts + at.head * p.o_hs;
+      const int64_t to = (int64_t(u.start) + at.token) * p.o_ts + at.head * p.o_hs;
       before += chunks;
       more = next_unit(++k, before, u);
       if (more) {
@@ -715,6 +748,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
       if (!ok) break;
       {
         tc_after();
+        const uint32_t reals = __ballot_sync(0xffffffffu, real);
+        T *out[4];  // this lane's pieces: of four lanes' rows, or of its own
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          out[i] = static_cast<T *>(p.out) +
+                   (L::WRITE4 ? __shfl_sync(0xffffffffu, to, (lane & ~3) | i) + 8 * (lane & 3) : to + 8 * i);
         const float by = slot >= 0 ? pow2(unit) : l == 0.0f ? 0.0f : pow2(unit) / l;
         float *const part = p.tile_partial + int64_t(slot) * (D + 2) * (2 * TILE) + x * TILE + r;
         const uint32_t *bits = reinterpret_cast<const uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8));
@@ -732,16 +771,19 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
             // a part: O, and below its maximum and sum, a column of 256 rows each
 #pragma unroll
             for (int i = 0; i < 32; ++i) __stcg(&part[(c + i) * (2 * TILE)], __uint_as_float(o[i]) * by);
-          } else if (real) {
+          } else {
+            uint4 w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              uint4 w;
-              w.x = pack2<T>(__uint_as_float(o[8 * i]) * by, __uint_as_float(o[8 * i + 1]) * by);
-              w.y = pack2<T>(__uint_as_float(o[8 * i + 2]) * by, __uint_as_float(o[8 * i + 3]) * by);
-              w.z = pack2<T>(__uint_as_float(o[8 * i + 4]) * by, __uint_as_float(o[8 * i + 5]) * by);
-              w.w = pack2<T>(__uint_as_float(o[8 * i + 6]) * by, __uint_as_float(o[8 * i + 7]) * by);
-              *reinterpret_cast<uint4 *>(out + c + 8 * i) = w;
+              w[i].x = pack2<T>(__uint_as_float(o[8 * i]) * by, __uint_as_float(o[8 * i + 1]) * by);
+              w[i].y = pack2<T>(__uint_as_float(o[8 * i + 2]) * by, __uint_as_float(o[8 * i + 3]) * by);
+              w[i].z = pack2<T>(__uint_as_float(o[8 * i + 4]) * by, __uint_as_float(o[8 * i + 5]) * by);
+              w[i].w = pack2<T>(__uint_as_float(o[8 * i + 6]) * by, __uint_as_float(o[8 * i + 7]) * by);
             }
+            if constexpr (L::WRITE4) transpose4(w, lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (reals >> (L::WRITE4 ? (lane & ~3) | i : lane) & 1) *reinterpret_cast<uint4 *>(out[i] + c) = w[i];
           }
         }
         if (slot >= 0) {
