@@ -47,9 +47,10 @@ constexpr int REGS_LAUNCH = 128, REGS_ISSUE = 80, REGS_SOFTMAX = 168, REGS_LOAD 
 static_assert(REGS_ISSUE + 2 * REGS_SOFTMAX + REGS_LOAD == 4 * REGS_LAUNCH, "register split");
 constexpr float LAZY = 8.0f, LEAST = 1e-37f;
 // Weights are 2^(s rm - m) with one rounding of the difference, m = round(max s
-// rm): the two differ by up to 2^-25 |m|, a factor common to the row, which
-// stays in range up to this |m|.  Beyond it f32 scores are whole multiples of
-// 16 and more, and the factor rm is made a power of two, so that m is exact.
+// rm): the two differ by up to 2^-24 |m|, a factor common to the row, which
+// stays in f16's range up to this |m|.  Beyond it f32 scores are whole multiples
+// of 16 and more, and s rm is rounded first, as m was, so that the largest
+// weight is 1.
 constexpr float HUGE_SCORE = 134217728.0f;
 constexpr int UNIT_LAZY = 6;
 constexpr int Q_COL = 4 * CHUNK + 2 * 64;  // TMEM column of the query rows, d = 64 only
@@ -159,8 +160,6 @@ __device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
     }
   }
 }
-// Exponent of a normal f32 above 0, least -126.
-__device__ __forceinline__ int ilogb_f32(float x) { return max(int(__float_as_uint(x) >> 23) - 127, -126); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -677,13 +676,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         const bool fix = __any_sync(0xffffffffu, best > m + LAZY || move);
         float alpha = 1.0f;
         if (fix) {
-          float to = fmaxf(m, best);
-          if (fabsf(to) > HUGE_SCORE && m != to) {
-            // (rare) a power of two from here on: products are exact
-            mult = pow2(ilogb_f32(mult));
-            rm = fmaxf(mult * sc.x, LEAST);
-            to = fmaxf(m, raw * rm);
-          }
+          const float to = fmaxf(m, best);
           alpha = exp2_fast(m - to);
           m = to;
           l *= alpha;
@@ -692,6 +685,11 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
           if (move || big) {
             alpha *= pow2(unit - ev);
             unit = ev;
+          }
+          if (__any_sync(0xffffffffu, fabsf(m) > HUGE_SCORE && m != NONE)) {  // (rare)
+#pragma unroll
+            for (int i = 0; i < 64; ++i) sv[i / 32][i % 32] = __float_as_uint(score(i) * rm);
+            rm = 1.0f;
           }
         }
         const float shift = float(ev - unit) - m;

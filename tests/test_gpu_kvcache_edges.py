@@ -1,0 +1,80 @@
+"""The paged 8-bit cache where its arithmetic ends: scores past f32's whole
+numbers."""
+
+import numpy as np
+import pytest
+
+from tests import kv8_oracle as ref
+from tests.test_gpu_kvcache import attend_gpu, gpu  # noqa: F401 - a fixture
+
+pytestmark = pytest.mark.gpu
+
+
+def filled(pages, D, keys, values, P=64):
+    """Codes and exponents of one head whose key j is keys[j] (code, exponent)
+    in its first element, zeros elsewhere, and whose value j is values[j]
+    (element, number that e4m3 holds); a page has one exponent for its keys."""
+    codes, exps = np.zeros((pages, 2, 1, P, D), np.uint8), np.zeros((pages, 2, 1), np.int8)
+    for j, (number, e) in keys.items():
+        codes[j // P, 0, 0, j % P, 0] = ref.encode(number)
+        exps[j // P, 0, 0] = e
+    for j, (d, number) in values.items():
+        codes[j // P, 1, 0, j % P, d] = ref.encode(number)
+    return codes, exps
+
+
+def log2_score(D, scale, q, number, e):
+    return (D ** -0.5 if scale is None else scale) * np.log2(np.e) * q * number * 2.0 ** e
+
+
+# K of the two keys in units of 2^6: scores below and above 2^27, whose ratio is
+# less than the scale's over its power of two
+@pytest.mark.parametrize("D,scale,small,large", [(64, None, 352, 384), (128, 0.17, 256, 288)])
+@pytest.mark.parametrize("first", ["small", "large"])
+@pytest.mark.parametrize("L,n,at", [
+    (200, 100, (5, 70)),            # one unit, two of its chunks
+    (3000, 40, (130, 2500)),        # two parts of a unit cut along its keys
+    (300, 1, (5, 150)),             # the row kernel
+])
+def test_a_maximum_that_crosses_whole_numbers(gpu, D, scale, small, large, first, L, n, at):  # noqa: F811
+    """Of two keys with scores of 2^27 and less and of 2^27 and more, 10^7
+    apart, the larger takes all: the output is its value, exactly."""
+    q = 2.0 ** 15
+    a, b = (log2_score(D, scale, q, k, 6) for k in (small, large))
+    assert 1.2e8 < a < 2.0 ** 27 < b < 1.6e8 and b - a > 1e7
+    keys = {at[0]: (small, 6), at[1]: (large, 6)} if first == "small" else {at[0]: (large, 6), at[1]: (small, 6)}
+    winner = at[1] if first == "small" else at[0]
+    values = {j: (0, 2.0 if j == winner else 1.0) for j in at}
+    pages = -(-L // 64)
+    codes, exps = filled(pages, D, keys, values)
+    rows = np.zeros((n, 1, D), np.float16)
+    rows[:, :, 0] = q
+    got = attend_gpu(gpu, codes, exps, np.arange(pages, dtype=np.int32)[None], [L], [n], rows, "f16", scale=scale)
+    assert (got[:, 0, 0] == 2.0).all() and not got[:, 0, 1:].any()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("L,n,low,at", [
+    (200, 100, range(64), (70, 90)),                    # a first chunk far below the next
+    (3000, 40, range(64, 3000), (10, 20)),              # later parts of a cut unit far below the first
+    (200, 2, range(64), (70, 90)),
+])
+def test_scores_far_below_the_others(gpu, D, L, n, low, at):  # noqa: F811
+    """Chunks of scores of -1.4e8 leave the weights of two ordinary keys as
+    they are: exp(s0 - s1) over their sum."""
+    q = 2.0 ** 15
+    keys = {j: (-256.0 if (j // 64) * 64 in low else -448.0, 7 if (j // 64) * 64 in low else -12) for j in range(L)}
+    keys[at[0]], keys[at[1]] = (10.0, -12), (11.0, -12)
+    assert log2_score(D, 0.125, q, -256.0, 7) < -2.0 ** 27
+    pages = -(-L // 64)
+    codes, exps = filled(pages, D, keys, {at[0]: (0, 1.0), at[1]: (1, 1.0)})
+    rows = np.zeros((n, 1, D), np.float16)
+    rows[:, :, 0] = q
+    got = attend_gpu(gpu, codes, exps, np.arange(pages, dtype=np.int32)[None], [L], [n], rows, "f16", scale=0.125)
+    w = np.exp(-0.125 * q * 2.0 ** -12)
+    want = np.zeros(D)
+    want[:2] = w / (1 + w), 1 / (1 + w)
+    # the other keys' weights are below 2^-600; weights and output are f16, and a
+    # score of 16 in log2 units is rounded by 2^-20 at most, which moves a weight by ln 2 of that
+    tol = want * (2 * 2.0 ** -11 + 2.0 ** -18)
+    assert (np.abs(got[:, 0].astype(float) - want) <= tol).all()
