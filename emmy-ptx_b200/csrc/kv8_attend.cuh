@@ -144,7 +144,9 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 // Maxima beyond this (log2 units) leave no room in f32 for the exponents that are
 // added to them elsewhere: V's unit is then kept at the page's own exponent.
 constexpr float BIG = 65536.0f;
-constexpr float NONE = -1e30f;  // the maximum of a row that has seen no key
+// The maximum of a row that has seen no key: f32's lowest, below every score but
+// -inf.  (Not -inf: hidden scores are that, and -inf - -inf is NaN.)
+constexpr float NONE = -3.402823466e38f;
 __device__ __forceinline__ bool is_big(float m) { return fabsf(m) > BIG && m != NONE; }
 
 // 2^x: subnormal results are zero, 2^-inf = 0.

@@ -1,6 +1,7 @@
 """The paged 8-bit cache where its arithmetic ends: scores past f32's whole
-numbers."""
+numbers and near the end of its range."""
 
+import ml_dtypes
 import numpy as np
 import pytest
 
@@ -78,3 +79,25 @@ def test_scores_far_below_the_others(gpu, D, L, n, low, at):  # noqa: F811
     # score of 16 in log2 units is rounded by 2^-20 at most, which moves a weight by ln 2 of that
     tol = want * (2 * 2.0 ** -11 + 2.0 ** -18)
     assert (np.abs(got[:, 0].astype(float) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("window", [1, 2])
+def test_scores_near_the_end_of_f32(gpu, n, window):  # noqa: F811
+    """Every visible key has a score of -2^105 and less, far below -1e30: a
+    row that sees one key is its value, one that sees two the larger's."""
+    D, L, q = 64, 130, 2.0 ** 90
+    rng = np.random.default_rng(4)
+    pages = 3
+    codes, exps = filled(pages, D, {j: (-448.0 if j % 2 else -224.0, 10) for j in range(L)}, {})
+    codes[:, 1, 0] = ref.encode(rng.standard_normal((pages, 64, D)) * 10)
+    assert -3.4e38 < log2_score(D, None, q, -448.0, 10) < log2_score(D, None, q, -224.0, 10) < -1e31
+    rows = np.zeros((n, 1, D), ml_dtypes.bfloat16)
+    rows[:, :, 0] = q
+    table = np.arange(pages, dtype=np.int32)[None]
+    got = attend_gpu(gpu, codes, exps, table, [L], [n], rows, "bf16", window=window)
+    _, v = ref.held(codes, exps, table, 0, L, 0)
+    for i in range(n):
+        p = L - n + i
+        key = p if window == 1 or p % 2 == 0 else p - 1
+        assert (got[i, 0].astype(float) == v[key]).all()       # e4m3 is exact in bf16
