@@ -168,6 +168,8 @@ int check_counts(const char *what, const emmy_kv8 *c);  // of the sequences, wit
 int check_seqs(const char *what, const emmy_kv8 *c);
 Seqs seqs_of(const emmy_kv8 &c);
 int sm_count(int device);
+// Limit of the kernels' waits, in ns, and the blocks that are to wait in vain.
+void wait_limit(unsigned long long &ns, int &stall);
 // Whether [a, a + na) and [b, b + nb) share a byte.
 inline bool overlap(emmy_dptr a, uint64_t na, emmy_dptr b, uint64_t nb) {
   return a < b + nb && b < a + na;

@@ -7,7 +7,7 @@
 
 namespace kv8 {
 
-constexpr unsigned long long WAIT_NS = 2000000000ull;
+constexpr unsigned long long WAIT_NS = EMMY_KV8_WAIT_NS;
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -34,16 +34,16 @@ __device__ __forceinline__ unsigned long long now_ns() {
   return t;
 }
 // Waits with a whole warp, which stays converged, for the phase of parity
-// `parity`; false when the kernel gives up.
+// `parity`; false when the kernel gives up, after `limit` ns.
 __device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, volatile unsigned *stop,
-                                          unsigned *status) {
+                                          unsigned *status, unsigned long long limit) {
   const uint32_t at = smem_addr(b);
   if (__all_sync(0xffffffffu, bar_try(at, parity))) return true;
   const unsigned long long t0 = now_ns();
   for (;;) {
     if (__all_sync(0xffffffffu, bar_try(at, parity))) return true;
     bool over = *stop != 0;
-    if (now_ns() - t0 > WAIT_NS) {
+    if (now_ns() - t0 > limit) {
       *stop = 1;
       report(status, STATUS_WAIT);
       over = true;

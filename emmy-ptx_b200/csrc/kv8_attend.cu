@@ -174,6 +174,7 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   p.partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO);
   p.tile_partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO + shape.partial_bytes);
   p.scale_log2 = scale_log2;
+  wait_limit(p.wait_ns, p.stall);
   const OnDevice on(cache->device);
   if (on.err != cudaSuccess) return cuda_fail(what, on.err);
   const bool bf16 = a->dtype == EMMY_KV8_BF16;

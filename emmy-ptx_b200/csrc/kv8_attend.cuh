@@ -43,6 +43,8 @@ struct AttendParams {
   PartRec *parts;
   UnitRec *units;
   JoinRec *joins;
+  unsigned long long wait_ns;  // limit of the kernels' waits
+  int stall;                   // one block in so many withholds its first keys (0: none)
   float scale_log2;  // scale * log2(e)
   int group;         // query heads of a kv head
   int window, sinks;

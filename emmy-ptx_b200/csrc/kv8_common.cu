@@ -76,7 +76,21 @@ int sm_count(int device) {
   return n;
 }
 
+static std::atomic<uint64_t> g_wait_limit{EMMY_KV8_WAIT_NS};
+static std::atomic<int32_t> g_stall{0};
+void wait_limit(unsigned long long &ns, int &stall) {
+  ns = g_wait_limit.load(std::memory_order_relaxed);
+  stall = g_stall.load(std::memory_order_relaxed);
+}
+
 }  // namespace kv8
+
+extern "C" int emmy_kv8_wait_limit(uint64_t ns, int32_t stall) {
+  if (stall < 0) return kv8::fail(EMMY_EINVAL, "emmy_kv8_wait_limit", "stall must not be negative");
+  kv8::g_stall.store(stall, std::memory_order_relaxed);
+  kv8::g_wait_limit.store(ns, std::memory_order_relaxed);
+  return EMMY_OK;
+}
 
 extern "C" int emmy_stream_capturing(emmy_stream stream, int *capturing) {
   if (capturing == nullptr) return kv8::fail(EMMY_EINVAL, "emmy_stream_capturing", "null result");

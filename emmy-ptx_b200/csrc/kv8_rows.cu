@@ -356,7 +356,7 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
     const uint32_t who = elected();
     const int *table = s.table + int64_t(g.b) * s.width;
     Ring ring;
-    bool ok = true;
+    bool ok = true, stalled = p.stall > 0 && blockIdx.x % p.stall == 0;
     for (int base = c0; ok && base < c1; base += 32) {
       ChunkInfo mine = {0, 0, 0, 0};
       int64_t unit = 0;
@@ -390,7 +390,7 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
       for (int i = 0; i < early; ++i) copy(i, i);
       for (int i = 0; i < count; ++i, ring.next(L::STAGES)) {
         if (i >= early) {
-          ok = warp_wait(&empty[ring.slot], ring.phase ^ 1, stop, s.status);
+          ok = warp_wait(&empty[ring.slot], ring.phase ^ 1, stop, s.status, p.wait_ns);
           if (!ok) break;
           copy(i, ring.slot);
         }
@@ -401,8 +401,9 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
         c.dead = __shfl_sync(0xffffffffu, mine.dead, i);
         if (who) {
           infos[ring.slot] = c;
-          bar_arrive(&full[ring.slot]);
+          if (!stalled) bar_arrive(&full[ring.slot]);
         }
+        stalled = false;
       }
     }
   } else {
@@ -449,7 +450,7 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
     // ---- 16 keys of each chunk a warp ----
     Ring ring;
     for (int chunk = c0; chunk < c1; ++chunk, ring.next(L::STAGES)) {
-      if (!warp_wait(&full[ring.slot], ring.phase, stop, s.status)) break;
+      if (!warp_wait(&full[ring.slot], ring.phase, stop, s.status, p.wait_ns)) break;
       const uint8_t *rows = dyn + ring.slot * L::CHUNK + 16 * warp * D;
       const ChunkInfo info = infos[ring.slot];
       // S^T = K Q^T, in two chains of sums
@@ -503,11 +504,12 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
   // ---- join the warps ----
   __syncthreads();
   if (*stop != 0) {
-    // given up: copies in flight land before the block may end (50 ms)
+    // given up: copies in flight land first (50 ms).  The block then goes on: a
+    // cluster's others read its shared memory, and the parts of a segment count
+    // each other in the workspace, whose counters go back to zero only if all come.
     const unsigned long long t0 = now_ns();
     while (now_ns() - t0 < 50000000ull) {
     }
-    if (!CLUSTER) return;  // a cluster's blocks stay until all have read
   }
   // Value gr D / 8 + 2 j + e of a row lies at 16 j + 2 gr + e: the lanes that
   // store together (gr and 8 q) then meet in no bank.

@@ -313,12 +313,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
     Unit u;
     for (int k = 0; ok && load_unit(k, u); ++k)
       for (int g = 0; ok && g < u.chunks; ++g, kv.next(STAGES)) {
-        ok = warp_wait(&bars.kv_full[kv.slot], kv.phase, stop, s.status);
+        ok = warp_wait(&bars.kv_full[kv.slot], kv.phase, stop, s.status, p.wait_ns);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (!ok || x >= u.tiles) break;
           const int buf = n[x] & 1;
-          ok = warp_wait(&bars.p_full[x][buf], n[x] >> 1 & 1, stop, s.status);
+          ok = warp_wait(&bars.p_full[x][buf], n[x] >> 1 & 1, stop, s.status, p.wait_ns);
           if (!ok) break;
           ++n[x];
           tc_after();
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
     // ---- bulk copies: K and V of a page's chunk are one contiguous piece
     // each; 32 chunks' pages and exponents are read at once, a lane a chunk ----
     const uint32_t who = elected();
-    bool ok = true;
+    bool ok = p.stall == 0 || blockIdx.x % p.stall != 0;
     int so_far = 0;
     Ring copied;
     Unit u;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(q + D - 8));
       }
       for (int g = 0; g < u.chunks; ++g, ++so_far) {
-        if (so_far >= RAW) ok = warp_wait(&bars.raw_empty[copied.slot], copied.phase ^ 1, stop, s.status);
+        if (so_far >= RAW) ok = warp_wait(&bars.raw_empty[copied.slot], copied.phase ^ 1, stop, s.status, p.wait_ns);
         if (!ok) break;
         fetch(g);
       }
@@ -407,14 +407,14 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
     int n = 0, mine = 0;  // chunks and units of this tile so far
     Unit u;
     for (int k = 0; ok && load_unit(k, u); ++k) {
-      if (x < u.tiles) ok = warp_wait(&bars.q_full[x], mine++ & 1, stop, s.status);
+      if (x < u.tiles) ok = warp_wait(&bars.q_full[x], mine++ & 1, stop, s.status, p.wait_ns);
       for (int g = 0; ok && g < u.chunks; ++g, kv.next(STAGES)) {
-        ok = warp_wait(&bars.kv_full[kv.slot], kv.phase, stop, s.status);
+        ok = warp_wait(&bars.kv_full[kv.slot], kv.phase, stop, s.status, p.wait_ns);
         if (x == 1 && who) bar_arrive(&bars.kv_empty[kv.slot]);
         if (x >= u.tiles) continue;
         const int buf = n & 1;
         // the buffer holds P of chunk n - 2 until its P V is done
-        if (ok && n >= 2) ok = warp_wait(&bars.pv_done[x][buf], (n >> 1 & 1) ^ 1, stop, s.status);
+        if (ok && n >= 2) ok = warp_wait(&bars.pv_done[x][buf], (n >> 1 & 1) ^ 1, stop, s.status, p.wait_ns);
         if (!ok) break;
         ++n;
         tc_after();
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
     Unit u;
     for (int k = 0; ok && load_unit(k, u); ++k)
       for (int g = 0; g < u.chunks; ++g, ++c, raw.next(RAW), kv.next(STAGES)) {
-        ok = warp_wait(&bars.raw_full[raw.slot], raw.phase, stop, s.status);
+        ok = warp_wait(&bars.raw_full[raw.slot], raw.phase, stop, s.status, p.wait_ns);
         if (!ok) break;
         const uint8_t *src = dyn + L::RAW0 + raw.slot * L::KV + from;
         uint4 k[PASSES], v[PASSES];
@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         const ChunkInfo info = raw_info[raw.slot];
         warp_arrive(&bars.raw_empty[raw.slot]);
         const int st = kv.slot;
-        if (c >= STAGES) ok = warp_wait(&bars.kv_empty[st], kv.phase ^ 1, stop, s.status);
+        if (c >= STAGES) ok = warp_wait(&bars.kv_empty[st], kv.phase ^ 1, stop, s.status, p.wait_ns);
         if (!ok) break;
         // chunks some row does not see whole: values no row sees are zeroed and
         // a NaN is taken out here (0 * NaN would reach rows it is hidden from)
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
       }
       for (int g = 0; g < chunks; ++g, ++n) {
         const int buf = n & 1;
-        ok = warp_wait(&bars.s_full[x][buf], n >> 1 & 1, stop, s.status);
+        ok = warp_wait(&bars.s_full[x][buf], n >> 1 & 1, stop, s.status, p.wait_ns);
         if (!ok) break;
         if (g == 0 && x == 1) stagger();
         const int c = before + g;  // chunks of the CTA so far
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         tm_wait_st();
         if (fix && !first) {
           // P V of chunk n - 1 is the last to have touched O
-          ok = warp_wait(&bars.pv_done[x][(n - 1) & 1], (n - 1) >> 1 & 1, stop, s.status);
+          ok = warp_wait(&bars.pv_done[x][(n - 1) & 1], (n - 1) >> 1 & 1, stop, s.status, p.wait_ns);
           if (!ok) break;
           tc_after();
 #pragma unroll
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         at = row_of(u);
         mult = put_query(u, at);
       }
-      ok = warp_wait(&bars.pv_done[x][(n - 1) & 1], (n - 1) >> 1 & 1, stop, s.status);
+      ok = warp_wait(&bars.pv_done[x][(n - 1) & 1], (n - 1) >> 1 & 1, stop, s.status, p.wait_ns);
       if (!ok) break;
       {
         tc_after();

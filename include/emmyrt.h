@@ -265,6 +265,15 @@ int emmy_kv8_attend_sizes(const emmy_kv8 *cache, int32_t heads, uint64_t *worksp
 int emmy_kv8_attend_plan(const emmy_kv8 *cache, const emmy_kv8_attend_args *args, emmy_stream stream);
 int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args *args, emmy_stream stream);
 
+/* How long attend's kernels, launched from now on by this process, wait for a
+ * copy or a product of their own before they give up (default
+ * EMMY_KV8_WAIT_NS).  A call whose kernel gave up reports it in *status and
+ * leaves its rows of `out` undefined; its workspace is as after any call.
+ * `stall` is for tests: one block in `stall` withholds its first keys, so that
+ * its waits run out (0: none does). */
+enum { EMMY_KV8_WAIT_NS = 2000000000 };
+int emmy_kv8_wait_limit(uint64_t ns, int32_t stall);
+
 /* In each of `layers` layers, laid out one after another, copy page src[i]
  * with its exponents to page dst[i], i < n (host arrays, read during the
  * call; n at most EMMY_KV8_MAX_PAIRS).  No page may be in dst twice, or in
