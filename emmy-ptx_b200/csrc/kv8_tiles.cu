@@ -50,7 +50,7 @@ constexpr float LAZY = 8.0f, LEAST = 1e-37f;
 // rm): the two differ by up to 2^-24 |m|, a factor common to the row, which
 // stays in f16's range up to this |m|.  Beyond it f32 scores are whole multiples
 // of 16 and more, and s rm is rounded first, as m was, so that the largest
-// weight is 1.
+// weight is 1: the chunk's scores are replaced by the products in TMEM.
 constexpr float HUGE_SCORE = 134217728.0f;
 constexpr int UNIT_LAZY = 6;
 constexpr int Q_COL = 4 * CHUNK + 2 * 64;  // TMEM column of the query rows, d = 64 only
@@ -183,6 +183,16 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+__device__ __forceinline__ void tm_ld8(uint32_t (&r)[8], uint32_t at) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(at));
+}
+__device__ __forceinline__ void tm_st8(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -608,7 +618,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         *reinterpret_cast<uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8) + 4 * i) = 0;
       float m = NONE, l = 0.0f;
       int unit = 0;
-      bool nan_seen = false, big = false;
+      bool nan_seen = false, big = false, rounded = false;
       // chunks whole_lo .. whole_hi - 1 every row sees whole
       int whole_lo = 0, whole_hi = chunks;
       {
@@ -629,7 +639,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         const int c = before + g;  // chunks of the CTA so far
         const float2 sc = chunk_scale[c & 3];
         const int ev = int(sc.y);
-        float rm = fmaxf(mult * sc.x, LEAST);
+        const float rm = rounded ? 1.0f : fmaxf(mult * sc.x, LEAST);
         tc_after();
         uint32_t sv[2][32];
         tm_ld32(sv[0], s_at + buf * CHUNK);
@@ -677,6 +687,24 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         float alpha = 1.0f;
         if (fix) {
           const float to = fmaxf(m, best);
+          if (!rounded && __any_sync(0xffffffffu, fabsf(to) > HUGE_SCORE && to != NONE)) {
+            // (rare) this chunk again, from products rounded first.  A loop, and the
+            // scores' registers left alone: the same unrolled over them cost every
+            // call (a prompt of 8191 tokens with a window of 512: 198 for 186 us).
+#pragma unroll 1
+            for (int c = 0; c < CHUNK; c += 8) {
+              uint32_t w[8];
+              tm_ld8(w, s_at + buf * CHUNK + c);
+              tm_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * rm);
+              tm_st8(s_at + buf * CHUNK + c, w);
+            }
+            tm_wait_st();
+            rounded = true;
+            --g, --n;
+            continue;
+          }
           alpha = exp2_fast(m - to);
           m = to;
           l *= alpha;
@@ -685,11 +713,6 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
           if (move || big) {
             alpha *= pow2(unit - ev);
             unit = ev;
-          }
-          if (__any_sync(0xffffffffu, fabsf(m) > HUGE_SCORE && m != NONE)) {  // (rare)
-#pragma unroll
-            for (int i = 0; i < 64; ++i) sv[i / 32][i % 32] = __float_as_uint(score(i) * rm);
-            rm = 1.0f;
           }
         }
         const float shift = float(ev - unit) - m;
@@ -705,6 +728,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
           sum[i & 3] = add2(sum[i & 3], pair(a, b));
           pk[i] = pack2<__half>(a, b);
         }
+        rounded = false;
         tm_st32(s_at + buf * CHUNK, pk);
         float even, odd;
         unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), even, odd);
