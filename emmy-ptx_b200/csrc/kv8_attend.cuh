@@ -43,8 +43,6 @@ struct AttendParams {
   PartRec *parts;
   UnitRec *units;
   JoinRec *joins;
-  unsigned long long wait_ns;  // limit of the kernels' waits
-  int stall;                   // one block in so many withholds its first keys (0: none)
   float scale_log2;  // scale * log2(e)
   int group;         // query heads of a kv head
   int window, sinks;
@@ -52,6 +50,8 @@ struct AttendParams {
   int nt;            // 8-row blocks of the row kernel
   int cluster;       // CTAs of a cluster of the row kernel, 0: none
   bool beside;       // the row kernel was launched to run beside the tile kernel
+  int stall;         // one block in so many withholds its first keys (0: none)
+  unsigned long long wait_ns;  // limit of the kernels' waits
 };
 
 // How large a plan gets and what it aims at, from what the host knows.
