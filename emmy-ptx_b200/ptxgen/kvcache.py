@@ -172,7 +172,8 @@ class _Pool:
         return pool
 
     def __init__(self, dev: Device):
-        self.dev, self.held, self.bytes, self.lock = dev, {}, 0, threading.Lock()
+        self.dev, self.held, self.bytes = dev, {}, 0
+        self.lock = threading.RLock()   # a collection inside of it may close a batch
 
     def take(self, use: str, nbytes: int, stream: int) -> tuple[int, tuple]:
         """(address, key to give it back by) of a buffer for work on ``stream``."""
