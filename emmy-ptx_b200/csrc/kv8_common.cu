@@ -100,3 +100,12 @@ extern "C" int emmy_stream_capturing(emmy_stream stream, int *capturing) {
   *capturing = st != cudaStreamCaptureStatusNone;
   return EMMY_OK;
 }
+
+extern "C" int emmy_stream_id(emmy_stream stream, uint64_t *id) {
+  if (id == nullptr) return kv8::fail(EMMY_EINVAL, "emmy_stream_id", "null result");
+  unsigned long long word = 0;
+  const cudaError_t e = cudaStreamGetId(static_cast<cudaStream_t>(stream), &word);
+  if (e != cudaSuccess) return kv8::cuda_fail("emmy_stream_id", e);
+  *id = word;
+  return EMMY_OK;
+}

@@ -53,6 +53,7 @@ PAGE_SIZES = (64, 128, 256)
 MAX_SEQS = 4096
 MAX_PAIRS = 480            # pages a launch of copy_pages takes
 WORKSPACE_ZERO = 16384     # bytes of a workspace that start as zeros
+PER_THREAD = 2             # the per-thread default stream's handle
 
 STATUS = {0x401: "a page number outside the pool",
           0x402: "a sequence longer than its row of the table, or more new tokens than keys or rows",
@@ -129,6 +130,14 @@ def _stream_of(stream, dev: Device) -> int:
     return stream if isinstance(stream, int) else stream.value or 0
 
 
+def _stream_id(dev: Device, st: int) -> int:
+    """Of the stream itself: handles of destroyed streams come again, and
+    PER_THREAD is another stream in each thread."""
+    word = C.c_uint64()
+    check(dev.L.emmy_stream_id(st, C.byref(word)), "stream")
+    return word.value or st
+
+
 def _capturing(dev: Device, st: int) -> bool:
     word = C.c_int()
     check(dev.L.emmy_stream_capturing(st, C.byref(word)), "stream")
@@ -158,18 +167,16 @@ def _ints(x, name: str) -> np.ndarray:
 
 
 class _Pool:
-    """Buffers of closed batches on one device, by (use, bytes, the one stream
-    they were used on): the next batch on that stream takes them with no
-    wait.  Kept for the process, up to ``MOST`` bytes."""
+    """Buffers of closed batches on one device, by (use, bytes, the id of the
+    one stream they were used on): the next batch on that stream takes them
+    with no wait.  Kept for the process, up to ``MOST`` bytes; those of the
+    stream that was first kept go first."""
 
     MOST = 512 << 20
 
     @classmethod
     def of(cls, dev: Device) -> "_Pool":
-        pool = dev.__dict__.get("_kv_pool")
-        if pool is None:
-            pool = dev._kv_pool = cls(dev)
-        return pool
+        return dev.__dict__.get("_kv_pool") or dev.__dict__.setdefault("_kv_pool", cls(dev))
 
     def __init__(self, dev: Device):
         self.dev, self.held, self.bytes = dev, {}, 0
@@ -177,7 +184,7 @@ class _Pool:
 
     def take(self, use: str, nbytes: int, stream: int) -> tuple[int, tuple]:
         """(address, key to give it back by) of a buffer for work on ``stream``."""
-        key = (use, 1 << max(12, (nbytes - 1).bit_length()), stream)
+        key = (use, 1 << max(12, (nbytes - 1).bit_length()), _stream_id(self.dev, stream))
         with self.lock:
             held = self.held.get(key)
             if held:
@@ -189,12 +196,22 @@ class _Pool:
         return ptr, key
 
     def give(self, ptr: int, key: tuple, reuse: bool) -> None:
+        gone = [] if reuse else [ptr]
         with self.lock:
-            reuse = reuse and self.bytes + key[1] <= self.MOST
             if reuse:
-                self.held.setdefault(key, []).append(ptr)
-                self.bytes += key[1]
-        if not reuse:
+                for other in [k for k in self.held if k[2] != key[2]]:
+                    spare = self.held.get(other)
+                    while spare and self.bytes + key[1] > self.MOST:
+                        gone.append(spare.pop())
+                        self.bytes -= other[1]
+                    if not spare:
+                        self.held.pop(other, None)
+                if self.bytes + key[1] <= self.MOST:
+                    self.held.setdefault(key, []).append(ptr)
+                    self.bytes += key[1]
+                else:
+                    gone.append(ptr)
+        for ptr in gone:
             self.dev.free(ptr)          # waits for what still runs on it
 
 
@@ -317,7 +334,8 @@ class Batch:
     ``append`` and ``attend`` are the new tokens, sequence after sequence;
     rows behind the last one are left alone.  Calls of one batch share a
     workspace, so they must not overlap on the GPU: two captured graphs, or
-    two streams, that run at once need a batch each.  A graph captured over
+    two streams, that run at once need a batch each.  One made on the
+    per-thread default stream is for that thread and stream.  A graph captured over
     ``append`` and ``attend`` replays with what ``update`` last put there; the
     batch has to live as long as the graph may run.  Making, ``reserve`` (or
     the first ``attend`` with some heads, window and sinks), ``update`` and
@@ -343,6 +361,7 @@ class Batch:
         self._stream, self._reuse = _stream_of(stream, self.dev), True
         _outside_capture(self.dev, self._stream, "lengths and page numbers are copied from the host")
         self._pool = _Pool.of(self.dev)
+        self._who = self._same(self._stream)
         self._others: set[int] = set()             # further streams it was used on
         self._buf = self._take("batch", host.nbytes, self._stream)
         _copy_in(self.dev, self._buf, host, self._stream)
@@ -363,12 +382,19 @@ class Batch:
         self._held.append(held)
         return held[0]
 
+    def _same(self, st: int) -> int:
+        """What tells whether a handle means the stream that it did before."""
+        return st if st != PER_THREAD else _stream_id(self.dev, st)
+
     def _on(self, stream) -> int:
         """The handle of ``stream``; one other than the batch's own waits, the
         first time, for what is queued on that (its lengths, a page copy).
         One that is being captured cannot wait: its graph is replayed after."""
         st = _stream_of(stream, self.dev)
-        if st != self._stream and st not in self._others:
+        who = st if st != PER_THREAD else self._same(st)
+        if who != self._who and who not in self._others:
+            if self._stream == PER_THREAD:
+                raise EmmyError("a batch made on the per-thread default stream is for that thread and stream")
             self._reuse = False
             if _capturing(self.dev, st):
                 return st
@@ -378,7 +404,7 @@ class Batch:
                 check(self.L.emmy_stream_wait_event(st, ev), "stream wait event")
             finally:
                 self.L.emmy_event_destroy(ev)
-            self._others.add(st)
+            self._others.add(who)
         return st
 
     def _packed(self, table, kv_lens, q_lens) -> np.ndarray:

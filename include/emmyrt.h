@@ -154,6 +154,11 @@ int emmy_stream_wait_event(emmy_stream stream, emmy_event ev);
 /* Whether `stream` is being captured into a graph (no counterpart either). */
 int emmy_stream_capturing(emmy_stream stream, int *capturing);
 
+/* A number that no other stream of the process has, had or will have: a handle
+ * comes again once its stream is destroyed, and the per-thread default stream's
+ * means another stream in each thread (no counterpart either). */
+int emmy_stream_id(emmy_stream stream, uint64_t *id);
+
 /* ---- kernel error word ---- */
 /* Kernels that can fail (bounded waits that expire, index checks in the
  * checked build) write a nonzero code into the module global `emmy_err`

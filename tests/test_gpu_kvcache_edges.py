@@ -1,5 +1,7 @@
 """The paged 8-bit cache where its arithmetic ends: scores past f32's whole
-numbers and near the end of its range."""
+numbers and near the end of its range; streams that share a handle."""
+
+import threading
 
 import ml_dtypes
 import numpy as np
@@ -101,3 +103,40 @@ def test_scores_near_the_end_of_f32(gpu, n, window):  # noqa: F811
         p = L - n + i
         key = p if window == 1 or p % 2 == 0 else p - 1
         assert (got[i, 0].astype(float) == v[key]).all()       # e4m3 is exact in bf16
+
+
+def test_threads_on_their_default_streams():
+    """One handle, a stream for each thread: batches made and closed one after
+    another in each, with work still queued."""
+    torch = pytest.importorskip("torch")
+    from ptxgen import KVCache
+    rng = np.random.default_rng(5)
+    P, D, H, kv, ql = 64, 64, 1, [900, 70, 300], [1, 2, 1]
+    codes, exps = ref.pool(rng, 24, H, P, D)
+    table = ref.tables(rng, 24, kv, P)
+    c, e = torch.from_numpy(codes)[None].cuda(), torch.from_numpy(exps)[None].cuda()
+    cache = KVCache(24, H, D, storage=(c, e))
+    q = torch.from_numpy(rng.standard_normal((4, 2, D))).half().cuda()
+    outs, failed = [torch.zeros_like(q) for _ in range(4)], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            pick = [0, 1, 2] if i % 2 else [2, 0, 1]                    # unlike tables and lengths
+            rows = torch.cat([q[sum(ql[:b]):sum(ql[:b + 1])] for b in pick])
+            torch.cuda.synchronize()
+            for _ in range(20):
+                batch = cache.batch(table[pick], [kv[b] for b in pick], [ql[b] for b in pick], stream=2)
+                batch.attend(0, rows, outs[i], stream=2)
+                batch.close()
+            batch = cache.batch(table[pick], [kv[b] for b in pick], [ql[b] for b in pick], stream=2)
+            batch.check_errors(stream=2)                                # waits for the stream
+            want, bound = ref.attend(codes, exps, table[pick], [kv[b] for b in pick], [ql[b] for b in pick],
+                                     rows.cpu().numpy().astype(float), D ** -0.5)
+            assert ref.close(outs[i].cpu().numpy(), want, bound, "f16")
+        except BaseException as exc:  # noqa: BLE001 - reported below
+            failed.append(exc)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed

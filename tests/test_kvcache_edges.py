@@ -1,8 +1,13 @@
-"""The cache's host side where calls meet: collections inside its own locks."""
+"""The cache's host side where calls meet: collections inside its own locks,
+streams whose handles say too little."""
 
 import threading
 
+import pytest
+
 from ptxgen import kvcache as kv
+from ptxgen.kvcache import DeviceArray
+from ptxgen.runtime import EmmyError
 from ptxgen.kvcache import DeviceArray, KVCache, KVSequences
 from tests.test_kvcache import dev, small  # noqa: F401 - a fixture
 
@@ -40,3 +45,63 @@ def test_a_batch_that_goes_while_buffers_are_given_or_taken(dev):  # noqa: F811
     Held.victims.append(cache.batch([[1]], [9]))
     assert ends(lambda: cache.batch([[1]], [9]).close())
     assert not Held.victims and pool.bytes == sum(k[1] * len(v) for k, v in pool.held.items())
+
+
+def arrays():
+    return DeviceArray(1 << 20, "bf16", (1, 4, 64)), DeviceArray(1 << 21, "bf16", (1, 4, 64))
+
+
+def used_and_closed(cache, stream):
+    b = cache.batch([[1]], [9], stream=stream)
+    b.attend(0, *arrays(), stream=stream)
+    held = {p for p, _ in b._held}
+    b.close()
+    return held
+
+
+def test_a_handle_that_comes_again_is_another_stream(dev):  # noqa: F811
+    """Buffers of a stream that was destroyed, perhaps with work queued, do
+    not go to the next one with its handle."""
+    ids = {77: 1000}
+    dev.L.emmy_stream_id = lambda st, word: setattr(word._obj, "value", ids[st]) or 0
+    cache = small(dev)
+    first = used_and_closed(cache, 77)
+    assert used_and_closed(cache, 77) == first
+    ids[77] = 1001                                   # destroyed, and made anew
+    assert not used_and_closed(cache, 77) & first
+
+
+def test_the_per_thread_default_stream(dev):  # noqa: F811
+    """One handle, a stream in each thread: buffers stay with their thread,
+    and a batch with the thread that made it."""
+    dev.L.emmy_stream_id = lambda st, word: setattr(word._obj, "value", threading.get_ident() if st == 2 else 5) or 0
+    cache, got = small(dev), []
+    mine = used_and_closed(cache, 2)
+    assert ends(lambda: got.append(used_and_closed(cache, 2))) and not got[0] & mine
+    assert used_and_closed(cache, 2) == mine
+    b = cache.batch([[1]], [9], stream=2)
+    b.attend(0, *arrays(), stream=2)
+
+    def elsewhere():
+        with pytest.raises(EmmyError, match="per-thread"):
+            b.attend(0, *arrays(), stream=2)
+        got.append("refused")
+    assert ends(elsewhere) and got[-1] == "refused"
+    with pytest.raises(EmmyError, match="per-thread"):
+        b.attend(0, *arrays(), stream=9)
+    b = cache.batch([[1]], [9], stream=9)            # one of another stream waits in each thread
+    dev.L.calls.clear()
+    for _ in range(2):
+        b.attend(0, *arrays(), stream=2)
+    assert ends(lambda: b.attend(0, *arrays(), stream=2))
+    assert [a[0] for name, a in dev.L.calls if name == "emmy_stream_wait_event"] == [2, 2]
+
+
+def test_spare_buffers_of_streams_that_are_gone_make_room(dev, monkeypatch):  # noqa: F811
+    monkeypatch.setattr(kv._Pool, "MOST", 3 * 4096)
+    cache = small(dev)
+    for stream in (1, 3, 4, 5, 6):
+        cache.batch([[1]], [9], stream=stream).close()
+    pool = kv._Pool.of(dev)
+    assert {k[2] for k in pool.held} == {4, 5, 6} and pool.bytes == 3 * 4096
+    assert len(dev.live - set(cache._own)) == 3
