@@ -168,6 +168,8 @@ int check_counts(const char *what, const emmy_kv8 *c);  // of the sequences, wit
 int check_seqs(const char *what, const emmy_kv8 *c);
 Seqs seqs_of(const emmy_kv8 &c);
 int sm_count(int device);
+// Counts a call that goes into a capture of `stream` (40 ns a call).
+void note_capture(cudaStream_t stream);
 // Limit of the kernels' waits, in ns, and the blocks that are to wait in vain.
 void wait_limit(unsigned long long &ns, int &stall);
 // Whether [a, a + na) and [b, b + nb) share a byte.

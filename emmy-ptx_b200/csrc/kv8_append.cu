@@ -328,6 +328,7 @@ extern "C" int emmy_kv8_append(const emmy_kv8 *cache, emmy_dptr k, emmy_dptr v, 
   const int64_t slots = (int64_t(cache->tokens) >> p.s.page_shift) + 2 * int64_t(cache->seqs);
   if (slots > 0x7fffffff) return fail(EMMY_EINVAL, what, "too many tokens");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  note_capture(st);
   return cache->head_dim == 64 ? launch_type<64>(p, dtype, cache->max_q == 1, slots, cache->device, st)
                                : launch_type<128>(p, dtype, cache->max_q == 1, slots, cache->device, st);
 }

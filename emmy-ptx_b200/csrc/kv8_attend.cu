@@ -179,6 +179,7 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   if (on.err != cudaSuccess) return cuda_fail(what, on.err);
   const bool bf16 = a->dtype == EMMY_KV8_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  note_capture(st);
   if (shape.tiles) rc = tiles_attend(p, *cache, shape, bf16, st);
   p.beside = shape.tiles;
   if (rc == EMMY_OK && shape.rows) rc = rows_attend(p, *cache, shape, bf16, st);

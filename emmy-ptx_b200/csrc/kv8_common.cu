@@ -83,7 +83,23 @@ void wait_limit(unsigned long long &ns, int &stall) {
   stall = g_stall.load(std::memory_order_relaxed);
 }
 
+static std::atomic<uint64_t> g_captured{0};
+void note_capture(cudaStream_t stream) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  // what is wrong with the stream the launch will say
+  if (cudaStreamIsCapturing(stream, &st) != cudaSuccess)
+    cudaGetLastError();
+  else if (st != cudaStreamCaptureStatusNone)
+    g_captured.fetch_add(1, std::memory_order_relaxed);
+}
+
 }  // namespace kv8
+
+extern "C" int emmy_kv8_captured(uint64_t *calls) {
+  if (calls == nullptr) return kv8::fail(EMMY_EINVAL, "emmy_kv8_captured", "null result");
+  *calls = kv8::g_captured.load(std::memory_order_relaxed);
+  return EMMY_OK;
+}
 
 extern "C" int emmy_kv8_wait_limit(uint64_t ns, int32_t stall) {
   if (stall < 0) return kv8::fail(EMMY_EINVAL, "emmy_kv8_wait_limit", "stall must not be negative");

@@ -144,6 +144,13 @@ def _capturing(dev: Device, st: int) -> bool:
     return word.value != 0
 
 
+def _captured(dev: Device) -> int:
+    """Calls of this process that went into captures so far."""
+    word = C.c_uint64()
+    check(dev.L.emmy_kv8_captured(C.byref(word)), "captured calls")
+    return word.value
+
+
 def _outside_capture(dev: Device, st: int, why: str) -> None:
     """A graph would keep the address of host memory that is gone when it
     runs, or do what later calls count on only then."""
@@ -179,12 +186,13 @@ class _Pool:
         return dev.__dict__.get("_kv_pool") or dev.__dict__.setdefault("_kv_pool", cls(dev))
 
     def __init__(self, dev: Device):
-        self.dev, self.held, self.bytes = dev, {}, 0
+        self.dev, self.held, self.bytes, self.gone = dev, {}, 0, []
         self.lock = threading.RLock()   # a collection inside of it may close a batch
 
     def take(self, use: str, nbytes: int, stream: int) -> tuple[int, tuple]:
         """(address, key to give it back by) of a buffer for work on ``stream``."""
         key = (use, 1 << max(12, (nbytes - 1).bit_length()), _stream_id(self.dev, stream))
+        self.drain()
         with self.lock:
             held = self.held.get(key)
             if held:
@@ -195,7 +203,19 @@ class _Pool:
             check(self.dev.L.emmy_memset_d32(ptr, 0, WORKSPACE_ZERO // 4, stream), "memset")
         return ptr, key
 
-    def give(self, ptr: int, key: tuple, reuse: bool) -> None:
+    def drain(self) -> None:
+        """Free what is not to be used again: waits for what still runs on it."""
+        while self.gone:
+            try:
+                ptr = self.gone.pop()
+            except IndexError:          # another thread's turn
+                break
+            self.dev.free(ptr)
+
+    def give(self, ptr: int, key: tuple, reuse: bool, later: bool = False) -> None:
+        """``later``: what is to be freed is at the next call of ``take``, for a
+        collection may come while some stream is captured, and memory that is
+        freed then ends the capture."""
         gone = [] if reuse else [ptr]
         with self.lock:
             if reuse:
@@ -211,8 +231,9 @@ class _Pool:
                     self.bytes += key[1]
                 else:
                     gone.append(ptr)
-        for ptr in gone:
-            self.dev.free(ptr)          # waits for what still runs on it
+        self.gone += gone
+        if not later:
+            self.drain()
 
 
 class KVCache:
@@ -261,6 +282,7 @@ class KVCache:
         self.dev = Device.get(device)
         self.L = load_library()
         if storage is None:
+            _Pool.of(self.dev).drain()
             for attr, n in (("codes", layers * self.layer_codes), ("exps", layers * self.layer_exps)):
                 ptr = self.dev.alloc(n)
                 self._own.append(ptr)
@@ -360,7 +382,7 @@ class Batch:
         host = self._packed(table, kv_lens, q_lens)
         self._stream, self._reuse = _stream_of(stream, self.dev), True
         _outside_capture(self.dev, self._stream, "lengths and page numbers are copied from the host")
-        self._pool = _Pool.of(self.dev)
+        self._pool, self._captured = _Pool.of(self.dev), _captured(self.dev)
         self._who = self._same(self._stream)
         self._others: set[int] = set()             # further streams it was used on
         self._buf = self._take("batch", host.nbytes, self._stream)
@@ -586,15 +608,22 @@ class Batch:
 
     def close(self) -> None:
         """Give the batch's buffers back for later batches: nothing that is
-        not queued on the batch's stream yet may use them after this."""
+        not queued yet may use them after this.  Where a graph may still be
+        running that was captured while the batch lived -- on any stream -- or
+        another stream was used, they are freed instead, which waits."""
+        self._close(later=False)
+
+    def _close(self, later: bool) -> None:
         held, self._held = self._held, []
         self._buf, self._ws, self._plans = 0, (0, 0), {}
-        for ptr, key in held:
-            self._pool.give(ptr, key, self._reuse)
+        if held:
+            reuse = self._reuse and _captured(self.dev) == self._captured
+            for ptr, key in held:
+                self._pool.give(ptr, key, reuse, later)
 
     def __del__(self):
         try:
-            self.close()
+            self._close(later=True)
         except Exception:  # the context may be gone when the process ends
             pass
 

@@ -109,6 +109,7 @@ def load_library():
         "emmy_kv8_attend_plan": (i32, [vp, vp, vp]),
         "emmy_kv8_attend": (i32, [vp, vp, vp]),
         "emmy_kv8_wait_limit": (i32, [u64, i32]),
+        "emmy_kv8_captured": (i32, [C.POINTER(u64)]),
         "emmy_kv8_copy_pages": (i32, [vp, i32, vp, vp, i32, vp]),
     }
     for name, (res, args) in sig.items():

@@ -279,6 +279,10 @@ int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args *args, emm
 enum { EMMY_KV8_WAIT_NS = 2000000000 };
 int emmy_kv8_wait_limit(uint64_t ns, int32_t stall);
 
+/* How many calls of append and attend this process has queued into captures of
+ * streams: buffers that such a call was given are read by graphs. */
+int emmy_kv8_captured(uint64_t *calls);
+
 /* In each of `layers` layers, laid out one after another, copy page src[i]
  * with its exponents to page dst[i], i < n (host arrays, read during the
  * call; n at most EMMY_KV8_MAX_PAIRS).  No page may be in dst twice, or in

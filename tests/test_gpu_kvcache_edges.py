@@ -140,3 +140,38 @@ def test_threads_on_their_default_streams():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not failed
+
+
+def test_a_batch_that_goes_while_its_graph_runs():
+    """Captured on the batch's own stream, replayed on another, dropped while
+    replays are queued there: the next batches on its stream have other memory."""
+    torch = pytest.importorskip("torch")
+    from ptxgen import KVCache
+    rng = np.random.default_rng(6)
+    P, D, H, kv = 64, 64, 1, [3000, 500]
+    codes, exps = ref.pool(rng, 60, H, P, D)
+    table = ref.tables(rng, 60, kv, P)
+    c, e = torch.from_numpy(codes)[None].cuda(), torch.from_numpy(exps)[None].cuda()
+    cache = KVCache(60, H, D, storage=(c, e))
+    q = torch.from_numpy(rng.standard_normal((2, 2, D))).half().cuda()
+    out, other = torch.zeros_like(q), torch.zeros_like(q)
+    st, elsewhere = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    batch = cache.batch(table, kv, stream=st)
+    batch.reserve(2, stream=st)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        for _ in range(50):
+            batch.attend(0, q, out, stream=st)
+    with torch.cuda.stream(elsewhere):
+        for _ in range(10):
+            graph.replay()
+    del batch
+    for _ in range(5):
+        b = cache.batch([[0] * 47], [47 * P], [1], stream=st)          # other lengths, over the same sizes
+        b.attend(0, q, other, stream=st)
+        del b
+    torch.cuda.synchronize()
+    want, bound = ref.attend(codes, exps, table, kv, [1, 1], q.cpu().numpy().astype(float), D ** -0.5)
+    assert ref.close(out.cpu().numpy(), want, bound, "f16")

@@ -1,5 +1,5 @@
 """The cache's host side where calls meet: collections inside its own locks,
-streams whose handles say too little."""
+streams whose handles say too little, graphs that outlive a call."""
 
 import threading
 
@@ -105,3 +105,31 @@ def test_spare_buffers_of_streams_that_are_gone_make_room(dev, monkeypatch):  # 
     pool = kv._Pool.of(dev)
     assert {k[2] for k in pool.held} == {4, 5, 6} and pool.bytes == 3 * 4096
     assert len(dev.live - set(cache._own)) == 3
+
+
+def test_buffers_that_a_graph_was_given_are_not_used_again(dev):  # noqa: F811
+    """The graph may be running, on a stream that the batch never saw, when the
+    batch goes: freeing waits for it, the next batch would not."""
+    calls = [0]
+    dev.L.emmy_kv8_captured = lambda word: setattr(word._obj, "value", calls[0]) or 0
+    cache = small(dev)
+    b = cache.batch([[1]], [9], stream=5)
+    b.attend(0, *arrays(), stream=5)
+    calls[0] += 1                                    # one more call, into a capture of stream 5
+    held = {p for p, _ in b._held}
+    b.close()
+    assert not held & dev.live and not kv._Pool.of(dev).bytes
+    first = used_and_closed(cache, 5)                # made after: as ever
+    assert used_and_closed(cache, 5) == first
+
+
+def test_a_collection_frees_nothing_at_once(dev):  # noqa: F811
+    """It may come while some stream is captured."""
+    cache = small(dev)
+    b = cache.batch([[1]], [9], stream=5)
+    b.attend(0, *arrays(), stream=6)
+    held = {p for p, _ in b._held}
+    del b
+    assert held <= dev.live
+    cache.batch([[1]], [9], stream=7)
+    assert not held & dev.live
