@@ -740,6 +740,7 @@ class KVSequences:
                 pages[sid] += taken[at:at + more]
                 at += more
         lens = [self._len[sid] + n for sid, n in zip(sids, q)]
+        self._outside_capture(stream)
         self.cache.copy_pages(src, taken[:len(src)], stream)
         b = Batch(self.cache, self._table(list(pages.values())), lens, q, stream)
         # the books follow once nothing can fail
@@ -752,6 +753,10 @@ class KVSequences:
         self._len.update(zip(sids, lens))
         self._track(b)
         return b
+
+    def _outside_capture(self, stream) -> None:
+        dev = self.cache.dev
+        _outside_capture(dev, _stream_of(stream, dev), "the books move on once, a graph's page copies at each replay")
 
     def table(self, sids) -> np.ndarray:
         """Page numbers [sequences, pages of the longest], rows filled up with 0."""
@@ -780,6 +785,7 @@ class KVSequences:
         holes = [p for p in range(n) if not self._refs[p]]
         moved = dict(zip([p for p in used if p >= n], holes))
         if moved:
+            self._outside_capture(stream)
             self.cache.copy_pages(list(moved), list(moved.values()), stream)
             for old, new in moved.items():
                 self._refs[new], self._refs[old] = self._refs[old], 0

@@ -6,7 +6,7 @@ import threading
 import pytest
 
 from ptxgen import kvcache as kv
-from ptxgen.kvcache import DeviceArray
+from ptxgen.kvcache import DeviceArray, KVSequences
 from ptxgen.runtime import EmmyError
 from ptxgen.kvcache import DeviceArray, KVCache, KVSequences
 from tests.test_kvcache import dev, small  # noqa: F401 - a fixture
@@ -133,3 +133,32 @@ def test_a_collection_frees_nothing_at_once(dev):  # noqa: F811
     assert held <= dev.live
     cache.batch([[1]], [9], stream=7)
     assert not held & dev.live
+
+
+def test_page_moves_of_a_captured_stream_are_refused(dev):  # noqa: F811
+    """A graph would make the copies at each replay, from and to pages that
+    belong to others by then, while the books move on once."""
+    cache = small(dev)
+    seqs = KVSequences(cache)
+    a = seqs.new()
+    seqs.batch([a], [70])
+    b, c = seqs.fork(a), seqs.new()
+    seqs.batch([c], [65])
+    seqs.free(a)
+    d = seqs.fork(b)
+
+    def books():
+        return [seqs.pages(s) for s in (b, c, d)], [seqs.length(s) for s in (b, c, d)], list(seqs._refs), list(seqs._free)
+    before = books()
+    dev.L.calls.clear()
+    dev.L.emmy_stream_capturing = lambda st, word: setattr(word._obj, "value", 1) or 0
+    with pytest.raises(EmmyError, match="captured"):
+        seqs.batch([b, d], stream=5)                 # a shared page would be copied
+    assert books() == before
+    seqs.free(b)
+    seqs.free(d)
+    before = [seqs.pages(c)], [seqs.length(c)], list(seqs._refs), list(seqs._free)
+    with pytest.raises(EmmyError, match="captured"):
+        seqs.compact(stream=5)                       # c's pages would move
+    assert before == ([seqs.pages(c)], [seqs.length(c)], list(seqs._refs), list(seqs._free))
+    assert not [name for name, _ in dev.L.calls if name == "emmy_kv8_copy_pages"]
