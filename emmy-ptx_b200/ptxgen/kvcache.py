@@ -474,7 +474,7 @@ class Batch:
             st = self._on(stream)
             _outside_capture(self.dev, st, "lengths and page numbers are copied from the host")
             _copy_in(self.dev, self._buf + 16, host[4:], st)
-        except EmmyError:
+        except BaseException:
             self._clash = clash         # of what the device still holds
             raise
         for key in self._plans:

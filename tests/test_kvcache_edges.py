@@ -162,3 +162,12 @@ def test_page_moves_of_a_captured_stream_are_refused(dev):  # noqa: F811
         seqs.compact(stream=5)                       # c's pages would move
     assert before == ([seqs.pages(c)], [seqs.length(c)], list(seqs._refs), list(seqs._free))
     assert not [name for name, _ in dev.L.calls if name == "emmy_kv8_copy_pages"]
+
+
+def test_an_update_that_raises_anything_keeps_what_append_knows(dev):  # noqa: F811
+    cache = small(dev)
+    b = cache.batch([[1], [2]], [9, 9])
+    x = DeviceArray(1 << 20, "bf16", (2, 2, 64))
+    with pytest.raises(AttributeError):
+        b.update([[1], [1]], [9, 9], stream="no stream")
+    b.append(0, x, x)                                # the device still holds two pages
