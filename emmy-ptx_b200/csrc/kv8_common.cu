@@ -125,3 +125,17 @@ extern "C" int emmy_stream_id(emmy_stream stream, uint64_t *id) {
   *id = word;
   return EMMY_OK;
 }
+
+extern "C" int emmy_device_enter(int device, int *before) {
+  if (before == nullptr) return kv8::fail(EMMY_EINVAL, "emmy_device_enter", "null result");
+  cudaError_t e = cudaGetDevice(before);
+  if (e == cudaSuccess) e = cudaSetDevice(device);
+  return e == cudaSuccess ? EMMY_OK : kv8::cuda_fail("emmy_device_enter", e);
+}
+
+extern "C" int emmy_device_leave(int before) {
+  int now = before;
+  cudaError_t e = cudaGetDevice(&now);
+  if (e == cudaSuccess && now != before) e = cudaSetDevice(before);
+  return e == cudaSuccess ? EMMY_OK : kv8::cuda_fail("emmy_device_leave", e);
+}

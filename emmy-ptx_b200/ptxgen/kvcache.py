@@ -39,6 +39,7 @@ was made on waits for that once).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import threading
 import weakref
 from array import array
@@ -128,6 +129,31 @@ def _stream_of(stream, dev: Device) -> int:
         stream = dev.stream
     stream = getattr(stream, "cuda_stream", stream)
     return stream if isinstance(stream, int) else stream.value or 0
+
+
+class _Current:
+    """A device as the thread's current one for a scope: what allocates, copies
+    and records here goes by that, and callers find their own back."""
+
+    def __init__(self, L, ordinal: int):
+        self.L, self.ordinal = L, ordinal
+
+    def __enter__(self):
+        word = C.c_int()
+        check(self.L.emmy_device_enter(self.ordinal, C.byref(word)), "device")
+        self.before = word.value
+
+    def __exit__(self, *exc):
+        self.L.emmy_device_leave(self.before)
+
+
+def _at_home(method):
+    """A method of a cache or batch, with its device the current one."""
+    @functools.wraps(method)
+    def call(self, *a, **kw):
+        with _Current(self.L, self.ordinal):
+            return method(self, *a, **kw)
+    return call
 
 
 def _stream_id(dev: Device, st: int) -> int:
@@ -279,9 +305,16 @@ class KVCache:
             self.codes, self.exps = codes.data_ptr(), exps.data_ptr()
             if self.codes % 16:
                 raise EmmyError("storage: codes must be 16-byte aligned")
-        self.dev = Device.get(device)
         self.L = load_library()
-        if storage is None:
+        with _Current(self.L, device):
+            self._open(storage is None)
+        self._cdesc = self._desc()
+        self._cref = C.byref(self._cdesc)
+
+    def _open(self, allocate: bool) -> None:
+        layers = self.layers
+        self.dev = Device.get(self.ordinal)
+        if allocate:
             _Pool.of(self.dev).drain()
             for attr, n in (("codes", layers * self.layer_codes), ("exps", layers * self.layer_exps)):
                 ptr = self.dev.alloc(n)
@@ -291,8 +324,6 @@ class KVCache:
             self.dev.memset32(self.codes, 0, (layers * self.layer_codes + 3) // 4)
             self.dev.memset32(self.exps, 0, (layers * self.layer_exps + 3) // 4)
             self.dev.sync()
-        self._cdesc = self._desc()
-        self._cref = C.byref(self._cdesc)
 
     def _desc(self) -> _Cache:
         d = _Cache()
@@ -337,6 +368,7 @@ class KVCache:
             if rc:
                 check(rc, "copy_pages")
 
+    @_at_home
     def close(self) -> None:
         """Free what this cache allocated (not adopted storage)."""
         own, self._own = self._own, []
@@ -364,7 +396,12 @@ class Batch:
     ``check_errors`` stay outside of captures."""
 
     def __init__(self, cache: KVCache, page_table, kv_lens, q_lens=None, stream=None):
-        self.cache, self.dev, self.L = cache, cache.dev, cache.L
+        self.cache, self.dev, self.L, self.ordinal = cache, cache.dev, cache.L, cache.ordinal
+        self._make(page_table, kv_lens, q_lens, stream)
+
+    @_at_home
+    def _make(self, page_table, kv_lens, q_lens, stream) -> None:
+        cache = self.cache
         table = _ints(page_table, "page_table")
         if table.ndim != 2 or table.shape[0] < 1 or table.shape[1] < 1:
             raise EmmyError("page_table must be [sequences, pages]")
@@ -418,14 +455,15 @@ class Batch:
             if self._stream == PER_THREAD:
                 raise EmmyError("a batch made on the per-thread default stream is for that thread and stream")
             self._reuse = False
-            if _capturing(self.dev, st):
-                return st
-            ev = self.dev.event()
-            try:
-                check(self.L.emmy_event_record(ev, self._stream), "event record")
-                check(self.L.emmy_stream_wait_event(st, ev), "stream wait event")
-            finally:
-                self.L.emmy_event_destroy(ev)
+            with _Current(self.L, self.ordinal):
+                if _capturing(self.dev, st):
+                    return st
+                ev = self.dev.event()
+                try:
+                    check(self.L.emmy_event_record(ev, self._stream), "event record")
+                    check(self.L.emmy_stream_wait_event(st, ev), "stream wait event")
+                finally:
+                    self.L.emmy_event_destroy(ev)
             self._others.add(who)
         return st
 
@@ -463,6 +501,7 @@ class Batch:
         host[5 + 2 * B:] = np.where(used, table, 0).reshape(-1)
         return host
 
+    @_at_home
     def update(self, page_table, kv_lens, q_lens=None, stream=None) -> None:
         """New contents in the same device arrays, for the next replay of a
         graph or the next step: as many sequences, a table as wide, no more
@@ -537,8 +576,12 @@ class Batch:
         otherwise; before a graph is captured it has to be done."""
         self._live()
         key = (heads, window, sinks)
-        if key in self._plans:
-            return
+        if key not in self._plans:
+            self._reserve(key, stream)
+
+    @_at_home
+    def _reserve(self, key: tuple, stream) -> None:
+        heads, window, sinks = key
         if not 0 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31:
             raise EmmyError("attend: window and sinks are between 0 and 2^31 - 1")
         if not 1 <= heads <= 2 ** 20:
@@ -591,6 +634,7 @@ class Batch:
             check(rc, "attend")
         return out
 
+    @_at_home
     def check_errors(self, stream=None) -> None:
         """Wait for ``stream`` and raise if a kernel of this batch reported
         something in its status word; clears it."""
@@ -616,7 +660,9 @@ class Batch:
     def _close(self, later: bool) -> None:
         held, self._held = self._held, []
         self._buf, self._ws, self._plans = 0, (0, 0), {}
-        if held:
+        if not held:
+            return
+        with _Current(self.L, self.ordinal):
             reuse = self._reuse and _captured(self.dev) == self._captured
             for ptr, key in held:
                 self._pool.give(ptr, key, reuse, later)
@@ -756,7 +802,9 @@ class KVSequences:
 
     def _outside_capture(self, stream) -> None:
         dev = self.cache.dev
-        _outside_capture(dev, _stream_of(stream, dev), "the books move on once, a graph's page copies at each replay")
+        with _Current(self.cache.L, self.cache.ordinal):
+            _outside_capture(dev, _stream_of(stream, dev),
+                             "the books move on once, a graph's page copies at each replay")
 
     def table(self, sids) -> np.ndarray:
         """Page numbers [sequences, pages of the longest], rows filled up with 0."""

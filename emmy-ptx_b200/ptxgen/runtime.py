@@ -104,6 +104,8 @@ def load_library():
         "emmy_nccl_destroy": (i32, [vp]),
         "emmy_stream_capturing": (i32, [vp, C.POINTER(i32)]),
         "emmy_stream_id": (i32, [vp, C.POINTER(u64)]),
+        "emmy_device_enter": (i32, [i32, C.POINTER(i32)]),
+        "emmy_device_leave": (i32, [i32]),
         "emmy_kv8_append": (i32, [vp, u64, u64, i32, vp, vp, vp]),
         "emmy_kv8_attend_sizes": (i32, [vp, i32, C.POINTER(u64), C.POINTER(u64)]),
         "emmy_kv8_attend_plan": (i32, [vp, vp, vp]),

@@ -154,6 +154,12 @@ int emmy_stream_wait_event(emmy_stream stream, emmy_event ev);
 /* Whether `stream` is being captured into a graph (no counterpart either). */
 int emmy_stream_capturing(emmy_stream stream, int *capturing);
 
+/* Makes `device` the calling thread's current one and says which was; leave
+ * puts that back.  Allocations, copies and events go by the current device, and
+ * some calls of this library change it (no counterpart either). */
+int emmy_device_enter(int device, int *before);
+int emmy_device_leave(int before);
+
 /* A number that no other stream of the process has, had or will have: a handle
  * comes again once its stream is destroyed, and the per-thread default stream's
  * means another stream in each thread (no counterpart either). */

@@ -1,5 +1,6 @@
 """The cache's host side where calls meet: collections inside its own locks,
-streams whose handles say too little, graphs that outlive a call."""
+streams whose handles say too little, graphs that outlive a call, other current
+devices."""
 
 import threading
 
@@ -171,3 +172,47 @@ def test_an_update_that_raises_anything_keeps_what_append_knows(dev):  # noqa: F
     with pytest.raises(AttributeError):
         b.update([[1], [1]], [9, 9], stream="no stream")
     b.append(0, x, x)                                # the device still holds two pages
+
+
+def test_the_callers_current_device_stays(dev, monkeypatch):  # noqa: F811
+    """All that goes by the current device happens with the cache's as that
+    one, and the caller's is back after each call."""
+    now = [3]
+    by_device = {"alloc", "free", "emmy_memcpy_htod", "emmy_memcpy_dtoh", "emmy_memset_d32", "event", "memset32",
+                 "emmy_event_record", "emmy_stream_wait_event", "emmy_stream_sync", "emmy_stream_capturing",
+                 "emmy_stream_id", "sync"}
+    seen = set()
+
+    def enter(device, word):
+        word._obj.value = now[0]
+        now[0] = device
+        return 0
+
+    def leave(before):
+        now[0] = before
+        return 0
+    dev.L.emmy_device_enter, dev.L.emmy_device_leave = enter, leave
+
+    def watched(name, call):
+        def f(*a):
+            assert now[0] == 1, name
+            seen.add(name)
+            return call(*a)
+        return f
+    for name in by_device:
+        at = dev.L if name.startswith("emmy") else dev
+        setattr(at, name, watched(name, getattr(at, name)))
+    monkeypatch.setattr(kv.Device, "get", classmethod(lambda cls, ordinal=0: watched("get", lambda: dev)()))
+    cache = small(dev, device=1)
+    seqs = KVSequences(cache)
+    a = seqs.new()
+    b = seqs.batch([a], [1], stream=5)
+    q, out = (DeviceArray(1 << n, "bf16", (1, 4, 64), None, 1) for n in (20, 21))
+    k = DeviceArray(1 << 22, "f32", (1, 2, 64), None, 1)
+    for call in (lambda: b.append(0, k, k, stream=6), lambda: b.attend(0, q, out, stream=7),
+                 lambda: b.update([[1]], [2], stream=8), lambda: b.reserve(8, stream=5),
+                 lambda: b.check_errors(stream=5), b.close, lambda: seqs.batch([a], stream=5),
+                 lambda: seqs.compact(), cache.close):
+        call()
+        assert now[0] == 3
+    assert seen >= by_device - {"sync"}
