@@ -26,9 +26,10 @@ int shape_of(const char *what, const emmy_kv8 *c, int heads, PlanShape &p) {
   const int64_t segments = int64_t(c->seqs) * c->kv_heads * ((few + ROWS_BLOCK - 1) / ROWS_BLOCK);
   const int wave = sms * ROWS_PER_SM;
   p.spread = segments > wave;
-  // Workspace slots, two counters each.  Two waves: a cut segment has c >= 1.5 q
+  // Workspace slots, two counters each, but the last two of the zeros are
+  // AttendParams::ready.  Two waves: a cut segment has c >= 1.5 q
   // chunks and at most c / q + 1/2 parts, a third above its share.
-  const int fit = EMMY_KV8_WORKSPACE_ZERO / 8;
+  const int fit = EMMY_KV8_WORKSPACE_ZERO / 8 - 1;
   p.slots = 3 * wave < fit ? 3 * wave : fit;
   p.target = p.spread ? p.slots * 2 / 3 : wave < p.slots ? wave : p.slots;
   // The parts wanted, or, where no try fitted, one of each segment more; but
@@ -180,9 +181,13 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   const bool bf16 = a->dtype == EMMY_KV8_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   note_capture(st);
+  p.beside = shape.tiles && shape.rows;
+  p.ready = p.counters + EMMY_KV8_WORKSPACE_ZERO / 4 - 2;
   if (shape.tiles) rc = tiles_attend(p, *cache, shape, bf16, st);
-  p.beside = shape.tiles;
-  if (rc == EMMY_OK && shape.rows) rc = rows_attend(p, *cache, shape, bf16, st);
+  if (rc == EMMY_OK && shape.rows) {
+    rc = rows_attend(p, *cache, shape, bf16, st);
+    if (rc != EMMY_OK && p.beside) cudaMemsetAsync(p.ready, 0, 8, st);  // nobody else will
+  }
   if (rc == EMMY_OK && shape.tile_target > 0) rc = tiles_join(p, *cache, shape, bf16, st);
   return rc;
 }

@@ -50,6 +50,7 @@ struct AttendParams {
   int nt;            // 8-row blocks of the row kernel
   int cluster;       // CTAs of a cluster of the row kernel, 0: none
   bool beside;       // the row kernel was launched to run beside the tile kernel
+  unsigned *ready;   // there: what came before both is done, and the row kernel's blocks that know
   int stall;         // one block in so many withholds its first keys (0: none)
   unsigned long long wait_ns;  // limit of the kernels' waits
 };

@@ -705,17 +705,39 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
 }
 
 // Beside the tile kernel, which was launched before it and whose sequences are
-// others, it starts when all of that kernel's CTAs run: what they waited for is
-// done then, so nothing is read early, and SMs without a unit, or past their
-// last, take parts (512 tokens behind 3584 keys with 47 single tokens of
-// 700-8191 keys: 175 -> 131 us a call).  One block waits for that kernel in the
-// end, so that what comes after this kernel comes after both.
+// others, it starts when all of that kernel's CTAs run: SMs without a unit, or
+// past their last, take parts (512 tokens behind 3584 keys with 47 single tokens
+// of 700-8191 keys: 175 -> 131 us a call).  What came before both is done then;
+// that it is also visible here, without this kernel's own wait, follows from
+// the word that the tile kernel released after its wait, and a block that does
+// not find it there waits.  The last block to have looked takes the word back.
+// One block waits for the tile kernel in the end, so that what comes after this
+// kernel comes after both.
+__device__ __forceinline__ void ready_or_wait(const AttendParams &p) {
+  __shared__ unsigned ready;
+  if (threadIdx.x == 0)
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(ready) : "l"(p.ready) : "memory");
+  __syncthreads();
+  if (ready == 0) grid_dependency_wait();
+  // and to the copies that the loading warp will start
+  asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+__device__ __forceinline__ void took_ready(const AttendParams &p) {
+  if (threadIdx.x == 0 && atomicAdd(p.ready + 1, 1u) == gridDim.x - 1) p.ready[0] = p.ready[1] = 0;
+}
+
 template <int D, int NT, bool CLUSTER, typename T>
 __global__ void __launch_bounds__(THREADS, ROWS_PER_SM)
 rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map) {
-  if (!p.beside) grid_dependency_wait();
+  if (p.beside)
+    ready_or_wait(p);
+  else
+    grid_dependency_wait();
   attend_part<D, NT, CLUSTER, T>(p, codes_map);
-  if (p.beside && blockIdx.x == 0) grid_dependency_wait();
+  if (p.beside) {
+    took_ready(p);
+    if (blockIdx.x == 0) grid_dependency_wait();
+  }
 }
 
 template <int D, int NT, bool CLUSTER, typename T>

@@ -261,6 +261,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
   const Seqs &s = p.s;
 
   grid_dependency_wait();
+  if (p.beside && blockIdx.x == 0 && tid == 0)
+    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p.ready), "r"(1u) : "memory");
   const PlanHead head = *p.plan;
   const UnitRec first_rec = p.units[blockIdx.x];
   grid_dependency_done();

@@ -175,3 +175,41 @@ def test_a_batch_that_goes_while_its_graph_runs():
     torch.cuda.synchronize()
     want, bound = ref.attend(codes, exps, table, kv, [1, 1], q.cpu().numpy().astype(float), D ** -0.5)
     assert ref.close(out.cpu().numpy(), want, bound, "f16")
+
+
+@pytest.mark.parametrize("prompts,singles", [([300, 90], 40), ([64], 300)])
+def test_prompts_beside_single_tokens_right_behind_append(prompts, singles):
+    """Both kernels of the call read what the append right before it wrote."""
+    torch = pytest.importorskip("torch")
+    from ptxgen import KVCache
+    rng = np.random.default_rng(8)
+    P, D, H, G = 64, 128, 2, 2
+    ql = prompts + [1] * singles
+    kv = [n + int(rng.integers(0, 200)) for n in prompts] + rng.integers(1, 500, singles).tolist()
+    pages = sum(-(-n // P) for n in kv)
+    codes, exps = ref.pool(rng, pages, H, P, D)
+    table = ref.tables(rng, pages, kv, P)
+    c, e = torch.from_numpy(codes)[None].cuda(), torch.from_numpy(exps)[None].cuda()
+    cache = KVCache(pages, H, D, storage=(c, e))
+    n = sum(ql)
+    k, v = (rng.standard_normal((2, n, H, D)) * 4).astype(np.float16)
+    q = torch.from_numpy(rng.standard_normal((n, H * G, D))).half().cuda()
+    kd, vd, c0, e0 = torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), c.clone(), e.clone()
+    st = torch.cuda.current_stream()
+    batch, outs = cache.batch(table, kv, ql, stream=st), []
+    for _ in range(10):
+        c.copy_(c0)
+        e.copy_(e0)
+        outs.append(torch.empty_like(q))
+        batch.append(0, kd, vd, stream=st)
+        batch.attend(0, q, outs[-1], stream=st)
+    batch.check_errors(stream=st)
+    after = ref.append(codes, exps, table, kv, ql, k.astype(float), v.astype(float))
+    assert (c[0].cpu().numpy() == after[0]).all() and (e[0].cpu().numpy() == after[1]).all()
+    want, bound = ref.attend(*after, table, kv, ql, q.cpu().numpy().astype(float), D ** -0.5)
+    assert ref.close(outs[0].cpu().numpy(), want, bound, "f16")
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    counters = torch.empty(16384, dtype=torch.uint8)
+    cache.dev.dtoh(counters.numpy(), batch._ws[0])
+    cache.dev.sync()
+    assert not counters.any()
