@@ -1,5 +1,6 @@
 """The paged 8-bit cache where its arithmetic ends: scores past f32's whole
-numbers and near the end of its range; streams that share a handle."""
+numbers and near the end of its range; streams that share a handle;
+segments of more parts than one level of joins takes, the largest pages of f32."""
 
 import threading
 
@@ -8,7 +9,7 @@ import numpy as np
 import pytest
 
 from tests import kv8_oracle as ref
-from tests.test_gpu_kvcache import attend_gpu, gpu  # noqa: F401 - a fixture
+from tests.test_gpu_kvcache import NP, attend_gpu, cache_of, gpu  # noqa: F401 - a fixture
 
 pytestmark = pytest.mark.gpu
 
@@ -213,3 +214,44 @@ def test_prompts_beside_single_tokens_right_behind_append(prompts, singles):
     cache.dev.dtoh(counters.numpy(), batch._ws[0])
     cache.dev.sync()
     assert not counters.any()
+
+
+@pytest.mark.parametrize("H,G,D,dtype,seqs", [
+    (1, 8, 128, "bf16", [(70000, 1)]),                         # clusters of four, 28 results
+    (2, 2, 64, "f16", [(131071, 2)]),                          # 47
+    (1, 3, 64, "bf16", [(45001, 1)] + [(200 + i, 1) for i in range(60)]),      # single parts, more than 200
+])
+def test_joins_of_two_levels(gpu, H, G, D, dtype, seqs):  # noqa: F811
+    """Segments with more results than one CTA joins at once."""
+    rng = np.random.default_rng(H + G)
+    P = 64
+    kv, ql = [a for a, _ in seqs], [b for _, b in seqs]
+    pages = sum(-(-n // P) for n in kv)
+    codes, exps = ref.pool(rng, pages, H, P, D)
+    table = ref.tables(rng, pages, kv, P)
+    q = rng.standard_normal((sum(ql), H * G, D)).astype(NP[dtype])
+    got = attend_gpu(gpu, codes, exps, table, kv, ql, q, dtype)
+    want, bound = ref.attend(codes, exps, table, kv, ql, q.astype(np.float64), D ** -0.5)
+    assert ref.close(got, want, bound, dtype)
+
+
+@pytest.mark.parametrize("H,dtype,seqs", [(2, "f32", [(600, 345), (257, 2)]), (1, "f32", [(256, 256), (300, 44)])])
+def test_append_pages_of_one_buffer(gpu, H, dtype, seqs):  # noqa: F811
+    """f32 pages of 256 tokens and 128 elements fill the shared memory: one
+    buffer, one (side, head) a CTA."""
+    rng = np.random.default_rng(H)
+    P, D = 256, 128
+    kv, ql = [a for a, _ in seqs], [b for _, b in seqs]
+    pages = sum(-(-n // P) for n in kv) + 1
+    codes, exps = ref.pool(rng, pages, H, P, D)
+    table = ref.tables(rng, pages, kv, P)
+    x = rng.standard_normal((2, sum(ql), H, D)) * 2.0 ** rng.integers(-6, 7, (2, sum(ql), H, 1))
+    x = x.astype(NP[dtype])
+    cache, cd, ed = cache_of(gpu, codes[None], exps[None])
+    batch = cache.batch(table, kv, ql)
+    batch.append(0, gpu.put(x[0], dtype), gpu.put(x[1], dtype))
+    batch.check_errors()
+    want = ref.append(codes, exps, table, kv, ql, x[0].astype(float), x[1].astype(float))
+    assert (gpu.get(ed, exps.shape, np.int8) == want[1]).all()
+    assert (gpu.get(cd, codes.shape, np.uint8) == want[0]).all()
+    batch.close()
