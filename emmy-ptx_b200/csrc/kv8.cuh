@@ -72,6 +72,10 @@ __device__ __forceinline__ uint32_t f32x2_e4m3x2(float hi, float lo) {
   return r;
 }
 
+// Exponent of a page's side and head as the kernels take it: adopted storage may
+// hold any.
+__device__ __forceinline__ int held_exponent(int held) { return max(min(held, E_MAX), E_MIN); }
+
 __device__ __forceinline__ float pow2(int e) {  // -126 <= e <= 127
   return __int_as_float((e + 127) << 23);
 }

@@ -113,9 +113,6 @@ __device__ __forceinline__ void store_codes(uint8_t *at, const Vec<T> &v, int e)
     *reinterpret_cast<uint32_t *>(at) = w[0];
 }
 
-// Exponent of a page's side and head that was `held` before, as it may be.
-__device__ __forceinline__ int held_exponent(int8_t held) { return max(min(int(held), E_MAX), E_MIN); }
-
 // Slot of this grid's page list -> its sequence's lengths and the page of the
 // sequence; false: none.  The pages that n tokens touch are at most n / P + 2,
 // and floor((s + n) / P) - floor(s / P) >= floor(n / P), so sequence b may own

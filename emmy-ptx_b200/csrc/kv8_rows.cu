@@ -396,8 +396,9 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
         }
         ChunkInfo c;
         c.key0 = __shfl_sync(0xffffffffu, mine.key0, i);
-        c.ek = __shfl_sync(0xffffffffu, mine.ek, i);
-        c.ev = __shfl_sync(0xffffffffu, mine.ev, i);
+        // (not where they were loaded: their first use would hold up the early copies)
+        c.ek = held_exponent(__shfl_sync(0xffffffffu, mine.ek, i));
+        c.ev = held_exponent(__shfl_sync(0xffffffffu, mine.ev, i));
         c.dead = __shfl_sync(0xffffffffu, mine.dead, i);
         if (who) {
           infos[ring.slot] = c;

@@ -377,8 +377,8 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         }
         const int64_t at = __shfl_sync(0xffffffffu, next_unit, g & 31);
         ChunkInfo c;
-        c.ek = __shfl_sync(0xffffffffu, next.ek, g & 31);
-        c.ev = __shfl_sync(0xffffffffu, next.ev, g & 31);
+        c.ek = held_exponent(__shfl_sync(0xffffffffu, next.ek, g & 31));
+        c.ev = held_exponent(__shfl_sync(0xffffffffu, next.ev, g & 31));
         c.key0 = __shfl_sync(0xffffffffu, next.key0, g & 31);
         c.dead = __shfl_sync(0xffffffffu, next.dead, g & 31);
         if (who) {

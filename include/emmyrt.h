@@ -206,7 +206,8 @@ int emmy_sum_f32_noalloc(emmy_dptr x, size_t n, emmy_dptr out, emmy_stream strea
  * layer of the cache is a pool of pages in caller-owned device memory:
  *   codes  uint8  [pages][2][kv_heads][page_size][head_dim]   (K, then V)
  *   exps   int8   [pages][2][kv_heads]
- * A held value is e4m3(code) * 2^exp, exp in [-32, 63].  A sequence is a row
+ * A held value is e4m3(code) * 2^exp, exp in [-32, 63] (one outside counts as
+ * the nearer end).  A sequence is a row
  * of page numbers and a length; its new tokens, consecutive rows of the
  * tensors given, are the last ones of that length.  The arrays below are
  * device memory, read by the kernels, so a captured CUDA graph replays with

@@ -255,3 +255,22 @@ def test_append_pages_of_one_buffer(gpu, H, dtype, seqs):  # noqa: F811
     assert (gpu.get(ed, exps.shape, np.int8) == want[1]).all()
     assert (gpu.get(cd, codes.shape, np.uint8) == want[0]).all()
     batch.close()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_exponents_outside_their_range(gpu, n):  # noqa: F811
+    """Adopted storage may hold any int8: attend takes it for the range's end,
+    as append does with a page that held tokens."""
+    rng = np.random.default_rng(9)
+    P, D, L = 64, 64, 64 * 4 + 30
+    codes, exps = ref.pool(rng, 5, 1, P, D, spread=0.0)
+    codes[:, 0] = 0                                           # every key alike
+    table = ref.tables(rng, 5, [L], P)
+    for odd in ([0, -128, 3, -33, 0], [64, 0, 127, 0, -128]):
+        exps[:, 1, 0] = odd
+        exps[:, 0, 0] = odd[::-1]
+        q = rng.standard_normal((n, 2, D)).astype(ml_dtypes.bfloat16)
+        got = attend_gpu(gpu, codes, exps, table, [L], [n], q, "bf16")
+        kept = np.clip(exps, ref.E_MIN, ref.E_MAX)
+        want, bound = ref.attend(codes, kept, table, [L], [n], q.astype(float), D ** -0.5)
+        assert ref.close(got, want, bound, "bf16")
