@@ -1,6 +1,7 @@
 // emmy_kv8_attend -- attention of new queries over the paged 8-bit cache:
 // checks, workspace and plan, and which kernel takes which sequences.
 #include <cmath>
+#include <numeric>
 
 #include "kv8_attend.cuh"
 
@@ -163,8 +164,19 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   const auto extent = [&](const int64_t st[2]) {
     return uint64_t((cache->tokens - 1) * st[0] + (a->heads - 1) * st[1] + cache->head_dim) * 2;
   };
-  if (overlap(a->q, extent(a->q_strides), a->out, extent(a->out_strides)))
-    return fail(EMMY_EINVAL, what, "q and out overlap");
+  // rows of q and out in turn, as slices of one wider array are: of heads, of
+  // tokens where heads come first, or of elements
+  const auto in_turn = [&](int64_t step_q, int64_t step_out, int64_t wide_q, int64_t wide_out) {
+    if (step_q != step_out || step_q == 0) return false;
+    const int64_t by = int64_t(a->out - a->q) / 2 % step_q, off = by < 0 ? by + step_q : by;
+    return off >= wide_q && off + wide_out <= step_q;
+  };
+  if (overlap(a->q, extent(a->q_strides), a->out, extent(a->out_strides))) {
+    const int64_t qt = a->q_strides[0], qh = a->q_strides[1], step = std::gcd(std::gcd(qt, qh), std::gcd(ts, hs));
+    if (!in_turn(qt, ts, (Hq - 1) * qh + D, (Hq - 1) * hs + D) && !in_turn(qh, hs, (T - 1) * qt + D, (T - 1) * ts + D) &&
+        !in_turn(step, step, D, D))
+      return fail(EMMY_EINVAL, what, "q and out overlap");
+  }
   if (a->workspace == 0 || a->workspace % 16 || a->workspace_bytes < shape.workspace_bytes)
     return fail(EMMY_EINVAL, what, "workspace is missing, unaligned or too small");
   p.q = reinterpret_cast<const void *>(a->q);

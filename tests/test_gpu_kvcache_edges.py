@@ -274,3 +274,34 @@ def test_exponents_outside_their_range(gpu, n):  # noqa: F811
         kept = np.clip(exps, ref.E_MIN, ref.E_MAX)
         want, bound = ref.attend(codes, kept, table, [L], [n], q.astype(float), D ** -0.5)
         assert ref.close(got, want, bound, "bf16")
+
+
+def test_q_and_out_as_slices_of_one_array():
+    """Rows in turn do not overlap; rows that share an element do."""
+    torch = pytest.importorskip("torch")
+    from ptxgen import KVCache
+    from ptxgen.runtime import EmmyError
+    rng = np.random.default_rng(10)
+    P, D, H, G, kv, ql = 64, 64, 2, 2, [70, 300, 9], [1, 40, 2]
+    codes, exps = ref.pool(rng, 8, H, P, D)
+    table = ref.tables(rng, 8, kv, P)
+    c, e = torch.from_numpy(codes)[None].cuda(), torch.from_numpy(exps)[None].cuda()
+    cache, T, heads = KVCache(8, H, D, storage=(c, e)), sum(ql), H * G
+    q0 = torch.from_numpy(rng.standard_normal((T, heads, D))).half().cuda()
+    want, bound = ref.attend(codes, exps, table, kv, ql, q0.cpu().numpy().astype(float), D ** -0.5)
+    batch = cache.batch(table, kv, ql, stream=0)
+    wide = torch.zeros((T, 3 * heads, D), dtype=torch.float16, device="cuda")
+    cols = torch.zeros((T, heads, 3 * D), dtype=torch.float16, device="cuda")
+    deep = torch.zeros((heads, 3 * T, D), dtype=torch.float16, device="cuda")
+    for q, out in ((wide[:, :heads], wide[:, 2 * heads:]), (wide[:, heads:2 * heads], wide[:, :heads]),
+                   (cols[..., D:2 * D], cols[..., :D]), (cols[..., :D], cols[..., 2 * D:]),
+                   (deep[:, :T].transpose(0, 1), deep[:, T:2 * T].transpose(0, 1))):
+        q.copy_(q0)
+        batch.attend(0, q, out, stream=0)
+        assert ref.close(out.cpu().numpy(), want, bound, "f16") and torch.equal(q, q0)
+    for q, out in ((wide[:, :heads], wide[:, heads - 1:2 * heads - 1]), (wide[:, 1:heads + 1], wide[:, :heads]),
+                   (cols[..., :D], cols[..., D - 8:2 * D - 8]), (wide[:, :heads], wide[:, :heads]),
+                   (deep[:, :T].transpose(0, 1), deep[:, T - 1:2 * T - 1].transpose(0, 1))):
+        with pytest.raises(EmmyError, match="q and out overlap"):
+            batch.attend(0, q, out, stream=0)
+    batch.check_errors(stream=0)
