@@ -458,6 +458,7 @@ class Batch:
             with _Current(self.L, self.ordinal):
                 if _capturing(self.dev, st):
                     return st
+                _outside_capture(self.dev, self._stream, "another stream that waited for it would become part of the graph")
                 ev = self.dev.event()
                 try:
                     check(self.L.emmy_event_record(ev, self._stream), "event record")

@@ -216,3 +216,20 @@ def test_the_callers_current_device_stays(dev, monkeypatch):  # noqa: F811
         call()
         assert now[0] == 3
     assert seen >= by_device - {"sync"}
+
+
+def test_another_stream_does_not_join_a_capture(dev):  # noqa: F811
+    """A stream that waits for one that is captured becomes part of the graph."""
+    cache = small(dev)
+    b = cache.batch([[1]], [9], stream=5)
+    b.reserve(4, stream=5)
+    dev.L.emmy_stream_capturing = lambda st, word: setattr(word._obj, "value", int(st == 5)) or 0
+    dev.L.calls.clear()
+    with pytest.raises(EmmyError, match="captured"):
+        b.attend(0, *arrays(), stream=6)
+    assert not [name for name, _ in dev.L.calls if name in ("emmy_event_record", "emmy_kv8_attend")]
+    b.attend(0, *arrays(), stream=5)                 # the capture goes on
+    dev.L.emmy_stream_capturing = lambda st, word: setattr(word._obj, "value", int(st == 6)) or 0
+    b.attend(0, *arrays(), stream=6)                 # into a capture that does not wait
+    b.attend(0, *arrays(), stream=7)
+    assert [a[0] for name, a in dev.L.calls if name == "emmy_stream_wait_event"] == [7]
