@@ -31,6 +31,7 @@ Arrays are device arrays: anything with ``data_ptr()``, ``stride()``,
 queued on ``stream`` (an address, or an object with ``cuda_stream``; default
 the device's stream, ``Device.stream``; 0 is the legacy default stream),
 return at once and allocate nothing after the first ``attend`` of a batch;
+they leave the thread's current device as it was;
 the caller keeps the arrays alive until the work is done and orders streams,
 as with every other call here (a batch used on a stream other than the one it
 was made on waits for that once).
@@ -144,7 +145,8 @@ class _Current:
         self.before = word.value
 
     def __exit__(self, *exc):
-        self.L.emmy_device_leave(self.before)
+        if self.before != self.ordinal:
+            self.L.emmy_device_leave(self.before)
 
 
 def _at_home(method):
@@ -208,17 +210,19 @@ class _Pool:
     MOST = 512 << 20
 
     @classmethod
-    def of(cls, dev: Device) -> "_Pool":
-        return dev.__dict__.get("_kv_pool") or dev.__dict__.setdefault("_kv_pool", cls(dev))
+    def of(cls, dev: Device, ordinal: int = 0) -> "_Pool":
+        return dev.__dict__.get("_kv_pool") or dev.__dict__.setdefault("_kv_pool", cls(dev, ordinal))
 
-    def __init__(self, dev: Device):
-        self.dev, self.held, self.bytes, self.gone = dev, {}, 0, []
+    def __init__(self, dev: Device, ordinal: int):
+        self.dev, self.ordinal, self.held, self.bytes, self.gone = dev, ordinal, {}, 0, []
         self.lock = threading.RLock()   # a collection inside of it may close a batch
 
-    def take(self, use: str, nbytes: int, stream: int) -> tuple[int, tuple]:
-        """(address, key to give it back by) of a buffer for work on ``stream``."""
-        key = (use, 1 << max(12, (nbytes - 1).bit_length()), _stream_id(self.dev, stream))
-        self.drain()
+    def take(self, use: str, nbytes: int, stream: int, sid: int) -> tuple[int, tuple]:
+        """(address, key to give it back by) of a buffer for work on ``stream``,
+        whose id is ``sid``."""
+        key = (use, 1 << max(12, (nbytes - 1).bit_length()), sid)
+        if self.gone:
+            self.drain()
         with self.lock:
             held = self.held.get(key)
             if held:
@@ -231,35 +235,37 @@ class _Pool:
 
     def drain(self) -> None:
         """Free what is not to be used again: waits for what still runs on it."""
-        while self.gone:
-            try:
-                ptr = self.gone.pop()
-            except IndexError:          # another thread's turn
-                break
-            self.dev.free(ptr)
+        with _Current(self.dev.L, self.ordinal):
+            while self.gone:
+                try:
+                    ptr = self.gone.pop()
+                except IndexError:      # another thread's turn
+                    break
+                self.dev.free(ptr)
 
     def give(self, ptr: int, key: tuple, reuse: bool, later: bool = False) -> None:
         """``later``: what is to be freed is at the next call of ``take``, for a
         collection may come while some stream is captured, and memory that is
         freed then ends the capture."""
-        gone = [] if reuse else [ptr]
         with self.lock:
-            if reuse:
-                for other in [k for k in self.held if k[2] != key[2]]:
-                    spare = self.held.get(other)
-                    while spare and self.bytes + key[1] > self.MOST:
-                        gone.append(spare.pop())
-                        self.bytes -= other[1]
-                    if not spare:
-                        self.held.pop(other, None)
-                if self.bytes + key[1] <= self.MOST:
-                    self.held.setdefault(key, []).append(ptr)
-                    self.bytes += key[1]
-                else:
-                    gone.append(ptr)
-        self.gone += gone
-        if not later:
+            if reuse and self.bytes + key[1] > self.MOST:
+                self._make_room(key)
+            if reuse and self.bytes + key[1] <= self.MOST:
+                self.held.setdefault(key, []).append(ptr)
+                self.bytes += key[1]
+            else:
+                self.gone.append(ptr)
+        if self.gone and not later:
             self.drain()
+
+    def _make_room(self, key: tuple) -> None:
+        for other in [k for k in self.held if k[2] != key[2]]:
+            spare = self.held.get(other)
+            while spare and self.bytes + key[1] > self.MOST:
+                self.gone.append(spare.pop())
+                self.bytes -= other[1]
+            if not spare:
+                self.held.pop(other, None)
 
 
 class KVCache:
@@ -315,7 +321,7 @@ class KVCache:
         layers = self.layers
         self.dev = Device.get(self.ordinal)
         if allocate:
-            _Pool.of(self.dev).drain()
+            _Pool.of(self.dev, self.ordinal).drain()
             for attr, n in (("codes", layers * self.layer_codes), ("exps", layers * self.layer_exps)):
                 ptr = self.dev.alloc(n)
                 self._own.append(ptr)
@@ -419,8 +425,9 @@ class Batch:
         host = self._packed(table, kv_lens, q_lens)
         self._stream, self._reuse = _stream_of(stream, self.dev), True
         _outside_capture(self.dev, self._stream, "lengths and page numbers are copied from the host")
-        self._pool, self._captured = _Pool.of(self.dev), _captured(self.dev)
-        self._who = self._same(self._stream)
+        self._pool, self._captured = _Pool.of(self.dev, cache.ordinal), _captured(self.dev)
+        self._id = _stream_id(self.dev, self._stream)
+        self._who = self._id if self._stream == PER_THREAD else self._stream
         self._others: set[int] = set()             # further streams it was used on
         self._buf = self._take("batch", host.nbytes, self._stream)
         _copy_in(self.dev, self._buf, host, self._stream)
@@ -437,20 +444,16 @@ class Batch:
         self._append, self._attend = self.L.emmy_kv8_append, self.L.emmy_kv8_attend
 
     def _take(self, use: str, nbytes: int, st: int) -> int:
-        held = self._pool.take(use, nbytes, st)
+        held = self._pool.take(use, nbytes, st, self._id if st == self._stream else _stream_id(self.dev, st))
         self._held.append(held)
         return held[0]
-
-    def _same(self, st: int) -> int:
-        """What tells whether a handle means the stream that it did before."""
-        return st if st != PER_THREAD else _stream_id(self.dev, st)
 
     def _on(self, stream) -> int:
         """The handle of ``stream``; one other than the batch's own waits, the
         first time, for what is queued on that (its lengths, a page copy).
         One that is being captured cannot wait: its graph is replayed after."""
         st = _stream_of(stream, self.dev)
-        who = st if st != PER_THREAD else self._same(st)
+        who = st if st != PER_THREAD else _stream_id(self.dev, st)
         if who != self._who and who not in self._others:
             if self._stream == PER_THREAD:
                 raise EmmyError("a batch made on the per-thread default stream is for that thread and stream")
@@ -458,7 +461,8 @@ class Batch:
             with _Current(self.L, self.ordinal):
                 if _capturing(self.dev, st):
                     return st
-                _outside_capture(self.dev, self._stream, "another stream that waited for it would become part of the graph")
+                _outside_capture(self.dev, self._stream,
+                                 "another stream that waited for it would become part of the graph")
                 ev = self.dev.event()
                 try:
                     check(self.L.emmy_event_record(ev, self._stream), "event record")
@@ -495,7 +499,8 @@ class Batch:
         span = np.arange(self.width)
         written = table[(span >= ((kv - q) // P)[:, None]) & (span <= ((kv - 1) // P)[:, None])
                         & (q > 0)[:, None]]
-        self._clash = len(np.unique(written)) != len(written)
+        # (np.unique costs 6 us however few there are)
+        self._clash = len(set(written.tolist()) if len(written) < 256 else np.unique(written)) != len(written)
         host = np.zeros(4 + 2 * B + 1 + B * self.width, np.int32)
         host[4:4 + B] = kv
         host[5 + B:5 + 2 * B] = np.cumsum(q)
@@ -661,9 +666,7 @@ class Batch:
     def _close(self, later: bool) -> None:
         held, self._held = self._held, []
         self._buf, self._ws, self._plans = 0, (0, 0), {}
-        if not held:
-            return
-        with _Current(self.L, self.ordinal):
+        if held:
             reuse = self._reuse and _captured(self.dev) == self._captured
             for ptr, key in held:
                 self._pool.give(ptr, key, reuse, later)
@@ -730,7 +733,9 @@ class KVSequences:
             self._free.append(page)
 
     def truncate(self, sid: int, length: int) -> None:
-        """Forget the tokens from position ``length`` on (rejected drafts)."""
+        """Forget the tokens from position ``length`` on (rejected drafts).  The
+        last page keeps the scale that forgotten ones asked for, and its older
+        tokens the rounding to that."""
         self._known(sid)
         if not 0 <= length <= self._len[sid]:
             raise EmmyError(f"truncate: sequence {sid} has {self._len[sid]} tokens")
@@ -827,8 +832,9 @@ class KVSequences:
 
     def compact(self, stream=None) -> int:
         """Move pages so that those in use are the first ones of the pool;
-        returns how many are in use.  Batches made before name old pages and
-        refuse to run until updated."""
+        returns how many are in use.  Batches that ``batch`` made before name
+        old pages and refuse to run until updated; graphs captured over them,
+        and batches of tables kept elsewhere, must not run until then."""
         used = [p for p, n in enumerate(self._refs) if n]
         n = len(used)
         holes = [p for p in range(n) if not self._refs[p]]
