@@ -168,8 +168,12 @@ __device__ __forceinline__ int row_exponent(float amax) {
 
 // Rows of a kv head up to which a sequence is the row kernel's, in blocks of at
 // most ROWS_BLOCK rows that each read the keys again, from L2, as neighbours: 16
-// rows' sums are what registers hold at three CTAs an SM (blocks of 32 at two:
-// 28.4 us against 29.5 for five drafts of 16 sequences, but spills from 25 rows on).
+// rows' sums are what registers hold at three CTAs an SM, but for one register's
+// spill where d = 128 and clusters join (blocks of 32 at two CTAs: 28.4 us against
+// 29.5 for five drafts of 16 sequences, but spills from 25 rows on).  Row kernel |
+// tile kernel, 16 sequences of 500-6000 keys, by rows, us: d = 128, 5 heads: 17:
+// 33 | 57, 32: 36 | 58, 40: 51 | 58, 48: 53 | 58, 64: 61 | 58; d = 64, 8 heads: 17:
+// 36 | 58, 32: 38 | 60, 40: 65 | 60, 48: 65 | 76, 64: 74 | 76.
 constexpr int ROWS_MOST = 32, ROWS_BLOCK = 16;
 constexpr int ROWS_PER_SM = 3;  // CTAs of the row kernel, by its launch bounds
 constexpr int TILE_ROWS = 256;  // rows of a unit of the tile kernel

@@ -5,10 +5,11 @@
 // its visible 64-key chunks.  Where all segments fit on the GPU at once, parts
 // of at most q chunks, q the least of a few tries that leaves them one wave:
 // equal parts that start together.  Otherwise (spread) two waves of parts of
-// about equal length, which the order of arrival evens out.  Measured before
-// the plan was a kernel of its own (us, one wave | two): 2 sequences of 131071
-// keys 37 | 43, 48 with a window of 1024 19 | 28, 16 with five drafts 33 | 41;
-// but 64 of 700-8191 keys, 512 segments on 444 CTAs, 111 | 97.  Short segments
+// about equal length, which the order of arrival evens out.  Measured, without
+// clusters (us, one wave | two): 2 sequences of 131071 keys 34.8 | 40.0, 48 with
+// a window of 1024 16.4 | 24.9, 16 with five drafts 33.0 | 39.3; but, with more
+// segments than the 444 CTAs that fit, 64 of 700-8191 keys 117.8 | 112.8 and 56
+// of 4000 92.4 | 89.3.  Short segments
 // (by what the table can hold) are a cluster each, whose CTAs join in shared
 // memory, and a few long ones some clusters each: fewer partial results go
 // through the workspace.  Some of a cluster's parts may be empty.
@@ -19,8 +20,9 @@
 // the longest of one round get the shortest of the next.
 //
 // One CTA: a thread takes a few sequences, scans give each its first record,
-// and the records are then written a thread each.  A layer's worth of work for
-// attend is some microseconds, and every layer of a step shares the plan.
+// and the records are then written a thread each.  Every layer of a step shares
+// the plan: 7.6 us for one sequence of 1025 keys, 10.4 for 64 of 700-8191, 21 for
+// 4096 of 1-200, 35 for six prompts of 200-1500 tokens.
 #include "kv8_attend.cuh"
 
 namespace kv8 {

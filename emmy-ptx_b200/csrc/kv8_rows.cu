@@ -11,8 +11,13 @@
 // from it).  A query row is scaled by a power of two so that its largest
 // element lies in [1, 2) before it becomes f16: a bf16 row is exact down to
 // 2^-14 of that element and rounded by at most 2^-25 of it below.  Scores,
-// maxima, sums and O are f32; p is rounded to f16 (2^-12 relative), the only
-// rounding of width before the output's.
+// maxima, sums and O are f32; p is rounded to f16, because both products are
+// f16's: by up to 2^-11 of it, and where it is below 2^-14 by up to 2^-25 of its
+// unit, which is at most 2^6 of the row's (V's exponent may stray by so much).
+// Their sum l is of the weights before that rounding -- of those after it would
+// cost a conversion a weight -- so an f16 output differs from f32 arithmetic's
+// in its last bit (2.4e-4 from 64 bits where f32 weights are 2.1e-4, very long
+// keys), and many small weights beside a large one lose bits that l has.
 //
 // The order of a contraction's terms is free, so a lane's 16 consecutive bytes
 // of a key serve as its shares of four k-steps, and of a value row as the rows
@@ -22,14 +27,15 @@
 // that HBM's latency asks for cost no registers.  The TMA's swizzle spreads
 // the rows that the lanes of a load read over all banks.
 //
-// Bound by memory: codes are read once per kv head.  A segment -- one sequence,
-// kv head and block of rows -- is cut into about as many parts of 64-key chunks as its share
-// of a target number of parts, a CTA a part, so uneven lengths balance and
+// Bound by memory: codes are read once for each block of up to 16 rows of a kv
+// head, by neighbours, so from memory once.  A segment -- one sequence, kv head
+// and block of rows -- is cut into about as many parts of 64-key chunks as its
+// share of a target number of parts, a CTA a part, so uneven lengths balance and
 // one long sequence fills the GPU, while a segment of about a part's length
 // stays whole and needs no join.  Parts of a cut segment leave (m, l, O) in
-// the workspace; the last of each 16 parts to arrive joins them in their
-// order, the last of those their sums, so results do not depend on the order
-// of arrival.  Where there are few segments, clusters of CTAs join their parts
+// the workspace; up to ONE_LEVEL of them are joined by the last to arrive, in
+// their order, more in groups by the last of each group and then the groups by
+// the last of those, so results do not depend on the order of arrival.  Where there are few segments, clusters of CTAs join their parts
 // first, each a share of the rows' values out of the others' shared memory:
 // a short segment is one cluster and needs neither the workspace nor its round
 // trips to L2, a long one leaves a result a cluster there.
@@ -45,8 +51,10 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = 160, ALL_WARPS = 5;  // four that compute, one that loads
 constexpr float LAZY = 8.0f;  // log2 units that scores may pass the reference before O moves
-constexpr int GROUP = 16;     // parts of a segment that one CTA joins at once,
-constexpr int ONE_LEVEL = 24; // or up to this many where that leaves one level
+// Parts of a segment that one CTA joins at once, or up to ONE_LEVEL where that
+// leaves one level (one level | two, us: 23 results 33.5 | 35.0, 28 results 17.6 |
+// 18.5, 52 results 23.5 | 21.5).
+constexpr int GROUP = 16, ONE_LEVEL = 24;
 constexpr int MOST_CLUSTER = 8;
 constexpr int UNIT_LAZY = 6;  // the same for V's exponent: p stays below 2^14 in f16
 
@@ -695,7 +703,7 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
       __stcg(part_slot(a) + ROWS * D + ROWS + tid, row_l[tid]);
     }
   };
-  // up to 64 at once where one level does, else groups of GROUP
+  // all at once up to ONE_LEVEL, else groups of GROUP, or more if there were over 64
   const int group = results <= ONE_LEVEL ? results : max(GROUP, (results + 63) / 64);
   const int lead = result / group * group, count = min(group, results - lead);
   const int groups = (results + group - 1) / group;
