@@ -35,10 +35,11 @@
 // stays whole and needs no join.  Parts of a cut segment leave (m, l, O) in
 // the workspace; up to ONE_LEVEL of them are joined by the last to arrive, in
 // their order, more in groups by the last of each group and then the groups by
-// the last of those, so results do not depend on the order of arrival.  Where there are few segments, clusters of CTAs join their parts
-// first, each a share of the rows' values out of the others' shared memory:
-// a short segment is one cluster and needs neither the workspace nor its round
-// trips to L2, a long one leaves a result a cluster there.
+// the last of those, so results do not depend on the order of arrival.  Where
+// there are few segments, clusters of CTAs join their parts first, each a share
+// of the rows' values out of the others' shared memory: a short segment is one
+// cluster and needs neither the workspace nor its round trips to L2, a long one
+// leaves a result a cluster there.
 #include <cuda_bf16.h>
 
 #include <cuda.h>  // CUtensorMap
@@ -716,7 +717,7 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
 // Beside the tile kernel, which was launched before it and whose sequences are
 // others, it starts when all of that kernel's CTAs run: SMs without a unit, or
 // past their last, take parts (512 tokens behind 3584 keys with 47 single tokens
-// of 700-8191 keys: 175 -> 131 us a call).  What came before both is done then;
+// of 700-8191 keys: 175 -> 129 us a call).  What came before both is done then;
 // that it is also visible here, without this kernel's own wait, follows from
 // the word that the tile kernel released after its wait, and a block that does
 // not find it there waits.  The last block to have looked takes the word back.

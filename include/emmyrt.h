@@ -250,7 +250,8 @@ int emmy_kv8_append(const emmy_kv8 *cache, emmy_dptr k, emmy_dptr v, int32_t dty
 /* out = softmax(scale * q K^T, hidden keys left out) V for the new tokens'
  * queries, q and out [tokens][heads][head_dim] of `dtype` (bf16 or f16),
  * laid out as for append and not overlapping; heads a multiple of kv_heads, query head h
- * reads kv head h / (heads / kv_heads).  Scores are f32: one past its range is
+ * reads kv head h / (heads / kv_heads).  Scores are f32, and so is
+ * scale * log2(e) times a query row's largest magnitude: one past its range is
  * an infinity, with f32's consequences.  Query i of n in a sequence of L keys
  * stands at position p = L - n + i and sees key j when j <= p and (window ==
  * 0, or p - j < window, or j < sinks).  A query that sees no key gives zeros.
