@@ -180,5 +180,13 @@ void wait_limit(unsigned long long &ns, int &stall);
 inline bool overlap(emmy_dptr a, uint64_t na, emmy_dptr b, uint64_t nb) {
   return a < b + nb && b < a + na;
 }
+// What is wrong with an array [T][q_heads][D] that a call reads and one [T][H][D]
+// that it writes (strides in elements of so many bytes): a negative stride, rows of
+// the output that overlap each other, or the input.  `in_place`: they are the same.
+enum { ROWS_FINE = 0, ROWS_NEGATIVE, ROWS_SELF, ROWS_BOTH };
+int rows_trouble(emmy_dptr q, const int64_t q_strides[2], int64_t q_heads, int q_size, emmy_dptr out,
+                 const int64_t out_strides[2], int64_t H, int size, int64_t T, int64_t D, bool in_place);
+// What is wrong with a description of rotary positions, null: nothing.
+const char *rotary_trouble(const emmy_rotary *r);
 
 }  // namespace kv8

@@ -1,7 +1,6 @@
 // emmy_kv8_attend -- attention of new queries over the paged 8-bit cache:
 // checks, workspace and plan, and which kernel takes which sequences.
 #include <cmath>
-#include <numeric>
 
 #include "kv8_attend.cuh"
 
@@ -154,29 +153,12 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   if (a->q % 16 || a->out % 16 || a->q_strides[0] % 8 || a->q_strides[1] % 8 || a->out_strides[0] % 8 ||
       a->out_strides[1] % 8)
     return fail(EMMY_EINVAL, what, "q and out: base and strides must be multiples of 16 bytes");
-  if (a->q_strides[0] < 0 || a->q_strides[1] < 0 || a->out_strides[0] < 0 || a->out_strides[1] < 0)
-    return fail(EMMY_EINVAL, what, "q and out: strides must not be negative");
-  // rows of out one after another, tokens within heads or heads within tokens
-  const int64_t ts = a->out_strides[0], hs = a->out_strides[1], D = cache->head_dim;
-  const int64_t T = cache->tokens, Hq = a->heads;
-  if ((T > 1 && ts < D) || (Hq > 1 && hs < D) || (T > 1 && Hq > 1 && (ts <= hs ? hs < ts * (T - 1) + D : ts < hs * (Hq - 1) + D)))
-    return fail(EMMY_EINVAL, what, "rows of out overlap");
-  const auto extent = [&](const int64_t st[2]) {
-    return uint64_t((cache->tokens - 1) * st[0] + (a->heads - 1) * st[1] + cache->head_dim) * 2;
-  };
-  // rows of q and out in turn, as slices of one wider array are: of heads, of
-  // tokens where heads come first, or of elements
-  const auto in_turn = [&](int64_t step_q, int64_t step_out, int64_t wide_q, int64_t wide_out) {
-    if (step_q != step_out || step_q == 0) return false;
-    const int64_t by = int64_t(a->out - a->q) / 2 % step_q, off = by < 0 ? by + step_q : by;
-    return off >= wide_q && off + wide_out <= step_q;
-  };
-  if (overlap(a->q, extent(a->q_strides), a->out, extent(a->out_strides))) {
-    const int64_t qt = a->q_strides[0], qh = a->q_strides[1], step = std::gcd(std::gcd(qt, qh), std::gcd(ts, hs));
-    if (!in_turn(qt, ts, (Hq - 1) * qh + D, (Hq - 1) * hs + D) && !in_turn(qh, hs, (T - 1) * qt + D, (T - 1) * ts + D) &&
-        !in_turn(step, step, D, D))
-      return fail(EMMY_EINVAL, what, "q and out overlap");
-  }
+  const int bad = rows_trouble(a->q, a->q_strides, a->heads, 2, a->out, a->out_strides, a->heads, 2, cache->tokens,
+                               cache->head_dim, false);
+  if (bad != ROWS_FINE)
+    return fail(EMMY_EINVAL, what, bad == ROWS_NEGATIVE ? "q and out: strides must not be negative"
+                                   : bad == ROWS_SELF   ? "rows of out overlap"
+                                                        : "q and out overlap");
   if (a->workspace == 0 || a->workspace % 16 || a->workspace_bytes < shape.workspace_bytes)
     return fail(EMMY_EINVAL, what, "workspace is missing, unaligned or too small");
   p.q = reinterpret_cast<const void *>(a->q);

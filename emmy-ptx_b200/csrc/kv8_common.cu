@@ -1,5 +1,7 @@
 // Host-side checks shared by the entry points of the paged 8-bit cache.
+#include <cmath>
 #include <cstdio>
+#include <numeric>
 
 #include "kv8.cuh"
 
@@ -65,6 +67,40 @@ int check_counts(const char *what, const emmy_kv8 *c) {
   if (int64_t(c->table_width) * c->page_size > (int64_t(1) << 30))
     return fail(EMMY_EINVAL, what, "a sequence holds at most 2^30 keys");
   return EMMY_OK;
+}
+
+int rows_trouble(emmy_dptr q, const int64_t q_strides[2], int64_t q_heads, int q_size, emmy_dptr out,
+                 const int64_t out_strides[2], int64_t H, int size, int64_t T, int64_t D, bool in_place) {
+  const int64_t qt = q_strides[0], qh = q_strides[1], ts = out_strides[0], hs = out_strides[1];
+  if (qt < 0 || qh < 0 || ts < 0 || hs < 0) return ROWS_NEGATIVE;
+  // rows of out one after another, tokens within heads or heads within tokens
+  if ((T > 1 && ts < D) || (H > 1 && hs < D) || (T > 1 && H > 1 && (ts <= hs ? hs < ts * (T - 1) + D : ts < hs * (H - 1) + D)))
+    return ROWS_SELF;
+  if (in_place) return ROWS_FINE;
+  if (!overlap(q, uint64_t((T - 1) * qt + (q_heads - 1) * qh + D) * q_size, out,
+               uint64_t((T - 1) * ts + (H - 1) * hs + D) * size))
+    return ROWS_FINE;
+  if (q_size != size) return ROWS_BOTH;
+  // rows of both in turn, as slices of one wider array are: of heads, of
+  // tokens where heads come first, or of elements
+  const auto in_turn = [&](int64_t step_q, int64_t step_out, int64_t wide_q, int64_t wide_out) {
+    if (step_q != step_out || step_q == 0) return false;
+    const int64_t by = int64_t(out - q) / size % step_q, off = by < 0 ? by + step_q : by;
+    return off >= wide_q && off + wide_out <= step_q;
+  };
+  const int64_t step = std::gcd(std::gcd(qt, qh), std::gcd(ts, hs));
+  if (in_turn(qt, ts, (q_heads - 1) * qh + D, (H - 1) * hs + D) || in_turn(qh, hs, (T - 1) * qt + D, (T - 1) * ts + D) ||
+      in_turn(step, step, D, D))
+    return ROWS_FINE;
+  return ROWS_BOTH;
+}
+
+const char *rotary_trouble(const emmy_rotary *r) {
+  if (r == nullptr) return "null rotary description";
+  if (r->head_dim < 2 || r->head_dim > 2 * EMMY_ROTARY_PAIRS) return "head_dim must be between 2 and 512";
+  if (r->dims < 2 || r->dims % 2 != 0 || r->dims > r->head_dim) return "dims must be even, between 2 and head_dim";
+  if (!std::isfinite(r->gain)) return "gain must be finite";
+  return nullptr;
 }
 
 int sm_count(int device) {

@@ -24,12 +24,16 @@ def run_problem(pdir, **kw):
 
 
 def __getattr__(name):
-    # the paged key/value cache needs the runtime library, the compiler does not
+    # the paged key/value cache and rotary positions need the runtime library, the
+    # compiler does not
     if name in ("KVCache", "KVSequences", "DeviceArray"):
         from . import kvcache
         return getattr(kvcache, name)
+    if name == "Rotary":
+        from .rotary import Rotary
+        return Rotary
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 __all__ = ["load_kernel", "compile_kernel", "compile_file", "run_kernel", "run_problem",
-           "KVCache", "KVSequences", "DeviceArray"]
+           "KVCache", "KVSequences", "DeviceArray", "Rotary"]

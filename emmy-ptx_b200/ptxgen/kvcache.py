@@ -83,9 +83,17 @@ class _Attend(C.Structure):
 _Strides = C.c_int64 * 2
 
 
+class _Rotated(C.Structure):
+    """``emmy_kv8_rotated_args``."""
+    _fields_ = [("positions", C.c_uint64), ("q", C.c_uint64), ("q_out", C.c_uint64),
+                ("position_stride", C.c_int64), ("q_strides", _Strides), ("out_strides", _Strides),
+                ("wide", C.c_int32), ("heads", C.c_int32), ("out_dtype", C.c_int32)]
+
+
 class DeviceArray:
     """A view of device memory at a raw address: ``dtype`` one of "f32",
-    "bf16", "f16", "u8", "i8"; strides in elements, row-major by default."""
+    "bf16", "f16", "u8", "i8", "i32", "i64"; strides in elements, row-major by
+    default."""
 
     def __init__(self, ptr: int, dtype: str, shape, strides=None, device: int = 0):
         self.ptr, self.dtype, self.shape, self.device = int(ptr), dtype, tuple(shape), device
@@ -107,9 +115,9 @@ class DeviceArray:
         return self.device
 
 
-_DTYPES = {"f32": 0, "bf16": 1, "f16": 2, "u8": 3, "i8": 4}
+_DTYPES = {"f32": 0, "bf16": 1, "f16": 2, "u8": 3, "i8": 4, "i32": 5, "i64": 6}
 _NAMES = {"float32": "f32", "bfloat16": "bf16", "float16": "f16", "half": "f16", "uint8": "u8",
-          "int8": "i8", "float8_e4m3fn": "u8"}
+          "int8": "i8", "float8_e4m3fn": "u8", "int32": "i32", "int64": "i64"}
 
 
 def _dtype_code(dtype) -> int:
@@ -121,6 +129,27 @@ def _dtype_code(dtype) -> int:
             raise EmmyError(f"unsupported dtype {dtype}")
         _DTYPES[dtype] = code
     return code
+
+
+def _positions(positions, tokens: int, ordinal: int) -> tuple[int, int, int, int]:
+    """(address or 0, stride, whether they are int64, first) of positions: an
+    int32 or int64 device array, or the first of consecutive ones."""
+    if hasattr(positions, "data_ptr"):
+        if len(positions.shape) != 1 or positions.shape[0] < tokens:
+            raise EmmyError(f"positions has shape {tuple(positions.shape)}, expected [>= {tokens}]")
+        code = _dtype_code(positions.dtype)
+        if code not in (5, 6):
+            raise EmmyError("positions must be int32 or int64")
+        if positions.get_device() != ordinal:
+            raise EmmyError(f"positions is not on device {ordinal}")
+        return positions.data_ptr(), positions.stride()[0], int(code == 6), 0
+    try:
+        first = positions.__index__()
+    except AttributeError:
+        raise EmmyError("positions is a device array, or a whole number") from None
+    if not -2 ** 63 <= first <= 2 ** 63 - 1 - tokens:
+        raise EmmyError("positions must fit 64 bits")
+    return 0, 0, 0, first
 
 
 def _stream_of(stream, dev: Device) -> int:
@@ -560,9 +589,15 @@ class Batch:
         code = _DTYPES.get(x.dtype)
         return x.data_ptr(), _dtype_code(x.dtype) if code is None else code, stride, shape[1]
 
-    def append(self, layer: int, k, v, stream=None) -> None:
+    def append(self, layer: int, k, v, stream=None, *, rotary=None, q=None, q_out=None,
+               positions=None) -> None:
         """Write the new tokens' keys and values (f32, bf16 or f16) into
-        their pages of ``layer``."""
+        their pages of ``layer``.  ``rotary``, a ``Rotary``: the keys are
+        turned to their places in their sequences on the way (or to
+        ``positions``, an int32 or int64 device array of one a token), and so
+        are queries ``q`` [tokens, heads, head_dim], of the keys' type, into
+        ``q_out`` (f32, bf16 or f16; ``q`` itself, or no element of q, k or
+        v)."""
         self._usable(layer)
         if self._clash:
             raise EmmyError("append: two sequences of the batch write to the same page")
@@ -572,9 +607,37 @@ class Batch:
             raise EmmyError("append: k and v must both be f32, bf16 or f16")
         sk, sv = self._ks, self._vs
         sk[0], sk[1], sv[0], sv[1] = ks[0], ks[1], vs[0], vs[1]
+        if rotary is not None:
+            a = self._rotated(rotary, kt, q, q_out, positions)
+            rc = self.L.emmy_kv8_append_rotated(self._ref, kp, vp, kt, sk, sv, rotary._ref, C.byref(a),
+                                                self._on(stream))
+            if rc:
+                check(rc, "append")
+            return
+        if q is not None or q_out is not None or positions is not None:
+            raise EmmyError("append: q, q_out and positions are for a rotary")
         rc = self._append(self._ref, kp, vp, kt, sk, sv, self._on(stream))
         if rc:
             check(rc, "append")
+
+    def _rotated(self, rotary, kt: int, q, q_out, positions) -> _Rotated:
+        if getattr(rotary, "head_dim", None) != self.cache.head_dim:
+            raise EmmyError(f"append: rotary is for heads of {getattr(rotary, 'head_dim', 'no')} values, "
+                            f"not {self.cache.head_dim}")
+        at = step = wide = 0
+        if positions is not None:
+            if not hasattr(positions, "data_ptr"):
+                raise EmmyError("append: positions is a device array")
+            at, step, wide, _ = _positions(positions, self.tokens, self.cache.ordinal)
+        if (q is None) != (q_out is None):
+            raise EmmyError("append: q and q_out go together")
+        if q is None:
+            return _Rotated(position_stride=step, positions=at, wide=wide)
+        qp, qt, qs, heads = self._array(q, "q", None)
+        op, ot, os_, _ = self._array(q_out, "q_out", heads)
+        if qt != kt or ot > 2:
+            raise EmmyError("append: q must be of the keys' type, and q_out f32, bf16 or f16")
+        return _Rotated(at, qp, op, step, (qs[0], qs[1]), (os_[0], os_[1]), wide, heads, ot)
 
     def reserve(self, heads: int, window: int = 0, sinks: int = 0, stream=None) -> None:
         """What ``attend`` needs for ``heads`` query heads, a window and sinks

@@ -45,7 +45,7 @@ enum {
   EMMY_ENOENTRY = -4,   /* entry point not in module (runner stage "lookup") */
   EMMY_EKERNEL = -5,    /* a kernel reported an error in its error word */
   EMMY_ESYMBOL = -6,    /* module global not found */
-  EMMY_ECUDART = -7     /* a CUDA runtime call failed (emmy_sum_f32_noalloc, emmy_kv8_*) */
+  EMMY_ECUDART = -7     /* a CUDA runtime call failed (emmy_sum_f32_noalloc, emmy_kv8_*, emmy_rotate) */
 };
 
 /* Library identity and the last error message of the calling thread. */
@@ -201,6 +201,39 @@ int emmy_nccl_destroy(emmy_comm *comm);
  * emmy_last_error()), never a raw cudaError_t. */
 int emmy_sum_f32_noalloc(emmy_dptr x, size_t n, emmy_dptr out, emmy_stream stream);
 
+/* types of rows of queries, keys and values */
+enum { EMMY_KV8_F32 = 0, EMMY_KV8_BF16 = 1, EMMY_KV8_F16 = 2 };
+
+/* ---- rotary positions ----
+ * No counterpart in the reference.  The first `dims` values of each head are
+ * pairs (a, b): neighbours where `interleaved`, else dims / 2 apart.  Pair i of
+ * a token at position p turns by p * turns[i] * 2^-64 whole turns and is scaled
+ * by `gain`; the values behind `dims` stay as they are.  The multiplication is
+ * modulo 2^64, so angles are exact at any position, negative ones too. */
+enum { EMMY_ROTARY_PAIRS = 256 };
+typedef struct {
+  uint64_t turns[EMMY_ROTARY_PAIRS]; /* frequency / (2 pi) * 2^64, rounded */
+  float gain;
+  int32_t head_dim, dims; /* head_dim 2 .. 512, dims even */
+  int32_t interleaved;
+} emmy_rotary;
+
+/* out = the rows x [tokens][heads][head_dim] turned (or, `backward`, turned back
+ * and scaled by gain: the gradient of x from that of out), f32, bf16 or f16 (the
+ * EMMY_KV8_* types), computed in f32 and rounded once.  Innermost dimension
+ * contiguous, strides in elements (token, head), none negative; 16-byte pieces
+ * where addresses, strides and dims allow, else smaller ones.  `out` may be x
+ * itself, or share no element with it.  Token t stands at positions[t *
+ * position_stride] (int32, or int64 where `wide`), or at first + t where
+ * positions is 0.  Allocates nothing and does not synchronise. */
+typedef struct {
+  emmy_dptr x, out, positions;
+  int64_t x_strides[2], out_strides[2];
+  int64_t position_stride, first, tokens;
+  int32_t heads, dtype, wide, backward, device;
+} emmy_rotate_args;
+int emmy_rotate(const emmy_rotary *rotary, const emmy_rotate_args *args, emmy_stream stream);
+
 /* ---- paged 8-bit key/value cache ----
  * No counterpart in the reference, whose attention recomputes every key.  A
  * layer of the cache is a pool of pages in caller-owned device memory:
@@ -235,7 +268,6 @@ typedef struct {
 } emmy_kv8;
 
 enum { EMMY_KV8_MAX_SEQS = 4096, EMMY_KV8_MAX_PAIRS = 480 };
-enum { EMMY_KV8_F32 = 0, EMMY_KV8_BF16 = 1, EMMY_KV8_F16 = 2 };
 
 /* Write the new tokens' keys and values, k and v [tokens][kv_heads][head_dim]
  * of `dtype`, innermost dimension contiguous, strides in elements (token,
@@ -246,6 +278,24 @@ enum { EMMY_KV8_F32 = 0, EMMY_KV8_BF16 = 1, EMMY_KV8_F16 = 2 };
  * 448 * 2^63 and infinities saturate; NaN stays NaN. */
 int emmy_kv8_append(const emmy_kv8 *cache, emmy_dptr k, emmy_dptr v, int32_t dtype,
                     const int64_t k_strides[2], const int64_t v_strides[2], emmy_stream stream);
+
+/* The same of keys turned to their positions on the way (in f32, rounded only to
+ * codes), `rotary` for the cache's head_dim; and of `heads` query heads (0:
+ * none), q [tokens][heads][head_dim] of `dtype` turned into q_out of
+ * `out_dtype`, laid out as k.  q_out may be q itself where their types are the
+ * same, and shares no element with k, v or q otherwise.  A token stands at its
+ * place in its sequence, or where `positions` (as emmy_rotate's, a row of them
+ * for each of `tokens`) says.  A sequence that is skipped keeps its rows of
+ * q_out as they were; queries whose keys' page is left out are turned all the same. */
+typedef struct {
+  emmy_dptr positions, q, q_out;
+  int64_t position_stride, q_strides[2], out_strides[2];
+  int32_t wide, heads, out_dtype;
+} emmy_kv8_rotated_args;
+int emmy_kv8_append_rotated(const emmy_kv8 *cache, emmy_dptr k, emmy_dptr v, int32_t dtype,
+                            const int64_t k_strides[2], const int64_t v_strides[2],
+                            const emmy_rotary *rotary, const emmy_kv8_rotated_args *args,
+                            emmy_stream stream);
 
 /* out = softmax(scale * q K^T, hidden keys left out) V for the new tokens'
  * queries, q and out [tokens][heads][head_dim] of `dtype` (bf16 or f16),
