@@ -1,5 +1,6 @@
 // emmy_kv8_attend -- attention of new queries over the paged 8-bit cache:
 // checks, workspace and plan, and which kernel takes which sequences.
+#include <algorithm>
 #include <cmath>
 
 #include "kv8_attend.cuh"
@@ -11,6 +12,7 @@ namespace {
 // the tile kernel's; a call's only sequence is whichever's its most rows ask
 // for.
 int shape_of(const char *what, const emmy_kv8 *c, int heads, PlanShape &p) {
+  p = PlanShape{};
   if (heads < 1 || heads % c->kv_heads != 0)
     return fail(EMMY_EINVAL, what, "heads must be a positive multiple of kv_heads");
   if (int64_t(heads) * c->tokens > 0x7fffffff) return fail(EMMY_EINVAL, what, "too many query rows");
@@ -76,13 +78,62 @@ int shape_of(const char *what, const emmy_kv8 *c, int heads, PlanShape &p) {
   return EMMY_OK;
 }
 
+// A call with shared keys: the run's rows over those first, by the row kernel where
+// no run has more than ROWS_MOST of a kv head, else by the tile kernel, all cut
+// along the keys; then each sequence's own keys by the row kernel, which takes the
+// others' results in at the end.  Longer sequences' rows fill tiles by themselves,
+// and a window leaves few shared keys: those calls are as without sharing.
+int shape_shared(const char *what, const emmy_kv8 *c, const emmy_kv8_shared *sh, int heads, int window, PlanShape &p) {
+  const int rc = shape_of(what, c, heads, p);
+  if (rc != EMMY_OK) return rc;
+  if (p.tiles || window > 0 || sh->max_runs == 0 || sh->max_tokens == 0) return EMMY_OK;
+  const int sms = sm_count(c->device);
+  const int64_t group = heads / c->kv_heads, few = group * c->max_q;
+  const int64_t segments = int64_t(c->seqs) * c->kv_heads * ((few + ROWS_BLOCK - 1) / ROWS_BLOCK);
+  const int64_t cap = int64_t(c->table_width) * c->page_size / 64;
+  const int wave = sms * ROWS_PER_SM;
+  p.max_runs = sh->max_runs, p.max_tokens = sh->max_tokens;
+  p.cluster = 0, p.single = false;
+  p.target = p.spread ? p.slots * 2 / 3 : wave < p.slots ? wave : p.slots;
+  p.most_parts = std::min((p.spread ? p.slots : p.target) + segments, cap * segments);
+  const int64_t run_rows = group * p.max_tokens;
+  int64_t units;
+  if (run_rows <= ROWS_MOST) {
+    p.shared = SHARED_ROWS;
+    p.pre_nt = rows_blocks(run_rows);
+    p.pre_rows = 8 * p.pre_nt;
+    units = int64_t(p.max_runs) * ((run_rows + p.pre_rows - 1) / p.pre_rows) * c->kv_heads;
+    p.pre_target = units < wave ? wave : 0;
+  } else {
+    p.shared = SHARED_TILES;
+    p.pre_rows = TILE_ROWS;
+    units = (c->tokens * group / TILE_ROWS + p.max_runs) * c->kv_heads;
+    p.pre_target = units < sms ? sms : 0;
+  }
+  p.most_pre = units + p.pre_target;
+  if (p.most_pre > 0x7fffffff) return fail(EMMY_EINVAL, what, "too many sequences and heads for one call");
+  if (p.shared == SHARED_TILES) p.most_units = p.most_pre;
+  p.workspace_bytes = EMMY_KV8_WORKSPACE_ZERO + p.partial_bytes + uint64_t(p.most_pre) * p.pre_rows * (c->head_dim + 2) * 4;
+  p.plan_bytes = sizeof(PlanHead) + uint64_t(p.most_parts) * sizeof(PartRec) + uint64_t(c->seqs) * sizeof(PrefixRec) +
+                 uint64_t(p.most_pre) * (p.shared == SHARED_TILES ? sizeof(UnitRec) : sizeof(PartRec));
+  return EMMY_OK;
+}
+
+int check_shared(const char *what, const emmy_kv8 *c, const emmy_kv8_shared *sh) {
+  if (sh == nullptr) return fail(EMMY_EINVAL, what, "null description of what is shared");
+  if (sh->max_runs < 0 || sh->max_runs > c->seqs || sh->max_tokens < 0 || sh->max_tokens > c->tokens)
+    return fail(EMMY_EINVAL, what, "bad max_runs or max_tokens");
+  return EMMY_OK;
+}
+
 // The checks that attend and its plan share.
-int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_attend_args *a, PlanShape &shape, AttendParams &p) {
+int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_shared *shared, const emmy_kv8_attend_args *a,
+               PlanShape &shape, AttendParams &p) {
   int rc = check_cache(what, cache);
   if (rc == EMMY_OK) rc = check_seqs(what, cache);
   if (rc != EMMY_OK) return rc;
   if (a == nullptr) return fail(EMMY_EINVAL, what, "null arguments");
-  rc = shape_of(what, cache, a->heads, shape);
+  rc = shared == nullptr ? shape_of(what, cache, a->heads, shape) : shape_shared(what, cache, shared, a->heads, a->window, shape);
   if (rc != EMMY_OK) return rc;
   if (a->window < 0 || a->sinks < 0) return fail(EMMY_EINVAL, what, "window and sinks must not be negative");
   if (a->sinks > 0 && a->window == 0) return fail(EMMY_EINVAL, what, "sinks need a window");
@@ -103,16 +154,20 @@ int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_attend_ar
   p.row_limit = shape.rows ? ROWS_MOST : 0;
   p.nt = shape.nt;
   p.cluster = shape.cluster;
+  p.shared = shape.shared;
+  if (shape.shared != SHARED_NONE) {
+    if (shared->runs == 0 || shared->runs % 4) return fail(EMMY_EINVAL, what, "runs is missing or unaligned");
+    p.runs = reinterpret_cast<const int *>(shared->runs);
+    p.prefix = reinterpret_cast<PrefixRec *>(p.parts + shape.most_parts);
+    p.pre_parts = reinterpret_cast<PartRec *>(p.prefix + cache->seqs);
+    p.units = reinterpret_cast<UnitRec *>(p.pre_parts);
+    p.pre_rows = shape.pre_rows;
+  }
   return EMMY_OK;
 }
 
-}  // namespace
-}  // namespace kv8
-
-extern "C" int emmy_kv8_attend_sizes(const emmy_kv8 *cache, int32_t heads, uint64_t *workspace_bytes,
-                                     uint64_t *plan_bytes) {
-  using namespace kv8;
-  static const char *what = "emmy_kv8_attend_sizes";
+int sizes(const char *what, const emmy_kv8 *cache, const emmy_kv8_shared *shared, int32_t heads, uint64_t *workspace_bytes,
+          uint64_t *plan_bytes) {
   int rc = check_cache(what, cache);
   if (rc == EMMY_OK) rc = check_counts(what, cache);
   if (rc == EMMY_OK && (workspace_bytes == nullptr || plan_bytes == nullptr))
@@ -122,27 +177,31 @@ extern "C" int emmy_kv8_attend_sizes(const emmy_kv8 *cache, int32_t heads, uint6
   if (rc != EMMY_OK) return rc;
   *workspace_bytes = shape.workspace_bytes;
   *plan_bytes = shape.plan_bytes;
+  if (shared == nullptr) return EMMY_OK;
+  // with a window the call is as without sharing, so the larger ones
+  rc = shape_shared(what, cache, shared, heads, 0, shape);
+  if (rc != EMMY_OK) return rc;
+  *workspace_bytes = std::max(*workspace_bytes, shape.workspace_bytes);
+  *plan_bytes = std::max(*plan_bytes, shape.plan_bytes);
   return EMMY_OK;
 }
 
-extern "C" int emmy_kv8_attend_plan(const emmy_kv8 *cache, const emmy_kv8_attend_args *a, emmy_stream stream) {
-  using namespace kv8;
-  static const char *what = "emmy_kv8_attend_plan";
+int plan(const char *what, const emmy_kv8 *cache, const emmy_kv8_shared *shared, const emmy_kv8_attend_args *a, emmy_stream stream) {
   PlanShape shape;
   AttendParams p;
-  const int rc = check_args(what, cache, a, shape, p);
+  const int rc = check_args(what, cache, shared, a, shape, p);
   if (rc != EMMY_OK) return rc;
   const OnDevice on(cache->device);
   if (on.err != cudaSuccess) return cuda_fail(what, on.err);
-  return plan_attend(p, shape, static_cast<cudaStream_t>(stream));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return shape.shared != SHARED_NONE ? plan_shared(p, shape, st) : plan_attend(p, shape, st);
 }
 
-extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args *a, emmy_stream stream) {
-  using namespace kv8;
-  static const char *what = "emmy_kv8_attend";
+int attend(const char *what, const emmy_kv8 *cache, const emmy_kv8_shared *shared, const emmy_kv8_attend_args *a,
+           emmy_stream stream) {
   PlanShape shape;
   AttendParams p;
-  int rc = check_args(what, cache, a, shape, p);
+  int rc = check_args(what, cache, shared, a, shape, p);
   if (rc != EMMY_OK) return rc;
   if (a->dtype != EMMY_KV8_BF16 && a->dtype != EMMY_KV8_F16)
     return fail(EMMY_EINVAL, what, "dtype must be bf16 or f16");
@@ -168,6 +227,7 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   p.counters = reinterpret_cast<unsigned *>(a->workspace);
   p.partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO);
   p.tile_partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO + shape.partial_bytes);
+  p.pre_partial = p.tile_partial;
   p.scale_log2 = scale_log2;
   wait_limit(p.wait_ns, p.stall);
   const OnDevice on(cache->device);
@@ -175,6 +235,10 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   const bool bf16 = a->dtype == EMMY_KV8_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   note_capture(st);
+  if (shape.shared != SHARED_NONE) {
+    rc = shape.shared == SHARED_TILES ? tiles_attend(p, *cache, shape, bf16, st) : rows_shared(p, *cache, shape, bf16, true, st);
+    return rc == EMMY_OK ? rows_shared(p, *cache, shape, bf16, false, st) : rc;
+  }
   p.beside = shape.tiles && shape.rows;
   p.ready = p.counters + EMMY_KV8_WORKSPACE_ZERO / 4 - 2;
   if (shape.tiles) rc = tiles_attend(p, *cache, shape, bf16, st);
@@ -184,4 +248,44 @@ extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args
   }
   if (rc == EMMY_OK && shape.tile_target > 0) rc = tiles_join(p, *cache, shape, bf16, st);
   return rc;
+}
+
+}  // namespace
+}  // namespace kv8
+
+extern "C" int emmy_kv8_attend_sizes(const emmy_kv8 *cache, int32_t heads, uint64_t *workspace_bytes,
+                                     uint64_t *plan_bytes) {
+  return kv8::sizes("emmy_kv8_attend_sizes", cache, nullptr, heads, workspace_bytes, plan_bytes);
+}
+
+extern "C" int emmy_kv8_attend_plan(const emmy_kv8 *cache, const emmy_kv8_attend_args *a, emmy_stream stream) {
+  return kv8::plan("emmy_kv8_attend_plan", cache, nullptr, a, stream);
+}
+
+extern "C" int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args *a, emmy_stream stream) {
+  return kv8::attend("emmy_kv8_attend", cache, nullptr, a, stream);
+}
+
+extern "C" int emmy_kv8_attend_shared_sizes(const emmy_kv8 *cache, const emmy_kv8_shared *shared, int32_t heads,
+                                            uint64_t *workspace_bytes, uint64_t *plan_bytes) {
+  static const char *what = "emmy_kv8_attend_shared_sizes";
+  int rc = kv8::check_cache(what, cache);
+  if (rc == EMMY_OK) rc = kv8::check_shared(what, cache, shared);
+  return rc != EMMY_OK ? rc : kv8::sizes(what, cache, shared, heads, workspace_bytes, plan_bytes);
+}
+
+extern "C" int emmy_kv8_attend_shared_plan(const emmy_kv8 *cache, const emmy_kv8_shared *shared,
+                                           const emmy_kv8_attend_args *a, emmy_stream stream) {
+  static const char *what = "emmy_kv8_attend_shared_plan";
+  int rc = kv8::check_cache(what, cache);
+  if (rc == EMMY_OK) rc = kv8::check_shared(what, cache, shared);
+  return rc != EMMY_OK ? rc : kv8::plan(what, cache, shared, a, stream);
+}
+
+extern "C" int emmy_kv8_attend_shared(const emmy_kv8 *cache, const emmy_kv8_shared *shared,
+                                      const emmy_kv8_attend_args *a, emmy_stream stream) {
+  static const char *what = "emmy_kv8_attend_shared";
+  int rc = kv8::check_cache(what, cache);
+  if (rc == EMMY_OK) rc = kv8::check_shared(what, cache, shared);
+  return rc != EMMY_OK ? rc : kv8::attend(what, cache, shared, a, stream);
 }

@@ -11,8 +11,8 @@ namespace kv8 {
 // for those of the tile kernel, and for the tile kernel's units that were cut.
 struct alignas(16) PlanHead {
   int parts, units, joins;
-  int group, window, sinks, row_limit, seqs, kv_heads, nt, width, page_shift, cluster;  // what it was made for
-  int pad[3];
+  int group, window, sinks, row_limit, seqs, kv_heads, nt, width, page_shift, cluster, shared;  // what it was made for
+  int pad[2];
 };
 struct alignas(16) PartRec {
   int b, head, c0, c1;  // chunks c0 .. c1 - 1 of the segment's line
@@ -28,6 +28,18 @@ struct alignas(16) JoinRec {
   int head, row0, start, rows;  // rows of the sequence's kv head
   int slot0, parts, b, pad;
 };
+
+// What a sequence's keys that it shares with its run came to: results of some
+// parts of the run's query rows, block after block of p.prefix_rows rows.
+struct alignas(16) PrefixRec {
+  int chunks;        // 64-key chunks that are shared, 0: none
+  int slot0, parts;  // workspace slots of block 0 of kv head 0, one a part
+  int blocks, row;   // of the run's rows of a kv head; the sequence's first row among them
+  int pad[3];
+};
+
+// Which kernel, if any, attends to shared keys first.
+enum { SHARED_NONE = 0, SHARED_ROWS, SHARED_TILES };
 
 struct AttendParams {
   Seqs s;
@@ -51,6 +63,12 @@ struct AttendParams {
   int cluster;       // CTAs of a cluster of the row kernel, 0: none
   bool beside;       // the row kernel was launched to run beside the tile kernel
   unsigned *ready;   // there: what came before both is done, and the row kernel's blocks that know
+  int shared;           // SHARED_..: the rows' shared keys are the first kernel's, others the second's
+  const int *runs;      // [3][seqs]: see emmy_kv8_shared
+  PrefixRec *prefix;    // of each sequence
+  PartRec *pre_parts;   // of the row kernel, where it is the first, too
+  float *pre_partial;   // results for shared keys
+  int pre_rows;         // rows of a slot there
   int stall;         // one block in so many withholds its first keys (0: none)
   unsigned long long wait_ns;  // limit of the kernels' waits
 };
@@ -68,13 +86,19 @@ struct PlanShape {
   int64_t most_parts, most_units, most_joins;
   uint64_t partial_bytes;  // of the row kernel's parts
   uint64_t workspace_bytes, plan_bytes;
+  // of a call with shared keys
+  int shared;              // SHARED_..
+  int64_t most_pre;        // parts of the first kernel
+  int pre_target;          // that it aims at, 0: nothing is cut
+  int pre_nt, pre_rows;    // its 8-row blocks (of the row kernel), and rows of a slot of its results
+  int max_runs, max_tokens;
 };
 
 // The record is for this call, and what it says is within the arrays.
 __device__ __forceinline__ bool plan_fits(const AttendParams &p, const PlanHead &h, int b, int start, int n, int len) {
   const bool ok = h.group == p.group && h.window == p.window && h.sinks == p.sinks && h.row_limit == p.row_limit &&
                   h.seqs == p.s.seqs && h.kv_heads == p.s.kv_heads && h.nt == p.nt && h.width == p.s.width && h.cluster == p.cluster &&
-                  h.page_shift == p.s.page_shift && start + n <= p.s.tokens &&
+                  h.page_shift == p.s.page_shift && h.shared == p.shared && start + n <= p.s.tokens &&
                   len <= (int64_t(p.s.width) << p.s.page_shift);
   if (!ok) report(p.s.status, STATUS_PLAN);
   return ok;
@@ -181,6 +205,8 @@ constexpr int TILE_CUT = 8;     // chunks of a unit's part at least: a cut has t
 // 8-row blocks of a CTA of the row kernel, for the rows of the largest sequence.
 inline int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
+int plan_shared(const AttendParams &p, const PlanShape &shape, cudaStream_t stream);
+int rows_shared(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, bool first, cudaStream_t stream);
 int plan_attend(const AttendParams &p, const PlanShape &shape, cudaStream_t stream);
 int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream);
 int tiles_join(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream);

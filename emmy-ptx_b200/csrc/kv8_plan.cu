@@ -34,6 +34,7 @@ struct PlanParams {
   AttendParams a;
   int target, min_chunks, most_parts, most_units, most_joins, tile_target;
   bool spread, single;
+  int most_pre, pre_target, max_runs, max_tokens;  // of shared keys
 };
 
 __device__ __forceinline__ int warp_scan(int x, int lane) {  // inclusive
@@ -236,12 +237,185 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
   // the launches have room for so many (see shape_of)
   if (tid == 0)
     *p.a.plan = PlanHead{n_parts, min(n_records, p.most_units), min(joins, p.most_joins), p.a.group, p.a.window,
-                         p.a.sinks, p.a.row_limit, s.seqs, H, p.a.nt, s.width, s.page_shift, p.a.cluster, {}};
+                         p.a.sinks, p.a.row_limit, s.seqs, H, p.a.nt, s.width, s.page_shift, p.a.cluster, p.a.shared, {}};
 }
 
-}  // namespace
+// What a run that begins at sequence b comes to: its new tokens' rows of a kv
+// head and its shared keys; 0 keys where b begins none, or one that cannot be.
+struct Run {
+  int start, tokens, keys;
+  __device__ __forceinline__ Run(const PlanParams &p, int b) : start(0), tokens(0), keys(0) {
+    const Seqs &s = p.a.s;
+    const int count = p.a.runs[s.seqs + b], held = p.a.runs[2 * s.seqs + b];
+    if (p.a.runs[b] != b || count < 2 || held == 0) return;
+    if (count > s.seqs - b || held < 0 || held % (1 << s.page_shift) != 0 || held > int64_t(s.width) << s.page_shift) {
+      report(s.status, STATUS_LENGTH);
+      return;
+    }
+    start = s.q_starts[b];
+    tokens = s.q_starts[b + count] - start;
+    if (start < 0 || tokens <= 0 || start > s.tokens - tokens || tokens > p.max_tokens) return;
+    keys = held;
+  }
+};
 
-int plan_attend(const AttendParams &a, const PlanShape &shape, cudaStream_t stream) {
+// The plan of a call with shared keys.  A run's blocks of query rows (of the
+// tile kernel's units, or the row kernel's) are each cut into the same number of
+// parts, so a row finds its results by where it stands in the run; their keys are
+// the same, and blocks of a part are neighbours.  Then segments and parts as
+// above, of each sequence's own keys.
+__global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p) {
+  __shared__ int part_at[EMMY_KV8_MAX_SEQS], slot_at[EMMY_KV8_MAX_SEQS];
+  __shared__ int sums[WARPS];
+  grid_dependency_wait();
+  grid_dependency_done();
+  const Seqs &s = p.a.s;
+  const int tid = threadIdx.x, H = s.kv_heads, b0 = tid * EACH, G = p.a.group, RB = p.a.pre_rows;
+  // ---- runs ----
+  int pre_chunks[EACH], pre_blocks[EACH], runs = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    pre_chunks[i] = pre_blocks[i] = 0;
+    if (b0 + i < s.seqs) {
+      const Run r(p, b0 + i);
+      if (r.keys > 0) {
+        pre_chunks[i] = r.keys >> 6;
+        pre_blocks[i] = (r.tokens * G + RB - 1) / RB;
+        ++runs;
+      }
+    }
+  }
+  int all, nth = block_scan(runs, all, sums), mine = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    if (pre_chunks[i] > 0 && nth++ >= p.max_runs) pre_chunks[i] = pre_blocks[i] = 0;  // one more than there is room for
+    mine += pre_chunks[i] * pre_blocks[i];
+  }
+  block_scan(mine, all, sums);
+  int limit = 1 << 24;  // chunks of a part
+  if (p.pre_target > 0) {
+    const int64_t share = (int64_t(all) * H + p.pre_target - 1) / p.pre_target;
+    limit = int(min(max(share, int64_t(p.a.shared == SHARED_TILES ? TILE_CUT : 2)), int64_t(1) << 24));
+  }
+  int pre = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) pre += pre_blocks[i] * H * ((pre_chunks[i] + limit - 1) / limit);
+  int n_pre, pre_at = block_scan(pre, n_pre, sums);
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+    if (b0 + i < s.seqs) {
+      const int k = (pre_chunks[i] + limit - 1) / limit;
+      slot_at[b0 + i] = pre_at;
+      p.a.prefix[b0 + i] = PrefixRec{pre_chunks[i], pre_at, k, pre_blocks[i], 0, {}};
+      pre_at += pre_blocks[i] * H * k;
+    }
+  __syncthreads();
+  n_pre = min(n_pre, p.most_pre);
+  for (int i = tid; i < n_pre; i += THREADS) {
+    const int b = owner_of(slot_at, s.seqs, i), rel = i - slot_at[b];
+    const PrefixRec f = p.a.prefix[b];
+    const Run r(p, b);
+    const int block = rel % f.blocks, part = rel / f.blocks % f.parts, head = rel / (f.blocks * f.parts);
+    const int slot0 = f.slot0 + (head * f.blocks + block) * f.parts;
+    const int c0 = int(int64_t(f.chunks) * part / f.parts), c1 = int(int64_t(f.chunks) * (part + 1) / f.parts);
+    // its tokens as if they came behind the shared keys
+    if (p.a.shared == SHARED_TILES)
+      p.a.units[i] = UnitRec{b, head, block * RB, r.start, r.tokens, r.keys + r.tokens, c0, c1, slot0 + part, {}};
+    else
+      p.a.pre_parts[i] = PartRec{b, head, c0, c1, part, f.parts, slot0, block * RB,
+                                 r.start, r.tokens, r.keys + r.tokens, min(RB, r.tokens * G - block * RB)};
+  }
+  // ---- each sequence's own keys ----
+  int chunks[EACH], blocks[EACH];  // row blocks
+  mine = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    chunks[i] = blocks[i] = 0;
+    const int b = b0 + i;
+    if (b < s.seqs) {
+      int start, n, len;
+      lengths(s, b, start, n, len);
+      const int lead = p.a.runs[b];
+      PrefixRec f = {};
+      // a run that cannot be, or not here, leaves its sequences to themselves
+      if (lead >= 0 && lead <= b && p.a.runs[lead] == lead && b - lead < max(p.a.runs[s.seqs + lead], 1) &&
+          p.a.prefix[lead].chunks > 0) {
+        const Run r(p, lead);
+        f = p.a.prefix[lead];
+        f.row = (start - r.start) * G;
+        // new tokens among the shared keys, or rows that are not the run's
+        if (n > 0 && (f.chunks << 6 > len - n || start < r.start || start + n > r.start + r.tokens)) {
+          report(s.status, STATUS_LENGTH);
+          n = 0;
+        }
+      }
+      if (n > 0) {
+        chunks[i] = Span(p.a, len - n, len - 1).chunks - f.chunks;
+        blocks[i] = (n * G + ROWS_BLOCK - 1) / ROWS_BLOCK;
+      }
+      // (a lead's own record stays, and others read only that)
+      if (lead != b) p.a.prefix[b] = f;
+    }
+    mine += chunks[i] * blocks[i];
+  }
+  block_scan(mine, all, sums);
+  const int64_t work = int64_t(all) * H;
+  const int64_t share = (work + p.target - 1) / p.target;
+  const int q0 = max(p.min_chunks, int(min(share, int64_t(1) << 24)));
+  int q = q0;
+  if (!p.spread)
+    for (int t = 1; t <= 16; t += t < 4 ? 1 : t < 8 ? 2 : 4) {
+      int parts = 0, total;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) parts += parts_of(p, chunks[i], q) * blocks[i];
+      block_scan(parts, total, sums);
+      if (int64_t(total) * H <= p.target) break;
+      q = q0 + (q0 * t + 15) / 16;
+    }
+  int parts = 0, slots = 0, n_parts, n_slots;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int k = parts_of(p, chunks[i], q);
+    parts += k * blocks[i] * H;
+    slots += slots_of(p, k) * blocks[i] * H;
+  }
+  int at = block_scan(parts, n_parts, sums), slot = block_scan(slots, n_slots, sums);
+  __syncthreads();  // slot_at is read above
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+    if (b0 + i < s.seqs) {
+      const int k = parts_of(p, chunks[i], q);
+      part_at[b0 + i] = at;
+      slot_at[b0 + i] = slot;
+      at += k * blocks[i] * H;
+      slot += slots_of(p, k) * blocks[i] * H;
+    }
+  __syncthreads();
+  n_parts = min(n_parts, p.most_parts);
+  for (int i = tid; i < n_parts; i += THREADS) {
+    const int b = owner_of(part_at, s.seqs, i), rel = i - part_at[b];
+    PartRec r;
+    r.b = b;
+    lengths(s, b, r.start, r.n, r.len);
+    const int base = p.a.prefix[b].chunks, c = Span(p.a, r.len - r.n, r.len - 1).chunks - base, k = parts_of(p, c, q);
+    const int rows = r.n * G, nb = (rows + ROWS_BLOCK - 1) / ROWS_BLOCK, each = (rows + nb - 1) / nb;
+    const int block = rel % nb, cut = rel / nb;
+    r.head = cut / k;
+    r.part = cut - r.head * k;
+    r.parts = k;
+    r.slot0 = slot_at[b] + (r.head * nb + block) * slots_of(p, k);
+    r.c0 = base + int(int64_t(c) * r.part / k);
+    r.c1 = base + int(int64_t(c) * (r.part + 1) / k);
+    r.row0 = block * each;
+    r.rows = min(each, rows - r.row0);
+    p.a.parts[i] = r;
+  }
+  if (tid == 0)
+    *p.a.plan = PlanHead{n_parts, n_pre, 0, G, p.a.window, p.a.sinks, p.a.row_limit, s.seqs, H, p.a.nt,
+                         s.width, s.page_shift, p.a.cluster, p.a.shared, {}};
+}
+
+PlanParams params_of(const AttendParams &a, const PlanShape &shape) {
   PlanParams p;
   p.a = a;
   p.target = shape.target;
@@ -253,7 +427,20 @@ int plan_attend(const AttendParams &a, const PlanShape &shape, cudaStream_t stre
   p.most_units = int(shape.most_units);
   p.most_joins = int(shape.most_joins);
   p.tile_target = shape.tile_target;
-  return launch_kernel("emmy_kv8_attend_plan", plan_kernel, dim3(1), THREADS, 0, stream, p);
+  p.most_pre = int(shape.most_pre);
+  p.pre_target = shape.pre_target;
+  p.max_runs = shape.max_runs;
+  p.max_tokens = shape.max_tokens;
+  return p;
+}
+
+}  // namespace
+
+int plan_attend(const AttendParams &a, const PlanShape &shape, cudaStream_t stream) {
+  return launch_kernel("emmy_kv8_attend_plan", plan_kernel, dim3(1), THREADS, 0, stream, params_of(a, shape));
+}
+int plan_shared(const AttendParams &a, const PlanShape &shape, cudaStream_t stream) {
+  return launch_kernel("emmy_kv8_attend_shared_plan", plan_shared_kernel, dim3(1), THREADS, 0, stream, params_of(a, shape));
 }
 
 }  // namespace kv8

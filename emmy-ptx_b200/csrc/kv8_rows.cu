@@ -301,8 +301,39 @@ __device__ __forceinline__ int query_row(uint32_t (&f)[D / 8], const T *row, int
   return e;
 }
 
+// A call's only kernel of its kind; the first of two, which leaves results for
+// shared keys in the workspace; or the second, which takes them in.
+enum { ALONE = 0, FIRST, SECOND };
+
+// Results for the shared keys of row r's sequence join x, values d .. d + N - 1 of
+// the row, and its maximum and sum, in the parts' order.
+template <int D, int N>
+__device__ __forceinline__ void take_shared(const AttendParams &p, const PrefixRec &f, int head, int row, int d, float (&x)[N],
+                                            float &m, float &l) {
+  if (f.chunks == 0) return;
+  const int at = f.row + row, block = at / p.pre_rows, r = at - block * p.pre_rows;
+  const int64_t size = int64_t(p.pre_rows) * (D + 2);
+  const float *part = p.pre_partial + (f.slot0 + (int64_t(head) * f.blocks + block) * f.parts) * size;
+  // the tile kernel's results lie column by column
+  const bool columns = p.shared == SHARED_TILES;
+  const int64_t rs = columns ? 1 : D, ds = columns ? p.pre_rows : 1;
+  float top = m;
+  for (int i = 0; i < f.parts; ++i) top = fmaxf(top, __ldcg(part + i * size + p.pre_rows * D + r));
+  const float own = exp2_fast(m - top);
+  l *= own;
+#pragma unroll
+  for (int j = 0; j < N; ++j) x[j] *= own;
+  for (int i = 0; i < f.parts; ++i, part += size) {
+    const float w = exp2_fast(__ldcg(part + p.pre_rows * D + r) - top);
+    l += w * __ldcg(part + p.pre_rows * (D + 1) + r);
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] += w * __ldcg(part + r * rs + (d + j) * ds);
+  }
+  m = top;
+}
+
 // Shared memory: first the joined rows of the four warps, over the staged queries.
-template <int D, int NT, bool CLUSTER, typename T>
+template <int D, int NT, bool CLUSTER, int MODE, typename T>
 __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtensorMap &codes_map) {
   using L = Layout<D, NT>;
   constexpr int ROWS = 8 * NT, LD = L::LD;
@@ -319,12 +350,15 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gr = lane >> 2, q = lane & 3;
   const Seqs &s = p.s;
   const PlanHead head = *p.plan;
-  const PartRec rec = p.parts[blockIdx.x];
+  const PartRec rec = (MODE == FIRST ? p.pre_parts : p.parts)[blockIdx.x];
   // (the block that waits in the end lets the next kernel start after that only:
   // its CTAs would take SMs in the order that these leave them, 257 for 248 us a
   // batch of prompts)
   if (!p.beside || blockIdx.x != 0) grid_dependency_done();
-  if (blockIdx.x >= head.parts || !plan_fits(p, head, rec.b, rec.start, rec.n, rec.len)) return;
+  // (the tokens of a run stand behind its shared keys as if they were one sequence's)
+  if (blockIdx.x >= (MODE == FIRST ? head.units : head.parts) ||
+      !plan_fits(p, head, rec.b, rec.start, rec.n, MODE == FIRST ? rec.len - rec.n : rec.len))
+    return;
   const Segment g = {rec.b, rec.head, rec.start, rec.n, rec.len, rec.row0, rec.rows, rec.part, rec.parts, rec.slot0,
                      Span(p, rec.len - rec.n, rec.len - 1)};
   const int c0 = rec.c0, c1 = rec.c1;
@@ -542,8 +576,10 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
     if (lane == 0) sm_unit[warp] = st.unit;
   }
   __syncthreads();
-  const bool whole = !CLUSTER && g.parts == 1;
+  const bool whole = !CLUSTER && MODE != FIRST && g.parts == 1;
   const int rows = g.rows;
+  PrefixRec shared = {};
+  if constexpr (MODE == SECOND) shared = p.prefix[g.b];
   const auto store = [&](int r, int d, const float (&x)[8], float l) {
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     uint4 w;
@@ -555,7 +591,9 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
   };
   const auto part_slot = [&](int c) { return p.partial + int64_t(g.slot0 + c) * ROWS * (D + 2); };
   // a cluster's parts stay in shared memory, behind what is joined here
-  float *const slot = CLUSTER ? join + WARPS * ROWS * LD : part_slot(g.part);
+  float *const slot = CLUSTER         ? join + WARPS * ROWS * LD
+                      : MODE == FIRST ? p.pre_partial + int64_t(g.slot0 + g.part) * ROWS * (D + 2)
+                                      : part_slot(g.part);
   for (int i = tid; i < rows * (D / 8); i += THREADS) {
     const int r = i / (D / 8), d = i % (D / 8) * 8;
     float m = NONE, l = 0.0f, x[8] = {};
@@ -575,6 +613,7 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
     }
     if (!whole && d == 0) row_m[r] = m, row_l[r] = l;
     if (whole) {
+      if constexpr (MODE == SECOND) take_shared<D>(p, shared, g.head, g.row0 + r, d, x, m, l);
       store(r, d, x, l);
     } else {
       *reinterpret_cast<float4 *>(slot + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
@@ -630,6 +669,7 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
       __stcg(slot + ROWS * D + tid, row_m[tid]);
       __stcg(slot + ROWS * D + ROWS + tid, row_l[tid]);
     }
+    if constexpr (MODE == FIRST) return;
   }
   // ---- parts join in groups of GROUP, groups in the segment: the last of
   // each to arrive does it, in the parts' order ----
@@ -692,7 +732,13 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
           }
       }
       if (last) {
-        const float by = row_l[r] == 0.0f ? 0.0f : 1.0f / row_l[r];
+        float l = row_l[r];
+        if constexpr (MODE == SECOND) {
+          float m = row_m[r], v[4] = {x.x, x.y, x.z, x.w};
+          take_shared<D>(p, shared, g.head, g.row0 + r, d, v, m, l);
+          x = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        const float by = l == 0.0f ? 0.0f : 1.0f / l;
         *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) =
             make_uint2(pack2<T>(x.x * by, x.y * by), pack2<T>(x.z * by, x.w * by));
       } else {  // only this thread reads or writes these values of part a now
@@ -736,42 +782,41 @@ __device__ __forceinline__ void took_ready(const AttendParams &p) {
   if (threadIdx.x == 0 && atomicAdd(p.ready + 1, 1u) == gridDim.x - 1) p.ready[0] = p.ready[1] = 0;
 }
 
-template <int D, int NT, bool CLUSTER, typename T>
+template <int D, int NT, bool CLUSTER, int MODE, typename T>
 __global__ void __launch_bounds__(THREADS, ROWS_PER_SM)
 rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map) {
   if (p.beside)
     ready_or_wait(p);
   else
     grid_dependency_wait();
-  attend_part<D, NT, CLUSTER, T>(p, codes_map);
+  attend_part<D, NT, CLUSTER, MODE, T>(p, codes_map);
   if (p.beside) {
     took_ready(p);
     if (blockIdx.x == 0) grid_dependency_wait();
   }
 }
 
-template <int D, int NT, bool CLUSTER, typename T>
+template <int D, int NT, bool CLUSTER, int MODE, typename T>
 int launch(const AttendParams &p, const CUtensorMap &map, int device, int grid, cudaStream_t stream) {
   static KernelSetup setup;
-  const int rc = setup.ready("emmy_kv8_attend", rows_kernel<D, NT, CLUSTER, T>, device, Layout<D, NT>::DYN);
+  const int rc = setup.ready("emmy_kv8_attend", rows_kernel<D, NT, CLUSTER, MODE, T>, device, Layout<D, NT>::DYN);
   if (rc != EMMY_OK) return rc;
-  return launch_clusters("emmy_kv8_attend", rows_kernel<D, NT, CLUSTER, T>, CLUSTER ? p.cluster : 1, dim3(grid),
+  return launch_clusters("emmy_kv8_attend", rows_kernel<D, NT, CLUSTER, MODE, T>, CLUSTER ? p.cluster : 1, dim3(grid),
                          THREADS, Layout<D, NT>::DYN, stream, p, map);
 }
 
-template <int D, typename T>
-int launch_nt(const AttendParams &p, const CUtensorMap &map, int device, int grid, cudaStream_t stream) {
-  if (p.cluster > 0)
-    return p.nt == 1 ? launch<D, 1, true, T>(p, map, device, grid, stream)
-                     : launch<D, 2, true, T>(p, map, device, grid, stream);
-  return p.nt == 1 ? launch<D, 1, false, T>(p, map, device, grid, stream)
-                   : launch<D, 2, false, T>(p, map, device, grid, stream);
+template <int D, int MODE, typename T>
+int launch_nt(const AttendParams &p, int nt, const CUtensorMap &map, int device, int grid, cudaStream_t stream) {
+  if constexpr (MODE == ALONE)
+    if (p.cluster > 0)
+      return nt == 1 ? launch<D, 1, true, MODE, T>(p, map, device, grid, stream)
+                     : launch<D, 2, true, MODE, T>(p, map, device, grid, stream);
+  return nt == 1 ? launch<D, 1, false, MODE, T>(p, map, device, grid, stream)
+                 : launch<D, 2, false, MODE, T>(p, map, device, grid, stream);
 }
 
-}  // namespace
-
-int rows_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream) {
-  const int64_t grid = shape.most_parts;
+template <int MODE>
+int launch_mode(const AttendParams &p, const emmy_kv8 &cache, int nt, int64_t grid, bool bf16, cudaStream_t stream) {
   // the pool as rows of head_dim bytes, 64 of them a box
   const int64_t rows = int64_t(cache.pages) * 2 * cache.kv_heads * cache.page_size;
   emmy_tmap_desc d = {};
@@ -788,10 +833,21 @@ int rows_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &s
   const int rc = emmy_tmap_encode(&d, &map);
   if (rc != EMMY_OK) return rc;
   if (cache.head_dim == 64)
-    return bf16 ? launch_nt<64, __nv_bfloat16>(p, map, cache.device, int(grid), stream)
-                : launch_nt<64, __half>(p, map, cache.device, int(grid), stream);
-  return bf16 ? launch_nt<128, __nv_bfloat16>(p, map, cache.device, int(grid), stream)
-              : launch_nt<128, __half>(p, map, cache.device, int(grid), stream);
+    return bf16 ? launch_nt<64, MODE, __nv_bfloat16>(p, nt, map, cache.device, int(grid), stream)
+                : launch_nt<64, MODE, __half>(p, nt, map, cache.device, int(grid), stream);
+  return bf16 ? launch_nt<128, MODE, __nv_bfloat16>(p, nt, map, cache.device, int(grid), stream)
+              : launch_nt<128, MODE, __half>(p, nt, map, cache.device, int(grid), stream);
+}
+
+}  // namespace
+
+int rows_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream) {
+  return launch_mode<ALONE>(p, cache, p.nt, shape.most_parts, bf16, stream);
+}
+
+int rows_shared(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, bool first, cudaStream_t stream) {
+  return first ? launch_mode<FIRST>(p, cache, shape.pre_nt, shape.most_pre, bf16, stream)
+               : launch_mode<SECOND>(p, cache, p.nt, shape.most_parts, bf16, stream);
 }
 
 }  // namespace kv8

@@ -210,6 +210,11 @@ constexpr uint32_t IDESC = 1u << 4 | uint32_t(B_MN) << 16 | uint32_t(N >> 3) << 
 // 16-byte piece j (0-7) of 128-byte row r of a swizzled tile.
 __device__ __forceinline__ uint32_t swizzled(int r, int j) { return r * 128 + ((j ^ (r & 7)) << 4); }
 
+// Keys that the record's rows may look up: the tokens of a run stand behind its
+// shared keys as if they were one sequence's.
+__device__ __forceinline__ int held(const AttendParams &p, const UnitRec &r) {
+  return p.shared != SHARED_NONE ? r.len - r.n : r.len;
+}
 // The record's rows and keys are within the arrays.
 __device__ __forceinline__ bool plan_holds(const AttendParams &p, int start, int n, int len) {
   const bool ok = start + n <= p.s.tokens && len <= (int64_t(p.s.width) << p.s.page_shift);
@@ -266,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
   const PlanHead head = *p.plan;
   const UnitRec first_rec = p.units[blockIdx.x];
   grid_dependency_done();
-  if (blockIdx.x >= head.units || !plan_fits(p, head, first_rec.b, first_rec.start, first_rec.n, first_rec.len)) return;
+  if (blockIdx.x >= head.units || !plan_fits(p, head, first_rec.b, first_rec.start, first_rec.n, held(p, first_rec))) return;
   // The units of this CTA: one of each gridDim.x, in turn from the front and
   // from the back, since the longest come first.
   const int units = head.units;
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
     const int i = index_of(k);
     if (i >= units) return false;
     const UnitRec r = p.units[i];
-    if (!plan_holds(p, r.start, r.n, r.len)) return false;
+    if (!plan_holds(p, r.start, r.n, held(p, r))) return false;
     u = Unit(p, r);
     return true;
   };

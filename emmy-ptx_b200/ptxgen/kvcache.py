@@ -55,6 +55,7 @@ PAGE_SIZES = (64, 128, 256)
 MAX_SEQS = 4096
 MAX_PAIRS = 480            # pages a launch of copy_pages takes
 WORKSPACE_ZERO = 16384     # bytes of a workspace that start as zeros
+MIN_SAVED = 1              # keys not read again that a run is to save at least
 PER_THREAD = 2             # the per-thread default stream's handle
 
 STATUS = {0x401: "a page number outside the pool",
@@ -88,6 +89,11 @@ class _Rotated(C.Structure):
     _fields_ = [("positions", C.c_uint64), ("q", C.c_uint64), ("q_out", C.c_uint64),
                 ("position_stride", C.c_int64), ("q_strides", _Strides), ("out_strides", _Strides),
                 ("wide", C.c_int32), ("heads", C.c_int32), ("out_dtype", C.c_int32)]
+
+
+class _Shared(C.Structure):
+    """``emmy_kv8_shared``."""
+    _fields_ = [("runs", C.c_uint64), ("max_runs", C.c_int32), ("max_tokens", C.c_int32)]
 
 
 class DeviceArray:
@@ -230,6 +236,55 @@ def _ints(x, name: str) -> np.ndarray:
     return a.astype(np.int64)
 
 
+def _best_runs(alike: list) -> list[tuple[int, int, int]]:
+    """(first, sequences, pages) of runs that save many page reads, where
+    alike[i] > 0 is how many leading pages sequence i + 1 has in common with
+    sequence i.  A run shares the least of its pairs' and saves that many pages a
+    pair: a stretch of pairs with a common least one is one run, or what the
+    stretches within it make, whichever saves more.  A stack builds that tree;
+    what is left between its runs is gone through again."""
+    open_: list = []       # (first pair, pages, closed stretches within), pages rising
+    closed: list = []
+    for i, n in enumerate([*alike, 0]):
+        first, closed = i, []
+        while open_ and open_[-1][1] >= n:
+            first, pages, inside = open_.pop()
+            inside += closed
+            saved, apart = (i - first) * pages, sum(c[0] for c in inside)
+            closed = [(saved, [(first, i - first + 1, pages)]) if saved >= apart
+                      else (apart, [r for c in inside for r in c[1]])]
+        open_.append((first, n, closed))
+    runs = [r for c in closed for r in c[1]]
+    ends = [0, *(first + count for first, count, _ in runs)]
+    starts = [*(first for first, _, _ in runs), len(alike) + 1]
+    for lo, hi in zip(ends, starts):        # sequences between two runs
+        if runs and hi - lo > 1:
+            runs = runs + [(lo + first, *r) for first, *r in _best_runs(alike[lo:hi - 1])]
+    return sorted(runs)
+
+
+def _runs_of(table: np.ndarray, kv: np.ndarray, q: np.ndarray, page: int) -> list[tuple[int, int, int]]:
+    """(first, sequences, pages) of sequences that follow one another and begin
+    with the same pages, all of them before any new token."""
+    before = (kv - q) // page
+    most = np.minimum(before[1:], before[:-1])
+    if not most.any():
+        return []
+    other = table[1:] != table[:-1]
+    alike = np.where(other.any(1), other.argmax(1), table.shape[1])
+    alike = np.minimum(alike, most)
+    # stretches between pairs that have nothing in common
+    edge = np.flatnonzero(np.diff(np.concatenate([[0], alike > 0, [0]])))
+    runs = []
+    for lo, hi in zip(edge[::2].tolist(), edge[1::2].tolist()):
+        part = alike[lo:hi]
+        if (part == part[0]).all():
+            runs.append((lo, hi - lo + 1, int(part[0])))
+        else:
+            runs += [(lo + first, count, n) for first, count, n in _best_runs(part.tolist())]
+    return [r for r in runs if (r[1] - 1) * r[2] * page >= MIN_SAVED]
+
+
 class _Pool:
     """Buffers of closed batches on one device, by (use, bytes, the id of the
     one stream they were used on): the next batch on that stream takes them
@@ -367,12 +422,14 @@ class KVCache:
         d.head_dim, d.page_size = self.head_dim, self.page_size
         return d
 
-    def batch(self, page_table, kv_lens, q_lens=None, stream=None) -> "Batch":
+    def batch(self, page_table, kv_lens, q_lens=None, stream=None, shared: bool = False) -> "Batch":
         """The sequences of one step: ``page_table`` [seqs, width] page
         numbers, ``kv_lens`` keys of each sequence with its new tokens,
         ``q_lens`` new tokens of each (default 1).  Host arrays, checked
-        here and copied to the device on ``stream``."""
-        return Batch(self, page_table, kv_lens, q_lens, stream)
+        here and copied to the device on ``stream``.  ``shared``: where
+        sequences that follow one another begin with the same pages, as forks
+        do, ``attend`` reads those once for all of them."""
+        return Batch(self, page_table, kv_lens, q_lens, stream, shared)
 
     def copy_pages(self, src, dst, stream=None) -> None:
         """Copy pages ``src[i]`` to ``dst[i]`` in every layer (host lists);
@@ -428,10 +485,16 @@ class Batch:
     ``append`` and ``attend`` replays with what ``update`` last put there; the
     batch has to live as long as the graph may run.  Making, ``reserve`` (or
     the first ``attend`` with some heads, window and sinks), ``update`` and
-    ``check_errors`` stay outside of captures."""
+    ``check_errors`` stay outside of captures.  With ``shared`` the batch is made
+    for as many runs of sequences with common pages, of as many new tokens, as
+    it has then; what ``update`` brings beyond that is read for each sequence, as
+    are all keys in calls with a window, or with more than 32 query rows of a
+    kv head in some sequence.  Results differ from unshared ones by roundings
+    only."""
 
-    def __init__(self, cache: KVCache, page_table, kv_lens, q_lens=None, stream=None):
+    def __init__(self, cache: KVCache, page_table, kv_lens, q_lens=None, stream=None, shared: bool = False):
         self.cache, self.dev, self.L, self.ordinal = cache, cache.dev, cache.L, cache.ordinal
+        self._share = bool(shared)
         self._make(page_table, kv_lens, q_lens, stream)
 
     @_at_home
@@ -446,6 +509,7 @@ class Batch:
         if self.width * cache.page_size > 2 ** 30:
             raise EmmyError("a sequence holds at most 2^30 keys")
         self.tokens = self.max_q = None
+        self._s = None                             # what is shared, of a batch with runs
         self._buf = 0
         self._held: list[tuple[int, tuple]] = []   # buffers of this batch, to give back
         self._ws: tuple[int, int] = (0, 0)         # workspace: address, bytes
@@ -466,6 +530,9 @@ class Batch:
         d.q_starts = d.kv_lens + 4 * self.seqs
         d.page_table = d.q_starts + 4 * (self.seqs + 1)
         d.seqs, d.table_width, d.tokens, d.max_q = self.seqs, self.width, self.tokens, self.max_q
+        if self._s is not None:
+            self._s.runs = d.page_table + 4 * self.seqs * self.width
+            self._sref = C.byref(self._s)
         self._ref, self._layer = C.byref(d), 0
         self._a = _Attend()
         self._aref = C.byref(self._a)
@@ -503,7 +570,7 @@ class Batch:
 
     def _packed(self, table, kv_lens, q_lens) -> np.ndarray:
         """Checked lengths and table as one int32 array: status word and
-        padding, kv_lens, q_starts, table."""
+        padding, kv_lens, q_starts, table, and in a batch with runs those."""
         P, B = self.cache.page_size, self.seqs
         kv = _ints(kv_lens, "kv_lens").reshape(-1)
         q = np.ones(B, np.int64) if q_lens is None else _ints(q_lens, "q_lens").reshape(-1)
@@ -519,7 +586,8 @@ class Batch:
         tokens, most = int(q.sum()), int(q.max())
         if tokens >= 2 ** 31:
             raise EmmyError("too many new tokens")
-        if self.tokens is None:
+        first = self.tokens is None
+        if first:
             self.tokens, self.max_q = tokens, most
         elif tokens > self.tokens or most > self.max_q:
             raise EmmyError(f"update: the batch was made for {self.tokens} new tokens, "
@@ -530,11 +598,43 @@ class Batch:
                         & (q > 0)[:, None]]
         # (np.unique costs 6 us however few there are)
         self._clash = len(set(written.tolist()) if len(written) < 256 else np.unique(written)) != len(written)
-        host = np.zeros(4 + 2 * B + 1 + B * self.width, np.int32)
+        runs = self._runs(np.where(used, table, -1), kv, q, first) if self._share else None
+        end = 5 + 2 * B + B * self.width
+        host = np.zeros(end + (0 if runs is None else 3 * B), np.int32)
         host[4:4 + B] = kv
         host[5 + B:5 + 2 * B] = np.cumsum(q)
-        host[5 + 2 * B:] = np.where(used, table, 0).reshape(-1)
+        host[5 + 2 * B:end] = np.where(used, table, 0).reshape(-1)
+        if runs is not None:
+            host[end:] = runs.reshape(-1)
         return host
+
+    def _runs(self, table, kv, q, first: bool) -> np.ndarray | None:
+        """[3, seqs]: the sequence that each one's run begins with, how many the
+        run that begins there has, and the keys they share; None in a batch that
+        was made without runs."""
+        if not first and self._s is None:
+            return None
+        runs = _runs_of(table, kv, q, self.cache.page_size)
+        rows = np.concatenate([[0], np.cumsum(q)])
+        if first:
+            if not runs or max(rows[a + n] - rows[a] for a, n, _ in runs) == 0:
+                return None
+            self._s = _Shared(max_runs=len(runs), max_tokens=int(max(rows[a + n] - rows[a] for a, n, _ in runs)))
+        room = self._s.max_tokens
+        split = []
+        for a, n, pages in runs:               # a run of more tokens than there is room for as several
+            while n > 0:
+                take = int(np.searchsorted(rows[a + 1:a + n + 1] - rows[a], room, "right"))
+                take = min(n, max(1, take))
+                split.append((a, take, pages))
+                a, n = a + take, n - take
+        split = sorted((r for r in split if r[1] > 1 and rows[r[0] + r[1]] - rows[r[0]] <= room),
+                       key=lambda r: (1 - r[1]) * r[2])[:self._s.max_runs]
+        out = np.zeros((3, self.seqs), np.int32)
+        out[0], out[1] = np.arange(self.seqs), 1
+        for a, n, pages in split:
+            out[0, a:a + n], out[1, a], out[2, a:a + n] = a, n, pages * self.cache.page_size
+        return out
 
     @_at_home
     def update(self, page_table, kv_lens, q_lens=None, stream=None) -> None:
@@ -658,7 +758,10 @@ class Batch:
         st = self._on(stream)
         _outside_capture(self.dev, st, "reserve() for these heads, window and sinks comes before")
         ws, plan = C.c_uint64(), C.c_uint64()
-        check(self.L.emmy_kv8_attend_sizes(self._ref, heads, C.byref(ws), C.byref(plan)), "attend")
+        if self._s is None:
+            check(self.L.emmy_kv8_attend_sizes(self._ref, heads, C.byref(ws), C.byref(plan)), "attend")
+        else:
+            check(self.L.emmy_kv8_attend_shared_sizes(self._ref, self._sref, heads, C.byref(ws), C.byref(plan)), "attend")
         if ws.value > self._ws[1]:
             self._ws = self._take("workspace", ws.value, st), ws.value
         self._plans[key] = self._take("plan", plan.value, st), plan.value
@@ -672,7 +775,10 @@ class Batch:
         a = self._a
         a.heads, a.window, a.sinks = key
         a.plan, a.plan_bytes = self._plans[key]
-        check(self.L.emmy_kv8_attend_plan(self._ref, self._aref, st), "attend")
+        if self._s is None:
+            check(self.L.emmy_kv8_attend_plan(self._ref, self._aref, st), "attend")
+        else:
+            check(self.L.emmy_kv8_attend_shared_plan(self._ref, self._sref, self._aref, st), "attend")
 
     def attend(self, layer: int, q, out, scale: float | None = None, window: int = 0,
                sinks: int = 0, stream=None):
@@ -698,7 +804,10 @@ class Batch:
         a.out_strides[0], a.out_strides[1] = os_[0], os_[1]
         a.dtype, a.heads, a.window, a.sinks = qt, heads, window, sinks
         a.scale = self.cache.head_dim ** -0.5 if scale is None else scale
-        rc = self._attend(self._ref, self._aref, self._on(stream))
+        if self._s is None:
+            rc = self._attend(self._ref, self._aref, self._on(stream))
+        else:
+            rc = self.L.emmy_kv8_attend_shared(self._ref, self._sref, self._aref, self._on(stream))
         if rc:
             check(rc, "attend")
         return out
@@ -815,11 +924,12 @@ class KVSequences:
 
     # -- steps --------------------------------------------------------------
 
-    def batch(self, sids, q_lens=None, stream=None) -> Batch:
+    def batch(self, sids, q_lens=None, stream=None, shared: bool = False) -> Batch:
         """Room for ``q_lens[i]`` (default 1) more tokens of each sequence:
         pages are taken, shared ones about to be written to copied, and the
         lengths moved on.  Where it raises (pages ran out), nothing has
-        changed."""
+        changed.  ``shared``: as in ``KVCache.batch``; name forks of one
+        sequence one after another."""
         sids = list(sids)
         q = [1] * len(sids) if q_lens is None else [int(n) for n in _ints(q_lens, "q_lens")]
         if not sids or len(q) != len(sids):
@@ -857,7 +967,7 @@ class KVSequences:
         lens = [self._len[sid] + n for sid, n in zip(sids, q)]
         self._outside_capture(stream)
         self.cache.copy_pages(src, taken[:len(src)], stream)
-        b = Batch(self.cache, self._table(list(pages.values())), lens, q, stream)
+        b = Batch(self.cache, self._table(list(pages.values())), lens, q, stream, shared)
         # the books follow once nothing can fail
         del self._free[len(self._free) - need:]
         for page in src:

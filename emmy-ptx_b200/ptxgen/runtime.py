@@ -112,6 +112,9 @@ def load_library():
         "emmy_kv8_attend": (i32, [vp, vp, vp]),
         "emmy_kv8_wait_limit": (i32, [u64, i32]),
         "emmy_kv8_captured": (i32, [C.POINTER(u64)]),
+        "emmy_kv8_attend_shared_sizes": (i32, [vp, vp, i32, C.POINTER(u64), C.POINTER(u64)]),
+        "emmy_kv8_attend_shared_plan": (i32, [vp, vp, vp, vp]),
+        "emmy_kv8_attend_shared": (i32, [vp, vp, vp, vp]),
         "emmy_kv8_append_rotated": (i32, [vp, u64, u64, i32, vp, vp, vp, vp, vp]),
         "emmy_rotate": (i32, [vp, vp, vp]),
         "emmy_kv8_copy_pages": (i32, [vp, i32, vp, vp, i32, vp]),

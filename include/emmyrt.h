@@ -328,6 +328,30 @@ int emmy_kv8_attend_sizes(const emmy_kv8 *cache, int32_t heads, uint64_t *worksp
 int emmy_kv8_attend_plan(const emmy_kv8 *cache, const emmy_kv8_attend_args *args, emmy_stream stream);
 int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args *args, emmy_stream stream);
 
+/* attend for a batch some of whose sequences begin with the same pages: those
+ * keys are attended to once for all of them.  A run is sequences that follow one
+ * another; `runs` says of each sequence b which one its run begins with (itself,
+ * where it is in none), how many sequences the run that begins at b has, and how
+ * many keys they share: a multiple of page_size, at most the keys before the new
+ * tokens of each, and on the same pages (those of the first are read).  At most
+ * max_runs runs of two or more, of at most max_tokens new tokens each, are
+ * taken so, and only where no sequence has more than 32 query rows of a kv head
+ * and there is no window; all others' keys are read for each sequence, with the
+ * same results up to rounding.  A sequence with new tokens among its run's
+ * shared keys is skipped and reported.  Everything else is as for
+ * emmy_kv8_attend; a plan and workspace for one kind of call is not for the
+ * other. */
+typedef struct {
+  emmy_dptr runs; /* int32 [3][seqs] */
+  int32_t max_runs, max_tokens;
+} emmy_kv8_shared;
+int emmy_kv8_attend_shared_sizes(const emmy_kv8 *cache, const emmy_kv8_shared *shared, int32_t heads,
+                                 uint64_t *workspace_bytes, uint64_t *plan_bytes);
+int emmy_kv8_attend_shared_plan(const emmy_kv8 *cache, const emmy_kv8_shared *shared,
+                                const emmy_kv8_attend_args *args, emmy_stream stream);
+int emmy_kv8_attend_shared(const emmy_kv8 *cache, const emmy_kv8_shared *shared,
+                           const emmy_kv8_attend_args *args, emmy_stream stream);
+
 /* How long attend's kernels, launched from now on by this process, wait for a
  * copy or a product of their own before they give up (default
  * EMMY_KV8_WAIT_NS).  A call whose kernel gave up reports it in *status and
