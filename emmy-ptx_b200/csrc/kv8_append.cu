@@ -15,9 +15,12 @@
 // more than one new token, a warp does one (sequence, side, head).
 //
 // emmy_kv8_append_rotated -- the same of keys turned to their positions on the
-// way, in f32 and unrounded, and queries turned into an array of their own: more
-// (query head)s behind the (side, head)s, with the same copies, maxima and page
-// left out.
+// way, in f32 and unrounded, and queries turned into an array of their own: where
+// no sequence has more than one new token they are more (query head)s behind the
+// (side, head)s, else rows for the kernel of emmy_rotate.  In a page's rows a key's
+// angle is that of a thread's first row and a multiple of the rows between:
+// cos(a + b) = cos a cos b - sin a sin b, with the first angle in registers and the
+// multiples' in shared memory, 4 products a pair instead of 40 instructions.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -139,38 +142,21 @@ __device__ __forceinline__ int64_t position_of(const RotatedParams &p, int64_t t
                 : static_cast<const int *>(p.positions)[token * p.position_stride];
 }
 
-// Values col .. col + N - 1 of a row in shared memory, turned to a position.
-template <typename T, int N>
-__device__ __forceinline__ void turn_piece(const RotatedParams &p, const T *row, int col, int64_t pos, float (&y)[N]) {
-  using rotary::to_float;
-  if (p.interleaved) {
+// Values col .. col + 15 bytes of a row in shared memory, turned one by one.
+template <typename T>
+__device__ __forceinline__ void turn_apart(const RotatedParams &p, const T *row, int col, int64_t pos, float *y) {
+  const int half = p.dims / 2;
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float a = to_float(row[col + i]), b = to_float(row[col + i + 1]);
-      y[i] = a, y[i + 1] = b;
-      if (col + i < p.dims) {
-        float c, s;
-        rotary::turn_of(pos, p.frequency[(col + i) / 2], c, s);
-        c *= p.gain, s *= p.gain;
-        y[i] = a * c - b * s;
-        y[i + 1] = a * s + b * c;
-      }
-    }
-  } else {
-    const int half = p.dims / 2;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = col + i;
-      y[i] = to_float(row[at]);
-      if (at < p.dims) {
-        const bool low = at < half;
-        const float other = to_float(row[low ? at + half : at - half]);
-        float c, s;
-        rotary::turn_of(pos, p.frequency[low ? at : at - half], c, s);
-        c *= p.gain, s *= p.gain;
-        y[i] = low ? y[i] * c - other * s : other * s + y[i] * c;
-      }
-    }
+  for (int i = 0; i < Vec<T>::N; ++i) {
+    const int at = col + i;
+    y[i] = rotary::to_float(row[at]);
+    if (at >= p.dims) continue;
+    const bool low = p.interleaved ? at % 2 == 0 : at < half;
+    const int away = p.interleaved ? 1 : half, other = low ? at + away : at - away;
+    float c, s;
+    rotary::turn_of(pos, p.frequency[p.interleaved ? at / 2 : low ? at : other], c, s);
+    c *= p.gain, s *= p.gain;
+    y[i] = y[i] * c + rotary::to_float(row[other]) * (low ? -s : s);
   }
 }
 
@@ -184,7 +170,7 @@ __device__ __forceinline__ float max_finite(const float (&y)[N], float amax) {
   return amax;
 }
 template <int N>
-__device__ __forceinline__ void store_codes(uint8_t *at, const float (&y)[N], int e) {
+__device__ __forceinline__ void store_codes(uint8_t *at, const float *y, int e) {
   uint32_t w[2] = {};
 #pragma unroll
   for (int j = 0; j < N; j += 2)
@@ -254,12 +240,15 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool real)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 
-template <int D, typename T, typename Params>
+// How a page's keys are turned: not at all; with the pairs of a piece in another
+// whole piece, or within it, at their places in the sequence; or in any other way.
+enum { PLAIN = 0, HALVES, NEIGHBOURS, ANY };
+
+template <int D, typename T, int MODE, typename Params>
 __global__ void __launch_bounds__(MOST_THREADS<D, T>) append_kernel(const __grid_constant__ Params p) {
-  constexpr bool ROTATED = std::is_same<Params, RotatedParams>::value;
+  constexpr bool ROTATED = MODE != PLAIN;
   using V = Vec<T>;
   constexpr int LPR = D / V::N;  // lanes per row, 16 bytes each
-  constexpr int RPW = 32 / LPR;  // rows per warp and pass
   constexpr int PASSES = 8;
   extern __shared__ uint4 pieces[];  // [2][PASSES][threads]
   __shared__ float part[2][32];
@@ -273,71 +262,125 @@ __global__ void __launch_bounds__(MOST_THREADS<D, T>) append_kernel(const __grid
   const int pos0 = page_of_seq << s.page_shift;
   const int lo = max(first - pos0, 0), hi = min(len - pos0, P);  // new rows of the page
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
-  const int col = lane % LPR * V::N, row0 = warp * RPW + lane / LPR, step = warps * RPW;
+  // The thread's piece of each row, or (turned) its two pieces that pair up, of half
+  // as many rows: row i is row0 + i * step.
+  constexpr int ROWS = ROTATED ? PASSES / 2 : PASSES, LANES = ROTATED ? LPR / 2 : LPR;
+  int col = lane % LANES * V::N, col2 = col + D / 2;
+  bool pairs = true;  // the pieces are turned
+  if constexpr (MODE == HALVES) {
+    const int half = p.dims / 2, at = lane % LANES - half / V::N;
+    pairs = at < 0;
+    if (!pairs) col = p.dims + at * V::N;  // behind the turned ones, as far from each other as fits
+    col2 = pairs ? col + half : col + (D - p.dims) / 2;
+  }
+  const int row0 = warp * (32 / LANES) + lane / LANES, step = warps * (32 / LANES);
   const int64_t token0 = int64_t(start) + pos0 - first;  // row 0 of the page, were it new
+  // a buffer holds the page's rows, one after another
+  const int mine = row0 * LPR + col / V::N;
   const auto fetch = [&](int u, int buf) {
     const int side = u >= H, head = u - side * H;
-    int64_t ts = side ? p.ts[1] : p.ts[0];
+    const int64_t ts = side ? p.ts[1] : p.ts[0];
     const T *x = static_cast<const T *>(side ? p.x[1] : p.x[0]) + head * (side ? p.hs[1] : p.hs[0]) + col;
-    if constexpr (ROTATED)
-      if (u >= 2 * H) x = static_cast<const T *>(p.q) + (u - 2 * H) * p.q_hs + col, ts = p.q_ts;
-    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(pieces + buf * PASSES * threads + tid));
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(pieces + buf * PASSES * threads + mine));
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       const int r = row0 + i * step;
       const bool real = r >= lo && r < hi;
-      copy16(to + i * threads * 16, x + (token0 + (real ? r : lo)) * ts, real);
+      const T *from = x + (token0 + (real ? r : lo)) * ts;
+      copy16(to + i * step * (D * int(sizeof(T))), from, real);
+      if constexpr (ROTATED) copy16(to + i * step * (D * int(sizeof(T))) + (col2 - col) * int(sizeof(T)), from + (col2 - col), real);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  int all = 2 * H;
-  if constexpr (ROTATED) all += p.heads;
-  const int u0 = blockIdx.y * p.units, u1 = min(u0 + p.units, all);
+  const int u0 = blockIdx.y * p.units, u1 = min(u0 + p.units, 2 * H);
   fetch(u0, 0);
   const bool bad = page < 0 || page >= s.pages;
   if (bad && tid == 0) report(s.status, STATUS_PAGE);
   const int64_t unit0 = int64_t(bad ? 0 : page) * 2 * H;
-  const auto held_at = [&](int u) { return lo > 0 && (!ROTATED || u < 2 * H) ? p.exps[unit0 + u] : 0; };
-  int held = held_at(u0);
+  int held = lo > 0 ? p.exps[unit0 + u0] : 0;
+  // angles of keys: of row row0, and of i * step rows
+  constexpr int PAIRS = ROTATED ? V::N : 1;
+  float first_c[PAIRS], first_s[PAIRS];
+  __shared__ __align__(16) float2 steps[ROTATED ? ROWS : 1][D / 2];
+  // the j-th pair of the thread's pieces
+  const auto pair_at = [&](int j) { return MODE == HALVES ? col + j : j < V::N / 2 ? col / 2 + j : col2 / 2 + j - V::N / 2; };
+  if constexpr (MODE == HALVES || MODE == NEIGHBOURS)
+    if (u0 < H) {
+      for (int i = tid; i < ROWS * (D / 2); i += threads) {
+        float c, s;
+        rotary::turn_of(int64_t(i / (D / 2)) * step, p.frequency[i % (D / 2)], c, s);
+        steps[i / (D / 2)][i % (D / 2)] = make_float2(c, s);
+      }
+      if (pairs) {
+#pragma unroll
+        for (int j = 0; j < V::N; ++j) {
+          rotary::turn_of(int64_t(pos0) + row0, p.frequency[pair_at(j)], first_c[j], first_s[j]);
+          first_c[j] *= p.gain, first_s[j] *= p.gain;
+        }
+      }
+      __syncthreads();
+    }
   for (int u = u0; u < u1; ++u) {
     const int buf = (u - u0) & 1, old = lo > 0 ? held_exponent(held) : E_MIN;
     if (u + 1 < u1) {
       fetch(u + 1, buf ^ 1);
-      held = held_at(u + 1);
+      held = lo > 0 ? p.exps[unit0 + u + 1] : 0;
       asm volatile("cp.async.wait_group 1;" ::: "memory");
     } else {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     // every thread reads only the pieces it copied
-    const uint4 *mine = pieces + buf * PASSES * threads + tid;
+    const uint4 *held_rows = pieces + buf * PASSES * threads + mine;
     float amax = 0.0f;
-    float turned[ROTATED ? PASSES : 1][V::N];
-    bool turn = false;  // keys, which are turned, or queries
+    float turned[ROTATED ? ROWS : 1][2 * V::N];
+    const bool turn = ROTATED && u < H;
     if constexpr (ROTATED) {
-      turn = u < H || u >= 2 * H;
-      __syncwarp();  // but turned ones are paired with others of the row, which its warp copied
       if (turn) {
+        if (MODE == ANY) __syncwarp();  // but for these, paired with any value of a row that their warp copied
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
+        for (int i = 0; i < ROWS; ++i) {
           const int r = row0 + i * step;
           if (r < lo || r >= hi) continue;
-          const T *row = reinterpret_cast<const T *>(pieces + buf * PASSES * threads + i * threads + (tid & ~(LPR - 1)));
-          turn_piece<T>(p, row, col, position_of(p, token0 + r, pos0 + r), turned[i]);
-          if (u >= 2 * H)
-            store_query(p, token0 + r, u - 2 * H, col, turned[i]);
-          else
-            amax = max_finite(turned[i], amax);
+          const uint4 *at = held_rows + i * step * LPR;
+          float(&y)[2 * V::N] = turned[i];
+          if constexpr (MODE == ANY) {
+            const int64_t pos = position_of(p, token0 + r, pos0 + r);
+            turn_apart<T>(p, reinterpret_cast<const T *>(at - col / V::N), col, pos, &y[0]);
+            turn_apart<T>(p, reinterpret_cast<const T *>(at - col / V::N), col2, pos, &y[V::N]);
+          } else {
+            V a, b;
+            a.load(at);
+            b.load(at + (col2 - col) / V::N);
+#pragma unroll
+            for (int j = 0; j < V::N; ++j) y[j] = a.at(j), y[V::N + j] = b.at(j);
+            if (pairs) {
+#pragma unroll
+              for (int j = 0; j < V::N; ++j) {
+                const int u = MODE == HALVES ? j : 2 * j, v = MODE == HALVES ? V::N + j : 2 * j + 1, pair = pair_at(j);
+                if (MODE == NEIGHBOURS && 2 * pair >= p.dims) continue;
+                const float2 by = steps[i][pair];
+                const float c = first_c[j] * by.x - first_s[j] * by.y, s = first_s[j] * by.x + first_c[j] * by.y;
+                const float x = y[u];
+                y[u] = x * c - y[v] * s;
+                y[v] = x * s + y[v] * c;
+              }
+            }
+          }
+          amax = max_finite(y, amax);
         }
-        __syncwarp();  // before this buffer's next copies
-        if (u >= 2 * H) continue;
+        if (MODE == ANY) __syncwarp();  // before this buffer's next copies
       }
     }
     if (!turn) {
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
+      for (int i = 0; i < ROWS; ++i) {
         V v;
-        v.load(mine + i * threads);
+        v.load(held_rows + i * step * LPR);
         amax = max_finite(v, amax);
+        if constexpr (ROTATED) {
+          v.load(held_rows + i * step * LPR + (col2 - col) / V::N);
+          amax = max_finite(v, amax);
+        }
       }
     }
     amax = warp_max(amax);
@@ -349,17 +392,22 @@ __global__ void __launch_bounds__(MOST_THREADS<D, T>) append_kernel(const __grid
     uint8_t *codes = p.codes + ((unit0 + u) << s.page_shift) * D;
     if (tid == 0) p.exps[unit0 + u] = int8_t(e);
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       const int r = row0 + i * step;
       if (r >= lo && r < hi) {
         if constexpr (ROTATED)
           if (turn) {
-            store_codes(codes + r * D + col, turned[i], e);
+            store_codes<V::N>(codes + r * D + col, &turned[i][0], e);
+            store_codes<V::N>(codes + r * D + col2, &turned[i][V::N], e);
             continue;
           }
         V v;
-        v.load(mine + i * threads);
+        v.load(held_rows + i * step * LPR);
         store_codes(codes + r * D + col, v, e);
+        if constexpr (ROTATED) {
+          v.load(held_rows + i * step * LPR + (col2 - col) / V::N);
+          store_codes(codes + r * D + col2, v, e);
+        }
       }
     }
     if (lo > 0 && e > old) recode_rows<D>(codes, lo, old, e, tid, threads);
@@ -404,7 +452,9 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
       uint4 *row = rows[threadIdx.x >> 5];
       if (lane < LPR) row[lane] = v.w;
       __syncwarp();
-      if (lane < LPR) turn_piece<T>(p, reinterpret_cast<const T *>(row), lane * V::N, position_of(p, start, len - 1), turned);
+      if (lane < LPR) {
+        turn_apart(p, reinterpret_cast<const T *>(row), lane * V::N, position_of(p, start, len - 1), turned);
+      }
       if (query) {
         if (lane < LPR) store_query(p, start, unit_of_seq - 2 * s.kv_heads, lane * V::N, turned);
         return;
@@ -425,7 +475,7 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
   if (lane < LPR) {
     uint8_t *at = codes + int64_t(lo) * D + lane * V::N;
     if (turn)
-      store_codes(at, turned, e);
+      store_codes<V::N>(at, turned, e);
     else
       store_codes(at, v, e);
   }
@@ -435,7 +485,8 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
 template <int D, typename T, typename Params>
 int launch(Params p, bool one, int64_t slots, int device, cudaStream_t stream) {
   int units = 2 * p.s.kv_heads;
-  if constexpr (std::is_same<Params, RotatedParams>::value) units += p.heads;
+  if constexpr (std::is_same<Params, RotatedParams>::value)
+    if (one) units += p.heads;
   if (one)
     return launch_kernel("emmy_kv8_append", append_one_kernel<D, T, Params>, dim3(p.s.seqs, (units + 3) / 4), 128, 0, stream, p);
   // several (side, head)s a CTA once there are more than fill the GPU twice
@@ -445,12 +496,20 @@ int launch(Params p, bool one, int64_t slots, int device, cudaStream_t stream) {
   int smem = 2 * 8 * 16 * threads;
   constexpr int ROOM = 200 * 1024;
   if (smem > ROOM) smem /= 2, p.units = 1;  // no second buffer, so no second unit (f32 pages of 128 KB)
-  static KernelSetup setup;
-  const int rc = setup.ready("emmy_kv8_append", append_kernel<D, T, Params>, device,
-                             std::min(ROOM, 2 * 8 * 16 * MOST_THREADS<D, T>));
-  if (rc != EMMY_OK) return rc;
-  return launch_kernel("emmy_kv8_append", append_kernel<D, T, Params>, dim3(unsigned(slots), (units + p.units - 1) / p.units),
-                       threads, smem, stream, p);
+  const auto run = [&](auto kernel, KernelSetup &setup) {
+    const int rc = setup.ready("emmy_kv8_append", kernel, device, std::min(ROOM, 2 * 8 * 16 * MOST_THREADS<D, T>));
+    if (rc != EMMY_OK) return rc;
+    return launch_kernel("emmy_kv8_append", kernel, dim3(unsigned(slots), (units + p.units - 1) / p.units), threads, smem,
+                         stream, p);
+  };
+  static KernelSetup setup[4];
+  if constexpr (std::is_same<Params, RotatedParams>::value) {
+    if (p.positions == nullptr && p.interleaved) return run(append_kernel<D, T, NEIGHBOURS, Params>, setup[NEIGHBOURS]);
+    if (p.positions == nullptr && p.dims / 2 % Vec<T>::N == 0) return run(append_kernel<D, T, HALVES, Params>, setup[HALVES]);
+    return run(append_kernel<D, T, ANY, Params>, setup[ANY]);
+  } else {
+    return run(append_kernel<D, T, PLAIN, Params>, setup[PLAIN]);
+  }
 }
 
 template <int D, typename Params>
@@ -561,5 +620,20 @@ extern "C" int emmy_kv8_append_rotated(const emmy_kv8 *cache, emmy_dptr k, emmy_
     p.q_ts = qs[0], p.q_hs = qs[1], p.o_ts = os[0], p.o_hs = os[1];
     p.out_type = a->out_dtype;
   }
-  return append(what, p, cache, dtype, stream);
+  const int rc2 = append(what, p, cache, dtype, stream);
+  if (rc2 != EMMY_OK || a->heads == 0 || cache->max_q == 1) return rc2;
+  rotary::Params r;
+  for (int i = 0; i < EMMY_ROTARY_PAIRS; ++i) r.frequency[i] = rotary->turns[i];
+  r.x = p.q, r.out = p.out;
+  r.positions = p.positions, r.position_stride = p.position_stride, r.wide = p.wide;
+  r.first = 0, r.tokens = cache->tokens;
+  r.x_ts = p.q_ts, r.x_hs = p.q_hs, r.o_ts = p.o_ts, r.o_hs = p.o_hs;
+  r.heads = p.heads, r.dims = p.dims, r.head_dim = cache->head_dim;
+  r.interleaved = p.interleaved, r.copy = a->q != a->q_out;
+  r.gain = p.gain, r.sign = 1.0f;
+  r.s = p.s;
+  r.s.status = nullptr;  // what is wrong with the lengths is reported already
+  const OnDevice on(cache->device);
+  if (on.err != cudaSuccess) return cuda_fail(what, on.err);
+  return rotary::rotate_rows(what, r, dtype, a->out_dtype, static_cast<cudaStream_t>(stream));
 }

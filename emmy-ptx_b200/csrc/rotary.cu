@@ -9,129 +9,152 @@
 // Bound by memory: each value is read and written once.  A thread holds one piece
 // (16 bytes, or less where sizes or addresses ask for it) of a token's row, with
 // the piece that it is paired with, and does the same of HEADS heads: the angles
-// cost about 40 instructions each and are computed once for all of them.
-#include "kv8.cuh"
+// cost about 40 instructions each and are computed once for all of them, while the
+// values are on their way.
 #include "rotary.cuh"
 
 namespace rotary {
 namespace {
 
-constexpr int THREADS = 256, HEADS = 4;
+constexpr int THREADS = 256;
+// Heads of a thread: as many as are eight loads.
+template <bool INTERLEAVED>
+constexpr int heads_of = INTERLEAVED ? 8 : 4;
 
-struct Params {
-  uint64_t frequency[EMMY_ROTARY_PAIRS];
-  const void *x;
-  void *out;
-  const void *positions;  // null: first, first + 1, ..
-  int64_t first, position_stride, tokens;
-  int64_t x_ts, x_hs, o_ts, o_hs;  // token and head strides, elements
-  int heads, dims, head_dim;
-  int pieces, turned;     // pieces of a head that threads hold (with those paired with them), those turned
-  int slices;             // of a token's heads: thread slice i has heads i, i + slices, ..
-  int width, block_tokens;  // threads of a token, tokens of a block
-  bool wide, interleaved, copy;
-  float gain, sign;
-};
+// Place of a new token in its sequence; false: it is in none that can be.
+__device__ __forceinline__ bool place_of(const kv8::Seqs &s, int64_t token, int64_t &place) {
+  int lo = 0, hi = s.seqs - 1;  // the last sequence that begins at or before it
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s.q_starts[mid] <= token) lo = mid; else hi = mid - 1;
+  }
+  int start, n, len;
+  kv8::lengths(s, lo, start, n, len);
+  place = len - n + token - start;
+  return token >= start && token < int64_t(start) + n;
+}
 
-template <typename T, int N, bool INTERLEAVED>
+template <typename T, typename U, int N, bool INTERLEAVED>
 __global__ void __launch_bounds__(THREADS) rotate_kernel(const __grid_constant__ Params p) {
   using P = Piece<T, N>;
+  using O = Piece<U, N>;
+  constexpr int HEADS = heads_of<INTERLEAVED>;
   constexpr int PAIRS = INTERLEAVED ? N / 2 : N;  // that a thread holds
   kv8::grid_dependency_wait();
   kv8::grid_dependency_done();
-  const int sub = threadIdx.x / p.width;
-  const int64_t token = int64_t(blockIdx.x) * p.block_tokens + sub;
-  if (sub >= p.block_tokens || token >= p.tokens) return;
-  int64_t pos = p.first + token;
-  if (p.positions != nullptr)
-    pos = p.wide ? static_cast<const int64_t *>(p.positions)[token * p.position_stride]
-                 : static_cast<const int *>(p.positions)[token * p.position_stride];
-  for (int t = threadIdx.x - sub * p.width; t < p.width; t += p.block_tokens == 1 ? THREADS : p.width) {
-    const int slice = t / p.pieces, piece = t - slice * p.pieces;
-    const T *x = static_cast<const T *>(p.x) + token * p.x_ts;
-    T *out = static_cast<T *>(p.out) + token * p.o_ts;
-    if (piece >= p.turned) {
-      // behind the turned ones
-      const int at = p.dims + (piece - p.turned) * N;
-      for (int h = slice; h < p.heads; h += p.slices)
-        *reinterpret_cast<P *>(out + h * p.o_hs + at) = *reinterpret_cast<const P *>(x + h * p.x_hs + at);
-      continue;
-    }
+  for (int t = threadIdx.x; t < p.block_tokens * p.width; t += THREADS) {
+    const int sub = t / p.width, of_token = t - sub * p.width, slice = of_token / p.pieces, piece = of_token - slice * p.pieces;
+    const int64_t token = int64_t(blockIdx.x) * p.block_tokens + sub;
+    if (token >= p.tokens) return;
+    int64_t pos = p.first + token;
+    if (p.s.seqs > 0 && !place_of(p.s, token, pos)) continue;
+    if (p.positions != nullptr)
+      pos = p.wide ? static_cast<const int64_t *>(p.positions)[token * p.position_stride]
+                   : static_cast<const int *>(p.positions)[token * p.position_stride];
     // single values of an interleaved row: pairs are neighbours all the same
-    const bool near = N == 1 && p.interleaved;
-    const int at = near ? 2 * piece : piece * N, other = near ? 1 : p.dims / 2;
-    float c[PAIRS], s[PAIRS];
+    const bool near = N == 1 && p.interleaved, turned = piece < p.turned;
+    const int at = !turned ? p.dims + (piece - p.turned) * N : near ? 2 * piece : piece * N;
+    const int other = at + (near ? 1 : p.dims / 2);
+    const T *x = static_cast<const T *>(p.x) + token * p.x_ts;
+    U *out = static_cast<U *>(p.out) + token * p.o_ts;
+    // on their way while the angles are computed
+    P a[HEADS], b[INTERLEAVED ? 1 : HEADS];
 #pragma unroll
-    for (int i = 0; i < PAIRS; ++i) {
-      turn_of(pos, p.frequency[piece * PAIRS + i], c[i], s[i]);
-      c[i] *= p.gain;
-      s[i] *= p.gain * p.sign;
+    for (int j = 0; j < HEADS; ++j) {
+      const int h = slice + j * p.slices;
+      if (h >= p.heads) continue;
+      a[j] = *reinterpret_cast<const P *>(x + h * p.x_hs + at);
+      if constexpr (!INTERLEAVED)
+        if (turned) b[j] = *reinterpret_cast<const P *>(x + h * p.x_hs + other);
     }
-    for (int h0 = slice; h0 < p.heads; h0 += HEADS * p.slices) {
-      P a[HEADS], b[INTERLEAVED ? 1 : HEADS];
+    float c[PAIRS], s[PAIRS];
+    if (turned) {
 #pragma unroll
-      for (int j = 0; j < HEADS; ++j) {
-        const int h = h0 + j * p.slices;
-        if (h >= p.heads) continue;
-        a[j] = *reinterpret_cast<const P *>(x + h * p.x_hs + at);
-        if constexpr (!INTERLEAVED) b[j] = *reinterpret_cast<const P *>(x + h * p.x_hs + at + other);
+      for (int i = 0; i < PAIRS; ++i) {
+        turn_of(pos, p.frequency[piece * PAIRS + i], c[i], s[i]);
+        c[i] *= p.gain;
+        s[i] *= p.gain * p.sign;
       }
+    }
 #pragma unroll
-      for (int j = 0; j < HEADS; ++j) {
-        const int h = h0 + j * p.slices;
-        if (h >= p.heads) continue;
+    for (int j = 0; j < HEADS; ++j) {
+      const int h = slice + j * p.slices;
+      if (h >= p.heads) continue;
+      O u, v;
+      if (turned) {
+        if constexpr (INTERLEAVED)
+          turn_neighbours<T, U, N>(a[j], c, s, u);
+        else
+          turn_pieces<T, U, N>(a[j], b[j], c, s, u, v);
+        if constexpr (!INTERLEAVED) *reinterpret_cast<O *>(out + h * p.o_hs + other) = v;
+      } else {
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
-          T &u = INTERLEAVED ? a[j].v[2 * i] : a[j].v[i], &v = INTERLEAVED ? a[j].v[2 * i + 1] : b[INTERLEAVED ? 0 : j].v[i];
-          const float fu = to_float(u), fv = to_float(v);
-          u = rounded<T>(fu * c[i] - fv * s[i]);
-          v = rounded<T>(fu * s[i] + fv * c[i]);
+        for (int i = 0; i < N; ++i) {
+          if constexpr (std::is_same<T, U>::value)
+            u.v[i] = a[j].v[i];
+          else
+            u.v[i] = rounded<U>(to_float(a[j].v[i]));
         }
-        *reinterpret_cast<P *>(out + h * p.o_hs + at) = a[j];
-        if constexpr (!INTERLEAVED) *reinterpret_cast<P *>(out + h * p.o_hs + at + other) = b[j];
       }
+      *reinterpret_cast<O *>(out + h * p.o_hs + at) = u;
     }
   }
 }
 
-template <typename T, int N, bool INTERLEAVED>
-int launch(Params p, cudaStream_t stream) {
+template <typename T, typename U, int N, bool INTERLEAVED>
+int launch(const char *what, Params &p, cudaStream_t stream) {
+  constexpr int HEADS = heads_of<INTERLEAVED>;
   p.turned = INTERLEAVED ? p.dims / N : p.dims / 2 / N;
   p.pieces = p.turned + (p.copy ? (p.head_dim - p.dims) / N : 0);
   p.slices = (p.heads + HEADS - 1) / HEADS;
-  const int64_t width = int64_t(p.slices) * p.pieces;
-  p.width = int(width);
-  p.block_tokens = width >= THREADS ? 1 : THREADS / int(width);
+  p.width = p.slices * p.pieces;  // at most 2^18 * 512
+  // tokens of a block: those that leave the fewest threads idle
+  p.block_tokens = 1;
+  double best = 0;
+  for (int n = 1; n <= 16 && n * int64_t(p.width) <= 4 * THREADS; ++n) {
+    const double used = double(n * p.width) / ((n * p.width + THREADS - 1) / THREADS * THREADS);
+    if (used > best + 0.05) best = used, p.block_tokens = n;
+  }
   const int64_t blocks = (p.tokens + p.block_tokens - 1) / p.block_tokens;
-  return kv8::launch_kernel("emmy_rotate", rotate_kernel<T, N, INTERLEAVED>, dim3(unsigned(blocks)),
-                            THREADS, 0, stream, p);
+  return kv8::launch_kernel(what, rotate_kernel<T, U, N, INTERLEAVED>, dim3(unsigned(blocks)), THREADS, 0, stream, p);
 }
 
-template <typename T, int N>
-int launch_layout(const Params &p, cudaStream_t stream) {
+template <typename T, typename U, int N>
+int launch_layout(const char *what, Params &p, cudaStream_t stream) {
   if constexpr (N > 1)
-    if (p.interleaved) return launch<T, N, true>(p, stream);
-  return launch<T, N, false>(p, stream);
+    if (p.interleaved) return launch<T, U, N, true>(what, p, stream);
+  return launch<T, U, N, false>(what, p, stream);
 }
 
 // The widest pieces that start everywhere on a multiple of their size.
-template <typename T>
-int launch_type(const Params &p, cudaStream_t stream) {
+template <typename T, typename U>
+int launch_type(const char *what, Params &p, cudaStream_t stream) {
   const auto fits = [&](int n) {
-    const int64_t size = int64_t(n) * sizeof(T);
-    const int64_t half = p.interleaved ? p.dims : p.dims / 2;
-    return reinterpret_cast<uintptr_t>(p.x) % size == 0 && reinterpret_cast<uintptr_t>(p.out) % size == 0 &&
+    const int half = p.interleaved ? p.dims : p.dims / 2;
+    return reinterpret_cast<uintptr_t>(p.x) % (n * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.out) % (n * sizeof(U)) == 0 &&
            p.x_ts % n == 0 && p.x_hs % n == 0 && p.o_ts % n == 0 && p.o_hs % n == 0 && half % n == 0 &&
            (!p.copy || (p.head_dim - p.dims) % n == 0);
   };
-  if constexpr (sizeof(T) == 2)
-    if (fits(8)) return launch_layout<T, 8>(p, stream);
-  if (fits(4)) return launch_layout<T, 4>(p, stream);
-  if (fits(2)) return launch_layout<T, 2>(p, stream);
-  return launch_layout<T, 1>(p, stream);
+  if constexpr (sizeof(T) == 2 && sizeof(U) == 2)
+    if (fits(8)) return launch_layout<T, U, 8>(what, p, stream);
+  if (fits(4)) return launch_layout<T, U, 4>(what, p, stream);
+  if (fits(2)) return launch_layout<T, U, 2>(what, p, stream);
+  return launch_layout<T, U, 1>(what, p, stream);
+}
+
+template <typename T>
+int launch_out(const char *what, Params &p, int out_type, cudaStream_t stream) {
+  if (out_type == EMMY_KV8_F32) return launch_type<T, float>(what, p, stream);
+  return out_type == EMMY_KV8_BF16 ? launch_type<T, __nv_bfloat16>(what, p, stream) : launch_type<T, __half>(what, p, stream);
 }
 
 }  // namespace
+
+int rotate_rows(const char *what, Params &p, int type, int out_type, cudaStream_t stream) {
+  if (type == EMMY_KV8_F32) return launch_out<float>(what, p, out_type, stream);
+  return type == EMMY_KV8_BF16 ? launch_out<__nv_bfloat16>(what, p, out_type, stream) : launch_out<__half>(what, p, out_type, stream);
+}
+
 }  // namespace rotary
 
 extern "C" int emmy_rotate(const emmy_rotary *r, const emmy_rotate_args *a, emmy_stream stream) {
@@ -172,11 +195,10 @@ extern "C" int emmy_rotate(const emmy_rotary *r, const emmy_rotate_args *a, emmy
   p.wide = a->wide != 0;
   p.interleaved = r->interleaved != 0;
   p.copy = !in_place;
+  p.s.seqs = 0;
   p.gain = r->gain;
   p.sign = a->backward ? -1.0f : 1.0f;
   const kv8::OnDevice on(a->device);
   if (on.err != cudaSuccess) return kv8::cuda_fail(what, on.err);
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dtype == EMMY_KV8_F32) return launch_type<float>(p, st);
-  return a->dtype == EMMY_KV8_BF16 ? launch_type<__nv_bfloat16>(p, st) : launch_type<__half>(p, st);
+  return rotate_rows(what, p, a->dtype, a->dtype, static_cast<cudaStream_t>(stream));
 }

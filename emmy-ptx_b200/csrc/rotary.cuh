@@ -5,6 +5,9 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
+
+#include "kv8.cuh"
 
 namespace rotary {
 
@@ -28,6 +31,25 @@ __device__ __forceinline__ void turn_of(int64_t position, uint64_t frequency, fl
   if (quarter & 2) s = -s;
 }
 
+// Rows to turn: those of a call by themselves, or a cache's new tokens.
+struct Params {
+  uint64_t frequency[EMMY_ROTARY_PAIRS];
+  const void *x;
+  void *out;
+  const void *positions;  // null: first, first + 1, .., or the places in the sequences
+  int64_t first, position_stride, tokens;
+  int64_t x_ts, x_hs, o_ts, o_hs;  // token and head strides, elements
+  int heads, dims, head_dim;
+  int pieces, turned;     // pieces of a head that threads hold (with those paired with them), those turned
+  int slices;             // of a token's heads: thread slice i has heads i, i + slices, ..
+  int width, block_tokens;  // threads of a token, tokens of a block
+  bool wide, interleaved, copy;
+  float gain, sign;
+  kv8::Seqs s;            // s.seqs = 0: no sequences
+};
+// Launches on the current device; types are EMMY_KV8_F32 and so on.
+int rotate_rows(const char *what, Params &p, int type, int out_type, cudaStream_t stream);
+
 // N neighbouring values as one access of at most 16 bytes.
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Piece {
@@ -45,5 +67,68 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <>
 __device__ __forceinline__ __half rounded<__half>(float x) { return __float2half_rn(x); }
+
+// Two neighbouring values of a 32-bit word, and back with one rounding each.
+template <typename T>
+__device__ __forceinline__ float2 unpacked(uint32_t w) {
+  if constexpr (sizeof(T) == 4) {
+    return make_float2(0.0f, 0.0f);  // a word is one value
+  } else if constexpr (std::is_same<T, __half>::value) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  } else {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t packed(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+}
+
+// (a, b) turned into (u, v), of pieces a and b whose values pair up (half layout), or of one
+// piece a of neighbours; c, s of each pair.
+template <typename T, typename U, int N>
+__device__ __forceinline__ void turn_pieces(const Piece<T, N> &a, const Piece<T, N> &b, const float (&c)[N], const float (&s)[N],
+                                            Piece<U, N> &u, Piece<U, N> &v) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, U>::value && N >= 2) {
+    const uint32_t *x = reinterpret_cast<const uint32_t *>(&a), *y = reinterpret_cast<const uint32_t *>(&b);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 p = unpacked<T>(x[i]), q = unpacked<T>(y[i]);
+      reinterpret_cast<uint32_t *>(&u)[i] = packed<T>(p.x * c[2 * i] - q.x * s[2 * i], p.y * c[2 * i + 1] - q.y * s[2 * i + 1]);
+      reinterpret_cast<uint32_t *>(&v)[i] = packed<T>(p.x * s[2 * i] + q.x * c[2 * i], p.y * s[2 * i + 1] + q.y * c[2 * i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float x = to_float(a.v[i]), y = to_float(b.v[i]);
+      u.v[i] = rounded<U>(x * c[i] - y * s[i]);
+      v.v[i] = rounded<U>(x * s[i] + y * c[i]);
+    }
+  }
+}
+template <typename T, typename U, int N>
+__device__ __forceinline__ void turn_neighbours(const Piece<T, N> &a, const float (&c)[N / 2], const float (&s)[N / 2], Piece<U, N> &u) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, U>::value) {
+    const uint32_t *x = reinterpret_cast<const uint32_t *>(&a);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 p = unpacked<T>(x[i]);
+      reinterpret_cast<uint32_t *>(&u)[i] = packed<T>(p.x * c[i] - p.y * s[i], p.x * s[i] + p.y * c[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float x = to_float(a.v[2 * i]), y = to_float(a.v[2 * i + 1]);
+      u.v[2 * i] = rounded<U>(x * c[i] - y * s[i]);
+      u.v[2 * i + 1] = rounded<U>(x * s[i] + y * c[i]);
+    }
+  }
+}
 
 }  // namespace rotary

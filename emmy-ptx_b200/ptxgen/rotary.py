@@ -41,6 +41,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from fractions import Fraction
 
 from .kvcache import _dtype_code, _positions, _stream_of
@@ -59,13 +60,10 @@ class _Rotary(C.Structure):
                 ("dims", C.c_int32), ("interleaved", C.c_int32)]
 
 
-class _Rotate(C.Structure):
-    """``emmy_rotate_args``."""
-    _fields_ = [("x", C.c_uint64), ("out", C.c_uint64), ("positions", C.c_uint64),
-                ("x_strides", C.c_int64 * 2), ("out_strides", C.c_int64 * 2),
-                ("position_stride", C.c_int64), ("first", C.c_int64), ("tokens", C.c_int64),
-                ("heads", C.c_int32), ("dtype", C.c_int32), ("wide", C.c_int32),
-                ("backward", C.c_int32), ("device", C.c_int32)]
+# emmy_rotate_args: x, out, positions; strides of x and out, position_stride, first,
+# tokens; heads, dtype, wide, backward, device (packed at once: a ctypes structure
+# costs 2 us more a call)
+_ARGS = struct.Struct("@3Q7q5i4x")
 
 
 def _scaled(dims: int, base: float, scaling) -> tuple[list[float], float]:
@@ -166,22 +164,21 @@ class Rotary:
         shape, xs, os_ = x.shape, x.stride(), out.stride()
         if len(shape) != 3 or shape[2] != self.head_dim:
             raise EmmyError(f"x has shape {tuple(shape)}, expected [tokens, heads, {self.head_dim}]")
-        if tuple(out.shape) != tuple(shape):
+        if out.shape != shape:
             raise EmmyError(f"out has shape {tuple(out.shape)}, expected {tuple(shape)}")
         if xs[2] != 1 or os_[2] != 1:
             raise EmmyError("x and out: the last dimension must be contiguous")
         code = _dtype_code(x.dtype)
         if code > 2 or _dtype_code(out.dtype) != code:
             raise EmmyError("x and out must both be f32, bf16 or f16")
-        ordinal = x.get_device()
+        ordinal, (tokens, heads, _) = x.get_device(), shape
         if ordinal < 0 or out.get_device() != ordinal:
             raise EmmyError("x and out must be on one device")
-        at, step, wide, first = _positions(positions, shape[0], ordinal)
-        L = load_library()
-        st = _stream_of(stream, None) if stream is not None else _stream_of(None, Device.get(ordinal))
-        a = _Rotate(x.data_ptr(), out.data_ptr(), at, (xs[0], xs[1]), (os_[0], os_[1]), step, first,
-                    shape[0], shape[1], code, wide, backward, ordinal)
-        rc = L.emmy_rotate(self._ref, C.byref(a), st)
+        at, step, wide, first = _positions(positions, tokens, ordinal)
+        st = _stream_of(stream, None if stream is not None else Device.get(ordinal))
+        rc = load_library().emmy_rotate(
+            self._ref, _ARGS.pack(x.data_ptr(), out.data_ptr(), at, xs[0], xs[1], os_[0], os_[1], step, first,
+                                  tokens, heads, code, wide, backward, ordinal), st)
         if rc:
             check(rc, "rotate")
         return out

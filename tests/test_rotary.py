@@ -4,11 +4,12 @@ formulas, how they are held, what the calls refuse, and what they hand on."""
 import ctypes as C
 import math
 from fractions import Fraction
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
 
-from ptxgen import Rotary, rotary as ro
+from ptxgen import Rotary, kvcache as kv, rotary as ro
 from ptxgen.kvcache import DeviceArray
 from ptxgen.runtime import EmmyError
 from tests.test_kvcache import dev, small  # noqa: F401 - a fixture
@@ -125,18 +126,22 @@ def test_rotate_refusals(lib, x, pos, out, says):
     assert not lib.calls
 
 
+def unpacked(form, raw, names):
+    return SimpleNamespace(**dict(zip(names.split(), form.unpack(raw))))
+
+
 def test_rotate_hands_on(lib):
     rot = Rotary(64, 32, interleaved=True)
     out = arr(X, ptr=8192)
     assert rot.backward(arr(X, strides=(640, 128, 1)), arr((9,), "i32", 512, (2,)), out, stream=11) is out
     (name, (ref, args, st)), = lib.calls
-    a = args._obj
+    a = unpacked(ro._ARGS, args, "x out positions x_t x_h out_t out_h position_stride first tokens heads dtype wide backward device")
     assert (name, st, ref._obj.dims, ref._obj.interleaved) == ("emmy_rotate", 11, 32, 1)
-    assert (a.x, a.out, a.positions, list(a.x_strides), list(a.out_strides)) == (4096, 8192, 512, [640, 128], [192, 64])
+    assert (a.x, a.out, a.positions, a.x_t, a.x_h, a.out_t, a.out_h) == (4096, 8192, 512, 640, 128, 192, 64)
     assert (a.position_stride, a.wide, a.tokens, a.heads, a.dtype, a.backward) == (2, 0, 5, 3, 1, 1)
     rot.rotate(out, np.int64(-7), out)
-    a = lib.calls[-1][1][1]._obj
-    assert (a.positions, a.first, a.backward, lib.calls[-1][1][2]) == (0, -7, 0, 7)
+    a = ro._ARGS.unpack(lib.calls[-1][1][1])
+    assert (a[2], a[8], a[13], lib.calls[-1][1][2]) == (0, -7, 0, 7)
 
 
 KV, Q = (5, 2, 64), (5, 6, 64)
@@ -168,12 +173,9 @@ def test_append_hands_on(dev):  # noqa: F811
                  positions=arr((5,), "i64", 64), stream=3)
     name, a = dev.L.calls[-1]
     assert name == "emmy_kv8_append_rotated" and a[1:4] == (4096, 8192, 1) and a[6] is rot._ref and a[8] == 3
-    r = a[7]._obj
-    assert (r.positions, r.q, r.q_out, r.position_stride, r.wide, r.heads, r.out_dtype) == (64, 512, 1024, 1, 1, 6, 2)
-    assert (list(r.q_strides), list(r.out_strides)) == ([384, 64], [384, 64])
+    assert kv._ROTATED.unpack(a[7]) == (64, 512, 1024, 1, 384, 64, 384, 64, 1, 6, 2)
     batch.append(1, arr(KV), arr(KV, ptr=8192), rotary=rot, stream=3)
-    r = dev.L.calls[-1][1][7]._obj
-    assert (r.positions, r.q, r.heads) == (0, 0, 0)
+    assert kv._ROTATED.unpack(dev.L.calls[-1][1][7]) == (0,) * 11
 
 
 def real():
@@ -181,11 +183,29 @@ def real():
     return load_library()
 
 
+class RotateArgs(C.Structure):
+    """``emmy_rotate_args``."""
+    _fields_ = [("x", C.c_uint64), ("out", C.c_uint64), ("positions", C.c_uint64),
+                ("x_strides", C.c_int64 * 2), ("out_strides", C.c_int64 * 2),
+                ("position_stride", C.c_int64), ("first", C.c_int64), ("tokens", C.c_int64),
+                ("heads", C.c_int32), ("dtype", C.c_int32), ("wide", C.c_int32),
+                ("backward", C.c_int32), ("device", C.c_int32)]
+
+
 def rotate_args(**kw):
-    a = ro._Rotate(4096, 1 << 20, 0, (128, 64), (128, 64), 0, 0, 5, 2, 1, 0, 0, 0)
+    a = RotateArgs(4096, 1 << 20, 0, (128, 64), (128, 64), 0, 0, 5, 2, 1, 0, 0, 0)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
+
+
+def test_packed_arguments():
+    """The packed form lies as the structure does."""
+    values = (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15)
+    a = RotateArgs.from_buffer_copy(ro._ARGS.pack(*values))
+    assert C.sizeof(RotateArgs) == ro._ARGS.size
+    assert (a.x, a.out, a.positions, *a.x_strides, *a.out_strides, a.position_stride, a.first, a.tokens, a.heads,
+            a.dtype, a.wide, a.backward, a.device) == values
 
 
 @pytest.mark.parametrize("kw,says", [
