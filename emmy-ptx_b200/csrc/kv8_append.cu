@@ -143,7 +143,7 @@ __device__ __forceinline__ int64_t position_of(const RotatedParams &p, int64_t t
 }
 
 // Values col .. col + 15 bytes of a row in shared memory, turned one by one.
-template <typename T>
+template <bool EXACT, typename T>
 __device__ __forceinline__ void turn_apart(const RotatedParams &p, const T *row, int col, int64_t pos, float *y) {
   const int half = p.dims / 2;
 #pragma unroll
@@ -154,8 +154,7 @@ __device__ __forceinline__ void turn_apart(const RotatedParams &p, const T *row,
     const bool low = p.interleaved ? at % 2 == 0 : at < half;
     const int away = p.interleaved ? 1 : half, other = low ? at + away : at - away;
     float c, s;
-    rotary::turn_of(pos, p.frequency[p.interleaved ? at / 2 : low ? at : other], c, s);
-    c *= p.gain, s *= p.gain;
+    rotary::turn<EXACT>(pos, p.frequency[p.interleaved ? at / 2 : low ? at : other], p.gain, c, s);
     y[i] = y[i] * c + rotary::to_float(row[other]) * (low ? -s : s);
   }
 }
@@ -170,7 +169,7 @@ __device__ __forceinline__ float max_finite(const float (&y)[N], float amax) {
   return amax;
 }
 template <int N>
-__device__ __forceinline__ void store_codes(uint8_t *at, const float *y, int e) {
+__device__ __forceinline__ void store_codes(uint8_t *at, const float (&y)[N], int e) {
   uint32_t w[2] = {};
 #pragma unroll
   for (int j = 0; j < N; j += 2)
@@ -240,15 +239,11 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool real)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 
-// How a page's keys are turned: not at all; with the pairs of a piece in another
-// whole piece, or within it, at their places in the sequence; or in any other way.
-enum { PLAIN = 0, HALVES, NEIGHBOURS, ANY };
-
-template <int D, typename T, int MODE, typename Params>
-__global__ void __launch_bounds__(MOST_THREADS<D, T>) append_kernel(const __grid_constant__ Params p) {
-  constexpr bool ROTATED = MODE != PLAIN;
+template <int D, typename T>
+__global__ void __launch_bounds__(MOST_THREADS<D, T>) append_kernel(const AppendParams p) {
   using V = Vec<T>;
   constexpr int LPR = D / V::N;  // lanes per row, 16 bytes each
+  constexpr int RPW = 32 / LPR;  // rows per warp and pass
   constexpr int PASSES = 8;
   extern __shared__ uint4 pieces[];  // [2][PASSES][threads]
   __shared__ float part[2][32];
@@ -262,33 +257,18 @@ __global__ void __launch_bounds__(MOST_THREADS<D, T>) append_kernel(const __grid
   const int pos0 = page_of_seq << s.page_shift;
   const int lo = max(first - pos0, 0), hi = min(len - pos0, P);  // new rows of the page
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
-  // The thread's piece of each row, or (turned) its two pieces that pair up, of half
-  // as many rows: row i is row0 + i * step.
-  constexpr int ROWS = ROTATED ? PASSES / 2 : PASSES, LANES = ROTATED ? LPR / 2 : LPR;
-  int col = lane % LANES * V::N, col2 = col + D / 2;
-  bool pairs = true;  // the pieces are turned
-  if constexpr (MODE == HALVES) {
-    const int half = p.dims / 2, at = lane % LANES - half / V::N;
-    pairs = at < 0;
-    if (!pairs) col = p.dims + at * V::N;  // behind the turned ones, as far from each other as fits
-    col2 = pairs ? col + half : col + (D - p.dims) / 2;
-  }
-  const int row0 = warp * (32 / LANES) + lane / LANES, step = warps * (32 / LANES);
+  const int col = lane % LPR * V::N, row0 = warp * RPW + lane / LPR, step = warps * RPW;
   const int64_t token0 = int64_t(start) + pos0 - first;  // row 0 of the page, were it new
-  // a buffer holds the page's rows, one after another
-  const int mine = row0 * LPR + col / V::N;
   const auto fetch = [&](int u, int buf) {
     const int side = u >= H, head = u - side * H;
     const int64_t ts = side ? p.ts[1] : p.ts[0];
     const T *x = static_cast<const T *>(side ? p.x[1] : p.x[0]) + head * (side ? p.hs[1] : p.hs[0]) + col;
-    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(pieces + buf * PASSES * threads + mine));
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(pieces + buf * PASSES * threads + tid));
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
+    for (int i = 0; i < PASSES; ++i) {
       const int r = row0 + i * step;
       const bool real = r >= lo && r < hi;
-      const T *from = x + (token0 + (real ? r : lo)) * ts;
-      copy16(to + i * step * (D * int(sizeof(T))), from, real);
-      if constexpr (ROTATED) copy16(to + i * step * (D * int(sizeof(T))) + (col2 - col) * int(sizeof(T)), from + (col2 - col), real);
+      copy16(to + i * threads * 16, x + (token0 + (real ? r : lo)) * ts, real);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -298,28 +278,6 @@ __global__ void __launch_bounds__(MOST_THREADS<D, T>) append_kernel(const __grid
   if (bad && tid == 0) report(s.status, STATUS_PAGE);
   const int64_t unit0 = int64_t(bad ? 0 : page) * 2 * H;
   int held = lo > 0 ? p.exps[unit0 + u0] : 0;
-  // angles of keys: of row row0, and of i * step rows
-  constexpr int PAIRS = ROTATED ? V::N : 1;
-  float first_c[PAIRS], first_s[PAIRS];
-  __shared__ __align__(16) float2 steps[ROTATED ? ROWS : 1][D / 2];
-  // the j-th pair of the thread's pieces
-  const auto pair_at = [&](int j) { return MODE == HALVES ? col + j : j < V::N / 2 ? col / 2 + j : col2 / 2 + j - V::N / 2; };
-  if constexpr (MODE == HALVES || MODE == NEIGHBOURS)
-    if (u0 < H) {
-      for (int i = tid; i < ROWS * (D / 2); i += threads) {
-        float c, s;
-        rotary::turn_of(int64_t(i / (D / 2)) * step, p.frequency[i % (D / 2)], c, s);
-        steps[i / (D / 2)][i % (D / 2)] = make_float2(c, s);
-      }
-      if (pairs) {
-#pragma unroll
-        for (int j = 0; j < V::N; ++j) {
-          rotary::turn_of(int64_t(pos0) + row0, p.frequency[pair_at(j)], first_c[j], first_s[j]);
-          first_c[j] *= p.gain, first_s[j] *= p.gain;
-        }
-      }
-      __syncthreads();
-    }
   for (int u = u0; u < u1; ++u) {
     const int buf = (u - u0) & 1, old = lo > 0 ? held_exponent(held) : E_MIN;
     if (u + 1 < u1) {
@@ -330,58 +288,13 @@ __global__ void __launch_bounds__(MOST_THREADS<D, T>) append_kernel(const __grid
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     // every thread reads only the pieces it copied
-    const uint4 *held_rows = pieces + buf * PASSES * threads + mine;
+    const uint4 *mine = pieces + buf * PASSES * threads + tid;
     float amax = 0.0f;
-    float turned[ROTATED ? ROWS : 1][2 * V::N];
-    const bool turn = ROTATED && u < H;
-    if constexpr (ROTATED) {
-      if (turn) {
-        if (MODE == ANY) __syncwarp();  // but for these, paired with any value of a row that their warp copied
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-          const int r = row0 + i * step;
-          if (r < lo || r >= hi) continue;
-          const uint4 *at = held_rows + i * step * LPR;
-          float(&y)[2 * V::N] = turned[i];
-          if constexpr (MODE == ANY) {
-            const int64_t pos = position_of(p, token0 + r, pos0 + r);
-            turn_apart<T>(p, reinterpret_cast<const T *>(at - col / V::N), col, pos, &y[0]);
-            turn_apart<T>(p, reinterpret_cast<const T *>(at - col / V::N), col2, pos, &y[V::N]);
-          } else {
-            V a, b;
-            a.load(at);
-            b.load(at + (col2 - col) / V::N);
-#pragma unroll
-            for (int j = 0; j < V::N; ++j) y[j] = a.at(j), y[V::N + j] = b.at(j);
-            if (pairs) {
-#pragma unroll
-              for (int j = 0; j < V::N; ++j) {
-                const int u = MODE == HALVES ? j : 2 * j, v = MODE == HALVES ? V::N + j : 2 * j + 1, pair = pair_at(j);
-                if (MODE == NEIGHBOURS && 2 * pair >= p.dims) continue;
-                const float2 by = steps[i][pair];
-                const float c = first_c[j] * by.x - first_s[j] * by.y, s = first_s[j] * by.x + first_c[j] * by.y;
-                const float x = y[u];
-                y[u] = x * c - y[v] * s;
-                y[v] = x * s + y[v] * c;
-              }
-            }
-          }
-          amax = max_finite(y, amax);
-        }
-        if (MODE == ANY) __syncwarp();  // before this buffer's next copies
-      }
-    }
-    if (!turn) {
-#pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        V v;
-        v.load(held_rows + i * step * LPR);
-        amax = max_finite(v, amax);
-        if constexpr (ROTATED) {
-          v.load(held_rows + i * step * LPR + (col2 - col) / V::N);
-          amax = max_finite(v, amax);
-        }
-      }
+    for (int i = 0; i < PASSES; ++i) {
+      V v;
+      v.load(mine + i * threads);
+      amax = max_finite(v, amax);
     }
     amax = warp_max(amax);
     if (lane == 0) part[buf][warp] = amax;
@@ -392,22 +305,207 @@ __global__ void __launch_bounds__(MOST_THREADS<D, T>) append_kernel(const __grid
     uint8_t *codes = p.codes + ((unit0 + u) << s.page_shift) * D;
     if (tid == 0) p.exps[unit0 + u] = int8_t(e);
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
+    for (int i = 0; i < PASSES; ++i) {
       const int r = row0 + i * step;
       if (r >= lo && r < hi) {
-        if constexpr (ROTATED)
-          if (turn) {
-            store_codes<V::N>(codes + r * D + col, &turned[i][0], e);
-            store_codes<V::N>(codes + r * D + col2, &turned[i][V::N], e);
-            continue;
-          }
         V v;
-        v.load(held_rows + i * step * LPR);
+        v.load(mine + i * threads);
         store_codes(codes + r * D + col, v, e);
-        if constexpr (ROTATED) {
-          v.load(held_rows + i * step * LPR + (col2 - col) / V::N);
-          store_codes(codes + r * D + col2, v, e);
+      }
+    }
+    if (lo > 0 && e > old) recode_rows<D>(codes, lo, old, e, tid, threads);
+  }
+}
+
+// How a page's keys are turned: the pairs of a piece in another whole piece, or
+// within it, at their places in the sequence; or in any other way.
+enum { HALVES, NEIGHBOURS, ANY };
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// append_kernel with keys turned on the way.  A thread's pieces of a row are two
+// that pair up (or, at the end of a row with fewer dims, two of those behind), of
+// half as many rows; it holds their values as f32 through the maximum.  Bound by
+// instructions as much as by memory: two values an instruction where there is one
+// for that, angles by steps, (side, head)s in turn so that blocks are alike.
+template <int D, typename T, int MODE, int ROWS, int MOST>
+__global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append_turned_kernel(const __grid_constant__ RotatedParams p) {
+  using V = Vec<T>;
+  using P = rotary::Piece<T, V::N>;
+  using rotary::mul2, rotary::fma2, rotary::two, rotary::apart;
+  constexpr int N = V::N, HALF = N / 2, LPR = D / N, LANES = LPR / 2;
+  extern __shared__ uint4 pieces[];  // [2] pages' rows
+  __shared__ float part[2][32];
+  __shared__ __align__(16) float steps_c[MODE == ANY ? 1 : ROWS][D / 2], steps_s[MODE == ANY ? 1 : ROWS][D / 2];
+  const Seqs &s = p.s;
+  grid_dependency_wait();
+  grid_dependency_done();
+  int b, start, n, len, page_of_seq;
+  if (!owner(s, blockIdx.x, b, start, n, len, page_of_seq)) return;
+  const int size = 1 << s.page_shift, first = len - n, H = s.kv_heads;
+  const int page = s.table[int64_t(b) * s.width + page_of_seq];
+  const int pos0 = page_of_seq << s.page_shift;
+  const int lo = max(first - pos0, 0), hi = min(len - pos0, size);  // new rows of the page
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
+  int col = lane % LANES * N, col2 = col + D / 2;
+  bool pairs = true;  // the pieces are turned
+  if constexpr (MODE == HALVES) {
+    const int half = p.dims / 2, behind = lane % LANES - half / N;
+    pairs = behind < 0;
+    if (!pairs) col = p.dims + behind * N;
+    col2 = pairs ? col + half : col + (D - p.dims) / 2;
+  }
+  const int row0 = warp * (32 / LANES) + lane / LANES, step = warps * (32 / LANES), away = col2 - col;
+  const int64_t token0 = int64_t(start) + pos0 - first;  // row 0 of the page, were it new
+  const int mine = row0 * LPR + col / N, page_pieces = LPR << s.page_shift;
+  const auto fetch = [&](int u, int buf) {
+    const int side = u & 1, head = u >> 1;
+    const int64_t ts = side ? p.ts[1] : p.ts[0];
+    const T *x = static_cast<const T *>(side ? p.x[1] : p.x[0]) + head * (side ? p.hs[1] : p.hs[0]) + col;
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(pieces + buf * page_pieces + mine));
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = row0 + i * step;
+      const bool real = r >= lo && r < hi;
+      const T *from = x + (token0 + (real ? r : lo)) * ts;
+      copy16(to + i * step * (D * int(sizeof(T))), from, real);
+      copy16(to + (i * step * D + away) * int(sizeof(T)), from + away, real);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int u0 = blockIdx.y * p.units, u1 = min(u0 + p.units, 2 * H);
+  fetch(u0, 0);
+  const bool bad = page < 0 || page >= s.pages;
+  if (bad && tid == 0) report(s.status, STATUS_PAGE);
+  const int64_t unit0 = int64_t(bad ? 0 : page) * 2 * H;
+  const auto unit_of = [&](int u) { return unit0 + (u & 1 ? H : 0) + (u >> 1); };
+  int held = lo > 0 ? p.exps[unit_of(u0)] : 0;
+  // angles of keys: of row row0, and of i * step rows
+  uint64_t first_c[HALF], first_s[HALF];
+  const auto pair_at = [&](int j) { return MODE == HALVES ? col + j : (j < HALF ? col : col2 - N) / 2 + j; };
+  if constexpr (MODE != ANY) {
+    for (int i = tid; i < ROWS * (D / 2); i += threads) {
+      const int row = i / (D / 2), pair = i % (D / 2);
+      rotary::turn_of(int64_t(row) * step, p.frequency[pair], steps_c[row][pair], steps_s[row][pair]);
+    }
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      float c[2], s[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) rotary::turn<false>(pos0 + row0, p.frequency[min(pair_at(j + i), D / 2 - 1)], p.gain, c[i], s[i]);
+      first_c[j / 2] = two(c[0], c[1]);
+      first_s[j / 2] = two(s[0], s[1]);
+    }
+    __syncthreads();
+  }
+  for (int u = u0; u < u1; ++u) {
+    const int buf = (u - u0) & 1, old = lo > 0 ? held_exponent(held) : E_MIN;
+    if (u + 1 < u1) {
+      fetch(u + 1, buf ^ 1);
+      held = lo > 0 ? p.exps[unit_of(u + 1)] : 0;
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    // every thread reads only the pieces it copied
+    const uint4 *rows = pieces + buf * page_pieces + mine;
+    const bool turn = (u & 1) == 0;
+    uint64_t x[ROWS][HALF], y[ROWS][HALF];
+    float amax = 0.0f;
+    if (MODE == ANY && turn) __syncwarp();  // but for these, paired with any value of a row that their warp copied
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = row0 + i * step;
+      if (r < lo || r >= hi) continue;
+      const uint4 *at = rows + i * step * LPR;
+      if (MODE == ANY && turn) {
+        float v[2 * N];
+        const T *row = reinterpret_cast<const T *>(at - col / N);
+        const int64_t pos = position_of(p, token0 + r, pos0 + r);
+        turn_apart<false>(p, row, col, pos, &v[0]);
+        turn_apart<false>(p, row, col2, pos, &v[N]);
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) x[i][j] = two(v[2 * j], v[2 * j + 1]), y[i][j] = two(v[N + 2 * j], v[N + 2 * j + 1]);
+      } else {
+        rotary::spread<T, N>(*reinterpret_cast<const P *>(at), x[i]);
+        rotary::spread<T, N>(*reinterpret_cast<const P *>(at + away / N), y[i]);
+      }
+      if (MODE == HALVES && turn && pairs) {
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) {
+          const float2 bc = *reinterpret_cast<const float2 *>(&steps_c[i][col + 2 * j]);
+          const float2 bs = *reinterpret_cast<const float2 *>(&steps_s[i][col + 2 * j]);
+          const uint64_t c2 = two(bc.x, bc.y), s2 = two(bs.x, bs.y);
+          const uint64_t c = fma2(first_c[j], c2, mul2(first_s[j], s2 ^ rotary::SIGNS));
+          const uint64_t s = fma2(first_s[j], c2, mul2(first_c[j], s2));
+          rotary::turn2(x[i][j], y[i][j], c, s, s ^ rotary::SIGNS);
         }
+      }
+      if (MODE == NEIGHBOURS && turn) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const int pair = pair_at(j);
+          if (2 * pair >= p.dims) continue;
+          const float2 fc = apart(first_c[j / 2]), fs = apart(first_s[j / 2]);
+          const float c0 = j & 1 ? fc.y : fc.x, s0 = j & 1 ? fs.y : fs.x, bc = steps_c[i][pair], bs = steps_s[i][pair];
+          const float c = c0 * bc - s0 * bs, s = s0 * bc + c0 * bs;
+          uint64_t &w = j < HALF ? x[i][j] : y[i][j - HALF];
+          const float2 f = apart(w);
+          w = two(f.x * c - f.y * s, f.x * s + f.y * c);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < HALF; ++j) {
+        const float2 f = apart(x[i][j]), g = apart(y[i][j]);
+        amax = max3(amax, fabsf(f.x), fabsf(f.y));
+        amax = max3(amax, fabsf(g.x), fabsf(g.y));
+      }
+    }
+    if (MODE == ANY && turn) __syncwarp();  // before this buffer's next copies
+    if (amax == INFINITY) {  // (rare) the largest finite one
+      amax = 0.0f;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (row0 + i * step >= lo && row0 + i * step < hi)
+#pragma unroll
+          for (int j = 0; j < HALF; ++j) {
+            const float2 f = apart(x[i][j]), g = apart(y[i][j]);
+            const float v[4] = {f.x, f.y, g.x, g.y};
+            amax = max_finite(v, amax);
+          }
+    }
+    amax = warp_max(amax);
+    if (lane == 0) part[buf][warp] = amax;
+    __syncthreads();
+    amax = warp_max(lane < warps ? part[buf][lane] : 0.0f);
+    if (bad) continue;
+    const int e = fit_exponent(amax, old);
+    const int64_t unit = unit_of(u);
+    uint8_t *codes = p.codes + (unit << s.page_shift) * D;
+    if (tid == 0) p.exps[unit] = int8_t(e);
+    const uint64_t by = two(pow2(-e), pow2(-e));
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = row0 + i * step;
+      if (r < lo || r >= hi) continue;
+      uint32_t w[2][2] = {};
+#pragma unroll
+      for (int j = 0; j < HALF; ++j) {
+        const float2 f = apart(mul2(x[i][j], by)), g = apart(mul2(y[i][j], by));
+        w[0][j / 2] |= f32x2_e4m3x2(f.y, f.x) << (16 * (j & 1));
+        w[1][j / 2] |= f32x2_e4m3x2(g.y, g.x) << (16 * (j & 1));
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint8_t *at = codes + r * D + (k == 0 ? col : col2);
+        if constexpr (N == 8)
+          *reinterpret_cast<uint2 *>(at) = make_uint2(w[k][0], w[k][1]);
+        else
+          *reinterpret_cast<uint32_t *>(at) = w[k][0];
       }
     }
     if (lo > 0 && e > old) recode_rows<D>(codes, lo, old, e, tid, threads);
@@ -453,7 +551,11 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
       if (lane < LPR) row[lane] = v.w;
       __syncwarp();
       if (lane < LPR) {
-        turn_apart(p, reinterpret_cast<const T *>(row), lane * V::N, position_of(p, start, len - 1), turned);
+        const int64_t pos = position_of(p, start, len - 1);
+        if (query && p.out_type == EMMY_KV8_F32)
+          turn_apart<true>(p, reinterpret_cast<const T *>(row), lane * V::N, pos, turned);
+        else
+          turn_apart<false>(p, reinterpret_cast<const T *>(row), lane * V::N, pos, turned);
       }
       if (query) {
         if (lane < LPR) store_query(p, start, unit_of_seq - 2 * s.kv_heads, lane * V::N, turned);
@@ -475,7 +577,7 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
   if (lane < LPR) {
     uint8_t *at = codes + int64_t(lo) * D + lane * V::N;
     if (turn)
-      store_codes<V::N>(at, turned, e);
+      store_codes(at, turned, e);
     else
       store_codes(at, v, e);
   }
@@ -496,19 +598,26 @@ int launch(Params p, bool one, int64_t slots, int device, cudaStream_t stream) {
   int smem = 2 * 8 * 16 * threads;
   constexpr int ROOM = 200 * 1024;
   if (smem > ROOM) smem /= 2, p.units = 1;  // no second buffer, so no second unit (f32 pages of 128 KB)
-  const auto run = [&](auto kernel, KernelSetup &setup) {
-    const int rc = setup.ready("emmy_kv8_append", kernel, device, std::min(ROOM, 2 * 8 * 16 * MOST_THREADS<D, T>));
+  constexpr int MOST = MOST_THREADS<D, T>;
+  const auto run = [&](auto kernel, KernelSetup &setup, int by) {
+    const int rc = setup.ready("emmy_kv8_append", kernel, device, std::min(ROOM, 2 * 8 * 16 * MOST));
     if (rc != EMMY_OK) return rc;
-    return launch_kernel("emmy_kv8_append", kernel, dim3(unsigned(slots), (units + p.units - 1) / p.units), threads, smem,
+    return launch_kernel("emmy_kv8_append", kernel, dim3(unsigned(slots), (units + p.units - 1) / p.units), by * threads, smem,
                          stream, p);
   };
-  static KernelSetup setup[4];
+  static KernelSetup setup[10];
   if constexpr (std::is_same<Params, RotatedParams>::value) {
-    if (p.positions == nullptr && p.interleaved) return run(append_kernel<D, T, NEIGHBOURS, Params>, setup[NEIGHBOURS]);
-    if (p.positions == nullptr && p.dims / 2 % Vec<T>::N == 0) return run(append_kernel<D, T, HALVES, Params>, setup[HALVES]);
-    return run(append_kernel<D, T, ANY, Params>, setup[ANY]);
+    const auto pick = [&](auto mode, KernelSetup *of) {
+      constexpr int M = decltype(mode)::value;
+      if (2 * threads <= 256) return run(append_turned_kernel<D, T, M, 2, 256>, of[0], 2);
+      if (2 * threads <= 512) return run(append_turned_kernel<D, T, M, 2, 512>, of[1], 2);
+      return run(append_turned_kernel<D, T, M, 4, MOST>, of[2], 1);
+    };
+    if (p.positions == nullptr && p.interleaved) return pick(std::integral_constant<int, NEIGHBOURS>(), setup);
+    if (p.positions == nullptr && p.dims / 2 % Vec<T>::N == 0) return pick(std::integral_constant<int, HALVES>(), setup + 3);
+    return pick(std::integral_constant<int, ANY>(), setup + 6);
   } else {
-    return run(append_kernel<D, T, PLAIN, Params>, setup[PLAIN]);
+    return run(append_kernel<D, T>, setup[9], 1);
   }
 }
 

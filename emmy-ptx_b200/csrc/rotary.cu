@@ -8,9 +8,8 @@
 //
 // Bound by memory: each value is read and written once.  A thread holds one piece
 // (16 bytes, or less where sizes or addresses ask for it) of a token's row, with
-// the piece that it is paired with, and does the same of HEADS heads: the angles
-// cost about 40 instructions each and are computed once for all of them, while the
-// values are on their way.
+// the piece that it is paired with, and does the same of HEADS heads: their angles
+// are computed once, while the values are on their way.
 #include "rotary.cuh"
 
 namespace rotary {
@@ -71,9 +70,8 @@ __global__ void __launch_bounds__(THREADS) rotate_kernel(const __grid_constant__
     if (turned) {
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        turn_of(pos, p.frequency[piece * PAIRS + i], c[i], s[i]);
-        c[i] *= p.gain;
-        s[i] *= p.gain * p.sign;
+        turn<sizeof(U) == 4>(pos, p.frequency[piece * PAIRS + i], p.gain, c[i], s[i]);
+        s[i] *= p.sign;
       }
     }
 #pragma unroll

@@ -31,6 +31,53 @@ __device__ __forceinline__ void turn_of(int64_t position, uint64_t frequency, fl
   if (quarter & 2) s = -s;
 }
 
+// The same to 2^-20.6: the angle rounded to f32 (2^-22.3) and the special function
+// unit (at most 2^-21.2, as CUDA documents __cosf and __sinf there), 10 instructions
+// for 45.  For results of 16 bits, which round by 2^-12 or more, and of 8.
+__device__ __forceinline__ void turn_near(int64_t position, uint64_t frequency, float &c, float &s) {
+  const uint32_t t = static_cast<uint32_t>((static_cast<uint64_t>(position) * frequency) >> 32);
+  const float x = static_cast<float>(static_cast<int32_t>(t)) * 1.4629180792671596e-9f;
+  c = __cosf(x);
+  s = __sinf(x);
+}
+template <bool EXACT>
+__device__ __forceinline__ void turn(int64_t position, uint64_t frequency, float gain, float &c, float &s) {
+  if constexpr (EXACT)
+    turn_of(position, frequency, c, s);
+  else
+    turn_near(position, frequency, c, s);
+  c *= gain, s *= gain;
+}
+
+// Two f32 in one register pair, and products of those: one instruction for two.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 apart(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+constexpr uint64_t SIGNS = 0x8000000080000000ull;
+// (x, y) -> (x c - y s, x s + y c), two pairs at once; ns = -s.
+__device__ __forceinline__ void turn2(uint64_t &x, uint64_t &y, uint64_t c, uint64_t s, uint64_t ns) {
+  const uint64_t a = fma2(x, c, mul2(y, ns));
+  y = fma2(x, s, mul2(y, c));
+  x = a;
+}
+
 // Rows to turn: those of a call by themselves, or a cache's new tokens.
 struct Params {
   uint64_t frequency[EMMY_ROTARY_PAIRS];
@@ -90,26 +137,51 @@ __device__ __forceinline__ uint32_t packed(float lo, float hi) {
   }
 }
 
-// (a, b) turned into (u, v), of pieces a and b whose values pair up (half layout), or of one
-// piece a of neighbours; c, s of each pair.
+// Piece a's values, two to a register pair, and back with one rounding each.
+template <typename T, int N>
+__device__ __forceinline__ void spread(const Piece<T, N> &a, uint64_t (&x)[N / 2]) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      const float2 f = unpacked<T>(reinterpret_cast<const uint32_t *>(&a)[i]);
+      x[i] = two(f.x, f.y);
+    } else {
+      x[i] = two(a.v[2 * i], a.v[2 * i + 1]);
+    }
+  }
+}
+template <typename U, int N>
+__device__ __forceinline__ void gathered(const uint64_t (&x)[N / 2], Piece<U, N> &u) {
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    const float2 f = apart(x[i]);
+    if constexpr (sizeof(U) == 2)
+      reinterpret_cast<uint32_t *>(&u)[i] = packed<U>(f.x, f.y);
+    else
+      u.v[2 * i] = f.x, u.v[2 * i + 1] = f.y;
+  }
+}
+
+// (a, b) turned into (u, v), of pieces a and b whose values pair up (half layout),
+// or of one piece a of neighbours; c, s of each pair.
 template <typename T, typename U, int N>
 __device__ __forceinline__ void turn_pieces(const Piece<T, N> &a, const Piece<T, N> &b, const float (&c)[N], const float (&s)[N],
                                             Piece<U, N> &u, Piece<U, N> &v) {
-  if constexpr (sizeof(T) == 2 && std::is_same<T, U>::value && N >= 2) {
-    const uint32_t *x = reinterpret_cast<const uint32_t *>(&a), *y = reinterpret_cast<const uint32_t *>(&b);
+  if constexpr (N >= 2) {
+    uint64_t x[N / 2], y[N / 2];
+    spread<T, N>(a, x);
+    spread<T, N>(b, y);
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-      const float2 p = unpacked<T>(x[i]), q = unpacked<T>(y[i]);
-      reinterpret_cast<uint32_t *>(&u)[i] = packed<T>(p.x * c[2 * i] - q.x * s[2 * i], p.y * c[2 * i + 1] - q.y * s[2 * i + 1]);
-      reinterpret_cast<uint32_t *>(&v)[i] = packed<T>(p.x * s[2 * i] + q.x * c[2 * i], p.y * s[2 * i + 1] + q.y * c[2 * i + 1]);
+      const uint64_t s2 = two(s[2 * i], s[2 * i + 1]);
+      turn2(x[i], y[i], two(c[2 * i], c[2 * i + 1]), s2, s2 ^ SIGNS);
     }
+    gathered<U, N>(x, u);
+    gathered<U, N>(y, v);
   } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float x = to_float(a.v[i]), y = to_float(b.v[i]);
-      u.v[i] = rounded<U>(x * c[i] - y * s[i]);
-      v.v[i] = rounded<U>(x * s[i] + y * c[i]);
-    }
+    const float x = to_float(a.v[0]), y = to_float(b.v[0]);
+    u.v[0] = rounded<U>(x * c[0] - y * s[0]);
+    v.v[0] = rounded<U>(x * s[0] + y * c[0]);
   }
 }
 template <typename T, typename U, int N>

@@ -48,7 +48,7 @@ def test_rotate(gpu, shape, interleaved, dtype):  # noqa: F811
             call = rot.backward if backward else rot.rotate
             assert call(xd, positions, view) is view
             got = gpu.get(od, (T + 2, H, D), NP[dtype])
-            want, bound = ref.rotate(rot, x, pos, backward)
+            want, bound = ref.rotate(rot, x, pos, backward, ref.kind(dtype))
             assert ref.close(got[:T], want, bound, dtype)
             assert (got[T:].astype(np.float32) == 77).all()
             if D > r:
@@ -57,7 +57,7 @@ def test_rotate(gpu, shape, interleaved, dtype):  # noqa: F811
     call(xd, positions, xd)
     assert gpu.get(xd, x.shape, NP[dtype]).tobytes() == got[:T].tobytes()
     rot.rotate(gpu.put(x, dtype), 12345, view)
-    want, bound = ref.rotate(rot, x, 12345 + np.arange(T))
+    want, bound = ref.rotate(rot, x, 12345 + np.arange(T), to=ref.kind(dtype))
     assert ref.close(gpu.get(view, x.shape, NP[dtype]), want, bound, dtype)
 
 
@@ -85,7 +85,7 @@ def test_strides(gpu, layout, interleaved, dims, dtype):  # noqa: F811
     rot.rotate(DeviceArray(xd.ptr + xo * size, dtype, (6, 3, 32), (*xs, 1)), gpu.put(pos, "i64"), out)
     got = gpu.get(od, back.shape, NP[dtype])
     at = lambda o, s: o + np.arange(6)[:, None, None] * s[0] + np.arange(3)[None, :, None] * s[1] + np.arange(32)  # noqa: E731
-    want, bound = ref.rotate(rot, flat[at(xo, xs)], pos)
+    want, bound = ref.rotate(rot, flat[at(xo, xs)], pos, to=ref.kind(dtype))
     assert ref.close(got[at(oo, os_)], want, bound, dtype)
     rest = np.ones(4000, bool)
     rest[at(oo, os_)] = False
@@ -103,7 +103,7 @@ def test_slices_of_one_array(gpu):  # noqa: F811
     rot.rotate(q, 5, q)
     rot.rotate(k, 5, k)
     got = gpu.get(d, x.shape, np.float16)
-    want, bound = ref.rotate(rot, x, 5 + np.arange(9))
+    want, bound = ref.rotate(rot, x, 5 + np.arange(9), to="16")
     assert ref.close(got[:, :6], want[:, :6], bound[:, :6], "f16")
     assert got[:, 6:].tobytes() == x[:, 6:].tobytes()
     # and into a slice behind its own
@@ -111,7 +111,7 @@ def test_slices_of_one_array(gpu):  # noqa: F811
     before = got
     rot.backward(k, 5, out)
     got = gpu.get(d, x.shape, np.float16)
-    want, bound = ref.rotate(rot, before[:, 4:6], 5 + np.arange(9), True)
+    want, bound = ref.rotate(rot, before[:, 4:6], 5 + np.arange(9), True, "16")
     assert ref.close(got[:, 6:], want, bound, "f16") and got[:, :6].tobytes() == before[:, :6].tobytes()
 
 
@@ -185,7 +185,7 @@ def test_graph_streams_and_threads(gpu):  # noqa: F811
     host = x.float().cpu().numpy().astype(NP["bf16"])
 
     def check(at):
-        want, bound = ref.rotate(rot, host, at)
+        want, bound = ref.rotate(rot, host, at, to="16")
         assert ref.close(out.float().cpu().numpy().astype(NP["bf16"]), want, bound, "bf16")
     rot.rotate(x, pos, out, stream=side)
     side.synchronize()
@@ -244,7 +244,7 @@ def append_gpu(gpu, case, rot, rng, positions=None, garbage=None):  # noqa: F811
     batch.append(0, gpu.put(k, dtype), gpu.put(v, dtype), rotary=rot, q=gpu.put(q, dtype), q_out=out, positions=pd)
     batch.check_errors()
     got_c, got_e = gpu.get(c, codes.shape, np.uint8), gpu.get(e, exps.shape, np.int8)
-    turned, bound = ref.rotate(rot, k.astype(np.float64), place)
+    turned, bound = ref.rotate(rot, k.astype(np.float64), place, to="8")
     want_c, want_e = kv8.append(codes, exps, table, kv, ql, turned, v.astype(np.float64))
     assert (got_e == want_e).all()
     assert (got_c[:, 1] == want_c[:, 1]).all()          # values are not turned
@@ -270,7 +270,7 @@ def append_gpu(gpu, case, rot, rng, positions=None, garbage=None):  # noqa: F811
             old[table[b][i // P], 0, :, i % P] = True
     assert (got_c[~old] == want_c[~old]).all()
     got_q = gpu.get(out, q.shape, NP[out_dtype])
-    want, bound = ref.rotate(rot, q[:T].astype(np.float64), place)
+    want, bound = ref.rotate(rot, q[:T].astype(np.float64), place, to=ref.kind(out_dtype))
     fine = np.isfinite(want)
     assert ref.close(np.where(fine, got_q[:T], 0), np.where(fine, want, 0), np.where(fine, bound, 0), out_dtype)
     assert (np.isnan(got_q[:T]) == np.isnan(want)).all()
@@ -336,7 +336,7 @@ def test_append_in_place_of_one_array(gpu):  # noqa: F811
         got = gpu.get(d, x.shape, NP["bf16"])
         assert got[:, 4:].tobytes() == x[:, 4:].tobytes()
         if with_q:
-            want, bound = ref.rotate(rot, x[:, :4], 5 + np.arange(70))
+            want, bound = ref.rotate(rot, x[:, :4], 5 + np.arange(70), to="16")
             assert ref.close(got[:, :4], want, bound, "bf16")
         results.append(gpu.get(c, codes.shape, np.uint8).tobytes())
         from ptxgen.runtime import EmmyError
@@ -369,7 +369,7 @@ def test_append_bad_page(gpu):  # noqa: F811
         batch.append(0, gpu.put(k, "bf16"), gpu.put(k, "bf16"), rotary=rot, q=gpu.put(q, "bf16"), q_out=out)
         with pytest.raises(EmmyError, match="outside the pool"):
             batch.check_errors()
-        want, bound = ref.rotate(rot, q, np.tile(np.arange(5 - m, 5), 2))
+        want, bound = ref.rotate(rot, q, np.tile(np.arange(5 - m, 5), 2), to="16")
         assert ref.close(gpu.get(out, q.shape, NP["bf16"]), want, bound, "bf16")
         assert (gpu.get(c, codes.shape, np.uint8)[1:] == codes[1:]).all()
         batch.close()

@@ -292,7 +292,7 @@ def test_forks_generate_together(gpu):  # noqa: F811
             batch.append(layer, x[:, H * G:H * G + H], x[:, H * G + H:], stream=st, rotary=rot, q=x[:, :H * G], q_out=q)
             batch.attend(layer, q, out, stream=st)
             batch.check_errors(stream=st)
-            want_q, bq = rotary_oracle.rotate(rot, x[:, :H * G].double().cpu().numpy(), place)
+            want_q, bq = rotary_oracle.rotate(rot, x[:, :H * G].double().cpu().numpy(), place, to="16")
             assert rotary_oracle.close(q.double().cpu().numpy(), want_q, bq, "bf16")
             want, bound = ref.attend(codes[layer].cpu().numpy(), exps[layer].cpu().numpy(), seqs.table(ids).tolist(),
                                      [seqs.length(s) for s in ids], counts, q.double().cpu().numpy(), D ** -0.5)
