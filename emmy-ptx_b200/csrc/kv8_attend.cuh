@@ -30,13 +30,17 @@ struct alignas(16) JoinRec {
 };
 
 // What a sequence's keys that it shares with its run came to: results of some
-// parts of the run's query rows, block after block of p.prefix_rows rows.
+// parts of the run's query rows, block after block of p.pre_rows rows; a result is
+// O [pre_rows][head_dim], then maxima, then sums.
 struct alignas(16) PrefixRec {
   int chunks;        // 64-key chunks that are shared, 0: none
   int slot0, parts;  // workspace slots of block 0 of kv head 0, one a part
   int blocks, row;   // of the run's rows of a kv head; the sequence's first row among them
   int pad[3];
 };
+
+// Parts of a block at most: those that the row kernel joins at once.
+constexpr int MOST_SHARED = 160;
 
 // Which kernel, if any, attends to shared keys first.
 enum { SHARED_NONE = 0, SHARED_ROWS, SHARED_TILES };

@@ -292,10 +292,28 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
     mine += pre_chunks[i] * pre_blocks[i];
   }
   block_scan(mine, all, sums);
-  int limit = 1 << 24;  // chunks of a part
+  // Chunks of a part: as many as leave one wave of parts, if any of some tries do,
+  // and so many that a block has no more parts than are joined at once.
+  __shared__ int longest;
+  if (tid == 0) longest = 1;
+  __syncthreads();
+  for (int i = 0; i < EACH; ++i)
+    if (pre_chunks[i] > 0) atomicMax(&longest, pre_chunks[i]);
+  __syncthreads();
+  const int least = (longest + MOST_SHARED - 1) / MOST_SHARED;
+  int limit = max(longest, least);
   if (p.pre_target > 0) {
     const int64_t share = (int64_t(all) * H + p.pre_target - 1) / p.pre_target;
-    limit = int(min(max(share, int64_t(p.a.shared == SHARED_TILES ? TILE_CUT : 2)), int64_t(1) << 24));
+    const int l0 = max(int(min(share, int64_t(1) << 24)), max(least, p.a.shared == SHARED_TILES ? TILE_CUT : 2));
+    limit = l0;
+    for (int t = 1; t <= 16; ++t) {
+      int parts = 0, total;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) parts += pre_blocks[i] * ((pre_chunks[i] + limit - 1) / limit);
+      block_scan(parts, total, sums);
+      if (int64_t(total) * H <= p.pre_target) break;
+      limit = l0 + (l0 * t + 15) / 16;
+    }
   }
   int pre = 0;
 #pragma unroll

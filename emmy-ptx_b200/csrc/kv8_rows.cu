@@ -96,6 +96,7 @@ struct Layout {
   static constexpr int LD = D + 4;        // floats of a row of the join
   static_assert((WARPS * LD + D) * 8 * NT * 4 <= QUERIES, "the join and a cluster's part fit over the ring");
   static_assert(2 * 64 * 8 * NT * 4 <= QUERIES, "so do the maxima and sums of 64 parts");
+  static_assert((WARPS * LD + D + 2 * MOST_SHARED) * 8 * NT * 4 <= QUERIES, "and those of the shared keys' parts beside the rows");
 };
 
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, int row, uint64_t *bar) {
@@ -304,33 +305,6 @@ __device__ __forceinline__ int query_row(uint32_t (&f)[D / 8], const T *row, int
 // A call's only kernel of its kind; the first of two, which leaves results for
 // shared keys in the workspace; or the second, which takes them in.
 enum { ALONE = 0, FIRST, SECOND };
-
-// Results for the shared keys of row r's sequence join x, values d .. d + N - 1 of
-// the row, and its maximum and sum, in the parts' order.
-template <int D, int N>
-__device__ __forceinline__ void take_shared(const AttendParams &p, const PrefixRec &f, int head, int row, int d, float (&x)[N],
-                                            float &m, float &l) {
-  if (f.chunks == 0) return;
-  const int at = f.row + row, block = at / p.pre_rows, r = at - block * p.pre_rows;
-  const int64_t size = int64_t(p.pre_rows) * (D + 2);
-  const float *part = p.pre_partial + (f.slot0 + (int64_t(head) * f.blocks + block) * f.parts) * size;
-  // the tile kernel's results lie column by column
-  const bool columns = p.shared == SHARED_TILES;
-  const int64_t rs = columns ? 1 : D, ds = columns ? p.pre_rows : 1;
-  float top = m;
-  for (int i = 0; i < f.parts; ++i) top = fmaxf(top, __ldcg(part + i * size + p.pre_rows * D + r));
-  const float own = exp2_fast(m - top);
-  l *= own;
-#pragma unroll
-  for (int j = 0; j < N; ++j) x[j] *= own;
-  for (int i = 0; i < f.parts; ++i, part += size) {
-    const float w = exp2_fast(__ldcg(part + p.pre_rows * D + r) - top);
-    l += w * __ldcg(part + p.pre_rows * (D + 1) + r);
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] += w * __ldcg(part + r * rs + (d + j) * ds);
-  }
-  m = top;
-}
 
 // Shared memory: first the joined rows of the four warps, over the staged queries.
 template <int D, int NT, bool CLUSTER, int MODE, typename T>
@@ -591,6 +565,8 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
   };
   const auto part_slot = [&](int c) { return p.partial + int64_t(g.slot0 + c) * ROWS * (D + 2); };
   // a cluster's parts stay in shared memory, behind what is joined here
+  // (so do the sequence's own, until those for its shared keys join them)
+  float *const held = join + WARPS * ROWS * LD, *const shared_m = held + ROWS * D, *const shared_l = shared_m + MOST_SHARED * ROWS;
   float *const slot = CLUSTER         ? join + WARPS * ROWS * LD
                       : MODE == FIRST ? p.pre_partial + int64_t(g.slot0 + g.part) * ROWS * (D + 2)
                                       : part_slot(g.part);
@@ -611,16 +587,85 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
         x[2 * j] += f * u.x, x[2 * j + 1] += f * u.y;
       }
     }
-    if (!whole && d == 0) row_m[r] = m, row_l[r] = l;
-    if (whole) {
-      if constexpr (MODE == SECOND) take_shared<D>(p, shared, g.head, g.row0 + r, d, x, m, l);
+    if ((!whole || MODE == SECOND) && d == 0) row_m[r] = m, row_l[r] = l;
+    if (whole && MODE != SECOND) {
       store(r, d, x, l);
     } else {
-      *reinterpret_cast<float4 *>(slot + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-      *reinterpret_cast<float4 *>(slot + r * D + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
+      float *const to = whole ? held : slot;
+      *reinterpret_cast<float4 *>(to + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4 *>(to + r * D + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
     }
   }
-  if (whole) return;
+  // The rows in `held`, with maxima and sums in row_m and row_l, and the results for
+  // their shared keys as one, in the parts' order, into the output.
+  const auto finish = [&]() {
+    const int64_t size = int64_t(p.pre_rows) * (D + 2);
+    const auto part_of = [&](int r, int &row) {  // of row r, part 0
+      const int at = shared.row + g.row0 + r, block = at / p.pre_rows;
+      row = at - block * p.pre_rows;
+      return p.pre_partial + (shared.slot0 + (int64_t(g.head) * shared.blocks + block) * shared.parts) * size;
+    };
+    const int parts = shared.chunks > 0 ? min(shared.parts, MOST_SHARED) : 0;
+    for (int i = tid; i < parts * rows; i += THREADS) {
+      const int part = i / rows, r = i - part * rows;
+      int row;
+      const float *at = part_of(r, row);
+      at += part * size + p.pre_rows * D + row;
+      shared_m[part * ROWS + r] = __ldcg(at);
+      shared_l[part * ROWS + r] = __ldcg(at + p.pre_rows);
+    }
+    __syncthreads();
+    for (int r = warp; r < rows; r += ALL_WARPS) {
+      const float own = row_m[r];
+      float m = own;
+      for (int i = lane; i < parts; i += 32) m = fmaxf(m, shared_m[i * ROWS + r]);
+      for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      float l = 0.0f;
+      for (int i = lane; i < parts; i += 32) {
+        const float f = exp2_fast(shared_m[i * ROWS + r] - m);
+        l += f * shared_l[i * ROWS + r];
+        shared_m[i * ROWS + r] = f;
+      }
+      for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      if (lane == 0) {
+        const float f = exp2_fast(own - m);
+        row_l[r] = f * row_l[r] + l;
+        row_m[r] = f;
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * (D / 4); i += THREADS) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      int row;
+      const float *at = part_of(r, row);
+      at += row * D + d;
+      const float4 own = *reinterpret_cast<const float4 *>(held + r * D + d);
+      const float f0 = row_m[r];
+      float4 x = make_float4(f0 * own.x, f0 * own.y, f0 * own.z, f0 * own.w);
+      for (int c0 = 0; c0 < parts; c0 += 16) {  // sixteen loads in flight
+        float4 u[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          if (c0 + c < parts) u[c] = __ldcg(reinterpret_cast<const float4 *>(at + (c0 + c) * size));
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          if (c0 + c < parts) {
+            const float f = shared_m[(c0 + c) * ROWS + r];
+            x.x += f * u[c].x, x.y += f * u[c].y, x.z += f * u[c].z, x.w += f * u[c].w;
+          }
+      }
+      const float by = row_l[r] == 0.0f ? 0.0f : 1.0f / row_l[r];
+      *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) =
+          make_uint2(pack2<T>(x.x * by, x.y * by), pack2<T>(x.z * by, x.w * by));
+    }
+  };
+  if (whole) {
+    if constexpr (MODE == SECOND) {
+      __syncthreads();
+      finish();
+    }
+    return;
+  }
   // results of the segment that go through the workspace, and which is this
   const int results = CLUSTER ? g.parts / p.cluster : g.parts, result = CLUSTER ? g.part / p.cluster : g.part;
   if constexpr (CLUSTER) {
@@ -732,13 +777,11 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
           }
       }
       if (last) {
-        float l = row_l[r];
         if constexpr (MODE == SECOND) {
-          float m = row_m[r], v[4] = {x.x, x.y, x.z, x.w};
-          take_shared<D>(p, shared, g.head, g.row0 + r, d, v, m, l);
-          x = make_float4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<float4 *>(held + r * D + d) = x;
+          continue;
         }
-        const float by = l == 0.0f ? 0.0f : 1.0f / l;
+        const float by = row_l[r] == 0.0f ? 0.0f : 1.0f / row_l[r];
         *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) =
             make_uint2(pack2<T>(x.x * by, x.y * by), pack2<T>(x.z * by, x.w * by));
       } else {  // only this thread reads or writes these values of part a now
@@ -756,8 +799,14 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
   const int groups = (results + group - 1) / group;
   if (!last_of(lead, 0, count)) return;
   gather(lead, count, 1, groups == 1);
-  if (groups == 1 || !last_of(0, 1, groups)) return;
-  gather(0, groups, group, true);
+  if (groups > 1) {
+    if (!last_of(0, 1, groups)) return;
+    gather(0, groups, group, true);
+  }
+  if constexpr (MODE == SECOND) {
+    __syncthreads();
+    finish();
+  }
 }
 
 // Beside the tile kernel, which was launched before it and whose sequences are

@@ -248,7 +248,8 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_
                : "memory");
 }
 
-template <int D, typename T>
+// SHARED: the units are runs' rows over shared keys, and every one leaves a result.
+template <int D, typename T, bool SHARED>
 __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p) {
   using L = Layout<D>;
   extern __shared__ uint8_t dyn_raw[];
@@ -783,8 +784,12 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         for (int i = 0; i < 4; ++i)
           out[i] = static_cast<T *>(p.out) +
                    (L::WRITE4 ? __shfl_sync(0xffffffffu, to, (lane & ~3) | i) + 8 * (lane & 3) : to + 8 * i);
-        const float by = slot >= 0 ? pow2(unit) : l == 0.0f ? 0.0f : pow2(unit) / l;
+        const float by = SHARED || slot >= 0 ? pow2(unit) : l == 0.0f ? 0.0f : pow2(unit) / l;
         float *const part = p.tile_partial + int64_t(slot) * (D + 2) * (2 * TILE) + x * TILE + r;
+        float *rows[4];  // SHARED: this lane's pieces of four lanes' rows
+        if constexpr (SHARED)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rows[i] = p.pre_partial + int64_t(slot) * (D + 2) * (2 * TILE) + (x * TILE + (r & ~3) + i) * D + 4 * (lane & 3);
         const uint32_t *bits = reinterpret_cast<const uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8));
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
@@ -796,7 +801,18 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (nan >> i & 1) o[i] = 0x7fc00000u;
-          if (slot >= 0) {
+          if constexpr (SHARED) {
+            // O, row after row, four lanes 64 bytes of one together
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+              uint4 w[4];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) (&w[i / 4].x)[i % 4] = __float_as_uint(__uint_as_float(o[h + i]) * by);
+              transpose4(w, lane);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) __stcg(reinterpret_cast<uint4 *>(rows[i] + c + h), w[i]);
+            }
+          } else if (slot >= 0) {
             // a part: O, and below its maximum and sum, a column of 256 rows each
 #pragma unroll
             for (int i = 0; i < 32; ++i) __stcg(&part[(c + i) * (2 * TILE)], __uint_as_float(o[i]) * by);
@@ -815,7 +831,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
               if (reals >> (L::WRITE4 ? (lane & ~3) | i : lane) & 1) *reinterpret_cast<uint4 *>(out[i] + c) = w[i];
           }
         }
-        if (slot >= 0) {
+        if (SHARED || slot >= 0) {
           __stcg(&part[D * (2 * TILE)], m);
           __stcg(&part[(D + 1) * (2 * TILE)], l);
         }
@@ -886,14 +902,18 @@ __global__ void __launch_bounds__(2 * TILE) join_kernel(const AttendParams p) {
   *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + (int64_t(j.start) + token) * p.o_ts + h * p.o_hs + d0) = w;
 }
 
-template <int D, typename T>
-int launch(const AttendParams &p, int device, const PlanShape &shape, cudaStream_t stream) {
+template <int D, typename T, bool SHARED>
+int launch_kind(const AttendParams &p, int device, const PlanShape &shape, cudaStream_t stream) {
   static KernelSetup setup;
-  const int rc = setup.ready("emmy_kv8_attend", tiles_kernel<D, T>, device, Layout<D>::DYN, REGS_LAUNCH);
+  const int rc = setup.ready("emmy_kv8_attend", tiles_kernel<D, T, SHARED>, device, Layout<D>::DYN, REGS_LAUNCH);
   if (rc != EMMY_OK) return rc;
-  return launch_kernel("emmy_kv8_attend", tiles_kernel<D, T>,
+  return launch_kernel("emmy_kv8_attend", tiles_kernel<D, T, SHARED>,
                        dim3(unsigned(std::min<int64_t>(shape.most_units, sm_count(device)))), THREADS, Layout<D>::DYN,
                        stream, p);
+}
+template <int D, typename T>
+int launch(const AttendParams &p, int device, const PlanShape &shape, cudaStream_t stream) {
+  return p.shared != SHARED_NONE ? launch_kind<D, T, true>(p, device, shape, stream) : launch_kind<D, T, false>(p, device, shape, stream);
 }
 template <int D, typename T>
 int launch_join(const AttendParams &p, const PlanShape &shape, cudaStream_t stream) {
