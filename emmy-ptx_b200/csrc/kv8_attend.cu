@@ -78,30 +78,27 @@ int shape_of(const char *what, const emmy_kv8 *c, int heads, PlanShape &p) {
   return EMMY_OK;
 }
 
-// A call with shared keys: the run's rows over those first, by the row kernel where
-// no run has more than ROWS_MOST of a kv head, else by the tile kernel, all cut
-// along the keys; then each sequence's own keys by the row kernel, which takes the
-// others' results in at the end.  Longer sequences' rows fill tiles by themselves,
-// and a window leaves few shared keys: those calls are as without sharing.
+// A call with shared keys: the runs' rows over those, by the row kernel where no run
+// has more than ROWS_MOST of a kv head, else by the tile kernel, and beside it each
+// sequence's own keys by the row kernel; every part leaves a result, and a kernel
+// joins them.  Longer sequences' rows fill tiles by themselves, and a window leaves
+// few shared keys: those calls are as without sharing.
 int shape_shared(const char *what, const emmy_kv8 *c, const emmy_kv8_shared *sh, int heads, int window, PlanShape &p) {
   const int rc = shape_of(what, c, heads, p);
   if (rc != EMMY_OK) return rc;
   if (p.tiles || window > 0 || sh->max_runs == 0 || sh->max_tokens == 0) return EMMY_OK;
   const int sms = sm_count(c->device);
-  const int64_t group = heads / c->kv_heads, few = group * c->max_q;
+  const int64_t group = heads / c->kv_heads, few = group * c->max_q, run_rows = group * sh->max_tokens;
   const int64_t segments = int64_t(c->seqs) * c->kv_heads * ((few + ROWS_BLOCK - 1) / ROWS_BLOCK);
   const int64_t cap = int64_t(c->table_width) * c->page_size / 64;
   const int wave = sms * ROWS_PER_SM;
   p.max_runs = sh->max_runs, p.max_tokens = sh->max_tokens;
   p.cluster = 0, p.single = false;
-  p.target = p.spread ? p.slots * 2 / 3 : wave < p.slots ? wave : p.slots;
-  p.most_parts = std::min((p.spread ? p.slots : p.target) + segments, cap * segments);
-  const int64_t run_rows = group * p.max_tokens;
   int64_t units;
   if (run_rows <= ROWS_MOST) {
     p.shared = SHARED_ROWS;
-    p.pre_nt = rows_blocks(run_rows);
-    p.pre_rows = 8 * p.pre_nt;
+    p.nt = std::max(p.nt, rows_blocks(run_rows));
+    p.pre_rows = 8 * p.nt;
     units = int64_t(p.max_runs) * ((run_rows + p.pre_rows - 1) / p.pre_rows) * c->kv_heads;
     p.pre_target = units < wave ? wave : 0;
   } else {
@@ -111,11 +108,15 @@ int shape_shared(const char *what, const emmy_kv8 *c, const emmy_kv8_shared *sh,
     p.pre_target = units < sms ? sms : 0;
   }
   p.most_pre = units + p.pre_target;
-  if (p.most_pre > 0x7fffffff) return fail(EMMY_EINVAL, what, "too many sequences and heads for one call");
+  p.target = wave;
+  p.most_parts = std::min(p.target + segments, cap * segments) + (p.shared == SHARED_ROWS ? p.most_pre : 0);
+  if (p.most_pre > 0x7fffffff || p.most_parts > 0x7fffffff) return fail(EMMY_EINVAL, what, "too many sequences and heads for one call");
   if (p.shared == SHARED_TILES) p.most_units = p.most_pre;
-  p.workspace_bytes = EMMY_KV8_WORKSPACE_ZERO + p.partial_bytes + uint64_t(p.most_pre) * p.pre_rows * (c->head_dim + 2) * 4;
-  p.plan_bytes = sizeof(PlanHead) + uint64_t(p.most_parts) * sizeof(PartRec) + uint64_t(c->seqs) * sizeof(PrefixRec) +
-                 uint64_t(p.most_pre) * (p.shared == SHARED_TILES ? sizeof(UnitRec) : sizeof(PartRec));
+  p.partial_bytes = uint64_t(p.most_parts) * 8 * p.nt * (c->head_dim + 2) * 4;
+  p.workspace_bytes = EMMY_KV8_WORKSPACE_ZERO + p.partial_bytes +
+                      uint64_t(p.most_units) * p.pre_rows * (c->head_dim + 2) * 4;
+  p.plan_bytes = sizeof(PlanHead) + uint64_t(p.most_parts) * sizeof(PartRec) + uint64_t(p.most_units) * sizeof(UnitRec) +
+                 uint64_t(c->seqs) * sizeof(ResultRec) + uint64_t(c->tokens) * 4;
   return EMMY_OK;
 }
 
@@ -158,9 +159,8 @@ int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_shared *s
   if (shape.shared != SHARED_NONE) {
     if (shared->runs == 0 || shared->runs % 4) return fail(EMMY_EINVAL, what, "runs is missing or unaligned");
     p.runs = reinterpret_cast<const int *>(shared->runs);
-    p.prefix = reinterpret_cast<PrefixRec *>(p.parts + shape.most_parts);
-    p.pre_parts = reinterpret_cast<PartRec *>(p.prefix + cache->seqs);
-    p.units = reinterpret_cast<UnitRec *>(p.pre_parts);
+    p.results = reinterpret_cast<ResultRec *>(p.units + shape.most_units);
+    p.seq_of = reinterpret_cast<int *>(p.results + cache->seqs);
     p.pre_rows = shape.pre_rows;
   }
   return EMMY_OK;
@@ -227,7 +227,6 @@ int attend(const char *what, const emmy_kv8 *cache, const emmy_kv8_shared *share
   p.counters = reinterpret_cast<unsigned *>(a->workspace);
   p.partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO);
   p.tile_partial = reinterpret_cast<float *>(a->workspace + EMMY_KV8_WORKSPACE_ZERO + shape.partial_bytes);
-  p.pre_partial = p.tile_partial;
   p.scale_log2 = scale_log2;
   wait_limit(p.wait_ns, p.stall);
   const OnDevice on(cache->device);
@@ -235,18 +234,16 @@ int attend(const char *what, const emmy_kv8 *cache, const emmy_kv8_shared *share
   const bool bf16 = a->dtype == EMMY_KV8_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   note_capture(st);
-  if (shape.shared != SHARED_NONE) {
-    rc = shape.shared == SHARED_TILES ? tiles_attend(p, *cache, shape, bf16, st) : rows_shared(p, *cache, shape, bf16, true, st);
-    return rc == EMMY_OK ? rows_shared(p, *cache, shape, bf16, false, st) : rc;
-  }
-  p.beside = shape.tiles && shape.rows;
+  const bool tiles = shape.tiles || shape.shared == SHARED_TILES;
+  p.beside = tiles && shape.rows;
   p.ready = p.counters + EMMY_KV8_WORKSPACE_ZERO / 4 - 2;
-  if (shape.tiles) rc = tiles_attend(p, *cache, shape, bf16, st);
+  if (tiles) rc = tiles_attend(p, *cache, shape, bf16, st);
   if (rc == EMMY_OK && shape.rows) {
     rc = rows_attend(p, *cache, shape, bf16, st);
     if (rc != EMMY_OK && p.beside) cudaMemsetAsync(p.ready, 0, 8, st);  // nobody else will
   }
   if (rc == EMMY_OK && shape.tile_target > 0) rc = tiles_join(p, *cache, shape, bf16, st);
+  if (rc == EMMY_OK && shape.shared != SHARED_NONE) rc = shared_join(p, *cache, bf16, st);
   return rc;
 }
 

@@ -29,20 +29,18 @@ struct alignas(16) JoinRec {
   int slot0, parts, b, pad;
 };
 
-// What a sequence's keys that it shares with its run came to: results of some
-// parts of the run's query rows, block after block of p.pre_rows rows; a result is
-// O [pre_rows][head_dim], then maxima, then sums.
-struct alignas(16) PrefixRec {
+// Which results a sequence's rows have, in a call with shared keys.  A result is
+// O [rows of its slot][head_dim], then maxima, then sums.
+struct alignas(16) ResultRec {
   int chunks;        // 64-key chunks that are shared, 0: none
-  int slot0, parts;  // workspace slots of block 0 of kv head 0, one a part
-  int blocks, row;   // of the run's rows of a kv head; the sequence's first row among them
-  int pad[3];
+  int slot0, parts;  // their slots, of block 0 of kv head 0: one a part
+  int blocks, row;   // of the run's rows of a kv head, shape.pre_rows each; the sequence's first row among them
+  // of its own keys: the slot of row block 0 of part 0 of kv head 0; parts of a kv
+  // head; row blocks of a part, which are neighbours
+  int own_slot0, own_parts, own_blocks;
 };
 
-// Parts of a block at most: those that the row kernel joins at once.
-constexpr int MOST_SHARED = 160;
-
-// Which kernel, if any, attends to shared keys first.
+// Which kernel attends to shared keys.
 enum { SHARED_NONE = 0, SHARED_ROWS, SHARED_TILES };
 
 struct AttendParams {
@@ -67,12 +65,11 @@ struct AttendParams {
   int cluster;       // CTAs of a cluster of the row kernel, 0: none
   bool beside;       // the row kernel was launched to run beside the tile kernel
   unsigned *ready;   // there: what came before both is done, and the row kernel's blocks that know
-  int shared;           // SHARED_..: the rows' shared keys are the first kernel's, others the second's
+  int shared;           // SHARED_..
   const int *runs;      // [3][seqs]: see emmy_kv8_shared
-  PrefixRec *prefix;    // of each sequence
-  PartRec *pre_parts;   // of the row kernel, where it is the first, too
-  float *pre_partial;   // results for shared keys
-  int pre_rows;         // rows of a slot there
+  ResultRec *results;   // of each sequence
+  int *seq_of;          // of each token, -1: it is in none that can be
+  int pre_rows;         // rows of a slot of results for shared keys
   int stall;         // one block in so many withholds its first keys (0: none)
   unsigned long long wait_ns;  // limit of the kernels' waits
 };
@@ -92,9 +89,9 @@ struct PlanShape {
   uint64_t workspace_bytes, plan_bytes;
   // of a call with shared keys
   int shared;              // SHARED_..
-  int64_t most_pre;        // parts of the first kernel
-  int pre_target;          // that it aims at, 0: nothing is cut
-  int pre_nt, pre_rows;    // its 8-row blocks (of the row kernel), and rows of a slot of its results
+  int64_t most_pre;        // parts for shared keys
+  int pre_target;          // that are aimed at, 0: nothing is cut
+  int pre_rows;            // rows of a slot of their results
   int max_runs, max_tokens;
 };
 
@@ -210,7 +207,7 @@ constexpr int TILE_CUT = 8;     // chunks of a unit's part at least: a cut has t
 inline int rows_blocks(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
 int plan_shared(const AttendParams &p, const PlanShape &shape, cudaStream_t stream);
-int rows_shared(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, bool first, cudaStream_t stream);
+int shared_join(const AttendParams &p, const emmy_kv8 &cache, bool bf16, cudaStream_t stream);
 int plan_attend(const AttendParams &p, const PlanShape &shape, cudaStream_t stream);
 int tiles_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream);
 int tiles_join(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream);

@@ -259,18 +259,21 @@ struct Run {
   }
 };
 
-// The plan of a call with shared keys.  A run's blocks of query rows (of the
-// tile kernel's units, or the row kernel's) are each cut into the same number of
-// parts, so a row finds its results by where it stands in the run; their keys are
-// the same, and blocks of a part are neighbours.  Then segments and parts as
-// above, of each sequence's own keys.
+// The plan of a call with shared keys.  A run's blocks of query rows (the tile
+// kernel's units, or the row kernel's) are each cut into the same number of parts:
+// their keys are the same, so blocks of a part are neighbours.  Each sequence's own
+// keys are segments and parts as above.  Part `part` of row block `block` of a kv
+// head leaves its result in slot slot0 + (head * parts + part) * blocks + block, so
+// a row finds its results by where it stands.
 __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p) {
-  __shared__ int part_at[EMMY_KV8_MAX_SEQS], slot_at[EMMY_KV8_MAX_SEQS];
-  __shared__ int sums[WARPS];
+  __shared__ int at_of[EMMY_KV8_MAX_SEQS];
+  __shared__ int sums[WARPS], longest;
   grid_dependency_wait();
   grid_dependency_done();
   const Seqs &s = p.a.s;
   const int tid = threadIdx.x, H = s.kv_heads, b0 = tid * EACH, G = p.a.group, RB = p.a.pre_rows;
+  const bool tiles = p.a.shared == SHARED_TILES;
+  for (int i = tid; i < s.tokens; i += THREADS) p.a.seq_of[i] = -1;
   // ---- runs ----
   int pre_chunks[EACH], pre_blocks[EACH], runs = 0;
 #pragma unroll
@@ -285,26 +288,20 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
       }
     }
   }
+  if (tid == 0) longest = 1;
   int all, nth = block_scan(runs, all, sums), mine = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     if (pre_chunks[i] > 0 && nth++ >= p.max_runs) pre_chunks[i] = pre_blocks[i] = 0;  // one more than there is room for
+    if (pre_chunks[i] > 0) atomicMax(&longest, pre_chunks[i]);
     mine += pre_chunks[i] * pre_blocks[i];
   }
   block_scan(mine, all, sums);
-  // Chunks of a part: as many as leave one wave of parts, if any of some tries do,
-  // and so many that a block has no more parts than are joined at once.
-  __shared__ int longest;
-  if (tid == 0) longest = 1;
-  __syncthreads();
-  for (int i = 0; i < EACH; ++i)
-    if (pre_chunks[i] > 0) atomicMax(&longest, pre_chunks[i]);
-  __syncthreads();
-  const int least = (longest + MOST_SHARED - 1) / MOST_SHARED;
-  int limit = max(longest, least);
+  // Chunks of a part: as many as leave one wave of parts, if any of some tries do.
+  int limit = longest;
   if (p.pre_target > 0) {
     const int64_t share = (int64_t(all) * H + p.pre_target - 1) / p.pre_target;
-    const int l0 = max(int(min(share, int64_t(1) << 24)), max(least, p.a.shared == SHARED_TILES ? TILE_CUT : 2));
+    const int l0 = max(int(min(share, int64_t(1) << 24)), tiles ? TILE_CUT : 2);
     limit = l0;
     for (int t = 1; t <= 16; ++t) {
       int parts = 0, total;
@@ -323,27 +320,27 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
   for (int i = 0; i < EACH; ++i)
     if (b0 + i < s.seqs) {
       const int k = (pre_chunks[i] + limit - 1) / limit;
-      slot_at[b0 + i] = pre_at;
-      p.a.prefix[b0 + i] = PrefixRec{pre_chunks[i], pre_at, k, pre_blocks[i], 0, {}};
+      at_of[b0 + i] = pre_at;
+      p.a.results[b0 + i] = ResultRec{pre_chunks[i], pre_at, k, pre_blocks[i], 0, 0, 0, 1};
       pre_at += pre_blocks[i] * H * k;
     }
   __syncthreads();
   n_pre = min(n_pre, p.most_pre);
   for (int i = tid; i < n_pre; i += THREADS) {
-    const int b = owner_of(slot_at, s.seqs, i), rel = i - slot_at[b];
-    const PrefixRec f = p.a.prefix[b];
+    const int b = owner_of(at_of, s.seqs, i), rel = i - at_of[b];
+    const ResultRec f = p.a.results[b];
     const Run r(p, b);
     const int block = rel % f.blocks, part = rel / f.blocks % f.parts, head = rel / (f.blocks * f.parts);
-    const int slot0 = f.slot0 + (head * f.blocks + block) * f.parts;
     const int c0 = int(int64_t(f.chunks) * part / f.parts), c1 = int(int64_t(f.chunks) * (part + 1) / f.parts);
     // its tokens as if they came behind the shared keys
-    if (p.a.shared == SHARED_TILES)
-      p.a.units[i] = UnitRec{b, head, block * RB, r.start, r.tokens, r.keys + r.tokens, c0, c1, slot0 + part, {}};
+    if (tiles)
+      p.a.units[i] = UnitRec{b, head, block * RB, r.start, r.tokens, r.keys + r.tokens, c0, c1, i, {}};
     else
-      p.a.pre_parts[i] = PartRec{b, head, c0, c1, part, f.parts, slot0, block * RB,
-                                 r.start, r.tokens, r.keys + r.tokens, min(RB, r.tokens * G - block * RB)};
+      p.a.parts[i] = PartRec{b, head, c0, c1, part, f.parts, 0, block * RB,
+                             r.start, r.tokens, r.keys + r.tokens, min(RB, r.tokens * G - block * RB)};
   }
   // ---- each sequence's own keys ----
+  const int first_part = tiles ? 0 : n_pre;
   int chunks[EACH], blocks[EACH];  // row blocks
   mine = 0;
 #pragma unroll
@@ -354,12 +351,12 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
       int start, n, len;
       lengths(s, b, start, n, len);
       const int lead = p.a.runs[b];
-      PrefixRec f = {};
+      ResultRec f = {0, 0, 0, 1, 0, 0, 0, 1};
       // a run that cannot be, or not here, leaves its sequences to themselves
       if (lead >= 0 && lead <= b && p.a.runs[lead] == lead && b - lead < max(p.a.runs[s.seqs + lead], 1) &&
-          p.a.prefix[lead].chunks > 0) {
+          p.a.results[lead].chunks > 0) {
         const Run r(p, lead);
-        f = p.a.prefix[lead];
+        f = p.a.results[lead];
         f.row = (start - r.start) * G;
         // new tokens among the shared keys, or rows that are not the run's
         if (n > 0 && (f.chunks << 6 > len - n || start < r.start || start + n > r.start + r.tokens)) {
@@ -370,9 +367,10 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
       if (n > 0) {
         chunks[i] = Span(p.a, len - n, len - 1).chunks - f.chunks;
         blocks[i] = (n * G + ROWS_BLOCK - 1) / ROWS_BLOCK;
+        for (int t = 0; t < n; ++t) p.a.seq_of[start + t] = b;
       }
       // (a lead's own record stays, and others read only that)
-      if (lead != b) p.a.prefix[b] = f;
+      if (lead != b) p.a.results[b] = f;
     }
     mine += chunks[i] * blocks[i];
   }
@@ -390,47 +388,46 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
       if (int64_t(total) * H <= p.target) break;
       q = q0 + (q0 * t + 15) / 16;
     }
-  int parts = 0, slots = 0, n_parts, n_slots;
+  int parts = 0, n_parts;
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const int k = parts_of(p, chunks[i], q);
-    parts += k * blocks[i] * H;
-    slots += slots_of(p, k) * blocks[i] * H;
-  }
-  int at = block_scan(parts, n_parts, sums), slot = block_scan(slots, n_slots, sums);
-  __syncthreads();  // slot_at is read above
+  for (int i = 0; i < EACH; ++i) parts += parts_of(p, chunks[i], q) * blocks[i] * H;
+  int at = block_scan(parts, n_parts, sums);
+  __syncthreads();  // at_of and the leads' records are read above
 #pragma unroll
   for (int i = 0; i < EACH; ++i)
     if (b0 + i < s.seqs) {
       const int k = parts_of(p, chunks[i], q);
-      part_at[b0 + i] = at;
-      slot_at[b0 + i] = slot;
+      at_of[b0 + i] = at;
+      ResultRec &f = p.a.results[b0 + i];
+      f.own_slot0 = first_part + at;
+      f.own_parts = k;
+      f.own_blocks = max(blocks[i], 1);
       at += k * blocks[i] * H;
-      slot += slots_of(p, k) * blocks[i] * H;
     }
   __syncthreads();
-  n_parts = min(n_parts, p.most_parts);
+  n_parts = min(n_parts, p.most_parts - first_part);
   for (int i = tid; i < n_parts; i += THREADS) {
-    const int b = owner_of(part_at, s.seqs, i), rel = i - part_at[b];
+    const int b = owner_of(at_of, s.seqs, i), rel = i - at_of[b];
+    const ResultRec f = p.a.results[b];
     PartRec r;
     r.b = b;
     lengths(s, b, r.start, r.n, r.len);
-    const int base = p.a.prefix[b].chunks, c = Span(p.a, r.len - r.n, r.len - 1).chunks - base, k = parts_of(p, c, q);
-    const int rows = r.n * G, nb = (rows + ROWS_BLOCK - 1) / ROWS_BLOCK, each = (rows + nb - 1) / nb;
+    const int c = Span(p.a, r.len - r.n, r.len - 1).chunks - f.chunks, k = f.own_parts, nb = f.own_blocks;
+    const int rows = r.n * G, each = (rows + nb - 1) / nb;
     const int block = rel % nb, cut = rel / nb;
     r.head = cut / k;
     r.part = cut - r.head * k;
     r.parts = k;
-    r.slot0 = slot_at[b] + (r.head * nb + block) * slots_of(p, k);
-    r.c0 = base + int(int64_t(c) * r.part / k);
-    r.c1 = base + int(int64_t(c) * (r.part + 1) / k);
+    r.slot0 = 0;
+    r.c0 = f.chunks + int(int64_t(c) * r.part / k);
+    r.c1 = f.chunks + int(int64_t(c) * (r.part + 1) / k);
     r.row0 = block * each;
     r.rows = min(each, rows - r.row0);
-    p.a.parts[i] = r;
+    p.a.parts[first_part + i] = r;
   }
   if (tid == 0)
-    *p.a.plan = PlanHead{n_parts, n_pre, 0, G, p.a.window, p.a.sinks, p.a.row_limit, s.seqs, H, p.a.nt,
-                         s.width, s.page_shift, p.a.cluster, p.a.shared, {}};
+    *p.a.plan = PlanHead{first_part + n_parts, tiles ? n_pre : 0, 0, G, p.a.window, p.a.sinks, p.a.row_limit, s.seqs, H,
+                         p.a.nt, s.width, s.page_shift, p.a.cluster, p.a.shared, {}};
 }
 
 PlanParams params_of(const AttendParams &a, const PlanShape &shape) {
@@ -440,7 +437,7 @@ PlanParams params_of(const AttendParams &a, const PlanShape &shape) {
   p.spread = shape.spread;
   p.single = shape.single;
   // a join through the workspace costs about what ten chunks do
-  p.min_chunks = shape.cluster > 0 ? 10 : 2;
+  p.min_chunks = shape.cluster > 0 ? 10 : shape.shared != SHARED_NONE ? 4 : 2;
   p.most_parts = int(shape.most_parts);
   p.most_units = int(shape.most_units);
   p.most_joins = int(shape.most_joins);

@@ -96,7 +96,6 @@ struct Layout {
   static constexpr int LD = D + 4;        // floats of a row of the join
   static_assert((WARPS * LD + D) * 8 * NT * 4 <= QUERIES, "the join and a cluster's part fit over the ring");
   static_assert(2 * 64 * 8 * NT * 4 <= QUERIES, "so do the maxima and sums of 64 parts");
-  static_assert((WARPS * LD + D + 2 * MOST_SHARED) * 8 * NT * 4 <= QUERIES, "and those of the shared keys' parts beside the rows");
 };
 
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, int row, uint64_t *bar) {
@@ -302,12 +301,10 @@ __device__ __forceinline__ int query_row(uint32_t (&f)[D / 8], const T *row, int
   return e;
 }
 
-// A call's only kernel of its kind; the first of two, which leaves results for
-// shared keys in the workspace; or the second, which takes them in.
-enum { ALONE = 0, FIRST, SECOND };
-
 // Shared memory: first the joined rows of the four warps, over the staged queries.
-template <int D, int NT, bool CLUSTER, int MODE, typename T>
+// RESULT: every part, of a sequence's own keys or of those that a run shares, leaves
+// its rows in a slot of its own, for a kernel that joins them all.
+template <int D, int NT, bool CLUSTER, bool RESULT, typename T>
 __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtensorMap &codes_map) {
   using L = Layout<D, NT>;
   constexpr int ROWS = 8 * NT, LD = L::LD;
@@ -324,15 +321,13 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gr = lane >> 2, q = lane & 3;
   const Seqs &s = p.s;
   const PlanHead head = *p.plan;
-  const PartRec rec = (MODE == FIRST ? p.pre_parts : p.parts)[blockIdx.x];
+  const PartRec rec = p.parts[blockIdx.x];
   // (the block that waits in the end lets the next kernel start after that only:
   // its CTAs would take SMs in the order that these leave them, 257 for 248 us a
   // batch of prompts)
   if (!p.beside || blockIdx.x != 0) grid_dependency_done();
-  // (the tokens of a run stand behind its shared keys as if they were one sequence's)
-  if (blockIdx.x >= (MODE == FIRST ? head.units : head.parts) ||
-      !plan_fits(p, head, rec.b, rec.start, rec.n, MODE == FIRST ? rec.len - rec.n : rec.len))
-    return;
+  // (a run's tokens stand behind its shared keys as if they were one sequence's)
+  if (blockIdx.x >= head.parts || !plan_fits(p, head, rec.b, rec.start, rec.n, RESULT ? rec.len - rec.n : rec.len)) return;
   const Segment g = {rec.b, rec.head, rec.start, rec.n, rec.len, rec.row0, rec.rows, rec.part, rec.parts, rec.slot0,
                      Span(p, rec.len - rec.n, rec.len - 1)};
   const int c0 = rec.c0, c1 = rec.c1;
@@ -550,10 +545,8 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
     if (lane == 0) sm_unit[warp] = st.unit;
   }
   __syncthreads();
-  const bool whole = !CLUSTER && MODE != FIRST && g.parts == 1;
+  const bool whole = !CLUSTER && !RESULT && g.parts == 1;
   const int rows = g.rows;
-  PrefixRec shared = {};
-  if constexpr (MODE == SECOND) shared = p.prefix[g.b];
   const auto store = [&](int r, int d, const float (&x)[8], float l) {
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     uint4 w;
@@ -565,11 +558,7 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
   };
   const auto part_slot = [&](int c) { return p.partial + int64_t(g.slot0 + c) * ROWS * (D + 2); };
   // a cluster's parts stay in shared memory, behind what is joined here
-  // (so do the sequence's own, until those for its shared keys join them)
-  float *const held = join + WARPS * ROWS * LD, *const shared_m = held + ROWS * D, *const shared_l = shared_m + MOST_SHARED * ROWS;
-  float *const slot = CLUSTER         ? join + WARPS * ROWS * LD
-                      : MODE == FIRST ? p.pre_partial + int64_t(g.slot0 + g.part) * ROWS * (D + 2)
-                                      : part_slot(g.part);
+  float *const slot = CLUSTER ? join + WARPS * ROWS * LD : RESULT ? p.partial + int64_t(blockIdx.x) * ROWS * (D + 2) : part_slot(g.part);
   for (int i = tid; i < rows * (D / 8); i += THREADS) {
     const int r = i / (D / 8), d = i % (D / 8) * 8;
     float m = NONE, l = 0.0f, x[8] = {};
@@ -587,85 +576,15 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
         x[2 * j] += f * u.x, x[2 * j + 1] += f * u.y;
       }
     }
-    if ((!whole || MODE == SECOND) && d == 0) row_m[r] = m, row_l[r] = l;
-    if (whole && MODE != SECOND) {
+    if (!whole && d == 0) row_m[r] = m, row_l[r] = l;
+    if (whole) {
       store(r, d, x, l);
     } else {
-      float *const to = whole ? held : slot;
-      *reinterpret_cast<float4 *>(to + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-      *reinterpret_cast<float4 *>(to + r * D + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
+      *reinterpret_cast<float4 *>(slot + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4 *>(slot + r * D + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
     }
   }
-  // The rows in `held`, with maxima and sums in row_m and row_l, and the results for
-  // their shared keys as one, in the parts' order, into the output.
-  const auto finish = [&]() {
-    const int64_t size = int64_t(p.pre_rows) * (D + 2);
-    const auto part_of = [&](int r, int &row) {  // of row r, part 0
-      const int at = shared.row + g.row0 + r, block = at / p.pre_rows;
-      row = at - block * p.pre_rows;
-      return p.pre_partial + (shared.slot0 + (int64_t(g.head) * shared.blocks + block) * shared.parts) * size;
-    };
-    const int parts = shared.chunks > 0 ? min(shared.parts, MOST_SHARED) : 0;
-    for (int i = tid; i < parts * rows; i += THREADS) {
-      const int part = i / rows, r = i - part * rows;
-      int row;
-      const float *at = part_of(r, row);
-      at += part * size + p.pre_rows * D + row;
-      shared_m[part * ROWS + r] = __ldcg(at);
-      shared_l[part * ROWS + r] = __ldcg(at + p.pre_rows);
-    }
-    __syncthreads();
-    for (int r = warp; r < rows; r += ALL_WARPS) {
-      const float own = row_m[r];
-      float m = own;
-      for (int i = lane; i < parts; i += 32) m = fmaxf(m, shared_m[i * ROWS + r]);
-      for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-      float l = 0.0f;
-      for (int i = lane; i < parts; i += 32) {
-        const float f = exp2_fast(shared_m[i * ROWS + r] - m);
-        l += f * shared_l[i * ROWS + r];
-        shared_m[i * ROWS + r] = f;
-      }
-      for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-      if (lane == 0) {
-        const float f = exp2_fast(own - m);
-        row_l[r] = f * row_l[r] + l;
-        row_m[r] = f;
-      }
-    }
-    __syncthreads();
-    for (int i = tid; i < rows * (D / 4); i += THREADS) {
-      const int r = i / (D / 4), d = i % (D / 4) * 4;
-      int row;
-      const float *at = part_of(r, row);
-      at += row * D + d;
-      const float4 own = *reinterpret_cast<const float4 *>(held + r * D + d);
-      const float f0 = row_m[r];
-      float4 x = make_float4(f0 * own.x, f0 * own.y, f0 * own.z, f0 * own.w);
-      for (int c0 = 0; c0 < parts; c0 += 16) {  // sixteen loads in flight
-        float4 u[16];
-#pragma unroll
-        for (int c = 0; c < 16; ++c)
-          if (c0 + c < parts) u[c] = __ldcg(reinterpret_cast<const float4 *>(at + (c0 + c) * size));
-#pragma unroll
-        for (int c = 0; c < 16; ++c)
-          if (c0 + c < parts) {
-            const float f = shared_m[(c0 + c) * ROWS + r];
-            x.x += f * u[c].x, x.y += f * u[c].y, x.z += f * u[c].z, x.w += f * u[c].w;
-          }
-      }
-      const float by = row_l[r] == 0.0f ? 0.0f : 1.0f / row_l[r];
-      *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) =
-          make_uint2(pack2<T>(x.x * by, x.y * by), pack2<T>(x.z * by, x.w * by));
-    }
-  };
-  if (whole) {
-    if constexpr (MODE == SECOND) {
-      __syncthreads();
-      finish();
-    }
-    return;
-  }
+  if (whole) return;
   // results of the segment that go through the workspace, and which is this
   const int results = CLUSTER ? g.parts / p.cluster : g.parts, result = CLUSTER ? g.part / p.cluster : g.part;
   if constexpr (CLUSTER) {
@@ -714,8 +633,8 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
       __stcg(slot + ROWS * D + tid, row_m[tid]);
       __stcg(slot + ROWS * D + ROWS + tid, row_l[tid]);
     }
-    if constexpr (MODE == FIRST) return;
   }
+  if constexpr (RESULT) return;
   // ---- parts join in groups of GROUP, groups in the segment: the last of
   // each to arrive does it, in the parts' order ----
   const auto last_of = [&](int c, int level, int count) {
@@ -777,10 +696,6 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
           }
       }
       if (last) {
-        if constexpr (MODE == SECOND) {
-          *reinterpret_cast<float4 *>(held + r * D + d) = x;
-          continue;
-        }
         const float by = row_l[r] == 0.0f ? 0.0f : 1.0f / row_l[r];
         *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row_at(r, p.o_ts, p.o_hs) + d) =
             make_uint2(pack2<T>(x.x * by, x.y * by), pack2<T>(x.z * by, x.w * by));
@@ -799,14 +714,8 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
   const int groups = (results + group - 1) / group;
   if (!last_of(lead, 0, count)) return;
   gather(lead, count, 1, groups == 1);
-  if (groups > 1) {
-    if (!last_of(0, 1, groups)) return;
-    gather(0, groups, group, true);
-  }
-  if constexpr (MODE == SECOND) {
-    __syncthreads();
-    finish();
-  }
+  if (groups == 1 || !last_of(0, 1, groups)) return;
+  gather(0, groups, group, true);
 }
 
 // Beside the tile kernel, which was launched before it and whose sequences are
@@ -831,41 +740,45 @@ __device__ __forceinline__ void took_ready(const AttendParams &p) {
   if (threadIdx.x == 0 && atomicAdd(p.ready + 1, 1u) == gridDim.x - 1) p.ready[0] = p.ready[1] = 0;
 }
 
-template <int D, int NT, bool CLUSTER, int MODE, typename T>
+template <int D, int NT, bool CLUSTER, bool RESULT, typename T>
 __global__ void __launch_bounds__(THREADS, ROWS_PER_SM)
 rows_kernel(const AttendParams p, const __grid_constant__ CUtensorMap codes_map) {
   if (p.beside)
     ready_or_wait(p);
   else
     grid_dependency_wait();
-  attend_part<D, NT, CLUSTER, MODE, T>(p, codes_map);
+  attend_part<D, NT, CLUSTER, RESULT, T>(p, codes_map);
   if (p.beside) {
     took_ready(p);
     if (blockIdx.x == 0) grid_dependency_wait();
   }
 }
 
-template <int D, int NT, bool CLUSTER, int MODE, typename T>
+template <int D, int NT, bool CLUSTER, bool RESULT, typename T>
 int launch(const AttendParams &p, const CUtensorMap &map, int device, int grid, cudaStream_t stream) {
   static KernelSetup setup;
-  const int rc = setup.ready("emmy_kv8_attend", rows_kernel<D, NT, CLUSTER, MODE, T>, device, Layout<D, NT>::DYN);
+  const int rc = setup.ready("emmy_kv8_attend", rows_kernel<D, NT, CLUSTER, RESULT, T>, device, Layout<D, NT>::DYN);
   if (rc != EMMY_OK) return rc;
-  return launch_clusters("emmy_kv8_attend", rows_kernel<D, NT, CLUSTER, MODE, T>, CLUSTER ? p.cluster : 1, dim3(grid),
+  return launch_clusters("emmy_kv8_attend", rows_kernel<D, NT, CLUSTER, RESULT, T>, CLUSTER ? p.cluster : 1, dim3(grid),
                          THREADS, Layout<D, NT>::DYN, stream, p, map);
 }
 
-template <int D, int MODE, typename T>
-int launch_nt(const AttendParams &p, int nt, const CUtensorMap &map, int device, int grid, cudaStream_t stream) {
-  if constexpr (MODE == ALONE)
-    if (p.cluster > 0)
-      return nt == 1 ? launch<D, 1, true, MODE, T>(p, map, device, grid, stream)
-                     : launch<D, 2, true, MODE, T>(p, map, device, grid, stream);
-  return nt == 1 ? launch<D, 1, false, MODE, T>(p, map, device, grid, stream)
-                 : launch<D, 2, false, MODE, T>(p, map, device, grid, stream);
+template <int D, typename T>
+int launch_nt(const AttendParams &p, const CUtensorMap &map, int device, int grid, cudaStream_t stream) {
+  if (p.shared != SHARED_NONE)
+    return p.nt == 1 ? launch<D, 1, false, true, T>(p, map, device, grid, stream)
+                     : launch<D, 2, false, true, T>(p, map, device, grid, stream);
+  if (p.cluster > 0)
+    return p.nt == 1 ? launch<D, 1, true, false, T>(p, map, device, grid, stream)
+                     : launch<D, 2, true, false, T>(p, map, device, grid, stream);
+  return p.nt == 1 ? launch<D, 1, false, false, T>(p, map, device, grid, stream)
+                   : launch<D, 2, false, false, T>(p, map, device, grid, stream);
 }
 
-template <int MODE>
-int launch_mode(const AttendParams &p, const emmy_kv8 &cache, int nt, int64_t grid, bool bf16, cudaStream_t stream) {
+}  // namespace
+
+int rows_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream) {
+  const int64_t grid = shape.most_parts;
   // the pool as rows of head_dim bytes, 64 of them a box
   const int64_t rows = int64_t(cache.pages) * 2 * cache.kv_heads * cache.page_size;
   emmy_tmap_desc d = {};
@@ -882,21 +795,10 @@ int launch_mode(const AttendParams &p, const emmy_kv8 &cache, int nt, int64_t gr
   const int rc = emmy_tmap_encode(&d, &map);
   if (rc != EMMY_OK) return rc;
   if (cache.head_dim == 64)
-    return bf16 ? launch_nt<64, MODE, __nv_bfloat16>(p, nt, map, cache.device, int(grid), stream)
-                : launch_nt<64, MODE, __half>(p, nt, map, cache.device, int(grid), stream);
-  return bf16 ? launch_nt<128, MODE, __nv_bfloat16>(p, nt, map, cache.device, int(grid), stream)
-              : launch_nt<128, MODE, __half>(p, nt, map, cache.device, int(grid), stream);
-}
-
-}  // namespace
-
-int rows_attend(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, cudaStream_t stream) {
-  return launch_mode<ALONE>(p, cache, p.nt, shape.most_parts, bf16, stream);
-}
-
-int rows_shared(const AttendParams &p, const emmy_kv8 &cache, const PlanShape &shape, bool bf16, bool first, cudaStream_t stream) {
-  return first ? launch_mode<FIRST>(p, cache, shape.pre_nt, shape.most_pre, bf16, stream)
-               : launch_mode<SECOND>(p, cache, p.nt, shape.most_parts, bf16, stream);
+    return bf16 ? launch_nt<64, __nv_bfloat16>(p, map, cache.device, int(grid), stream)
+                : launch_nt<64, __half>(p, map, cache.device, int(grid), stream);
+  return bf16 ? launch_nt<128, __nv_bfloat16>(p, map, cache.device, int(grid), stream)
+              : launch_nt<128, __half>(p, map, cache.device, int(grid), stream);
 }
 
 }  // namespace kv8

@@ -789,7 +789,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         float *rows[4];  // SHARED: this lane's pieces of four lanes' rows
         if constexpr (SHARED)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) rows[i] = p.pre_partial + int64_t(slot) * (D + 2) * (2 * TILE) + (x * TILE + (r & ~3) + i) * D + 4 * (lane & 3);
+          for (int i = 0; i < 4; ++i) rows[i] = p.tile_partial + int64_t(slot) * (D + 2) * (2 * TILE) + (x * TILE + (r & ~3) + i) * D + 4 * (lane & 3);
         const uint32_t *bits = reinterpret_cast<const uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8));
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
