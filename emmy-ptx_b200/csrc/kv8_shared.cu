@@ -2,7 +2,7 @@
 // run's shared keys and those of its sequence's own, in the parts' order,
 //   m = max m_i,  l = sum l_i 2^(m_i - m),  O = sum O_i 2^(m_i - m) / l.
 // A warp a row: a lane first has a part's maximum and sum, then D / 32 values of
-// O.  Bound by the results, 4 (D + 2) bytes a part and row, from L2; sixteen loads in
+// O.  Bound by the results, 4 (D + 2) bytes a part and row, from L2; eight loads in
 // flight a lane.
 #include "kv8_attend.cuh"
 
@@ -27,58 +27,56 @@ __global__ void __launch_bounds__(32 * WARPS) shared_join_kernel(const AttendPar
   lengths(p.s, b, start, n, len);
   if (token < start || token >= start + n) return;  // lengths that changed since the plan
   const int kv_head = h / p.group, r = (token - start) * p.group + h - kv_head * p.group;
-  // its results for shared keys, then for its own
-  const int pre_size = p.pre_rows * (D + 2), own_size = 8 * p.nt * (D + 2);
-  const int at = f.row + r, block = at / p.pre_rows, pre_row = at - block * p.pre_rows;
-  const float *pre = (p.shared == SHARED_TILES ? p.tile_partial : p.partial) +
-                     (f.slot0 + int64_t(kv_head) * f.parts * f.blocks + block) * pre_size;
-  const int each = (n * p.group + f.own_blocks - 1) / f.own_blocks, own_block = r / each, own_row = r - own_block * each;
-  const float *own = p.partial + (f.own_slot0 + int64_t(kv_head) * f.own_parts * f.own_blocks + own_block) * own_size;
-  const int parts = f.parts + f.own_parts;
-  const auto values_of = [&](int i) {  // the row in part i
-    return i < f.parts ? pre + int64_t(i) * f.blocks * pre_size + pre_row * D
-                       : own + int64_t(i - f.parts) * f.own_blocks * own_size + own_row * D;
-  };
-  const auto sums_of = [&](int i) {  // its maximum, and so many floats on its sum
-    return i < f.parts ? pre + int64_t(i) * f.blocks * pre_size + p.pre_rows * D + pre_row
-                       : own + int64_t(i - f.parts) * f.own_blocks * own_size + 8 * p.nt * D + own_row;
-  };
   float m = NONE, l = 0.0f, x[N] = {};
-  for (int i0 = 0; i0 < parts; i0 += 32) {
-    const int count = min(32, parts - i0), i = i0 + min(lane, count - 1);
-    const float *sums = sums_of(i);
-    const float mi = __ldcg(sums), li = __ldcg(sums + (i < f.parts ? p.pre_rows : 8 * p.nt));
-    float top = fmaxf(mi, m);
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const float before = exp2_fast(m - top), w = lane < count ? exp2_fast(mi - top) : 0.0f;
-    float sum = lane < count ? w * li : 0.0f;
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    l = l * before + sum;
-    m = top;
+  // `parts` results, so many floats apart, of slots of so many rows
+  const auto take = [&](const float *first, int64_t apart, int slot_rows, int slot_row, int parts) {
+    const float *sums = first + slot_rows * D + slot_row, *values = first + slot_row * D + lane * N;
+    for (; parts > 0; parts -= 32, sums += 32 * apart) {
+      const int count = min(32, parts);
+      const float *mine = sums + min(lane, count - 1) * apart;
+      const float mi = __ldcg(mine), li = __ldcg(mine + slot_rows);
+      float top = fmaxf(mi, m);
+      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float before = exp2_fast(m - top), w = lane < count ? exp2_fast(mi - top) : 0.0f;
+      float sum = lane < count ? w * li : 0.0f;
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      l = l * before + sum;
+      m = top;
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] *= before;
-    for (int c0 = 0; c0 < count; c0 += 16) {
-      float u[16][N];
+      for (int j = 0; j < N; ++j) x[j] *= before;
+      for (int c0 = 0; c0 < count; c0 += 8) {
+        float u[8][N];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float *from = values_of(i0 + min(c0 + c, count - 1)) + lane * N;
-        if constexpr (N == 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4 *>(from));
-          u[c][0] = v.x, u[c][1] = v.y, u[c][2] = v.z, u[c][3] = v.w;
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2 *>(from));
-          u[c][0] = v.x, u[c][1] = v.y;
+        for (int c = 0; c < 8; ++c) {
+          const bool real = c0 + c < count;
+          if constexpr (N == 4) {
+            const float4 v = real ? __ldcg(reinterpret_cast<const float4 *>(values)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            u[c][0] = v.x, u[c][1] = v.y, u[c][2] = v.z, u[c][3] = v.w;
+          } else {
+            const float2 v = real ? __ldcg(reinterpret_cast<const float2 *>(values)) : make_float2(0.0f, 0.0f);
+            u[c][0] = v.x, u[c][1] = v.y;
+          }
+          values += apart;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float by = __shfl_sync(0xffffffffu, w, (c0 + c) & 31);  // 0 where there is none
+#pragma unroll
+          for (int j = 0; j < N; ++j) x[j] += by * u[c][j];
         }
       }
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        if (c0 + c >= count) break;
-        const float by = __shfl_sync(0xffffffffu, w, c0 + c);
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[j] += by * u[c][j];
-      }
     }
+  };
+  // its results for shared keys, then for its own
+  const int pre_size = p.pre_rows * (D + 2), own_size = 8 * p.nt * (D + 2);
+  if (f.parts > 0) {
+    const int at = f.row + r, block = at / p.pre_rows;
+    take((p.shared == SHARED_TILES ? p.tile_partial : p.partial) + (f.slot0 + int64_t(kv_head) * f.parts * f.blocks + block) * pre_size,
+         int64_t(f.blocks) * pre_size, p.pre_rows, at - block * p.pre_rows, f.parts);
   }
+  const int each = (n * p.group + f.own_blocks - 1) / f.own_blocks, own_block = r / each;
+  take(p.partial + (f.own_slot0 + int64_t(kv_head) * f.own_parts * f.own_blocks + own_block) * own_size,
+       int64_t(f.own_blocks) * own_size, 8 * p.nt, r - own_block * each, f.own_parts);
   const float by = l == 0.0f ? 0.0f : 1.0f / l;
   T *to = static_cast<T *>(p.out) + token * p.o_ts + h * p.o_hs + lane * N;
   if constexpr (N == 4)

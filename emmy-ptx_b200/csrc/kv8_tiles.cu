@@ -31,6 +31,7 @@
 // exponent of p; O moves (a pass over its columns) only when a row's maximum
 // grew by more than 2^8 or V's exponent strayed by more than 2^6.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv8_async.cuh"
 #include "kv8_attend.cuh"
@@ -246,6 +247,77 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(smem_addr(bar))
                : "memory");
+}
+
+// Largest magnitudes of two pairs of 16-bit floats: their bits order as whole
+// numbers do.
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) { return __vmaxu2(a, b & 0x7fff7fffu); }
+template <typename T>
+__device__ __forceinline__ float magnitude(uint32_t bits) {  // of one value, bits 0-15
+  if constexpr (std::is_same<T, __half>::value)
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+  else
+    return __uint_as_float(bits << 16);
+}
+// A unit's query rows as put_query does them, where a part has few chunks: four lanes
+// do four rows together, each its 16-byte pieces of all, with no exchange but that of
+// the maxima, two values an instruction (a thread a row, pieces transposed: 5.2 us
+// from the barriers to the first product's operands, so 2.9).
+template <int D, typename T>
+__device__ __forceinline__ float put_queries_of_four(const AttendParams &p, uint8_t *tile, int r, int lane, int64_t mine, uint64_t *full) {
+  constexpr int PIECES = D / 32;  // of a row, a lane
+  constexpr uint32_t INF = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  uint4 w[4][PIECES];
+  const int quarter = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const T *src = static_cast<const T *>(p.q) + __shfl_sync(0xffffffffu, mine, (lane & ~3) | i) + 8 * quarter;
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) w[i][k] = *reinterpret_cast<const uint4 *>(src + 32 * k);
+  }
+  float own = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k)
+      top = larger2(larger2(larger2(larger2(top, w[i][k].x), w[i][k].y), w[i][k].z), w[i][k].w);
+    uint32_t most = max(top & 0xffffu, top >> 16);
+    if (most >= INF) {  // (rare) the largest finite one
+      most = 0;
+#pragma unroll
+      for (int k = 0; k < PIECES; ++k) {
+        const uint32_t *v = &w[i][k].x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t lo = v[j] & 0x7fffu, hi = v[j] >> 16 & 0x7fffu;
+          if (lo < INF) most = max(most, lo);
+          if (hi < INF) most = max(most, hi);
+        }
+      }
+    }
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const int e = row_exponent(magnitude<T>(most));
+    const float by = p.scale_log2 < 0.0f ? -pow2(-e) : pow2(-e);
+    const int row = (r & ~3) | i;
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      uint32_t *v = &w[i][k].x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float a, b;
+        unpack2<T>(v[j], a, b);
+        v[j] = pack2<__half>(a * by, b * by);
+      }
+      const int piece = 4 * k + quarter;
+      *reinterpret_cast<uint4 *>(tile + piece / 8 * (TILE * 128) + swizzled(row, piece % 8)) = w[i][k];
+    }
+    if (i == quarter) own = fabsf(p.scale_log2) * pow2(e);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  warp_arrive(full);
+  return own;
 }
 
 // SHARED: the units are runs' rows over shared keys, and every one leaves a result.
@@ -552,6 +624,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
     // them; returns the factor of the row's scores.  The products that read the
     // rows before are done: their scores were here.
     const auto put_query = [&](const Unit &u, const Row &row) {
+      if constexpr (SHARED && !L::Q_TMEM) return put_queries_of_four<D, T>(p, dyn + x * L::Q_TILE, r, lane, (int64_t(u.start) + row.token) * p.q_ts + row.head * p.q_hs, &bars.q_full[x]);
       const int64_t mine = (int64_t(u.start) + row.token) * p.q_ts + row.head * p.q_hs;
       const T *const q = static_cast<const T *>(p.q);
       uint4 w[D / 8];
