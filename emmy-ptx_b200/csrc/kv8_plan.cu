@@ -297,19 +297,69 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
     mine += pre_chunks[i] * pre_blocks[i];
   }
   block_scan(mine, all, sums);
-  // Chunks of a part: as many as leave one wave of parts, if any of some tries do.
+  const int pre_work = all;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+    if (b0 + i < s.seqs) p.a.results[b0 + i] = ResultRec{pre_chunks[i], 0, 0, pre_blocks[i], 0, 0, 0, 1};
+  __syncthreads();
+  // ---- each sequence's own keys ----
+  int chunks[EACH], blocks[EACH];  // row blocks
+  mine = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    chunks[i] = blocks[i] = 0;
+    const int b = b0 + i;
+    if (b < s.seqs) {
+      int start, n, len;
+      lengths(s, b, start, n, len);
+      const int lead = p.a.runs[b];
+      int shared = 0;
+      // a run that cannot be, or not here, leaves its sequences to themselves
+      if (lead >= 0 && lead <= b && p.a.runs[lead] == lead && b - lead < max(p.a.runs[s.seqs + lead], 1)) {
+        const Run r(p, lead);
+        shared = p.a.results[lead].chunks;
+        // new tokens among the shared keys, or rows that are not the run's
+        if (shared > 0 && n > 0 && (shared << 6 > len - n || start < r.start || start + n > r.start + r.tokens)) {
+          report(s.status, STATUS_LENGTH);
+          n = 0;
+        }
+      }
+      if (n > 0) {
+        chunks[i] = Span(p.a, len - n, len - 1).chunks - shared;
+        blocks[i] = (n * G + ROWS_BLOCK - 1) / ROWS_BLOCK;
+        for (int t = 0; t < n; ++t) p.a.seq_of[start + t] = b;
+      }
+    }
+    mine += chunks[i] * blocks[i];
+  }
+  int own_work;
+  block_scan(mine, own_work, sums);
+  // ---- chunks of a part of shared keys ----
+  // Row kernel: as many as leave one wave of parts, if any of some tries do.  Tile
+  // kernel: those for which this ends first: a block has FIXED and CHUNK us a chunk;
+  // it runs beside the row kernel, whose chunks of own keys take OWN us of an SM
+  // each; and a result costs RESULT us to write and join.
   int limit = longest;
   if (p.pre_target > 0) {
-    const int64_t share = (int64_t(all) * H + p.pre_target - 1) / p.pre_target;
+    const int64_t share = (int64_t(pre_work) * H + p.pre_target - 1) / p.pre_target;
     const int l0 = max(int(min(share, int64_t(1) << 24)), tiles ? TILE_CUT : 2);
-    limit = l0;
+    constexpr float FIXED = 10.0f, CHUNK = 1.03f, OWN = 0.46f, RESULT = 0.053f;
+    float best = 0.0f;
+    limit = 0;
+    int tried = l0;
     for (int t = 1; t <= 16; ++t) {
       int parts = 0, total;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) parts += pre_blocks[i] * ((pre_chunks[i] + limit - 1) / limit);
+      for (int i = 0; i < EACH; ++i) parts += pre_blocks[i] * ((pre_chunks[i] + tried - 1) / tried);
       block_scan(parts, total, sums);
-      if (int64_t(total) * H <= p.pre_target) break;
-      limit = l0 + (l0 * t + 15) / 16;
+      const bool fits = int64_t(total) * H <= p.pre_target;
+      if (fits || t == 16) {
+        const float n = float(total) * H, tile = FIXED + CHUNK * tried;
+        const float ends = fmaxf(tile, (n * tile + OWN * own_work * H) / p.pre_target) + RESULT * n;
+        if (limit == 0 || (tiles && ends < best)) limit = tried, best = ends;
+        if (!tiles) break;
+      }
+      tried += max(1, tried >> 3);
     }
   }
   int pre = 0;
@@ -321,7 +371,8 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
     if (b0 + i < s.seqs) {
       const int k = (pre_chunks[i] + limit - 1) / limit;
       at_of[b0 + i] = pre_at;
-      p.a.results[b0 + i] = ResultRec{pre_chunks[i], pre_at, k, pre_blocks[i], 0, 0, 0, 1};
+      p.a.results[b0 + i].slot0 = pre_at;
+      p.a.results[b0 + i].parts = k;
       pre_at += pre_blocks[i] * H * k;
     }
   __syncthreads();
@@ -339,43 +390,9 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
       p.a.parts[i] = PartRec{b, head, c0, c1, part, f.parts, 0, block * RB,
                              r.start, r.tokens, r.keys + r.tokens, min(RB, r.tokens * G - block * RB)};
   }
-  // ---- each sequence's own keys ----
+  // ---- parts of own keys ----
   const int first_part = tiles ? 0 : n_pre;
-  int chunks[EACH], blocks[EACH];  // row blocks
-  mine = 0;
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    chunks[i] = blocks[i] = 0;
-    const int b = b0 + i;
-    if (b < s.seqs) {
-      int start, n, len;
-      lengths(s, b, start, n, len);
-      const int lead = p.a.runs[b];
-      ResultRec f = {0, 0, 0, 1, 0, 0, 0, 1};
-      // a run that cannot be, or not here, leaves its sequences to themselves
-      if (lead >= 0 && lead <= b && p.a.runs[lead] == lead && b - lead < max(p.a.runs[s.seqs + lead], 1) &&
-          p.a.results[lead].chunks > 0) {
-        const Run r(p, lead);
-        f = p.a.results[lead];
-        f.row = (start - r.start) * G;
-        // new tokens among the shared keys, or rows that are not the run's
-        if (n > 0 && (f.chunks << 6 > len - n || start < r.start || start + n > r.start + r.tokens)) {
-          report(s.status, STATUS_LENGTH);
-          n = 0;
-        }
-      }
-      if (n > 0) {
-        chunks[i] = Span(p.a, len - n, len - 1).chunks - f.chunks;
-        blocks[i] = (n * G + ROWS_BLOCK - 1) / ROWS_BLOCK;
-        for (int t = 0; t < n; ++t) p.a.seq_of[start + t] = b;
-      }
-      // (a lead's own record stays, and others read only that)
-      if (lead != b) p.a.results[b] = f;
-    }
-    mine += chunks[i] * blocks[i];
-  }
-  block_scan(mine, all, sums);
-  const int64_t work = int64_t(all) * H;
+  const int64_t work = int64_t(own_work) * H;
   const int64_t share = (work + p.target - 1) / p.target;
   const int q0 = max(p.min_chunks, int(min(share, int64_t(1) << 24)));
   int q = q0;
@@ -392,17 +409,26 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
 #pragma unroll
   for (int i = 0; i < EACH; ++i) parts += parts_of(p, chunks[i], q) * blocks[i] * H;
   int at = block_scan(parts, n_parts, sums);
-  __syncthreads();  // at_of and the leads' records are read above
+  __syncthreads();  // at_of is read above
 #pragma unroll
   for (int i = 0; i < EACH; ++i)
     if (b0 + i < s.seqs) {
-      const int k = parts_of(p, chunks[i], q);
-      at_of[b0 + i] = at;
-      ResultRec &f = p.a.results[b0 + i];
-      f.own_slot0 = first_part + at;
-      f.own_parts = k;
-      f.own_blocks = max(blocks[i], 1);
+      const int b = b0 + i, k = parts_of(p, chunks[i], q), lead = p.a.runs[b];
+      at_of[b] = at;
+      ResultRec f = {0, 0, 0, 1, 0, first_part + at, k, max(blocks[i], 1)};
+      if (chunks[i] > 0 && lead >= 0 && lead <= b && p.a.runs[lead] == lead && b - lead < max(p.a.runs[s.seqs + lead], 1)) {
+        const ResultRec of = p.a.results[lead];  // (others write only what comes behind `row`)
+        f.chunks = of.chunks, f.slot0 = of.slot0, f.parts = of.parts, f.blocks = max(of.blocks, 1);
+        f.row = (s.q_starts[b] - s.q_starts[lead]) * G;
+      }
       at += k * blocks[i] * H;
+      if (lead == b) {
+        p.a.results[b].own_slot0 = f.own_slot0;
+        p.a.results[b].own_parts = k;
+        p.a.results[b].own_blocks = f.own_blocks;
+      } else {
+        p.a.results[b] = f;
+      }
     }
   __syncthreads();
   n_parts = min(n_parts, p.most_parts - first_part);
