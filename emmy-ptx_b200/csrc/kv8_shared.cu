@@ -67,16 +67,19 @@ __global__ void __launch_bounds__(32 * WARPS) shared_join_kernel(const AttendPar
       }
     }
   };
-  // its results for shared keys, then for its own
-  const int pre_size = p.pre_rows * (D + 2), own_size = 8 * p.nt * (D + 2);
-  if (f.parts > 0) {
-    const int at = f.row + r, block = at / p.pre_rows;
-    take((p.shared == SHARED_TILES ? p.tile_partial : p.partial) + (f.slot0 + int64_t(kv_head) * f.parts * f.blocks + block) * pre_size,
-         int64_t(f.blocks) * pre_size, p.pre_rows, at - block * p.pre_rows, f.parts);
+  // its results for shared keys, then for its own (one loop's code, not two)
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    const bool of_run = i == 0;
+    const int slot_rows = of_run ? p.pre_rows : 8 * p.nt, size = slot_rows * (D + 2);
+    const int parts = of_run ? f.parts : f.own_parts, blocks = of_run ? f.blocks : f.own_blocks;
+    const int at = of_run ? f.row + r : r, each = of_run ? slot_rows : (n * p.group + blocks - 1) / blocks;
+    if (parts == 0) continue;
+    const int block = at / each;
+    take((of_run && p.shared == SHARED_TILES ? p.tile_partial : p.partial) +
+             ((of_run ? f.slot0 : f.own_slot0) + int64_t(kv_head) * parts * blocks + block) * size,
+         int64_t(blocks) * size, slot_rows, at - block * each, parts);
   }
-  const int each = (n * p.group + f.own_blocks - 1) / f.own_blocks, own_block = r / each;
-  take(p.partial + (f.own_slot0 + int64_t(kv_head) * f.own_parts * f.own_blocks + own_block) * own_size,
-       int64_t(f.own_blocks) * own_size, 8 * p.nt, r - own_block * each, f.own_parts);
   const float by = l == 0.0f ? 0.0f : 1.0f / l;
   T *to = static_cast<T *>(p.out) + token * p.o_ts + h * p.o_hs + lane * N;
   if constexpr (N == 4)

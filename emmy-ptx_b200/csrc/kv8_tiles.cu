@@ -190,6 +190,12 @@ __device__ __forceinline__ void tm_ld8(uint32_t (&r)[8], uint32_t at) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(at));
 }
+__device__ __forceinline__ void tm_ld16(uint32_t (&r)[16], uint32_t at) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(at));
+}
 __device__ __forceinline__ void tm_st8(uint32_t at, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]),
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -276,18 +282,19 @@ __device__ __forceinline__ float put_queries_of_four(const AttendParams &p, uint
     for (int k = 0; k < PIECES; ++k) w[i][k] = *reinterpret_cast<const uint4 *>(src + 32 * k);
   }
   float own = 0.0f;
-#pragma unroll
+  // (a loop, the rows moving up: code that a block runs once comes from memory)
+#pragma unroll 1
   for (int i = 0; i < 4; ++i) {
     uint32_t top = 0;
 #pragma unroll
     for (int k = 0; k < PIECES; ++k)
-      top = larger2(larger2(larger2(larger2(top, w[i][k].x), w[i][k].y), w[i][k].z), w[i][k].w);
+      top = larger2(larger2(larger2(larger2(top, w[0][k].x), w[0][k].y), w[0][k].z), w[0][k].w);
     uint32_t most = max(top & 0xffffu, top >> 16);
     if (most >= INF) {  // (rare) the largest finite one
       most = 0;
 #pragma unroll
       for (int k = 0; k < PIECES; ++k) {
-        const uint32_t *v = &w[i][k].x;
+        const uint32_t *v = &w[0][k].x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t lo = v[j] & 0x7fffu, hi = v[j] >> 16 & 0x7fffu;
@@ -303,7 +310,7 @@ __device__ __forceinline__ float put_queries_of_four(const AttendParams &p, uint
     const int row = (r & ~3) | i;
 #pragma unroll
     for (int k = 0; k < PIECES; ++k) {
-      uint32_t *v = &w[i][k].x;
+      uint32_t *v = &w[0][k].x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float a, b;
@@ -311,7 +318,8 @@ __device__ __forceinline__ float put_queries_of_four(const AttendParams &p, uint
         v[j] = pack2<__half>(a * by, b * by);
       }
       const int piece = 4 * k + quarter;
-      *reinterpret_cast<uint4 *>(tile + piece / 8 * (TILE * 128) + swizzled(row, piece % 8)) = w[i][k];
+      *reinterpret_cast<uint4 *>(tile + piece / 8 * (TILE * 128) + swizzled(row, piece % 8)) = w[0][k];
+      w[0][k] = w[1][k], w[1][k] = w[2][k], w[2][k] = w[3][k];
     }
     if (i == quarter) own = fabsf(p.scale_log2) * pow2(e);
   }
@@ -859,11 +867,25 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
                    (L::WRITE4 ? __shfl_sync(0xffffffffu, to, (lane & ~3) | i) + 8 * (lane & 3) : to + 8 * i);
         const float by = SHARED || slot >= 0 ? pow2(unit) : l == 0.0f ? 0.0f : pow2(unit) / l;
         float *const part = p.tile_partial + int64_t(slot) * (D + 2) * (2 * TILE) + x * TILE + r;
-        float *rows[4];  // SHARED: this lane's pieces of four lanes' rows
-        if constexpr (SHARED)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) rows[i] = p.tile_partial + int64_t(slot) * (D + 2) * (2 * TILE) + (x * TILE + (r & ~3) + i) * D + 4 * (lane & 3);
         const uint32_t *bits = reinterpret_cast<const uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8));
+        if constexpr (SHARED) {
+          // O, row after row, four lanes 64 bytes of one together.  A loop: code that
+          // a block runs once comes from memory (unrolled: 6.2 us, so 2.0).
+          float *to = p.tile_partial + int64_t(slot) * (D + 2) * (2 * TILE) + (x * TILE + (r & ~3)) * D + 4 * (lane & 3);
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16, to += 16) {
+            uint32_t o[16];
+            tm_ld16(o, o_at + c);
+            tm_wait_ld();
+            const uint32_t nan = nan_seen ? bits[c / 32] >> (c & 16) : 0;
+            uint4 w[4];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) (&w[i / 4].x)[i % 4] = nan >> i & 1 ? 0x7fc00000u : __float_as_uint(__uint_as_float(o[i]) * by);
+            transpose4(w, lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) __stcg(reinterpret_cast<uint4 *>(to + i * D), w[i]);
+          }
+        } else
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
@@ -874,18 +896,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (nan >> i & 1) o[i] = 0x7fc00000u;
-          if constexpr (SHARED) {
-            // O, row after row, four lanes 64 bytes of one together
-#pragma unroll
-            for (int h = 0; h < 32; h += 16) {
-              uint4 w[4];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) (&w[i / 4].x)[i % 4] = __float_as_uint(__uint_as_float(o[h + i]) * by);
-              transpose4(w, lane);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) __stcg(reinterpret_cast<uint4 *>(rows[i] + c + h), w[i]);
-            }
-          } else if (slot >= 0) {
+          if (slot >= 0) {
             // a part: O, and below its maximum and sum, a column of 256 rows each
 #pragma unroll
             for (int i = 0; i < 32; ++i) __stcg(&part[(c + i) * (2 * TILE)], __uint_as_float(o[i]) * by);
