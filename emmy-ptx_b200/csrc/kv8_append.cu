@@ -49,7 +49,8 @@ struct RotatedParams : AppendParams {
   void *out;
   int64_t q_ts, q_hs, o_ts, o_hs;
   int dims, heads, out_type;  // heads: 0 where there is no q
-  bool wide, interleaved;
+  int head_dim;
+  bool wide, interleaved, copy;  // copy: q_out is not q
   float gain;
 };
 
@@ -75,6 +76,9 @@ __device__ __forceinline__ float Vec<__half>::at(int i) const {
   const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&(&w.x)[i / 2]));
   return i & 1 ? f.y : f.x;
 }
+template <typename T>
+constexpr int type_of = sizeof(T) == 4 ? EMMY_KV8_F32 : std::is_same<T, __half>::value ? EMMY_KV8_F16 : EMMY_KV8_BF16;
+
 // The largest finite magnitude, and amax.
 template <typename T>
 __device__ __forceinline__ float max_finite(const Vec<T> &v, float amax) {
@@ -327,13 +331,22 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// Keys and values by pages, and rows of queries: the blocks of both mixed evenly, so
+// that those that copy and those that compute run side by side.
+struct MixedParams {
+  RotatedParams kv;
+  rotary::Params q;
+  int page_blocks, kv_blocks, blocks;  // blocks of a page; of all pages, and with the queries'
+};
+
 // append_kernel with keys turned on the way.  A thread's pieces of a row are two
 // that pair up (or, at the end of a row with fewer dims, two of those behind), of
 // half as many rows; it holds their values as f32 through the maximum.  Bound by
 // instructions as much as by memory: two values an instruction where there is one
 // for that, angles by steps, (side, head)s in turn so that blocks are alike.
 template <int D, typename T, int MODE, int ROWS, int MOST>
-__global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append_turned_kernel(const __grid_constant__ RotatedParams p) {
+__global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append_turned_kernel(const __grid_constant__ MixedParams all) {
+  const RotatedParams &p = all.kv;
   using V = Vec<T>;
   using P = rotary::Piece<T, V::N>;
   using rotary::mul2, rotary::fma2, rotary::two, rotary::apart;
@@ -344,8 +357,14 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
   const Seqs &s = p.s;
   grid_dependency_wait();
   grid_dependency_done();
+  const int kv_block = blockIdx.x;
+  if (kv_block >= all.kv_blocks) {
+    if constexpr (MODE != ANY) rotary::rotate_block<T, T, N, MODE == NEIGHBOURS>(all.q, kv_block - all.kv_blocks, blockDim.x);
+    return;
+  }
+  const int nth_page = kv_block / all.page_blocks, nth = kv_block - nth_page * all.page_blocks;
   int b, start, n, len, page_of_seq;
-  if (!owner(s, blockIdx.x, b, start, n, len, page_of_seq)) return;
+  if (!owner(s, nth_page, b, start, n, len, page_of_seq)) return;
   const int size = 1 << s.page_shift, first = len - n, H = s.kv_heads;
   const int page = s.table[int64_t(b) * s.width + page_of_seq];
   const int pos0 = page_of_seq << s.page_shift;
@@ -377,7 +396,7 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  const int u0 = blockIdx.y * p.units, u1 = min(u0 + p.units, 2 * H);
+  const int u0 = nth * p.units, u1 = min(u0 + p.units, 2 * H);
   fetch(u0, 0);
   const bool bad = page < 0 || page >= s.pages;
   if (bad && tid == 0) report(s.status, STATUS_PAGE);
@@ -584,6 +603,30 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
   if (lo > 0 && e > old) recode_rows<D>(codes, lo, old, e, lane, 32);
 }
 
+// Whether the queries of pages go with their keys and values: at their places, of
+// the same type, in whole pieces.  (Others are a launch of the row kernel's.)
+template <typename T>
+bool mixes(const RotatedParams &p) {
+  constexpr int N = Vec<T>::N;
+  return p.heads > 0 && p.positions == nullptr && p.out_type == type_of<T> && (p.interleaved ? p.dims : p.dims / 2) % N == 0;
+}
+
+// The queries as rows to turn.
+rotary::Params query_rows(const RotatedParams &p) {
+  rotary::Params r = {};
+  for (int i = 0; i < 64; ++i) r.frequency[i] = p.frequency[i];
+  r.x = p.q, r.out = p.out;
+  r.positions = p.positions, r.position_stride = p.position_stride, r.wide = p.wide;
+  r.tokens = p.s.tokens;
+  r.x_ts = p.q_ts, r.x_hs = p.q_hs, r.o_ts = p.o_ts, r.o_hs = p.o_hs;
+  r.heads = p.heads, r.dims = p.dims, r.head_dim = p.head_dim;
+  r.interleaved = p.interleaved, r.copy = p.copy;
+  r.gain = p.gain, r.sign = 1.0f;
+  r.s = p.s;
+  r.s.status = nullptr;  // the keys' blocks report what is wrong with the lengths
+  return r;
+}
+
 template <int D, typename T, typename Params>
 int launch(Params p, bool one, int64_t slots, int device, cudaStream_t stream) {
   int units = 2 * p.s.kv_heads;
@@ -599,16 +642,29 @@ int launch(Params p, bool one, int64_t slots, int device, cudaStream_t stream) {
   constexpr int ROOM = 200 * 1024;
   if (smem > ROOM) smem /= 2, p.units = 1;  // no second buffer, so no second unit (f32 pages of 128 KB)
   constexpr int MOST = MOST_THREADS<D, T>;
-  const auto run = [&](auto kernel, KernelSetup &setup, int by) {
-    const int rc = setup.ready("emmy_kv8_append", kernel, device, std::min(ROOM, 2 * 8 * 16 * MOST));
-    if (rc != EMMY_OK) return rc;
-    return launch_kernel("emmy_kv8_append", kernel, dim3(unsigned(slots), (units + p.units - 1) / p.units), by * threads, smem,
-                         stream, p);
-  };
-  static KernelSetup setup[10];
+  const int page_blocks = (units + p.units - 1) / p.units;
   if constexpr (std::is_same<Params, RotatedParams>::value) {
+    MixedParams m;
+    m.kv = p;
+    m.page_blocks = page_blocks;
+    if (slots * page_blocks > 0x7fffffff) return fail(EMMY_EINVAL, "emmy_kv8_append_rotated", "too many tokens and heads");
+    m.kv_blocks = m.blocks = int(slots * page_blocks);
+    const auto run = [&](auto kernel, KernelSetup &setup, int by) {
+      const int rc = setup.ready("emmy_kv8_append_rotated", kernel, device, std::min(ROOM, 2 * 8 * 16 * MOST));
+      if (rc != EMMY_OK) return rc;
+      return launch_kernel("emmy_kv8_append_rotated", kernel, dim3(m.blocks), by * threads, smem, stream, m);
+    };
+    static KernelSetup setup[9];
     const auto pick = [&](auto mode, KernelSetup *of) {
       constexpr int M = decltype(mode)::value;
+      const int by = 2 * threads <= 512 ? 2 : 1;
+      if constexpr (M != ANY)
+        if (mixes<T>(p)) {
+          m.q = query_rows(p);
+          const int64_t rows = rotary::shape_blocks<Vec<T>::N, M == NEIGHBOURS>(m.q, by * threads);
+          if (m.kv_blocks + rows > 0x7fffffff) return fail(EMMY_EINVAL, "emmy_kv8_append_rotated", "too many tokens and heads");
+          m.blocks = int(m.kv_blocks + rows);
+        }
       if (2 * threads <= 256) return run(append_turned_kernel<D, T, M, 2, 256>, of[0], 2);
       if (2 * threads <= 512) return run(append_turned_kernel<D, T, M, 2, 512>, of[1], 2);
       return run(append_turned_kernel<D, T, M, 4, MOST>, of[2], 1);
@@ -617,7 +673,10 @@ int launch(Params p, bool one, int64_t slots, int device, cudaStream_t stream) {
     if (p.positions == nullptr && p.dims / 2 % Vec<T>::N == 0) return pick(std::integral_constant<int, HALVES>(), setup + 3);
     return pick(std::integral_constant<int, ANY>(), setup + 6);
   } else {
-    return run(append_kernel<D, T>, setup[9], 1);
+    static KernelSetup setup;
+    const int rc = setup.ready("emmy_kv8_append", append_kernel<D, T>, device, std::min(ROOM, 2 * 8 * 16 * MOST));
+    if (rc != EMMY_OK) return rc;
+    return launch_kernel("emmy_kv8_append", append_kernel<D, T>, dim3(unsigned(slots), page_blocks), threads, smem, stream, p);
   }
 }
 
@@ -701,6 +760,8 @@ extern "C" int emmy_kv8_append_rotated(const emmy_kv8 *cache, emmy_dptr k, emmy_
   p.wide = a->wide != 0;
   p.dims = rotary->dims, p.interleaved = rotary->interleaved != 0, p.gain = rotary->gain;
   p.heads = a->heads;
+  p.head_dim = cache->head_dim;
+  p.copy = a->q != a->q_out;
   if (a->heads > 0) {
     if (a->q == 0 || a->q_out == 0) return fail(EMMY_EINVAL, what, "null q or q_out");
     if (a->out_dtype != EMMY_KV8_F32 && a->out_dtype != EMMY_KV8_BF16 && a->out_dtype != EMMY_KV8_F16)
@@ -730,18 +791,11 @@ extern "C" int emmy_kv8_append_rotated(const emmy_kv8 *cache, emmy_dptr k, emmy_
     p.out_type = a->out_dtype;
   }
   const int rc2 = append(what, p, cache, dtype, stream);
-  if (rc2 != EMMY_OK || a->heads == 0 || cache->max_q == 1) return rc2;
-  rotary::Params r;
-  for (int i = 0; i < EMMY_ROTARY_PAIRS; ++i) r.frequency[i] = rotary->turns[i];
-  r.x = p.q, r.out = p.out;
-  r.positions = p.positions, r.position_stride = p.position_stride, r.wide = p.wide;
-  r.first = 0, r.tokens = cache->tokens;
-  r.x_ts = p.q_ts, r.x_hs = p.q_hs, r.o_ts = p.o_ts, r.o_hs = p.o_hs;
-  r.heads = p.heads, r.dims = p.dims, r.head_dim = cache->head_dim;
-  r.interleaved = p.interleaved, r.copy = a->q != a->q_out;
-  r.gain = p.gain, r.sign = 1.0f;
-  r.s = p.s;
-  r.s.status = nullptr;  // what is wrong with the lengths is reported already
+  if (rc2 != EMMY_OK || a->heads == 0 || cache->max_q == 1 || (dtype == EMMY_KV8_F32    ? mixes<float>(p)
+                                                               : dtype == EMMY_KV8_BF16 ? mixes<__nv_bfloat16>(p)
+                                                                                        : mixes<__half>(p)))
+    return rc2;
+  rotary::Params r = query_rows(p);
   const OnDevice on(cache->device);
   if (on.err != cudaSuccess) return cuda_fail(what, on.err);
   return rotary::rotate_rows(what, r, dtype, a->out_dtype, static_cast<cudaStream_t>(stream));

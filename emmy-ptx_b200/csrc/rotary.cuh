@@ -203,4 +203,104 @@ __device__ __forceinline__ void turn_neighbours(const Piece<T, N> &a, const floa
   }
 }
 
+// Heads of a thread: as many as are eight loads.
+template <bool INTERLEAVED>
+constexpr int heads_of = INTERLEAVED ? 8 : 4;
+
+// Place of a new token in its sequence; false: it is in none that can be.
+__device__ __forceinline__ bool place_of(const kv8::Seqs &s, int64_t token, int64_t &place) {
+  int lo = 0, hi = s.seqs - 1;  // the last sequence that begins at or before it
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s.q_starts[mid] <= token) lo = mid; else hi = mid - 1;
+  }
+  int start, n, len;
+  kv8::lengths(s, lo, start, n, len);
+  place = len - n + token - start;
+  return token >= start && token < int64_t(start) + n;
+}
+
+// The work of one block of `threads` threads.
+template <typename T, typename U, int N, bool INTERLEAVED>
+__device__ __forceinline__ void rotate_block(const Params &p, int64_t block, int threads) {
+  using P = Piece<T, N>;
+  using O = Piece<U, N>;
+  constexpr int HEADS = heads_of<INTERLEAVED>;
+  constexpr int PAIRS = INTERLEAVED ? N / 2 : N;  // that a thread holds
+  for (int t = threadIdx.x; t < p.block_tokens * p.width; t += threads) {
+    const int sub = t / p.width, of_token = t - sub * p.width, slice = of_token / p.pieces, piece = of_token - slice * p.pieces;
+    const int64_t token = block * p.block_tokens + sub;
+    if (token >= p.tokens) return;
+    // single values of an interleaved row: pairs are neighbours all the same
+    const bool near = N == 1 && p.interleaved, turned = piece < p.turned;
+    const int at = !turned ? p.dims + (piece - p.turned) * N : near ? 2 * piece : piece * N;
+    const int other = at + (near ? 1 : p.dims / 2);
+    const T *x = static_cast<const T *>(p.x) + token * p.x_ts;
+    U *out = static_cast<U *>(p.out) + token * p.o_ts;
+    // on their way while the position is looked up and the angles are computed
+    P a[HEADS], b[INTERLEAVED ? 1 : HEADS];
+#pragma unroll
+    for (int j = 0; j < HEADS; ++j) {
+      const int h = slice + j * p.slices;
+      if (h >= p.heads) continue;
+      a[j] = *reinterpret_cast<const P *>(x + h * p.x_hs + at);
+      if constexpr (!INTERLEAVED)
+        if (turned) b[j] = *reinterpret_cast<const P *>(x + h * p.x_hs + other);
+    }
+    int64_t pos = p.first + token;
+    if (p.s.seqs > 0 && !place_of(p.s, token, pos)) continue;
+    if (p.positions != nullptr)
+      pos = p.wide ? static_cast<const int64_t *>(p.positions)[token * p.position_stride]
+                   : static_cast<const int *>(p.positions)[token * p.position_stride];
+    float c[PAIRS], s[PAIRS];
+    if (turned) {
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        turn<sizeof(U) == 4>(pos, p.frequency[piece * PAIRS + i], p.gain, c[i], s[i]);
+        s[i] *= p.sign;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < HEADS; ++j) {
+      const int h = slice + j * p.slices;
+      if (h >= p.heads) continue;
+      O u, v;
+      if (turned) {
+        if constexpr (INTERLEAVED)
+          turn_neighbours<T, U, N>(a[j], c, s, u);
+        else
+          turn_pieces<T, U, N>(a[j], b[j], c, s, u, v);
+        if constexpr (!INTERLEAVED) *reinterpret_cast<O *>(out + h * p.o_hs + other) = v;
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if constexpr (std::is_same<T, U>::value)
+            u.v[i] = a[j].v[i];
+          else
+            u.v[i] = rounded<U>(to_float(a[j].v[i]));
+        }
+      }
+      *reinterpret_cast<O *>(out + h * p.o_hs + at) = u;
+    }
+  }
+}
+
+// How a call's rows go to blocks of `threads` threads; returns how many.
+template <int N, bool INTERLEAVED>
+int64_t shape_blocks(Params &p, int threads) {
+  constexpr int HEADS = heads_of<INTERLEAVED>;
+  p.turned = INTERLEAVED ? p.dims / N : p.dims / 2 / N;
+  p.pieces = p.turned + (p.copy ? (p.head_dim - p.dims) / N : 0);
+  p.slices = (p.heads + HEADS - 1) / HEADS;
+  p.width = p.slices * p.pieces;  // at most 2^18 * 512
+  // tokens of a block: those that leave the fewest threads idle
+  p.block_tokens = 1;
+  double best = 0;
+  for (int n = 1; n <= 16 && n * int64_t(p.width) <= 4 * threads; ++n) {
+    const double used = double(n * p.width) / ((n * p.width + threads - 1) / threads * threads);
+    if (used > best + 0.05) best = used, p.block_tokens = n;
+  }
+  return (p.tokens + p.block_tokens - 1) / p.block_tokens;
+}
+
 }  // namespace rotary
