@@ -93,6 +93,7 @@ int shape_shared(const char *what, const emmy_kv8 *c, const emmy_kv8_shared *sh,
   const int64_t cap = int64_t(c->table_width) * c->page_size / 64;
   const int wave = sms * ROWS_PER_SM;
   p.max_runs = sh->max_runs, p.max_tokens = sh->max_tokens;
+  p.wide = c->head_dim == 128;
   p.cluster = 0, p.single = false;
   int64_t units;
   if (run_rows <= ROWS_MOST) {
@@ -108,7 +109,7 @@ int shape_shared(const char *what, const emmy_kv8 *c, const emmy_kv8_shared *sh,
     p.pre_target = units < sms ? sms : 0;
   }
   p.most_pre = units + p.pre_target;
-  p.target = wave;
+  p.target = p.shared == SHARED_TILES ? 2 * wave : wave;
   p.most_parts = std::min(p.target + segments, cap * segments) + (p.shared == SHARED_ROWS ? p.most_pre : 0);
   if (p.most_pre > 0x7fffffff || p.most_parts > 0x7fffffff) return fail(EMMY_EINVAL, what, "too many sequences and heads for one call");
   if (p.shared == SHARED_TILES) p.most_units = p.most_pre;

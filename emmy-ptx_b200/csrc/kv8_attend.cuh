@@ -93,6 +93,7 @@ struct PlanShape {
   int pre_target;          // that are aimed at, 0: nothing is cut
   int pre_rows;            // rows of a slot of their results
   int max_runs, max_tokens;
+  bool wide;               // heads of 128 values
 };
 
 // The record is for this call, and what it says is within the arrays.

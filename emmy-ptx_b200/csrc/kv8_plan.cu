@@ -35,6 +35,7 @@ struct PlanParams {
   int target, min_chunks, most_parts, most_units, most_joins, tile_target;
   bool spread, single;
   int most_pre, pre_target, max_runs, max_tokens;  // of shared keys
+  bool wide;                                       // heads of 128
 };
 
 __device__ __forceinline__ int warp_scan(int x, int lane) {  // inclusive
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
   if (p.pre_target > 0) {
     const int64_t share = (int64_t(pre_work) * H + p.pre_target - 1) / p.pre_target;
     const int l0 = max(int(min(share, int64_t(1) << 24)), tiles ? TILE_CUT : 2);
-    constexpr float FIXED = 10.0f, CHUNK = 1.03f, OWN = 0.46f, RESULT = 0.053f;
+    const float FIXED = p.wide ? 10.0f : 7.0f, CHUNK = p.wide ? 1.03f : 0.88f, OWN = 0.46f, RESULT = p.wide ? 0.053f : 0.027f;
     float best = 0.0f;
     limit = 0;
     int tried = l0;
@@ -387,33 +388,22 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
     if (tiles)
       p.a.units[i] = UnitRec{b, head, block * RB, r.start, r.tokens, r.keys + r.tokens, c0, c1, i, {}};
     else
-      p.a.parts[i] = PartRec{b, head, c0, c1, part, f.parts, 0, block * RB,
+      p.a.parts[i] = PartRec{b, head, c0, c1, part, f.parts, i, block * RB,
                              r.start, r.tokens, r.keys + r.tokens, min(RB, r.tokens * G - block * RB)};
   }
   // ---- parts of own keys ----
   const int first_part = tiles ? 0 : n_pre;
-  const int64_t work = int64_t(own_work) * H;
-  const int64_t share = (work + p.target - 1) / p.target;
-  const int q0 = max(p.min_chunks, int(min(share, int64_t(1) << 24)));
-  int q = q0;
-  if (!p.spread)
-    for (int t = 1; t <= 16; t += t < 4 ? 1 : t < 8 ? 2 : 4) {
-      int parts = 0, total;
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) parts += parts_of(p, chunks[i], q) * blocks[i];
-      block_scan(parts, total, sums);
-      if (int64_t(total) * H <= p.target) break;
-      q = q0 + (q0 * t + 15) / 16;
-    }
+  const int64_t share = (int64_t(own_work) * H + p.target - 1) / p.target;
+  const int q = max(p.min_chunks, int(min(share, int64_t(1) << 24)));  // chunks of a part at most
   int parts = 0, n_parts;
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) parts += parts_of(p, chunks[i], q) * blocks[i] * H;
+  for (int i = 0; i < EACH; ++i) parts += (chunks[i] + q - 1) / q * blocks[i] * H;
   int at = block_scan(parts, n_parts, sums);
   __syncthreads();  // at_of is read above
 #pragma unroll
   for (int i = 0; i < EACH; ++i)
     if (b0 + i < s.seqs) {
-      const int b = b0 + i, k = parts_of(p, chunks[i], q), lead = p.a.runs[b];
+      const int b = b0 + i, k = (chunks[i] + q - 1) / q, lead = p.a.runs[b];
       at_of[b] = at;
       ResultRec f = {0, 0, 0, 1, 0, first_part + at, k, max(blocks[i], 1)};
       if (chunks[i] > 0 && lead >= 0 && lead <= b && p.a.runs[lead] == lead && b - lead < max(p.a.runs[s.seqs + lead], 1)) {
@@ -432,7 +422,7 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
     }
   __syncthreads();
   n_parts = min(n_parts, p.most_parts - first_part);
-  for (int i = tid; i < n_parts; i += THREADS) {
+  const auto part_of = [&](int i) {
     const int b = owner_of(at_of, s.seqs, i), rel = i - at_of[b];
     const ResultRec f = p.a.results[b];
     PartRec r;
@@ -444,12 +434,28 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
     r.head = cut / k;
     r.part = cut - r.head * k;
     r.parts = k;
-    r.slot0 = 0;
+    r.slot0 = first_part + i;
     r.c0 = f.chunks + int(int64_t(c) * r.part / k);
     r.c1 = f.chunks + int(int64_t(c) * (r.part + 1) / k);
     r.row0 = block * each;
     r.rows = min(each, rows - r.row0);
-    p.a.parts[first_part + i] = r;
+    return r;
+  };
+  // the longest first, so that the last ones to start are short (by 256 steps of q)
+  constexpr int STEPS = 256;
+  __shared__ int count[STEPS];
+  if (tid < STEPS) count[tid] = 0;
+  __syncthreads();
+  const auto step_of = [&](const PartRec &r) { return int(int64_t(max(q - (r.c1 - r.c0), 0)) * (STEPS - 1) / q); };
+  for (int i = tid; i < n_parts; i += THREADS) atomicAdd(&count[step_of(part_of(i))], 1);
+  __syncthreads();
+  int n_records;
+  const int before = block_scan(tid < STEPS ? count[tid] : 0, n_records, sums);
+  if (tid < STEPS) count[tid] = before;
+  __syncthreads();
+  for (int i = tid; i < n_parts; i += THREADS) {
+    const PartRec r = part_of(i);
+    p.a.parts[first_part + atomicAdd(&count[step_of(r)], 1)] = r;
   }
   if (tid == 0)
     *p.a.plan = PlanHead{first_part + n_parts, tiles ? n_pre : 0, 0, G, p.a.window, p.a.sinks, p.a.row_limit, s.seqs, H,
@@ -463,7 +469,7 @@ PlanParams params_of(const AttendParams &a, const PlanShape &shape) {
   p.spread = shape.spread;
   p.single = shape.single;
   // a join through the workspace costs about what ten chunks do
-  p.min_chunks = shape.cluster > 0 ? 10 : shape.shared != SHARED_NONE ? 4 : 2;
+  p.min_chunks = shape.cluster > 0 ? 10 : shape.shared == SHARED_TILES ? 8 : shape.shared == SHARED_ROWS ? 4 : 2;
   p.most_parts = int(shape.most_parts);
   p.most_units = int(shape.most_units);
   p.most_joins = int(shape.most_joins);
@@ -472,6 +478,7 @@ PlanParams params_of(const AttendParams &a, const PlanShape &shape) {
   p.pre_target = shape.pre_target;
   p.max_runs = shape.max_runs;
   p.max_tokens = shape.max_tokens;
+  p.wide = shape.wide;
   return p;
 }
 

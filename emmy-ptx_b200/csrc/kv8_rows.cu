@@ -558,7 +558,7 @@ __device__ __forceinline__ void attend_part(const AttendParams &p, const CUtenso
   };
   const auto part_slot = [&](int c) { return p.partial + int64_t(g.slot0 + c) * ROWS * (D + 2); };
   // a cluster's parts stay in shared memory, behind what is joined here
-  float *const slot = CLUSTER ? join + WARPS * ROWS * LD : RESULT ? p.partial + int64_t(blockIdx.x) * ROWS * (D + 2) : part_slot(g.part);
+  float *const slot = CLUSTER ? join + WARPS * ROWS * LD : RESULT ? part_slot(0) : part_slot(g.part);
   for (int i = tid; i < rows * (D / 8); i += THREADS) {
     const int r = i / (D / 8), d = i % (D / 8) * 8;
     float m = NONE, l = 0.0f, x[8] = {};
