@@ -341,11 +341,11 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
   // it runs beside the row kernel, whose chunks of own keys take OWN us of an SM
   // each; and a result costs RESULT us to write and join.
   int limit = longest;
+  float best = 0.0f;
   if (p.pre_target > 0) {
     const int64_t share = (int64_t(pre_work) * H + p.pre_target - 1) / p.pre_target;
     const int l0 = max(int(min(share, int64_t(1) << 24)), tiles ? TILE_CUT : 2);
     const float FIXED = p.wide ? 10.0f : 7.0f, CHUNK = p.wide ? 1.03f : 0.88f, OWN = 0.46f, RESULT = p.wide ? 0.053f : 0.027f;
-    float best = 0.0f;
     limit = 0;
     int tried = l0;
     for (int t = 1; t <= 16; ++t) {
@@ -394,7 +394,9 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
   // ---- parts of own keys ----
   const int first_part = tiles ? 0 : n_pre;
   const int64_t share = (int64_t(own_work) * H + p.target - 1) / p.target;
-  const int q = max(p.min_chunks, int(min(share, int64_t(1) << 24)));  // chunks of a part at most
+  // chunks of a part at most: the start of a block costs what three chunks do, and
+  // the last blocks should not take long
+  const int q = max(max(p.min_chunks, int(best / 3.5f)), int(min(share, int64_t(1) << 24)));
   int parts = 0, n_parts;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) parts += (chunks[i] + q - 1) / q * blocks[i] * H;
