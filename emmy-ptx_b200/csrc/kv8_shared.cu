@@ -14,14 +14,13 @@ constexpr int WARPS = 8;
 template <int D, typename T>
 __global__ void __launch_bounds__(32 * WARPS) shared_join_kernel(const AttendParams p) {
   constexpr int N = D / 32;  // values of a lane
-  grid_dependency_wait();
-  const PlanHead head = *p.plan;
-  grid_dependency_done();
   const int lane = threadIdx.x & 31, heads = p.group * p.s.kv_heads;
   const int row = blockIdx.x * WARPS + (threadIdx.x >> 5), token = row / heads, h = row - token * heads;
-  if (!plan_fits(p, head, 0, 0, 0, 0) || token >= p.s.tokens) return;
-  const int b = p.seq_of[token];
-  if (b < 0 || b >= p.s.seqs) return;
+  grid_dependency_wait();
+  const PlanHead head = *p.plan;
+  const int b = token < p.s.tokens ? p.seq_of[token] : -1;
+  grid_dependency_done();
+  if (!plan_fits(p, head, 0, 0, 0, 0) || b < 0 || b >= p.s.seqs) return;
   const ResultRec f = p.results[b];
   int start, n, len;
   lengths(p.s, b, start, n, len);
