@@ -346,21 +346,23 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
     const int64_t share = (int64_t(pre_work) * H + p.pre_target - 1) / p.pre_target;
     const int l0 = max(int(min(share, int64_t(1) << 24)), tiles ? TILE_CUT : 2);
     const float FIXED = p.wide ? 10.0f : 7.0f, CHUNK = p.wide ? 1.03f : 0.88f, OWN = 0.46f, RESULT = p.wide ? 0.053f : 0.027f;
-    limit = 0;
-    int tried = l0;
-    for (int t = 1; t <= 16; ++t) {
-      int parts = 0, total;
+    // parts for l0 chunks, and for an eighth more each time
+    constexpr int TRIES = 16;
+    __shared__ int parts_for[TRIES];
+    if (tid < TRIES) parts_for[tid] = 0;
+    __syncthreads();
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) parts += pre_blocks[i] * ((pre_chunks[i] + tried - 1) / tried);
-      block_scan(parts, total, sums);
-      const bool fits = int64_t(total) * H <= p.pre_target;
-      if (fits || t == 16) {
-        const float n = float(total) * H, tile = FIXED + CHUNK * tried;
-        const float ends = fmaxf(tile, (n * tile + OWN * own_work * H) / p.pre_target) + RESULT * n;
-        if (limit == 0 || (tiles && ends < best)) limit = tried, best = ends;
-        if (!tiles) break;
-      }
-      tried += max(1, tried >> 3);
+    for (int i = 0; i < EACH; ++i)
+      if (pre_chunks[i] > 0)
+        for (int t = 0, tried = l0; t < TRIES; ++t, tried += max(1, tried >> 3))
+          atomicAdd(&parts_for[t], pre_blocks[i] * ((pre_chunks[i] + tried - 1) / tried));
+    __syncthreads();
+    limit = 0;
+    for (int t = 0, tried = l0; t < TRIES; ++t, tried += max(1, tried >> 3)) {
+      const float n = float(parts_for[t]) * H, tile = FIXED + CHUNK * tried;
+      if (n > p.pre_target && t < TRIES - 1) continue;
+      const float ends = fmaxf(tile, (n * tile + OWN * own_work * H) / p.pre_target) + RESULT * n;
+      if (limit == 0 || (tiles && ends < best)) limit = tried, best = ends;
     }
   }
   int pre = 0;
