@@ -109,7 +109,8 @@ int shape_shared(const char *what, const emmy_kv8 *c, const emmy_kv8_shared *sh,
     p.pre_target = units < sms ? sms : 0;
   }
   p.most_pre = units + p.pre_target;
-  p.target = p.shared == SHARED_TILES ? 2 * wave : wave;
+  // (more segments than blocks that fit: parts of thirds of a block's share even out)
+  p.target = p.spread ? 3 * wave : p.shared == SHARED_TILES ? 2 * wave : wave;
   p.most_parts = std::min(p.target + segments, cap * segments) + (p.shared == SHARED_ROWS ? p.most_pre : 0);
   if (p.most_pre > 0x7fffffff || p.most_parts > 0x7fffffff) return fail(EMMY_EINVAL, what, "too many sequences and heads for one call");
   if (p.shared == SHARED_TILES) p.most_units = p.most_pre;

@@ -56,7 +56,14 @@ PAGE_SIZES = (64, 128, 256)
 MAX_SEQS = 4096
 MAX_PAIRS = 480            # pages a launch of copy_pages takes
 WORKSPACE_ZERO = 16384     # bytes of a workspace that start as zeros
-MIN_SAVED = 1              # keys not read again that a run is to save at least
+# Reads of 64 keys of a kv head that sharing is to save a batch, by head_dim.  It costs
+# a kernel more, a block of query rows for keys that few sequences share, and some
+# balance.  Measured, us shared | not, one token each, 4 query heads a kv head, own keys
+# 50-600: d = 128, 8 kv heads: 4 sequences behind 4096 keys (1536 reads saved) 14 | 12,
+# 8 (3584) 18.4 | 18.8, 16 (7680) 18.5 | 24.7, 64 (32256) 28 | 79; 64 behind 256 (2016)
+# 20.6 | 20.4, behind 1024 (8064) 24 | 31.5.  d = 64, 2 kv heads, 8 query heads each: 8
+# behind 16384 (3584) 17 | 15, 16 (7680) 18 | 21, 64 behind 4096 (8064) 19 | 20.
+MIN_SAVED = {64: 6000, 128: 4000}
 PER_THREAD = 2             # the per-thread default stream's handle
 
 STATUS = {0x401: "a page number outside the pool",
@@ -283,7 +290,7 @@ def _runs_of(table: np.ndarray, kv: np.ndarray, q: np.ndarray, page: int) -> lis
             runs.append((lo, hi - lo + 1, int(part[0])))
         else:
             runs += [(lo + first, count, n) for first, count, n in _best_runs(part.tolist())]
-    return [r for r in runs if (r[1] - 1) * r[2] * page >= MIN_SAVED]
+    return runs
 
 
 class _Pool:
@@ -429,7 +436,7 @@ class KVCache:
         ``q_lens`` new tokens of each (default 1).  Host arrays, checked
         here and copied to the device on ``stream``.  ``shared``: where
         sequences that follow one another begin with the same pages, as forks
-        do, ``attend`` reads those once for all of them."""
+        do, ``attend`` reads those once for all of them, if that saves enough."""
         return Batch(self, page_table, kv_lens, q_lens, stream, shared)
 
     def copy_pages(self, src, dst, stream=None) -> None:
@@ -618,7 +625,9 @@ class Batch:
         runs = _runs_of(table, kv, q, self.cache.page_size)
         rows = np.concatenate([[0], np.cumsum(q)])
         if first:
-            if not runs or max(rows[a + n] - rows[a] for a, n, _ in runs) == 0:
+            c = self.cache
+            saved = sum((n - 1) * pages for _, n, pages in runs) * (c.page_size // 64) * c.kv_heads
+            if not runs or saved < MIN_SAVED[c.head_dim] or max(rows[a + n] - rows[a] for a, n, _ in runs) == 0:
                 return None
             self._s = _Shared(max_runs=len(runs), max_tokens=int(max(rows[a + n] - rows[a] for a, n, _ in runs)))
         room = self._s.max_tokens

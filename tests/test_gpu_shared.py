@@ -11,6 +11,13 @@ from tests.test_gpu_kvcache import NP, cache_of, gpu  # noqa: F401 - gpu is a fi
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def share_all(monkeypatch):
+    """Sharing however little it saves."""
+    from ptxgen import kvcache
+    monkeypatch.setattr(kvcache, "MIN_SAVED", {64: 0, 128: 0})
+
+
 def layout(rng, runs, P, spare=2):
     """(table, keys, new tokens, pages) of runs [(shared keys, [(own keys, new
     tokens), ..]), ..]."""
@@ -305,3 +312,36 @@ def test_forks_generate_together(gpu):  # noqa: F811
         assert batch._s.max_runs == 1
     assert seqs.pages(ids[0])[:n // 64] == seqs.pages(ids[7])[:n // 64]
     cache.close()
+
+
+@pytest.mark.parametrize("case", [CASES[1], CASES[6], CASES[14]], ids=name)
+def test_waits_that_run_out(gpu, case):  # noqa: F811
+    """Blocks that withhold their own first keys: reported, and the batch then
+    computes as if nothing had been."""
+    from ptxgen.kvcache import WORKSPACE_ZERO
+    from ptxgen.runtime import EmmyError, load_library
+    H, G, D, P, dtype, runs = case
+    rng = np.random.default_rng(28)
+    table, kv, ql, pages = layout(rng, runs, P)
+    codes, exps = ref.pool(rng, pages, H, P, D)
+    cache, _, _ = cache_of(gpu, codes[None], exps[None])
+    q = rng.standard_normal((sum(ql), H * G, D)).astype(NP[dtype])
+    qd, od = gpu.put(q, dtype), gpu.put(np.zeros_like(q), dtype)
+    want, bound = ref.attend(codes, exps, table, kv, ql, q.astype(np.float64), D ** -0.5)
+    batch, L = cache.batch(table, kv, ql, shared=True), load_library()
+    for stall in (1, 2, 3):
+        L.emmy_kv8_wait_limit(1000000, stall)
+        try:
+            batch.attend(0, qd, od)
+        finally:
+            L.emmy_kv8_wait_limit(2000000000, 0)
+        with pytest.raises(EmmyError, match="0x403"):
+            batch.check_errors()
+        counters = np.empty(WORKSPACE_ZERO, np.uint8)
+        gpu.dev.dtoh(counters, batch._ws[0])
+        gpu.dev.sync()
+        assert not counters.any()
+        batch.attend(0, qd, od)
+        batch.check_errors()
+        assert ref.close(gpu.get(od, q.shape, NP[dtype]), want, bound, dtype)
+    batch.close()

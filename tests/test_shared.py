@@ -12,6 +12,11 @@ from ptxgen.kvcache import DeviceArray, KVSequences
 from tests.test_kvcache import dev, small  # noqa: F401 - a fixture
 
 
+@pytest.fixture(autouse=True)
+def share_all(monkeypatch):
+    monkeypatch.setattr(kv, "MIN_SAVED", {64: 0, 128: 0})
+
+
 def check(runs, alike):
     """Runs do not overlap, and share what all their sequences have in common."""
     end = 0
@@ -94,6 +99,21 @@ def test_batch_without_runs_is_as_ever(dev):  # noqa: F811
         assert batch._s is None
         batch.attend(0, DeviceArray(4096, "f16", (2, 4, 64)), DeviceArray(8192, "f16", (2, 4, 64)), stream=3)
     assert not any("shared" in n for n, _ in dev.L.calls)
+
+
+@pytest.mark.parametrize("d,seqs,pages,shares", [(128, 16, 34, True), (128, 16, 33, False), (64, 11, 300, True),
+                                                 (64, 11, 299, False), (128, 2, 500, True), (128, 1, 999, False)])
+def test_little_is_not_shared(dev, monkeypatch, d, seqs, pages, shares):  # noqa: F811
+    """(sequences - 1) * pages * kv heads reads saved, against what it costs."""
+    monkeypatch.setattr(kv, "MIN_SAVED", {64: 6000, 128: 4000})
+    heads = 8 if d == 128 and seqs > 2 else 2 if d == 64 else 8
+    cache = small(dev, pages=4000, kv_heads=heads, head_dim=d)
+    table = np.concatenate([np.tile(np.arange(pages), (seqs, 1)), 1000 + np.arange(seqs)[:, None]], 1)
+    batch = cache.batch(table, [64 * pages + 1] * seqs, stream=3, shared=True)
+    assert (batch._s is not None) == shares
+    if shares:      # what it was made for stays, however little an update saves
+        batch.update(table, [65] * seqs, stream=3)
+        assert batch._s.max_runs == 1
 
 
 def test_forks_are_runs(dev, monkeypatch):  # noqa: F811
