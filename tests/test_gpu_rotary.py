@@ -427,3 +427,73 @@ def test_steps_of_generation(gpu):  # noqa: F811
         tol += 2.0 ** -8 * (np.abs(want) + tol) + 2.0 ** -10 * np.abs(v).max()   # weights in f16, bf16 outputs
         for got in outs:
             assert (np.abs(got[:, h] - want) <= tol).all()
+
+
+def test_append_graph(gpu):  # noqa: F811
+    """A captured append replays with the lengths, positions and rows of the replay,
+    for single tokens and for pages; rows behind the last sequence stay."""
+    import torch
+    rng = np.random.default_rng(16)
+    H, G, D, P = 2, 2, 64, 64
+    rot = rotary(D, 48, False)
+    side = torch.cuda.Stream()
+    for first, later in (([(70, 1), (3, 1)], [(71, 1), (64, 0)]), ([(70, 60), (3, 3)], [(100, 30), (90, 31)])):
+        codes, exps = kv8.pool(rng, 6, H, P, D)
+        cache, c, e = cache_of(gpu, codes[None], exps[None])
+        gpu.dev.sync()
+        table = np.array([[5, 0], [2, 4]], np.int32)
+        T = sum(m for _, m in first)
+        batch = cache.batch(table, [n for n, _ in first], [m for _, m in first], stream=side)
+        k, v = (torch.randn((T, H, D), device="cuda").half() for _ in range(2))
+        q, pos = torch.randn((T, H * G, D), device="cuda").half(), torch.zeros(T, dtype=torch.int32, device="cuda")
+        out = torch.zeros_like(q)
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            batch.append(0, k, v, stream=side, rotary=rot, q=q, q_out=out, positions=pos)
+        assert gpu.get(c, codes.shape, np.uint8).tobytes() == codes.tobytes()
+        for seqs, shift in ((first, 0), (later, 1 << 20)):
+            gpu.dev.htod(c.ptr, codes)
+            gpu.dev.htod(e.ptr, exps)
+            gpu.dev.sync()
+            n = sum(m for _, m in seqs)
+            place = np.concatenate([np.arange(a - b, a) for a, b in seqs]) + shift
+            batch.update(table, [a for a, _ in seqs], [b for _, b in seqs], stream=side)
+            pos[:n] = torch.from_numpy(place.astype(np.int32)).cuda()
+            k.copy_(torch.randn_like(k))
+            out.fill_(77)
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                graph.replay()
+            batch.check_errors(stream=side)
+            want, bound = ref.rotate(rot, q[:n].cpu().numpy(), place, to="16")
+            assert ref.close(out[:n].cpu().numpy(), want, bound, "f16") and (out[n:] == 77).all()
+            turned, bound = ref.rotate(rot, k[:n].cpu().numpy(), place, to="8")
+            want_c, want_e = kv8.append(codes, exps, table, [a for a, _ in seqs], [b for _, b in seqs], turned,
+                                        v[:n].cpu().numpy().astype(np.float64))
+            got_c, got_e = gpu.get(c, codes.shape, np.uint8), gpu.get(e, exps.shape, np.int8)
+            assert (got_e == want_e).all() and (got_c[:, 1] == want_c[:, 1]).all()
+            # a code may round to either side of a border that the bound reaches over
+            off = np.abs(kv8.DECODE[got_c[:, 0]] - kv8.DECODE[want_c[:, 0]])
+            assert (off <= 2.0 ** -3 * np.abs(kv8.DECODE[want_c[:, 0]]) + 2.0 ** -9).all() and (off > 0).mean() < 1e-3
+        torch.cuda.synchronize()
+        del graph
+        batch.close()
+
+
+def test_many_heads_and_wide_strides(gpu):  # noqa: F811
+    """Offsets of rows and heads past 2^31 bytes."""
+    import torch
+    rot = rotary(8, 8, False)
+    x = torch.empty((3, (1 << 30) + 64), dtype=torch.bfloat16, device="cuda")
+    step = 1 << 29
+    view = x.as_strided((3, 3, 8), ((1 << 30) + 64, step, 1))
+    view.copy_(torch.randn((3, 3, 8), device="cuda").bfloat16())
+    host = view.float().cpu().numpy()
+    out = torch.empty((3, 3, 8), dtype=torch.bfloat16, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    rot.rotate(view, 7, out, stream=st)
+    want, bound = ref.rotate(rot, host, 7 + np.arange(3), to="16")
+    assert ref.close(out.float().cpu().numpy(), want, bound, "bf16")
+    rot.rotate(view, 7, view, stream=st)
+    assert (view == out).all()

@@ -275,6 +275,65 @@ def test_runs_that_cannot_be(gpu):  # noqa: F811
         a._plans[H * G, 0, 0] = kept
 
 
+def test_more_runs_than_there_is_room_for(gpu):  # noqa: F811
+    """Device arrays that name more runs, or longer ones, than the call was made for:
+    those beyond are attended to by themselves."""
+    rng = np.random.default_rng(29)
+    H, G, D, P = 2, 4, 128, 64
+    for sizes in ((4, 4, 4), (12, 12, 12)):              # row kernel, tile kernel
+        runs = [(128, [(30 + i, 1) for i in range(n)]) for n in sizes]
+        table, kv, ql, pages = layout(rng, runs, P)
+        codes, exps = ref.pool(rng, pages, H, P, D)
+        cache, _, _ = cache_of(gpu, codes[None], exps[None])
+        T = len(kv)
+        q = rng.standard_normal((T, H * G, D)).astype(np.float16)
+        want, bound = ref.attend(codes, exps, table, kv, ql, q.astype(np.float64), D ** -0.5)
+        for max_runs, max_tokens in ((1, sizes[0]), (2, sizes[0]), (3, sizes[0] - 1), (3, T)):
+            batch = cache.batch(table, kv, ql, shared=True)
+            batch._s.max_runs, batch._s.max_tokens = max_runs, max_tokens
+            out = gpu.put(np.zeros_like(q), "f16")
+            batch.attend(0, gpu.put(q, "f16"), out)
+            batch.check_errors()
+            assert ref.close(gpu.get(out, q.shape, np.float16), want, bound, "f16")
+            batch.close()
+
+
+def test_most_sequences(gpu):  # noqa: F811
+    """4096 sequences in one run, and in 1024 of four."""
+    rng = np.random.default_rng(30)
+    H, G, D, P, n = 1, 2, 64, 64, 4096
+    codes, exps = ref.pool(rng, 1100, H, P, D)
+    q = rng.standard_normal((n, H * G, D)).astype(np.float16)
+    kv = [64 + 1 + i % 5 for i in range(n)]
+    for members in (n, 4):
+        table = np.stack([np.arange(n) // members % 1024, 1024 + np.arange(n) % 70], 1).astype(np.int32)
+        got = attend(gpu, codes, exps, table, kv, [1] * n, q, "f16", runs=n // members)
+        some = rng.integers(0, n, 64)
+        want, bound = ref.attend(codes, exps, table[some], [kv[i] for i in some], [1] * 64, q[some].astype(np.float64), D ** -0.5)
+        assert ref.close(got[some], want, bound, "f16")
+
+
+def test_streams_and_slices(gpu):  # noqa: F811
+    """On a stream that is not the batch's own; q and out slices of one array; layers."""
+    import torch
+    rng = np.random.default_rng(31)
+    H, G, D, P, dtype, runs = CASES[6]
+    table, kv, ql, pages = layout(rng, runs, P)
+    both = [ref.pool(rng, pages, H, P, D) for _ in range(2)]
+    cache, _, _ = cache_of(gpu, np.stack([c for c, _ in both]), np.stack([e for _, e in both]))
+    batch = cache.batch(table, kv, ql, shared=True)
+    x = torch.randn((len(ql), 2 * H * G, D), device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    q, out = x[:, :H * G], x[:, H * G:]
+    side = torch.cuda.Stream()
+    for layer, (codes, exps) in enumerate(both):
+        batch.attend(layer, q, out, stream=side)
+        batch.check_errors(stream=side)
+        want, bound = ref.attend(codes, exps, table, kv, ql, q.double().cpu().numpy(), D ** -0.5)
+        assert ref.close(out.float().cpu().numpy(), want, bound, dtype)
+    batch.close()
+
+
 def test_forks_generate_together(gpu):  # noqa: F811
     """A prompt, forks of it, and steps of all of them at once: rotated appends and
     shared attention, against the same in 64 bits over what the cache holds."""

@@ -241,3 +241,50 @@ def test_library_accepts_nothing_to_do():
     L, rot = real(), Rotary(64)
     assert L.emmy_rotate(rot._ref, C.byref(rotate_args(tokens=0, x=0, out=0)), None) == 0
     assert L.emmy_rotate(rot._ref, C.byref(rotate_args(heads=0, x=0, out=0)), None) == 0
+
+
+class RotatedArgs(C.Structure):
+    """``emmy_kv8_rotated_args``."""
+    _fields_ = [("positions", C.c_uint64), ("q", C.c_uint64), ("q_out", C.c_uint64), ("position_stride", C.c_int64),
+                ("q_strides", C.c_int64 * 2), ("out_strides", C.c_int64 * 2), ("wide", C.c_int32), ("heads", C.c_int32),
+                ("out_dtype", C.c_int32)]
+
+
+def test_packed_append_arguments():
+    a = RotatedArgs.from_buffer_copy(kv._ROTATED.pack(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11))
+    assert C.sizeof(RotatedArgs) == kv._ROTATED.size
+    assert (a.positions, a.q, a.q_out, a.position_stride, *a.q_strides, *a.out_strides, a.wide, a.heads, a.out_dtype) \
+        == tuple(range(1, 12))
+
+
+def two(a, b):
+    return (C.c_int64 * 2)(a, b)
+
+
+@pytest.mark.parametrize("kw,says", [
+    ({"positions": 6}, "positions must"), ({"positions": 4, "wide": 1}, "positions must"),
+    ({"heads": -1}, "heads"), ({"heads": 2 ** 20 + 1}, "heads"), ({"q": 0}, "null q"), ({"q_out": 0}, "null q"),
+    ({"out_dtype": 3}, "q_out must"), ({"q": 4096 + 8}, "16 bytes"), ({"q_out": (1 << 20) + 8}, "16 bytes"),
+    ({"q_strides": two(260, 64)}, "16 bytes"), ({"out_strides": two(256, 68)}, "16 bytes"),
+    ({"q_strides": two(-256, 64)}, "negative"), ({"out_strides": two(64, 64)}, "rows of q_out"),
+    ({"q_out": 4096 + 128}, "q_out overlaps"), ({"q_out": 4096, "out_dtype": 2}, "q_out overlaps"),
+    ({"q_out": 4096, "out_strides": two(512, 64)}, "q_out overlaps"),
+    ({"q_out": 1 << 24}, "q_out overlaps"), ({"q_out": (1 << 25) - 64}, "q_out overlaps"),      # k, v
+])
+def test_library_append_refusals(kw, says):
+    """The C entry itself, before it touches a device: q and q_out of 4 heads."""
+    L = real()
+    cache = kv._Cache(codes=4096, exps=4096, page_table=4096, kv_lens=4096, q_starts=4096, status=0, device=0,
+                      pages=9, kv_heads=2, head_dim=64, page_size=64, seqs=4, table_width=2, tokens=4, max_q=1)
+    a = RotatedArgs(0, 4096, 1 << 20, 0, two(256, 64), two(256, 64), 0, 4, 1)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    rot, st = Rotary(64), two(128, 64)
+    call = lambda cache, rot, a: L.emmy_kv8_append_rotated(C.byref(cache), 1 << 24, 1 << 25, 1, st, st, rot, a, None)  # noqa: E731
+    assert call(cache, rot._ref, C.byref(a)) == -3 and says.encode() in L.emmy_last_error()
+    for bad in (None, Rotary(128)._ref):
+        assert call(cache, bad, C.byref(a)) == -3 and b"rotary" in L.emmy_last_error()
+    assert call(cache, rot._ref, None) == -3
+    cache.tokens = cache.max_q = 0          # nothing to do
+    if says in ("16 bytes", "q_out must", "null q", "negative", "rows of q_out", "q_out overlaps"):
+        assert call(cache, rot._ref, C.byref(a)) == 0
