@@ -560,36 +560,70 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
   } else if (lane < LPR)
     v.load(static_cast<const T *>(side ? p.x[1] : p.x[0]) + start * (side ? p.ts[1] : p.ts[0]) +
            head * (side ? p.hs[1] : p.hs[0]) + lane * V::N);
+  const bool bad = page < 0 || page >= s.pages;
+  const int64_t unit = (int64_t(bad ? 0 : page) * 2 + side) * s.kv_heads + head;
+  const int lo = (len - 1) & ((1 << s.page_shift) - 1);
+  const int held = lo > 0 && !query ? p.exps[unit] : 0;
   float turned[V::N];
   bool turn = false;
   if constexpr (ROTATED) {
     turn = unit_of_seq < s.kv_heads || query;
     if (turn) {
+      constexpr int N = V::N;
+      const int col = lane * N, half = p.dims / 2;
+      // pieces whose values pair up with each other's or within: angles while the
+      // values are on their way
+      const bool whole = (p.interleaved || half % N == 0) && !(query && p.out_type == EMMY_KV8_F32), low = col < half;
+      const int64_t pos = position_of(p, start, len - 1);
+      float c[N], sn[N];
+      if (whole && lane < LPR && col < p.dims) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (p.interleaved && j % 2 == 1) continue;
+          const int pair = p.interleaved ? (col + j) / 2 : (low ? col : col - half) + j;
+          rotary::turn<false>(pos, p.frequency[pair], p.gain, c[j], sn[j]);
+        }
+      }
       __shared__ uint4 rows[4][LPR];
       uint4 *row = rows[threadIdx.x >> 5];
       if (lane < LPR) row[lane] = v.w;
       __syncwarp();
       if (lane < LPR) {
-        const int64_t pos = position_of(p, start, len - 1);
-        if (query && p.out_type == EMMY_KV8_F32)
-          turn_apart<true>(p, reinterpret_cast<const T *>(row), lane * V::N, pos, turned);
-        else
-          turn_apart<false>(p, reinterpret_cast<const T *>(row), lane * V::N, pos, turned);
+        if (!whole) {
+          if (query && p.out_type == EMMY_KV8_F32)
+            turn_apart<true>(p, reinterpret_cast<const T *>(row), col, pos, turned);
+          else
+            turn_apart<false>(p, reinterpret_cast<const T *>(row), col, pos, turned);
+        } else {
+          V other;
+          other.w = p.interleaved || col >= p.dims ? v.w : row[(low ? col + half : col - half) / N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            turned[j] = v.at(j);
+            if (p.interleaved) {
+              if (j % 2 == 1 && col + j < p.dims) {
+                const float x = v.at(j - 1), y = v.at(j);
+                turned[j - 1] = x * c[j - 1] - y * sn[j - 1];
+                turned[j] = x * sn[j - 1] + y * c[j - 1];
+              }
+            } else if (col < p.dims) {
+              turned[j] = turned[j] * c[j] + other.at(j) * (low ? -sn[j] : sn[j]);
+            }
+          }
+        }
       }
       if (query) {
-        if (lane < LPR) store_query(p, start, unit_of_seq - 2 * s.kv_heads, lane * V::N, turned);
+        if (lane < LPR) store_query(p, start, unit_of_seq - 2 * s.kv_heads, col, turned);
         return;
       }
     }
   }
-  if (page < 0 || page >= s.pages) {
+  if (bad) {
     report(s.status, STATUS_PAGE);
     return;
   }
-  const int64_t unit = (int64_t(page) * 2 + side) * s.kv_heads + head;
   uint8_t *codes = p.codes + (unit << s.page_shift) * D;
-  const int lo = (len - 1) & ((1 << s.page_shift) - 1);
-  const int old = lo > 0 ? held_exponent(p.exps[unit]) : E_MIN;
+  const int old = lo > 0 ? held_exponent(held) : E_MIN;
   const float amax = turn && lane < LPR ? max_finite(turned, 0.0f) : max_finite(v, 0.0f);
   const int e = fit_exponent(warp_max(amax), old);
   if (lane == 0) p.exps[unit] = int8_t(e);
