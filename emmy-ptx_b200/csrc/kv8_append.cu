@@ -538,6 +538,13 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
   using V = Vec<T>;
   constexpr int LPR = D / V::N;
   const Seqs &s = p.s;
+  // (lanes read other frequencies each, which kernel parameters serve one by one:
+  // once a block, while the kernel before this one ends)
+  __shared__ uint64_t frequency[ROTATED ? D / 2 : 1];
+  if constexpr (ROTATED) {
+    if (threadIdx.x < D / 2) frequency[threadIdx.x] = p.frequency[threadIdx.x];
+    __syncthreads();
+  }
   grid_dependency_wait();
   grid_dependency_done();
   const int b = blockIdx.x, unit_of_seq = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -581,7 +588,7 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
         for (int j = 0; j < N; ++j) {
           if (p.interleaved && j % 2 == 1) continue;
           const int pair = p.interleaved ? (col + j) / 2 : (low ? col : col - half) + j;
-          rotary::turn<false>(pos, p.frequency[pair], p.gain, c[j], sn[j]);
+          rotary::turn<false>(pos, frequency[pair], p.gain, c[j], sn[j]);
         }
       }
       __shared__ uint4 rows[4][LPR];
