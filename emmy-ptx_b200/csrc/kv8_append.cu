@@ -355,11 +355,16 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
   __shared__ float part[2][32];
   __shared__ __align__(16) float steps_c[MODE == ANY ? 1 : ROWS][D / 2], steps_s[MODE == ANY ? 1 : ROWS][D / 2];
   const Seqs &s = p.s;
+  // (lanes read other frequencies each, which kernel parameters serve one by one)
+  __shared__ uint64_t frequency[D / 2];
+  if (threadIdx.x < D / 2) frequency[threadIdx.x] = p.frequency[threadIdx.x];
+  __syncthreads();
   grid_dependency_wait();
   grid_dependency_done();
   const int kv_block = blockIdx.x;
   if (kv_block >= all.kv_blocks) {
-    if constexpr (MODE != ANY) rotary::rotate_block<T, T, N, MODE == NEIGHBOURS>(all.q, kv_block - all.kv_blocks, blockDim.x);
+    if constexpr (MODE != ANY) rotary::rotate_block<T, T, N, MODE == NEIGHBOURS>(
+          all.q, [&](int i) { return frequency[i]; }, kv_block - all.kv_blocks, blockDim.x);
     return;
   }
   const int nth_page = kv_block / all.page_blocks, nth = kv_block - nth_page * all.page_blocks;
@@ -409,13 +414,13 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
   if constexpr (MODE != ANY) {
     for (int i = tid; i < ROWS * (D / 2); i += threads) {
       const int row = i / (D / 2), pair = i % (D / 2);
-      rotary::turn_of(int64_t(row) * step, p.frequency[pair], steps_c[row][pair], steps_s[row][pair]);
+      rotary::turn_of(int64_t(row) * step, frequency[pair], steps_c[row][pair], steps_s[row][pair]);
     }
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
       float c[2], s[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) rotary::turn<false>(pos0 + row0, p.frequency[min(pair_at(j + i), D / 2 - 1)], p.gain, c[i], s[i]);
+      for (int i = 0; i < 2; ++i) rotary::turn<false>(pos0 + row0, frequency[min(pair_at(j + i), D / 2 - 1)], p.gain, c[i], s[i]);
       first_c[j / 2] = two(c[0], c[1]);
       first_s[j / 2] = two(s[0], s[1]);
     }

@@ -220,9 +220,9 @@ __device__ __forceinline__ bool place_of(const kv8::Seqs &s, int64_t token, int6
   return token >= start && token < int64_t(start) + n;
 }
 
-// The work of one block of `threads` threads.
-template <typename T, typename U, int N, bool INTERLEAVED>
-__device__ __forceinline__ void rotate_block(const Params &p, int64_t block, int threads) {
+// The work of one block of `threads` threads; frequency(i) is pair i's.
+template <typename T, typename U, int N, bool INTERLEAVED, typename F>
+__device__ __forceinline__ void rotate_block(const Params &p, const F &frequency, int64_t block, int threads) {
   using P = Piece<T, N>;
   using O = Piece<U, N>;
   constexpr int HEADS = heads_of<INTERLEAVED>;
@@ -256,7 +256,7 @@ __device__ __forceinline__ void rotate_block(const Params &p, int64_t block, int
     if (turned) {
 #pragma unroll
       for (int i = 0; i < PAIRS; ++i) {
-        turn<sizeof(U) == 4>(pos, p.frequency[piece * PAIRS + i], p.gain, c[i], s[i]);
+        turn<sizeof(U) == 4>(pos, frequency(piece * PAIRS + i), p.gain, c[i], s[i]);
         s[i] *= p.sign;
       }
     }
