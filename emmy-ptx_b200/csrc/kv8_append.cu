@@ -17,10 +17,15 @@
 // emmy_kv8_append_rotated -- the same of keys turned to their positions on the
 // way, in f32 and unrounded, and queries turned into an array of their own: where
 // no sequence has more than one new token they are more (query head)s behind the
-// (side, head)s, else rows for the kernel of emmy_rotate.  In a page's rows a key's
-// angle is that of a thread's first row and a multiple of the rows between:
-// cos(a + b) = cos a cos b - sin a sin b, with the first angle in registers and the
-// multiples' in shared memory, 4 products a pair instead of 40 instructions.
+// (side, head)s, else blocks behind the pages' that do what emmy_rotate does.  In a
+// page's rows a key's angle is that of a thread's first row and a multiple of the rows
+// between: cos(a + b) = cos a cos b - sin a sin b, with the first angle in registers
+// and the multiples' in shared memory, 4 products a pair (an angle's function each
+// value: 854 us, so 173, for the case below).  Sines and cosines are good to 2^-18 of
+// the values, whose codes are rounded by 2^-4.  41536 tokens in 6 sequences, 8 heads
+// and 32 query heads of 128, bf16: 147 us, 6.2 TB/s; the queries' blocks mixed with
+// the pages' 164, before them 160, in a launch of their own 157.  One token 2.3 us, 64
+// of as many sequences 3.3.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -268,7 +268,7 @@ __device__ __forceinline__ float magnitude(uint32_t bits) {  // of one value, bi
 // A unit's query rows as put_query does them, where a part has few chunks: four lanes
 // do four rows together, each its 16-byte pieces of all, with no exchange but that of
 // the maxima, two values an instruction (a thread a row, pieces transposed: 5.2 us
-// from the barriers to the first product's operands, so 2.9).
+// from the barriers to the first product's operands, so 3.6).
 template <int D, typename T>
 __device__ __forceinline__ float put_queries_of_four(const AttendParams &p, uint8_t *tile, int r, int lane, int64_t mine, uint64_t *full) {
   constexpr int PIECES = D / 32;  // of a row, a lane
@@ -870,7 +870,7 @@ __global__ void __launch_bounds__(THREADS, 1) tiles_kernel(const AttendParams p)
         const uint32_t *bits = reinterpret_cast<const uint32_t *>(dyn + L::NAN_ROWS + (x * TILE + r) * (D / 8));
         if constexpr (SHARED) {
           // O, row after row, four lanes 64 bytes of one together.  A loop: code that
-          // a block runs once comes from memory (unrolled: 6.2 us, so 2.0).
+          // a block runs once comes from memory (unrolled: 6.2 us a block, so 2.8).
           float *to = p.tile_partial + int64_t(slot) * (D + 2) * (2 * TILE) + (x * TILE + (r & ~3)) * D + 4 * (lane & 3);
 #pragma unroll 1
           for (int c = 0; c < D; c += 16, to += 16) {

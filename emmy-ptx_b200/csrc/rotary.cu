@@ -9,7 +9,11 @@
 // Bound by memory: each value is read and written once.  A thread holds one piece
 // (16 bytes, or less where sizes or addresses ask for it) of a token's row, with
 // the piece that it is paired with, and does the same of HEADS heads: their angles
-// are computed once, while the values are on their way.
+// are computed once, while the values are on their way (8191 tokens of 32 heads of
+// 128, bf16: 34 us with the loads behind the angles, 24 before them, 22 with sines and
+// cosines of 16-bit results from the special function unit; a copy takes 20.5).
+// 32768 tokens of 16 heads: 40.5 us, 6.6 TB/s; 4093 of 20 heads of 80, f32, which stay
+// in L2: 8.6 us; one token: 2.3.
 #include "rotary.cuh"
 
 namespace rotary {

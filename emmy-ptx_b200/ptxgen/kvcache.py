@@ -159,7 +159,7 @@ def _positions(positions, tokens: int, ordinal: int) -> tuple[int, int, int, int
         return ptr(), positions.stride()[0], code - 5, 0
     try:
         first = positions.__index__()
-    except AttributeError:
+    except (AttributeError, TypeError):
         raise EmmyError("positions is a device array, or a whole number") from None
     if not -2 ** 63 <= first <= 2 ** 63 - 1 - tokens:
         raise EmmyError("positions must fit 64 bits")
@@ -278,8 +278,9 @@ def _runs_of(table: np.ndarray, kv: np.ndarray, q: np.ndarray, page: int) -> lis
     most = np.minimum(before[1:], before[:-1])
     if not most.any():
         return []
-    other = table[1:] != table[:-1]
-    alike = np.where(other.any(1), other.argmax(1), table.shape[1])
+    width = int(most.max())
+    other = table[1:, :width] != table[:-1, :width]
+    alike = np.where(other.any(1), other.argmax(1), width)
     alike = np.minimum(alike, most)
     # stretches between pairs that have nothing in common
     edge = np.flatnonzero(np.diff(np.concatenate([[0], alike > 0, [0]])))

@@ -116,6 +116,7 @@ X = (5, 3, 64)
     (arr(X), 0, arr(X, strides=(384, 128, 2)), "contiguous"), (arr(X), 0, arr(X, device=1), "one device"),
     (arr(X), arr((4,), "i32"), arr(X), "positions has shape"), (arr(X), arr((5, 1), "i32"), arr(X), "positions has shape"),
     (arr(X), arr((5,), "f32"), arr(X), "int32 or int64"), (arr(X), arr((5,), "i64", device=1), arr(X), "not on device"),
+    (arr(X), np.arange(5), arr(X), "whole number"), (arr(X), None, arr(X), "whole number"),
     (arr(X), 1.5, arr(X), "whole number"), (arr(X), [1, 2, 3, 4, 5], arr(X), "whole number"),
     (arr(X), 2 ** 63 - 3, arr(X), "64 bits"),
 ])
