@@ -151,9 +151,11 @@ __device__ __forceinline__ int64_t position_of(const RotatedParams &p, int64_t t
                 : static_cast<const int *>(p.positions)[token * p.position_stride];
 }
 
-// Values col .. col + 15 bytes of a row in shared memory, turned one by one.
+// Values col .. col + 15 bytes of a row in shared memory, as the frequencies are,
+// turned one by one.
 template <bool EXACT, typename T>
-__device__ __forceinline__ void turn_apart(const RotatedParams &p, const T *row, int col, int64_t pos, float *y) {
+__device__ __forceinline__ void turn_apart(const RotatedParams &p, const uint64_t *frequency, const T *row, int col, int64_t pos,
+                                           float *y) {
   const int half = p.dims / 2;
 #pragma unroll
   for (int i = 0; i < Vec<T>::N; ++i) {
@@ -163,7 +165,7 @@ __device__ __forceinline__ void turn_apart(const RotatedParams &p, const T *row,
     const bool low = p.interleaved ? at % 2 == 0 : at < half;
     const int away = p.interleaved ? 1 : half, other = low ? at + away : at - away;
     float c, s;
-    rotary::turn<EXACT>(pos, p.frequency[p.interleaved ? at / 2 : low ? at : other], p.gain, c, s);
+    rotary::turn<EXACT>(pos, frequency[p.interleaved ? at / 2 : low ? at : other], p.gain, c, s);
     y[i] = y[i] * c + rotary::to_float(row[other]) * (low ? -s : s);
   }
 }
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
   // angles of keys: of row row0, and of i * step rows
   uint64_t first_c[HALF], first_s[HALF];
   const auto pair_at = [&](int j) { return MODE == HALVES ? col + j : (j < HALF ? col : col2 - N) / 2 + j; };
-  if constexpr (MODE != ANY) {
+  if (MODE != ANY && (u1 - u0 > 1 || u0 % 2 == 0)) {  // there are keys
     for (int i = tid; i < ROWS * (D / 2); i += threads) {
       const int row = i / (D / 2), pair = i % (D / 2);
       rotary::turn_of(int64_t(row) * step, frequency[pair], steps_c[row][pair], steps_s[row][pair]);
@@ -455,8 +457,8 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
         float v[2 * N];
         const T *row = reinterpret_cast<const T *>(at - col / N);
         const int64_t pos = position_of(p, token0 + r, pos0 + r);
-        turn_apart<false>(p, row, col, pos, &v[0]);
-        turn_apart<false>(p, row, col2, pos, &v[N]);
+        turn_apart<false>(p, frequency, row, col, pos, &v[0]);
+        turn_apart<false>(p, frequency, row, col2, pos, &v[N]);
 #pragma unroll
         for (int j = 0; j < HALF; ++j) x[i][j] = two(v[2 * j], v[2 * j + 1]), y[i][j] = two(v[N + 2 * j], v[N + 2 * j + 1]);
       } else {
@@ -608,9 +610,9 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
       if (lane < LPR) {
         if (!whole) {
           if (query && p.out_type == EMMY_KV8_F32)
-            turn_apart<true>(p, reinterpret_cast<const T *>(row), col, pos, turned);
+            turn_apart<true>(p, frequency, reinterpret_cast<const T *>(row), col, pos, turned);
           else
-            turn_apart<false>(p, reinterpret_cast<const T *>(row), col, pos, turned);
+            turn_apart<false>(p, frequency, reinterpret_cast<const T *>(row), col, pos, turned);
         } else {
           V other;
           other.w = p.interleaved || col >= p.dims ? v.w : row[(low ? col + half : col - half) / N];
@@ -687,7 +689,8 @@ int launch(Params p, bool one, int64_t slots, int device, cudaStream_t stream) {
     return launch_kernel("emmy_kv8_append", append_one_kernel<D, T, Params>, dim3(p.s.seqs, (units + 3) / 4), 128, 0, stream, p);
   // several (side, head)s a CTA once there are more than fill the GPU twice
   const int threads = page_threads<D, T>(1 << p.s.page_shift);
-  const int64_t fill = int64_t(sm_count(device)) * 2 * (2048 / threads < 7 ? 2048 / threads : 7);
+  int64_t fill = int64_t(sm_count(device)) * 2 * (2048 / threads < 7 ? 2048 / threads : 7);
+  if constexpr (std::is_same<Params, RotatedParams>::value) fill = int64_t(sm_count(device)) * 2 * std::max(768 / (2 * threads), 1);
   p.units = int(std::min<int64_t>(units, std::max<int64_t>(1, slots * units / std::max<int64_t>(fill, 1))));
   int smem = 2 * 8 * 16 * threads;
   constexpr int ROOM = 200 * 1024;
