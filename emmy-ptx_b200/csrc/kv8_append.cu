@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
 template <typename T>
 bool mixes(const RotatedParams &p) {
   constexpr int N = Vec<T>::N;
-  return p.heads > 0 && p.positions == nullptr && p.out_type == type_of<T> && (p.interleaved ? p.dims : p.dims / 2) % N == 0;
+  return p.heads > 0 && p.positions == nullptr && p.out_type == type_of<T> && (p.interleaved || p.dims / 2 % N == 0);
 }
 
 // The queries as rows to turn.

@@ -36,10 +36,83 @@ int launch(const char *what, Params &p, cudaStream_t stream) {
   return kv8::launch_kernel(what, rotate_kernel<T, U, N, INTERLEAVED>, dim3(unsigned(blocks)), THREADS, 0, stream, p);
 }
 
+// Halves whose values pair up across pieces: rows go through shared memory, piece by
+// piece as they lie, and a thread turns its own values with those that it finds
+// there.  A block takes whole rows: so many (token, heads slice, slice + slices, ..)
+// of `pieces` threads each.  (Pairs of single values instead: 6333 tokens of 4 heads
+// of 80 with 6 turned 10 us, so MEASURED.)
+template <typename T, typename U, int N>
+__global__ void __launch_bounds__(THREADS) rotate_apart_kernel(const __grid_constant__ Params p) {
+  using P = Piece<T, N>;
+  constexpr int HEADS = 4;
+  __shared__ P rows[HEADS][THREADS];
+  __shared__ uint64_t frequency[EMMY_ROTARY_PAIRS];
+  const int tid = threadIdx.x, r = tid / p.pieces, piece = tid - r * p.pieces, half = p.dims / 2;
+  if (tid < half) frequency[tid] = p.frequency[tid];
+  kv8::grid_dependency_wait();
+  kv8::grid_dependency_done();
+  const int64_t unit = int64_t(blockIdx.x) * p.block_tokens + r, token = unit / p.slices;
+  const int slice = int(unit - token * p.slices);
+  const bool real = r < p.block_tokens && token < p.tokens;
+  const T *x = static_cast<const T *>(p.x) + token * p.x_ts + piece * N;
+  U *out = static_cast<U *>(p.out) + token * p.o_ts + piece * N;
+  P a[HEADS];
+#pragma unroll
+  for (int j = 0; j < HEADS; ++j) {
+    const int h = slice + j * p.slices;
+    if (real && h < p.heads) a[j] = *reinterpret_cast<const P *>(x + h * p.x_hs);
+  }
+  __syncthreads();
+  int64_t pos = p.first + token;
+  bool placed = real;
+  if (real && p.s.seqs > 0) placed = place_of(p.s, token, pos);
+  if (real && p.positions != nullptr)
+    pos = p.wide ? static_cast<const int64_t *>(p.positions)[token * p.position_stride]
+                 : static_cast<const int *>(p.positions)[token * p.position_stride];
+  float c[N], s[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int at = piece * N + i;
+    if (at >= p.dims) break;
+    turn<sizeof(U) == 4>(pos, frequency[at < half ? at : at - half], p.gain, c[i], s[i]);
+    if ((at < half) == (p.sign > 0.0f)) s[i] = -s[i];
+  }
+#pragma unroll
+  for (int j = 0; j < HEADS; ++j)
+    if (real && slice + j * p.slices < p.heads) rows[j][tid] = a[j];
+  __syncthreads();
+  if (!placed || (!p.copy && piece * N >= p.dims)) return;
+#pragma unroll
+  for (int j = 0; j < HEADS; ++j) {
+    const int h = slice + j * p.slices;
+    if (h >= p.heads) break;
+    const T *row = reinterpret_cast<const T *>(&rows[j][r * p.pieces]);
+    Piece<U, N> u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = piece * N + i;
+      u.v[i] = at >= p.dims ? as_type<U>(a[j].v[i])
+                            : rounded<U>(to_float(a[j].v[i]) * c[i] + to_float(row[at < half ? at + half : at - half]) * s[i]);
+    }
+    *reinterpret_cast<Piece<U, N> *>(out + h * p.o_hs) = u;
+  }
+}
+
+template <typename T, typename U, int N>
+int launch_apart(const char *what, Params &p, cudaStream_t stream) {
+  p.pieces = p.head_dim / N;
+  p.slices = (p.heads + 3) / 4;
+  p.block_tokens = THREADS / p.pieces;
+  const int64_t blocks = (p.tokens * p.slices + p.block_tokens - 1) / p.block_tokens;
+  if (blocks > 0x7fffffff) return kv8::fail(EMMY_EINVAL, what, "too many tokens and heads");
+  return kv8::launch_kernel(what, rotate_apart_kernel<T, U, N>, dim3(unsigned(blocks)), THREADS, 0, stream, p);
+}
+
 template <typename T, typename U, int N>
 int launch_layout(const char *what, Params &p, cudaStream_t stream) {
   if constexpr (N > 1)
     if (p.interleaved) return launch<T, U, N, true>(what, p, stream);
+  if (!p.interleaved && p.dims / 2 % N != 0 && p.head_dim / N <= THREADS) return launch_apart<T, U, N>(what, p, stream);
   return launch<T, U, N, false>(what, p, stream);
 }
 
@@ -47,10 +120,8 @@ int launch_layout(const char *what, Params &p, cudaStream_t stream) {
 template <typename T, typename U>
 int launch_type(const char *what, Params &p, cudaStream_t stream) {
   const auto fits = [&](int n) {
-    const int half = p.interleaved ? p.dims : p.dims / 2;
     return reinterpret_cast<uintptr_t>(p.x) % (n * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.out) % (n * sizeof(U)) == 0 &&
-           p.x_ts % n == 0 && p.x_hs % n == 0 && p.o_ts % n == 0 && p.o_hs % n == 0 && half % n == 0 &&
-           (!p.copy || (p.head_dim - p.dims) % n == 0);
+           p.x_ts % n == 0 && p.x_hs % n == 0 && p.o_ts % n == 0 && p.o_hs % n == 0 && p.head_dim % n == 0;
   };
   if constexpr (sizeof(T) == 2 && sizeof(U) == 2)
     if (fits(8)) return launch_layout<T, U, 8>(what, p, stream);

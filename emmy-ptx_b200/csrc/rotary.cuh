@@ -115,6 +115,15 @@ __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float x) { retur
 template <>
 __device__ __forceinline__ __half rounded<__half>(float x) { return __float2half_rn(x); }
 
+// The same value, or rounded where the types differ.
+template <typename U, typename T>
+__device__ __forceinline__ U as_type(T x) {
+  if constexpr (std::is_same<T, U>::value)
+    return x;
+  else
+    return rounded<U>(to_float(x));
+}
+
 // Two neighbouring values of a 32-bit word, and back with one rounding each.
 template <typename T>
 __device__ __forceinline__ float2 unpacked(uint32_t w) {
@@ -233,7 +242,7 @@ __device__ __forceinline__ void rotate_block(const Params &p, const F &frequency
     if (token >= p.tokens) return;
     // single values of an interleaved row: pairs are neighbours all the same
     const bool near = N == 1 && p.interleaved, turned = piece < p.turned;
-    const int at = !turned ? p.dims + (piece - p.turned) * N : near ? 2 * piece : piece * N;
+    const int at = near && turned ? 2 * piece : INTERLEAVED || turned ? piece * N : p.dims + (piece - p.turned) * N;
     const int other = at + (near ? 1 : p.dims / 2);
     const T *x = static_cast<const T *>(p.x) + token * p.x_ts;
     U *out = static_cast<U *>(p.out) + token * p.o_ts;
@@ -266,19 +275,18 @@ __device__ __forceinline__ void rotate_block(const Params &p, const F &frequency
       if (h >= p.heads) continue;
       O u, v;
       if (turned) {
-        if constexpr (INTERLEAVED)
+        if constexpr (INTERLEAVED) {
           turn_neighbours<T, U, N>(a[j], c, s, u);
-        else
+          if (at + N > p.dims)  // the last turned ones share a piece with those behind
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+              if (at + i >= p.dims) u.v[i] = as_type<U>(a[j].v[i]);
+        } else
           turn_pieces<T, U, N>(a[j], b[j], c, s, u, v);
         if constexpr (!INTERLEAVED) *reinterpret_cast<O *>(out + h * p.o_hs + other) = v;
       } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if constexpr (std::is_same<T, U>::value)
-            u.v[i] = a[j].v[i];
-          else
-            u.v[i] = rounded<U>(to_float(a[j].v[i]));
-        }
+        for (int i = 0; i < N; ++i) u.v[i] = as_type<U>(a[j].v[i]);
       }
       *reinterpret_cast<O *>(out + h * p.o_hs + at) = u;
     }
@@ -289,8 +297,8 @@ __device__ __forceinline__ void rotate_block(const Params &p, const F &frequency
 template <int N, bool INTERLEAVED>
 int64_t shape_blocks(Params &p, int threads) {
   constexpr int HEADS = heads_of<INTERLEAVED>;
-  p.turned = INTERLEAVED ? p.dims / N : p.dims / 2 / N;
-  p.pieces = p.turned + (p.copy ? (p.head_dim - p.dims) / N : 0);
+  p.turned = INTERLEAVED ? (p.dims + N - 1) / N : p.dims / 2 / N;
+  p.pieces = !p.copy ? p.turned : INTERLEAVED ? p.head_dim / N : p.turned + (p.head_dim - p.dims) / N;
   p.slices = (p.heads + HEADS - 1) / HEADS;
   p.width = p.slices * p.pieces;  // at most 2^18 * 512
   // tokens of a block: those that leave the fewest threads idle
