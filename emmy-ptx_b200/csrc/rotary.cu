@@ -12,8 +12,8 @@
 // are computed once, while the values are on their way (8191 tokens of 32 heads of
 // 128, bf16: 34 us with the loads behind the angles, 24 before them, 22 with sines and
 // cosines of 16-bit results from the special function unit; a copy takes 20.5).
-// 32768 tokens of 16 heads: 40.5 us, 6.6 TB/s; 4093 of 20 heads of 80, f32, which stay
-// in L2: 8.6 us; one token: 2.3.
+// 32768 tokens of 16 heads: 40.6 us, 6.6 TB/s; 4093 of 20 heads of 80, f32, which stay
+// in L2: 9.2 us; one token: 2.3.
 #include "rotary.cuh"
 
 namespace rotary {
@@ -33,6 +33,7 @@ __global__ void __launch_bounds__(THREADS) rotate_kernel(const __grid_constant__
 template <typename T, typename U, int N, bool INTERLEAVED>
 int launch(const char *what, Params &p, cudaStream_t stream) {
   const int64_t blocks = shape_blocks<N, INTERLEAVED>(p, THREADS);
+  if (blocks > 0x7fffffff) return kv8::fail(EMMY_EINVAL, what, "too many tokens and heads");
   return kv8::launch_kernel(what, rotate_kernel<T, U, N, INTERLEAVED>, dim3(unsigned(blocks)), THREADS, 0, stream, p);
 }
 
@@ -40,7 +41,7 @@ int launch(const char *what, Params &p, cudaStream_t stream) {
 // piece as they lie, and a thread turns its own values with those that it finds
 // there.  A block takes whole rows: so many (token, heads slice, slice + slices, ..)
 // of `pieces` threads each.  (Pairs of single values instead: 6333 tokens of 4 heads
-// of 80 with 6 turned 10 us, so MEASURED.)
+// of 80 with 6 turned 10 us, so 5.)
 template <typename T, typename U, int N>
 __global__ void __launch_bounds__(THREADS) rotate_apart_kernel(const __grid_constant__ Params p) {
   using P = Piece<T, N>;
@@ -51,9 +52,9 @@ __global__ void __launch_bounds__(THREADS) rotate_apart_kernel(const __grid_cons
   if (tid < half) frequency[tid] = p.frequency[tid];
   kv8::grid_dependency_wait();
   kv8::grid_dependency_done();
-  const int64_t unit = int64_t(blockIdx.x) * p.block_tokens + r, token = unit / p.slices;
+  const int64_t unit = int64_t(blockIdx.x) * p.block_rows + r, token = unit / p.slices;
   const int slice = int(unit - token * p.slices);
-  const bool real = r < p.block_tokens && token < p.tokens;
+  const bool real = r < p.block_rows && token < p.tokens;
   const T *x = static_cast<const T *>(p.x) + token * p.x_ts + piece * N;
   U *out = static_cast<U *>(p.out) + token * p.o_ts + piece * N;
   P a[HEADS];
@@ -102,8 +103,8 @@ template <typename T, typename U, int N>
 int launch_apart(const char *what, Params &p, cudaStream_t stream) {
   p.pieces = p.head_dim / N;
   p.slices = (p.heads + 3) / 4;
-  p.block_tokens = THREADS / p.pieces;
-  const int64_t blocks = (p.tokens * p.slices + p.block_tokens - 1) / p.block_tokens;
+  p.block_rows = THREADS / p.pieces;
+  const int64_t blocks = (p.tokens * p.slices + p.block_rows - 1) / p.block_rows;
   if (blocks > 0x7fffffff) return kv8::fail(EMMY_EINVAL, what, "too many tokens and heads");
   return kv8::launch_kernel(what, rotate_apart_kernel<T, U, N>, dim3(unsigned(blocks)), THREADS, 0, stream, p);
 }

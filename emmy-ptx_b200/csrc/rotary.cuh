@@ -89,7 +89,8 @@ struct Params {
   int heads, dims, head_dim;
   int pieces, turned;     // pieces of a head that threads hold (with those paired with them), those turned
   int slices;             // of a token's heads: thread slice i has heads i, i + slices, ..
-  int width, block_tokens;  // threads of a token, tokens of a block
+  int width;              // threads of a token
+  int block_rows;         // rows of a block that takes whole ones
   bool wide, interleaved, copy;
   float gain, sign;
   kv8::Seqs s;            // s.seqs = 0: no sequences
@@ -236,60 +237,60 @@ __device__ __forceinline__ void rotate_block(const Params &p, const F &frequency
   using O = Piece<U, N>;
   constexpr int HEADS = heads_of<INTERLEAVED>;
   constexpr int PAIRS = INTERLEAVED ? N / 2 : N;  // that a thread holds
-  for (int t = threadIdx.x; t < p.block_tokens * p.width; t += threads) {
-    const int sub = t / p.width, of_token = t - sub * p.width, slice = of_token / p.pieces, piece = of_token - slice * p.pieces;
-    const int64_t token = block * p.block_tokens + sub;
-    if (token >= p.tokens) return;
-    // single values of an interleaved row: pairs are neighbours all the same
-    const bool near = N == 1 && p.interleaved, turned = piece < p.turned;
-    const int at = near && turned ? 2 * piece : INTERLEAVED || turned ? piece * N : p.dims + (piece - p.turned) * N;
-    const int other = at + (near ? 1 : p.dims / 2);
-    const T *x = static_cast<const T *>(p.x) + token * p.x_ts;
-    U *out = static_cast<U *>(p.out) + token * p.o_ts;
-    // on their way while the position is looked up and the angles are computed
-    P a[HEADS], b[INTERLEAVED ? 1 : HEADS];
+  // a thread a (token, heads slice, piece)
+  const int64_t at_all = block * threads + threadIdx.x, all = p.tokens * p.width;
+  if (at_all >= all) return;
+  const int64_t token = all <= 0x7fffffff ? int64_t(unsigned(at_all) / unsigned(p.width)) : at_all / p.width;
+  const int of_token = int(at_all - token * p.width), slice = of_token / p.pieces, piece = of_token - slice * p.pieces;
+  // single values of an interleaved row: pairs are neighbours all the same
+  const bool near = N == 1 && p.interleaved, turned = piece < p.turned;
+  const int at = near && turned ? 2 * piece : INTERLEAVED || turned ? piece * N : p.dims + (piece - p.turned) * N;
+  const int other = at + (near ? 1 : p.dims / 2);
+  const T *x = static_cast<const T *>(p.x) + token * p.x_ts;
+  U *out = static_cast<U *>(p.out) + token * p.o_ts;
+  // on their way while the position is looked up and the angles are computed
+  P a[HEADS], b[INTERLEAVED ? 1 : HEADS];
 #pragma unroll
-    for (int j = 0; j < HEADS; ++j) {
-      const int h = slice + j * p.slices;
-      if (h >= p.heads) continue;
-      a[j] = *reinterpret_cast<const P *>(x + h * p.x_hs + at);
-      if constexpr (!INTERLEAVED)
-        if (turned) b[j] = *reinterpret_cast<const P *>(x + h * p.x_hs + other);
+  for (int j = 0; j < HEADS; ++j) {
+    const int h = slice + j * p.slices;
+    if (h >= p.heads) continue;
+    a[j] = *reinterpret_cast<const P *>(x + h * p.x_hs + at);
+    if constexpr (!INTERLEAVED)
+      if (turned) b[j] = *reinterpret_cast<const P *>(x + h * p.x_hs + other);
+  }
+  int64_t pos = p.first + token;
+  if (p.s.seqs > 0 && !place_of(p.s, token, pos)) return;
+  if (p.positions != nullptr)
+    pos = p.wide ? static_cast<const int64_t *>(p.positions)[token * p.position_stride]
+                 : static_cast<const int *>(p.positions)[token * p.position_stride];
+  float c[PAIRS], s[PAIRS];
+  if (turned) {
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      turn<sizeof(U) == 4>(pos, frequency(piece * PAIRS + i), p.gain, c[i], s[i]);
+      s[i] *= p.sign;
     }
-    int64_t pos = p.first + token;
-    if (p.s.seqs > 0 && !place_of(p.s, token, pos)) continue;
-    if (p.positions != nullptr)
-      pos = p.wide ? static_cast<const int64_t *>(p.positions)[token * p.position_stride]
-                   : static_cast<const int *>(p.positions)[token * p.position_stride];
-    float c[PAIRS], s[PAIRS];
+  }
+#pragma unroll
+  for (int j = 0; j < HEADS; ++j) {
+    const int h = slice + j * p.slices;
+    if (h >= p.heads) continue;
+    O u, v;
     if (turned) {
+      if constexpr (INTERLEAVED) {
+        turn_neighbours<T, U, N>(a[j], c, s, u);
+        if (at + N > p.dims)  // the last turned ones share a piece with those behind
 #pragma unroll
-      for (int i = 0; i < PAIRS; ++i) {
-        turn<sizeof(U) == 4>(pos, frequency(piece * PAIRS + i), p.gain, c[i], s[i]);
-        s[i] *= p.sign;
-      }
+          for (int i = 0; i < N; ++i)
+            if (at + i >= p.dims) u.v[i] = as_type<U>(a[j].v[i]);
+      } else
+        turn_pieces<T, U, N>(a[j], b[j], c, s, u, v);
+      if constexpr (!INTERLEAVED) *reinterpret_cast<O *>(out + h * p.o_hs + other) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) u.v[i] = as_type<U>(a[j].v[i]);
     }
-#pragma unroll
-    for (int j = 0; j < HEADS; ++j) {
-      const int h = slice + j * p.slices;
-      if (h >= p.heads) continue;
-      O u, v;
-      if (turned) {
-        if constexpr (INTERLEAVED) {
-          turn_neighbours<T, U, N>(a[j], c, s, u);
-          if (at + N > p.dims)  // the last turned ones share a piece with those behind
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-              if (at + i >= p.dims) u.v[i] = as_type<U>(a[j].v[i]);
-        } else
-          turn_pieces<T, U, N>(a[j], b[j], c, s, u, v);
-        if constexpr (!INTERLEAVED) *reinterpret_cast<O *>(out + h * p.o_hs + other) = v;
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) u.v[i] = as_type<U>(a[j].v[i]);
-      }
-      *reinterpret_cast<O *>(out + h * p.o_hs + at) = u;
-    }
+    *reinterpret_cast<O *>(out + h * p.o_hs + at) = u;
   }
 }
 
@@ -301,14 +302,7 @@ int64_t shape_blocks(Params &p, int threads) {
   p.pieces = !p.copy ? p.turned : INTERLEAVED ? p.head_dim / N : p.turned + (p.head_dim - p.dims) / N;
   p.slices = (p.heads + HEADS - 1) / HEADS;
   p.width = p.slices * p.pieces;  // at most 2^18 * 512
-  // tokens of a block: those that leave the fewest threads idle
-  p.block_tokens = 1;
-  double best = 0;
-  for (int n = 1; n <= 16 && n * int64_t(p.width) <= 4 * threads; ++n) {
-    const double used = double(n * p.width) / ((n * p.width + threads - 1) / threads * threads);
-    if (used > best + 0.05) best = used, p.block_tokens = n;
-  }
-  return (p.tokens + p.block_tokens - 1) / p.block_tokens;
+  return (p.tokens * p.width + threads - 1) / threads;
 }
 
 }  // namespace rotary
