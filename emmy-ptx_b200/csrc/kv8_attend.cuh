@@ -38,6 +38,8 @@ struct alignas(16) ResultRec {
   // of its own keys: the slot of row block 0 of part 0 of kv head 0; parts of a kv
   // head; row blocks of a part, which are neighbours
   int own_slot0, own_parts, own_blocks;
+  int start, n;      // its new tokens
+  int pad[2];
 };
 
 // Which kernel attends to shared keys.

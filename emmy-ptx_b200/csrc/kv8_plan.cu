@@ -269,6 +269,7 @@ struct Run {
 __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p) {
   __shared__ int at_of[EMMY_KV8_MAX_SEQS];
   __shared__ int sums[WARPS], longest;
+  __shared__ unsigned long long run_tokens, run_work;  // of all runs
   grid_dependency_wait();
   grid_dependency_done();
   const Seqs &s = p.a.s;
@@ -276,39 +277,50 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
   const bool tiles = p.a.shared == SHARED_TILES;
   for (int i = tid; i < s.tokens; i += THREADS) p.a.seq_of[i] = -1;
   // ---- runs ----
-  int pre_chunks[EACH], pre_blocks[EACH], runs = 0;
+  int pre_chunks[EACH], pre_blocks[EACH], pre_tokens[EACH], runs = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    pre_chunks[i] = pre_blocks[i] = 0;
+    pre_chunks[i] = pre_blocks[i] = pre_tokens[i] = 0;
     if (b0 + i < s.seqs) {
       const Run r(p, b0 + i);
       if (r.keys > 0) {
         pre_chunks[i] = r.keys >> 6;
         pre_blocks[i] = (r.tokens * G + RB - 1) / RB;
+        pre_tokens[i] = r.tokens;
         ++runs;
       }
     }
   }
-  if (tid == 0) longest = 1;
-  int all, nth = block_scan(runs, all, sums), mine = 0;
+  if (tid == 0) longest = 1, run_tokens = run_work = 0;
+  int all, nth = block_scan(runs, all, sums), mine;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     if (pre_chunks[i] > 0 && nth++ >= p.max_runs) pre_chunks[i] = pre_blocks[i] = 0;  // one more than there is room for
-    if (pre_chunks[i] > 0) atomicMax(&longest, pre_chunks[i]);
-    mine += pre_chunks[i] * pre_blocks[i];
+    if (pre_chunks[i] == 0) continue;
+    atomicMax(&longest, pre_chunks[i]);
+    atomicAdd(&run_tokens, static_cast<unsigned long long>(pre_tokens[i]));
+    atomicAdd(&run_work, static_cast<unsigned long long>(pre_chunks[i]) * pre_blocks[i]);
   }
-  block_scan(mine, all, sums);
-  const int pre_work = all;
+  __syncthreads();
+  // runs that overlap: there may not be room for so many blocks of rows, so all
+  // sequences are left to themselves
+  const bool overlap = run_tokens > static_cast<unsigned long long>(s.tokens);
+  const int64_t pre_work = overlap ? 0 : static_cast<int64_t>(run_work);
+  if (overlap) {
+    if (tid == 0) report(s.status, STATUS_LENGTH);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) pre_chunks[i] = pre_blocks[i] = 0;
+  }
 #pragma unroll
   for (int i = 0; i < EACH; ++i)
-    if (b0 + i < s.seqs) p.a.results[b0 + i] = ResultRec{pre_chunks[i], 0, 0, pre_blocks[i], 0, 0, 0, 1};
+    if (b0 + i < s.seqs) p.a.results[b0 + i] = ResultRec{pre_chunks[i], 0, 0, pre_blocks[i], 0, 0, 0, 1, 0, 0, {}};
   __syncthreads();
   // ---- each sequence's own keys ----
-  int chunks[EACH], blocks[EACH];  // row blocks
+  int chunks[EACH], blocks[EACH], first[EACH], tokens[EACH];  // blocks: of rows
   mine = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    chunks[i] = blocks[i] = 0;
+    chunks[i] = blocks[i] = first[i] = tokens[i] = 0;
     const int b = b0 + i;
     if (b < s.seqs) {
       int start, n, len;
@@ -328,6 +340,7 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
       if (n > 0) {
         chunks[i] = Span(p.a, len - n, len - 1).chunks - shared;
         blocks[i] = (n * G + ROWS_BLOCK - 1) / ROWS_BLOCK;
+        first[i] = start, tokens[i] = n;
         for (int t = 0; t < n; ++t) p.a.seq_of[start + t] = b;
       }
     }
@@ -345,7 +358,7 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
   int limit = longest;
   float best = 0.0f;
   if (p.pre_target > 0) {
-    const int64_t share = (int64_t(pre_work) * H + p.pre_target - 1) / p.pre_target;
+    const int64_t share = (pre_work * H + p.pre_target - 1) / p.pre_target;
     const int l0 = max(int(min(share, int64_t(1) << 24)), tiles ? TILE_CUT : 2);
     const float FIXED = p.wide ? 10.0f : 7.0f, CHUNK = p.wide ? 1.03f : 0.88f, OWN = 0.46f, RESULT = p.wide ? 0.053f : 0.027f;
     // parts for l0 chunks, and for an eighth more each time
@@ -411,7 +424,7 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
     if (b0 + i < s.seqs) {
       const int b = b0 + i, k = (chunks[i] + q - 1) / q, lead = p.a.runs[b];
       at_of[b] = at;
-      ResultRec f = {0, 0, 0, 1, 0, first_part + at, k, max(blocks[i], 1)};
+      ResultRec f = {0, 0, 0, 1, 0, first_part + at, k, max(blocks[i], 1), first[i], tokens[i], {}};
       if (chunks[i] > 0 && lead >= 0 && lead <= b && p.a.runs[lead] == lead && b - lead < max(p.a.runs[s.seqs + lead], 1)) {
         const ResultRec of = p.a.results[lead];  // (others write only what comes behind `row`)
         f.chunks = of.chunks, f.slot0 = of.slot0, f.parts = of.parts, f.blocks = max(of.blocks, 1);
@@ -422,6 +435,8 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
         p.a.results[b].own_slot0 = f.own_slot0;
         p.a.results[b].own_parts = k;
         p.a.results[b].own_blocks = f.own_blocks;
+        p.a.results[b].start = f.start;
+        p.a.results[b].n = f.n;
       } else {
         p.a.results[b] = f;
       }

@@ -23,10 +23,8 @@ __global__ void __launch_bounds__(32 * WARPS) shared_join_kernel(const AttendPar
   grid_dependency_done();
   if (!plan_fits(p, head, 0, 0, 0, 0) || b < 0 || b >= p.s.seqs) return;
   const ResultRec f = p.results[b];
-  int start, n, len;
-  lengths(p.s, b, start, n, len);
-  if (token < start || token >= start + n) return;  // lengths that changed since the plan
-  const int kv_head = h / p.group, r = (token - start) * p.group + h - kv_head * p.group;
+  const int n = f.n;
+  const int kv_head = h / p.group, r = (token - f.start) * p.group + h - kv_head * p.group;
   float m = NONE, l = 0.0f, x[N] = {};
   // `parts` results, so many floats apart, of slots of so many rows
   const auto take = [&](const float *first, int64_t apart, int slot_rows, int slot_row, int parts) {

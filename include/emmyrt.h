@@ -338,7 +338,8 @@ int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args *args, emm
  * taken so, and only where no sequence has more than 32 query rows of a kv head
  * and there is no window; all others' keys are read for each sequence, with the
  * same results up to rounding.  A sequence with new tokens among its run's
- * shared keys is skipped and reported.  Everything else is as for
+ * shared keys is skipped and reported; runs that overlap so far that they have more
+ * new tokens than the batch are reported, and nothing is shared.  Everything else is as for
  * emmy_kv8_attend; a plan and workspace for one kind of call is not for the
  * other. */
 typedef struct {

@@ -275,6 +275,54 @@ def test_runs_that_cannot_be(gpu):  # noqa: F811
         a._plans[H * G, 0, 0] = kept
 
 
+@pytest.mark.parametrize("group,seqs", [(4, 8), (8, 40)], ids=["rows", "tiles"])
+def test_runs_that_overlap(gpu, group, seqs):  # noqa: F811
+    """Device arrays that make each sequence the first of a run of all behind it: more
+    rows than a call has room for, so nothing is shared, and that is reported."""
+    from ptxgen.runtime import EmmyError
+    rng = np.random.default_rng(33)
+    H, D, P = 2, 64, 64
+    table, kv, ql, pages = layout(rng, [(192, [(1 + i, 1) for i in range(seqs)])], P)
+    codes, exps = ref.pool(rng, pages, H, P, D)
+    cache, _, _ = cache_of(gpu, codes[None], exps[None])
+    q = rng.standard_normal((seqs, H * group, D)).astype(np.float16)
+    want, bound = ref.attend(codes, exps, table, kv, ql, q.astype(np.float64), D ** -0.5)
+    batch = cache.batch(table, kv, ql, shared=True)
+    batch._s.max_runs = seqs
+    batch.reserve(H * group)
+    each = np.arange(seqs)
+    gpu.dev.htod(batch._s.runs, np.stack([each, seqs - each, 0 * each + 192]).astype(np.int32))
+    batch._plan((H * group, 0, 0), gpu.dev.stream)
+    out = gpu.put(np.zeros_like(q), "f16")
+    batch.attend(0, gpu.put(q, "f16"), out)
+    assert ref.close(gpu.get(out, q.shape, np.float16), want, bound, "f16")
+    with pytest.raises(EmmyError, match="longer than its row"):
+        batch.check_errors()
+    batch.close()
+
+
+@pytest.mark.parametrize("group,seqs", [(4, 4), (8, 20)], ids=["rows", "tiles"])
+def test_lengths_that_change_after_the_plan(gpu, group, seqs):  # noqa: F811
+    """A plan computes the rows of the lengths that it was made from."""
+    rng = np.random.default_rng(34)
+    H, D, P = 1, 128, 64
+    table, kv, ql, pages = layout(rng, [(256, [(2 + 3 * i, 1 + i % 2) for i in range(seqs)])], P)
+    codes, exps = ref.pool(rng, pages, H, P, D)
+    cache, _, _ = cache_of(gpu, codes[None], exps[None])
+    q = rng.standard_normal((sum(ql), H * group, D)).astype(np.float16)
+    want, bound = ref.attend(codes, exps, table, kv, ql, q.astype(np.float64), D ** -0.5)
+    batch = cache.batch(table, kv, ql, shared=True)
+    batch.reserve(H * group)
+    # the first ones' tokens are another's: none of the even ones, two of each odd one
+    starts = np.concatenate([[0], np.cumsum([2 * (i % 2) for i in range(seqs)])]).astype(np.int32)
+    gpu.dev.htod(batch._d.q_starts, starts)
+    out = gpu.put(np.zeros_like(q), "f16")
+    batch.attend(0, gpu.put(q, "f16"), out)
+    batch.check_errors()
+    assert ref.close(gpu.get(out, q.shape, np.float16), want, bound, "f16")
+    batch.close()
+
+
 def test_more_runs_than_there_is_room_for(gpu):  # noqa: F811
     """Device arrays that name more runs, or longer ones, than the call was made for:
     those beyond are attended to by themselves."""
