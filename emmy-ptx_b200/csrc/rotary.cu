@@ -40,13 +40,18 @@ int launch(const char *what, Params &p, cudaStream_t stream) {
 // Halves whose values pair up across pieces: rows go through shared memory, piece by
 // piece as they lie, and a thread turns its own values with those that it finds
 // there.  A block takes whole rows: so many (token, heads slice, slice + slices, ..)
-// of `pieces` threads each.  (Pairs of single values instead: 6333 tokens of 4 heads
-// of 80 with 6 turned 10 us, so 5.)
+// of `pieces` threads each; a row's threads compute the angle of each of its pairs
+// once, and those whose pieces are not turned copy them as they come.  (Pairs of single
+// values instead: 6333 tokens of 4 heads of 80 with 6 turned, bf16, 10 us, so 3.8; a
+// thread its own values' angles, most of which idle threads wait for: 8191 tokens of
+// 32 heads of 128 with 20 or 116 turned 50, so 32 and 35, a few tokens 4.2, so 2.7.
+// Words of pieces apart, with no bank conflicts but 34 KB a block: 41 and 44.)
 template <typename T, typename U, int N>
 __global__ void __launch_bounds__(THREADS) rotate_apart_kernel(const __grid_constant__ Params p) {
   using P = Piece<T, N>;
   constexpr int HEADS = 4;
   __shared__ P rows[HEADS][THREADS];
+  __shared__ float2 turns[THREADS * N / 2];  // (c, s) of each pair of each row
   __shared__ uint64_t frequency[EMMY_ROTARY_PAIRS];
   const int tid = threadIdx.x, r = tid / p.pieces, piece = tid - r * p.pieces, half = p.dims / 2;
   if (tid < half) frequency[tid] = p.frequency[tid];
@@ -63,38 +68,57 @@ __global__ void __launch_bounds__(THREADS) rotate_apart_kernel(const __grid_cons
     const int h = slice + j * p.slices;
     if (real && h < p.heads) a[j] = *reinterpret_cast<const P *>(x + h * p.x_hs);
   }
-  __syncthreads();
   int64_t pos = p.first + token;
   bool placed = real;
   if (real && p.s.seqs > 0) placed = place_of(p.s, token, pos);
   if (real && p.positions != nullptr)
     pos = p.wide ? static_cast<const int64_t *>(p.positions)[token * p.position_stride]
                  : static_cast<const int *>(p.positions)[token * p.position_stride];
-  float c[N], s[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int at = piece * N + i;
-    if (at >= p.dims) break;
-    turn<sizeof(U) == 4>(pos, frequency[at < half ? at : at - half], p.gain, c[i], s[i]);
-    if ((at < half) == (p.sign > 0.0f)) s[i] = -s[i];
-  }
+  __syncthreads();
+  float2 *const mine = turns + r * half;
+  if (real)
+#pragma unroll 1
+    for (int i = piece; i < half; i += p.pieces) {
+      float c, s;
+      turn<sizeof(U) == 4>(pos, frequency[i], p.gain, c, s);
+      mine[i] = make_float2(c, p.sign * s);
+    }
 #pragma unroll
   for (int j = 0; j < HEADS; ++j)
     if (real && slice + j * p.slices < p.heads) rows[j][tid] = a[j];
+  if (placed && p.copy && piece * N >= p.dims) {
+#pragma unroll
+    for (int j = 0; j < HEADS; ++j) {
+      const int h = slice + j * p.slices;
+      if (h >= p.heads) break;
+      Piece<U, N> u;
+#pragma unroll
+      for (int i = 0; i < N; ++i) u.v[i] = as_type<U>(a[j].v[i]);
+      *reinterpret_cast<Piece<U, N> *>(out + h * p.o_hs) = u;
+    }
+  }
   __syncthreads();
-  if (!placed || (!p.copy && piece * N >= p.dims)) return;
+  if (!placed || piece * N >= p.dims) return;
+  float c[N], s[N];
+  int other[N];  // where the value that each pairs up with is
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int at = piece * N + i;
+    const bool low = at < half;
+    const float2 t = at < p.dims ? mine[low ? at : at - half] : make_float2(1.0f, 0.0f);
+    c[i] = t.x, s[i] = low ? -t.y : t.y;
+    other[i] = at >= p.dims ? at : low ? at + half : at - half;
+  }
 #pragma unroll
   for (int j = 0; j < HEADS; ++j) {
     const int h = slice + j * p.slices;
     if (h >= p.heads) break;
     const T *row = reinterpret_cast<const T *>(&rows[j][r * p.pieces]);
+    const P own = rows[j][tid];
     Piece<U, N> u;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = piece * N + i;
-      u.v[i] = at >= p.dims ? as_type<U>(a[j].v[i])
-                            : rounded<U>(to_float(a[j].v[i]) * c[i] + to_float(row[at < half ? at + half : at - half]) * s[i]);
-    }
+    for (int i = 0; i < N; ++i)
+      u.v[i] = piece * N + i < p.dims ? rounded<U>(to_float(own.v[i]) * c[i] + to_float(row[other[i]]) * s[i]) : as_type<U>(own.v[i]);
     *reinterpret_cast<Piece<U, N> *>(out + h * p.o_hs) = u;
   }
 }
@@ -111,9 +135,10 @@ int launch_apart(const char *what, Params &p, cudaStream_t stream) {
 
 template <typename T, typename U, int N>
 int launch_layout(const char *what, Params &p, cudaStream_t stream) {
-  if constexpr (N > 1)
+  if constexpr (N > 1) {
     if (p.interleaved) return launch<T, U, N, true>(what, p, stream);
-  if (!p.interleaved && p.dims / 2 % N != 0 && p.head_dim / N <= THREADS) return launch_apart<T, U, N>(what, p, stream);
+    if (p.dims / 2 % N != 0) return launch_apart<T, U, N>(what, p, stream);  // (at most 512 / N threads a row)
+  }
   return launch<T, U, N, false>(what, p, stream);
 }
 
