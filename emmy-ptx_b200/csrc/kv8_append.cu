@@ -390,18 +390,19 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
     if (!pairs) col = p.dims + behind * N;
     col2 = pairs ? col + half : col + (D - p.dims) / 2;
   }
+  // of the new rows
   const int row0 = warp * (32 / LANES) + lane / LANES, step = warps * (32 / LANES), away = col2 - col;
   const int64_t token0 = int64_t(start) + pos0 - first;  // row 0 of the page, were it new
-  const int mine = row0 * LPR + col / N, page_pieces = LPR << s.page_shift;
+  const int mine = row0 * LPR + col / N, buffer = ROWS * step * LPR;
   const auto fetch = [&](int u, int buf) {
     const int side = u & 1, head = u >> 1;
     const int64_t ts = side ? p.ts[1] : p.ts[0];
     const T *x = static_cast<const T *>(side ? p.x[1] : p.x[0]) + head * (side ? p.hs[1] : p.hs[0]) + col;
-    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(pieces + buf * page_pieces + mine));
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(pieces + buf * buffer + mine));
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const int r = row0 + i * step;
-      const bool real = r >= lo && r < hi;
+      const int r = lo + row0 + i * step;
+      const bool real = r < hi;
       const T *from = x + (token0 + (real ? r : lo)) * ts;
       copy16(to + i * step * (D * int(sizeof(T))), from, real);
       copy16(to + (i * step * D + away) * int(sizeof(T)), from + away, real);
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
   const int64_t unit0 = int64_t(bad ? 0 : page) * 2 * H;
   const auto unit_of = [&](int u) { return unit0 + (u & 1 ? H : 0) + (u >> 1); };
   int held = lo > 0 ? p.exps[unit_of(u0)] : 0;
-  // angles of keys: of row row0, and of i * step rows
+  // angles of keys: of row lo + row0, and of i * step rows
   uint64_t first_c[HALF], first_s[HALF];
   const auto pair_at = [&](int j) { return MODE == HALVES ? col + j : (j < HALF ? col : col2 - N) / 2 + j; };
   if (MODE != ANY && (u1 - u0 > 1 || u0 % 2 == 0)) {  // there are keys
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
     for (int j = 0; j < N; j += 2) {
       float c[2], s[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) rotary::turn<false>(pos0 + row0, frequency[min(pair_at(j + i), D / 2 - 1)], p.gain, c[i], s[i]);
+      for (int i = 0; i < 2; ++i) rotary::turn<false>(pos0 + lo + row0, frequency[min(pair_at(j + i), D / 2 - 1)], p.gain, c[i], s[i]);
       first_c[j / 2] = two(c[0], c[1]);
       first_s[j / 2] = two(s[0], s[1]);
     }
@@ -443,15 +444,15 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     // every thread reads only the pieces it copied
-    const uint4 *rows = pieces + buf * page_pieces + mine;
+    const uint4 *rows = pieces + buf * buffer + mine;
     const bool turn = (u & 1) == 0;
     uint64_t x[ROWS][HALF], y[ROWS][HALF];
     float amax = 0.0f;
     if (MODE == ANY && turn) __syncwarp();  // but for these, paired with any value of a row that their warp copied
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const int r = row0 + i * step;
-      if (r < lo || r >= hi) continue;
+      const int r = lo + row0 + i * step;
+      if (r >= hi) continue;
       const uint4 *at = rows + i * step * LPR;
       if (MODE == ANY && turn) {
         float v[2 * N];
@@ -501,7 +502,7 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
       amax = 0.0f;
 #pragma unroll
       for (int i = 0; i < ROWS; ++i)
-        if (row0 + i * step >= lo && row0 + i * step < hi)
+        if (lo + row0 + i * step < hi)
 #pragma unroll
           for (int j = 0; j < HALF; ++j) {
             const float2 f = apart(x[i][j]), g = apart(y[i][j]);
@@ -521,8 +522,8 @@ __global__ void __launch_bounds__(MOST, ROWS == 2 && MOST == 256 ? 3 : 1) append
     const uint64_t by = two(pow2(-e), pow2(-e));
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const int r = row0 + i * step;
-      if (r < lo || r >= hi) continue;
+      const int r = lo + row0 + i * step;
+      if (r >= hi) continue;
       uint32_t w[2][2] = {};
 #pragma unroll
       for (int j = 0; j < HALF; ++j) {
@@ -688,7 +689,10 @@ int launch(Params p, bool one, int64_t slots, int device, cudaStream_t stream) {
   if (one)
     return launch_kernel("emmy_kv8_append", append_one_kernel<D, T, Params>, dim3(p.s.seqs, (units + 3) / 4), 128, 0, stream, p);
   // several (side, head)s a CTA once there are more than fill the GPU twice
-  const int threads = page_threads<D, T>(1 << p.s.page_shift);
+  int threads = page_threads<D, T>(1 << p.s.page_shift);
+  // no more rows than a sequence has new ones
+  if constexpr (std::is_same<Params, RotatedParams>::value)
+    while (threads > 64 && int64_t(p.s.max_q) * D * int(sizeof(T)) / 128 <= threads / 2) threads /= 2;
   int64_t fill = int64_t(sm_count(device)) * 2 * (2048 / threads < 7 ? 2048 / threads : 7);
   if constexpr (std::is_same<Params, RotatedParams>::value) fill = int64_t(sm_count(device)) * 2 * std::max(768 / (2 * threads), 1);
   p.units = int(std::min<int64_t>(units, std::max<int64_t>(1, slots * units / std::max<int64_t>(fill, 1))));
