@@ -15,13 +15,14 @@ namespace rotary {
 // A multiple of 2^64 is a whole number of turns, so the product's low 64 bits are
 // the angle: exact, but for the frequency's own rounding, at any position, where an
 // f32 angle at position 131071 is off by 0.004.  What is left of the nearest
-// quarter turn, at most an eighth of one, goes through the Taylor series to x^9
-// and x^10, which are off by less than 2^-29 there.
+// quarter turn, at most an eighth of one, is rounded to f32 as a whole, so that small
+// angles keep its precision (of the upper 32 bits alone, a frequency of 1e-9 does not
+// turn position 1 at all), and goes through the Taylor series to x^9 and x^10, which
+// are off by less than 2^-29 there.
 __device__ __forceinline__ void turn_of(int64_t position, uint64_t frequency, float &c, float &s) {
-  const uint32_t t = static_cast<uint32_t>((static_cast<uint64_t>(position) * frequency) >> 32);
-  const uint32_t quarter = (t + 0x20000000u) >> 30;
-  // 2 pi 2^-32
-  const float x = static_cast<float>(static_cast<int32_t>(t - (quarter << 30))) * 1.4629180792671596e-9f, y = x * x;
+  const uint64_t t = static_cast<uint64_t>(position) * frequency, quarter = (t + (uint64_t(1) << 61)) >> 62;
+  // 2 pi 2^-64
+  const float x = static_cast<float>(static_cast<int64_t>(t - (quarter << 62))) * 3.4061215800304705e-19f, y = x * x;
   const float sine = fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), x);
   const float cosine =
       fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);

@@ -497,3 +497,57 @@ def test_many_heads_and_wide_strides(gpu):  # noqa: F811
     assert ref.close(out.float().cpu().numpy(), want, bound, "bf16")
     rot.rotate(view, 7, view, stream=st)
     assert (view == out).all()
+
+
+SLOW = [1e6 ** (-126 / 128) / 32, 1e-9, 3e-11]     # the slowest pair of a stretched context, and slower ones
+
+
+def slow_bound(angle, positions):
+    """f32, small angles: the rest of a turn, 2 pi 2^-64 and their product are rounded
+    by 2.5 * 2^-24 of it, the sine's last sum by 2^-24; one times it and nothing times
+    the cosine are exact.  The frequency is held to 2^-65 turns."""
+    return 2.0 ** -22 * np.abs(angle) + np.abs(positions)[:, None] * 2 * np.pi * 2.0 ** -65
+
+
+@pytest.mark.parametrize("head_dim,dims,interleaved", [(8, 6, True), (12, 6, True), (7, 6, True), (8, 6, False), (7, 6, False), (12, 8, False)])
+def test_slow_frequencies(gpu, head_dim, dims, interleaved):  # noqa: F811
+    """Small angles keep f32's precision, and a turn back undoes a turn."""
+    fs = (SLOW + [1e-8])[:dims // 2]
+    rot = rotary(head_dim, dims, interleaved, frequencies=fs)
+    pos = np.array([1, -1, 3, -7, 1000, -999])
+    low, high = (slice(0, dims, 2), slice(1, dims, 2)) if interleaved else (slice(0, dims // 2), slice(dims // 2, dims))
+    x = np.zeros((6, 2, head_dim), np.float32)
+    x[..., high] = 1
+    out = gpu.put(x, "f32")
+    rot.rotate(out, gpu.put(pos, "i64"), out)
+    got = gpu.get(out, x.shape, np.float32).astype(np.float64)
+    angle = pos[:, None] * np.array(fs)
+    tol = slow_bound(angle, pos)[:, None]
+    assert (np.abs(got[..., low] + np.sin(angle)[:, None]) <= tol).all()
+    assert (np.abs(got[..., high] - np.cos(angle)[:, None]) <= 2.0 ** -22).all()
+    # -s c + c s, of the same c and s: each product and the sum once more
+    for undo, at in ((rot.rotate, -pos), (rot.backward, pos)):
+        back = gpu.put(got.astype(np.float32), "f32")
+        undo(back, gpu.put(at, "i64"), back)
+        assert (np.abs(gpu.get(back, x.shape, np.float32)[..., low]) <= 2.0 ** -22 * np.abs(angle)[:, None]).all()
+
+
+def test_slow_frequencies_of_appended_queries(gpu):  # noqa: F811
+    """So do queries on the way into f32, of single tokens and of pages."""
+    rng = np.random.default_rng(17)
+    D, r = 64, 6
+    rot = rotary(D, r, False, frequencies=SLOW)
+    for ql in ([1, 1, 1], [1, 2, 3]):
+        T, places = sum(ql), np.concatenate([np.arange(5, 5 + m) for m in ql])
+        codes, exps = kv8.pool(rng, 3, 1, 64, D)
+        cache, _, _ = cache_of(gpu, codes[None], exps[None])
+        batch = cache.batch([[0], [1], [2]], [5 + m for m in ql], ql)
+        q = np.zeros((T, 2, D), np.float32)
+        q[..., 3:6] = 1
+        k, out = gpu.put(values(rng, (T, 1, D), "f32"), "f32"), gpu.put(q, "f32")
+        batch.append(0, k, k, rotary=rot, q=gpu.put(q, "f32"), q_out=out)
+        batch.check_errors()
+        got = gpu.get(out, q.shape, np.float32).astype(np.float64)
+        angle = places[:, None] * np.array(SLOW)
+        assert (np.abs(got[..., :3] + np.sin(angle)[:, None]) <= slow_bound(angle, places)[:, None]).all()
+        batch.close()
