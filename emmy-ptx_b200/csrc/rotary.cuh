@@ -32,9 +32,12 @@ __device__ __forceinline__ void turn_of(int64_t position, uint64_t frequency, fl
   if (quarter & 2) s = -s;
 }
 
-// The same to 2^-20.6: the angle rounded to f32 (2^-22.3) and the special function
-// unit (at most 2^-21.2, as CUDA documents __cosf and __sinf there), 10 instructions
-// for 45.  For results of 16 bits, which round by 2^-12 or more, and of 8.
+// The same to 2^-20, whatever the angle: it is at most pi, rounded three times on its
+// way to f32 (3 * 2^-24 of it, 2^-20.8; its lowest bits, below 2^-32 turns, do not
+// count), and the special function unit is off by at most 2^-21.2, as CUDA documents
+// __cosf and __sinf there.  10 instructions for 45.  For results of 16 bits, which
+// round by 2^-12 or more of the larger of a pair, and of 8: the smaller one, and what
+// a small angle makes of it, is good to 2^-20 of the larger, not to its own last bit.
 __device__ __forceinline__ void turn_near(int64_t position, uint64_t frequency, float &c, float &s) {
   const uint32_t t = static_cast<uint32_t>((static_cast<uint64_t>(position) * frequency) >> 32);
   const float x = static_cast<float>(static_cast<int32_t>(t)) * 1.4629180792671596e-9f;

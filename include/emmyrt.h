@@ -209,7 +209,9 @@ enum { EMMY_KV8_F32 = 0, EMMY_KV8_BF16 = 1, EMMY_KV8_F16 = 2 };
  * pairs (a, b): neighbours where `interleaved`, else dims / 2 apart.  Pair i of
  * a token at position p turns by p * turns[i] * 2^-64 whole turns and is scaled
  * by `gain`; the values behind `dims` stay as they are.  The multiplication is
- * modulo 2^64, so angles are exact at any position, negative ones too. */
+ * modulo 2^64, so angles are exact at any position, negative ones too.  Sines and
+ * cosines are good to 2^-22 of themselves where results are f32, and to 2^-20 (of a
+ * whole) where they have 16 bits. */
 enum { EMMY_ROTARY_PAIRS = 256 };
 typedef struct {
   uint64_t turns[EMMY_ROTARY_PAIRS]; /* frequency / (2 pi) * 2^64, rounded */
@@ -218,14 +220,15 @@ typedef struct {
   int32_t interleaved;
 } emmy_rotary;
 
-/* out = the rows x [tokens][heads][head_dim] turned (or, `backward`, turned back
- * and scaled by gain: the gradient of x from that of out), f32, bf16 or f16 (the
- * EMMY_KV8_* types), computed in f32 and rounded once.  Innermost dimension
- * contiguous, strides in elements (token, head), none negative; 16-byte pieces
- * where addresses, strides and dims allow, else smaller ones.  `out` may be x
- * itself, or share no element with it.  Token t stands at positions[t *
- * position_stride] (int32, or int64 where `wide`), or at first + t where
- * positions is 0.  Allocates nothing and does not synchronise. */
+/* out = the rows x [tokens][heads][head_dim] turned (or, `backward`, turned back and
+ * scaled by gain: the gradient of x from that of out), f32, bf16 or f16 (the
+ * EMMY_KV8_* types), computed in f32 and rounded once: 16-bit results are off by
+ * gain (|a| + |b|) 2^-19 at most before that, which a small one beside a large may
+ * show. Innermost dimension contiguous, strides in elements (token, head), none
+ * negative; 16-byte pieces where addresses, strides and dims allow, else smaller
+ * ones. `out` may be x itself, or share no element with it. Token t stands at
+ * positions[t * position_stride] (int32, or int64 where `wide`), or at first + t
+ * where positions is 0. Allocates nothing and does not synchronise. */
 typedef struct {
   emmy_dptr x, out, positions;
   int64_t x_strides[2], out_strides[2];
