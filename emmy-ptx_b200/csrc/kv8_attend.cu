@@ -160,6 +160,9 @@ int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_shared *s
   p.row_limit = shape.rows ? ROWS_MOST : 0;
   p.nt = shape.nt;
   p.cluster = shape.cluster;
+  p.most_parts = int(shape.most_parts);
+  p.most_units = int(shape.most_units);
+  p.most_joins = int(shape.most_joins);
   p.shared = shape.shared;
   if (shape.shared != SHARED_NONE) {
     if (shared->runs == 0 || shared->runs % 4) return fail(EMMY_EINVAL, what, "runs is missing or unaligned");

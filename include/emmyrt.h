@@ -344,7 +344,8 @@ int emmy_kv8_attend(const emmy_kv8 *cache, const emmy_kv8_attend_args *args, emm
  * shared keys is skipped and reported; runs that overlap so far that they have more
  * new tokens than the batch are reported, and nothing is shared.  Everything else is as for
  * emmy_kv8_attend; a plan and workspace for one kind of call is not for the
- * other. */
+ * other, nor for one with other max_runs, max_tokens, tokens or max_q (a plan that
+ * therefore lies elsewhere in its bytes is reported). */
 typedef struct {
   emmy_dptr runs; /* int32 [3][seqs] */
   int32_t max_runs, max_tokens;

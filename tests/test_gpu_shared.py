@@ -452,3 +452,75 @@ def test_waits_that_run_out(gpu, case):  # noqa: F811
         batch.check_errors()
         assert ref.close(gpu.get(od, q.shape, NP[dtype]), want, bound, dtype)
     batch.close()
+
+
+@pytest.mark.parametrize("group,members", [(4, 4), (8, 12)], ids=["rows", "tiles"])
+@pytest.mark.parametrize("field,value", [("max_runs", 1), ("max_runs", 2), ("max_tokens", 1), ("tokens", -1)])
+def test_plan_of_another_layout(gpu, group, members, field, value):  # noqa: F811
+    """A plan that was made for other runs or tokens lies elsewhere in the same bytes:
+    refused or reported, nothing written, and no harm to the next call."""
+    from ptxgen.runtime import EmmyError
+    rng = np.random.default_rng(35)
+    H, D, P = 2, 64, 64
+    runs = [(128, [(70, 2)] * members), (64, [(9, 1)] * members), (192, [(5, 1)] * members)]
+    table, kv, ql, pages = layout(rng, runs, P)
+    codes, exps = ref.pool(rng, pages, H, P, D)
+    cache, _, _ = cache_of(gpu, codes[None], exps[None])
+    q = rng.standard_normal((sum(ql), H * group, D)).astype(np.float16)
+    want, bound = ref.attend(codes, exps, table, kv, ql, q.astype(np.float64), D ** -0.5)
+    batch = cache.batch(table, kv, ql, shared=True)
+    assert (batch._s.max_runs, batch._s.max_tokens, batch.max_q) == (3, 2 * members, 2)
+    batch.reserve(H * group)
+    made = (batch._s.max_runs, batch._s.max_tokens, batch._d.tokens)
+    where = batch._s if field in ("max_runs", "max_tokens") else batch._d
+    setattr(where, field, getattr(where, field) + value if value < 0 else value)
+    import ctypes
+    ws, plan = ctypes.c_uint64(), ctypes.c_uint64()
+    assert batch.L.emmy_kv8_attend_shared_sizes(batch._ref, batch._sref, H * group, ctypes.byref(ws), ctypes.byref(plan)) == 0
+    at, held = batch._plans[H * group, 0, 0]
+    out = gpu.put(np.full(q.shape, 77).astype(np.float16), "f16")
+    if plan.value > held or ws.value > batch._ws[1]:     # the host knows already
+        assert (group, field) == (8, "max_tokens")
+        with pytest.raises(EmmyError, match="too small"):
+            batch.attend(0, gpu.put(q, "f16"), out)
+    else:
+        batch.attend(0, gpu.put(q, "f16"), out)
+        with pytest.raises(EmmyError, match="another call"):
+            batch.check_errors()
+    assert (gpu.get(out, q.shape, np.float16) == 77).all()
+    batch._s.max_runs, batch._s.max_tokens, batch._d.tokens = made       # as it was made
+    batch.attend(0, gpu.put(q, "f16"), out)
+    batch.check_errors()
+    assert ref.close(gpu.get(out, q.shape, np.float16), want, bound, "f16")
+    batch.close()
+
+
+@pytest.mark.parametrize("lens,ql,field,value", [
+    # 500 sequences of 20 rows of a kv head are 1000 blocks of rows, of 16 rows 500
+    ([200] * 500, [5] * 500, "max_q", 4),
+    # 500 tokens of 4 heads are 7 + 2 units of 256 rows at most, 400 are 6 + 2
+    ([300, 300], [300, 200], "tokens", 400),
+], ids=["rows", "tiles"])
+def test_plan_of_another_layout_unshared(gpu, lens, ql, field, value):  # noqa: F811
+    """The same of calls that share nothing."""
+    import ctypes
+    from ptxgen.runtime import EmmyError
+    rng = np.random.default_rng(36)
+    H, G, D, P = 1, 4, 64, 64
+    width = -(-max(lens) // P)
+    table = np.arange(width * len(lens)).reshape(len(lens), width)
+    codes, exps = ref.pool(rng, table.size, H, P, D)
+    cache, _, _ = cache_of(gpu, codes[None], exps[None])
+    q = rng.standard_normal((sum(ql), H * G, D)).astype(np.float16)
+    batch = cache.batch(table, lens, ql)
+    batch.reserve(H * G)
+    setattr(batch._d, field, value)
+    ws, plan = ctypes.c_uint64(), ctypes.c_uint64()
+    assert batch.L.emmy_kv8_attend_sizes(batch._ref, H * G, ctypes.byref(ws), ctypes.byref(plan)) == 0
+    assert plan.value < batch._plans[H * G, 0, 0][1] and ws.value <= batch._ws[1]
+    out = gpu.put(np.full(q.shape, 77).astype(np.float16), "f16")
+    batch.attend(0, gpu.put(q, "f16"), out)
+    with pytest.raises(EmmyError, match="another call"):
+        batch.check_errors()
+    assert (gpu.get(out, q.shape, np.float16) == 77).all()
+    batch.close()
