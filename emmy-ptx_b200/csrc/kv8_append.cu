@@ -724,8 +724,9 @@ int launch(Params p, bool one, int64_t slots, int device, cudaStream_t stream) {
           m.blocks = int(m.kv_blocks + rows);
         }
       if (2 * threads <= 256) return run(append_turned_kernel<D, T, M, 2, 256>, of[0], 2);
-      if (2 * threads <= 512) return run(append_turned_kernel<D, T, M, 2, 512>, of[1], 2);
-      return run(append_turned_kernel<D, T, M, 4, MOST>, of[2], 1);
+      if constexpr (2 * MOST > 512)
+        if (2 * threads > 512) return run(append_turned_kernel<D, T, M, 4, MOST>, of[2], 1);
+      return run(append_turned_kernel<D, T, M, 2, 512>, of[1], 2);
     };
     if (p.positions == nullptr && p.interleaved) return pick(std::integral_constant<int, NEIGHBOURS>(), setup);
     if (p.positions == nullptr && p.dims / 2 % Vec<T>::N == 0) return pick(std::integral_constant<int, HALVES>(), setup + 3);
