@@ -142,18 +142,23 @@ int launch_layout(const char *what, Params &p, cudaStream_t stream) {
   return launch<T, U, N, false>(what, p, stream);
 }
 
-// The widest pieces that start everywhere on a multiple of their size.
+// The widest pieces that start everywhere on a multiple of their size.  Results of
+// another type are an append's queries, which start on multiples of 16 bytes.
 template <typename T, typename U>
 int launch_type(const char *what, Params &p, cudaStream_t stream) {
   const auto fits = [&](int n) {
     return reinterpret_cast<uintptr_t>(p.x) % (n * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p.out) % (n * sizeof(U)) == 0 &&
            p.x_ts % n == 0 && p.x_hs % n == 0 && p.o_ts % n == 0 && p.o_hs % n == 0 && p.head_dim % n == 0;
   };
-  if constexpr (sizeof(T) == 2 && sizeof(U) == 2)
-    if (fits(8)) return launch_layout<T, U, 8>(what, p, stream);
-  if (fits(4)) return launch_layout<T, U, 4>(what, p, stream);
-  if (fits(2)) return launch_layout<T, U, 2>(what, p, stream);
-  return launch_layout<T, U, 1>(what, p, stream);
+  constexpr int WIDEST = sizeof(T) == 2 && sizeof(U) == 2 ? 8 : 4;
+  if (fits(WIDEST)) return launch_layout<T, U, WIDEST>(what, p, stream);
+  if constexpr (std::is_same<T, U>::value) {
+    if constexpr (WIDEST > 4)
+      if (fits(4)) return launch_layout<T, U, 4>(what, p, stream);
+    if (fits(2)) return launch_layout<T, U, 2>(what, p, stream);
+    return launch_layout<T, U, 1>(what, p, stream);
+  }
+  return kv8::fail(EMMY_EINVAL, what, "q and q_out: base and strides must be multiples of 16 bytes");
 }
 
 template <typename T>
