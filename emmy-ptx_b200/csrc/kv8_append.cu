@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(128) append_one_kernel(const __grid_constant__
   }
   grid_dependency_wait();
   grid_dependency_done();
-  const int b = blockIdx.x, unit_of_seq = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int b = blockIdx.x, unit_of_seq = (blockIdx.z * gridDim.y + blockIdx.y) * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   int all = 2 * s.kv_heads;
   if constexpr (ROTATED) all += p.heads;
   if (unit_of_seq >= all) return;
@@ -686,8 +686,11 @@ int launch(Params p, bool one, int64_t slots, int device, cudaStream_t stream) {
   int units = 2 * p.s.kv_heads;
   if constexpr (std::is_same<Params, RotatedParams>::value)
     if (one) units += p.heads;
-  if (one)
-    return launch_kernel("emmy_kv8_append", append_one_kernel<D, T, Params>, dim3(p.s.seqs, (units + 3) / 4), 128, 0, stream, p);
+  if (one) {
+    // (2^20 query heads are more than a grid's second dimension takes)
+    const int blocks = (units + 3) / 4, y = std::min(blocks, 65535);
+    return launch_kernel("emmy_kv8_append", append_one_kernel<D, T, Params>, dim3(p.s.seqs, y, (blocks + y - 1) / y), 128, 0, stream, p);
+  }
   // several (side, head)s a CTA once there are more than fill the GPU twice
   int threads = page_threads<D, T>(1 << p.s.page_shift);
   // no more rows than a sequence has new ones

@@ -551,3 +551,31 @@ def test_slow_frequencies_of_appended_queries(gpu):  # noqa: F811
         angle = places[:, None] * np.array(SLOW)
         assert (np.abs(got[..., :3] + np.sin(angle)[:, None]) <= slow_bound(angle, places)[:, None]).all()
         batch.close()
+
+
+def test_append_most_query_heads(gpu):  # noqa: F811
+    """One token of 2^20 query heads, the most there may be, and of 2^18."""
+    import torch
+    from ptxgen import KVCache
+    rot = rotary(64, 64, False)
+    st = torch.cuda.current_stream().cuda_stream
+    cache = KVCache(pages=2, kv_heads=2, head_dim=64)
+    cache.dev.sync()
+    k = torch.randn((1, 2, 64), device="cuda").bfloat16()
+    for heads in (1 << 18, 1 << 20):
+        batch = cache.batch([[1]], [4], stream=st)
+        q = torch.randn((1, heads, 64), device="cuda").bfloat16()
+        out = torch.zeros_like(q)
+        batch.append(0, k, k, stream=st, rotary=rot, q=q, q_out=out)
+        batch.check_errors(stream=st)
+        # some heads against the oracle, all against the row kernel: each is off by
+        # 2^-8 of the value and 2^-19 (|a| + |b|)
+        want = torch.empty_like(q)
+        rot.rotate(q, 3, want, stream=st)
+        some = torch.cat([torch.arange(9), torch.randint(heads, (50,)), torch.arange(heads - 9, heads)])
+        value, bound = ref.rotate(rot, q[:, some].float().cpu().numpy(), 3 + np.arange(1), to="16")
+        for got in (out, want):
+            assert ref.close(got[:, some].float().cpu().numpy(), value, bound, "bf16")
+        assert ((out.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 2.0 ** -17 * q.float().abs().max()).all()
+        batch.close()
+    cache.close()
