@@ -138,7 +138,7 @@ class Rotary:
                 raise EmmyError(f"base must be a positive number, got {base!r}")
             try:
                 f, own_gain = _scaled(dims, float(base), scaling)
-            except (OverflowError, ZeroDivisionError):
+            except (OverflowError, ValueError, ZeroDivisionError):
                 raise EmmyError("base and scaling give no finite frequencies") from None
         if not all(map(math.isfinite, f)):
             raise EmmyError(f"frequencies must be {dims // 2} finite numbers")

@@ -96,6 +96,18 @@ def test_refusals(kw, says):
         Rotary(**{"head_dim": 64, **kw})
 
 
+@pytest.mark.parametrize("kw", [{"length": 1e-300, "fast": 1e300}, {"length": 5, "fast": 1e308, "slow": 1e307, "factor": 1e-308},
+                                {"length": 1e308, "slow": 1e-308}])
+def test_ramps_past_all_numbers(kw):
+    """Refused as other numbers that give no frequencies, or fine."""
+    try:
+        rot = Rotary(64, scaling={"type": "ramp", "factor": 2.0, **kw})
+    except EmmyError as error:
+        assert "finite" in str(error)
+    else:
+        assert all(map(math.isfinite, rot.frequencies))
+
+
 @pytest.fixture
 def lib(dev, monkeypatch):  # noqa: F811
     monkeypatch.setattr(ro, "load_library", lambda: dev.L)
