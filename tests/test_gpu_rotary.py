@@ -579,3 +579,17 @@ def test_append_most_query_heads(gpu):  # noqa: F811
         assert ((out.float() - want.float()).abs() <= 2.0 ** -7 * want.float().abs() + 2.0 ** -17 * q.float().abs().max()).all()
         batch.close()
     cache.close()
+
+
+@pytest.mark.parametrize("dims,interleaved,positions", [(128, False, False), (128, True, False), (64, False, False), (20, False, False), (128, False, True)])
+@pytest.mark.parametrize("page,longest,dtype,heads", [(64, 40, "bf16", 8), (64, 40, "f32", 3), (256, 140, "f16", 3)])
+def test_append_many_pages(gpu, dims, interleaved, positions, page, longest, dtype, heads):  # noqa: F811
+    """More pages than fill the GPU, so that a block takes several keys' and values'
+    heads of a page, four of them one after another: 242 places for pages."""
+    rng = np.random.default_rng(18)
+    lens = [int(n) for n in rng.integers(1, 6, 119)]
+    seqs = [(longest + 30, longest)] + [(int(rng.integers(n, page + 40)), n) for n in lens]
+    rot = rotary(128, dims, interleaved, base=500000.0)
+    T = sum(m for _, m in seqs)
+    pos = rng.integers(0, 1 << 20, T) if positions else None
+    append_gpu(gpu, (heads, 1, 128, page, dtype, dtype, seqs), rot, rng, pos)

@@ -524,3 +524,16 @@ def test_plan_of_another_layout_unshared(gpu, lens, ql, field, value):  # noqa: 
         batch.check_errors()
     assert (gpu.get(out, q.shape, np.float16) == 77).all()
     batch.close()
+
+
+@pytest.mark.parametrize("heads,head_dim,dtype", [(160, 128, "bf16"), (320, 64, "f16")])
+def test_more_units_than_blocks(gpu, heads, head_dim, dtype):  # noqa: F811
+    """A run's 40 rows of each of many kv heads: blocks of the tile kernel take two or
+    three units one after another."""
+    rng = np.random.default_rng(37)
+    table, kv, ql, pages = layout(rng, [(640, [(3 + 40 * i, 1) for i in range(5)])], 64)
+    codes, exps = ref.pool(rng, pages, heads, 64, head_dim)
+    q = rng.standard_normal((5, heads * 8, head_dim)).astype(NP[dtype])
+    got = attend(gpu, codes, exps, table, kv, ql, q, dtype, runs=1)
+    want, bound = ref.attend(codes, exps, table, kv, ql, q.astype(np.float64), head_dim ** -0.5)
+    assert ref.close(got, want, bound, dtype)
