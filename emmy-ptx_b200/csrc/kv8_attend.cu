@@ -161,8 +161,7 @@ int check_args(const char *what, const emmy_kv8 *cache, const emmy_kv8_shared *s
   p.nt = shape.nt;
   p.cluster = shape.cluster;
   p.most_parts = int(shape.most_parts);
-  p.most_units = int(shape.most_units);
-  p.most_joins = int(shape.most_joins);
+  p.units_at = 2 * unsigned(shape.most_units) + (shape.tile_target > 0);  // at most 2^31 - 1 units
   p.shared = shape.shared;
   if (shape.shared != SHARED_NONE) {
     if (shared->runs == 0 || shared->runs % 4) return fail(EMMY_EINVAL, what, "runs is missing or unaligned");

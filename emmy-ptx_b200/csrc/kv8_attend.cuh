@@ -10,14 +10,13 @@ namespace kv8 {
 // A plan (see kv8_plan.cu): head, then records for the parts of the row kernel,
 // for those of the tile kernel, and for the tile kernel's units that were cut.
 struct alignas(16) PlanHead {
-  int parts, units, joins;
-  // what it was made for
-  int group, window, sinks, row_limit, seqs, kv_heads, width;
-  uint8_t nt, page_shift, cluster, shared;
-  // where its arrays are: records that there is room for, and, of a call with shared
-  // keys, tokens that have a sequence's number
-  int most_parts, most_units, most_joins, tokens;
-  int pad;
+  int parts, units;
+  int joins;  // of a call with shared keys, whose rows are joined: the tokens
+  int group, window, sinks, row_limit, seqs, kv_heads, nt, width, page_shift, cluster, shared;  // what it was made for
+  // where its arrays are: parts that there is room for; units, twice, and one more where
+  // they may be cut
+  int most_parts;
+  unsigned units_at;
 };
 static_assert(sizeof(PlanHead) == 64, "four loads of 16 bytes");
 struct alignas(16) PartRec {
@@ -71,7 +70,8 @@ struct AttendParams {
   int row_limit;     // sequences with more rows of a kv head than this are the tile kernel's
   int nt;            // 8-row blocks of the row kernel
   int cluster;       // CTAs of a cluster of the row kernel, 0: none
-  int most_parts, most_units, most_joins;  // records of the plan that there is room for
+  int most_parts;    // as in the plan's head
+  unsigned units_at;
   bool beside;       // the row kernel was launched to run beside the tile kernel
   unsigned *ready;   // there: what came before both is done, and the row kernel's blocks that know
   int shared;           // SHARED_..
@@ -105,16 +105,13 @@ struct PlanShape {
   bool wide;               // heads of 128 values
 };
 
-// Tokens whose sequence the plan names.
-__device__ __forceinline__ int plan_tokens(const AttendParams &p) { return p.shared != SHARED_NONE ? p.s.tokens : 0; }
 // The plan is for this call, its arrays where this call looks for them, and what the
 // record says is within the arrays.
 __device__ __forceinline__ bool plan_fits(const AttendParams &p, const PlanHead &h, int b, int start, int n, int len) {
   const bool ok = h.group == p.group && h.window == p.window && h.sinks == p.sinks && h.row_limit == p.row_limit &&
                   h.seqs == p.s.seqs && h.kv_heads == p.s.kv_heads && h.nt == p.nt && h.width == p.s.width && h.cluster == p.cluster &&
-                  h.page_shift == p.s.page_shift && h.shared == p.shared && h.most_parts == p.most_parts &&
-                  h.most_units == p.most_units && h.most_joins == p.most_joins && h.tokens == plan_tokens(p) &&
-                  start + n <= p.s.tokens && len <= (int64_t(p.s.width) << p.s.page_shift);
+                  h.page_shift == p.s.page_shift && h.shared == p.shared && start + n <= p.s.tokens &&
+                  len <= (int64_t(p.s.width) << p.s.page_shift) && h.most_parts == p.most_parts && h.units_at == p.units_at;
   if (!ok) report(p.s.status, STATUS_PLAN);
   return ok;
 }

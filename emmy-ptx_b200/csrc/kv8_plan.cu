@@ -32,7 +32,7 @@ constexpr int THREADS = 1024, WARPS = 32, EACH = EMMY_KV8_MAX_SEQS / THREADS;
 
 struct PlanParams {
   AttendParams a;
-  int target, min_chunks, tile_target;
+  int target, min_chunks, most_units, most_joins, tile_target;
   bool spread, single;
   int most_pre, pre_target, max_runs, max_tokens;  // of shared keys
   bool wide;                                       // heads of 128
@@ -82,9 +82,8 @@ __device__ __forceinline__ int owner_of(const int *first, int n, int x) {
 }
 
 __device__ __forceinline__ PlanHead head_of(const AttendParams &a, int parts, int units, int joins) {
-  return PlanHead{parts, units, joins, a.group, a.window, a.sinks, a.row_limit, a.s.seqs, a.s.kv_heads, a.s.width,
-                  uint8_t(a.nt), uint8_t(a.s.page_shift), uint8_t(a.cluster), uint8_t(a.shared), a.most_parts, a.most_units,
-                  a.most_joins, plan_tokens(a), 0};
+  return PlanHead{parts, units, joins, a.group, a.window, a.sinks, a.row_limit, a.s.seqs, a.s.kv_heads,
+                  a.nt, a.s.width, a.s.page_shift, a.cluster, a.shared, a.most_parts, a.units_at};
 }
 
 __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
@@ -233,17 +232,17 @@ __global__ void __launch_bounds__(THREADS) plan_kernel(const PlanParams p) {
       r.c0 = int(int64_t(c) * part / k);
       r.c1 = int(int64_t(c) * (part + 1) / k);
       if (k > 1) r.slot = slot0 + part;
-      if (at0 + part < p.a.most_units) p.a.units[at0 + part] = r;
+      if (at0 + part < p.most_units) p.a.units[at0 + part] = r;
     }
     if (k > 1) {
       const int j = atomicAdd(&joins, 1);
-      if (j < p.a.most_joins) p.a.joins[j] = JoinRec{r.head, r.row0, r.start, r.n * p.a.group, slot0, k, r.b, 0};
+      if (j < p.most_joins) p.a.joins[j] = JoinRec{r.head, r.row0, r.start, r.n * p.a.group, slot0, k, r.b, 0};
     }
   }
   __syncthreads();
   // the launches have room for so many (see shape_of)
   if (tid == 0)
-    *p.a.plan = head_of(p.a, n_parts, min(n_records, p.a.most_units), min(joins, p.a.most_joins));
+    *p.a.plan = head_of(p.a, n_parts, min(n_records, p.most_units), min(joins, p.most_joins));
 }
 
 // What a run that begins at sequence b comes to: its new tokens' rows of a kv
@@ -485,7 +484,7 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
     p.a.parts[first_part + atomicAdd(&count[step_of(r)], 1)] = r;
   }
   if (tid == 0)
-    *p.a.plan = head_of(p.a, first_part + n_parts, tiles ? n_pre : 0, 0);
+    *p.a.plan = head_of(p.a, first_part + n_parts, tiles ? n_pre : 0, s.tokens);
 }
 
 PlanParams params_of(const AttendParams &a, const PlanShape &shape) {
@@ -496,6 +495,8 @@ PlanParams params_of(const AttendParams &a, const PlanShape &shape) {
   p.single = shape.single;
   // a join through the workspace costs about what ten chunks do
   p.min_chunks = shape.cluster > 0 ? 10 : shape.shared == SHARED_TILES ? 8 : shape.shared == SHARED_ROWS ? 4 : 2;
+  p.most_units = int(shape.most_units);
+  p.most_joins = int(shape.most_joins);
   p.tile_target = shape.tile_target;
   p.most_pre = int(shape.most_pre);
   p.pre_target = shape.pre_target;

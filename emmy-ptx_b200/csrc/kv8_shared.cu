@@ -21,7 +21,12 @@ __global__ void __launch_bounds__(32 * WARPS) shared_join_kernel(const AttendPar
   const PlanHead head = *p.plan;
   const int b = token < p.s.tokens ? p.seq_of[token] : -1;
   grid_dependency_done();
-  if (!plan_fits(p, head, 0, 0, 0, 0) || b < 0 || b >= p.s.seqs) return;
+  if (!plan_fits(p, head, 0, 0, 0, 0)) return;
+  if (head.joins != p.s.tokens) {
+    report(p.s.status, STATUS_PLAN);
+    return;
+  }
+  if (b < 0 || b >= p.s.seqs) return;
   const ResultRec f = p.results[b];
   const int n = f.n;
   const int kv_head = h / p.group, r = (token - f.start) * p.group + h - kv_head * p.group;
