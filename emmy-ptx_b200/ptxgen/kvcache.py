@@ -64,6 +64,13 @@ WORKSPACE_ZERO = 16384     # bytes of a workspace that start as zeros
 # 20.6 | 20.4, behind 1024 (8064) 24 | 31.5.  d = 64, 2 kv heads, 8 query heads each: 8
 # behind 16384 (3584) 17 | 15, 16 (7680) 18 | 21, 64 behind 4096 (8064) 19 | 20.
 MIN_SAVED = {64: 6000, 128: 4000}
+# That much for as many other things as these in reads: every sequence's rows, of those
+# in no run too, go through a slot of f32 and a join, and its own keys through parts
+# that leave results.  8 behind 8192 keys beside 1000 of 50-60 (7168 saved) 142 | 99.5,
+# 4 behind 12288 beside 200 of 50-600 (4608) 58 | 48, beside 60 31.3 | 31.7.  Of 320
+# random batches that saved enough, 43 were slower shared by 3 % or more, the worst 1.49
+# times; with this 26, and 4 are no longer shared that were faster so.
+SAVED_FOR = 5000           # a quarter of own reads, and of a kv head 6 a sequence, 1 a new token
 PER_THREAD = 2             # the per-thread default stream's handle
 
 STATUS = {0x401: "a page number outside the pool",
@@ -627,8 +634,12 @@ class Batch:
         rows = np.concatenate([[0], np.cumsum(q)])
         if first:
             c = self.cache
-            saved = sum((n - 1) * pages for _, n, pages in runs) * (c.page_size // 64) * c.kv_heads
-            if not runs or saved < MIN_SAVED[c.head_dim] or max(rows[a + n] - rows[a] for a, n, _ in runs) == 0:
+            chunks = c.page_size // 64 * c.kv_heads
+            saved = sum((n - 1) * pages for _, n, pages in runs) * chunks
+            own = int((-(-kv // 64)).sum()) * c.kv_heads - sum(n * pages for _, n, pages in runs) * chunks
+            others = own / 4 + (6 * self.seqs + int(q.sum())) * c.kv_heads
+            if not runs or saved < MIN_SAVED[c.head_dim] * max(1, others / SAVED_FOR) \
+                    or max(rows[a + n] - rows[a] for a, n, _ in runs) == 0:
                 return None
             self._s = _Shared(max_runs=len(runs), max_tokens=int(max(rows[a + n] - rows[a] for a, n, _ in runs)))
         room = self._s.max_tokens

@@ -116,6 +116,19 @@ def test_little_is_not_shared(dev, monkeypatch, d, seqs, pages, shares):  # noqa
         assert batch._s.max_runs == 1
 
 
+@pytest.mark.parametrize("alone,long,shares", [(0, 1, True), (50, 1, True), (1000, 1, False), (50, 200, False)])
+def test_sharing_pays_for_other_sequences(dev, monkeypatch, alone, long, shares):  # noqa: F811
+    """8 sequences with 80 pages in common (4480 reads saved), beside others of so
+    many pages of their own, whose rows and keys cost more in a batch that shares."""
+    monkeypatch.setattr(kv, "MIN_SAVED", {64: 6000, 128: 4000})
+    cache = small(dev, pages=20000, kv_heads=8, head_dim=128)
+    table = np.zeros((8 + alone, 200), np.int32)
+    table[:8, :80], table[:8, 80] = np.arange(80), 100 + np.arange(8)
+    table[8:, :long] = 200 + np.arange(alone * long).reshape(alone, long)
+    batch = cache.batch(table, [64 * 80 + 1] * 8 + [64 * long - 3] * alone, stream=3, shared=True)
+    assert (batch._s is not None) == shares
+
+
 def test_forks_are_runs(dev, monkeypatch):  # noqa: F811
     copies = []
     monkeypatch.setattr(kv, "_copy_in", lambda d, dst, host, st: copies.append(host.copy()))
