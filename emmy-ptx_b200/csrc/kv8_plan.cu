@@ -415,8 +415,13 @@ __global__ void __launch_bounds__(THREADS) plan_shared_kernel(const PlanParams p
   // ---- parts of own keys ----
   const int first_part = tiles ? 0 : n_pre;
   const int64_t share = (int64_t(own_work) * H + p.target - 1) / p.target;
-  // chunks of a part at most: the start of a block costs what three chunks do, and
-  // the last blocks should not take long
+  // chunks of a part at most: their share; more, as the start of a block costs what three
+  // chunks do, up to two fifths of the time that the shared keys take by the estimate
+  // above (a chunk takes a block 1.4 us beside two others: best / 1.4 * 2 / 5), as the
+  // last blocks should not take long.  The estimate is the tile kernel's for runs of the
+  // row kernel, too; with their share and min_chunks alone: 8 runs of 4 behind 4096 keys
+  // 31.0 -> 29.5 us, 2 of 8 behind 8192 27.8 -> 26.1, but 32 of 2 with 2 tokens 50.3 ->
+  // 54.3.  Where shared keys are not cut there is no estimate, and it is 0.
   const int q = max(max(p.min_chunks, int(best / 3.5f)), int(min(share, int64_t(1) << 24)));
   int parts = 0, n_parts;
 #pragma unroll
