@@ -23,7 +23,7 @@
 // and the multiples' in shared memory, 4 products a pair (an angle's function each
 // value: 854 us, so 173, for the case below).  Sines and cosines are good to 2^-18 of
 // the values, whose codes are rounded by 2^-4.  41536 tokens in 6 sequences, 8 heads
-// and 32 query heads of 128, bf16: 142 us, 6.5 TB/s; the queries' blocks mixed with
+// and 32 query heads of 128, bf16: 141 us, 6.5 TB/s; the queries' blocks mixed with
 // the pages' 164, before them 160, in a launch of their own 157.  One token 2.3 us, 64
 // of as many sequences 3.3.
 #include <cuda_bf16.h>
